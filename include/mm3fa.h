@@ -74,6 +74,7 @@ enum mm3fa_status {
     MM3FA_ERR_DEVICE      = 10, /* current device is not an sm_100 part                   */
     MM3FA_ERR_SCRATCH_LIMIT = 11, /* needs more scratch than MM3FA_NOALLOC_SCRATCH_BYTES  */
     MM3FA_ERR_COMM        = 12, /* NCCL missing, or a collective / IPC call failed        */
+    MM3FA_ERR_PAGES       = 13, /* a page operation found too few free cache pages        */
 };
 
 /* Size of the fixed device scratch buffer behind mm3fa_flash_attn_ext_noalloc (8 MiB). */
@@ -182,8 +183,9 @@ MM3FA_API int mm3fa_supports(const mm3fa_tensor * q, const mm3fa_tensor * k, con
                    const mm3fa_tensor * mask, float max_bias, float logit_softcap, const mm3fa_tensor * dst);
 
 /*
- * Reads (and clears) the device status word of a workspace: MM3FA_OK, or MM3FA_ERR_TIMEOUT
- * when a bounded device-side wait of an earlier call on it expired (*status_out gets the raw
+ * Reads (and clears) the device status word of a workspace: MM3FA_OK, MM3FA_ERR_TIMEOUT
+ * when a bounded device-side wait of an earlier call on it expired, or MM3FA_ERR_PAGES when a page
+ * operation of the 8-bit cache found too few free pages (*status_out gets the raw
  * bits).  After a timeout the workspace must be zero-filled again before reuse.  This call
  * synchronises `stream`.
  * Replaces: the ggml_status the reference ignores (src/qwen3-lm.h:620,921; src/dit.h:385).
@@ -455,6 +457,125 @@ typedef struct mm3fa_ipc_handle {
 MM3FA_API int mm3fa_ipc_export(const void * dev_ptr, mm3fa_ipc_handle * out);
 MM3FA_API int mm3fa_ipc_open(const mm3fa_ipc_handle * h, void ** dev_ptr_out);
 MM3FA_API int mm3fa_ipc_close(void * dev_ptr);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit paged KV cache.  K and V are held as int8 codes in pages of page_tokens tokens, with one F32
+ * scale for each (layer, page, kv head) of K and of V: value = code * scale.
+ *   k, v               int8 [n_layers][n_pages][n_head_kv][page_tokens][head_dim], 16-byte aligned
+ *   k_scale, v_scale   F32  [n_layers][n_pages][n_head_kv]
+ * head_dim 64, 128 or 256; page_tokens 16, 32, 64 or 128.  A sequence's tokens [P*j, P*j + P) are in the
+ * page that entry j of its table row names, the same page in every layer; an entry outside
+ * [0, n_pages) names none: its keys are absent from the attention, its rows are neither stored nor
+ * read.  refs[page] counts the table entries that name a page; 0 is a free page.
+ * Table, lengths and counts are device memory, so that a step can be captured and replayed.
+ * No counterpart in the reference, whose cache is one F16 slab per set (src/qwen3-lm.h:215-267).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct mm3fa_kv8 {
+    int32_t  head_dim, page_tokens, n_head_kv, n_pages, n_layers;
+    int32_t  reserved; /* 0 */
+    int8_t * k;
+    int8_t * v;
+    float *  k_scale;
+    float *  v_scale;
+} mm3fa_kv8;
+
+typedef struct mm3fa_kv8_table {
+    const int32_t * pages;     /* device [n_seq][stride], of which [0, max_pages) are used */
+    int64_t         stride;    /* entries */
+    int32_t         max_pages;
+    int32_t         n_seq;
+} mm3fa_kv8_table;
+
+/*
+ * Stores new K and V rows behind the tokens that each sequence holds.
+ *   k_new, v_new  F32, F16 or BF16 [D, T, n_head_kv, n_seq], any strides along dims 1 to 3
+ *   start   device int32 [n_seq]: tokens before the new rows (a negative one stores nothing)
+ *   n_new   device int32 [n_seq] or NULL: rows [0, n_new[s]) of sequence s are stored (NULL: T)
+ * For each page that gets rows, and each kv head: with earlier tokens in the page the scale becomes
+ * max(scale, max|x| / 127) and, where it grew, their codes are rounded to it; without, it becomes
+ * max|x| / 127.  Codes are the quotients by the scale (F32), rounded to nearest even as if exact and
+ * clamped to +-127.  Values that are not finite do not enter the maximum; NaN is stored as 0,
+ * +-inf as +-127.  The pages written must not be shared (refs 1) nor named twice in one call.
+ */
+MM3FA_API int mm3fa_kv8_append(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * k_new,
+                               const mm3fa_tensor * v_new, const mm3fa_kv8_table * table, const int32_t * start,
+                               const int32_t * n_new, void * stream);
+
+/*
+ * Reads rows [start[s], start[s] + n[s]) of each sequence as values (code * scale, rounded once to the
+ * result's type) into rows [0, n[s]) of k_out and v_out, F32, F16 or BF16 [D, T, n_head_kv, n_seq] with
+ * any strides along dims 1 to 3; n NULL: T.  Other rows, and rows whose page is missing, are left as
+ * they were.  With F16 results it fills the K/V operands of mm3fa_flash_attn_ext.
+ */
+MM3FA_API int mm3fa_kv8_read(const mm3fa_kv8 * cache, int layer, const mm3fa_kv8_table * table, const int32_t * start,
+                             const int32_t * n, mm3fa_tensor * k_out, mm3fa_tensor * v_out, void * stream);
+
+/* Bytes of device workspace mm3fa_kv8_attn needs (0: operands it would refuse). */
+MM3FA_API size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q,
+                                          const mm3fa_kv8_table * table);
+
+/*
+ * dst = softmax(scale * q k^T [softcap]) v over each sequence's pages of one layer.
+ *   q      F32, F16 or BF16 [D, n_q, n_head, n_seq], any strides along dims 1 to 3; query head h reads
+ *          kv head h / (n_head / n_head_kv)
+ *   dst    [D, n_head, n_q, n_seq], F32 or q's type (an F32 result is computed to F32's precision: q and
+ *          the softmax weights keep 22 bits; a 16-bit one with weights of 11 bits)
+ *   kv_len device int32 [n_seq]: tokens that the cache holds, the query rows' own among them
+ *   q_len  device int32 [n_seq] or NULL: rows of sequence s (NULL: n_q); rows from q_len[s] on are left
+ *          as they were
+ *   causal row i sees keys [0, kv_len - (q_len - 1 - i)); otherwise every row sees [0, kv_len)
+ *   logit_softcap  0 disables; otherwise s <- softcap * tanh(s / softcap)
+ *   workspace      zero-filled once after allocation, 16-byte aligned; reused and replayed like
+ *                  mm3fa_flash_attn_ext's, one per stream
+ * A row that sees no key becomes zeros.
+ */
+MM3FA_API int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, const mm3fa_kv8_table * table,
+                             const int32_t * kv_len, const int32_t * q_len, float scale, float logit_softcap,
+                             int causal, mm3fa_tensor * dst, void * workspace, size_t workspace_bytes, void * stream);
+
+/* Bytes of device workspace the page operations below need for n_seq sequences (0: a cache that they
+ * would refuse).  Zero-fill it once; one per stream. */
+MM3FA_API size_t mm3fa_kv8_pages_workspace(const mm3fa_kv8 * cache, int n_seq);
+
+/*
+ * Gives each sequence the pages for n_tok[s] tokens: negative entries among the first
+ * ceil(n_tok / P) of its table row get free pages, the lowest first, in the order of sequence and
+ * entry, with refs 1.  Changes nothing, and sets the workspace's status (MM3FA_ERR_PAGES), where there
+ * are too few free pages or a row is too short.
+ */
+MM3FA_API int mm3fa_kv8_reserve(const mm3fa_kv8 * cache, mm3fa_kv8_table * table, int32_t * refs,
+                                const int32_t * n_tok, void * workspace, size_t workspace_bytes, void * stream);
+
+/* Flags of mm3fa_kv8_fork. */
+enum mm3fa_kv8_fork_flags {
+    MM3FA_KV8_FORK_DEEP = 1, /* copy every page instead of sharing the full ones */
+};
+
+/*
+ * Sequence dst[i] becomes a copy of sequence src[i], for every pair i; src[i] = -1, or src NULL, empties it.
+ * It shares the full pages of its source (refs + 1), and the partly filled last one is copied, in every
+ * layer, to the lowest free page (with MM3FA_KV8_FORK_DEEP every page is); the pages that dst[i] named
+ * before lose a reference.  Every source is taken as it was before the call, so pairs may permute
+ * sequences.  A pair with src[i] == dst[i] changes nothing, one with an index out of range is
+ * ignored, and of several pairs with one dst the first counts.  Fresh pages are ones that were free
+ * before the call, the lowest first, in the order of sequence and entry.
+ *   src, dst  device int32 [n_pairs]
+ *   table_out, kv_len_out, refs_out  the results (same sizes), in buffers that do not overlap the inputs
+ * Copies the input tables, and sets the workspace's status (MM3FA_ERR_PAGES), where too few pages are free.
+ */
+MM3FA_API int mm3fa_kv8_fork(const mm3fa_kv8 * cache, const mm3fa_kv8_table * table, const int32_t * kv_len,
+                             const int32_t * refs, const int32_t * src, const int32_t * dst, int n_pairs,
+                             uint32_t flags, mm3fa_kv8_table * table_out, int32_t * kv_len_out, int32_t * refs_out,
+                             void * workspace, size_t workspace_bytes, void * stream);
+
+/*
+ * Moves the live pages (refs > 0) to the front of the pool: with L of them, the r-th free page below L
+ * takes the contents and the count of the r-th live page from L on, in every layer.  The results go
+ * to table_out and refs_out, buffers that do not overlap the inputs; entries that name no page become -1.
+ */
+MM3FA_API int mm3fa_kv8_compact(const mm3fa_kv8 * cache, const mm3fa_kv8_table * table, const int32_t * refs,
+                                mm3fa_kv8_table * table_out, int32_t * refs_out, void * workspace,
+                                size_t workspace_bytes, void * stream);
 
 #ifdef __cplusplus
 }

@@ -9,6 +9,7 @@
 #include "fa_decode.cuh"
 #include "fa_dense.cuh"
 #include "fa_prologue.cuh"
+#include "kv8.cuh"
 
 #include <cuda_runtime.h>
 
@@ -426,6 +427,27 @@ __global__ void bounded_wait_selftest_kernel(uint32_t * status, uint64_t timeout
 
 }  // namespace
 
+// what the other translation units of the ABI need of the above
+namespace mm3fa {
+
+int host_record_cuda(cudaError_t e) {
+    return record_cuda(e);
+}
+
+int host_sm_count() {
+    return device_info().sms;
+}
+
+int host_device_major() {
+    return device_info().major;
+}
+
+uint64_t host_wait_timeout_ns() {
+    return wait_timeout_ns();
+}
+
+}  // namespace mm3fa
+
 extern "C" {
 
 int mm3fa_version(void) {
@@ -460,6 +482,8 @@ const char * mm3fa_status_string(int st) {
             return "operands need more scratch than the built-in no-allocation buffer holds";
         case MM3FA_ERR_COMM:
             return "NCCL unavailable, or a collective or CUDA IPC call failed";
+        case MM3FA_ERR_PAGES:
+            return "too few free cache pages";
         default:
             return "unknown status";
     }
@@ -1096,7 +1120,7 @@ int mm3fa_workspace_status(void * workspace, void * stream, uint32_t * status_ou
         if (e != cudaSuccess) {
             return record_cuda(e);
         }
-        return MM3FA_ERR_TIMEOUT;
+        return st[0] == ST_PAGES ? MM3FA_ERR_PAGES : MM3FA_ERR_TIMEOUT;
     }
     return MM3FA_OK;
 }

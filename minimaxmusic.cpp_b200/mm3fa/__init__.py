@@ -29,6 +29,7 @@ ERR_NULL, ERR_TYPE, ERR_SHAPE, ERR_STRIDE, ERR_ALIGN = 1, 2, 3, 4, 5
 ERR_WORKSPACE, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT, ERR_DEVICE = 6, 7, 8, 9, 10
 ERR_SCRATCH_LIMIT = 11
 ERR_COMM = 12
+ERR_PAGES = 13
 
 MAX_RANKS = 8
 
@@ -381,3 +382,6 @@ def ipc_close(ptr: int) -> None:
     st = lib().mm3fa_ipc_close(ctypes.c_void_p(ptr or None))
     if st != OK:
         raise MM3FAError(st, "mm3fa_ipc_close")
+
+
+from .kv8 import Kv8Cache  # noqa: E402,F401  (uses the names above)
