@@ -56,6 +56,7 @@ struct Kv8AttnParams {
     const int * kv_len;  // [N]
     const int * q_len;   // [N] or null: n_q
     int         n_q, n_head, ratio;
+    uint32_t    ratio_inv;  // floor(2^32 / ratio) + 1 (0: ratio 1)
     int         causal;
     float       scale, softcap;
     // workspace

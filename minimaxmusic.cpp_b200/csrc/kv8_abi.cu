@@ -275,7 +275,8 @@ int mm3fa_kv8_read(const mm3fa_kv8 * cache, int layer, const mm3fa_kv8_table * t
 
 size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q, const mm3fa_kv8_table * table) {
     if (!q || check_cache(cache) != MM3FA_OK || check_table(cache, table) != MM3FA_OK || q->ne[1] < 1 || q->ne[2] < 1 ||
-        q->ne[2] % cache->n_head_kv || q->ne[1] > (1 << 30)) {
+        q->ne[2] % cache->n_head_kv || q->ne[1] > (1 << 24) || q->ne[2] > (1 << 20) ||
+        q->ne[2] / cache->n_head_kv * q->ne[1] > (1 << 24)) {
         return 0;
     }
     return kv8_attn_workspace_bytes(cache->head_dim, (int) q->ne[1], (int) (q->ne[2] / cache->n_head_kv),
@@ -310,7 +311,10 @@ int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, c
         !std::isfinite(logit_softcap)) {
         return MM3FA_ERR_SHAPE;
     }
-    if (q->ne[1] > (1 << 24) || H > (1 << 20)) {
+    // rows of a kv head, and 32-key blocks of all rows at the table's full length, are counted in 32 bits
+    const int64_t rows = H / cache->n_head_kv * q->ne[1];
+    if (q->ne[1] > (1 << 24) || H > (1 << 20) || rows > (1 << 24) || rows * (H / cache->n_head_kv) > INT32_MAX ||
+        ((rows + 15) / 16) * cache->n_head_kv * table->n_seq > (int64_t) INT32_MAX / (((int64_t) table->max_pages * cache->page_tokens + 31) / 32)) {
         return MM3FA_ERR_UNSUPPORTED;
     }
     if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < mm3fa_kv8_attn_workspace(cache, q, table)) {

@@ -3,22 +3,27 @@
 //
 // Mathematics.  With codes c and page scales a (keys) and b (values), s_j = scale * a * (q . c_j) and
 //     o = sum_j 2^(s_j - m) b c_j / sum_j 2^(s_j - m)          (s in log2 units, m a running maximum).
-// The codes are exact in F16, so q . c and P . c run on the tensor cores without rounding the cache.
-//   * q is brought to [1, 2) at its row's largest element by a power of two (any F32 or BF16 row fits
-//     F16 so) and split into an F16 number and the F16 remainder when the result is F32 (25 bits of the
-//     row's largest element; one F16 number holds an F16 or BF16 row).
-//   * the value scale of a page goes into the weights, P = 2^(s - m) * 2^(m + e - R) * f with b = f 2^e,
-//     f in [1, 2), and R the running maximum of (a tile's largest s) + e: O is held in units of 2^R,
-//     the sum in units of 2^m, so that pages with scales of any size stay in F16's range.  Weights are
-//     rounded to F16 (half a step: 2^-12), and their remainder too when the result is F32.  O, sums
-//     and maxima are F32.
+//   * q . c in integers: a row of q becomes fixed-point numbers of three 8-bit digits, the largest element
+//     127.5 * 2^16 (two digits and 2^8 for 16-bit results: half a step is 2^-16 of the row's largest element, below
+//     what the result keeps), and each digit's dot with the codes is exact on the 8-bit tensor cores.
+//   * P . c in F16, which holds the codes exactly.  The value scale of a page goes into the weights,
+//     P = 2^(s - m) * 2^(m + e - R) * f with b = f 2^e, f in [1, 2), and R the running maximum of (a tile's
+//     largest s) + e: O is held in units of 2^R, the sum in units of 2^m, so that pages with scales of
+//     any size stay in F16's range.  Weights are rounded to F16 (half a step: 2^-12), and their remainder
+//     too when the result is F32.  O, sums and maxima are F32.
 //
 // Work.  A unit is (sequence, kv head, 16 query rows): rows of all query heads of the group share the
-// cache's bytes.  A unit's keys come in blocks of 32; all units' blocks are cut into equal contiguous
-// ranges, one per CTA (the lengths are read on the device: a graph replays with others).  In a CTA each of
-// the four warps takes every fourth block of a unit through its own ring of cp.async stages - no barrier
-// between warps - and keeps its own softmax state; the four are joined in shared memory, and a unit cut
-// over CTAs is joined by the last CTA to arrive, in the order of the ranges (no result depends on timing).
+// cache's bytes.  A unit's keys come in blocks of 32.  Every CTA finds its work from the lengths on the
+// device (a graph replays with others), by one of three cuts:
+//   whole  no unit above KD_WHOLE blocks: whole units, an equal number for each CTA;
+//   split  few units: each in parts of up to W blocks, one part per CTA, W so that all parts run at once;
+//   flat   otherwise: all units' blocks in a row, in equal contiguous ranges, one per CTA.
+// Flat ranges are even, but a CTA that crosses from one unit to the next pays a second start and end, about
+// KD_CROSS blocks of its time; parts are uneven by the last part of each unit: total / (G - U) against
+// total / G blocks for the longest of G CTAs with U units.
+// In a CTA each of the four warps takes every fourth block of a unit through its own ring of cp.async
+// stages - no barrier between warps - and keeps its own softmax state; the four are joined in shared
+// memory, and the parts of a unit by the last CTA to arrive, in their order (no result depends on timing).
 #include "kv8.cuh"
 
 namespace mm3fa {
@@ -28,19 +33,24 @@ constexpr int KD_THREADS = 32 * KD_WARPS;
 constexpr int KD_BLOCK   = 32;     // keys per block
 constexpr int KD_ROWS    = 16;     // query rows per unit
 constexpr int KD_OFF     = 12;     // P is held times 2^12: F16 keeps 11 bits down to 2^-26 of the largest weight
-constexpr int KD_MIN     = 4;      // blocks per CTA below which fewer CTAs take part
+constexpr int KD_WHOLE   = 16;
+constexpr int KD_PART    = 8;      // blocks of a part, at least
+constexpr int KD_CROSS   = 8;
 
 template <int D, int NT, bool HP>
 struct KdSmem {
-    static constexpr int NS    = D == 64 ? (NT == 1 ? 6 : 5) : (D == 128 ? (NT == 1 ? 3 : 2) : 2);  // stages per warp
-    static constexpr int TILE  = KD_BLOCK * D;                                    // bytes of K or V
-    static constexpr int HEAD  = 32;                                              // scales and flags
+    // CTAs per SM and stages per warp: what shared memory and registers hold
+    static constexpr int CTAS  = D == 64 ? (NT == 1 ? 4 : 3) : (D == 128 ? (NT == 1 ? 3 : 2) : 1);
+    static constexpr int NS    = D == 64 ? (NT == 1 ? 3 : 4) : (D == 128 ? 2 : (NT == 1 ? 3 : 2));
+    static constexpr int ND    = HP ? 3 : 2;           // digits of q
+    static constexpr int TILE  = KD_BLOCK * D;         // bytes of K or V
+    static constexpr int HEAD  = 32;                   // scales and flags
     static constexpr int STAGE = 2 * TILE + HEAD;
     static constexpr int RING  = KD_WARPS * NS * STAGE;
-    static constexpr int Q     = D / 16 * NT * 32 * (HP ? 16 : 8);  // B fragments
-    static constexpr int OROW  = D + 4;                             // floats per row of the merge buffer
-    static constexpr int STATE = 2 * NT * 8 * 3 * 4;                // m, l, R
-    static constexpr int FIXED = RING + Q + STATE + NT * 8 * 4 + 64;
+    static constexpr int Q     = ND * NT * 8 * D;      // [digit][row][dim], chunks swizzled like K's
+    static constexpr int OROW  = D + 4;                // floats per row of the merge buffer
+    static constexpr int STATE = 2 * NT * 8 * 3 * 4;   // m, l, R
+    static constexpr int FIXED = RING + Q + STATE + NT * 8 * 4;
     static size_t        bytes(int rows) { return FIXED + (size_t) 2 * rows * OROW * 4; }
 };
 
@@ -61,6 +71,13 @@ __device__ __forceinline__ void kd_mma(float (&c)[4], const uint32_t (&a)[4], ui
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void kd_mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t kd_movmatrix(uint32_t x) {
@@ -105,6 +122,12 @@ __device__ __forceinline__ int kd_swz(int r) {
     return D == 64 ? (r >> 1) & 3 : r & 7;
 }
 
+// r / d for r < 2^24 and inv = floor(2^32 / d) + 1: the error r (inv d - 2^32) / 2^32 d stays below 1 / d
+// while r d < 2^32
+__device__ __forceinline__ uint32_t kd_div(uint32_t r, uint32_t inv) {
+    return inv ? __umulhi(r, inv) : r;
+}
+
 struct KdSeq {
     int n;   // keys
     int m;   // query rows (positions)
@@ -120,19 +143,22 @@ __device__ __forceinline__ KdSeq kd_seq(const Kv8AttnParams & p, int s) {
     return q;
 }
 
-// A walk over the segments (unit, blocks [b, e)) of a CTA's range.
+// How units are cut: w = 0 flat, otherwise in parts of up to w blocks (one part where no unit is longer).
+struct KdCut {
+    int w;
+    // items of a unit with nb blocks: blocks, or parts
+    __device__ __forceinline__ int items(int nb) const { return w == 0 ? nb : (nb <= w ? 1 : (nb + w - 1) / w); }
+};
+
+// A walk over the segments (unit, blocks [b, e)) of a CTA's range of items.
 struct KdWalk {
-    int     s, u;  // sequence, unit of it
-    int     b, e;
-    int64_t left;  // blocks from b on
-    KdSeq   q;
-    __device__ __forceinline__ void open(const Kv8AttnParams & p) {
-        q = kd_seq(p, s);
-        e = (int) min((int64_t) q.nb, b + left);
-    }
+    int   s, u;  // sequence, unit of it
+    int   b, e;
+    int   left;  // items from this segment on
+    KdSeq q;
     // to the next segment; false at the end of the range
-    __device__ __forceinline__ bool next(const Kv8AttnParams & p, int units) {
-        left -= e - b;
+    __device__ __forceinline__ bool next(const Kv8AttnParams & p, int units, KdCut cut) {
+        left -= cut.w ? 1 : e - b;
         if (left <= 0) {
             return false;
         }
@@ -142,19 +168,22 @@ struct KdWalk {
             s++;
             q = kd_seq(p, s);
         }
-        e = (int) min((int64_t) q.nb, left);
+        e = cut.w ? q.nb : min(q.nb, left);  // parts of units run one per CTA: here units are whole
         return true;
     }
 };
 
-template <int D, int NT, bool HP>
-__global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnParams p) {
+// A unit of which this CTA holds a part: its c0 .. c0 + n - 1 hold all of it.
+struct KdPart {
+    int s, u, c0, n;
+};
+
+template <int D, int NT, bool HP, bool CAP>
+__global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decode_kernel(const Kv8AttnParams p) {
     using L          = KdSmem<D, NT, HP>;
-    constexpr int NS = L::NS, CH = D / 64, MT = D / 16;
+    constexpr int NS = L::NS, ND = L::ND, CH = D / 64, MT = D / 16, E = D / 32, QR = NT * 8 / KD_WARPS;
     extern __shared__ __align__(16) char smem[];
-    __shared__ int64_t sh_total;
-    __shared__ int64_t sh_scan[KD_WARPS];
-    __shared__ int     sh_s, sh_u, sh_b, sh_last;
+    __shared__ int sh_last[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     char *    ring   = smem + warp * NS * L::STAGE;
     char *    qf     = smem + L::RING;
@@ -165,49 +194,82 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
     const int units = p.c.n_head_kv * groups;  // of a sequence
     kv8_dep_wait();
 
-    // ---- this CTA's range of blocks: the sequences' block counts, scanned
-    int64_t   sum = 0;
-    const int per = (p.t.n_seq + KD_THREADS - 1) / KD_THREADS, s0 = min(tid * per, p.t.n_seq), s1 = min(s0 + per, p.t.n_seq);
-    for (int s = s0; s < s1; s++) {
-        sum += (int64_t) kd_seq(p, s).nb * units;
-    }
-    int64_t inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-        inc += lane >= o ? x : 0;
-    }
-    if (lane == 31) {
-        sh_scan[warp] = inc;
-    }
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < KD_WARPS; w++) {
-        inc += w < warp ? sh_scan[w] : 0;
-        total += sh_scan[w];
-    }
-    const int64_t ctas = min((int64_t) gridDim.x, (total + KD_MIN - 1) / KD_MIN);
-    const int64_t c    = blockIdx.x;
-    if (c >= ctas) {
-        return;
-    }
-    const int64_t begin = c * total / ctas, end = (c + 1) * total / ctas;
-    if (inc - sum <= begin && begin < inc) {  // the one thread whose sequences hold the first block
-        int64_t off = begin - (inc - sum);
-        int     s   = s0, nb = kd_seq(p, s).nb;
-        while (off >= (int64_t) nb * units) {
-            off -= (int64_t) nb * units;
-            nb = kd_seq(p, ++s).nb;
-        }
-        sh_s = s, sh_u = (int) (off / nb), sh_b = (int) (off % nb);
-        sh_total = begin - off;  // first block of sequence s
-    }
-    __syncthreads();
+    // ---- this CTA's range: the sequences' items, scanned by every warp for itself
     KdWalk seg;
-    seg.s = sh_s, seg.u = sh_u, seg.b = sh_b, seg.left = end - begin;
-    int64_t seq_first = sh_total;
-    seg.open(p);
+    KdCut  cut{ 0 };
+    KdPart part[2];         // of the range's first and last segment
+    int    total = 0, ctas = (int) gridDim.x, seq_first;  // seq_first: first item of sequence seg.s
+    const int c = (int) blockIdx.x;
+    {
+        const int per = (p.t.n_seq + 31) / 32, s0 = min(lane * per, p.t.n_seq), s1 = min(s0 + per, p.t.n_seq);
+        int       sum = 0, inc = 0;
+#pragma unroll 1
+        for (int round = 0; round < 2; round++) {
+            int top = 0;
+            sum = 0;
+            for (int s = s0; s < s1; s++) {
+                const int nb = kd_seq(p, s).nb;
+                sum += cut.items(nb) * units, top = max(top, nb);
+            }
+            inc = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, inc, o);
+                inc += lane >= o ? x : 0;
+            }
+            total = __shfl_sync(0xffffffffu, inc, 31);
+            if (round == 0) {
+                const int all = p.t.n_seq * units, spare = ctas - all;
+                top = (int) __reduce_max_sync(0xffffffffu, (unsigned) top);
+                if (top <= KD_WHOLE) {
+                    cut.w = KD_WHOLE;
+                } else if (spare > 0 && (int64_t) total * all <= (int64_t) KD_CROSS * ctas * spare) {
+                    cut.w = max(KD_PART, (total + spare - 1) / spare);
+                } else {
+                    break;
+                }
+            }
+        }
+        ctas = min(ctas, total);
+        if (c >= ctas) {
+            return;
+        }
+        const int each = total / ctas, more = total - each * ctas;
+        const int begin = c * each + min(c, more);
+        const int who   = __ffs(__ballot_sync(0xffffffffu, inc > begin)) - 1;  // its sequences hold the first item
+        int       at    = __shfl_sync(0xffffffffu, inc - sum, who);
+        int       s     = who * per;
+        for (; per > 1; s += 32) {  // 32 of them at a time
+            const int n  = s + lane < min((who + 1) * per, p.t.n_seq) ? cut.items(kd_seq(p, s + lane).nb) * units : 0;
+            int       in = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, in, o);
+                in += lane >= o ? x : 0;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, at + in > begin);
+            if (hit) {
+                const int k = __ffs(hit) - 1;
+                s += k;
+                at = __shfl_sync(0xffffffffu, at + in - n, k);
+                break;
+            }
+            at = __shfl_sync(0xffffffffu, at + in, 31);
+        }
+        seg.s = s;
+        seg.q = kd_seq(p, s);
+        seq_first = at;
+        const int n = cut.items(seg.q.nb), off = begin - at;
+        seg.u    = off / n;
+        seg.left = each + (c < more);
+        const int k = off - seg.u * n;
+        seg.b = cut.w == 0 ? k : (int) ((int64_t) k * seg.q.nb / n);
+        seg.e = cut.w == 0 ? min(seg.q.nb, k + seg.left) : (int) ((int64_t) (k + 1) * seg.q.nb / n);
+        part[0] = KdPart{ 0, 0, 0, 0 }, part[1] = KdPart{ s, seg.u, c - k, cut.w ? n : 0 };
+        if (n == 1) {
+            part[1].n = 0;
+        }
+    }
 
     // ---- the warp's loads: block after block of the same walk, NS - 1 stages ahead
     KdWalk ld     = seg;
@@ -216,7 +278,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
     int    pg0 = -1, pg1 = -1;  // pages of the next block's halves
     auto   settle = [&] {       // brings the load cursor to a block of this warp and reads its pages
         while (ld_on && ld_b >= ld.e) {
-            ld_on = ld.next(p, units);
+            ld_on = ld.next(p, units, cut);
             ld_b  = ld.b + warp;
         }
         if (ld_on) {
@@ -262,62 +324,128 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
     for (int i = 0; i < NS - 1; i++) {
         load();
     }
-    int stage = 0;
+    int           stage = 0;
+    const int64_t slot  = (int64_t) KD_ROWS * (D + 4);  // floats of a part
+    // dims lane * E .. + E of a result row: O (in units of 2^(R - KD_OFF)) over the sum (of 2^m); rows without
+    // keys, and without a value scale, are 0
+    auto emit = [&](int s, int h, int r, int nq, float (&v)[E], float mt, float lt, float rt) {
+        const int qi = (int) kd_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
+        if (qi >= nq) {
+            return;
+        }
+        const float inv = lt != 0.0f ? (1.0f / (1 << KD_OFF)) / lt : 0.0f, up = rt == -INFINITY ? 0.0f : kd_ex2(rt - mt);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            v[e] = v[e] * inv * up;
+        }
+        char * dst = p.o.data + (int64_t) hq * p.o.nb1 + (int64_t) qi * p.o.nb2 + (int64_t) s * p.o.nb3;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            if (HP) {
+                float * f = reinterpret_cast<float *>(dst) + lane * E + e;
+                if (p.o.vec) {
+                    *reinterpret_cast<float2 *>(f) = make_float2(v[e], v[e + 1]);
+                } else {
+                    f[0] = v[e], f[1] = v[e + 1];
+                }
+            } else {
+                uint32_t w;
+                if (p.o.type == KV_F16) {
+                    w = kd_pack(v[e], v[e + 1]);
+                } else {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[e], v[e + 1]);
+                    w = *reinterpret_cast<const uint32_t *>(&b);
+                }
+                uint16_t * f = reinterpret_cast<uint16_t *>(dst) + lane * E + e;
+                if (p.o.vec) {
+                    *reinterpret_cast<uint32_t *>(f) = w;
+                } else {
+                    f[0] = (uint16_t) w, f[1] = (uint16_t) (w >> 16);
+                }
+            }
+        }
+    };
 
     for (bool more = true; more;) {
-        const int  h = seg.u / groups, r0 = (seg.u % groups) * KD_ROWS;
+        const int  h = seg.u / groups, r0 = (seg.u - h * groups) * KD_ROWS;
         const int  rows  = min(all_rows - r0, min(KD_ROWS, NT * 8));
         const KdSeq sq   = seg.q;
         const int   low  = p.causal ? max(sq.n - (sq.m - 1), 0) : sq.n;  // keys below this are seen by every row
-        // ---- Q fragments: for k-step i, column n, lane (g = n, t): the dims of chunk list(t), bytes 4i .. 4i + 3
-        for (int rr = warp; rr < NT * 8; rr += KD_WARPS) {
-            constexpr int E = D / 32;
-            float         x[E], amax = 0.0f;
-            const int     r = r0 + rr, qi = r / p.ratio, hq = h * p.ratio + r % p.ratio;
-            const bool    live = rr < rows && qi < sq.m;
-            if (live) {
-                const char * src = p.q.data + (int64_t) qi * p.q.nb1 + (int64_t) hq * p.q.nb2 + (int64_t) seg.s * p.q.nb3;
+        // ---- the digits of q, row rr = warp + 4 i
+        float xq[QR][E];
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const int i = lane * E + e;
-                    x[e]        = p.q.type == KV_F32 ? reinterpret_cast<const float *>(src)[i]
-                                : p.q.type == KV_F16 ? __half2float(reinterpret_cast<const __half *>(src)[i])
-                                                     : __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(src)[i]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    x[e] = 0.0f;
-                }
-            }
+        for (int i = 0; i < QR; i++) {
+            const int    r = r0 + warp + KD_WARPS * i, qi = (int) kd_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
+            const char * src = p.q.data + (int64_t) qi * p.q.nb1 + (int64_t) hq * p.q.nb2 + (int64_t) seg.s * p.q.nb3;
+            const bool   live = r < all_rows && qi < sq.m;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                amax = fmaxf(amax, fabsf(x[e]));
+                xq[i][e] = 0.0f;
+                if (live) {
+                    const int      at = lane * E + e;
+                    if (p.q.type == KV_F32) {
+                        xq[i][e] = reinterpret_cast<const float *>(src)[at];
+                    } else {
+                        const uint16_t u = reinterpret_cast<const uint16_t *>(src)[at];
+                        xq[i][e]         = p.q.type == KV_F16 ? __half2float(__ushort_as_half(u)) : __bfloat162float(__ushort_as_bfloat16(u));
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < QR; i++) {
+            const int rr   = warp + KD_WARPS * i;
+            float     amax = 0.0f;
+            bool      odd  = false;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float a = fabsf(xq[i][e]);
+                amax          = fmaxf(amax, a);
+                odd |= !(a < INFINITY);
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) {
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             }
-            // exponent of the row's largest element; rows of zeros, infinities and NaN stay as they are
-            const int   ex = amax > 0.0f && amax < INFINITY ? kd_exponent(amax) : 0;
-            const float dn = kd_pow2(-ex);
+            odd = __any_sync(0xffffffffu, odd);
+            // digits 127, 127, 127 at the largest element (the lowest 63: room for the division's roundings).  A row
+            // far from 1 is brought near by an exact power of two; one with an infinity or NaN gives NaN
+            constexpr float TOP = HP ? 8355647.0f : 32639.0f;
+            const float     up  = amax > 0x1p100f ? 0x1p-80f : (amax < 0x1p-100f ? 0x1p80f : 1.0f);
+            const float     mul = odd || amax == 0.0f ? 0.0f : __fdividef(TOP, amax * up);
             if (lane == 0) {
-                qscale[rr] = kd_pow2(ex) * p.scale * (p.softcap > 0.0f ? 1.0f / p.softcap : LOG2E);
+                const float back = odd ? NAN : (mul > 0.0f ? __fdividef(1.0f, mul) / up : 0.0f);
+                qscale[rr]       = back * (CAP ? p.scale / p.softcap : p.scale * LOG2E);
+            }
+            uint32_t dig[ND][(E + 3) / 4];
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+#pragma unroll
+                for (int e = 0; e < (E + 3) / 4; e++) {
+                    dig[d][e] = 0;
+                }
             }
 #pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const int      d   = lane * E + e;  // even; its pair sits in one fragment register
-                const int      ck  = d >> 4, by = d & 15;
-                const int      tt  = D == 64 ? ck : (ck & 7) >> 1;
-                const int      jj  = D == 64 ? 0 : (ck & 1) + 2 * (ck >> 3);
-                const int      ks  = jj * 4 + (by >> 2), hi = (by >> 1) & 1;
-                const float    a = x[e] * dn, b = x[e + 1] * dn;
-                const __half2  w  = __floats2half2_rn(a, b);
-                uint32_t *     to = reinterpret_cast<uint32_t *>(qf) + ((ks * NT + (rr >> 3)) * 32 + (rr & 7) * 4 + tt) * (HP ? 4 : 2) + hi;
-                to[0]             = *reinterpret_cast<const uint32_t *>(&w);
-                if (HP) {
-                    const float2 f = __half22float2(w);
-                    to[2]          = kd_pack(a - f.x, b - f.y);
+            for (int e = 0; e < E; e++) {
+                int v = odd ? 0 : __float2int_rn(xq[i][e] * up * mul);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const int low8 = (int8_t) v;  // digits in [-128, 127], the last in [-127, 127]
+                    dig[d][e >> 2] |= (uint32_t) (low8 & 255) << (8 * (e & 3));
+                    v = (v - low8) >> 8;
+                }
+            }
+            const int at = rr * D + ((((lane * E) >> 4) ^ kd_swz<D>(rr)) << 4) + ((lane * E) & 15);
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                char * to = qf + d * NT * 8 * D + at;
+                if (E == 2) {
+                    *reinterpret_cast<uint16_t *>(to) = (uint16_t) dig[d][0];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E / 4; e++) {
+                        reinterpret_cast<uint32_t *>(to)[e] = dig[d][e];
+                    }
                 }
             }
         }
@@ -328,7 +456,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int rr = nt * 8 + 2 * t + i, qi = (r0 + rr) / p.ratio;
+                const int rr = nt * 8 + 2 * t + i, qi = (int) kd_div((uint32_t) (r0 + rr), p.ratio_inv);
                 qs[nt][i]  = qscale[rr];
                 lim[nt][i] = p.causal ? sq.n - (sq.m - 1 - qi) : sq.n;
                 m[nt][i] = -INFINITY, l[nt][i] = 0.0f, R[nt][i] = -INFINITY;
@@ -350,50 +478,51 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
             const float4   sc   = *reinterpret_cast<const float4 *>(st + 2 * L::TILE);  // a0, a1, b0, b1
             const int2     has  = *reinterpret_cast<const int2 *>(st + 2 * L::TILE + 16);
             float          s[2][NT][4];
-#pragma unroll
-            for (int a = 0; a < 2; a++) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    s[a][nt][0] = s[a][nt][1] = s[a][nt][2] = s[a][nt][3] = 0.0f;
-                }
-            }
             // S^T = K Q^T: keys 16a + g and 16a + g + 8 of lane g, in the chunks of lane t
+            // (one half of the keys at a time where two columns of rows would need more registers than there are)
+            constexpr int AP = NT == 1 ? 2 : 1;
 #pragma unroll
-            for (int j = 0; j < CH; j++) {
-                const int ck = D == 64 ? t : 2 * t + (j & 1) + 8 * (j >> 1);
-                uint4     w[2][2];
+            for (int a0 = 0; a0 < 2; a0 += AP) {
+                int acc[AP][NT][ND][4];
 #pragma unroll
-                for (int a = 0; a < 2; a++) {
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int r = 16 * a + 8 * i + g;
-                        w[a][i]     = *reinterpret_cast<const uint4 *>(st + r * D + ((ck ^ kd_swz<D>(r)) << 4));
-                    }
+                for (int i = 0; i < AP * NT * ND * 4; i++) {
+                    (&acc[0][0][0][0])[i] = 0;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t bq[NT][4];
+                for (int j = 0; j < CH; j++) {
+                    const int ck = D == 64 ? t : 2 * t + (j & 1) + 8 * (j >> 1);
+                    uint4     w[AP][2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        const char * f = qf + (((j * 4 + i) * NT + nt) * 32 + lane) * (HP ? 16 : 8);
-                        if (HP) {
-                            const uint4 u = *reinterpret_cast<const uint4 *>(f);
-                            bq[nt][0] = u.x, bq[nt][1] = u.y, bq[nt][2] = u.z, bq[nt][3] = u.w;
-                        } else {
-                            const uint2 u = *reinterpret_cast<const uint2 *>(f);
-                            bq[nt][0] = u.x, bq[nt][1] = u.y;
+                    for (int a = 0; a < AP; a++) {
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const int r = 16 * (a0 + a) + 8 * i + g;
+                            w[a][i]     = *reinterpret_cast<const uint4 *>(st + r * D + ((ck ^ kd_swz<D>(r)) << 4));
                         }
                     }
 #pragma unroll
-                    for (int a = 0; a < 2; a++) {
-                        const uint32_t x = (&w[a][0].x)[i] ^ 0x80808080u, y = (&w[a][1].x)[i] ^ 0x80808080u;
-                        const uint32_t f[4] = { kd_half2(x, 0x4140), kd_half2(y, 0x4140), kd_half2(x, 0x4342), kd_half2(y, 0x4342) };
+                    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            kd_mma(s[a][nt], f, bq[nt][0], bq[nt][1]);
-                            if (HP) {
-                                kd_mma(s[a][nt], f, bq[nt][2], bq[nt][3]);
+                        for (int d = 0; d < ND; d++) {
+                            const int   r = nt * 8 + g;
+                            const uint4 b = *reinterpret_cast<const uint4 *>(qf + (d * NT * 8 + r) * D + ((ck ^ kd_swz<D>(r)) << 4));
+#pragma unroll
+                            for (int a = 0; a < AP; a++) {
+                                kd_mma_s8(acc[a][nt][d], w[a][0].x, w[a][1].x, w[a][0].y, w[a][1].y, b.x, b.y);
+                                kd_mma_s8(acc[a][nt][d], w[a][0].z, w[a][1].z, w[a][0].w, w[a][1].w, b.z, b.w);
                             }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < AP; a++) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            // |digit dots| < 2^22 (D = 256): two of them fit an int
+                            const float lo   = (float) (acc[a][nt][1][e] * 256 + acc[a][nt][0][e]);
+                            s[a0 + a][nt][e] = HP ? fmaf((float) acc[a][nt][ND - 1][e], 65536.0f, lo) : lo;
                         }
                     }
                 }
@@ -410,7 +539,7 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         float x = s[a][nt][e] * (qs[nt][e & 1] * as);
-                        if (p.softcap > 0.0f) {
+                        if (CAP) {
                             x = p.softcap * LOG2E * tanhf(x);
                         }
                         if (part) {
@@ -551,19 +680,19 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
                 }
             }
         }
-#pragma unroll
+#pragma unroll 1
         for (int round = 0; round < 2; round++) {
             if (round == 1) {
                 __syncthreads();
             }
-            if (round == 0 ? warp >= 2 : warp < 2) {
+            if ((warp < 2) == (round == 1)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const int rr = nt * 8 + 2 * t + i;
                         float *   st = state + ((warp & 1) * NT * 8 + rr) * 3;
-                        float *   w  = obuf + ((warp & 1) * rows + rr) * L::OROW;
+                        float *   w  = obuf + ((warp & 1) * rows + rr) * L::OROW + (D == 64 ? 8 : 16) * g;
                         float     fa = 1.0f, fb = 0.0f;
                         if (round == 1) {
                             const float mb = st[0], lb = st[1], Rb = st[2];
@@ -580,22 +709,14 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
                         if (rr < rows) {
 #pragma unroll
                             for (int j = 0; j < MT / 2; j++) {
-                                // 4 dims at a time, rotated by t: no bank twice
-                                const int jj = MT / 2 < 4 ? (j + t) & 1 : (j & ~3) | ((j + t) & 3);
-                                const int d  = D == 64 ? 8 * g + 4 * jj : (jj >> 2) * 128 + 16 * g + 4 * (jj & 3);
-                                float4    v  = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                                for (int k = 0; k < MT / 2; k++) {
-                                    if (k == jj) {
-                                        v = make_float4(o[2 * k][nt][i], o[2 * k][nt][i + 2], o[2 * k + 1][nt][i], o[2 * k + 1][nt][i + 2]);
-                                    }
-                                }
+                                float4 v = make_float4(o[2 * j][nt][i], o[2 * j][nt][i + 2], o[2 * j + 1][nt][i], o[2 * j + 1][nt][i + 2]);
+                                float4 * to = reinterpret_cast<float4 *>(w + (j >> 2) * 128 + 4 * (j & 3));
                                 if (round == 1) {
-                                    const float4 y = *reinterpret_cast<const float4 *>(w + d);
+                                    const float4 y = *to;
                                     v.x = v.x * fa + y.x * fb, v.y = v.y * fa + y.y * fb;
                                     v.z = v.z * fa + y.z * fb, v.w = v.w * fa + y.w * fb;
                                 }
-                                *reinterpret_cast<float4 *>(w + d) = v;
+                                *to = v;
                             }
                         }
                     }
@@ -603,162 +724,197 @@ __global__ void __launch_bounds__(KD_THREADS) kv8_decode_kernel(const Kv8AttnPar
             }
         }
         __syncthreads();
-        const int64_t first = seq_first + (int64_t) seg.u * sq.nb;  // the unit's first block
-        const bool    whole = seg.b == 0 && seg.e == sq.nb;
-        float *       slot  = p.part + (2 * c + (seg.b == 0)) * (int64_t) KD_ROWS * (D + 4);
-        // O (in units of 2^(R - KD_OFF)) over the sum (of 2^m); rows without keys, and without a value scale, are 0
-        auto write = [&](int rr, int d, float4 v, float mt, float lt, float rt) {
-            const int r = r0 + rr, qi = r / p.ratio, hq = h * p.ratio + r % p.ratio;
-            if (qi >= sq.m) {
-                return;
-            }
-            const float inv = lt != 0.0f ? (1.0f / (1 << KD_OFF)) / lt : 0.0f, up = rt == -INFINITY ? 0.0f : kd_ex2(rt - mt);
-            v.x = v.x * inv * up, v.y = v.y * inv * up, v.z = v.z * inv * up, v.w = v.w * inv * up;
-            char * dst = p.o.data + (int64_t) hq * p.o.nb1 + (int64_t) qi * p.o.nb2 + (int64_t) seg.s * p.o.nb3;
-            if (p.o.type == KV_F32) {
-                float * f = reinterpret_cast<float *>(dst) + d;
-                if (p.o.vec) {
-                    *reinterpret_cast<float4 *>(f) = v;
-                } else {
-                    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-                }
-                return;
-            }
-            uint16_t * f = reinterpret_cast<uint16_t *>(dst) + d;
-            const float x[4] = { v.x, v.y, v.z, v.w };
-            uint16_t    y[4];
+        const bool whole = seg.b == 0 && seg.e == sq.nb;
+        // two states left: to dst, or, of a part of a unit, to the workspace
+#pragma unroll 1
+        for (int rr = warp; rr < rows; rr += KD_WARPS) {
+            const float * za = state + rr * 3, *zb = za + NT * 8 * 3;
+            const float * ya = obuf + rr * L::OROW + lane * E, *yb = ya + rows * L::OROW;
+            const float   mt = fmaxf(za[0], zb[0]), rt = fmaxf(za[2], zb[2]);
+            const float   ms = mt == -INFINITY ? 0.0f : mt, rs = rt == -INFINITY ? 0.0f : rt;
+            const float   lt = za[1] * kd_ex2(za[0] - ms) + zb[1] * kd_ex2(zb[0] - ms), fa = kd_ex2(za[2] - rs), fb = kd_ex2(zb[2] - rs);
+            float         v[E];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                y[e] = p.o.type == KV_F16 ? __half_as_ushort(__float2half_rn(x[e])) : __bfloat16_as_ushort(__float2bfloat16_rn(x[e]));
-            }
-            if (p.o.vec) {
-                *reinterpret_cast<uint2 *>(f) = make_uint2(y[0] | (uint32_t) y[1] << 16, y[2] | (uint32_t) y[3] << 16);
-            } else {
-                f[0] = y[0], f[1] = y[1], f[2] = y[2], f[3] = y[3];
-            }
-        };
-        for (int it = tid; it < rows * (D / 4); it += KD_THREADS) {
-            const int rr = it / (D / 4), d = it % (D / 4) * 4;
-            float     mt = -INFINITY, rt = -INFINITY, lt = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                const float * x = state + (w * NT * 8 + rr) * 3;
-                mt = fmaxf(mt, x[0]), rt = fmaxf(rt, x[2]);
-            }
-            const float ms = mt == -INFINITY ? 0.0f : mt, rs = rt == -INFINITY ? 0.0f : rt;
-            float4      v  = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                const float * x = state + (w * NT * 8 + rr) * 3;
-                const float   f = kd_ex2(x[2] - rs);
-                const float4  y = *reinterpret_cast<const float4 *>(obuf + (w * rows + rr) * L::OROW + d);
-                lt += x[1] * kd_ex2(x[0] - ms);
-                v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
+            for (int e = 0; e < E; e++) {
+                v[e] = ya[e] * fa + yb[e] * fb;
             }
             if (whole) {
-                write(rr, d, v, mt, lt, rt);
+                emit(seg.s, h, r0 + rr, sq.m, v, mt, lt, rt);
             } else {
-                *reinterpret_cast<float4 *>(slot + rr * (D + 4) + d) = v;
-                if (d == 0) {
-                    *reinterpret_cast<float4 *>(slot + rr * (D + 4) + D) = make_float4(mt, lt, rt, 0.0f);
+                float * w = p.part + (2 * c + (seg.b == 0)) * slot + rr * (D + 4);
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    w[lane * E + e] = v[e];
+                }
+                if (lane == 0) {
+                    *reinterpret_cast<float4 *>(w + D) = make_float4(mt, lt, rt, 0.0f);
                 }
             }
         }
-        if (!whole) {
-            // the CTAs that hold a part of the unit: range k is [k total / ctas, (k + 1) total / ctas)
-            const int64_t c0 = ((first + 1) * ctas - 1) / total, c1 = ((first + sq.nb) * ctas - 1) / total;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t seen = atomicAdd(&p.counters[c0], 1u);
-                sh_last             = seen == (uint32_t) (c1 - c0);
-                if (sh_last) {
-                    p.counters[c0] = 0;
-                }
-            }
-            __syncthreads();
-            if (sh_last) {
-                __threadfence();
-                for (int it = tid; it < rows * (D / 4); it += KD_THREADS) {
-                    const int rr = it / (D / 4), d = it % (D / 4) * 4;
-                    float     mt = -INFINITY, rt = -INFINITY, lt = 0.0f;
-                    float4    v  = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int64_t k = c0; k <= c1; k++) {
-                        const float * x = p.part + (2 * k + (k == c0)) * (int64_t) KD_ROWS * (D + 4) + rr * (D + 4);
-                        const float4  y = __ldcg(reinterpret_cast<const float4 *>(x + d));
-                        const float4  z = __ldcg(reinterpret_cast<const float4 *>(x + D));
-                        const float   mn = fmaxf(mt, z.x), rn = fmaxf(rt, z.z);
-                        const float   ms = mn == -INFINITY ? 0.0f : mn, rs = rn == -INFINITY ? 0.0f : rn;
-                        const float   f = kd_ex2(rt - rs), e = kd_ex2(z.z - rs);
-                        lt  = lt * kd_ex2(mt - ms) + z.y * kd_ex2(z.x - ms);
-                        v.x = v.x * f + y.x * e, v.y = v.y * f + y.y * e, v.z = v.z * f + y.z * e, v.w = v.w * f + y.w * e;
-                        mt = mn, rt = rn;
-                    }
-                    write(rr, d, v, mt, lt, rt);
-                }
-            }
+        if (!whole && cut.w == 0) {
+            // the CTAs that hold a part: the first `over` ranges are one block longer than `each`
+            const int  each = total / ctas, over = total - each * ctas, first = seq_first + seg.u * sq.nb;
+            const auto cta_of = [&](int x) { return x < over * (each + 1) ? x / (each + 1) : over + (x - over * (each + 1)) / each; };
+            const int  c0 = cta_of(first);
+            part[0] = part[1], part[1] = KdPart{ seg.s, seg.u, c0, cta_of(first + sq.nb - 1) - c0 + 1 };
         }
         const int s_before = seg.s;
-        more               = seg.next(p, units);
+        more               = seg.next(p, units, cut);
         if (more && seg.s != s_before) {
-            seq_first += (int64_t) sq.nb * units;
+            seq_first += sq.nb * units;  // of use in a flat cut only
         }
-        __syncthreads();  // state, obuf and the Q fragments are written again
+        __syncthreads();  // state, obuf and the Q digits are written again
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (part[0].n + part[1].n == 0) {
+        return;
+    }
+
+    // ---- the parts of a unit, joined by the last CTA that arrives
+    __threadfence();
+    __syncthreads();
+    if (tid < 2) {
+        const KdPart & x = tid ? part[1] : part[0];
+        sh_last[tid]     = x.n && atomicAdd(&p.counters[x.c0], 1u) == (uint32_t) (x.n - 1);
+        if (sh_last[tid]) {
+            p.counters[x.c0] = 0;
+        }
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < 2; i++) {
+        if (!sh_last[i]) {
+            continue;
+        }
+        __threadfence();
+        const KdPart x  = i ? part[1] : part[0];
+        const int    h = x.u / groups, r0 = (x.u - h * groups) * KD_ROWS, rows = min(all_rows - r0, min(KD_ROWS, NT * 8));
+        const int    nq = kd_seq(p, x.s).m;
+#pragma unroll 1
+        for (int rr = warp; rr < rows; rr += KD_WARPS) {
+            const float * w  = p.part + 2 * x.c0 * slot + rr * (D + 4);
+            float         mt = -INFINITY, rt = -INFINITY, lt = 0.0f, v[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                v[e] = 0.0f;
+            }
+#pragma unroll 1
+            for (int k0 = 0; k0 < x.n; k0 += 32) {
+                // a part's state per lane: its factor, and the row's sum
+                const int  k = k0 + lane;
+                float4     z = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+                if (k < x.n) {
+                    z = __ldcg(reinterpret_cast<const float4 *>(w + (2 * k + (k == 0)) * slot + D));
+                }
+                float mn = z.x, rn = z.z;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) {
+                    mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+                    rn = fmaxf(rn, __shfl_xor_sync(0xffffffffu, rn, o));
+                }
+                mn = fmaxf(mn, mt), rn = fmaxf(rn, rt);
+                const float ms = mn == -INFINITY ? 0.0f : mn, rs = rn == -INFINITY ? 0.0f : rn;
+                const float f = kd_ex2(z.z - rs), f0 = kd_ex2(rt - rs);
+                float       ls = z.y * kd_ex2(z.x - ms);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) {
+                    ls += __shfl_xor_sync(0xffffffffu, ls, o);
+                }
+                lt = lt * kd_ex2(mt - ms) + ls;
+                mt = mn, rt = rn;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    v[e] *= f0;
+                }
+                constexpr int B = E == 8 ? 4 : 8;  // parts in flight
+                const int     n = min(x.n - k0, 32);
+#pragma unroll 1
+                for (int j = 0; j < n; j += B) {
+                    float y[B][E];
+#pragma unroll
+                    for (int b = 0; b < B; b++) {
+                        const int     kk = k0 + j + b;
+                        const float * src = w + (2 * kk + (kk == 0)) * slot + lane * E;
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) {
+                            const float2 u = j + b < n ? __ldcg(reinterpret_cast<const float2 *>(src + e)) : make_float2(0.0f, 0.0f);
+                            y[b][e] = u.x, y[b][e + 1] = u.y;
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < B; b++) {
+                        const float fb = __shfl_sync(0xffffffffu, f, (j + b) & 31);
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            v[e] += y[b][e] * fb;
+                        }
+                    }
+                }
+            }
+            emit(x.s, h, r0 + rr, nq, v, mt, lt, rt);
+        }
+    }
 }
 
 namespace {
 
-template <int D, int NT, bool HP>
+template <int D, int NT, bool HP, bool CAP>
 cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
     const size_t smem = KdSmem<D, NT, HP>::bytes(rows);
-    // per device, so that a second device gets it too; cheap
-    const cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<D, NT, HP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    // on each call, so that every device gets it; a host-side setting, cheap
+    const cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<D, NT, HP, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int) KdSmem<D, NT, HP>::bytes(NT * 8));
-    return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, HP>, dim3(ctas), KD_THREADS, smem, stream, p);
+    return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, HP, CAP>, dim3(ctas), KD_THREADS, smem, stream, p);
+}
+
+template <int D, int NT>
+cudaError_t launch_nt(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
+    if (p.o.type == KV_F32) {
+        return p.softcap > 0.0f ? launch_one<D, NT, true, true>(p, ctas, rows, stream) : launch_one<D, NT, true, false>(p, ctas, rows, stream);
+    }
+    return p.softcap > 0.0f ? launch_one<D, NT, false, true>(p, ctas, rows, stream) : launch_one<D, NT, false, false>(p, ctas, rows, stream);
 }
 
 template <int D>
-cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, int rows, bool hp, cudaStream_t stream) {
-    if (rows <= 8) {
-        return hp ? launch_one<D, 1, true>(p, ctas, rows, stream) : launch_one<D, 1, false>(p, ctas, rows, stream);
-    }
-    return hp ? launch_one<D, 2, true>(p, ctas, rows, stream) : launch_one<D, 2, false>(p, ctas, rows, stream);
+cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
+    return rows <= 8 ? launch_nt<D, 1>(p, ctas, rows, stream) : launch_nt<D, 2>(p, ctas, rows, stream);
 }
 
-// CTAs that an SM holds at once: two, by shared memory, but for D = 256
-int ctas_per_sm(int D) {
-    return D == 256 ? 1 : 2;
+// CTAs that an SM holds at once: what KdSmem plans for
+int ctas_per_sm(int D, int rows) {
+    return rows <= 8 ? (D == 64 ? KdSmem<64, 1, true>::CTAS : D == 128 ? KdSmem<128, 1, true>::CTAS : KdSmem<256, 1, true>::CTAS)
+                     : (D == 64 ? KdSmem<64, 2, true>::CTAS : D == 128 ? KdSmem<128, 2, true>::CTAS : KdSmem<256, 2, true>::CTAS);
 }
 
 }  // namespace
 
 // Counters (one per CTA) and two partial results per CTA, whatever the lengths are.
 size_t kv8_attn_workspace_bytes(int D, int n_q, int ratio, int n_head_kv, int n_seq, int sms) {
-    const size_t ctas = (size_t) sms * (size_t) ctas_per_sm(D);
-    (void) n_q, (void) ratio, (void) n_head_kv, (void) n_seq;
+    const size_t ctas = (size_t) sms * (size_t) ctas_per_sm(D, ratio * n_q);
+    (void) n_head_kv, (void) n_seq;
     return WS_STATUS_BYTES + (ctas * 4 + 255) / 256 * 256 + 2 * ctas * KD_ROWS * (size_t) (D + 4) * 4;
 }
 
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p0, int sms, cudaStream_t stream) {
     Kv8AttnParams p    = p0;
-    const int     most = sms * ctas_per_sm(p.c.D);
+    const int     most = sms * ctas_per_sm(p.c.D, p.ratio * p.n_q);
     p.counters = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.status) + WS_STATUS_BYTES);
     p.part     = reinterpret_cast<float *>(reinterpret_cast<char *>(p.counters) + ((size_t) most * 4 + 255) / 256 * 256);
     const int     all = p.ratio * p.n_q, rows = all < KD_ROWS ? all : KD_ROWS;
     const int64_t units  = (int64_t) p.t.n_seq * p.c.n_head_kv * ((all + KD_ROWS - 1) / KD_ROWS);
     const int64_t blocks = units * (((int64_t) p.t.max_pages * p.c.P + KD_BLOCK - 1) / KD_BLOCK);  // at most
-    const int64_t want   = (blocks + KD_MIN - 1) / KD_MIN;
-    const unsigned ctas  = (unsigned) (want < most ? want : most);
-    const bool     hp    = p.o.type == KV_F32;
+    if (blocks > INT32_MAX) {
+        return cudaErrorInvalidValue;  // refused by the caller's checks
+    }
+    const unsigned ctas  = (unsigned) (blocks < most ? blocks : most);
+    p.ratio_inv          = p.ratio == 1 ? 0u : (uint32_t) ((1ull << 32) / (uint64_t) p.ratio + 1);
     switch (p.c.D) {
         case 64:
-            return launch_d<64>(p, ctas, rows, hp, stream);
+            return launch_d<64>(p, ctas, rows, stream);
         case 128:
-            return launch_d<128>(p, ctas, rows, hp, stream);
+            return launch_d<128>(p, ctas, rows, stream);
         default:
-            return launch_d<256>(p, ctas, rows, hp, stream);
+            return launch_d<256>(p, ctas, rows, stream);
     }
 }
 
