@@ -202,39 +202,41 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
     const int c = (int) blockIdx.x;
     {
         const int per = (p.t.n_seq + 31) / 32, s0 = min(lane * per, p.t.n_seq), s1 = min(s0 + per, p.t.n_seq);
-        int       sum = 0, inc = 0;
-#pragma unroll 1
-        for (int round = 0; round < 2; round++) {
-            int top = 0;
-            sum = 0;
-            for (int s = s0; s < s1; s++) {
-                const int nb = kd_seq(p, s).nb;
-                sum += cut.items(nb) * units, top = max(top, nb);
-            }
-            inc = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, inc, o);
-                inc += lane >= o ? x : 0;
-            }
-            total = __shfl_sync(0xffffffffu, inc, 31);
-            if (round == 0) {
-                const int all = p.t.n_seq * units, spare = ctas - all;
-                top = (int) __reduce_max_sync(0xffffffffu, (unsigned) top);
-                if (top <= KD_WHOLE) {
-                    cut.w = KD_WHOLE;
-                } else if (spare > 0 && (int64_t) total * all <= (int64_t) KD_CROSS * ctas * spare) {
-                    cut.w = max(KD_PART, (total + spare - 1) / spare);
-                } else {
-                    break;
-                }
+        int       sum = 0, top = 0, one = 0;  // one: blocks of the lane's sequence, where it has only one
+        for (int s = s0; s < s1; s++) {
+            one = kd_seq(p, s).nb;
+            sum += one, top = max(top, one);
+        }
+        total = (int) __reduce_add_sync(0xffffffffu, (unsigned) sum) * units;
+        top   = (int) __reduce_max_sync(0xffffffffu, (unsigned) top);
+        const int all = p.t.n_seq * units, spare = ctas - all;
+        if (top <= KD_WHOLE) {
+            cut.w = KD_WHOLE;
+        } else if (spare > 0 && (int64_t) total * all <= (int64_t) KD_CROSS * ctas * spare) {
+            cut.w = max(KD_PART, (total + spare - 1) / spare);
+        }
+        sum *= units;
+        if (cut.w) {
+            sum = per == 1 ? (s1 > s0 ? cut.items(one) * units : 0) : 0;
+            for (int s = s0; s < s1 && per > 1; s++) {
+                sum += cut.items(kd_seq(p, s).nb) * units;
             }
         }
-        ctas = min(ctas, total);
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, inc, o);
+            inc += lane >= o ? x : 0;
+        }
+        total = __shfl_sync(0xffffffffu, inc, 31);
+        ctas  = min(ctas, total);
         if (c >= ctas) {
             return;
         }
-        const int each = total / ctas, more = total - each * ctas;
+        int each = 1, more = 0;
+        if (ctas < total) {
+            each = total / ctas, more = total - each * ctas;
+        }
         const int begin = c * each + min(c, more);
         const int who   = __ffs(__ballot_sync(0xffffffffu, inc > begin)) - 1;  // its sequences hold the first item
         int       at    = __shfl_sync(0xffffffffu, inc - sum, who);
@@ -260,31 +262,66 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
         seg.q = kd_seq(p, s);
         seq_first = at;
         const int n = cut.items(seg.q.nb), off = begin - at;
-        seg.u    = off / n;
+        seg.u    = n == 1 ? off : off / n;
         seg.left = each + (c < more);
         const int k = off - seg.u * n;
-        seg.b = cut.w == 0 ? k : (int) ((int64_t) k * seg.q.nb / n);
-        seg.e = cut.w == 0 ? min(seg.q.nb, k + seg.left) : (int) ((int64_t) (k + 1) * seg.q.nb / n);
+        if (cut.w == 0) {
+            seg.b = k;
+            seg.e = min(seg.q.nb, k + seg.left);
+        } else {  // parts that differ by one block at most
+            const int base = n == 1 ? seg.q.nb : seg.q.nb / n, rest = seg.q.nb - base * n;
+            seg.b = k * base + min(k, rest);
+            seg.e = seg.b + base + (k < rest);
+        }
         part[0] = KdPart{ 0, 0, 0, 0 }, part[1] = KdPart{ s, seg.u, c - k, cut.w ? n : 0 };
         if (n == 1) {
             part[1].n = 0;
         }
     }
 
-    // ---- the warp's loads: block after block of the same walk, NS - 1 stages ahead
+    // ---- a segment's query rows rr = warp + 4 i, as they are: the first segment's before anything else
+    uint32_t xr[QR][E];
+    auto     load_q = [&] {
+        const int h = seg.u / groups, r0 = (seg.u - h * groups) * KD_ROWS;
+#pragma unroll
+        for (int i = 0; i < QR; i++) {
+            const int    r = r0 + warp + KD_WARPS * i, qi = (int) kd_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
+            const char * src = p.q.data + (int64_t) qi * p.q.nb1 + (int64_t) hq * p.q.nb2 + (int64_t) seg.s * p.q.nb3;
+            const bool   live = r < all_rows && qi < seg.q.m;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int at = lane * E + e;
+                xr[i][e]     = !live ? 0u : p.q.type == KV_F32 ? reinterpret_cast<const uint32_t *>(src)[at] : reinterpret_cast<const uint16_t *>(src)[at];
+            }
+        }
+    };
+    load_q();
+
+    // ---- the warp's loads: block after block of the same walk, NS - 1 stages ahead.  Lane i holds the table entries
+    // of the warp's i-th block from the cursor's base on, so that no load waits for a table entry but the first of 32
     KdWalk ld     = seg;
     int    ld_b   = ld.b + warp;
     bool   ld_on  = true;
-    int    pg0 = -1, pg1 = -1;  // pages of the next block's halves
-    auto   settle = [&] {       // brings the load cursor to a block of this warp and reads its pages
+    int    ld_i = 0, tab0 = -1, tab1 = -1;
+    auto   fetch = [&] {
+        const int k0 = (ld_b + KD_WARPS * lane) * KD_BLOCK, j = k0 >> p.c.log2p;
+        const bool in = ld_b + KD_WARPS * lane < ld.e && k0 < ld.q.n;
+        const int * row = p.t.pages + (int64_t) ld.s * p.t.stride;
+        ld_i = 0;
+        tab0 = in ? row[j] : -1;
+        if (p.c.log2p == 4) {
+            tab1 = in && k0 + 16 < ld.q.n ? row[j + 1] : -1;
+        }
+    };
+    auto settle = [&] {  // brings the load cursor to a block of this warp, with its entries
+        bool fresh = ld_i == 32;
         while (ld_on && ld_b >= ld.e) {
             ld_on = ld.next(p, units, cut);
             ld_b  = ld.b + warp;
+            fresh = true;
         }
-        if (ld_on) {
-            const int k0 = ld_b * KD_BLOCK, j = k0 >> p.c.log2p;
-            pg0 = k0 < ld.q.n ? kv8_page(p.t, p.c.n_pages, ld.s, j) : -1;
-            pg1 = p.c.log2p > 4 ? pg0 : (k0 + 16 < ld.q.n ? kv8_page(p.t, p.c.n_pages, ld.s, j + 1) : -1);
+        if (ld_on && fresh) {
+            fetch();
         }
     };
     int  ld_stage = 0;
@@ -293,16 +330,19 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
             char *         st  = ring + ld_stage * L::STAGE;
             const int      h   = ld.u / groups;
             const int      row = (ld_b * KD_BLOCK) & (p.c.P - 1);  // of the block in its page
-            const int64_t  ph0 = (int64_t) max(pg0, 0) * p.c.n_head_kv + h, ph1 = (int64_t) max(pg1, 0) * p.c.n_head_kv + h;
+            int            pg0 = __shfl_sync(0xffffffffu, tab0, ld_i), pg1 = p.c.log2p == 4 ? __shfl_sync(0xffffffffu, tab1, ld_i) : pg0;
+            const bool     ok0 = (unsigned) pg0 < (unsigned) p.c.n_pages, ok1 = (unsigned) pg1 < (unsigned) p.c.n_pages;
+            pg0 = ok0 ? pg0 : 0, pg1 = ok1 ? pg1 : 0;
+            const int64_t  ph0 = (int64_t) pg0 * p.c.n_head_kv + h, ph1 = (int64_t) pg1 * p.c.n_head_kv + h;
             const int64_t  o0 = (ph0 * p.c.P + row) * D;
-            const int64_t  o1 = (p.c.log2p > 4 ? o0 + 16 * D : ph1 * p.c.P * D);
-            const uint32_t z0 = pg0 >= 0 ? 16u : 0u, z1 = pg1 >= 0 ? 16u : 0u;
+            const int64_t  o1 = (p.c.log2p > 4 ? o0 : ph1 * p.c.P * D - 16 * D);
+            const uint32_t z0 = ok0 ? 16u : 0u, z1 = ok1 ? 16u : 0u;
             const uint32_t dst = smem_addr(st);
 #pragma unroll
             for (int i = 0; i < 4 * CH; i++) {  // 32 rows of D / 16 chunks, 32 chunks at a time
                 const int     idx  = i * 32 + lane, r = idx / (D / 16), ck = idx % (D / 16);
                 const bool    half = i >= 2 * CH;
-                const int64_t off  = (half ? o1 - 16 * D : o0) + (int64_t) idx * 16;
+                const int64_t off  = (half ? o1 : o0) + idx * 16;
                 const uint32_t to  = dst + (uint32_t) (r * D + ((ck ^ kd_swz<D>(r)) << 4));
                 kd_cp16(to, p.c.k + off, half ? z1 : z0);
                 kd_cp16(to + L::TILE, p.c.v + off, half ? z1 : z0);
@@ -311,14 +351,16 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                 const int64_t ph = lane & 1 ? ph1 : ph0;
                 kd_cp4(dst + 2 * L::TILE + lane * 4, (lane < 2 ? p.c.k_scale : p.c.v_scale) + ph, (lane & 1 ? z1 : z0) / 4);
             } else if (lane < 6) {
-                reinterpret_cast<int *>(st + 2 * L::TILE)[lane] = (lane & 1 ? pg1 : pg0) >= 0;
+                reinterpret_cast<int *>(st + 2 * L::TILE)[lane] = lane & 1 ? ok1 : ok0;
             }
             ld_b += KD_WARPS;
+            ld_i++;
             settle();
         }
         ld_stage = ld_stage + 1 == NS ? 0 : ld_stage + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    ld_i = 32;
     settle();
 #pragma unroll
     for (int i = 0; i < NS - 1; i++) {
@@ -375,21 +417,11 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
         float xq[QR][E];
 #pragma unroll
         for (int i = 0; i < QR; i++) {
-            const int    r = r0 + warp + KD_WARPS * i, qi = (int) kd_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
-            const char * src = p.q.data + (int64_t) qi * p.q.nb1 + (int64_t) hq * p.q.nb2 + (int64_t) seg.s * p.q.nb3;
-            const bool   live = r < all_rows && qi < sq.m;
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                xq[i][e] = 0.0f;
-                if (live) {
-                    const int      at = lane * E + e;
-                    if (p.q.type == KV_F32) {
-                        xq[i][e] = reinterpret_cast<const float *>(src)[at];
-                    } else {
-                        const uint16_t u = reinterpret_cast<const uint16_t *>(src)[at];
-                        xq[i][e]         = p.q.type == KV_F16 ? __half2float(__ushort_as_half(u)) : __bfloat162float(__ushort_as_bfloat16(u));
-                    }
-                }
+                const uint32_t u = xr[i][e];
+                xq[i][e] = p.q.type == KV_F32 ? __uint_as_float(u) : p.q.type == KV_F16 ? __half2float(__ushort_as_half((uint16_t) u))
+                                                                                       : __uint_as_float(u << 16);
             }
         }
 #pragma unroll
@@ -763,6 +795,9 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
         if (more && seg.s != s_before) {
             seq_first += sq.nb * units;  // of use in a flat cut only
         }
+        if (more) {
+            load_q();
+        }
         __syncthreads();  // state, obuf and the Q digits are written again
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -826,7 +861,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                 for (int e = 0; e < E; e++) {
                     v[e] *= f0;
                 }
-                constexpr int B = E == 8 ? 4 : 8;  // parts in flight
+                constexpr int B = E == 8 ? 8 : 16;  // parts in flight
                 const int     n = min(x.n - k0, 32);
 #pragma unroll 1
                 for (int j = 0; j < n; j += B) {
