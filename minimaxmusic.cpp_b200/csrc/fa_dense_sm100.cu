@@ -40,6 +40,7 @@
 // the softmax warps are made warp-uniform so the .sync.aligned TMEM accesses never diverge.
 #include "fa_dense.cuh"
 #include "fa_decode.cuh"
+#include "tc_sm100.cuh"
 
 #include <cuda.h>
 
@@ -141,124 +142,6 @@ __device__ __forceinline__ void dn_named_barrier(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
-__device__ __forceinline__ void dn_mbar_arrive(uint64_t * bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-// warp-uniform bounded wait: true only if every lane saw the phase complete
-__device__ __forceinline__ bool dn_wait_warp(uint64_t * bar, uint32_t parity, uint64_t deadline) {
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, deadline));
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t * dst, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)),
-                 "r"(ncols)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_relinquish() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-
-// The tcgen05.mma / tcgen05.commit wrappers below are executed by a whole converged warp: the
-// operands are computed by every lane (so they stay in the uniform datapath) and elect.sync picks
-// the one lane that issues the instruction.
-
-// D (TMEM) = A (smem desc) * B (smem desc) [+ D]
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                         uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// arrive on `bar` once every tcgen05 operation this thread issued before has completed
-__device__ __forceinline__ void umma_commit(uint64_t * bar) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
-        : "memory");
-}
-
-// 32 consecutive 32-bit columns of this thread's TMEM lane (r[0..31] must stay in registers)
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t * r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t * r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-        "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
-            taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
-// tcgen05.wait::ld that also names the 32 registers a tcgen05.ld wrote: the compiler cannot move
-// any use of them above the wait (the load writes them asynchronously)
-__device__ __forceinline__ void tmem_ld_wait_tie(uint32_t * r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_st_wait() {
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// 2^x on the special-function unit (PTX ex2.approx, flushes denormal results to zero); 2^-inf = 0
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Shared-memory matrix descriptor of a 128-byte-swizzled operand (sm_100 format, version 1).
-// K-major: sbo = 1024 (8-row groups), lbo unused (16).  MN-major: lbo = stride between 64-element
-// column blocks, sbo = 1024 (8-row groups along K).
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    uint64_t d = 0;
-    d |= (uint64_t) ((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t) ((lbo >> 4) & 0x3FFFu) << 16;
-    d |= (uint64_t) ((sbo >> 4) & 0x3FFFu) << 32;
-    d |= (uint64_t) 1 << 46;  // descriptor version of sm_100
-    d |= (uint64_t) 2 << 61;  // SWIZZLE_128B
-    return d;
-}
-
 // Instruction descriptor of kind::f16, F32 accumulator, M = 128, dense.
 __host__ __device__ constexpr uint32_t umma_idesc(bool bf16, int n, bool b_mn_major) {
     return (1u << 4)                              // D format: F32
@@ -267,11 +150,6 @@ __host__ __device__ constexpr uint32_t umma_idesc(bool bf16, int n, bool b_mn_ma
            | ((b_mn_major ? 1u : 0u) << 16)       // B major (A is K-major: bit 15 = 0)
            | ((uint32_t) (n >> 3) << 17)          // N / 8
            | ((uint32_t) (DN_M >> 4) << 24);      // M / 16
-}
-
-// byte offset of (row, 16-byte chunk) in a 128-byte-swizzled tile of 128-byte rows
-__device__ __forceinline__ uint32_t sw128_off(int row, int chunk) {
-    return (uint32_t) (row * 128 + ((chunk ^ (row & 7)) << 4));
 }
 
 template <bool BF16>
@@ -316,83 +194,6 @@ __device__ __forceinline__ int tile_class(const DenseParams & p, int plane, int 
     }
     const uint32_t f = p.blocks[((int64_t) plane * p.n_qt + qt) * p.n_kt + kt];
     return !(f & BLKF_FINITE) ? BLK_SKIP : (!(f & BLKF_NONZERO) ? BLK_NONE : BLK_MIXED);
-}
-
-// D (TMEM) = A (TMEM, 16-bit, row m = lane m) * B (smem desc) [+ D]; whole warp, one lane issues
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// max of three (PTX max.f32 with three sources, sm_100)
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
-// Packed pairs of f32 (PTX .f32x2 arithmetic, sm_100): lo in the low 32 bits.
-__device__ __forceinline__ uint64_t f2pack(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-
-__device__ __forceinline__ void f2unpack(uint64_t v, float & lo, float & hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
-__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
-// 2^x for a pair, on the FMA pipe: x = n + f with n = round(x) (added to the exponent field) and
-// f in [-1/2, 1/2]; 2^f by a degree-3 polynomial fitted here for minimum relative error on that
-// interval (max 7.5e-5, below half an f16 ulp).  x is clamped to >= -126 so n never underflows the
-// exponent; 2^-126 instead of 0 for x = -inf is far below what a 16-bit P can hold.
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x2) {
-    constexpr float C0 = 0.99992806f, C1 = 0.69326097f, C2 = 0.24261114f, C3 = 0.05517167f;
-    constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
-    float xl, xh;
-    f2unpack(x2, xl, xh);
-    x2                = f2pack(fmaxf(xl, -126.0f), fmaxf(xh, -126.0f));
-    const uint64_t r2 = fadd2(x2, f2pack(MAGIC, MAGIC));
-    const uint64_t n2 = fadd2(r2, f2pack(-MAGIC, -MAGIC));
-    const uint64_t f2 = ffma2(n2, f2pack(-1.0f, -1.0f), x2);
-    uint64_t       p2 = ffma2(f2pack(C3, C3), f2, f2pack(C2, C2));
-    p2                = ffma2(p2, f2, f2pack(C1, C1));
-    p2                = ffma2(p2, f2, f2pack(C0, C0));
-    float rl, rh, pl, ph;
-    f2unpack(r2, rl, rh);
-    f2unpack(p2, pl, ph);
-    // the low bits of r hold n; shifted by 23 they land in the exponent field (the magic's own bits
-    // shift out)
-    return f2pack(__int_as_float(__float_as_int(pl) + (__float_as_int(rl) << 23)),
-                  __int_as_float(__float_as_int(ph) + (__float_as_int(rh) << 23)));
 }
 
 // ------------------------------------------------------------------ kernel
