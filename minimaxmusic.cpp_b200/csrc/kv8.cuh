@@ -10,6 +10,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdlib>
 
 namespace mm3fa {
@@ -144,6 +145,28 @@ cudaError_t kv8_launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t sm
     }
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
+
+// A kernel's dynamic shared memory limit, raised once per device.
+struct Kv8Once {
+    std::atomic<uint64_t> done{ 0 };
+    template <typename Kern>
+    cudaError_t smem(Kern kern, size_t bytes) {
+        int         dev = 0;
+        cudaError_t e   = cudaGetDevice(&dev);
+        if (e != cudaSuccess) {
+            return e;
+        }
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (bit && (done.load(std::memory_order_acquire) & bit)) {
+            return cudaSuccess;
+        }
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
+        if (e == cudaSuccess) {
+            done.fetch_or(bit, std::memory_order_release);
+        }
+        return e;
+    }
+};
 
 cudaError_t launch_kv8_append(const Kv8StoreParams & p, cudaStream_t stream);
 cudaError_t launch_kv8_read(const Kv8StoreParams & p, int sms, cudaStream_t stream);

@@ -896,9 +896,8 @@ namespace {
 template <int D, int NT, bool HP, bool CAP>
 cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
     const size_t smem = KdSmem<D, NT, HP>::bytes(rows);
-    // on each call, so that every device gets it; a host-side setting, cheap
-    const cudaError_t e = cudaFuncSetAttribute(kv8_decode_kernel<D, NT, HP, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int) KdSmem<D, NT, HP>::bytes(NT * 8));
+    static Kv8Once once;
+    const cudaError_t e = once.smem(kv8_decode_kernel<D, NT, HP, CAP>, KdSmem<D, NT, HP>::bytes(NT * 8));
     return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, HP, CAP>, dim3(ctas), KD_THREADS, smem, stream, p);
 }
 

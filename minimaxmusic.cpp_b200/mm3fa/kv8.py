@@ -21,9 +21,9 @@ from .ggml import GGML_TYPE_BF16, GGML_TYPE_F16, GGML_TYPE_F32
 
 FORK_DEEP = 1  # MM3FA_KV8_FORK_DEEP
 
-_CACHE = struct.Struct("@6i4P")     # struct mm3fa_kv8
-_TABLE = struct.Struct("@Pq2i")     # struct mm3fa_kv8_table
-_TENSOR = struct.Struct("@2i4q4QP")  # struct mm3fa_tensor
+_CACHE = struct.Struct("@6i4P")                 # struct mm3fa_kv8
+_PACK_TABLE = struct.Struct("@Pq2i").pack       # struct mm3fa_kv8_table
+_PACK_TENSOR = struct.Struct("@2i4q4QP").pack   # struct mm3fa_tensor
 
 _fns = None
 
@@ -78,9 +78,12 @@ class Kv8Cache:
         self.n_layers, self.n_pages, self.n_head_kv, self.page_tokens, self.head_dim = k.shape
         self._desc = _CACHE.pack(self.head_dim, self.page_tokens, self.n_head_kv, self.n_pages, self.n_layers, 0,
                                  k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self._torch, self._int32 = torch, torch.int32
         self._dt = _types()
-        self._ws = {}    # (operation, stream) -> zero-filled workspace tensor
-        self._kept = []  # workspaces that were outgrown: a captured graph may still use them
+        self._dev = k.get_device()  # -1: host tensors, on which the C ABI's checks run but no kernel does
+        self._fns = None
+        self._ws = {}    # (operation, stream) -> address and bytes of a zero-filled workspace
+        self._kept = []  # the workspaces, outgrown ones too: a captured graph may still use them
         self._need = {}  # workspace bytes by shape
 
     @classmethod
@@ -95,6 +98,9 @@ class Kv8Cache:
 
     # ------------------------------------------------------------ descriptors
 
+    def _elsewhere(self, t):
+        return ValueError(f"Kv8Cache: a tensor on {t.device}, the cache is on {self.device}")
+
     def _rows(self, t):
         """mm3fa_tensor [D, rows, heads, seqs] of a torch tensor (seqs, heads, rows, D)."""
         if t.dim() != 4:
@@ -102,86 +108,77 @@ class Kv8Cache:
         ty = self._dt.get(t.dtype)
         if ty is None:
             raise MM3FAError(ERR_TYPE, "Kv8Cache")
-        if t.device != self.device:
-            raise ValueError(f"Kv8Cache: a tensor on {t.device}, the cache is on {self.device}")
+        if t.get_device() != self._dev:
+            raise self._elsewhere(t)
         a, b, c, d = t.shape
         sa, sb, sc, sd = t.stride()
         if sd != 1 and d > 1:
             raise MM3FAError(ERR_STRIDE, "Kv8Cache: the head dimension has to be contiguous")
-        e = ty[1]
-        return _TENSOR.pack(ty[0], 0, d, c, b, a, e, sc * e, sb * e, sa * e, t.data_ptr())
+        ty, e = ty
+        return _PACK_TENSOR(ty, 0, d, c, b, a, e, sc * e, sb * e, sa * e, t.data_ptr())
 
     def _table(self, t):
         if t.dim() != 2:
             raise MM3FAError(ERR_SHAPE, "Kv8Cache: table")
+        if t.dtype is not self._int32:
+            raise MM3FAError(ERR_TYPE, "Kv8Cache: table")
+        if t.get_device() != self._dev:
+            raise self._elsewhere(t)
         n, pages = t.shape
-        self._ints(t, None, "table")
         stride, one = t.stride()
         if one != 1 and pages > 1:
             raise MM3FAError(ERR_STRIDE, "Kv8Cache: table")
-        return _TABLE.pack(t.data_ptr(), stride if n > 1 else pages, pages, n)
+        return _PACK_TABLE(t.data_ptr(), stride if n > 1 else pages, pages, n)
 
     def _ints(self, t, n, what):
-        """Address of an int32 tensor of n entries (None: any)."""
-        import torch
-
-        if t.dtype != torch.int32:
+        """Address of an int32 tensor of n entries."""
+        if t.dtype is not self._int32:
             raise MM3FAError(ERR_TYPE, "Kv8Cache: " + what)
-        if t.device != self.device:
-            raise ValueError(f"Kv8Cache: {what} on {t.device}, the cache is on {self.device}")
-        if n is not None:
-            if t.dim() != 1 or t.shape[0] != n:
-                raise MM3FAError(ERR_SHAPE, "Kv8Cache: " + what)
-            if n > 1 and t.stride(0) != 1:
-                raise MM3FAError(ERR_STRIDE, "Kv8Cache: " + what)
+        if t.get_device() != self._dev:
+            raise self._elsewhere(t)
+        if t.dim() != 1 or t.shape[0] != n:
+            raise MM3FAError(ERR_SHAPE, "Kv8Cache: " + what)
+        if n > 1 and t.stride(0) != 1:
+            raise MM3FAError(ERR_STRIDE, "Kv8Cache: " + what)
         return t.data_ptr()
 
     def _stream(self, stream):
-        import torch
-
-        if self.device.type != "cuda":
-            return 0  # host tensors: the C ABI's checks run, no kernel does
-        if stream is not None:
-            return stream.cuda_stream
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        if self._dev < 0:
+            return 0
+        return self._torch._C._cuda_getCurrentRawStream(self._dev) if stream is None else stream.cuda_stream
 
     def _call(self, name, *args):
-        import torch
+        """A library call with the cache's device current; its result."""
+        fn = (self._fns or self._bind())[name]
+        if self._dev < 0 or self._torch._C._cuda_getDevice() == self._dev:
+            return fn(*args)
+        with self._torch.cuda.device(self.device):
+            return fn(*args)
 
-        fn = _calls()[name]
-        if self.device.type == "cuda" and torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
-                st = fn(*args)
-        else:
-            st = fn(*args)
-        if st != OK:
+    def _bind(self):
+        self._fns = _calls()
+        return self._fns
+
+    def _run(self, name, *args):
+        st = self._call(name, *args)
+        if st:
             raise MM3FAError(st, "mm3fa_kv8_" + name)
-
-    def _size(self, name, *args):
-        import torch
-
-        if self.device.type == "cuda" and torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
-                return _calls()[name](*args)
-        return _calls()[name](*args)
 
     def _workspace(self, key, nbytes):
         """(address, bytes) of the workspace of an operation on a stream, zero-filled when it is made."""
-        import torch
-
         buf = self._ws.get(key)
-        if buf is None or buf.numel() < nbytes:
-            if nbytes == 0:
-                return None, 0
+        if buf is not None and buf[1] >= nbytes:
+            return buf
+        torch = self._torch
+        if nbytes > 0:
             made = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=self.device)
-            if made.is_cuda and torch.cuda.is_current_stream_capturing():
-                # it is zeroed by each replay of the graph, so nothing but the graph may use it
-                self._kept.append(made)
-                return made.data_ptr(), made.numel()
-            if buf is not None:
-                self._kept.append(buf)
-            buf = self._ws[key] = made
-        return buf.data_ptr(), buf.numel()
+            self._kept.append(made)
+            at = made.data_ptr(), made.numel()
+            # one made during a capture is zeroed by each replay of the graph: nothing else may use it
+            if self._dev < 0 or not torch.cuda.is_current_stream_capturing():
+                self._ws[key] = at
+            return at
+        return None, 0
 
     # ------------------------------------------------------------ operators
 
@@ -189,7 +186,7 @@ class Kv8Cache:
         """Stores the rows k_new, v_new (N, n_head_kv, T, D), the first n_new[s] (default: T) of sequence s, behind
         its first start[s] tokens.  The pages' scales grow where the rows need it."""
         n = table.shape[0]
-        self._call("append", self._desc, layer, self._rows(k_new), self._rows(v_new), self._table(table),
+        self._run("append", self._desc, layer, self._rows(k_new), self._rows(v_new), self._table(table),
                    self._ints(start, n, "start"), None if n_new is None else self._ints(n_new, n, "n_new"),
                    self._stream(stream))
 
@@ -197,7 +194,7 @@ class Kv8Cache:
         """Values of tokens start[s] .. start[s] + n[s] (default: T) of each sequence into the first rows of
         k_out, v_out (N, n_head_kv, T, D)."""
         ns = table.shape[0]
-        self._call("read", self._desc, layer, self._table(table), self._ints(start, ns, "start"),
+        self._run("read", self._desc, layer, self._table(table), self._ints(start, ns, "start"),
                    None if n is None else self._ints(n, ns, "n"), self._rows(k_out), self._rows(v_out),
                    self._stream(stream))
 
@@ -210,37 +207,35 @@ class Kv8Cache:
         n = table.shape[0]
         qd, td, st = self._rows(q), self._table(table), self._stream(stream)
         if out is None:
-            import torch
-
-            make = torch.empty if q_len is None else torch.zeros
+            make = self._torch.empty if q_len is None else self._torch.zeros
             out = make((q.shape[0], q.shape[2], q.shape[1], q.shape[3]), dtype=q.dtype, device=q.device)
         if ws is None:
             shape = (q.shape[2], q.shape[1], n)
             need = self._need.get(shape)
             if need is None:
-                need = self._need[shape] = self._size("attn_workspace", self._desc, qd, td)
+                need = self._need[shape] = self._call("attn_workspace", self._desc, qd, td)
             ptr, cap = self._workspace(("attn", st), need)
         else:
             ptr, cap = ws.data_ptr(), ws.numel() * ws.element_size()
-        self._call("attn", self._desc, layer, qd, td, self._ints(kv_len, n, "kv_len"),
+        self._run("attn", self._desc, layer, qd, td, self._ints(kv_len, n, "kv_len"),
                    None if q_len is None else self._ints(q_len, n, "q_len"), scale, logit_softcap, 1 if causal else 0,
                    self._rows(out), ptr, cap, st)
         return out
 
     def attend_workspace(self, q, table) -> int:
         """Bytes of the workspace that `attend` needs for these operands."""
-        return self._size("attn_workspace", self._desc, self._rows(q), self._table(table))
+        return self._call("attn_workspace", self._desc, self._rows(q), self._table(table))
 
     def _pages_ws(self, n_seq, stream):
         need = self._need.get(n_seq)
         if need is None:
-            need = self._need[n_seq] = self._size("pages_workspace", self._desc, n_seq)
+            need = self._need[n_seq] = self._call("pages_workspace", self._desc, n_seq)
         return self._workspace(("pages", stream), need)
 
     def reserve(self, table, refs, n_tok, stream=None):
         """Gives each sequence's row of `table` the pages for n_tok[s] tokens (in place)."""
         st, n = self._stream(stream), table.shape[0]
-        self._call("reserve", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
+        self._run("reserve", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
                    self._ints(n_tok, n, "n_tok"), *self._pages_ws(n, st), st)
 
     def fork(self, src, dst, table, kv_len, refs, table_out, kv_len_out, refs_out, deep=False, stream=None):
@@ -248,7 +243,7 @@ class Kv8Cache:
         `deep`.  The results go to the *_out tensors, which may not overlap the others."""
         st, n = self._stream(stream), table.shape[0]
         pairs = dst.shape[0]
-        self._call("fork", self._desc, self._table(table), self._ints(kv_len, n, "kv_len"),
+        self._run("fork", self._desc, self._table(table), self._ints(kv_len, n, "kv_len"),
                    self._ints(refs, self.n_pages, "refs"), None if src is None else self._ints(src, pairs, "src"),
                    self._ints(dst, pairs, "dst"), pairs, FORK_DEEP if deep else 0, self._table(table_out),
                    self._ints(kv_len_out, n, "kv_len_out"), self._ints(refs_out, self.n_pages, "refs_out"),
@@ -261,7 +256,7 @@ class Kv8Cache:
     def compact(self, table, refs, table_out, refs_out, stream=None):
         """Moves the live pages to the front of the pool; the results go to the *_out tensors."""
         st, n = self._stream(stream), table.shape[0]
-        self._call("compact", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
+        self._run("compact", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
                    self._table(table_out), self._ints(refs_out, self.n_pages, "refs_out"), *self._pages_ws(n, st), st)
 
     def check(self, stream=None):
@@ -271,6 +266,6 @@ class Kv8Cache:
         for op in ("pages", "attn"):
             buf = self._ws.get((op, st))
             if buf is not None:
-                status, _ = workspace_status(buf.data_ptr(), st)
+                status, _ = workspace_status(buf[0], st)
                 if status != OK:
                     raise MM3FAError(status, "Kv8Cache")

@@ -40,7 +40,7 @@ def test_unsupported_sizes(D, P):
     x = torch.zeros(1, 2, 1, D)
     assert status(c.append, 0, x, x, t, n) == mm3fa.ERR_UNSUPPORTED
     assert status(c.reserve, t, torch.zeros(4, dtype=torch.int32), n) == mm3fa.ERR_UNSUPPORTED
-    assert c._size("pages_workspace", c._desc, 1) == 0
+    assert c._call("pages_workspace", c._desc, 1) == 0
 
 
 @no_gpu
@@ -132,7 +132,7 @@ def test_page_operation_refusals():
     args = lambda flags, nbytes: g(c._desc, c._table(s.table), s.len.data_ptr(), s.refs.data_ptr(), pair[0].data_ptr(),
                                    pair[1].data_ptr(), 1, flags, c._table(t2), l2.data_ptr(), r2.data_ptr(),
                                    ws.data_ptr(), nbytes, None)
-    need = c._size("pages_workspace", c._desc, 2)
+    need = c._call("pages_workspace", c._desc, 2)
     assert args(0, need) == mm3fa.ERR_DEVICE
     assert args(0, need - 1) == mm3fa.ERR_WORKSPACE
     assert args(2, need) == mm3fa.ERR_UNSUPPORTED
