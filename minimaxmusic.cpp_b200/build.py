@@ -21,7 +21,7 @@ LIB = os.path.join(LIBDIR, "libmm3fa.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["mm3fa_abi.cu", "fa_decode.cu", "fa_decode_mma.cu", "fa_dense_sm100.cu", "fa_prologue.cu", "mm3fa_noalloc.cu",
-           "mm3fa_exchange.cu", "kv8_abi.cu", "kv8_attn.cu", "kv8_pages.cu", "kv8_store.cu"]
+           "mm3fa_exchange.cu", "kv8_abi.cu", "kv8_attn.cu", "kv8_dense_sm100.cu", "kv8_pages.cu", "kv8_store.cu"]
 HEADERS = ["fa_common.cuh", "fa_decode.cuh", "fa_dense.cuh", "fa_prologue.cuh", "kv8.cuh", "tc_sm100.cuh"]
 
 NVCC_FLAGS = [

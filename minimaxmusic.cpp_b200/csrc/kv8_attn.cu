@@ -36,6 +36,7 @@ constexpr int KD_OFF     = 12;     // P is held times 2^12: F16 keeps 11 bits do
 constexpr int KD_WHOLE   = 16;
 constexpr int KD_PART    = 8;      // blocks of a part, at least
 constexpr int KD_CROSS   = 8;
+constexpr int KD_DENSE   = 64;     // rows of a kv head from which the kernel for many rows takes over (D <= 128)
 
 template <int D, int NT, bool HP>
 struct KdSmem {
@@ -931,6 +932,9 @@ size_t kv8_attn_workspace_bytes(int D, int n_q, int ratio, int n_head_kv, int n_
 
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p0, int sms, cudaStream_t stream) {
     Kv8AttnParams p    = p0;
+    if (p.c.D <= 128 && p.ratio * p.n_q >= KD_DENSE) {
+        return launch_kv8_dense(p, stream);
+    }
     const int     most = sms * ctas_per_sm(p.c.D, p.ratio * p.n_q);
     p.counters = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.status) + WS_STATUS_BYTES);
     p.part     = reinterpret_cast<float *>(reinterpret_cast<char *>(p.counters) + ((size_t) most * 4 + 255) / 256 * 256);

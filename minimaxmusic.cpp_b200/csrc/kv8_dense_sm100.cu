@@ -1,0 +1,694 @@
+// kv8_dense_sm100.cu - attention over the 8-bit paged KV cache for many query rows (prefill, chunks of a
+// prompt) on the 5th-generation tensor cores (tcgen05 + TMEM), sm_100a.
+//
+// One CTA per (256 rows, kv head, sequence), the rows being (query, head of the group) pairs in that order,
+// so that all query heads of a kv head share each K/V tile; two 128-row tiles t of Q.  512 threads:
+//   warpgroup 0   converts: codes of a 128-key tile go from global memory through registers (loaded one tile
+//                 ahead) into F16, which holds them exactly, in 128-byte-swizzled shared memory; the
+//                 scales of the tile's pages beside them.
+//   warpgroup 1   its first warp allocates TMEM and issues every tcgen05.mma:
+//                   S_t = Q_t K^T (columns [128t, 128t + 128)),  O_t += P_t V (columns [256 + D t, ...)),
+//                 P_t in TMEM over S_t, in the order QK0(j), PV1(j-1), QK1(j), PV0(j): one tile's softmax
+//                 runs beside the other's products.
+//   warpgroups 2, 3  softmax of tile 0, 1: one row per thread.
+// Q is brought to [1, 2) at its row's largest element by a power of two and rounded to F16; for an F32 result
+// (HP) the F16 remainder is a second operand, as is that of P: both products then run twice.
+//
+// Softmax.  s = S * (row factor * key scale of the column's page), in log2 units; weights 2^(s - m); the
+// value scale b = f 2^e of a page is multiplied into them, P = 2^(s - m) * 2^(m + e - R + KE_OFF) * f, so
+// that O is in units of 2^(R - KE_OFF).  m and R (the largest s + e of any page) are lazy: they follow only
+// when they would grow by more than 8 and 4, which F16's range allows, and O in TMEM is multiplied then.
+//
+// Bound: the exponentials (16 a cycle and SM: 2048 cycles for a tile pair), the products (1024 cycles at
+// D = 128, twice that for HP) and the issue of the conversions (about 400 slots per scheduler) overlap.
+#include "kv8.cuh"
+#include "tc_sm100.cuh"
+
+namespace mm3fa {
+
+constexpr int KE_THREADS = 512;
+constexpr int KE_M       = 128;  // rows per Q tile
+constexpr int KE_ROWS    = 256;
+constexpr int KE_N       = 128;  // keys per tile
+constexpr int KE_TMEM    = 512;
+constexpr int KE_OFF     = 8;    // P is held times 2^8: 2^14 at most with the lazy maxima
+constexpr int KE_EMU     = 3;    // of every 8 pairs of weights, those by polynomial where P is rounded to F16 anyway
+constexpr int KE_REGS_LAUNCH  = 128;  // 65536 / 512
+constexpr int KE_REGS_SOFTMAX = 192;  // 2 x 192 + 96 + 32 = 4 x 128
+constexpr int KE_REGS_CONVERT = 96;
+constexpr int KE_REGS_ISSUE   = 32;
+static_assert(2 * KE_REGS_SOFTMAX + KE_REGS_CONVERT + KE_REGS_ISSUE <= 4 * KE_REGS_LAUNCH, "more registers than the launch has");
+
+template <int D, bool HP>
+struct KeSmem {
+    static constexpr int HALVES = D / 64;             // 128-byte column blocks
+    static constexpr int QT     = HALVES * KE_M * 128;
+    static constexpr int KT     = HALVES * KE_N * 128;
+    static constexpr int QP     = HP ? 2 : 1;         // F16 parts of Q
+    static constexpr int NK     = 2;
+    static constexpr int NV     = D == 128 && HP ? 1 : 2;
+    static constexpr int OFF_Q    = 0;                           // [tile][part]
+    static constexpr int OFF_K    = OFF_Q + 2 * QP * QT;         // [NK]
+    static constexpr int OFF_V    = OFF_K + NK * KT;             // [NV]
+    static constexpr int OFF_SC   = OFF_V + NV * KT;             // [4 tiles][8 groups] (a, f, e, present)
+    static constexpr int OFF_BAR  = OFF_SC + 4 * 8 * 16;
+    static constexpr int OFF_MISC = OFF_BAR + 24 * 8;
+    static constexpr int TOTAL    = OFF_MISC + 32 + 1024;        // + alignment
+};
+
+enum : int {
+    KB_KFULL  = 0,   // [2] 128 converting threads
+    KB_KEMPTY = 2,   // [2]
+    KB_VFULL  = 4,   // [2]
+    KB_VEMPTY = 6,   // [2]
+    KB_SFULL  = 8,   // [2] per Q tile
+    KB_PREADY = 10,  // [2] 128 softmax threads
+    KB_ODONE  = 12,  // [2]
+    KB_QREADY = 14,  // [2] 128 softmax threads
+    KB_SCALES = 16,  // [4] 8 converting threads: a ring deeper than K's, for a softmax that is behind the products
+    KB_DONE   = 20,
+    KB_COUNT  = 21,
+};
+
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t ke_pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 16 codes -> 16 F16 numbers (0x6400 | u is 1024 + u; less 1152 the code)
+__device__ __forceinline__ void ke_convert(const uint4 & c, uint4 & lo, uint4 & hi) {
+    const uint32_t bias = 0x64806480u;
+    uint32_t       w[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t u = (&c.x)[i] ^ 0x80808080u;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint32_t x = __byte_perm(u, 0x64646464u, k ? 0x4342 : 0x4140);
+            const __half2  h = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&bias));
+            w[2 * i + k]     = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    }
+    lo = make_uint4(w[0], w[1], w[2], w[3]);
+    hi = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// kind::f16 instruction descriptor: F16 x F16 -> F32, M = 128
+__host__ __device__ constexpr uint32_t ke_idesc(int n, bool b_mn_major) {
+    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (KE_M >> 4) << 24);
+}
+
+template <int D, bool HP, bool CAP>
+__global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnParams p) {
+    using L          = KeSmem<D, HP>;
+    constexpr int NK = L::NK, NV = L::NV;
+    extern __shared__ __align__(16) char smem_raw[];
+    char *     smem      = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    uint64_t * bar       = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
+    int *      abort_f   = reinterpret_cast<int *>(smem + L::OFF_MISC + 4);
+    float4 *   scales    = reinterpret_cast<float4 *>(smem + L::OFF_SC);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
+    if (tid == 0) {
+        for (int i = 0; i < KB_COUNT; i++) {
+            const bool grp = i < KB_KEMPTY || (i >= KB_VFULL && i < KB_VEMPTY) || (i >= KB_PREADY && i < KB_ODONE) ||
+                             (i >= KB_QREADY && i < KB_SCALES);
+            mbar_init(&bar[i], grp ? 128u : (i >= KB_SCALES && i < KB_DONE ? 8u : 1u));
+        }
+        *abort_f = 0;
+        fence_mbar_init();
+    }
+    if (warp == 4) {
+        tmem_alloc(tmem_slot, KE_TMEM);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem     = *tmem_slot;
+    const uint64_t deadline = global_timer_ns() + p.timeout_ns;
+    kv8_dep_wait();
+
+    // ---- the work item: row blocks last first, so that the longest causal ones start first
+    const int hs = p.c.n_head_kv * p.t.n_seq, all_rows = p.ratio * p.n_q;
+    const int blk = (all_rows + KE_ROWS - 1) / KE_ROWS - 1 - (int) blockIdx.x / hs;
+    const int h = (int) blockIdx.x % hs % p.c.n_head_kv, s = (int) blockIdx.x % hs / p.c.n_head_kv;
+    const int nq = p.q_len ? min(max(p.q_len[s], 0), p.n_q) : p.n_q;
+    const int n  = min(max(p.kv_len[s], 0), p.t.max_pages * p.c.P);
+    const int row0 = blk * KE_ROWS, rows = min(nq * p.ratio - row0, KE_ROWS);  // rows of this block
+    const bool two = rows > KE_M;
+    // keys that its last row sees
+    const int q_last = rows > 0 ? (row0 + rows - 1) / p.ratio : 0;
+    const int keys   = rows > 0 ? (p.causal ? max(n - (nq - 1 - q_last), 0) : n) : 0;
+    const int tiles  = (keys + KE_N - 1) / KE_N;
+
+    if (wg == 0) {
+        // ======================================================= conversion
+        regs_dec<KE_REGS_CONVERT>();
+        constexpr int LD = D / 16 * KE_N / 128;  // 16-code pieces per thread and tile
+        // thread: rows 32 warp + 8 i + (lane & 7), pieces (lane >> 3) + 4 k: a warp reads whole 64-byte runs, and the
+        // stores of eight lanes fall into eight rows, so into different banks
+        const int * row = p.t.pages + (int64_t) s * p.t.stride;
+        int         pg0 = -1, pg1 = -1;
+        auto        fetch = [&](int j) {  // table entries of the warp's 32 rows of tile j
+            const int k0 = j * KE_N + 32 * warp, i = k0 >> p.c.log2p;
+            pg0 = k0 < keys ? row[i] : -1;
+            pg1 = p.c.log2p == 4 ? (k0 + 16 < keys ? row[i + 1] : -1) : pg0;
+        };
+        uint4 kx[LD], vx[LD];
+        auto  load = [&](int j, const int8_t * pool, uint4 (&x)[LD]) {
+#pragma unroll
+            for (int i = 0; i < LD; i++) {
+                const int  rr = 8 * (i & 3) + (lane & 7), pc = (lane >> 3) + 4 * (i >> 2);
+                const int  pg = (i & 3) < 2 ? pg0 : pg1;
+                const bool ok = (unsigned) pg < (unsigned) p.c.n_pages;
+                const int64_t at = (((int64_t) (ok ? pg : 0) * p.c.n_head_kv + h) * p.c.P + ((j * KE_N + 32 * warp + rr) & (p.c.P - 1))) * D + pc * 16;
+                x[i] = make_uint4(0, 0, 0, 0);
+                if (ok) {
+                    x[i] = __ldg(reinterpret_cast<const uint4 *>(pool + at));
+                }
+            }
+        };
+        auto store = [&](char * tile, const uint4 (&x)[LD]) {
+#pragma unroll
+            for (int i = 0; i < LD; i++) {
+                const int rr = 32 * warp + 8 * (i & 3) + (lane & 7), pc = (lane >> 3) + 4 * (i >> 2);
+                uint4     a, b;
+                ke_convert(x[i], a, b);
+                char * to = tile + (pc >> 2) * (KE_N * 128);
+                *reinterpret_cast<uint4 *>(to + sw128_off(rr, 2 * (pc & 3)))     = a;
+                *reinterpret_cast<uint4 *>(to + sw128_off(rr, 2 * (pc & 3) + 1)) = b;
+            }
+        };
+        bool ok = true;
+        if (tiles > 0) {
+            fetch(0);
+            load(0, p.c.k, kx);
+            load(0, p.c.v, vx);
+        }
+        for (int j = 0; j < tiles; j++) {
+            const int sk = j % NK, sv = j % NV;
+            if (j + 1 < tiles) {
+                fetch(j + 1);
+            }
+            float4 sc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (tid < 8) {  // 16-key groups of the tile
+                const int k0 = j * KE_N + 16 * tid, pg = k0 < keys ? row[k0 >> p.c.log2p] : -1;
+                if ((unsigned) pg < (unsigned) p.c.n_pages) {
+                    const int64_t ph = (int64_t) pg * p.c.n_head_kv + h;
+                    const float   v  = p.c.v_scale[ph];
+                    const int     e  = min(max((int) (__float_as_uint(v) >> 23 & 255u) - 127, -126), 126);
+                    sc = make_float4(p.c.k_scale[ph], v * __uint_as_float((uint32_t) (127 - e) << 23), (float) e, 1.0f);
+                }
+            }
+            if (j >= NK && !mbar_wait_bounded(&bar[KB_KEMPTY + sk], (uint32_t) ((j / NK - 1) & 1), deadline)) {
+                ok = false;
+                break;
+            }
+            if (tid < 8) {
+                scales[(j & 3) * 8 + tid] = sc;
+                dn_mbar_arrive(&bar[KB_SCALES + (j & 3)]);
+            }
+            store(smem + L::OFF_K + sk * L::KT, kx);
+            fence_proxy_async_smem();
+            dn_mbar_arrive(&bar[KB_KFULL + sk]);
+            if (j + 1 < tiles) {
+                load(j + 1, p.c.k, kx);
+            }
+            if (j >= NV && !mbar_wait_bounded(&bar[KB_VEMPTY + sv], (uint32_t) ((j / NV - 1) & 1), deadline)) {
+                ok = false;
+                break;
+            }
+            store(smem + L::OFF_V + sv * L::KT, vx);
+            fence_proxy_async_smem();
+            dn_mbar_arrive(&bar[KB_VFULL + sv]);
+            if (j + 1 < tiles) {
+                load(j + 1, p.c.v, vx);
+            }
+        }
+        if (!ok) {
+            atomicExch(abort_f, 1);
+        }
+    } else if (wg == 1) {
+        // ======================================================= MMA issue (one warp, elected lane)
+        regs_dec<KE_REGS_ISSUE>();
+        if (warp == 4) {
+            const uint32_t id_qk = ke_idesc(KE_N, false), id_pv = ke_idesc(D, true);
+            // descriptors of the buffers' first bytes; an offset adds to the address field (16-byte units)
+            const uint64_t q_d = sw128_desc(smem_addr(smem + L::OFF_Q), 16, 1024), k_d = sw128_desc(smem_addr(smem + L::OFF_K), 16, 1024);
+            const uint64_t v_d = sw128_desc(smem_addr(smem + L::OFF_V), (uint32_t) (KE_N * 128), 1024);
+            auto           qk  = [&](int t, int j) {
+                uint64_t a = q_d + (uint64_t) ((t * L::QP * L::QT) >> 4);
+                // rolled loops: unrolled ones keep every descriptor in registers that this warpgroup does not have
+#pragma unroll 1
+                for (int part = 0; part < L::QP; part++) {
+                    uint64_t b = k_d + (uint64_t) (((j % NK) * L::KT) >> 4);
+#pragma unroll 1
+                    for (int c = 0; c < L::HALVES; c++) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            umma_f16(tmem + (uint32_t) (t * KE_N), a + (uint64_t) (2 * k), b + (uint64_t) (2 * k), id_qk, part + c + k > 0 ? 1u : 0u);
+                        }
+                        a += (KE_M * 128) >> 4, b += (KE_N * 128) >> 4;
+                    }
+                }
+                umma_commit(&bar[KB_SFULL + t]);
+            };
+            auto pv = [&](int t, int j) {
+                uint32_t a = tmem + (uint32_t) (t * KE_N);
+#pragma unroll 1
+                for (int part = 0; part < L::QP; part++) {
+                    uint64_t b = v_d + (uint64_t) (((j % NV) * L::KT) >> 4);
+#pragma unroll 1
+                    for (int c = 0; c < 2; c++) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            umma_f16_ts(tmem + 256u + (uint32_t) (t * D), a + (uint32_t) (8 * k), b + (uint64_t) ((k * 16 * 128) >> 4), id_pv,
+                                        j + part + c + k > 0 ? 1u : 0u);
+                        }
+                        a += 32, b += (4 * 16 * 128) >> 4;
+                    }
+                }
+            };
+            auto wait = [&](int b, int i) {
+                const bool ok = dn_wait_warp(&bar[b], (uint32_t) (i & 1), deadline);
+                tc_fence_after();
+                return ok;
+            };
+            bool ok = true;
+            if (tiles > 0) {
+                ok = wait(KB_QREADY, 0) && wait(KB_KFULL, 0);
+                if (ok) {
+                    qk(0, 0);
+                    if (two) {
+                        ok = wait(KB_QREADY + 1, 0);
+                        if (ok) {
+                            qk(1, 0);
+                        }
+                    }
+                    umma_commit(&bar[KB_KEMPTY]);
+                }
+                for (int j = 0; ok && j < tiles; j++) {
+                    const bool next = j + 1 < tiles;
+                    ok = wait(KB_VFULL + j % NV, j / NV) && wait(KB_PREADY, j);
+                    if (!ok) {
+                        break;
+                    }
+                    pv(0, j);
+                    if (next) {
+                        ok = wait(KB_KFULL + (j + 1) % NK, (j + 1) / NK);
+                        if (!ok) {
+                            break;
+                        }
+                        qk(0, j + 1);
+                    } else {
+                        umma_commit(&bar[KB_ODONE]);
+                    }
+                    if (two) {
+                        ok = wait(KB_PREADY + 1, j);
+                        if (!ok) {
+                            break;
+                        }
+                        pv(1, j);
+                        umma_commit(&bar[KB_VEMPTY + j % NV]);
+                        if (next) {
+                            qk(1, j + 1);
+                        } else {
+                            umma_commit(&bar[KB_ODONE + 1]);
+                        }
+                    } else {
+                        umma_commit(&bar[KB_VEMPTY + j % NV]);
+                    }
+                    if (next) {
+                        umma_commit(&bar[KB_KEMPTY + (j + 1) % NK]);
+                    }
+                }
+            }
+            if (!ok) {
+                atomicExch(abort_f, 1);
+            }
+            // every MMA issued has to be complete before TMEM and shared memory are given up
+            umma_commit(&bar[KB_DONE]);
+            dn_wait_warp(&bar[KB_DONE], 0, global_timer_ns() + p.timeout_ns);
+        }
+    } else {
+        // ======================================================= softmax
+        regs_inc<KE_REGS_SOFTMAX>();
+        const int      t = wg - 2, quad = warp & 3, r = quad * 32 + lane;  // Q tile, TMEM lane quadrant, row of the tile
+        const uint32_t tl    = (uint32_t) (quad * 32) << 16;
+        const uint32_t s_col = tmem + tl + (uint32_t) (t * KE_N);
+        const uint32_t o_col = tmem + tl + 256u + (uint32_t) (t * D);
+        const int      tile_rows = min(rows - t * KE_M, KE_M);  // may be 0 or less
+        if (tile_rows > 0) {
+            // ---- Q: the warp's 32 rows, whole rows at a time
+            float factor = 0.0f;  // of this thread's row
+            char * qs    = smem + L::OFF_Q + t * L::QP * L::QT;
+            constexpr int E = D / 32;
+#pragma unroll 4
+            for (int it = 0; it < 32; it++) {
+                const int rr = quad * 32 + it, rw = row0 + t * KE_M + rr;
+                const int qi = rw / p.ratio, hq = h * p.ratio + rw - qi * p.ratio;
+                float     x[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    x[e] = 0.0f;
+                }
+                if (rr < tile_rows) {
+                    const char * src = p.q.data + (int64_t) qi * p.q.nb1 + (int64_t) hq * p.q.nb2 + (int64_t) s * p.q.nb3;
+                    if (p.q.type == KV_F32) {
+                        if (p.q.vec) {
+#pragma unroll
+                            for (int e = 0; e < E; e += 2) {
+                                const float2 f = reinterpret_cast<const float2 *>(src)[(lane * E + e) / 2];
+                                x[e] = f.x, x[e + 1] = f.y;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < E; e++) {
+                                x[e] = reinterpret_cast<const float *>(src)[lane * E + e];
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            const uint16_t u = reinterpret_cast<const uint16_t *>(src)[lane * E + e];
+                            x[e] = p.q.type == KV_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t) u << 16);
+                        }
+                    }
+                }
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                // the exponent of the largest element; a row with an infinity or NaN gives NaN
+                const bool  odd = top >= 0x7f800000u;
+                const int   ex  = top == 0 || odd ? 0 : min(max((int) (top >> 23) - 127, -126), 126);
+                const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23);
+                if (it == lane) {
+                    factor = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * (CAP ? p.scale / p.softcap : p.scale * LOG2E);
+                }
+                const int e0 = lane * E, hb = e0 / 64, ch = (e0 % 64) / 8, sub = (e0 % 8) * 2;
+                char *    to = qs + hb * (KE_M * 128) + sw128_off(rr, ch) + sub;
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float    a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
+                    const uint32_t w = ke_pack(a, b);
+                    *reinterpret_cast<uint32_t *>(to + 2 * e) = w;
+                    if (HP) {
+                        const float2 f = h2_to_f2(w);
+                        *reinterpret_cast<uint32_t *>(to + L::QT + 2 * e) = ke_pack(a - f.x, b - f.y);
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            dn_mbar_arrive(&bar[KB_QREADY + t]);
+
+            const int  rw    = row0 + t * KE_M + r;
+            const bool live  = r < tile_rows;
+            const int  my_q  = rw / p.ratio;
+            const int  lim   = !live ? 0 : p.causal ? n - (nq - 1 - my_q) : n;  // keys of this row
+            const int  warp_lim = (int) __reduce_min_sync(0xffffffffu, (unsigned) (live ? max(lim, 0) : 0x7fffffff));
+            float      m = -INFINITY, l = 0.0f, R = -INFINITY;
+            bool       ok = true;
+            for (int j = 0; j < tiles; j++) {
+                if (!dn_wait_warp(&bar[KB_SCALES + (j & 3)], (uint32_t) ((j >> 2) & 1), deadline) ||
+                    !dn_wait_warp(&bar[KB_SFULL + t], (uint32_t) (j & 1), deadline)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const float4 * sc  = scales + (j & 3) * 8;
+                const int      left = lim - j * KE_N;  // columns that the row sees
+                if (CAP) {
+                    // s = cap * tanh(S * factor * a), written back; the pass below takes it as it is
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t v[32];
+                        tmem_ld32(s_col + (uint32_t) (c * 32), v);
+                        tmem_ld_wait_tie(v);
+                        const float a0 = factor * sc[2 * c].x, a1 = factor * sc[2 * c + 1].x, cap = p.softcap * LOG2E;
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            v[e] = __float_as_uint(cap * tanhf(__uint_as_float(v[e]) * (e < 16 ? a0 : a1)));
+                        }
+                        tmem_st32(s_col + (uint32_t) (c * 32), v);
+                    }
+                    tmem_st_wait();
+                }
+                uint32_t sr[KE_N];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    tmem_ld32(s_col + (uint32_t) (c * 32), &sr[c * 32]);
+                }
+                bool whole = j * KE_N + KE_N <= warp_lim;  // every row of the warp sees every column
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    whole &= sc[g].w != 0.0f;
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    tmem_ld_wait_tie(&sr[c * 32]);
+                }
+                if (!CAP) {
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        const float    a  = factor * sc[g].x;
+                        const uint64_t a2 = f2pack(a, a);
+#pragma unroll
+                        for (int e = 16 * g; e < 16 * g + 16; e += 2) {
+                            float x, y;
+                            f2unpack(fmul2(f2pack(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), a2), x, y);
+                            sr[e] = __float_as_uint(x), sr[e + 1] = __float_as_uint(y);
+                        }
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        const int lg = sc[g].w != 0.0f ? left : 0;
+#pragma unroll
+                        for (int e = 16 * g; e < 16 * g + 16; e++) {
+                            sr[e] = e < lg ? sr[e] : 0xff800000u;
+                        }
+                    }
+                }
+                // the row's largest s, and the largest s + e over pages with a value scale
+                float top = -INFINITY, rtop = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    float a = __uint_as_float(sr[16 * g]), b = __uint_as_float(sr[16 * g + 1]);
+#pragma unroll
+                    for (int e = 16 * g + 2; e < 16 * g + 14; e += 4) {
+                        a = fmax3(a, __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+                        b = fmax3(b, __uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3]));
+                    }
+                    a    = fmaxf(fmax3(a, __uint_as_float(sr[16 * g + 14]), __uint_as_float(sr[16 * g + 15])), b);
+                    top  = fmaxf(top, a);
+                    rtop = sc[g].y != 0.0f ? fmaxf(rtop, a + sc[g].z) : rtop;
+                }
+                if (top > m + 8.0f) {
+                    l *= ex2(m - top);
+                    m = top;
+                }
+                float grow = 1.0f;
+                if (rtop > R + 4.0f) {
+                    grow = ex2(R - rtop);
+                    R    = rtop;
+                }
+                const float    ms = m == -INFINITY ? 0.0f : m, rs = R == -INFINITY ? 0.0f : R;
+                const uint64_t nm = f2pack(-ms, -ms);
+                uint64_t       acc[2] = { 0ull, 0ull };
+                uint32_t       pk[KE_N / 2], pl[HP ? KE_N / 2 : 1];
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    const float    f  = ex2(fminf(ms + sc[g].z - rs + KE_OFF, 90.0f)) * sc[g].y;
+                    const uint64_t f2 = f2pack(f, f);
+#pragma unroll
+                    for (int i = 8 * g; i < 8 * g + 8; i++) {
+                        const uint64_t x2 = fadd2(f2pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), nm);
+                        uint64_t       w2;
+                        if (!HP && (i & 7) < KE_EMU) {
+                            w2 = exp2_poly2(x2);
+                        } else {
+                            float x, y;
+                            f2unpack(x2, x, y);
+                            w2 = f2pack(ex2(x), ex2(y));
+                        }
+                        acc[i & 1] = fadd2(acc[i & 1], w2);
+                        float x, y;
+                        f2unpack(fmul2(w2, f2), x, y);
+                        pk[i] = ke_pack(x, y);
+                        if (HP) {
+                            const float2 b = h2_to_f2(pk[i]);
+                            pl[i]          = ke_pack(x - b.x, y - b.y);
+                        }
+                    }
+                }
+                float a0, a1;
+                f2unpack(fadd2(acc[0], acc[1]), a0, a1);
+                l += a0 + a1;
+                tmem_st32(s_col, &pk[0]);
+                tmem_st32(s_col + 32, &pk[32]);
+                if (HP) {
+                    tmem_st32(s_col + 64, &pl[0]);
+                    tmem_st32(s_col + 96, &pl[HP ? 32 : 0]);
+                }
+                // PV(j - 1) is complete: QK(j) was issued after it
+                if (j > 0 && __any_sync(0xffffffffu, grow != 1.0f)) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t o[32];
+                        tmem_ld32(o_col + (uint32_t) (c * 32), o);
+                        tmem_ld_wait_tie(o);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * grow);
+                        }
+                        tmem_st32(o_col + (uint32_t) (c * 32), o);
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                dn_mbar_arrive(&bar[KB_PREADY + t]);
+            }
+            bool have = ok && tiles > 0;
+            if (have) {
+                have = dn_wait_warp(&bar[KB_ODONE + t], 0, deadline);
+                tc_fence_after();
+            }
+            // Q's shared memory takes the result: every product has to be done, and every warp with its rows of Q
+            // (which no product waited for where there are no tiles)
+            if (!dn_wait_warp(&bar[KB_DONE], 0, deadline) || !dn_wait_warp(&bar[KB_QREADY + t], 0, deadline) || (!have && tiles > 0)) {
+                atomicExch(abort_f, 1);
+                have = false;
+            }
+            // ---- O (units of 2^(R - KE_OFF)) over the sum (2^m); the warp stores its rows one after another, each as
+            // one run of bytes.  Rows without keys, and without a value scale, are 0
+            const float inv = l != 0.0f ? (1.0f / (1 << KE_OFF)) / l : 0.0f, up = R == -INFINITY ? 0.0f : ex2(R - m);
+            char *      mine = qs + quad * 32 * (D * (HP ? 4 : 2));  // [32 rows][D] of the result's type
+            const int   esz  = HP ? 4 : 2;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t o[32];
+                if (have) {
+                    tmem_ld32(o_col + (uint32_t) (c * 32), o);
+                    tmem_ld_wait_tie(o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        o[e] = 0u;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    o[e] = __float_as_uint(have ? __uint_as_float(o[e]) * inv * up : 0.0f);
+                }
+                // 16-byte chunks, swizzled by the row against bank conflicts
+                constexpr int PER = HP ? 4 : 8;
+#pragma unroll
+                for (int k = 0; k < 32 / PER; k++) {
+                    uint4 w;
+                    if (HP) {
+                        w = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    } else {
+                        uint32_t u[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float x = __uint_as_float(o[(8 * k + 2 * i) & 31]), y = __uint_as_float(o[(8 * k + 2 * i + 1) & 31]);
+                            if (p.o.type == KV_F16) {
+                                u[i] = ke_pack(x, y);
+                            } else {
+                                const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+                                u[i] = *reinterpret_cast<const uint32_t *>(&b);
+                            }
+                        }
+                        w = make_uint4(u[0], u[1], u[2], u[3]);
+                    }
+                    const int ck = c * (32 / PER) + k;
+                    *reinterpret_cast<uint4 *>(mine + lane * (D * esz) + ((ck ^ (lane & 7)) << 4)) = w;
+                }
+            }
+            __syncwarp();
+            constexpr int CK = D * (HP ? 4 : 2) / 16;  // chunks of a row: 8, 16 or 32
+#pragma unroll 1
+            for (int it = 0; it < CK; it++) {
+                const int i = it * (32 / CK) + lane / CK, ck = lane % CK;  // row of the warp, chunk
+                const int rw = row0 + t * KE_M + quad * 32 + i;
+                if (quad * 32 + i >= tile_rows) {
+                    continue;
+                }
+                const int   qi = rw / p.ratio, hq = h * p.ratio + rw - qi * p.ratio;
+                char *      dst = p.o.data + (int64_t) hq * p.o.nb1 + (int64_t) qi * p.o.nb2 + (int64_t) s * p.o.nb3 + ck * 16;
+                const uint4 w   = *reinterpret_cast<const uint4 *>(mine + i * (D * esz) + ((ck ^ (i & 7)) << 4));
+                if (p.o.vec) {
+                    *reinterpret_cast<uint4 *>(dst) = w;
+                } else if (HP) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        reinterpret_cast<uint32_t *>(dst)[e] = (&w.x)[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t) ((&w.x)[e >> 1] >> (16 * (e & 1)));
+                    }
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        tmem_dealloc(tmem, KE_TMEM);
+    }
+    if (tid == 0 && *abort_f) {
+        atomicOr(&p.status[0], ST_TIMEOUT);
+        atomicExch(&p.status[1], blockIdx.x);
+    }
+}
+
+namespace {
+
+template <int D, bool HP, bool CAP>
+cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, cudaStream_t stream) {
+    auto            kern = kv8_dense_kernel<D, HP, CAP>;
+    static Kv8Once  once;
+    static const int regs = [&] {
+        cudaFuncAttributes a{};
+        return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
+    }();
+    // the register split draws on what the launch gives: another count would wait for registers that never come
+    if (regs != KE_REGS_LAUNCH) {
+        return cudaErrorInvalidConfiguration;
+    }
+    const cudaError_t e = once.smem(kern, KeSmem<D, HP>::TOTAL);
+    return e != cudaSuccess ? e : kv8_launch(kern, dim3(ctas), KE_THREADS, KeSmem<D, HP>::TOTAL, stream, p);
+}
+
+template <int D>
+cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, cudaStream_t stream) {
+    if (p.o.type == KV_F32) {
+        return p.softcap > 0.0f ? launch_one<D, true, true>(p, ctas, stream) : launch_one<D, true, false>(p, ctas, stream);
+    }
+    return p.softcap > 0.0f ? launch_one<D, false, true>(p, ctas, stream) : launch_one<D, false, false>(p, ctas, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_dense(const Kv8AttnParams & p, cudaStream_t stream) {
+    const int64_t rows = (int64_t) p.ratio * p.n_q, ctas = (rows + KE_ROWS - 1) / KE_ROWS * p.c.n_head_kv * p.t.n_seq;
+    return p.c.D == 64 ? launch_d<64>(p, (unsigned) ctas, stream) : launch_d<128>(p, (unsigned) ctas, stream);
+}
+
+}  // namespace mm3fa
