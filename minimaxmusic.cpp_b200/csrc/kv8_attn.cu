@@ -9,8 +9,8 @@
 //   * P . c in F16, which holds the codes exactly.  The value scale of a page goes into the weights,
 //     P = 2^(s - m) * 2^(m + e - R) * f with b = f 2^e, f in [1, 2), and R the running maximum of (a tile's
 //     largest s) + e: O is held in units of 2^R, the sum in units of 2^m, so that pages with scales of
-//     any size stay in F16's range.  Weights are rounded to F16 (half a step: 2^-12), and their remainder
-//     too when the result is F32.  O, sums and maxima are F32.
+//     any size stay in F16's range.  Weights are rounded to F16 (half a step: 2^-12), which
+//     is below what a BF16 result keeps; for F32 and F16 results their remainder is a second operand.  O, sums and maxima are F32.
 //
 // Work.  A unit is (sequence, kv head, 16 query rows): rows of all query heads of the group share the
 // cache's bytes.  A unit's keys come in blocks of 32.  Every CTA finds its work from the lengths on the
@@ -179,7 +179,8 @@ struct KdPart {
     int s, u, c0, n;
 };
 
-template <int D, int NT, bool HP, bool CAP>
+// HP: an F32 result; PL: the weights' remainders too
+template <int D, int NT, bool HP, bool PL, bool CAP>
 __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decode_kernel(const Kv8AttnParams p) {
     using L          = KdSmem<D, NT, HP>;
     constexpr int NS = L::NS, ND = L::ND, CH = D / 64, MT = D / 16, E = D / 32, QR = NT * 8 / KD_WARPS;
@@ -644,7 +645,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                     for (int k = 0; k < 2; k++) {
                         const uint32_t hi = kd_pack(s[a][nt][2 * k], s[a][nt][2 * k + 1]);
                         ph[a][nt][k]      = kd_movmatrix(hi);
-                        if (HP) {
+                        if (PL) {
                             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
                             pl[a][nt][k]   = kd_movmatrix(kd_pack(s[a][nt][2 * k] - f.x, s[a][nt][2 * k + 1] - f.y));
                         }
@@ -691,7 +692,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
                                 kd_mma(o[j * 8 + 2 * k + q][nt], f, ph[a][nt][0], ph[a][nt][1]);
-                                if (HP) {
+                                if (PL) {
                                     kd_mma(o[j * 8 + 2 * k + q][nt], f, pl[a][nt][0], pl[a][nt][1]);
                                 }
                             }
@@ -894,25 +895,27 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
 
 namespace {
 
-template <int D, int NT, bool HP, bool CAP>
+template <int D, int NT, bool HP, bool PL, bool CAP>
 cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
     const size_t smem = KdSmem<D, NT, HP>::bytes(rows);
     static Kv8Once once;
-    const cudaError_t e = once.smem(kv8_decode_kernel<D, NT, HP, CAP>, KdSmem<D, NT, HP>::bytes(NT * 8));
-    return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, HP, CAP>, dim3(ctas), KD_THREADS, smem, stream, p);
+    const cudaError_t e = once.smem(kv8_decode_kernel<D, NT, HP, PL, CAP>, KdSmem<D, NT, HP>::bytes(NT * 8));
+    return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, HP, PL, CAP>, dim3(ctas), KD_THREADS, smem, stream, p);
 }
 
-template <int D, int NT>
+template <int D, int NT, bool CAP>
 cudaError_t launch_nt(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
-    if (p.o.type == KV_F32) {
-        return p.softcap > 0.0f ? launch_one<D, NT, true, true>(p, ctas, rows, stream) : launch_one<D, NT, true, false>(p, ctas, rows, stream);
-    }
-    return p.softcap > 0.0f ? launch_one<D, NT, false, true>(p, ctas, rows, stream) : launch_one<D, NT, false, false>(p, ctas, rows, stream);
+    return p.o.type == KV_F32   ? launch_one<D, NT, true, true, CAP>(p, ctas, rows, stream)
+           : p.o.type == KV_F16 ? launch_one<D, NT, false, true, CAP>(p, ctas, rows, stream)
+                                : launch_one<D, NT, false, false, CAP>(p, ctas, rows, stream);
 }
 
 template <int D>
 cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
-    return rows <= 8 ? launch_nt<D, 1>(p, ctas, rows, stream) : launch_nt<D, 2>(p, ctas, rows, stream);
+    if (p.softcap > 0.0f) {
+        return rows <= 8 ? launch_nt<D, 1, true>(p, ctas, rows, stream) : launch_nt<D, 2, true>(p, ctas, rows, stream);
+    }
+    return rows <= 8 ? launch_nt<D, 1, false>(p, ctas, rows, stream) : launch_nt<D, 2, false>(p, ctas, rows, stream);
 }
 
 // CTAs that an SM holds at once: what KdSmem plans for

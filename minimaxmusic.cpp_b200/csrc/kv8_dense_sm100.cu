@@ -1,26 +1,36 @@
 // kv8_dense_sm100.cu - attention over the 8-bit paged KV cache for many query rows (prefill, chunks of a
 // prompt) on the 5th-generation tensor cores (tcgen05 + TMEM), sm_100a.
 //
-// One CTA per (256 rows, kv head, sequence), the rows being (query, head of the group) pairs in that order,
-// so that all query heads of a kv head share each K/V tile; two 128-row tiles t of Q.  512 threads:
+// Rows of a unit (kv head, sequence) are (query, head of the group) pairs in that order, so that all query heads of
+// a kv head share each K/V tile.  Q is brought to [1, 2) at its row's largest element by a power of two and
+// rounded to F16; an F32 result takes its F16 remainder as a second operand (QP = 2), an F32 or F16 result that of
+// the weights P (PP = 2): the product then runs twice, the remainder first, where the accumulator is small.
+//
+// The tensor core truncates what it adds to an F32 accumulator: each of a tile's K = 16 steps loses up to 2^-23 of
+// it, always towards zero.  Over thousands of keys that is 1e-5 and more (measured 7e-7 a tile of 128 keys), so
+// two forms:
+//   TWO       256 rows per CTA, two 128-row tiles t, O_t accumulated in TMEM over all tiles: BF16 results,
+//             whose half step is 2e-3, over up to KE_LONG tokens.
+//   not TWO   128 rows per CTA; each tile's P V starts afresh in one of two TMEM buffers, and a warpgroup adds it
+//             to O in registers, rounded to nearest.
+// 512 threads:
 //   warpgroup 0   converts: codes of a 128-key tile go from global memory through registers (loaded one tile
 //                 ahead) into F16, which holds them exactly, in 128-byte-swizzled shared memory; the
 //                 scales of the tile's pages beside them.
-//   warpgroup 1   its first warp allocates TMEM and issues every tcgen05.mma:
-//                   S_t = Q_t K^T (columns [128t, 128t + 128)),  O_t += P_t V (columns [256 + D t, ...)),
-//                 P_t in TMEM over S_t, in the order QK0(j), PV1(j-1), QK1(j), PV0(j): one tile's softmax
-//                 runs beside the other's products.
-//   warpgroups 2, 3  softmax of tile 0, 1: one row per thread.
-// Q is brought to [1, 2) at its row's largest element by a power of two and rounded to F16; for an F32 result
-// (HP) the F16 remainder is a second operand, as is that of P: both products then run twice.
+//   warpgroup 1   its first warp allocates TMEM and issues every tcgen05.mma, P being in TMEM over S.
+//                 TWO: S_t in columns [128 t, ..), O_t in [256 + D t, ..), in the order QK0(j), PV1(j-1), QK1(j),
+//                 PV0(j): one tile's softmax runs beside the other's products.  Otherwise S and P V of tile j in
+//                 buffers j & 1, in the order QK(j+1), PV(j): the products of one tile beside the softmax of the next.
+//   warpgroup 2   softmax, one row per thread.   warpgroup 3   the same for tile 1 (TWO), or O's sums.
 //
 // Softmax.  s = S * (row factor * key scale of the column's page), in log2 units; weights 2^(s - m); the
 // value scale b = f 2^e of a page is multiplied into them, P = 2^(s - m) * 2^(m + e - R + KE_OFF) * f, so
 // that O is in units of 2^(R - KE_OFF).  m and R (the largest s + e of any page) are lazy: they follow only
-// when they would grow by more than 8 and 4, which F16's range allows, and O in TMEM is multiplied then.
+// when they would grow by more than 8 and 4, which F16's range allows, and O is multiplied then.
 //
-// Bound: the exponentials (16 a cycle and SM: 2048 cycles for a tile pair), the products (1024 cycles at
-// D = 128, twice that for HP) and the issue of the conversions (about 400 slots per scheduler) overlap.
+// Bound: for BF16 the exponentials (16 a cycle and SM: 2048 cycles for 256 rows of a tile; 3 of 8 pairs go by polynomial)
+// and the issue of softmax and conversions, beside 1024 cycles of products at D = 128; for F32 the products (2048
+// cycles for 128 rows of a tile), for F16 those (1536) and the exponentials alike.
 #include "kv8.cuh"
 #include "tc_sm100.cuh"
 
@@ -28,7 +38,6 @@ namespace mm3fa {
 
 constexpr int KE_THREADS = 512;
 constexpr int KE_M       = 128;  // rows per Q tile
-constexpr int KE_ROWS    = 256;
 constexpr int KE_N       = 128;  // keys per tile
 constexpr int KE_TMEM    = 512;
 constexpr int KE_OFF     = 8;    // P is held times 2^8: 2^14 at most with the lazy maxima
@@ -39,21 +48,22 @@ constexpr int KE_REGS_CONVERT = 96;
 constexpr int KE_REGS_ISSUE   = 32;
 static_assert(2 * KE_REGS_SOFTMAX + KE_REGS_CONVERT + KE_REGS_ISSUE <= 4 * KE_REGS_LAUNCH, "more registers than the launch has");
 
-template <int D, bool HP>
+constexpr int KE_LONG  = 65536;  // tokens
+
+template <int D, int QP, bool TWO>
 struct KeSmem {
     static constexpr int HALVES = D / 64;             // 128-byte column blocks
     static constexpr int QT     = HALVES * KE_M * 128;
     static constexpr int KT     = HALVES * KE_N * 128;
-    static constexpr int QP     = HP ? 2 : 1;         // F16 parts of Q
-    static constexpr int NK     = 2;
-    static constexpr int NV     = D == 128 && HP ? 1 : 2;
-    static constexpr int OFF_Q    = 0;                           // [tile][part]
-    static constexpr int OFF_K    = OFF_Q + 2 * QP * QT;         // [NK]
-    static constexpr int OFF_V    = OFF_K + NK * KT;             // [NV]
-    static constexpr int OFF_SC   = OFF_V + NV * KT;             // [4 tiles][8 groups] (a, f, e, present)
-    static constexpr int OFF_BAR  = OFF_SC + 4 * 8 * 16;
-    static constexpr int OFF_MISC = OFF_BAR + 24 * 8;
-    static constexpr int TOTAL    = OFF_MISC + 32 + 1024;        // + alignment
+    static constexpr int NK = 2, NV = 2;
+    static constexpr int OFF_Q    = 0;                                  // [tile][part]
+    static constexpr int OFF_K    = OFF_Q + (TWO ? 2 : 1) * QP * QT;    // [NK]
+    static constexpr int OFF_V    = OFF_K + NK * KT;                    // [NV]
+    static constexpr int OFF_SC   = OFF_V + NV * KT;                    // [4 tiles][8 groups] (a, f, e, present)
+    static constexpr int OFF_G    = OFF_SC + 4 * 8 * 16;                // [4 tiles][row] growth of R, then [2][row]
+    static constexpr int OFF_BAR  = OFF_G + (TWO ? 0 : 6 * KE_M * 4);
+    static constexpr int OFF_MISC = OFF_BAR + 32 * 8;
+    static constexpr int TOTAL    = OFF_MISC + 32 + 1024;               // + alignment
 };
 
 enum : int {
@@ -61,14 +71,24 @@ enum : int {
     KB_KEMPTY = 2,   // [2]
     KB_VFULL  = 4,   // [2]
     KB_VEMPTY = 6,   // [2]
-    KB_SFULL  = 8,   // [2] per Q tile
+    KB_SFULL  = 8,   // [2] per Q tile (TWO) or S buffer
     KB_PREADY = 10,  // [2] 128 softmax threads
-    KB_ODONE  = 12,  // [2]
+    KB_OFULL  = 12,  // [2] the last P V of a Q tile (TWO), or the P V of a tile in a buffer
     KB_QREADY = 14,  // [2] 128 softmax threads
     KB_SCALES = 16,  // [4] 8 converting threads: a ring deeper than K's, for a softmax that is behind the products
-    KB_DONE   = 20,
-    KB_COUNT  = 21,
+    KB_GROW   = 20,  // [4] 128 softmax threads (not TWO): the growth of a tile's R, read beside its P V
+    KB_OFREE  = 24,  // [2] 128 summing threads (not TWO)
+    KB_LAST   = 26,  // 128 softmax threads (not TWO): the rows' sums
+    KB_DONE   = 27,
+    KB_COUNT  = 28,
 };
+
+__host__ __device__ constexpr uint32_t ke_arrivals(int b) {
+    return b < KB_KEMPTY || (b >= KB_VFULL && b < KB_VEMPTY) || (b >= KB_PREADY && b < KB_OFULL) || (b >= KB_QREADY && b < KB_SCALES) ||
+                   (b >= KB_GROW && b < KB_DONE)
+               ? 128u
+               : (b >= KB_SCALES && b < KB_GROW ? 8u : 1u);
+}
 
 __device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
     uint64_t d;
@@ -104,23 +124,23 @@ __host__ __device__ constexpr uint32_t ke_idesc(int n, bool b_mn_major) {
     return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t) (n >> 3) << 17) | ((uint32_t) (KE_M >> 4) << 24);
 }
 
-template <int D, bool HP, bool CAP>
+template <int D, int QP, int PP, bool TWO, bool CAP>
 __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnParams p) {
-    using L          = KeSmem<D, HP>;
-    constexpr int NK = L::NK, NV = L::NV;
+    using L          = KeSmem<D, QP, TWO>;
+    constexpr int NK = L::NK, NV = L::NV, KE_ROWS = TWO ? 256 : 128;
+    constexpr int ESZ = QP == 2 ? 4 : 2;  // bytes of a result value: F32 where Q has two parts
     extern __shared__ __align__(16) char smem_raw[];
     char *     smem      = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t * bar       = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
     int *      abort_f   = reinterpret_cast<int *>(smem + L::OFF_MISC + 4);
     float4 *   scales    = reinterpret_cast<float4 *>(smem + L::OFF_SC);
+    float *    grows     = reinterpret_cast<float *>(smem + L::OFF_G);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
     if (tid == 0) {
         for (int i = 0; i < KB_COUNT; i++) {
-            const bool grp = i < KB_KEMPTY || (i >= KB_VFULL && i < KB_VEMPTY) || (i >= KB_PREADY && i < KB_ODONE) ||
-                             (i >= KB_QREADY && i < KB_SCALES);
-            mbar_init(&bar[i], grp ? 128u : (i >= KB_SCALES && i < KB_DONE ? 8u : 1u));
+            mbar_init(&bar[i], ke_arrivals(i));
         }
         *abort_f = 0;
         fence_mbar_init();
@@ -143,7 +163,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
     const int nq = p.q_len ? min(max(p.q_len[s], 0), p.n_q) : p.n_q;
     const int n  = min(max(p.kv_len[s], 0), p.t.max_pages * p.c.P);
     const int row0 = blk * KE_ROWS, rows = min(nq * p.ratio - row0, KE_ROWS);  // rows of this block
-    const bool two = rows > KE_M;
+    const bool two = TWO && rows > KE_M;
     // keys that its last row sees
     const int q_last = rows > 0 ? (row0 + rows - 1) / p.ratio : 0;
     const int keys   = rows > 0 ? (p.causal ? max(n - (nq - 1 - q_last), 0) : n) : 0;
@@ -244,34 +264,36 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
             // descriptors of the buffers' first bytes; an offset adds to the address field (16-byte units)
             const uint64_t q_d = sw128_desc(smem_addr(smem + L::OFF_Q), 16, 1024), k_d = sw128_desc(smem_addr(smem + L::OFF_K), 16, 1024);
             const uint64_t v_d = sw128_desc(smem_addr(smem + L::OFF_V), (uint32_t) (KE_N * 128), 1024);
-            auto           qk  = [&](int t, int j) {
-                uint64_t a = q_d + (uint64_t) ((t * L::QP * L::QT) >> 4);
+            // S of tile j of Q tile t (buffer j & 1 where there is one Q tile); the remainder of Q first
+            auto qk = [&](int t, int j) {
+                const int buf = TWO ? t : j & 1;
                 // rolled loops: unrolled ones keep every descriptor in registers that this warpgroup does not have
 #pragma unroll 1
-                for (int part = 0; part < L::QP; part++) {
-                    uint64_t b = k_d + (uint64_t) (((j % NK) * L::KT) >> 4);
+                for (int part = QP - 1; part >= 0; part--) {
+                    uint64_t a = q_d + (uint64_t) (((t * QP + part) * L::QT) >> 4), b = k_d + (uint64_t) (((j % NK) * L::KT) >> 4);
 #pragma unroll 1
                     for (int c = 0; c < L::HALVES; c++) {
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            umma_f16(tmem + (uint32_t) (t * KE_N), a + (uint64_t) (2 * k), b + (uint64_t) (2 * k), id_qk, part + c + k > 0 ? 1u : 0u);
+                            umma_f16(tmem + (uint32_t) (buf * KE_N), a + (uint64_t) (2 * k), b + (uint64_t) (2 * k), id_qk, QP - 1 - part + c + k > 0 ? 1u : 0u);
                         }
                         a += (KE_M * 128) >> 4, b += (KE_N * 128) >> 4;
                     }
                 }
-                umma_commit(&bar[KB_SFULL + t]);
+                umma_commit(&bar[KB_SFULL + buf]);
             };
             auto pv = [&](int t, int j) {
-                uint32_t a = tmem + (uint32_t) (t * KE_N);
+                const int buf = TWO ? t : j & 1;
 #pragma unroll 1
-                for (int part = 0; part < L::QP; part++) {
+                for (int part = PP - 1; part >= 0; part--) {
+                    uint32_t a = tmem + (uint32_t) (buf * KE_N + part * 64);
                     uint64_t b = v_d + (uint64_t) (((j % NV) * L::KT) >> 4);
 #pragma unroll 1
                     for (int c = 0; c < 2; c++) {
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            umma_f16_ts(tmem + 256u + (uint32_t) (t * D), a + (uint32_t) (8 * k), b + (uint64_t) ((k * 16 * 128) >> 4), id_pv,
-                                        j + part + c + k > 0 ? 1u : 0u);
+                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), a + (uint32_t) (8 * k), b + (uint64_t) ((k * 16 * 128) >> 4), id_pv,
+                                        (TWO ? j : 0) + PP - 1 - part + c + k > 0 ? 1u : 0u);
                         }
                         a += 32, b += (4 * 16 * 128) >> 4;
                     }
@@ -283,7 +305,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 return ok;
             };
             bool ok = true;
-            if (tiles > 0) {
+            if (TWO && tiles > 0) {
                 ok = wait(KB_QREADY, 0) && wait(KB_KFULL, 0);
                 if (ok) {
                     qk(0, 0);
@@ -309,7 +331,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                         }
                         qk(0, j + 1);
                     } else {
-                        umma_commit(&bar[KB_ODONE]);
+                        umma_commit(&bar[KB_OFULL]);
                     }
                     if (two) {
                         ok = wait(KB_PREADY + 1, j);
@@ -321,7 +343,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                         if (next) {
                             qk(1, j + 1);
                         } else {
-                            umma_commit(&bar[KB_ODONE + 1]);
+                            umma_commit(&bar[KB_OFULL + 1]);
                         }
                     } else {
                         umma_commit(&bar[KB_VEMPTY + j % NV]);
@@ -329,6 +351,30 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                     if (next) {
                         umma_commit(&bar[KB_KEMPTY + (j + 1) % NK]);
                     }
+                }
+            }
+            if (!TWO && tiles > 0) {
+                ok = wait(KB_QREADY, 0) && wait(KB_KFULL, 0);
+                if (ok) {
+                    qk(0, 0);
+                    umma_commit(&bar[KB_KEMPTY]);
+                }
+                for (int j = 0; ok && j < tiles; j++) {
+                    if (j + 1 < tiles) {  // over P(j - 1), whose product was issued before
+                        ok = wait(KB_KFULL + (j + 1) % NK, (j + 1) / NK);
+                        if (!ok) {
+                            break;
+                        }
+                        qk(0, j + 1);
+                        umma_commit(&bar[KB_KEMPTY + (j + 1) % NK]);
+                    }
+                    ok = wait(KB_VFULL + j % NV, j / NV) && wait(KB_PREADY + (j & 1), j >> 1) && (j < 2 || wait(KB_OFREE + (j & 1), (j >> 1) - 1));
+                    if (!ok) {
+                        break;
+                    }
+                    pv(0, j);
+                    umma_commit(&bar[KB_VEMPTY + j % NV]);
+                    umma_commit(&bar[KB_OFULL + (j & 1)]);
                 }
             }
             if (!ok) {
@@ -341,15 +387,119 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
     } else {
         // ======================================================= softmax
         regs_inc<KE_REGS_SOFTMAX>();
-        const int      t = wg - 2, quad = warp & 3, r = quad * 32 + lane;  // Q tile, TMEM lane quadrant, row of the tile
+        const int      t = TWO ? wg - 2 : 0, quad = warp & 3, r = quad * 32 + lane;  // Q tile, TMEM lane quadrant, row of the tile
         const uint32_t tl    = (uint32_t) (quad * 32) << 16;
-        const uint32_t s_col = tmem + tl + (uint32_t) (t * KE_N);
         const uint32_t o_col = tmem + tl + 256u + (uint32_t) (t * D);
         const int      tile_rows = min(rows - t * KE_M, KE_M);  // may be 0 or less
-        if (tile_rows > 0) {
+        char *         qs = smem + L::OFF_Q + t * QP * L::QT;
+        // a warp's 32 rows of the result, from the tile's Q, [32 rows][D] with the 16-byte chunks swizzled by the row
+        // against bank conflicts: store_rows writes them one after another, each as one run of bytes
+        char * mine = qs + quad * 32 * (D * ESZ);
+        auto   stage_cols = [&](int c, const uint32_t (&o)[32]) {  // columns 32 c .. of this thread's row
+            constexpr int PER = 16 / ESZ;
+#pragma unroll
+            for (int k = 0; k < 32 / PER; k++) {
+                uint4 w;
+                if (ESZ == 4) {
+                    w = make_uint4(o[4 * k & 31], o[(4 * k + 1) & 31], o[(4 * k + 2) & 31], o[(4 * k + 3) & 31]);
+                } else {
+                    uint32_t u[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = __uint_as_float(o[(8 * k + 2 * i) & 31]), y = __uint_as_float(o[(8 * k + 2 * i + 1) & 31]);
+                        if (p.o.type == KV_F16) {
+                            u[i] = ke_pack(x, y);
+                        } else {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+                            u[i] = *reinterpret_cast<const uint32_t *>(&b);
+                        }
+                    }
+                    w = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+                const int ck = c * (32 / PER) + k;
+                *reinterpret_cast<uint4 *>(mine + lane * (D * ESZ) + ((ck ^ (lane & 7)) << 4)) = w;
+            }
+        };
+        auto store_rows = [&] {
+            __syncwarp();
+            constexpr int CK = D * ESZ / 16;  // chunks of a row: 8, 16 or 32
+#pragma unroll 1
+            for (int it = 0; it < CK; it++) {
+                const int i = it * (32 / CK) + lane / CK, ck = lane % CK;  // row of the warp, chunk
+                const int rw = row0 + t * KE_M + quad * 32 + i;
+                if (quad * 32 + i >= tile_rows) {
+                    continue;
+                }
+                const int   qi = rw / p.ratio, hq = h * p.ratio + rw - qi * p.ratio;
+                char *      dst = p.o.data + (int64_t) hq * p.o.nb1 + (int64_t) qi * p.o.nb2 + (int64_t) s * p.o.nb3 + ck * 16;
+                const uint4 w   = *reinterpret_cast<const uint4 *>(mine + i * (D * ESZ) + ((ck ^ (i & 7)) << 4));
+                if (p.o.vec) {
+                    *reinterpret_cast<uint4 *>(dst) = w;
+                } else if (ESZ == 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        reinterpret_cast<uint32_t *>(dst)[e] = (&w.x)[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t) ((&w.x)[e >> 1] >> (16 * (e & 1)));
+                    }
+                }
+            }
+        };
+        if (!TWO && wg == 3) {
+            // =================================================== O in registers
+            float acc[D];
+#pragma unroll
+            for (int e = 0; e < D; e++) {
+                acc[e] = 0.0f;
+            }
+            bool ok = true;
+            for (int j = 0; j < tiles; j++) {
+                if (!dn_wait_warp(&bar[KB_GROW + (j & 3)], (uint32_t) ((j >> 2) & 1), deadline) ||
+                    !dn_wait_warp(&bar[KB_OFULL + (j & 1)], (uint32_t) ((j >> 1) & 1), deadline)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const float g = grows[(j & 3) * KE_M + r];
+#pragma unroll
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t o[32];
+                    tmem_ld32(o_col + (uint32_t) ((j & 1) * D + c * 32), o);
+                    tmem_ld_wait_tie(o);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        acc[c * 32 + e] = fmaf(acc[c * 32 + e], g, __uint_as_float(o[e]));
+                    }
+                }
+                tc_fence_before();
+                dn_mbar_arrive(&bar[KB_OFREE + (j & 1)]);
+            }
+            // Q's shared memory takes the result: KB_LAST follows the last tile, and every warp's part of Q
+            if (rows > 0) {
+                if (!dn_wait_warp(&bar[KB_LAST], 0, deadline) || !dn_wait_warp(&bar[KB_DONE], 0, deadline)) {
+                    ok = false;
+                }
+                if (!ok) {
+                    atomicExch(abort_f, 1);
+                }
+                const float inv = grows[4 * KE_M + r], up = grows[5 * KE_M + r];
+#pragma unroll
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        o[e] = __float_as_uint(ok ? acc[c * 32 + e] * inv * up : 0.0f);
+                    }
+                    stage_cols(c, o);
+                }
+                store_rows();
+            }
+        } else if (tile_rows > 0) {
             // ---- Q: the warp's 32 rows, whole rows at a time
             float factor = 0.0f;  // of this thread's row
-            char * qs    = smem + L::OFF_Q + t * L::QP * L::QT;
             constexpr int E = D / 32;
 #pragma unroll 4
             for (int it = 0; it < 32; it++) {
@@ -403,7 +553,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                     const float    a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
                     const uint32_t w = ke_pack(a, b);
                     *reinterpret_cast<uint32_t *>(to + 2 * e) = w;
-                    if (HP) {
+                    if (QP == 2) {
                         const float2 f = h2_to_f2(w);
                         *reinterpret_cast<uint32_t *>(to + L::QT + 2 * e) = ke_pack(a - f.x, b - f.y);
                     }
@@ -420,8 +570,10 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
             float      m = -INFINITY, l = 0.0f, R = -INFINITY;
             bool       ok = true;
             for (int j = 0; j < tiles; j++) {
+                const int      buf   = TWO ? t : j & 1, phase = TWO ? j : j >> 1;
+                const uint32_t s_col = tmem + tl + (uint32_t) (buf * KE_N);
                 if (!dn_wait_warp(&bar[KB_SCALES + (j & 3)], (uint32_t) ((j >> 2) & 1), deadline) ||
-                    !dn_wait_warp(&bar[KB_SFULL + t], (uint32_t) (j & 1), deadline)) {
+                    !dn_wait_warp(&bar[KB_SFULL + buf], (uint32_t) (phase & 1), deadline)) {
                     ok = false;
                     break;
                 }
@@ -507,7 +659,11 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 const float    ms = m == -INFINITY ? 0.0f : m, rs = R == -INFINITY ? 0.0f : R;
                 const uint64_t nm = f2pack(-ms, -ms);
                 uint64_t       acc[2] = { 0ull, 0ull };
-                uint32_t       pk[KE_N / 2], pl[HP ? KE_N / 2 : 1];
+                uint32_t       pk[KE_N / 2], pl[PP == 2 ? KE_N / 2 : 1];
+                if (!TWO) {
+                    grows[(j & 3) * KE_M + r] = grow;
+                    dn_mbar_arrive(&bar[KB_GROW + (j & 3)]);
+                }
 #pragma unroll
                 for (int g = 0; g < 8; g++) {
                     const float    f  = ex2(fminf(ms + sc[g].z - rs + KE_OFF, 90.0f)) * sc[g].y;
@@ -516,7 +672,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                     for (int i = 8 * g; i < 8 * g + 8; i++) {
                         const uint64_t x2 = fadd2(f2pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), nm);
                         uint64_t       w2;
-                        if (!HP && (i & 7) < KE_EMU) {
+                        if (PP == 1 && (i & 7) < KE_EMU) {
                             w2 = exp2_poly2(x2);
                         } else {
                             float x, y;
@@ -527,7 +683,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                         float x, y;
                         f2unpack(fmul2(w2, f2), x, y);
                         pk[i] = ke_pack(x, y);
-                        if (HP) {
+                        if (PP == 2) {
                             const float2 b = h2_to_f2(pk[i]);
                             pl[i]          = ke_pack(x - b.x, y - b.y);
                         }
@@ -538,12 +694,12 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 l += a0 + a1;
                 tmem_st32(s_col, &pk[0]);
                 tmem_st32(s_col + 32, &pk[32]);
-                if (HP) {
+                if (PP == 2) {
                     tmem_st32(s_col + 64, &pl[0]);
-                    tmem_st32(s_col + 96, &pl[HP ? 32 : 0]);
+                    tmem_st32(s_col + 96, &pl[PP == 2 ? 32 : 0]);
                 }
                 // PV(j - 1) is complete: QK(j) was issued after it
-                if (j > 0 && __any_sync(0xffffffffu, grow != 1.0f)) {
+                if (TWO && j > 0 && __any_sync(0xffffffffu, grow != 1.0f)) {
 #pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
                         uint32_t o[32];
@@ -558,11 +714,22 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                dn_mbar_arrive(&bar[KB_PREADY + t]);
+                dn_mbar_arrive(&bar[KB_PREADY + buf]);
             }
+            // O (units of 2^(R - KE_OFF)) over the sum (2^m); rows without keys, and without a value scale, are 0
+            const float inv = l != 0.0f ? (1.0f / (1 << KE_OFF)) / l : 0.0f, up = R == -INFINITY ? 0.0f : ex2(R - m);
+            if (!TWO) {
+                // every warp has staged its rows of Q when warpgroup 3 writes over them
+                if (!dn_wait_warp(&bar[KB_QREADY], 0, deadline) || !ok) {
+                    atomicExch(abort_f, 1);
+                }
+                grows[4 * KE_M + r] = inv, grows[5 * KE_M + r] = up;
+                dn_mbar_arrive(&bar[KB_LAST]);
+            }
+            if (TWO) {
             bool have = ok && tiles > 0;
             if (have) {
-                have = dn_wait_warp(&bar[KB_ODONE + t], 0, deadline);
+                have = dn_wait_warp(&bar[KB_OFULL + t], 0, deadline);
                 tc_fence_after();
             }
             // Q's shared memory takes the result: every product has to be done, and every warp with its rows of Q
@@ -571,11 +738,6 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 atomicExch(abort_f, 1);
                 have = false;
             }
-            // ---- O (units of 2^(R - KE_OFF)) over the sum (2^m); the warp stores its rows one after another, each as
-            // one run of bytes.  Rows without keys, and without a value scale, are 0
-            const float inv = l != 0.0f ? (1.0f / (1 << KE_OFF)) / l : 0.0f, up = R == -INFINITY ? 0.0f : ex2(R - m);
-            char *      mine = qs + quad * 32 * (D * (HP ? 4 : 2));  // [32 rows][D] of the result's type
-            const int   esz  = HP ? 4 : 2;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[32];
@@ -592,56 +754,9 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 for (int e = 0; e < 32; e++) {
                     o[e] = __float_as_uint(have ? __uint_as_float(o[e]) * inv * up : 0.0f);
                 }
-                // 16-byte chunks, swizzled by the row against bank conflicts
-                constexpr int PER = HP ? 4 : 8;
-#pragma unroll
-                for (int k = 0; k < 32 / PER; k++) {
-                    uint4 w;
-                    if (HP) {
-                        w = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-                    } else {
-                        uint32_t u[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float x = __uint_as_float(o[(8 * k + 2 * i) & 31]), y = __uint_as_float(o[(8 * k + 2 * i + 1) & 31]);
-                            if (p.o.type == KV_F16) {
-                                u[i] = ke_pack(x, y);
-                            } else {
-                                const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-                                u[i] = *reinterpret_cast<const uint32_t *>(&b);
-                            }
-                        }
-                        w = make_uint4(u[0], u[1], u[2], u[3]);
-                    }
-                    const int ck = c * (32 / PER) + k;
-                    *reinterpret_cast<uint4 *>(mine + lane * (D * esz) + ((ck ^ (lane & 7)) << 4)) = w;
-                }
+                stage_cols(c, o);
             }
-            __syncwarp();
-            constexpr int CK = D * (HP ? 4 : 2) / 16;  // chunks of a row: 8, 16 or 32
-#pragma unroll 1
-            for (int it = 0; it < CK; it++) {
-                const int i = it * (32 / CK) + lane / CK, ck = lane % CK;  // row of the warp, chunk
-                const int rw = row0 + t * KE_M + quad * 32 + i;
-                if (quad * 32 + i >= tile_rows) {
-                    continue;
-                }
-                const int   qi = rw / p.ratio, hq = h * p.ratio + rw - qi * p.ratio;
-                char *      dst = p.o.data + (int64_t) hq * p.o.nb1 + (int64_t) qi * p.o.nb2 + (int64_t) s * p.o.nb3 + ck * 16;
-                const uint4 w   = *reinterpret_cast<const uint4 *>(mine + i * (D * esz) + ((ck ^ (i & 7)) << 4));
-                if (p.o.vec) {
-                    *reinterpret_cast<uint4 *>(dst) = w;
-                } else if (HP) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        reinterpret_cast<uint32_t *>(dst)[e] = (&w.x)[e];
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t) ((&w.x)[e >> 1] >> (16 * (e & 1)));
-                    }
-                }
+            store_rows();
             }
         }
     }
@@ -660,10 +775,10 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
 
 namespace {
 
-template <int D, bool HP, bool CAP>
-cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, cudaStream_t stream) {
-    auto            kern = kv8_dense_kernel<D, HP, CAP>;
-    static Kv8Once  once;
+template <int D, int QP, int PP, bool TWO, bool CAP>
+cudaError_t launch_one(const Kv8AttnParams & p, cudaStream_t stream) {
+    auto             kern = kv8_dense_kernel<D, QP, PP, TWO, CAP>;
+    static Kv8Once   once;
     static const int regs = [&] {
         cudaFuncAttributes a{};
         return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
@@ -672,23 +787,30 @@ cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, cudaStream_t stre
     if (regs != KE_REGS_LAUNCH) {
         return cudaErrorInvalidConfiguration;
     }
-    const cudaError_t e = once.smem(kern, KeSmem<D, HP>::TOTAL);
-    return e != cudaSuccess ? e : kv8_launch(kern, dim3(ctas), KE_THREADS, KeSmem<D, HP>::TOTAL, stream, p);
+    constexpr int   smem = KeSmem<D, QP, TWO>::TOTAL, step = TWO ? 256 : 128;
+    const int64_t   rows = (int64_t) p.ratio * p.n_q, ctas = (rows + step - 1) / step * p.c.n_head_kv * p.t.n_seq;
+    const cudaError_t e  = once.smem(kern, smem);
+    return e != cudaSuccess ? e : kv8_launch(kern, dim3((unsigned) ctas), KE_THREADS, smem, stream, p);
 }
 
-template <int D>
-cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, cudaStream_t stream) {
+template <int D, bool CAP>
+cudaError_t launch_d(const Kv8AttnParams & p, cudaStream_t stream) {
     if (p.o.type == KV_F32) {
-        return p.softcap > 0.0f ? launch_one<D, true, true>(p, ctas, stream) : launch_one<D, true, false>(p, ctas, stream);
+        return launch_one<D, 2, 2, false, CAP>(p, stream);
     }
-    return p.softcap > 0.0f ? launch_one<D, false, true>(p, ctas, stream) : launch_one<D, false, false>(p, ctas, stream);
+    if (p.o.type == KV_F16) {
+        return launch_one<D, 1, 2, false, CAP>(p, stream);
+    }
+    return (int64_t) p.t.max_pages * p.c.P > KE_LONG ? launch_one<D, 1, 1, false, CAP>(p, stream) : launch_one<D, 1, 1, true, CAP>(p, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_kv8_dense(const Kv8AttnParams & p, cudaStream_t stream) {
-    const int64_t rows = (int64_t) p.ratio * p.n_q, ctas = (rows + KE_ROWS - 1) / KE_ROWS * p.c.n_head_kv * p.t.n_seq;
-    return p.c.D == 64 ? launch_d<64>(p, (unsigned) ctas, stream) : launch_d<128>(p, (unsigned) ctas, stream);
+    if (p.c.D == 64) {
+        return p.softcap > 0.0f ? launch_d<64, true>(p, stream) : launch_d<64, false>(p, stream);
+    }
+    return p.softcap > 0.0f ? launch_d<128, true>(p, stream) : launch_d<128, false>(p, stream);
 }
 
 }  // namespace mm3fa
