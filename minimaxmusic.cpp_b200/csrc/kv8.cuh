@@ -111,6 +111,12 @@ __device__ __forceinline__ void kv8_dep_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// r / d for r < 2^24 and inv = floor(2^32 / d) + 1: the error r (inv d - 2^32) / 2^32 d stays below 1 / d
+// while r d < 2^32
+__device__ __forceinline__ uint32_t kv8_div(uint32_t r, uint32_t inv) {
+    return inv ? __umulhi(r, inv) : r;
+}
+
 // The page of a sequence's page slot j, or -1.
 __device__ __forceinline__ int kv8_page(const Kv8Table & t, int n_pages, int s, int j) {
     if (j < 0 || j >= t.max_pages) {

@@ -123,12 +123,6 @@ __device__ __forceinline__ int kd_swz(int r) {
     return D == 64 ? (r >> 1) & 3 : r & 7;
 }
 
-// r / d for r < 2^24 and inv = floor(2^32 / d) + 1: the error r (inv d - 2^32) / 2^32 d stays below 1 / d
-// while r d < 2^32
-__device__ __forceinline__ uint32_t kd_div(uint32_t r, uint32_t inv) {
-    return inv ? __umulhi(r, inv) : r;
-}
-
 struct KdSeq {
     int n;   // keys
     int m;   // query rows (positions)
@@ -287,7 +281,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
         const int h = seg.u / groups, r0 = (seg.u - h * groups) * KD_ROWS;
 #pragma unroll
         for (int i = 0; i < QR; i++) {
-            const int    r = r0 + warp + KD_WARPS * i, qi = (int) kd_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
+            const int    r = r0 + warp + KD_WARPS * i, qi = (int) kv8_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
             const char * src = p.q.data + (int64_t) qi * p.q.nb1 + (int64_t) hq * p.q.nb2 + (int64_t) seg.s * p.q.nb3;
             const bool   live = r < all_rows && qi < seg.q.m;
 #pragma unroll
@@ -373,7 +367,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
     // dims lane * E .. + E of a result row: O (in units of 2^(R - KD_OFF)) over the sum (of 2^m); rows without
     // keys, and without a value scale, are 0
     auto emit = [&](int s, int h, int r, int nq, float (&v)[E], float mt, float lt, float rt) {
-        const int qi = (int) kd_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
+        const int qi = (int) kv8_div((uint32_t) r, p.ratio_inv), hq = h * p.ratio + r - qi * p.ratio;
         if (qi >= nq) {
             return;
         }
@@ -490,7 +484,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int rr = nt * 8 + 2 * t + i, qi = (int) kd_div((uint32_t) (r0 + rr), p.ratio_inv);
+                const int rr = nt * 8 + 2 * t + i, qi = (int) kv8_div((uint32_t) (r0 + rr), p.ratio_inv);
                 qs[nt][i]  = qscale[rr];
                 lim[nt][i] = p.causal ? sq.n - (sq.m - 1 - qi) : sq.n;
                 m[nt][i] = -INFINITY, l[nt][i] = 0.0f, R[nt][i] = -INFINITY;
@@ -935,6 +929,7 @@ size_t kv8_attn_workspace_bytes(int D, int n_q, int ratio, int n_head_kv, int n_
 
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p0, int sms, cudaStream_t stream) {
     Kv8AttnParams p    = p0;
+    p.ratio_inv        = p.ratio == 1 ? 0u : (uint32_t) ((1ull << 32) / (uint64_t) p.ratio + 1);
     if (p.c.D <= 128 && p.ratio * p.n_q >= KD_DENSE) {
         return launch_kv8_dense(p, stream);
     }
@@ -948,7 +943,6 @@ cudaError_t launch_kv8_attn(const Kv8AttnParams & p0, int sms, cudaStream_t stre
         return cudaErrorInvalidValue;  // refused by the caller's checks
     }
     const unsigned ctas  = (unsigned) (blocks < most ? blocks : most);
-    p.ratio_inv          = p.ratio == 1 ? 0u : (uint32_t) ((1ull << 32) / (uint64_t) p.ratio + 1);
     switch (p.c.D) {
         case 64:
             return launch_d<64>(p, ctas, rows, stream);

@@ -41,7 +41,7 @@ constexpr int KE_M       = 128;  // rows per Q tile
 constexpr int KE_N       = 128;  // keys per tile
 constexpr int KE_TMEM    = 512;
 constexpr int KE_OFF     = 8;    // P is held times 2^8: 2^14 at most with the lazy maxima
-constexpr int KE_EMU     = 3;    // of every 8 pairs of weights, those by polynomial where P is rounded to F16 anyway
+constexpr int KE_EMU     = 1;    // of every 8 pairs of weights, those by polynomial where P is rounded to F16 anyway
 constexpr int KE_REGS_LAUNCH  = 128;  // 65536 / 512
 constexpr int KE_REGS_SOFTMAX = 192;  // 2 x 192 + 96 + 32 = 4 x 128
 constexpr int KE_REGS_CONVERT = 96;
@@ -61,7 +61,8 @@ struct KeSmem {
     static constexpr int OFF_V    = OFF_K + NK * KT;                    // [NV]
     static constexpr int OFF_SC   = OFF_V + NV * KT;                    // [4 tiles][8 groups] (a, f, e, present)
     static constexpr int OFF_G    = OFF_SC + 4 * 8 * 16;                // [4 tiles][row] growth of R, then [2][row]
-    static constexpr int OFF_BAR  = OFF_G + (TWO ? 0 : 6 * KE_M * 4);
+    static constexpr int OFF_F    = OFF_G + (TWO ? 0 : 6 * KE_M * 4);   // [tile][row] factors of the rows
+    static constexpr int OFF_BAR  = OFF_F + (TWO ? 2 : 1) * KE_M * 4;
     static constexpr int OFF_MISC = OFF_BAR + 32 * 8;
     static constexpr int TOTAL    = OFF_MISC + 32 + 1024;               // + alignment
 };
@@ -74,7 +75,7 @@ enum : int {
     KB_SFULL  = 8,   // [2] per Q tile (TWO) or S buffer
     KB_PREADY = 10,  // [2] 128 softmax threads
     KB_OFULL  = 12,  // [2] the last P V of a Q tile (TWO), or the P V of a tile in a buffer
-    KB_QREADY = 14,  // [2] 128 softmax threads
+    KB_QREADY = 14,  // [2] the threads that stage a Q tile: 128 (TWO), or the 256 of warpgroups 2 and 3
     KB_SCALES = 16,  // [4] 8 converting threads: a ring deeper than K's, for a softmax that is behind the products
     KB_GROW   = 20,  // [4] 128 softmax threads (not TWO): the growth of a tile's R, read beside its P V
     KB_OFREE  = 24,  // [2] 128 summing threads (not TWO)
@@ -83,8 +84,9 @@ enum : int {
     KB_COUNT  = 28,
 };
 
-__host__ __device__ constexpr uint32_t ke_arrivals(int b) {
-    return b < KB_KEMPTY || (b >= KB_VFULL && b < KB_VEMPTY) || (b >= KB_PREADY && b < KB_OFULL) || (b >= KB_QREADY && b < KB_SCALES) ||
+__host__ __device__ constexpr uint32_t ke_arrivals(int b, bool two) {
+    return b == KB_QREADY && !two ? 256u :
+           b < KB_KEMPTY || (b >= KB_VFULL && b < KB_VEMPTY) || (b >= KB_PREADY && b < KB_OFULL) || (b >= KB_QREADY && b < KB_SCALES) ||
                    (b >= KB_GROW && b < KB_DONE)
                ? 128u
                : (b >= KB_SCALES && b < KB_GROW ? 8u : 1u);
@@ -136,11 +138,12 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
     int *      abort_f   = reinterpret_cast<int *>(smem + L::OFF_MISC + 4);
     float4 *   scales    = reinterpret_cast<float4 *>(smem + L::OFF_SC);
     float *    grows     = reinterpret_cast<float *>(smem + L::OFF_G);
+    float *    factors   = reinterpret_cast<float *>(smem + L::OFF_F);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
     if (tid == 0) {
         for (int i = 0; i < KB_COUNT; i++) {
-            mbar_init(&bar[i], ke_arrivals(i));
+            mbar_init(&bar[i], ke_arrivals(i, TWO));
         }
         *abort_f = 0;
         fence_mbar_init();
@@ -183,28 +186,31 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
             pg1 = p.c.log2p == 4 ? (k0 + 16 < keys ? row[i + 1] : -1) : pg0;
         };
         uint4 kx[LD], vx[LD];
-        auto  load = [&](int j, const int8_t * pool, uint4 (&x)[LD]) {
+        // this lane's place in a 32-row run of codes, and in the F16 tile: piece pc holds the 16-byte chunks 2 pc, 2 pc + 1
+        const int      src_off = (lane & 7) * D + (lane >> 3) * 16;
+        const uint32_t dst_off = (uint32_t) ((32 * warp + (lane & 7)) * 128 + (((2 * (lane >> 3)) ^ (lane & 7)) << 4));
+        auto           load    = [&](int j, const int8_t * pool, uint4 (&x)[LD]) {
+            const bool     ok0 = (unsigned) pg0 < (unsigned) p.c.n_pages, ok1 = (unsigned) pg1 < (unsigned) p.c.n_pages;
+            const int      in  = (j * KE_N + 32 * warp) & (p.c.P - 1);  // first row of the run in its page
+            const int8_t * a   = pool + (((int64_t) (ok0 ? pg0 : 0) * p.c.n_head_kv + h) * p.c.P + in) * D + src_off;
+            const int8_t * b   = p.c.log2p > 4 ? a : pool + (((int64_t) (ok1 ? pg1 : 0) * p.c.n_head_kv + h) * p.c.P - 16) * D + src_off;
 #pragma unroll
             for (int i = 0; i < LD; i++) {
-                const int  rr = 8 * (i & 3) + (lane & 7), pc = (lane >> 3) + 4 * (i >> 2);
-                const int  pg = (i & 3) < 2 ? pg0 : pg1;
-                const bool ok = (unsigned) pg < (unsigned) p.c.n_pages;
-                const int64_t at = (((int64_t) (ok ? pg : 0) * p.c.n_head_kv + h) * p.c.P + ((j * KE_N + 32 * warp + rr) & (p.c.P - 1))) * D + pc * 16;
+                const int8_t * at = ((i & 3) < 2 ? a : b) + 8 * (i & 3) * D + 64 * (i >> 2);
                 x[i] = make_uint4(0, 0, 0, 0);
-                if (ok) {
-                    x[i] = __ldg(reinterpret_cast<const uint4 *>(pool + at));
+                if ((i & 3) < 2 ? ok0 : ok1) {
+                    x[i] = __ldg(reinterpret_cast<const uint4 *>(at));
                 }
             }
         };
         auto store = [&](char * tile, const uint4 (&x)[LD]) {
+            char * to = tile + dst_off, *to1 = tile + (dst_off ^ 16u);
 #pragma unroll
             for (int i = 0; i < LD; i++) {
-                const int rr = 32 * warp + 8 * (i & 3) + (lane & 7), pc = (lane >> 3) + 4 * (i >> 2);
-                uint4     a, b;
+                uint4 a, b;
                 ke_convert(x[i], a, b);
-                char * to = tile + (pc >> 2) * (KE_N * 128);
-                *reinterpret_cast<uint4 *>(to + sw128_off(rr, 2 * (pc & 3)))     = a;
-                *reinterpret_cast<uint4 *>(to + sw128_off(rr, 2 * (pc & 3) + 1)) = b;
+                *reinterpret_cast<uint4 *>(to + 8 * (i & 3) * 128 + (i >> 2) * (KE_N * 128))  = a;
+                *reinterpret_cast<uint4 *>(to1 + 8 * (i & 3) * 128 + (i >> 2) * (KE_N * 128)) = b;
             }
         };
         bool ok = true;
@@ -423,16 +429,17 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
         auto store_rows = [&] {
             __syncwarp();
             constexpr int CK = D * ESZ / 16;  // chunks of a row: 8, 16 or 32
-#pragma unroll 1
+            // lane i: the address of row i
+            const int      rl = row0 + t * KE_M + quad * 32 + lane, ql = (int) kv8_div((uint32_t) rl, p.ratio_inv), hl = h * p.ratio + rl - ql * p.ratio;
+            const uint64_t al = reinterpret_cast<uint64_t>(p.o.data + (int64_t) hl * p.o.nb1 + (int64_t) ql * p.o.nb2 + (int64_t) s * p.o.nb3);
+#pragma unroll 4
             for (int it = 0; it < CK; it++) {
-                const int i = it * (32 / CK) + lane / CK, ck = lane % CK;  // row of the warp, chunk
-                const int rw = row0 + t * KE_M + quad * 32 + i;
+                const int   i = it * (32 / CK) + lane / CK, ck = lane % CK;  // row of the warp, chunk
+                char *      dst = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, al, i)) + ck * 16;
+                const uint4 w   = *reinterpret_cast<const uint4 *>(mine + i * (D * ESZ) + ((ck ^ (i & 7)) << 4));
                 if (quad * 32 + i >= tile_rows) {
                     continue;
                 }
-                const int   qi = rw / p.ratio, hq = h * p.ratio + rw - qi * p.ratio;
-                char *      dst = p.o.data + (int64_t) hq * p.o.nb1 + (int64_t) qi * p.o.nb2 + (int64_t) s * p.o.nb3 + ck * 16;
-                const uint4 w   = *reinterpret_cast<const uint4 *>(mine + i * (D * ESZ) + ((ck ^ (i & 7)) << 4));
                 if (p.o.vec) {
                     *reinterpret_cast<uint4 *>(dst) = w;
                 } else if (ESZ == 4) {
@@ -448,8 +455,110 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 }
             }
         };
+        // ---- Q: rows [ra, ra + 16) of the tile by one warp, whole rows at a time, all loads in flight
+        auto stage_q = [&](int ra) {
+            constexpr int E = D / 32, B = 8;
+            // lane i: the address of row i
+            const int      rl = row0 + t * KE_M + ra + (lane & 15), ql = (int) kv8_div((uint32_t) rl, p.ratio_inv), hl = h * p.ratio + rl - ql * p.ratio;
+            const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) ql * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) s * p.q.nb3);
+            const int      e0 = lane * E, sub = (e0 % 8) * 2;
+            char *         to = qs + (e0 / 64) * (KE_M * 128) + sub;
+            const bool     f32 = p.q.type == KV_F32, f16 = p.q.type == KV_F16;
+#pragma unroll 1
+            for (int i0 = 0; i0 < 16; i0 += B) {
+                const int in = tile_rows - ra - i0;  // rows there are
+                uint32_t  u[B][E];  // F32 values, or 16-bit pairs in the first half
+                if (p.q.vec) {
+#pragma unroll
+                    for (int i = 0; i < B; i++) {
+                        const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i0 + i));
+                        if (E == 4) {
+                            uint4 w = make_uint4(0, 0, 0, 0);
+                            if (i < in && f32) {
+                                w = *reinterpret_cast<const uint4 *>(src + lane * 16);
+                            } else if (i < in) {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(src + lane * 8);
+                                w.x = v.x, w.y = v.y;
+                            }
+                            u[i][0] = w.x, u[i][1] = w.y, u[i][E - 2] = w.z, u[i][E - 1] = w.w;
+                        } else {
+                            uint2 w = make_uint2(0, 0);
+                            if (i < in && f32) {
+                                w = *reinterpret_cast<const uint2 *>(src + lane * 8);
+                            } else if (i < in) {
+                                w.x = *reinterpret_cast<const uint32_t *>(src + lane * 4);
+                            }
+                            u[i][0] = w.x, u[i][1] = w.y;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < B; i++) {
+                        const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i0 + i));
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            u[i][e] = i < in && f32 ? reinterpret_cast<const uint32_t *>(src)[e0 + e] : 0u;
+                        }
+                        if (i < in && !f32) {
+#pragma unroll
+                            for (int e = 0; e < E; e += 2) {
+                                u[i][e / 2] = reinterpret_cast<const uint16_t *>(src)[e0 + e] | (uint32_t) reinterpret_cast<const uint16_t *>(src)[e0 + e + 1] << 16;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    float x[E];
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const float2 a = h2_to_f2(u[i][e / 2]), b = bf2_to_f2(u[i][e / 2]);
+                        x[e]     = f32 ? __uint_as_float(u[i][e]) : f16 ? a.x : b.x;
+                        x[e + 1] = f32 ? __uint_as_float(u[i][e + 1]) : f16 ? a.y : b.y;
+                    }
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    // the exponent of the largest element; a row with an infinity or NaN gives NaN
+                    const bool  odd = top >= 0x7f800000u;
+                    const int   ex  = top == 0 || odd ? 0 : min(max((int) (top >> 23) - 127, -126), 126);
+                    const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23);
+                    if (lane == i) {
+                        factors[t * KE_M + ra + i0 + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * (CAP ? p.scale / p.softcap : p.scale * LOG2E);
+                    }
+                    uint32_t w[E / 2], v[E / 2];
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const float a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
+                        w[e / 2] = ke_pack(a, b);
+                        const float2 f = h2_to_f2(w[e / 2]);
+                        v[e / 2]       = ke_pack(a - f.x, b - f.y);
+                    }
+                    char * at = to + (ra + i0 + i) * 128 + ((((e0 % 64) / 8) ^ i) << 4);  // ra + i0: a multiple of 8
+                    if (E == 4) {
+                        *reinterpret_cast<uint2 *>(at) = make_uint2(w[0], w[E / 2 - 1]);
+                        if (QP == 2) {
+                            *reinterpret_cast<uint2 *>(at + L::QT) = make_uint2(v[0], v[E / 2 - 1]);
+                        }
+                    } else {
+                        *reinterpret_cast<uint32_t *>(at) = w[0];
+                        if (QP == 2) {
+                            *reinterpret_cast<uint32_t *>(at + L::QT) = v[0];
+                        }
+                    }
+                }
+            }
+        };
         if (!TWO && wg == 3) {
             // =================================================== O in registers
+            if (rows > 0) {
+                stage_q(quad * 32 + 16);
+                fence_proxy_async_smem();
+                dn_mbar_arrive(&bar[KB_QREADY]);
+            }
             float acc[D];
 #pragma unroll
             for (int e = 0; e < D; e++) {
@@ -477,7 +586,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 tc_fence_before();
                 dn_mbar_arrive(&bar[KB_OFREE + (j & 1)]);
             }
-            // Q's shared memory takes the result: KB_LAST follows the last tile, and every warp's part of Q
+            // Q's shared memory takes the result: KB_LAST follows QREADY, KB_DONE the last product
             if (rows > 0) {
                 if (!dn_wait_warp(&bar[KB_LAST], 0, deadline) || !dn_wait_warp(&bar[KB_DONE], 0, deadline)) {
                     ok = false;
@@ -498,75 +607,23 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 store_rows();
             }
         } else if (tile_rows > 0) {
-            // ---- Q: the warp's 32 rows, whole rows at a time
-            float factor = 0.0f;  // of this thread's row
-            constexpr int E = D / 32;
-#pragma unroll 4
-            for (int it = 0; it < 32; it++) {
-                const int rr = quad * 32 + it, rw = row0 + t * KE_M + rr;
-                const int qi = rw / p.ratio, hq = h * p.ratio + rw - qi * p.ratio;
-                float     x[E];
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    x[e] = 0.0f;
-                }
-                if (rr < tile_rows) {
-                    const char * src = p.q.data + (int64_t) qi * p.q.nb1 + (int64_t) hq * p.q.nb2 + (int64_t) s * p.q.nb3;
-                    if (p.q.type == KV_F32) {
-                        if (p.q.vec) {
-#pragma unroll
-                            for (int e = 0; e < E; e += 2) {
-                                const float2 f = reinterpret_cast<const float2 *>(src)[(lane * E + e) / 2];
-                                x[e] = f.x, x[e + 1] = f.y;
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < E; e++) {
-                                x[e] = reinterpret_cast<const float *>(src)[lane * E + e];
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            const uint16_t u = reinterpret_cast<const uint16_t *>(src)[lane * E + e];
-                            x[e] = p.q.type == KV_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t) u << 16);
-                        }
-                    }
-                }
-                uint32_t top = 0;
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                // the exponent of the largest element; a row with an infinity or NaN gives NaN
-                const bool  odd = top >= 0x7f800000u;
-                const int   ex  = top == 0 || odd ? 0 : min(max((int) (top >> 23) - 127, -126), 126);
-                const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23);
-                if (it == lane) {
-                    factor = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * (CAP ? p.scale / p.softcap : p.scale * LOG2E);
-                }
-                const int e0 = lane * E, hb = e0 / 64, ch = (e0 % 64) / 8, sub = (e0 % 8) * 2;
-                char *    to = qs + hb * (KE_M * 128) + sw128_off(rr, ch) + sub;
-#pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    const float    a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
-                    const uint32_t w = ke_pack(a, b);
-                    *reinterpret_cast<uint32_t *>(to + 2 * e) = w;
-                    if (QP == 2) {
-                        const float2 f = h2_to_f2(w);
-                        *reinterpret_cast<uint32_t *>(to + L::QT + 2 * e) = ke_pack(a - f.x, b - f.y);
-                    }
-                }
+            if (TWO) {
+                stage_q(quad * 32);
+                stage_q(quad * 32 + 16);
+            } else {
+                stage_q(quad * 32);  // the other half by warpgroup 3
             }
             fence_proxy_async_smem();
             dn_mbar_arrive(&bar[KB_QREADY + t]);
-
+            if (!dn_wait_warp(&bar[KB_QREADY + t], 0, deadline)) {
+                atomicExch(abort_f, 1);
+            }
+            const float factor = factors[t * KE_M + r];
             const int  rw    = row0 + t * KE_M + r;
             const bool live  = r < tile_rows;
-            const int  my_q  = rw / p.ratio;
-            const int  lim   = !live ? 0 : p.causal ? n - (nq - 1 - my_q) : n;  // keys of this row
-            const int  warp_lim = (int) __reduce_min_sync(0xffffffffu, (unsigned) (live ? max(lim, 0) : 0x7fffffff));
+            const int  my_q  = (int) kv8_div((uint32_t) rw, p.ratio_inv);
+            const int  lim   = !live ? 0x7fffffff : p.causal ? n - (nq - 1 - my_q) : n;  // keys of this row
+            const int  warp_lim = (int) __reduce_min_sync(0xffffffffu, (unsigned) max(lim, 0));
             float      m = -INFINITY, l = 0.0f, R = -INFINITY;
             bool       ok = true;
             for (int j = 0; j < tiles; j++) {
@@ -596,102 +653,117 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                     }
                     tmem_st_wait();
                 }
-                uint32_t sr[KE_N];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tmem_ld32(s_col + (uint32_t) (c * 32), &sr[c * 32]);
-                }
                 bool whole = j * KE_N + KE_N <= warp_lim;  // every row of the warp sees every column
+                bool plain = !CAP;                         // s = S * factor * a, with all of these positive
 #pragma unroll
                 for (int g = 0; g < 8; g++) {
                     whole &= sc[g].w != 0.0f;
+                    plain &= !(factor * sc[g].x <= 0.0f);  // NaN: a row of NaN, whose neighbours go on as without it
                 }
+                plain = __all_sync(0xffffffffu, plain);
+                // The weights are taken with the maxima as they are (only a row's first tile has none), and the maxima found
+                // and the weights taken again where a group's sum shows that one could leave F16's range
+                // - by the rows that need it: no row's result depends on its neighbours'
+                bool     need = m == -INFINITY || R == -INFINITY, full = __any_sync(0xffffffffu, need);
+                float    grow = 1.0f, lsum;
+                uint32_t pk[KE_N / 2], pl[PP == 2 ? KE_N / 2 : 1];
+#pragma unroll 1
+                for (;;) {
+                    uint32_t sr[KE_N];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tmem_ld_wait_tie(&sr[c * 32]);
-                }
-                if (!CAP) {
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld32(s_col + (uint32_t) (c * 32), &sr[c * 32]);
+                    }
 #pragma unroll
-                    for (int g = 0; g < 8; g++) {
-                        const float    a  = factor * sc[g].x;
-                        const uint64_t a2 = f2pack(a, a);
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld_wait_tie(&sr[c * 32]);
+                    }
+                    if (!CAP && !plain) {
 #pragma unroll
-                        for (int e = 16 * g; e < 16 * g + 16; e += 2) {
-                            float x, y;
-                            f2unpack(fmul2(f2pack(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), a2), x, y);
-                            sr[e] = __float_as_uint(x), sr[e + 1] = __float_as_uint(y);
+                        for (int e = 0; e < KE_N; e++) {
+                            sr[e] = __float_as_uint(__uint_as_float(sr[e]) * (factor * sc[e >> 4].x));
                         }
                     }
-                }
-                if (!whole) {
+                    if (!whole) {
 #pragma unroll
-                    for (int g = 0; g < 8; g++) {
-                        const int lg = sc[g].w != 0.0f ? left : 0;
+                        for (int g = 0; g < 8; g++) {
+                            const int lg = sc[g].w != 0.0f ? left : 0;
 #pragma unroll
-                        for (int e = 16 * g; e < 16 * g + 16; e++) {
-                            sr[e] = e < lg ? sr[e] : 0xff800000u;
+                            for (int e = 16 * g; e < 16 * g + 16; e++) {
+                                sr[e] = e < lg ? sr[e] : 0xff800000u;
+                            }
                         }
                     }
-                }
-                // the row's largest s, and the largest s + e over pages with a value scale
-                float top = -INFINITY, rtop = -INFINITY;
+                    if (full) {  // the row's largest s, and the largest s + e over pages with a value scale
+                        float top = m, rtop = R;
 #pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    float a = __uint_as_float(sr[16 * g]), b = __uint_as_float(sr[16 * g + 1]);
+                        for (int g = 0; g < 8; g++) {
+                            float a = __uint_as_float(sr[16 * g]), b = __uint_as_float(sr[16 * g + 1]);
 #pragma unroll
-                    for (int e = 16 * g + 2; e < 16 * g + 14; e += 4) {
-                        a = fmax3(a, __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
-                        b = fmax3(b, __uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3]));
+                            for (int e = 16 * g + 2; e < 16 * g + 14; e += 4) {
+                                a = fmax3(a, __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+                                b = fmax3(b, __uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3]));
+                            }
+                            a    = fmaxf(fmax3(a, __uint_as_float(sr[16 * g + 14]), __uint_as_float(sr[16 * g + 15])), b);
+                            a    = plain ? a * (factor * sc[g].x) : a;
+                            top  = fmaxf(top, a);
+                            rtop = sc[g].y != 0.0f ? fmaxf(rtop, a + sc[g].z) : rtop;
+                        }
+                        if (need) {
+                            l *= m == top ? 1.0f : ex2(m - top);
+                            grow = R == rtop ? 1.0f : ex2(R - rtop);
+                            m = top, R = rtop;
+                        }
                     }
-                    a    = fmaxf(fmax3(a, __uint_as_float(sr[16 * g + 14]), __uint_as_float(sr[16 * g + 15])), b);
-                    top  = fmaxf(top, a);
-                    rtop = sc[g].y != 0.0f ? fmaxf(rtop, a + sc[g].z) : rtop;
+                    const float    ms = m == -INFINITY ? 0.0f : m, base = ms - (R == -INFINITY ? 0.0f : R) + KE_OFF;
+                    const uint64_t nm = f2pack(-ms, -ms);
+                    bool           high = false;
+                    lsum                = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        const float4   q  = sc[g];
+                        const float    f  = ex2(fminf(base + q.z, 90.0f)) * q.y, a = plain ? factor * q.x : 1.0f;
+                        const uint64_t f2 = f2pack(f, f), a2 = f2pack(a, a);
+                        uint64_t       acc = 0ull;
+#pragma unroll
+                        for (int i = 8 * g; i < 8 * g + 8; i++) {
+                            const uint64_t x2 = ffma2(f2pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), a2, nm);
+                            uint64_t       w2;
+                            if (PP == 1 && (i & 7) < KE_EMU) {
+                                w2 = exp2_poly2(x2);
+                            } else {
+                                float x, y;
+                                f2unpack(x2, x, y);
+                                w2 = f2pack(ex2(x), ex2(y));
+                            }
+                            acc = fadd2(acc, w2);
+                            const uint64_t p2 = fmul2(w2, f2);
+                            float          x, y;
+                            f2unpack(p2, x, y);
+                            pk[i] = ke_pack(x, y);
+                            if (PP == 2) {
+                                const float2 b = h2_to_f2(pk[i]);
+                                f2unpack(ffma2(f2pack(b.x, b.y), f2pack(-1.0f, -1.0f), p2), x, y);
+                                pl[i] = ke_pack(x, y);
+                            }
+                        }
+                        float x, y;
+                        f2unpack(acc, x, y);
+                        x += y;
+                        lsum += x;
+                        // the sum bounds every weight of the group; NaN and infinities fail the comparison below
+                        high |= !(x * fabsf(f) <= 32768.0f);
+                    }
+                    if (full || !__any_sync(0xffffffffu, high)) {
+                        break;
+                    }
+                    need = high, full = true;
                 }
-                if (top > m + 8.0f) {
-                    l *= ex2(m - top);
-                    m = top;
-                }
-                float grow = 1.0f;
-                if (rtop > R + 4.0f) {
-                    grow = ex2(R - rtop);
-                    R    = rtop;
-                }
-                const float    ms = m == -INFINITY ? 0.0f : m, rs = R == -INFINITY ? 0.0f : R;
-                const uint64_t nm = f2pack(-ms, -ms);
-                uint64_t       acc[2] = { 0ull, 0ull };
-                uint32_t       pk[KE_N / 2], pl[PP == 2 ? KE_N / 2 : 1];
+                l += lsum;
                 if (!TWO) {
                     grows[(j & 3) * KE_M + r] = grow;
                     dn_mbar_arrive(&bar[KB_GROW + (j & 3)]);
                 }
-#pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    const float    f  = ex2(fminf(ms + sc[g].z - rs + KE_OFF, 90.0f)) * sc[g].y;
-                    const uint64_t f2 = f2pack(f, f);
-#pragma unroll
-                    for (int i = 8 * g; i < 8 * g + 8; i++) {
-                        const uint64_t x2 = fadd2(f2pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), nm);
-                        uint64_t       w2;
-                        if (PP == 1 && (i & 7) < KE_EMU) {
-                            w2 = exp2_poly2(x2);
-                        } else {
-                            float x, y;
-                            f2unpack(x2, x, y);
-                            w2 = f2pack(ex2(x), ex2(y));
-                        }
-                        acc[i & 1] = fadd2(acc[i & 1], w2);
-                        float x, y;
-                        f2unpack(fmul2(w2, f2), x, y);
-                        pk[i] = ke_pack(x, y);
-                        if (PP == 2) {
-                            const float2 b = h2_to_f2(pk[i]);
-                            pl[i]          = ke_pack(x - b.x, y - b.y);
-                        }
-                    }
-                }
-                float a0, a1;
-                f2unpack(fadd2(acc[0], acc[1]), a0, a1);
-                l += a0 + a1;
                 tmem_st32(s_col, &pk[0]);
                 tmem_st32(s_col + 32, &pk[32]);
                 if (PP == 2) {
@@ -719,8 +791,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
             // O (units of 2^(R - KE_OFF)) over the sum (2^m); rows without keys, and without a value scale, are 0
             const float inv = l != 0.0f ? (1.0f / (1 << KE_OFF)) / l : 0.0f, up = R == -INFINITY ? 0.0f : ex2(R - m);
             if (!TWO) {
-                // every warp has staged its rows of Q when warpgroup 3 writes over them
-                if (!dn_wait_warp(&bar[KB_QREADY], 0, deadline) || !ok) {
+                if (!ok) {
                     atomicExch(abort_f, 1);
                 }
                 grows[4 * KE_M + r] = inv, grows[5 * KE_M + r] = up;
@@ -732,9 +803,8 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 have = dn_wait_warp(&bar[KB_OFULL + t], 0, deadline);
                 tc_fence_after();
             }
-            // Q's shared memory takes the result: every product has to be done, and every warp with its rows of Q
-            // (which no product waited for where there are no tiles)
-            if (!dn_wait_warp(&bar[KB_DONE], 0, deadline) || !dn_wait_warp(&bar[KB_QREADY + t], 0, deadline) || (!have && tiles > 0)) {
+            // Q's shared memory takes the result: every product has to be done
+            if (!dn_wait_warp(&bar[KB_DONE], 0, deadline) || (!have && tiles > 0)) {
                 atomicExch(abort_f, 1);
                 have = false;
             }
