@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 // The weights are taken with the maxima as they are (only a row's first tile has none), and the maxima found
                 // and the weights taken again where a group's sum shows that one could leave F16's range
                 // - by the rows that need it: no row's result depends on its neighbours'
-                bool     need = m == -INFINITY || R == -INFINITY, full = __any_sync(0xffffffffu, need);
+                bool     need = m == -INFINITY || R == -INFINITY, full = __any_sync(0xffffffffu, need), fresh = false;
                 float    grow = 1.0f, lsum;
                 uint32_t pk[KE_N / 2], pl[PP == 2 ? KE_N / 2 : 1];
 #pragma unroll 1
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                         if (need) {
                             l *= m == top ? 1.0f : ex2(m - top);
                             grow = R == rtop ? 1.0f : ex2(R - rtop);
-                            m = top, R = rtop;
+                            m = top, R = rtop, fresh = true;
                         }
                     }
                     const float    ms = m == -INFINITY ? 0.0f : m, base = ms - (R == -INFINITY ? 0.0f : R) + KE_OFF;
@@ -754,10 +754,11 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                         // the sum bounds every weight of the group; NaN and infinities fail the comparison below
                         high |= !(x * fabsf(f) <= 32768.0f);
                     }
-                    if (full || !__any_sync(0xffffffffu, high)) {
+                    need = high && !fresh;
+                    if (!__any_sync(0xffffffffu, need)) {
                         break;
                     }
-                    need = high, full = true;
+                    full = true;
                 }
                 l += lsum;
                 if (!TWO) {

@@ -192,6 +192,31 @@ def test_attend_nan_stays_in_its_rows(cuda_device, n_q):
         assert torch.equal(out, good)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attend_rows_that_grow_beside_rows_that_start_late(cuda_device, dtype):
+    """Many rows whose scores rise by far from tile to tile beside causal rows that see no key yet, and beside rows
+    of NaN: each takes its maxima up when it needs to, whatever its neighbours do."""
+    dt = DTYPES[dtype]
+    st = R.State([600, 520], 1, 64, 64, seed=17, device=cuda_device)
+    st.k.zero_()
+    st.ks.fill_(1.0)
+    for s, n in enumerate((600, 520)):
+        for j in range(-(-n // 64)):
+            st.k[0, int(st.table[s, j]), 0, :, 0] = 12 * j  # 12 units of 2^s more each page
+    q = torch.zeros(2, 4, 130, 64, device=cuda_device)
+    q[..., 0] = torch.linspace(-2, 2, 130, device=cuda_device)
+    q = q.to(dt)
+    run_attend(st, 4, 130, dt, q=q, scale=1.0)
+    run_attend(st, 4, 130, dt, q=q, scale=1.0, causal=False)
+    want = st.cache().attend(0, q, st.table, st.len, 1.0)
+    q2 = q.clone()
+    q2[0, :, 5::8] = float("nan")
+    got = st.cache().attend(0, q2, st.table, st.len, 1.0)
+    assert got[0, 5::8].isnan().all()
+    got[0, 5::8] = want[0, 5::8]
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("N,H,Hkv,n_q", [(300, 4, 2, 1), (65, 2, 1, 40), (1, 64, 32, 1)])
 def test_attend_many_sequences(cuda_device, N, H, Hkv, n_q):
     st = R.State([(37 * i) % 211 for i in range(N)], Hkv, 64, 16, seed=N, device=cuda_device)
