@@ -175,7 +175,7 @@ struct Kv8Once {
 };
 
 cudaError_t launch_kv8_append(const Kv8StoreParams & p, cudaStream_t stream);
-cudaError_t launch_kv8_read(const Kv8StoreParams & p, int sms, cudaStream_t stream);
+cudaError_t launch_kv8_read(const Kv8StoreParams & p, cudaStream_t stream);
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p, int sms, cudaStream_t stream);
 cudaError_t launch_kv8_dense(const Kv8AttnParams & p, cudaStream_t stream);
 size_t      kv8_attn_workspace_bytes(int D, int n_q, int ratio, int n_head_kv, int n_seq, int sms);

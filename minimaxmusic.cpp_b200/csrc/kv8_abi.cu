@@ -269,8 +269,7 @@ int mm3fa_kv8_read(const mm3fa_kv8 * cache, int layer, const mm3fa_kv8_table * t
     if (host_device_major() != 10) {
         return MM3FA_ERR_DEVICE;
     }
-    return host_record_cuda(launch_kv8_read(store_params(cache, layer, k_out, v_out, table, start, n), host_sm_count(),
-                                            static_cast<cudaStream_t>(stream)));
+    return host_record_cuda(launch_kv8_read(store_params(cache, layer, k_out, v_out, table, start, n), static_cast<cudaStream_t>(stream)));
 }
 
 size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q, const mm3fa_kv8_table * table) {

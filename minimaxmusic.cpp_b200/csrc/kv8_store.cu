@@ -9,51 +9,40 @@
 // finite do not enter the maximum; NaN is stored as 0, +-inf as +-127.  Rows behind the last new one
 // keep their bytes.
 //
-// Bound by memory for a prompt (rows read once from HBM, codes written) and by latency for one token.
+// A page's rows stay in registers between the maximum and the codes, so that they are read once.  Bound by
+// memory for a prompt and by latency for one token.
 #include "kv8.cuh"
 
 namespace mm3fa {
 
-constexpr int KV8_STORE_THREADS = 256;
+constexpr int KS_VALUES = 32;  // of a page's rows that a thread of the append holds: 8 runs of 4
+constexpr int KS_READ_THREADS = 256;
+constexpr int KS_READ_ROWS    = 64;  // rows per CTA of the read
 
-// N consecutive elements of a row from element e (N * element size a multiple of 16 where vec).
-template <int N>
-__device__ __forceinline__ void kv8_load(const char * row, int type, int vec, int e, float (&x)[N]) {
+// 4 consecutive elements of a row from element e (a multiple of 4).
+__device__ __forceinline__ void ks_load(const char * row, int type, int vec, int e, float (&x)[4]) {
     if (type == KV_F32) {
         const float * p = reinterpret_cast<const float *>(row) + e;
         if (vec) {
-#pragma unroll
-            for (int i = 0; i < N; i += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(p + i);
-                x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
-            }
+            const float4 f = __ldcs(reinterpret_cast<const float4 *>(p));
+            x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < N; i++) {
+            for (int i = 0; i < 4; i++) {
                 x[i] = p[i];
             }
         }
         return;
     }
     const uint16_t * p = reinterpret_cast<const uint16_t *>(row) + e;
-    uint32_t         w[N / 2];
+    uint2            w;
     if (vec) {
-#pragma unroll
-        for (int i = 0; i < N / 2; i += 4) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(p + 2 * i);
-            w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
-        }
+        w = __ldcs(reinterpret_cast<const uint2 *>(p));
     } else {
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            w[i] = (uint32_t) p[2 * i] | ((uint32_t) p[2 * i + 1] << 16);
-        }
+        w.x = (uint32_t) p[0] | ((uint32_t) p[1] << 16), w.y = (uint32_t) p[2] | ((uint32_t) p[3] << 16);
     }
-#pragma unroll
-    for (int i = 0; i < N / 2; i++) {
-        const float2 f = type == KV_F16 ? h2_to_f2(w[i]) : bf2_to_f2(w[i]);
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    }
+    const float2 a = type == KV_F16 ? h2_to_f2(w.x) : bf2_to_f2(w.x), b = type == KV_F16 ? h2_to_f2(w.y) : bf2_to_f2(w.y);
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
 }
 
 // rne(x / d) clamped to +-127, exactly: q = rint(x * (1/d)) is at most one off next to a tie, and the
@@ -78,11 +67,11 @@ __device__ __forceinline__ int kv8_requant(int c, float d_old, float d, float ra
     return (int) rint((double) c * (double) d_old / (double) d);
 }
 
-__global__ void __launch_bounds__(KV8_STORE_THREADS) kv8_append_kernel(const Kv8StoreParams p) {
-    constexpr int THREADS = KV8_STORE_THREADS;
-    const int     tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int     s = (int) blockIdx.z, h = (int) blockIdx.y >> 1, is_v = (int) blockIdx.y & 1;
-    __shared__ float red[THREADS / 32];
+// P * D / KS_VALUES threads (at least 64)
+__global__ void __launch_bounds__(1024) kv8_append_kernel(const Kv8StoreParams p) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = (int) blockDim.x;
+    const int s = (int) blockIdx.z, h = (int) blockIdx.y >> 1, is_v = (int) blockIdx.y & 1;
+    __shared__ float red[32];
     kv8_dep_wait();
     const int P = p.c.P, D = p.c.D;
     const int start = p.start[s];
@@ -98,39 +87,44 @@ __global__ void __launch_bounds__(KV8_STORE_THREADS) kv8_append_kernel(const Kv8
     if (page < 0 || r1 <= r0) {
         return;
     }
-    const Kv8Rows & x   = is_v ? p.v : p.k;
-    const int64_t   ph  = (int64_t) page * p.c.n_head_kv + h;
-    int8_t *        dst = (is_v ? p.c.v : p.c.k) + ph * P * D;
-    float *         sc  = (is_v ? p.c.v_scale : p.c.k_scale) + ph;
-    const char *    src = x.data + (int64_t) h * x.nb2 + (int64_t) s * x.nb3;
-    const int       per = D / 16;  // 16-value pieces of a row
+    const Kv8Rows & x    = is_v ? p.v : p.k;
+    const int64_t   ph   = (int64_t) page * p.c.n_head_kv + h;
+    int8_t *        dst  = (is_v ? p.c.v : p.c.k) + ph * P * D;
+    float *         sc   = (is_v ? p.c.v_scale : p.c.k_scale) + ph;
+    const char *    src  = x.data + (int64_t) h * x.nb2 + (int64_t) s * x.nb3 + (first + r0 - start) * x.nb1;
+    const int       runs = (r1 - r0) * (D / 4), col = tid % (D / 4), step = threads / (D / 4);  // threads: a multiple of D / 4
+    float           v[KS_VALUES / 4][4];
     float           amax = 0.0f;
-    for (int i = tid; i < (r1 - r0) * per; i += THREADS) {
-        float v[16];
-        kv8_load<16>(src + (first + r0 + i / per - start) * x.nb1, x.type, x.vec, i % per * 16, v);
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const float a = fabsf(v[e]);
-            amax          = a < INFINITY ? fmaxf(amax, a) : amax;
+    for (int k = 0; k < KS_VALUES / 4; k++) {
+        if (tid + k * threads < runs) {
+            ks_load(src + (int64_t) (tid / (D / 4) + k * step) * x.nb1, x.type, x.vec, col * 4, v[k]);
         }
     }
+    const float before = r0 > 0 ? *sc : 0.0f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int k = 0; k < KS_VALUES / 4; k++) {
+        if (tid + k * threads < runs) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float a = fabsf(v[k][e]);
+                amax          = a < INFINITY ? fmaxf(amax, a) : amax;
+            }
+        }
     }
+    // magnitudes order like their bits
+    amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
     if (lane == 0) {
         red[warp] = amax;
     }
-    const float before = r0 > 0 ? *sc : 0.0f;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; w++) {
+    for (int w = 0; w < threads / 32; w++) {
         amax = fmaxf(amax, red[w]);
     }
     const float d = fmaxf(before, amax / 127.0f);
     if (r0 > 0 && d > before) {
         const float ratio = before / d;
-        for (int i = tid; i < r0 * per; i += THREADS) {
+        for (int i = tid; i < r0 * (D / 16); i += threads) {
             union {
                 uint4  u;
                 int8_t c[16];
@@ -146,108 +140,110 @@ __global__ void __launch_bounds__(KV8_STORE_THREADS) kv8_append_kernel(const Kv8
     // a scale whose reciprocal would overflow is brought up by an exact power of two, like its rows
     const float up = d < 1e-30f ? 18446744073709551616.0f : 1.0f, du = d * up;
     const float inv = d > 0.0f ? 1.0f / du : 0.0f;
-    for (int i = tid; i < (r1 - r0) * per; i += THREADS) {
-        float v[16];
-        kv8_load<16>(src + (first + r0 + i / per - start) * x.nb1, x.type, x.vec, i % per * 16, v);
-        union {
-            uint4  u;
-            int8_t c[16];
-        } w;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            w.c[e] = (int8_t) (d > 0.0f ? kv8_code(v[e] * up, du, inv) : (v[e] == INFINITY ? 127 : v[e] == -INFINITY ? -127 : 0));
+    for (int k = 0; k < KS_VALUES / 4; k++) {
+        if (tid + k * threads < runs) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float a = v[k][e];
+                const int   c = d > 0.0f ? kv8_code(a * up, du, inv) : (a == INFINITY ? 127 : a == -INFINITY ? -127 : 0);
+                w |= (uint32_t) (c & 255) << (8 * e);
+            }
+            reinterpret_cast<uint32_t *>(dst + (int64_t) r0 * D)[tid + k * threads] = w;
         }
-        *reinterpret_cast<uint4 *>(dst + (int64_t) r0 * D + (int64_t) i * 16) = w.u;
     }
     if (tid == 0) {
         *sc = d;
     }
 }
 
-// ---- read: rows start[s] .. start[s] + n[s] of each sequence as values; 16 codes per thread
-__global__ void __launch_bounds__(KV8_STORE_THREADS) kv8_read_kernel(const Kv8StoreParams p) {
+// ---- read: rows start[s] .. start[s] + n[s] of each sequence as values; a warp takes 8 rows, 4 codes a lane at a
+// time, so that loads and stores are runs of bytes
+template <int D>
+__global__ void __launch_bounds__(KS_READ_THREADS) kv8_read_kernel(const Kv8StoreParams p) {
+    constexpr int LPR = D / 4, ROWS = KS_READ_ROWS / (KS_READ_THREADS / 32), IT = ROWS * LPR / 32;  // lanes per row, rows per warp
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int s = (int) blockIdx.z, h = (int) blockIdx.y >> 1, is_v = (int) blockIdx.y & 1;
     kv8_dep_wait();
-    const int     D = p.c.D, P = p.c.P, per = D / 16;
-    const int64_t rows  = (int64_t) p.t.n_seq * p.c.n_head_kv * p.n_rows;
-    const int64_t items = 2 * rows * per;
-    for (int64_t i = (int64_t) blockIdx.x * KV8_STORE_THREADS + threadIdx.x; i < items;
-         i += (int64_t) gridDim.x * KV8_STORE_THREADS) {
-        const int     piece = (int) (i % per);
-        const int64_t r     = i / per;
-        const bool    is_v  = r >= rows;
-        const int64_t rr    = is_v ? r - rows : r;
-        const int     row   = (int) (rr % p.n_rows);
-        const int     h     = (int) (rr / p.n_rows % p.c.n_head_kv);
-        const int     s     = (int) (rr / p.n_rows / p.c.n_head_kv);
-        const int64_t tok   = (int64_t) p.start[s] + row;
-        if (tok < 0 || row >= (p.n ? p.n[s] : p.n_rows) || (tok >> p.c.log2p) >= p.t.max_pages) {
-            continue;
-        }
-        const int page = kv8_page(p.t, p.c.n_pages, s, (int) (tok >> p.c.log2p));
-        if (page < 0) {
-            continue;
-        }
-        const int64_t ph = (int64_t) page * p.c.n_head_kv + h;
-        const float   sc = (is_v ? p.c.v_scale : p.c.k_scale)[ph];
-        union {
-            uint4  u;
-            int8_t c[16];
-        } w;
-        w.u = *reinterpret_cast<const uint4 *>((is_v ? p.c.v : p.c.k) + (ph * P + (tok & (P - 1))) * D + piece * 16);
-        float v[16];
+    const int       n     = p.n ? min(p.n[s], p.n_rows) : p.n_rows;
+    const int64_t   start = p.start[s];
+    const Kv8Rows & o     = is_v ? p.v : p.k;
+    const int8_t *  pool  = is_v ? p.c.v : p.c.k;
+    const float *   scale = is_v ? p.c.v_scale : p.c.k_scale;
+    char *          out   = o.data + (int64_t) h * o.nb2 + (int64_t) s * o.nb3;
+    const int       r0    = (int) blockIdx.x * KS_READ_ROWS + warp * ROWS;
+    uint32_t        w[IT];
+    float           sc[IT];
+    bool            ok[IT];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            v[e] = (float) w.c[e] * sc;
+    for (int i = 0; i < IT; i++) {
+        const int     at = i * 32 + lane, row = r0 + at / LPR, col = at % LPR;
+        const int64_t tok = start + row;
+        ok[i] = false;
+        if (row < n && tok >= 0 && (tok >> p.c.log2p) < p.t.max_pages) {
+            const int page = kv8_page(p.t, p.c.n_pages, s, (int) (tok >> p.c.log2p));
+            if (page >= 0) {
+                const int64_t ph = (int64_t) page * p.c.n_head_kv + h;
+                ok[i] = true;
+                w[i]  = *reinterpret_cast<const uint32_t *>(pool + (ph * p.c.P + (tok & (p.c.P - 1))) * D + col * 4);
+                sc[i] = scale[ph];
+            }
         }
-        const Kv8Rows & o   = is_v ? p.v : p.k;
-        char *          out = o.data + (int64_t) row * o.nb1 + (int64_t) h * o.nb2 + (int64_t) s * o.nb3;
+    }
+#pragma unroll
+    for (int i = 0; i < IT; i++) {
+        if (!ok[i]) {
+            continue;
+        }
+        const int at = i * 32 + lane, row = r0 + at / LPR, col = at % LPR;
+        float     v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[e] = (float) (int8_t) (w[i] >> (8 * e)) * sc[i];
+        }
+        char * dst = out + (int64_t) row * o.nb1;
         if (o.type == KV_F32) {
-            float * f = reinterpret_cast<float *>(out) + piece * 16;
+            float * f = reinterpret_cast<float *>(dst) + col * 4;
             if (o.vec) {
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    *reinterpret_cast<float4 *>(f + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                }
+                __stcs(reinterpret_cast<float4 *>(f), make_float4(v[0], v[1], v[2], v[3]));
             } else {
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    f[e] = v[e];
-                }
+                f[0] = v[0], f[1] = v[1], f[2] = v[2], f[3] = v[3];
             }
             continue;
         }
-        union {
-            uint4    u[2];
-            uint16_t h[16];
-        } b;
+        uint16_t b[4];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            b.h[e] = o.type == KV_F16 ? __half_as_ushort(__float2half_rn(v[e])) : __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
+        for (int e = 0; e < 4; e++) {
+            b[e] = o.type == KV_F16 ? __half_as_ushort(__float2half_rn(v[e])) : __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
         }
-        uint16_t * f = reinterpret_cast<uint16_t *>(out) + piece * 16;
+        uint16_t * f = reinterpret_cast<uint16_t *>(dst) + col * 4;
         if (o.vec) {
-            reinterpret_cast<uint4 *>(f)[0] = b.u[0];
-            reinterpret_cast<uint4 *>(f)[1] = b.u[1];
+            __stcs(reinterpret_cast<uint2 *>(f), make_uint2(b[0] | (uint32_t) b[1] << 16, b[2] | (uint32_t) b[3] << 16));
         } else {
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                f[e] = b.h[e];
-            }
+            f[0] = b[0], f[1] = b[1], f[2] = b[2], f[3] = b[3];
         }
     }
 }
 
 cudaError_t launch_kv8_append(const Kv8StoreParams & p, cudaStream_t stream) {
     // T rows touch at most ceil((T - 1) / P) + 1 pages of a sequence
-    const unsigned pages = (unsigned) ((p.n_rows - 1 + p.c.P - 1) / p.c.P + 1);
-    return kv8_launch(kv8_append_kernel, dim3(pages, 2u * (unsigned) p.c.n_head_kv, (unsigned) p.t.n_seq), KV8_STORE_THREADS,
+    const unsigned pages   = (unsigned) ((p.n_rows - 1 + p.c.P - 1) / p.c.P + 1);
+    const int      threads = p.c.P * p.c.D / KS_VALUES;
+    return kv8_launch(kv8_append_kernel, dim3(pages, 2u * (unsigned) p.c.n_head_kv, (unsigned) p.t.n_seq), threads < 64 ? 64 : threads,
                       0, stream, p);
 }
 
-cudaError_t launch_kv8_read(const Kv8StoreParams & p, int sms, cudaStream_t stream) {
-    const int64_t items  = 2 * (int64_t) p.t.n_seq * p.c.n_head_kv * p.n_rows * (p.c.D / 16);
-    const int64_t blocks = (items + KV8_STORE_THREADS - 1) / KV8_STORE_THREADS;
-    return kv8_launch(kv8_read_kernel, dim3((unsigned) (blocks < 8 * sms ? blocks : 8 * sms)), KV8_STORE_THREADS, 0, stream, p);
+cudaError_t launch_kv8_read(const Kv8StoreParams & p, cudaStream_t stream) {
+    const dim3 grid((unsigned) ((p.n_rows + KS_READ_ROWS - 1) / KS_READ_ROWS), 2u * (unsigned) p.c.n_head_kv, (unsigned) p.t.n_seq);
+    switch (p.c.D) {
+        case 64:
+            return kv8_launch(kv8_read_kernel<64>, grid, KS_READ_THREADS, 0, stream, p);
+        case 128:
+            return kv8_launch(kv8_read_kernel<128>, grid, KS_READ_THREADS, 0, stream, p);
+        default:
+            return kv8_launch(kv8_read_kernel<256>, grid, KS_READ_THREADS, 0, stream, p);
+    }
 }
 
 }  // namespace mm3fa
