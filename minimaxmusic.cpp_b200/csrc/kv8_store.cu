@@ -105,10 +105,18 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const Kv8StoreParams p
 #pragma unroll
     for (int k = 0; k < KS_VALUES / 4; k++) {
         if (tid + k * threads < runs) {
+            amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v[k][0]), fabsf(v[k][1]))), fmaxf(fabsf(v[k][2]), fabsf(v[k][3])));  // not NaN
+        }
+    }
+    if (!(amax < INFINITY)) {  // without infinities
+        amax = 0.0f;
+#pragma unroll 1
+        for (int i = tid; i < runs; i += threads) {
+            float y[4];
+            ks_load(src + (int64_t) (i / (D / 4)) * x.nb1, x.type, x.vec, col * 4, y);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float a = fabsf(v[k][e]);
-                amax          = a < INFINITY ? fmaxf(amax, a) : amax;
+                amax = fabsf(y[e]) < INFINITY ? fmaxf(amax, fabsf(y[e])) : amax;
             }
         }
     }
@@ -143,12 +151,26 @@ __global__ void __launch_bounds__(1024) kv8_append_kernel(const Kv8StoreParams p
 #pragma unroll
     for (int k = 0; k < KS_VALUES / 4; k++) {
         if (tid + k * threads < runs) {
-            uint32_t w = 0;
+            // q = rne(x inv) in the low bits of x inv + 1.5 * 2^23.  x inv is within 127 * 2^-24 of the quotient, so q is
+            // right where x inv is 1e-5 away from a tie; the rest (NaN and infinities too) by the remainder
+            constexpr float MAGIC = 12582912.0f;
+            uint32_t        u[4];
+            bool            sure = d >= 1e-30f;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float a = v[k][e];
-                const int   c = d > 0.0f ? kv8_code(a * up, du, inv) : (a == INFINITY ? 127 : a == -INFINITY ? -127 : 0);
-                w |= (uint32_t) (c & 255) << (8 * e);
+                const float m = fmaf(v[k][e], inv, MAGIC);
+                u[e]          = __float_as_uint(m);
+                sure          = sure && fabsf(fmaf(v[k][e], inv, MAGIC - m)) <= 0.49999f;
+            }
+            uint32_t w = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+            if (!sure) {
+                w = 0;
+#pragma unroll 1
+                for (int e = 0; e < 4; e++) {
+                    const float a = e == 0 ? v[k][0] : e == 1 ? v[k][1] : e == 2 ? v[k][2] : v[k][3];
+                    const int   c = d > 0.0f ? kv8_code(a * up, du, inv) : (a == INFINITY ? 127 : a == -INFINITY ? -127 : 0);
+                    w |= (uint32_t) (c & 255) << (8 * e);
+                }
             }
             reinterpret_cast<uint32_t *>(dst + (int64_t) r0 * D)[tid + k * threads] = w;
         }
@@ -173,34 +195,36 @@ __global__ void __launch_bounds__(KS_READ_THREADS) kv8_read_kernel(const Kv8Stor
     const float *   scale = is_v ? p.c.v_scale : p.c.k_scale;
     char *          out   = o.data + (int64_t) h * o.nb2 + (int64_t) s * o.nb3;
     const int       r0    = (int) blockIdx.x * KS_READ_ROWS + warp * ROWS;
+    // the warp's rows lie in two pages at most (a page has 16 tokens or more)
+    const int64_t   tok0 = start + r0;
+    const int       in0  = (int) (tok0 & (p.c.P - 1)), split = p.c.P - in0;  // rows of the first page
+    const int       j0   = (tok0 >> p.c.log2p) < p.t.max_pages ? (int) (tok0 >> p.c.log2p) : p.t.max_pages;  // negative: kv8_page knows
+    const int       pg0  = kv8_page(p.t, p.c.n_pages, s, j0), pg1 = kv8_page(p.t, p.c.n_pages, s, j0 + 1);
+    const int64_t   ph0  = (int64_t) max(pg0, 0) * p.c.n_head_kv + h, ph1 = (int64_t) max(pg1, 0) * p.c.n_head_kv + h;
+    const float     sc0  = scale[ph0], sc1 = scale[ph1];
+    const int8_t *  a0   = pool + (ph0 * p.c.P + in0) * D, *a1 = pool + (ph1 * p.c.P - split) * D;
     uint32_t        w[IT];
-    float           sc[IT];
-    bool            ok[IT];
 #pragma unroll
     for (int i = 0; i < IT; i++) {
-        const int     at = i * 32 + lane, row = r0 + at / LPR, col = at % LPR;
-        const int64_t tok = start + row;
-        ok[i] = false;
-        if (row < n && tok >= 0 && (tok >> p.c.log2p) < p.t.max_pages) {
-            const int page = kv8_page(p.t, p.c.n_pages, s, (int) (tok >> p.c.log2p));
-            if (page >= 0) {
-                const int64_t ph = (int64_t) page * p.c.n_head_kv + h;
-                ok[i] = true;
-                w[i]  = *reinterpret_cast<const uint32_t *>(pool + (ph * p.c.P + (tok & (p.c.P - 1))) * D + col * 4);
-                sc[i] = scale[ph];
-            }
+        const int at = i * 32 + lane, rr = at / LPR;
+        w[i] = 0;
+        if (r0 + rr < n && tok0 + rr >= 0 && (rr < split ? pg0 : pg1) >= 0) {
+            w[i] = *reinterpret_cast<const uint32_t *>((rr < split ? a0 : a1) + at * 4);
         }
     }
 #pragma unroll
     for (int i = 0; i < IT; i++) {
-        if (!ok[i]) {
+        const int at = i * 32 + lane, rr = at / LPR, row = r0 + rr, col = at % LPR;
+        if (!(row < n && tok0 + rr >= 0 && (rr < split ? pg0 : pg1) >= 0)) {
             continue;
         }
-        const int at = i * 32 + lane, row = r0 + at / LPR, col = at % LPR;
-        float     v[4];
+        const float sc = rr < split ? sc0 : sc1;
+        float       v[4];
+        // 2^23 + (code + 128), exactly, less 2^23 + 128
+        const uint32_t u = w[i] ^ 0x80808080u;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            v[e] = (float) (int8_t) (w[i] >> (8 * e)) * sc[i];
+            v[e] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 | e)) - 8388736.0f) * sc;
         }
         char * dst = out + (int64_t) row * o.nb1;
         if (o.type == KV_F32) {
