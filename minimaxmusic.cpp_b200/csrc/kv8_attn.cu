@@ -34,8 +34,8 @@ constexpr int KD_BLOCK   = 32;     // keys per block
 constexpr int KD_ROWS    = 16;     // query rows per unit
 constexpr int KD_OFF     = 12;     // P is held times 2^12: F16 keeps 11 bits down to 2^-26 of the largest weight
 constexpr int KD_WHOLE   = 16;
-constexpr int KD_PART    = 8;      // blocks of a part, at least
-constexpr int KD_CROSS   = 8;
+constexpr int KD_PART    = 4;      // blocks of a part, at least
+constexpr int KD_CROSS   = 32;
 constexpr int KD_DENSE   = 64;     // rows of a kv head from which the kernel for many rows takes over (D <= 128)
 
 template <int D, int NT, bool HP>
@@ -320,6 +320,11 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
             fetch();
         }
     };
+    // Places in a stage, less what a loop adds or flips (kd_swz of a row is what its lane gives, xor what the loop
+    // gives): this lane's chunk of 512 bytes that are loaded; K's (and q's) chunk 2 t of row g; V's chunk g of row 2 t
+    const uint32_t ld_to = (uint32_t) ((lane / (D / 16)) * D + (((lane % (D / 16)) ^ (D == 64 ? (lane >> 3) & 3 : lane / (D / 16))) << 4));
+    const int      k_at  = g * D + (((D == 64 ? t : 2 * t) ^ kd_swz<D>(g)) << 4);
+    const int      v_at  = 2 * t * D + (D == 64 ? (((g >> 1) ^ t) << 4) + (g & 1) * 8 : (g ^ (2 * t)) << 4);
     int  ld_stage = 0;
     auto load     = [&] {
         if (ld_on) {
@@ -334,14 +339,13 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
             const int64_t  o1 = (p.c.log2p > 4 ? o0 : ph1 * p.c.P * D - 16 * D);
             const uint32_t z0 = ok0 ? 16u : 0u, z1 = ok1 ? 16u : 0u;
             const uint32_t dst = smem_addr(st);
+            const int8_t * k0 = p.c.k + o0 + lane * 16, *k1 = p.c.k + o1 + lane * 16, *v0 = p.c.v + o0 + lane * 16, *v1 = p.c.v + o1 + lane * 16;
 #pragma unroll
             for (int i = 0; i < 4 * CH; i++) {  // 32 rows of D / 16 chunks, 32 chunks at a time
-                const int     idx  = i * 32 + lane, r = idx / (D / 16), ck = idx % (D / 16);
-                const bool    half = i >= 2 * CH;
-                const int64_t off  = (half ? o1 : o0) + idx * 16;
-                const uint32_t to  = dst + (uint32_t) (r * D + ((ck ^ kd_swz<D>(r)) << 4));
-                kd_cp16(to, p.c.k + off, half ? z1 : z0);
-                kd_cp16(to + L::TILE, p.c.v + off, half ? z1 : z0);
+                const bool     half = i >= 2 * CH;
+                const uint32_t to   = dst + (ld_to ^ (uint32_t) ((D == 64 ? 0 : i * (512 / D) & 7) << 4)) + i * 512;
+                kd_cp16(to, (half ? k1 : k0) + i * 512, half ? z1 : z0);
+                kd_cp16(to + L::TILE, (half ? v1 : v0) + i * 512, half ? z1 : z0);
             }
             if (lane < 4) {
                 const int64_t ph = lane & 1 ? ph1 : ph0;
@@ -518,22 +522,20 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                 }
 #pragma unroll
                 for (int j = 0; j < CH; j++) {
-                    const int ck = D == 64 ? t : 2 * t + (j & 1) + 8 * (j >> 1);
+                    const int at = (k_at ^ ((j & 1) << 4)) + (j >> 1) * 128;
                     uint4     w[AP][2];
 #pragma unroll
                     for (int a = 0; a < AP; a++) {
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            const int r = 16 * (a0 + a) + 8 * i + g;
-                            w[a][i]     = *reinterpret_cast<const uint4 *>(st + r * D + ((ck ^ kd_swz<D>(r)) << 4));
+                            w[a][i] = *reinterpret_cast<const uint4 *>(st + (16 * (a0 + a) + 8 * i) * D + at);
                         }
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                         for (int d = 0; d < ND; d++) {
-                            const int   r = nt * 8 + g;
-                            const uint4 b = *reinterpret_cast<const uint4 *>(qf + (d * NT * 8 + r) * D + ((ck ^ kd_swz<D>(r)) << 4));
+                            const uint4 b = *reinterpret_cast<const uint4 *>(qf + (d * NT + nt) * 8 * D + at);
 #pragma unroll
                             for (int a = 0; a < AP; a++) {
                                 kd_mma_s8(acc[a][nt][d], w[a][0].x, w[a][1].x, w[a][0].y, w[a][1].y, b.x, b.y);
@@ -666,12 +668,12 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                     uint32_t      w[4][WORDS];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int r = 16 * a + 2 * t + (i & 1) + 8 * (i >> 1);
+                        const int r = (16 * a + (i & 1) + 8 * (i >> 1)) * D;  // beyond row 2 t
                         if (D == 64) {
-                            const uint2 u = *reinterpret_cast<const uint2 *>(vt + r * D + (((g >> 1) ^ kd_swz<D>(r)) << 4) + (g & 1) * 8);
+                            const uint2 u = *reinterpret_cast<const uint2 *>(vt + r + v_at);
                             w[i][0] = u.x, w[i][1] = u.y;
                         } else {
-                            const uint4 u = *reinterpret_cast<const uint4 *>(vt + r * D + (((g + 8 * j) ^ kd_swz<D>(r)) << 4));
+                            const uint4 u = *reinterpret_cast<const uint4 *>(vt + r + (v_at ^ ((i & 1) << 4)) + 128 * j);
                             w[i][0] = u.x, w[i][1] = u.y, w[i][WORDS - 2] = u.z, w[i][WORDS - 1] = u.w;
                         }
                     }
