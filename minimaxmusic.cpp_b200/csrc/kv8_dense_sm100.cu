@@ -40,6 +40,7 @@ constexpr int KE_THREADS = 512;
 constexpr int KE_M       = 128;  // rows per Q tile
 constexpr int KE_N       = 128;  // keys per tile
 constexpr int KE_TMEM    = 512;
+constexpr int KE_EMU     = 1;    // of every 8 pairs of weights, those by polynomial where P is rounded to F16 anyway
 constexpr int KE_OFF     = 8;    // P is held times 2^8: 2^14 at most with the lazy maxima
 constexpr int KE_REGS_LAUNCH  = 128;  // 65536 / 512
 constexpr int KE_REGS_SOFTMAX = 192;  // 2 x 192 + 96 + 32 = 4 x 128
@@ -89,14 +90,6 @@ __host__ __device__ constexpr uint32_t ke_arrivals(int b) {
                    (b >= KB_GROW && b < KB_DONE)
                ? 128u
                : (b >= KB_SCALES && b < KB_GROW ? 8u : 1u);
-}
-
-__device__ __forceinline__ void ke_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
 }
 
 __device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
@@ -295,21 +288,20 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 }
                 umma_commit(&bar[KB_SFULL + buf]);
             };
-            // P of 32 keys takes half of their scores' 32 columns, its remainder the other half
             auto pv = [&](int t, int j) {
                 const int buf = TWO ? t : j & 1;
 #pragma unroll 1
                 for (int part = PP - 1; part >= 0; part--) {
-                    uint32_t a = tmem + (uint32_t) (buf * KE_N + part * 16);
+                    uint32_t a = tmem + (uint32_t) (buf * KE_N + part * 64);
                     uint64_t b = v_d + (uint64_t) (((j % NV) * L::KT) >> 4);
 #pragma unroll 1
                     for (int c = 0; c < 2; c++) {
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), a + (uint32_t) (32 * (k >> 1) + 8 * (k & 1)), b + (uint64_t) ((k * 16 * 128) >> 4), id_pv,
+                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), a + (uint32_t) (8 * k), b + (uint64_t) ((k * 16 * 128) >> 4), id_pv,
                                         (TWO ? j : 0) + PP - 1 - part + c + k > 0 ? 1u : 0u);
                         }
-                        a += 64, b += (4 * 16 * 128) >> 4;
+                        a += 32, b += (4 * 16 * 128) >> 4;
                     }
                 }
             };
@@ -671,105 +663,122 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                     tmem_st_wait();
                 }
                 bool whole = j * KE_N + KE_N <= warp_lim;  // every row of the warp sees every column
+                bool plain = !CAP;                         // s = S * factor * a, with all of these positive
 #pragma unroll
                 for (int g = 0; g < 8; g++) {
                     whole &= sc[g].w != 0.0f;
+                    plain &= !(factor * sc[g].x <= 0.0f);  // NaN: a row of NaN, whose neighbours go on as without it
                 }
-                // 32 columns c of s, in log2 units (after CAP they are already)
-                auto scores = [&](int c, uint32_t (&sr)[32]) {
-                    tmem_ld32(s_col + (uint32_t) (c * 32), sr);
-                    const float a0 = CAP ? 1.0f : factor * sc[2 * c].x, a1 = CAP ? 1.0f : factor * sc[2 * c + 1].x;
-                    tmem_ld_wait_tie(sr);
+                plain = __all_sync(0xffffffffu, plain);
+                // The weights are taken with the maxima as they are (only a row's first tile has none), and the maxima found
+                // and the weights taken again where a group's sum shows that one could leave F16's range
+                // - by the rows that need it: no row's result depends on its neighbours'
+                bool     need = m == -INFINITY || R == -INFINITY, full = __any_sync(0xffffffffu, need), fresh = false;
+                float    grow = 1.0f, lsum;
+                uint32_t pk[KE_N / 2], pl[PP == 2 ? KE_N / 2 : 1];
+#pragma unroll 1
+                for (;;) {
+                    uint32_t sr[KE_N];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float a = e < 16 ? a0 : a1;
-                        float       x, y;
-                        f2unpack(fmul2(f2pack(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), f2pack(a, a)), x, y);
-                        sr[e] = __float_as_uint(x), sr[e + 1] = __float_as_uint(y);
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld32(s_col + (uint32_t) (c * 32), &sr[c * 32]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        tmem_ld_wait_tie(&sr[c * 32]);
+                    }
+                    if (!CAP && !plain) {
+#pragma unroll
+                        for (int e = 0; e < KE_N; e++) {
+                            sr[e] = __float_as_uint(__uint_as_float(sr[e]) * (factor * sc[e >> 4].x));
+                        }
                     }
                     if (!whole) {
-                        const int l0 = sc[2 * c].w != 0.0f ? left - 32 * c : 0, l1 = sc[2 * c + 1].w != 0.0f ? left - 32 * c : 0;
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            sr[e] = e < (e < 16 ? l0 : l1) ? sr[e] : 0xff800000u;
+                        for (int g = 0; g < 8; g++) {
+                            const int lg = sc[g].w != 0.0f ? left : 0;
+#pragma unroll
+                            for (int e = 16 * g; e < 16 * g + 16; e++) {
+                                sr[e] = e < lg ? sr[e] : 0xff800000u;
+                            }
                         }
                     }
-                };
-                // Rolled loops over the columns: unrolled, this is 16 KB of code that each warp streams for each tile.
-                // First the row's largest s, and the largest s + e over pages with a value scale
-                float top = -INFINITY, rtop = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    uint32_t sr[32];
-                    scores(c, sr);
+                    if (full) {  // the row's largest s, and the largest s + e over pages with a value scale
+                        float top = m, rtop = R;
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float4 q = sc[2 * c + g];
-                        float        a = __uint_as_float(sr[16 * g]), b = __uint_as_float(sr[16 * g + 1]);
+                        for (int g = 0; g < 8; g++) {
+                            float a = __uint_as_float(sr[16 * g]), b = __uint_as_float(sr[16 * g + 1]);
 #pragma unroll
-                        for (int e = 16 * g + 2; e < 16 * g + 14; e += 4) {
-                            a = fmax3(a, __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
-                            b = fmax3(b, __uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3]));
+                            for (int e = 16 * g + 2; e < 16 * g + 14; e += 4) {
+                                a = fmax3(a, __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
+                                b = fmax3(b, __uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3]));
+                            }
+                            a    = fmaxf(fmax3(a, __uint_as_float(sr[16 * g + 14]), __uint_as_float(sr[16 * g + 15])), b);
+                            a    = plain ? a * (factor * sc[g].x) : a;
+                            top  = fmaxf(top, a);
+                            rtop = sc[g].y != 0.0f ? fmaxf(rtop, a + sc[g].z) : rtop;
                         }
-                        a    = fmaxf(fmax3(a, __uint_as_float(sr[16 * g + 14]), __uint_as_float(sr[16 * g + 15])), b);
-                        top  = fmaxf(top, a);
-                        rtop = q.y != 0.0f ? fmaxf(rtop, a + q.z) : rtop;
+                        if (need) {
+                            l *= m == top ? 1.0f : ex2(m - top);
+                            grow = R == rtop ? 1.0f : ex2(R - rtop);
+                            m = top, R = rtop, fresh = true;
+                        }
                     }
-                }
-                float grow = 1.0f;
-                if (top > m + 8.0f) {
-                    l *= ex2(m - top);
-                    m = top;
-                }
-                if (rtop > R + 4.0f) {
-                    grow = ex2(R - rtop);
-                    R    = rtop;
-                }
-                if (!TWO) {
-                    grows[(j & 3) * KE_M + r] = grow;
-                    dn_mbar_arrive(&bar[KB_GROW + (j & 3)]);
-                }
-                const float    ms = m == -INFINITY ? 0.0f : m, base = ms - (R == -INFINITY ? 0.0f : R) + KE_OFF;
-                const uint64_t nm = f2pack(-ms, -ms);
-                uint64_t       acc0 = 0ull, acc1 = 0ull;
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    uint32_t sr[32], pk[16], pl[PP == 2 ? 16 : 1];
-                    scores(c, sr);
+                    const float    ms = m == -INFINITY ? 0.0f : m, base = ms - (R == -INFINITY ? 0.0f : R) + KE_OFF;
+                    const uint64_t nm = f2pack(-ms, -ms);
+                    bool           high = false;
+                    lsum                = 0.0f;
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float4   q  = sc[2 * c + g];
-                        const float    f  = ex2(fminf(base + q.z, 90.0f)) * q.y;
-                        const uint64_t f2 = f2pack(f, f);
+                    for (int g = 0; g < 8; g++) {
+                        const float4   q  = sc[g];
+                        const float    f  = ex2(fminf(base + q.z, 90.0f)) * q.y, a = plain ? factor * q.x : 1.0f;
+                        const uint64_t f2 = f2pack(f, f), a2 = f2pack(a, a);
+                        uint64_t       acc = 0ull;
 #pragma unroll
                         for (int i = 8 * g; i < 8 * g + 8; i++) {
-                            float x, y;
-                            f2unpack(fadd2(f2pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), nm), x, y);
-                            const uint64_t w2 = f2pack(ex2(x), ex2(y));
-                            if (i & 1) {
-                                acc1 = fadd2(acc1, w2);
+                            const uint64_t x2 = ffma2(f2pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), a2, nm);
+                            uint64_t       w2;
+                            if (PP == 1 && (i & 7) < KE_EMU) {
+                                w2 = exp2_poly2(x2);
                             } else {
-                                acc0 = fadd2(acc0, w2);
+                                float x, y;
+                                f2unpack(x2, x, y);
+                                w2 = f2pack(ex2(x), ex2(y));
                             }
+                            acc = fadd2(acc, w2);
                             const uint64_t p2 = fmul2(w2, f2);
+                            float          x, y;
                             f2unpack(p2, x, y);
                             pk[i] = ke_pack(x, y);
                             if (PP == 2) {
                                 const float2 b = h2_to_f2(pk[i]);
                                 f2unpack(ffma2(f2pack(b.x, b.y), f2pack(-1.0f, -1.0f), p2), x, y);
-                                pl[PP == 2 ? i : 0] = ke_pack(x, y);
+                                pl[i] = ke_pack(x, y);
                             }
                         }
+                        float x, y;
+                        f2unpack(acc, x, y);
+                        x += y;
+                        lsum += x;
+                        // the sum bounds every weight of the group; NaN and infinities fail the comparison below
+                        high |= !(x * fabsf(f) <= 32768.0f);
                     }
-                    ke_tmem_st16(s_col + (uint32_t) (c * 32), pk);
-                    if (PP == 2) {
-                        ke_tmem_st16(s_col + (uint32_t) (c * 32 + 16), reinterpret_cast<const uint32_t (&)[16]>(pl));
+                    need = high && !fresh;
+                    if (!__any_sync(0xffffffffu, need)) {
+                        break;
                     }
+                    full = true;
                 }
-                {
-                    float x, y;
-                    f2unpack(fadd2(acc0, acc1), x, y);
-                    l += x + y;
+                l += lsum;
+                if (!TWO) {
+                    grows[(j & 3) * KE_M + r] = grow;
+                    dn_mbar_arrive(&bar[KB_GROW + (j & 3)]);
+                }
+                tmem_st32(s_col, &pk[0]);
+                tmem_st32(s_col + 32, &pk[32]);
+                if (PP == 2) {
+                    tmem_st32(s_col + 64, &pl[0]);
+                    tmem_st32(s_col + 96, &pl[PP == 2 ? 32 : 0]);
                 }
                 // PV(j - 1) is complete: QK(j) was issued after it
                 if (TWO && j > 0 && __any_sync(0xffffffffu, grow != 1.0f)) {
