@@ -462,7 +462,8 @@ MM3FA_API int mm3fa_ipc_close(void * dev_ptr);
  * 8-bit paged KV cache.  K and V are held as int8 codes in pages of page_tokens tokens, with one F32
  * scale for each (layer, page, kv head) of K and of V: value = code * scale.
  *   k, v               int8 [n_layers][n_pages][n_head_kv][page_tokens][head_dim], 16-byte aligned
- *   k_scale, v_scale   F32  [n_layers][n_pages][n_head_kv]
+ *   k_scale, v_scale   F32  [n_layers][n_pages][n_head_kv] (append: finite and not negative where a page
+ *                      holds earlier tokens)
  * head_dim 64, 128 or 256; page_tokens 16, 32, 64 or 128.  A sequence's tokens [P*j, P*j + P) are in the
  * page that entry j of its table row names, the same page in every layer; an entry outside
  * [0, n_pages) names none: its keys are absent from the attention, its rows are neither stored nor
@@ -518,15 +519,16 @@ MM3FA_API size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_t
  * dst = softmax(scale * q k^T [softcap]) v over each sequence's pages of one layer.
  *   q      F32, F16 or BF16 [D, n_q, n_head, n_seq], any strides along dims 1 to 3; query head h reads
  *          kv head h / (n_head / n_head_kv)
- *   dst    [D, n_head, n_q, n_seq], F32 or q's type (an F32 result is computed to F32's precision: q and
- *          the softmax weights keep 22 bits; a 16-bit one with weights of 11 bits)
+ *   dst    [D, n_head, n_q, n_seq], F32 or q's type and not in q's memory.  An F32 result is computed to
+ *          F32's precision: q and the softmax weights keep 22 bits.  For a 16-bit one q keeps 11 bits or more
+ *          and the weights 22 (F16) or 11 (BF16)
  *   kv_len device int32 [n_seq]: tokens that the cache holds, the query rows' own among them
  *   q_len  device int32 [n_seq] or NULL: rows of sequence s (NULL: n_q); rows from q_len[s] on are left
  *          as they were
  *   causal row i sees keys [0, kv_len - (q_len - 1 - i)); otherwise every row sees [0, kv_len)
  *   logit_softcap  0 disables; otherwise s <- softcap * tanh(s / softcap)
- *   workspace      zero-filled once after allocation, 16-byte aligned; reused and replayed like
- *                  mm3fa_flash_attn_ext's, one per stream
+ *   workspace      zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this
+ *                  function alone, of any shapes and caches that it is large enough for
  * A row that sees no key becomes zeros.
  */
 MM3FA_API int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, const mm3fa_kv8_table * table,
@@ -534,7 +536,7 @@ MM3FA_API int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_ten
                              int causal, mm3fa_tensor * dst, void * workspace, size_t workspace_bytes, void * stream);
 
 /* Bytes of device workspace the page operations below need for n_seq sequences (0: a cache that they
- * would refuse).  Zero-fill it once; one per stream. */
+ * would refuse).  Zero-fill it once; one per stream.  A table's n_seq * max_pages stays below 2^31. */
 MM3FA_API size_t mm3fa_kv8_pages_workspace(const mm3fa_kv8 * cache, int n_seq);
 
 /*

@@ -178,7 +178,8 @@ cudaError_t launch_kv8_append(const Kv8StoreParams & p, cudaStream_t stream);
 cudaError_t launch_kv8_read(const Kv8StoreParams & p, cudaStream_t stream);
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p, int sms, cudaStream_t stream);
 cudaError_t launch_kv8_dense(const Kv8AttnParams & p, cudaStream_t stream);
-size_t      kv8_attn_workspace_bytes(int D, int n_q, int ratio, int n_head_kv, int n_seq, int sms);
+int         kv8_dense_tile(const Kv8AttnParams & p);  // rows of a CTA
+size_t      kv8_attn_workspace_bytes(int D, int n_q, int ratio, int sms);
 cudaError_t launch_kv8_fork(const Kv8PlanParams & p, const Kv8PoolCopy & c, int sms, cudaStream_t stream);
 cudaError_t launch_kv8_compact(const Kv8PlanParams & p, const Kv8PoolCopy & c, int sms, cudaStream_t stream);
 cudaError_t launch_kv8_reserve(const Kv8PlanParams & p, cudaStream_t stream);

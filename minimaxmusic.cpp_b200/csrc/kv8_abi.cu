@@ -173,7 +173,11 @@ size_t pages_workspace(const mm3fa_kv8 * c, int64_t n_seq) {
 }
 
 // The workspace's parts; MM3FA_ERR_WORKSPACE where it is missing, too small or not 4-byte aligned.
-int plan_workspace(const mm3fa_kv8 * c, int n_seq, void * ws, size_t bytes, Kv8PlanParams & p) {
+int plan_workspace(const mm3fa_kv8 * c, const mm3fa_kv8_table * t, void * ws, size_t bytes, Kv8PlanParams & p) {
+    const int n_seq = t->n_seq;
+    if ((int64_t) n_seq * t->max_pages > INT32_MAX) {  // the pages that a call needs are counted in 32 bits
+        return MM3FA_ERR_UNSUPPORTED;
+    }
     if (!ws || bytes < pages_workspace(c, n_seq) || !aligned_to(ws, 4)) {
         return MM3FA_ERR_WORKSPACE;
     }
@@ -279,7 +283,7 @@ size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q,
         return 0;
     }
     return kv8_attn_workspace_bytes(cache->head_dim, (int) q->ne[1], (int) (q->ne[2] / cache->n_head_kv),
-                                    cache->n_head_kv, table->n_seq, host_sm_count());
+                                    host_sm_count());
 }
 
 int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, const mm3fa_kv8_table * table,
@@ -355,7 +359,7 @@ int mm3fa_kv8_reserve(const mm3fa_kv8 * cache, mm3fa_kv8_table * table, int32_t 
     }
     Kv8PlanParams p{};
     if (st == MM3FA_OK) {
-        st = plan_workspace(cache, table->n_seq, workspace, workspace_bytes, p);
+        st = plan_workspace(cache, table, workspace, workspace_bytes, p);
     }
     if (st != MM3FA_OK) {
         return st;
@@ -387,7 +391,7 @@ int mm3fa_kv8_fork(const mm3fa_kv8 * cache, const mm3fa_kv8_table * table, const
     }
     Kv8PlanParams p{};
     if (st == MM3FA_OK) {
-        st = plan_workspace(cache, table->n_seq, workspace, workspace_bytes, p);
+        st = plan_workspace(cache, table, workspace, workspace_bytes, p);
     }
     if (st != MM3FA_OK) {
         return st;
@@ -418,7 +422,7 @@ int mm3fa_kv8_compact(const mm3fa_kv8 * cache, const mm3fa_kv8_table * table, co
     int           st = check_tables_out(cache, table, refs, table_out, refs_out);
     Kv8PlanParams p{};
     if (st == MM3FA_OK) {
-        st = plan_workspace(cache, table->n_seq, workspace, workspace_bytes, p);
+        st = plan_workspace(cache, table, workspace, workspace_bytes, p);
     }
     if (st != MM3FA_OK) {
         return st;

@@ -15,7 +15,8 @@
 // Work.  A unit is (sequence, kv head, 16 query rows): rows of all query heads of the group share the
 // cache's bytes.  A unit's keys come in blocks of 32.  Every CTA finds its work from the lengths on the
 // device (a graph replays with others), by one of three cuts:
-//   whole  no unit above KD_WHOLE blocks: whole units, an equal number for each CTA;
+//   whole  no unit above KD_WHOLE blocks, or units so much alike that no cut is worth a crossing: whole units, an
+//          equal number for each CTA;
 //   split  few units: each in parts of up to W blocks, one part per CTA, W so that all parts run at once;
 //   flat   otherwise: all units' blocks in a row, in equal contiguous ranges, one per CTA.
 // Flat ranges are even, but a CTA that crosses from one unit to the next pays a second start and end, about
@@ -24,6 +25,13 @@
 // In a CTA each of the four warps takes every fourth block of a unit through its own ring of cp.async
 // stages - no barrier between warps - and keeps its own softmax state; the four are joined in shared
 // memory, and the parts of a unit by the last CTA to arrive, in their order (no result depends on timing).
+//
+// Bound.  One token of 48 sequences of 1 to 10240 tokens (32 heads on 8, D = 128, BF16): the cache's bytes, 105 us
+// or 74 % of the copy bandwidth of 6.54 TB/s; 110 of 2000 each, 90 us and 77 %.  For two of 8192 (19 us, 33.6 MB, floor
+// 5.1 us) the start - lengths, table, first pages, one after another - and the join of the parts take 8 us, as
+// in an empty call, and each CTA's 20 blocks the rest.  From 16 rows on (NT = 2) it is issue: 0.05 us per
+// 32-key block and CTA, four times the load's.  Two stages for three CTAs of an SM against three stages for two, D = 128:
+// 105 us against 122 for the 48 sequences, 19.3 against 18.6 for the two.
 #include "kv8.cuh"
 
 namespace mm3fa {
@@ -33,10 +41,13 @@ constexpr int KD_THREADS = 32 * KD_WARPS;
 constexpr int KD_BLOCK   = 32;     // keys per block
 constexpr int KD_ROWS    = 16;     // query rows per unit
 constexpr int KD_OFF     = 12;     // P is held times 2^12: F16 keeps 11 bits down to 2^-26 of the largest weight
+// 2 sequences of 300: 8.0 us whole, 8.7 in parts; 100 of 400: 26.5 whole, 33 flat.
 constexpr int KD_WHOLE   = 16;
-constexpr int KD_PART    = 4;      // blocks of a part, at least
+// Blocks of a part, at least: 4, 8, 16 take 11.0, 11.2, 13.9 us for one sequence of 2000.
+constexpr int KD_PART    = 4;
+// What a crossing costs, in blocks.  0, 8, 32: 24.4, 19.2, 19.3 us for 2 sequences of 8192 (0: flat), 37.3, 37.4, 35.8
+// for 16 of 4096 (32: parts).  Whole against flat: 26.6 against 33.2 us for 50 of 1000, 89.9 against 91.6 for 110 of 2000.
 constexpr int KD_CROSS   = 32;
-constexpr int KD_DENSE   = 64;     // rows of a kv head from which the kernel for many rows takes over (D <= 128)
 
 template <int D, int NT, bool HP>
 struct KdSmem {
@@ -210,6 +221,8 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
             cut.w = KD_WHOLE;
         } else if (spare > 0 && (int64_t) total * all <= (int64_t) KD_CROSS * ctas * spare) {
             cut.w = max(KD_PART, (total + spare - 1) / spare);
+        } else if ((int64_t) ((all + ctas - 1) / ctas) * top * ctas <= total + (int64_t) KD_CROSS * ctas) {
+            cut.w = top;
         }
         sum *= units;
         if (cut.w) {
@@ -915,29 +928,44 @@ cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStrea
 }
 
 // CTAs that an SM holds at once: what KdSmem plans for
+constexpr int KD_CTAS_MOST = KdSmem<64, 1, true>::CTAS;
+
+size_t counter_bytes(int sms) {
+    return ((size_t) sms * KD_CTAS_MOST * 4 + 255) / 256 * 256;
+}
+
 int ctas_per_sm(int D, int rows) {
     return rows <= 8 ? (D == 64 ? KdSmem<64, 1, true>::CTAS : D == 128 ? KdSmem<128, 1, true>::CTAS : KdSmem<256, 1, true>::CTAS)
                      : (D == 64 ? KdSmem<64, 2, true>::CTAS : D == 128 ? KdSmem<128, 2, true>::CTAS : KdSmem<256, 2, true>::CTAS);
 }
 
+// The kernel for many rows (D <= 128) takes a call that gives every SM two units of this kernel, and every SM of each
+// wave of its own CTAs, which do not split a sequence's keys.
+bool many_rows(const Kv8AttnParams & p, int sms) {
+    const int64_t heads = (int64_t) p.t.n_seq * p.c.n_head_kv, rows = (int64_t) p.ratio * p.n_q;
+    const int     tile  = kv8_dense_tile(p);
+    const int64_t waves = (heads * ((rows + tile - 1) / tile) + sms - 1) / sms;
+    return p.c.D <= 128 && heads * ((rows + KD_ROWS - 1) / KD_ROWS) >= 2 * waves * sms;
+}
+
 }  // namespace
 
-// Counters (one per CTA) and two partial results per CTA, whatever the lengths are.
-size_t kv8_attn_workspace_bytes(int D, int n_q, int ratio, int n_head_kv, int n_seq, int sms) {
+// Counters (one per CTA, in a place of one size for every shape: a workspace serves them all, and no shape's
+// partial results may lie on another's counters) and two partial results per CTA, whatever the lengths are.
+size_t kv8_attn_workspace_bytes(int D, int n_q, int ratio, int sms) {
     const size_t ctas = (size_t) sms * (size_t) ctas_per_sm(D, ratio * n_q);
-    (void) n_head_kv, (void) n_seq;
-    return WS_STATUS_BYTES + (ctas * 4 + 255) / 256 * 256 + 2 * ctas * KD_ROWS * (size_t) (D + 4) * 4;
+    return WS_STATUS_BYTES + counter_bytes(sms) + 2 * ctas * KD_ROWS * (size_t) (D + 4) * 4;
 }
 
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p0, int sms, cudaStream_t stream) {
     Kv8AttnParams p    = p0;
     p.ratio_inv        = p.ratio == 1 ? 0u : (uint32_t) ((1ull << 32) / (uint64_t) p.ratio + 1);
-    if (p.c.D <= 128 && p.ratio * p.n_q >= KD_DENSE) {
+    if (many_rows(p, sms)) {
         return launch_kv8_dense(p, stream);
     }
     const int     most = sms * ctas_per_sm(p.c.D, p.ratio * p.n_q);
     p.counters = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.status) + WS_STATUS_BYTES);
-    p.part     = reinterpret_cast<float *>(reinterpret_cast<char *>(p.counters) + ((size_t) most * 4 + 255) / 256 * 256);
+    p.part     = reinterpret_cast<float *>(reinterpret_cast<char *>(p.counters) + counter_bytes(sms));
     const int     all = p.ratio * p.n_q, rows = all < KD_ROWS ? all : KD_ROWS;
     const int64_t units  = (int64_t) p.t.n_seq * p.c.n_head_kv * ((all + KD_ROWS - 1) / KD_ROWS);
     const int64_t blocks = units * (((int64_t) p.t.max_pages * p.c.P + KD_BLOCK - 1) / KD_BLOCK);  // at most

@@ -25,12 +25,15 @@
 //
 // Softmax.  s = S * (row factor * key scale of the column's page), in log2 units; weights 2^(s - m); the
 // value scale b = f 2^e of a page is multiplied into them, P = 2^(s - m) * 2^(m + e - R + KE_OFF) * f, so
-// that O is in units of 2^(R - KE_OFF).  m and R (the largest s + e of any page) are lazy: they follow only
-// when they would grow by more than 8 and 4, which F16's range allows, and O is multiplied then.
+// that O is in units of 2^(R - KE_OFF).  m and R (the largest s + e of any page) are lazy: a tile's weights are
+// taken with those of the tiles before, in one pass, and again with its own only by the rows where the weights of
+// a group of 16 columns, times f, sum to more than 2^15 (F16 holds 2^16) or the sum leaves F32's range; O is multiplied
+// then.  Finding the maxima first, in a pass of their own: 396 us for the 2048 rows below, 331 so.
 //
-// Bound: for BF16 the exponentials (16 a cycle and SM: 2048 cycles for 256 rows of a tile; 3 of 8 pairs go by polynomial)
-// and the issue of softmax and conversions, beside 1024 cycles of products at D = 128; for F32 the products (2048
-// cycles for 128 rows of a tile), for F16 those (1536) and the exponentials alike.
+// Bound: for BF16 the exponentials (16 a cycle and SM: 2048 cycles for 256 rows of a tile, of which the polynomial
+// takes 1 in 8: 331 us against 399 without it for 2048 rows over 8192 keys, 32 heads), as many cycles of products
+// at D = 128, and the issue of the conversions (about 470 slots a scheduler), which overlap in part: a tile
+// pair takes 5100 cycles.  For F32 the products (2048 cycles for 128 rows of a tile) beside a softmax of 3000.
 #include "kv8.cuh"
 #include "tc_sm100.cuh"
 
@@ -41,14 +44,15 @@ constexpr int KE_M       = 128;  // rows per Q tile
 constexpr int KE_N       = 128;  // keys per tile
 constexpr int KE_TMEM    = 512;
 constexpr int KE_EMU     = 1;    // of every 8 pairs of weights, those by polynomial where P is rounded to F16 anyway
-constexpr int KE_OFF     = 8;    // P is held times 2^8: 2^14 at most with the lazy maxima
+constexpr int KE_OFF     = 8;    // P is held times 2^8 at the maxima: a tile's may be 2^7 above those taken before
 constexpr int KE_REGS_LAUNCH  = 128;  // 65536 / 512
 constexpr int KE_REGS_SOFTMAX = 192;  // 2 x 192 + 96 + 32 = 4 x 128
 constexpr int KE_REGS_CONVERT = 96;
 constexpr int KE_REGS_ISSUE   = 32;
 static_assert(2 * KE_REGS_SOFTMAX + KE_REGS_CONVERT + KE_REGS_ISSUE <= 4 * KE_REGS_LAUNCH, "more registers than the launch has");
 
-constexpr int KE_LONG  = 65536;  // tokens
+// Tokens up to which the truncated sums in TMEM (7e-7 of the result a tile of 128) stay a fifth of BF16's half step.
+constexpr int KE_LONG = 65536;
 
 template <int D, int QP, bool TWO>
 struct KeSmem {
@@ -674,7 +678,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 // and the weights taken again where a group's sum shows that one could leave F16's range
                 // - by the rows that need it: no row's result depends on its neighbours'
                 bool     need = m == -INFINITY || R == -INFINITY, full = __any_sync(0xffffffffu, need), fresh = false;
-                float    grow = 1.0f, lsum;
+                float    grow = 1.0f, lsum, ms;
                 uint32_t pk[KE_N / 2], pl[PP == 2 ? KE_N / 2 : 1];
 #pragma unroll 1
                 for (;;) {
@@ -724,7 +728,8 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                             m = top, R = rtop, fresh = true;
                         }
                     }
-                    const float    ms = m == -INFINITY ? 0.0f : m, base = ms - (R == -INFINITY ? 0.0f : R) + KE_OFF;
+                    ms = m == -INFINITY ? 0.0f : m;
+                    const float    base = ms - (R == -INFINITY ? 0.0f : R) + KE_OFF;
                     const uint64_t nm = f2pack(-ms, -ms);
                     bool           high = false;
                     lsum                = 0.0f;
@@ -738,16 +743,17 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                         for (int i = 8 * g; i < 8 * g + 8; i++) {
                             const uint64_t x2 = ffma2(f2pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), a2, nm);
                             uint64_t       w2;
+                            float          x, y;
                             if (PP == 1 && (i & 7) < KE_EMU) {
-                                w2 = exp2_poly2(x2);
+                                // over a stale maximum x has no bound, and the polynomial's exponent field would wrap
+                                f2unpack(x2, x, y);
+                                w2 = exp2_poly2(f2pack(fminf(x, 127.0f), fminf(y, 127.0f)));
                             } else {
-                                float x, y;
                                 f2unpack(x2, x, y);
                                 w2 = f2pack(ex2(x), ex2(y));
                             }
                             acc = fadd2(acc, w2);
                             const uint64_t p2 = fmul2(w2, f2);
-                            float          x, y;
                             f2unpack(p2, x, y);
                             pk[i] = ke_pack(x, y);
                             if (PP == 2) {
@@ -763,13 +769,14 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                         // the sum bounds every weight of the group; NaN and infinities fail the comparison below
                         high |= !(x * fabsf(f) <= 32768.0f);
                     }
-                    need = high && !fresh;
+                    // (and where it leaves F32's: value scales near 2^-126 would let a sum grow that far with P still small)
+                    need = (high || !(lsum <= 0x1p100f)) && !fresh;
                     if (!__any_sync(0xffffffffu, need)) {
                         break;
                     }
                     full = true;
                 }
-                l += lsum;
+                l += lsum + (ms - ms);  // a score of +inf: NaN
                 if (!TWO) {
                     grows[(j & 3) * KE_M + r] = grow;
                     dn_mbar_arrive(&bar[KB_GROW + (j & 3)]);
@@ -881,10 +888,14 @@ cudaError_t launch_d(const Kv8AttnParams & p, cudaStream_t stream) {
     if (p.o.type == KV_F16) {
         return launch_one<D, 1, 2, false, CAP>(p, stream);
     }
-    return (int64_t) p.t.max_pages * p.c.P > KE_LONG ? launch_one<D, 1, 1, false, CAP>(p, stream) : launch_one<D, 1, 1, true, CAP>(p, stream);
+    return kv8_dense_tile(p) == KE_M ? launch_one<D, 1, 1, false, CAP>(p, stream) : launch_one<D, 1, 1, true, CAP>(p, stream);
 }
 
 }  // namespace
+
+int kv8_dense_tile(const Kv8AttnParams & p) {
+    return p.o.type == KV_BF16 && (int64_t) p.t.max_pages * p.c.P <= KE_LONG ? 2 * KE_M : KE_M;
+}
 
 cudaError_t launch_kv8_dense(const Kv8AttnParams & p, cudaStream_t stream) {
     if (p.c.D == 64) {

@@ -142,10 +142,14 @@ class Kv8Cache:
             raise MM3FAError(ERR_STRIDE, "Kv8Cache: " + what)
         return t.data_ptr()
 
-    def _stream(self, stream):
-        if self._dev < 0:
-            return 0
-        return self._torch._C._cuda_getCurrentRawStream(self._dev) if stream is None else stream.cuda_stream
+    def _stream(self):
+        return 0 if self._dev < 0 else self._torch._C._cuda_getCurrentRawStream(self._dev)
+
+    def _on(self, stream):
+        """A context in which `stream` is the current one."""
+        if stream.device_index != self._dev:
+            raise ValueError(f"Kv8Cache: a stream of device {stream.device_index}, the cache is on {self.device}")
+        return self._torch.cuda.stream(stream)
 
     def _call(self, name, *args):
         """A library call with the cache's device current; its result."""
@@ -185,18 +189,24 @@ class Kv8Cache:
     def append(self, layer, k_new, v_new, table, start, n_new=None, stream=None):
         """Stores the rows k_new, v_new (N, n_head_kv, T, D), the first n_new[s] (default: T) of sequence s, behind
         its first start[s] tokens.  The pages' scales grow where the rows need it."""
+        if stream is not None:
+            with self._on(stream):
+                return self.append(layer, k_new, v_new, table, start, n_new)
         n = table.shape[0]
         self._run("append", self._desc, layer, self._rows(k_new), self._rows(v_new), self._table(table),
                    self._ints(start, n, "start"), None if n_new is None else self._ints(n_new, n, "n_new"),
-                   self._stream(stream))
+                   self._stream())
 
     def read(self, layer, k_out, v_out, table, start, n=None, stream=None):
         """Values of tokens start[s] .. start[s] + n[s] (default: T) of each sequence into the first rows of
         k_out, v_out (N, n_head_kv, T, D)."""
+        if stream is not None:
+            with self._on(stream):
+                return self.read(layer, k_out, v_out, table, start, n)
         ns = table.shape[0]
         self._run("read", self._desc, layer, self._table(table), self._ints(start, ns, "start"),
                    None if n is None else self._ints(n, ns, "n"), self._rows(k_out), self._rows(v_out),
-                   self._stream(stream))
+                   self._stream())
 
     def attend(self, layer, q, table, kv_len, scale, out=None, q_len=None, causal=True, logit_softcap=0.0, ws=None,
                stream=None):
@@ -204,8 +214,11 @@ class Kv8Cache:
         sequence; causal: the rows are the last tokens.  out: (N, n_q, n_head, D), F32 or q's type; made in
         q's type when not given, with zeros in the rows behind q_len.  ws: a zero-filled uint8 tensor
         instead of the cache's own workspace of the stream, for graphs that may run at the same time."""
+        if stream is not None:  # what is allocated here belongs to that stream too
+            with self._on(stream):
+                return self.attend(layer, q, table, kv_len, scale, out, q_len, causal, logit_softcap, ws)
         n = table.shape[0]
-        qd, td, st = self._rows(q), self._table(table), self._stream(stream)
+        qd, td, st = self._rows(q), self._table(table), self._stream()
         if out is None:
             make = self._torch.empty if q_len is None else self._torch.zeros
             out = make((q.shape[0], q.shape[2], q.shape[1], q.shape[3]), dtype=q.dtype, device=q.device)
@@ -234,14 +247,20 @@ class Kv8Cache:
 
     def reserve(self, table, refs, n_tok, stream=None):
         """Gives each sequence's row of `table` the pages for n_tok[s] tokens (in place)."""
-        st, n = self._stream(stream), table.shape[0]
+        if stream is not None:
+            with self._on(stream):
+                return self.reserve(table, refs, n_tok)
+        st, n = self._stream(), table.shape[0]
         self._run("reserve", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
                    self._ints(n_tok, n, "n_tok"), *self._pages_ws(n, st), st)
 
     def fork(self, src, dst, table, kv_len, refs, table_out, kv_len_out, refs_out, deep=False, stream=None):
         """Sequence dst[i] becomes a copy of sequence src[i] (-1, or src None: empty); full pages are shared unless
         `deep`.  The results go to the *_out tensors, which may not overlap the others."""
-        st, n = self._stream(stream), table.shape[0]
+        if stream is not None:
+            with self._on(stream):
+                return self.fork(src, dst, table, kv_len, refs, table_out, kv_len_out, refs_out, deep)
+        st, n = self._stream(), table.shape[0]
         pairs = dst.shape[0]
         self._run("fork", self._desc, self._table(table), self._ints(kv_len, n, "kv_len"),
                    self._ints(refs, self.n_pages, "refs"), None if src is None else self._ints(src, pairs, "src"),
@@ -255,14 +274,20 @@ class Kv8Cache:
 
     def compact(self, table, refs, table_out, refs_out, stream=None):
         """Moves the live pages to the front of the pool; the results go to the *_out tensors."""
-        st, n = self._stream(stream), table.shape[0]
+        if stream is not None:
+            with self._on(stream):
+                return self.compact(table, refs, table_out, refs_out)
+        st, n = self._stream(), table.shape[0]
         self._run("compact", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
                    self._table(table_out), self._ints(refs_out, self.n_pages, "refs_out"), *self._pages_ws(n, st), st)
 
     def check(self, stream=None):
         """Synchronises the stream and raises MM3FAError where a page operation on it found too few free pages
         (ERR_PAGES) or a bounded device wait of an attention expired (ERR_TIMEOUT)."""
-        st = self._stream(stream)
+        if stream is not None:
+            with self._on(stream):
+                return self.check()
+        st = self._stream()
         for op in ("pages", "attn"):
             buf = self._ws.get((op, st))
             if buf is not None:

@@ -1,5 +1,7 @@
 """What the 8-bit paged cache refuses, on host tensors: every check of the C ABI and of the Python class runs
 before anything is launched (without a device an accepted call ends with ERR_DEVICE)."""
+import types
+
 import pytest
 import torch
 
@@ -128,7 +130,7 @@ def test_page_operation_refusals():
     assert status(c.reserve, s.table, s.refs, s.len) == mm3fa.ERR_DEVICE
     assert status(c.reserve, s.table, s.refs, s.len[:1]) == mm3fa.ERR_SHAPE
     # a workspace that is too small, an unknown flag
-    g, ws = kv8._calls()["fork"], torch.zeros(1 << 16, dtype=torch.uint8)
+    g, ws = kv8._calls()["fork"], torch.zeros(1 << 20, dtype=torch.uint8)
     args = lambda flags, nbytes: g(c._desc, c._table(s.table), s.len.data_ptr(), s.refs.data_ptr(), pair[0].data_ptr(),
                                    pair[1].data_ptr(), 1, flags, c._table(t2), l2.data_ptr(), r2.data_ptr(),
                                    ws.data_ptr(), nbytes, None)
@@ -136,6 +138,29 @@ def test_page_operation_refusals():
     assert args(0, need) == mm3fa.ERR_DEVICE
     assert args(0, need - 1) == mm3fa.ERR_WORKSPACE
     assert args(2, need) == mm3fa.ERR_UNSUPPORTED
+
+    # tables whose entries are not counted in 32 bits
+    big = lambda pages: kv8._PACK_TABLE(s.table.data_ptr(), pages, pages, 65535)
+    other = lambda pages: kv8._PACK_TABLE(t2.data_ptr() + (1 << 40), pages, pages, 65535)
+    need = c._call("pages_workspace", c._desc, 65535)
+    for pages, want in ((32768, mm3fa.ERR_DEVICE), (32769, mm3fa.ERR_UNSUPPORTED)):
+        got = c._call("reserve", c._desc, big(pages), s.refs.data_ptr(), s.len.data_ptr(), ws.data_ptr(), need, None)
+        assert got == want
+        got = c._call("compact", c._desc, big(pages), s.refs.data_ptr(), other(pages), r2.data_ptr(), ws.data_ptr(), need, None)
+        assert got == want
+
+
+@no_gpu
+def test_a_stream_of_another_device():
+    s = make()
+    c, x = s.cache(), torch.zeros(2, 2, 3, 64)
+    other = types.SimpleNamespace(device_index=0, cuda_stream=0)
+    with pytest.raises(ValueError):
+        c.append(0, x, x, s.table, s.len, stream=other)
+    with pytest.raises(ValueError):
+        c.attend(0, x, s.table, s.len, 1.0, stream=other)
+    with pytest.raises(ValueError):
+        c.check(other)
 
 
 def test_status_strings():

@@ -23,6 +23,21 @@ def ints(*v, dev="cuda"):
 
 # ---------------------------------------------------------------- attention
 
+def repeats(st, rows):
+    """How often a batch is repeated so that the kernel for many rows takes its `rows` rows per kv head (0: never): two
+    units of 16 rows for each SM, and each wave of CTAs of 128 rows."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    heads, units, tiles = st.N * st.Hkv, -(-rows // 16), -(-rows // 128)
+    return next((r for r in range(1, 400) if r * heads * units >= 2 * sms * -(-r * heads * tiles // sms)), 0) if st.D <= 128 else 0
+
+
+def many(st, rows):
+    """`st` with its sequences repeated where that brings the kernel for many rows."""
+    r = max(1, repeats(st, rows))
+    st.table, st.len, st.N = st.table.repeat(r, 1), st.len.repeat(r), st.N * r
+    return st
+
+
 def run_attend(st, H, n_q, dtype, out_dtype=None, q=None, q_len=None, causal=True, softcap=0.0, scale=None, layer=0,
                what=""):
     q = st.randn(st.N, n_q, H, st.D).to(dtype).transpose(1, 2) if q is None else q
@@ -37,6 +52,14 @@ def run_attend(st, H, n_q, dtype, out_dtype=None, q=None, q_len=None, causal=Tru
     assert torch.equal(first, out), f"{what}: two runs differ"
     ref, f32, p16 = R.attend(st, layer, q, scale, ql, causal, softcap, out=torch.full_like(out, 7.0).float())
     R.check_attend(out, ref, f32, p16, out.dtype, what)
+    reps = repeats(st, H // st.Hkv * n_q)
+    if reps > 1:  # the other kernel
+        both = torch.full_like(out, 7.0).repeat(reps, 1, 1, 1)
+        st_cache.attend(layer, q.repeat(reps, 1, 1, 1), st.table.repeat(reps, 1), st.len.repeat(reps), scale, out=both,
+                        q_len=None if ql is None else ql.repeat(reps), causal=causal, logit_softcap=softcap)
+        st_cache.check()
+        R.check_attend(both[:st.N], ref, f32, p16, out.dtype, what)
+        assert torch.equal(both, both[:st.N].repeat(reps, 1, 1, 1)), f"{what}: copies of a batch differ"
     return out
 
 
@@ -118,13 +141,13 @@ def test_attend_result_type(cuda_device, n_q):
 @pytest.mark.parametrize("n_q", [1, 3, 66])
 def test_attend_strides(cuda_device, n_q, dtype):
     """Queries at odd offsets and strides, results inside a larger buffer, a table that is a slice, layers."""
-    st = R.State([200, 99], 2, 64, 32, L=3, seed=10, device=cuda_device)
-    dt = DTYPES[dtype]
-    flat = st.randn(2 * 4 * n_q * 77 + 1).to(dt)
-    q = flat[1:].view(2, 4, n_q, 77)[..., 3:67]
-    big = torch.full((2, n_q + 2, 9, 65), 7.0, dtype=dt, device=cuda_device)
+    st = many(R.State([200, 99], 2, 64, 32, L=3, seed=10, device=cuda_device), 2 * n_q)
+    dt, n = DTYPES[dtype], st.N
+    flat = st.randn(n * 4 * n_q * 77 + 1).to(dt)
+    q = flat[1:].view(n, 4, n_q, 77)[..., 3:67]
+    big = torch.full((n, n_q + 2, 9, 65), 7.0, dtype=dt, device=cuda_device)
     out = big[:, 1:n_q + 1, 2:6, 1:]
-    wide = torch.full((2, st.table.shape[1] + 5), -7, dtype=I32, device=cuda_device)
+    wide = torch.full((n, st.table.shape[1] + 5), -7, dtype=I32, device=cuda_device)
     wide[:, 2:2 + st.table.shape[1]] = st.table
     table = wide[:, 2:2 + st.table.shape[1]]
     c = st.cache()
@@ -179,9 +202,9 @@ def test_attend_sharp_and_ordered_scores(cuda_device, n_q):
 
 @pytest.mark.parametrize("n_q", [1, 65])
 def test_attend_nan_stays_in_its_rows(cuda_device, n_q):
-    st = R.State([300, 37], 2, 64, 64, seed=14, device=cuda_device)
-    q = st.randn(2, 4, n_q, 64)
-    good = torch.empty(2, n_q, 4, 64, device=cuda_device)
+    st = many(R.State([300, 37], 2, 64, 64, seed=14, device=cuda_device), 2 * n_q)
+    q = st.randn(st.N, 4, n_q, 64)
+    good = torch.empty(st.N, n_q, 4, 64, device=cuda_device)
     st.cache().attend(0, q, st.table, st.len, 0.125, out=good)
     for bad in (float("nan"), float("inf")):
         q2, out = q.clone(), torch.empty_like(good)
@@ -208,6 +231,8 @@ def test_attend_rows_that_grow_beside_rows_that_start_late(cuda_device, dtype):
     q = q.to(dt)
     run_attend(st, 4, 130, dt, q=q, scale=1.0)
     run_attend(st, 4, 130, dt, q=q, scale=1.0, causal=False)
+    many(st, 4 * 130)
+    q = q.repeat(st.N // 2, 1, 1, 1)
     want = st.cache().attend(0, q, st.table, st.len, 1.0)
     q2 = q.clone()
     q2[0, :, 5::8] = float("nan")
@@ -215,6 +240,31 @@ def test_attend_rows_that_grow_beside_rows_that_start_late(cuda_device, dtype):
     assert got[0, 5::8].isnan().all()
     got[0, 5::8] = want[0, 5::8]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n_q", [1, 130])
+def test_attend_one_score_far_above_those_before(cuda_device, n_q, dtype):
+    """In a later block of keys a single key far above all before it (2^s up to 2^30000), at every place of a page."""
+    st = R.State([300], 1, 64, 16, seed=21, device=cuda_device)
+    st.ks.fill_(1.0)
+    st.k[..., 0] = 0
+    q = torch.zeros(1, 2, n_q, 64, device=cuda_device)
+    q[..., 1] = 0.01
+    for at in (160, 161, 162, 175, 271):
+        for jump in (1.0, 1.25, 2.0, 100.0):
+            st.k[0, int(st.table[0, at // 16]), 0, at % 16, 0] = 127
+            q[..., 0] = jump
+            run_attend(st, 2, n_q, DTYPES[dtype], q=q.to(DTYPES[dtype]), scale=1.0, causal=False, what=f"{at} {jump}")
+            st.k[..., 0] = 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_units_as_long_as_each_other(cuda_device, D):
+    """About as many units as CTAs, of more than a few blocks: whole units for each."""
+    for n in (50, 57, 110):
+        st = R.State([600 + 5 * i for i in range(n)], 8, D, 64, seed=n, device=cuda_device)
+        run_attend(st, 16, 1, torch.bfloat16)
 
 
 @pytest.mark.parametrize("N,H,Hkv,n_q", [(300, 4, 2, 1), (65, 2, 1, 40), (1, 64, 32, 1)])
@@ -233,11 +283,12 @@ def test_attend_long(cuda_device):
     run_attend(st, 8, 70, torch.float16)
 
 
-def test_attend_streams_and_graph(cuda_device):
+@pytest.mark.parametrize("n_q", [1, 130])
+def test_attend_streams_and_graph(cuda_device, n_q):
     """Two streams at once with a workspace each, then a graph that is replayed with other lengths and queries."""
     st = R.State([500, 1200], 4, 128, 64, seed=16, device=cuda_device)
     c = st.cache()
-    q = st.randn(2, 16, 1, 128)
+    q = st.randn(2, 16, n_q, 128)
     want = c.attend(0, q, st.table, st.len, 0.1).clone()
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -253,13 +304,94 @@ def test_attend_streams_and_graph(cuda_device):
         c.attend(0, q, st.table, st.len, 0.1, out=out)
     for lens in ((500, 1200), (1, 0), (333, 1199)):
         st.len.copy_(ints(*lens))
-        q.copy_(st.randn(2, 16, 1, 128))
+        q.copy_(st.randn(2, 16, n_q, 128))
         graph.replay()
         eager = c.attend(0, q, st.table, st.len, 0.1)
         torch.cuda.synchronize()
         assert torch.equal(eager, out)
         ref, f32, p16 = R.attend(st, 0, q, 0.1)
         R.check_attend(out, ref, f32, p16, torch.float32)
+
+
+def test_one_workspace_for_every_shape(cuda_device):
+    """Calls of different head dims and rows take turns with one workspace: the counters of one are not another's."""
+    cs = [R.State([9000, 7000], 8, D, 64, seed=D, device=cuda_device) for D in (128, 64, 256)]
+    shapes = [(st, n_q, dt) for st in cs for n_q in (1, 4, 2, 30) for dt in (torch.bfloat16, torch.float32)]
+    qs = [st.randn(2, 32, n_q, st.D).to(dt) for st, n_q, dt in shapes]
+    want = [st.cache().attend(0, q, st.table, st.len, 0.1) for (st, _, _), q in zip(shapes, qs)]
+    ws = torch.zeros(max(st.cache().attend_workspace(q, st.table) for (st, _, _), q in zip(shapes, qs)), dtype=torch.uint8,
+                     device=cuda_device)
+    order = torch.randperm(4 * len(shapes), generator=torch.Generator().manual_seed(1)).tolist()
+    for i in order:
+        i %= len(shapes)
+        st = shapes[i][0]
+        out = torch.full_like(want[i], 7.0)
+        st.cache().attend(0, qs[i], st.table, st.len, 0.1, out=out, ws=ws)
+        assert torch.equal(out, want[i]), shapes[i][1:]
+
+
+@pytest.mark.parametrize("n_q", [1, 70])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_attend_negative_and_zero_scales(cuda_device, n_q, scale):
+    """A softmax scale of 0 or below, and pages whose key or value scale is negative or 0."""
+    st = R.State([300, 90], 2, 128, 64, seed=18, device=cuda_device)
+    for dt in (torch.float32, torch.bfloat16):
+        run_attend(st, 8, n_q, dt, scale=scale)
+    st.ks[0, st.table[0, 1].long()] *= -1
+    st.ks[0, st.table[0, 2].long()] = 0
+    st.vs[0, st.table[0, 3].long()] *= -1
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        run_attend(st, 8, n_q, dt, scale=scale)
+        run_attend(st, 8, n_q, dt, scale=0.2)
+
+
+def test_on_a_given_stream(cuda_device):
+    """Calls on a stream that is not the current one: results and workspaces are made there."""
+    st = R.State([500, 1200], 4, 128, 64, room=[510, 1210], seed=19, device=cuda_device)
+    q, x = st.randn(2, 16, 1, 128), st.randn(2, 4, 1, 128)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    c = st.cache()
+    c.append(0, x, x, st.table, st.len, stream=side)
+    got = c.attend(0, q, st.table, st.len + 1, 0.1, stream=side)
+    side.synchronize()
+    c.check(side)
+    assert torch.equal(got, c.attend(0, q, st.table, st.len + 1, 0.1))
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """A pool of more than 2^31 codes (and scales far into it): the last pages give what a small pool gives."""
+    D, P, Hkv, n_pages = 128, 128, 8, 2 ** 31 // (128 * 128 * 8) + 40
+    small = R.State([300, 129], Hkv, D, P, room=[500, 300], seed=20, device=cuda_device)
+    k, v = (torch.zeros(1, n_pages, Hkv, P, D, dtype=torch.int8, device=cuda_device) for _ in range(2))
+    ks, vs = (torch.zeros(1, n_pages, Hkv, device=cuda_device) for _ in range(2))
+    off = n_pages - small.n_pages
+    for big, little in ((k, small.k), (v, small.v), (ks, small.ks), (vs, small.vs)):
+        big[:, off:] = little
+    table = torch.where(small.table >= 0, small.table + off, -1)
+    c, s = mm3fa.Kv8Cache(k, v, ks, vs), small.cache()
+    x = small.randn(2, Hkv, 100, D)
+    for cache, t in ((c, table), (s, small.table)):
+        cache.append(0, x, x, t, small.len)
+    assert torch.equal(k[:, off:], small.k) and torch.equal(ks[:, off:], small.ks) and not k[:, :off].any()
+    n = small.len + 100
+    for n_q in (1, 100):
+        for dt in (torch.float32, torch.bfloat16):
+            q = small.randn(2, 32, n_q, D).to(dt)
+            assert torch.equal(c.attend(0, q, table, n, 0.1), s.attend(0, q, small.table, n, 0.1))
+    ko, vo, k1, v1 = (torch.zeros(2, Hkv, 400, D, device=cuda_device) for _ in range(4))
+    c.read(0, ko, vo, table, torch.zeros_like(n), n)
+    s.read(0, k1, v1, small.table, torch.zeros_like(n), n)
+    assert torch.equal(ko, k1) and torch.equal(vo, v1)
+    refs = torch.zeros(n_pages, dtype=I32, device=cuda_device)
+    refs[table[table >= 0].long()] = 1
+    refs[:off] = 1  # the only free pages are far into the pool
+    t2, l2, r2 = torch.empty_like(table), torch.empty_like(n), torch.empty_like(refs)
+    c.fork(ints(0), ints(1), table, n, refs, t2, l2, r2)
+    c.check()
+    last = int(t2[1, 3])
+    assert last >= off and int(refs[last]) == 0 and t2[1, :3].tolist() == table[0, :3].tolist()
+    assert torch.equal(k[0, last], k[0, int(table[0, 3])]) and torch.equal(vs[0, last], vs[0, int(table[0, 3])])
 
 
 # ---------------------------------------------------------------- append and read
