@@ -64,6 +64,7 @@ struct Kv8AttnParams {
     uint32_t *  status;
     uint32_t *  counters;
     float *     part;
+    int         parts;  // of a block of rows' keys, at most (many rows)
     uint64_t    timeout_ns;
 };
 
@@ -179,7 +180,9 @@ cudaError_t launch_kv8_read(const Kv8StoreParams & p, cudaStream_t stream);
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p, int sms, cudaStream_t stream);
 cudaError_t launch_kv8_dense(const Kv8AttnParams & p, cudaStream_t stream);
 int         kv8_dense_tile(const Kv8AttnParams & p);  // rows of a CTA
-size_t      kv8_attn_workspace_bytes(int D, int n_q, int ratio, int sms);
+int         kv8_dense_parts(int64_t items, int64_t tokens, int sms);  // parts of a block of rows' keys, at most
+size_t      kv8_dense_part_bytes(int D, int64_t items, int tile, int parts);
+size_t      kv8_attn_workspace_bytes(int D, int64_t rows, int64_t heads, int64_t tokens, int sms);
 cudaError_t launch_kv8_fork(const Kv8PlanParams & p, const Kv8PoolCopy & c, int sms, cudaStream_t stream);
 cudaError_t launch_kv8_compact(const Kv8PlanParams & p, const Kv8PoolCopy & c, int sms, cudaStream_t stream);
 cudaError_t launch_kv8_reserve(const Kv8PlanParams & p, cudaStream_t stream);

@@ -282,8 +282,8 @@ size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q,
         q->ne[2] / cache->n_head_kv * q->ne[1] > (1 << 24)) {
         return 0;
     }
-    return kv8_attn_workspace_bytes(cache->head_dim, (int) q->ne[1], (int) (q->ne[2] / cache->n_head_kv),
-                                    host_sm_count());
+    return kv8_attn_workspace_bytes(cache->head_dim, q->ne[1] * (q->ne[2] / cache->n_head_kv), (int64_t) cache->n_head_kv * table->n_seq,
+                                    (int64_t) table->max_pages * cache->page_tokens, host_sm_count());
 }
 
 int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, const mm3fa_kv8_table * table,

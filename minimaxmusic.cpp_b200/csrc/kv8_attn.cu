@@ -28,11 +28,14 @@
 //
 // Bound.  One token of 48 sequences of 1 to 10240 tokens (32 heads on 8, D = 128, BF16): the cache's bytes, 105 us
 // or 74 % of the copy bandwidth of 6.54 TB/s; 110 of 2000 each, 90 us and 77 %.  For two of 8192 (19 us, 33.6 MB, floor
-// 5.1 us) the start - lengths, table, first pages, one after another - and the join of the parts take 8 us, as
-// in an empty call, and each CTA's 20 blocks the rest.  From 16 rows on (NT = 2) it is issue: 0.05 us per
-// 32-key block and CTA, four times the load's.  Two stages for three CTAs of an SM against three stages for two, D = 128:
+// 5.1 us) the start - lengths, table, first pages, one after another - and the join of the parts are the 8 us that a call
+// over a hundred tokens takes, and the 9 blocks of a CTA, 2 or 3 a warp, end before the rings reach their rate.  From 9
+// rows on (NT = 2) it is issue: 0.8 us for a block of a CTA, two CTAs an SM (16 sequences of 1024, 64 rows per kv head:
+// 51 us).  Two stages for three CTAs of an SM against three stages for two, D = 128, one row per head:
 // 105 us against 122 for the 48 sequences, 19.3 against 18.6 for the two.
 #include "kv8.cuh"
+
+#include <algorithm>
 
 namespace mm3fa {
 
@@ -939,33 +942,42 @@ int ctas_per_sm(int D, int rows) {
                      : (D == 64 ? KdSmem<64, 2, true>::CTAS : D == 128 ? KdSmem<128, 2, true>::CTAS : KdSmem<256, 2, true>::CTAS);
 }
 
-// The kernel for many rows (D <= 128) takes a call that gives every SM two units of this kernel, and every SM of each
-// wave of its own CTAs, which do not split a sequence's keys.
-bool many_rows(const Kv8AttnParams & p, int sms) {
+// The kernel for many rows (D <= 128) takes a call that gives every SM of each wave of its CTAs five units of this
+// kernel for two, a part of a block's keys counted like the whole.  BF16, D = 128, this kernel against that at 1.7 such
+// units per SM (4 sequences of 4096, 32 rows per kv head): 34 us against 35; at 2.0 (one of 8192, 32 rows) 27 against 35; at
+// 2.6 (16 of 1024, 48 rows) 45 against 31; at 3.5 (4 of 4096, 64 rows) 58 against 36; at 3.9 (one of 8192, 64 rows) 34
+// against 35, and of 256 rows 89 against 45.
+bool many_rows(Kv8AttnParams & p, int sms) {
     const int64_t heads = (int64_t) p.t.n_seq * p.c.n_head_kv, rows = (int64_t) p.ratio * p.n_q;
     const int     tile  = kv8_dense_tile(p);
-    const int64_t waves = (heads * ((rows + tile - 1) / tile) + sms - 1) / sms;
-    return p.c.D <= 128 && heads * ((rows + KD_ROWS - 1) / KD_ROWS) >= 2 * waves * sms;
+    const int64_t items = heads * ((rows + tile - 1) / tile), waves = (items + sms - 1) / sms;
+    p.parts             = kv8_dense_parts(items, (int64_t) p.t.max_pages * p.c.P, sms);
+    return p.c.D <= 128 && heads * ((rows + KD_ROWS - 1) / KD_ROWS) * p.parts * 2 >= 5 * waves * sms;
 }
 
 }  // namespace
 
 // Counters (one per CTA, in a place of one size for every shape: a workspace serves them all, and no shape's
-// partial results may lie on another's counters) and two partial results per CTA, whatever the lengths are.
-size_t kv8_attn_workspace_bytes(int D, int n_q, int ratio, int sms) {
-    const size_t ctas = (size_t) sms * (size_t) ctas_per_sm(D, ratio * n_q);
-    return WS_STATUS_BYTES + counter_bytes(sms) + 2 * ctas * KD_ROWS * (size_t) (D + 4) * 4;
+// partial results may lie on another's counters) and two partial results per CTA, whatever the lengths are, or
+// those of the kernel for many rows.
+size_t kv8_attn_workspace_bytes(int D, int64_t rows, int64_t heads, int64_t tokens, int sms) {
+    size_t most = 2 * (size_t) sms * (size_t) ctas_per_sm(D, (int) rows) * KD_ROWS * (size_t) (D + 4) * 4;
+    for (int tile = 128; tile <= 256 && D <= 128; tile += 128) {
+        const int64_t items = heads * ((rows + tile - 1) / tile);
+        most                = std::max(most, kv8_dense_part_bytes(D, items, tile, kv8_dense_parts(items, tokens, sms)));
+    }
+    return WS_STATUS_BYTES + counter_bytes(sms) + most;
 }
 
 cudaError_t launch_kv8_attn(const Kv8AttnParams & p0, int sms, cudaStream_t stream) {
     Kv8AttnParams p    = p0;
     p.ratio_inv        = p.ratio == 1 ? 0u : (uint32_t) ((1ull << 32) / (uint64_t) p.ratio + 1);
+    p.counters = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.status) + WS_STATUS_BYTES);
+    p.part     = reinterpret_cast<float *>(reinterpret_cast<char *>(p.counters) + counter_bytes(sms));
     if (many_rows(p, sms)) {
         return launch_kv8_dense(p, stream);
     }
     const int     most = sms * ctas_per_sm(p.c.D, p.ratio * p.n_q);
-    p.counters = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.status) + WS_STATUS_BYTES);
-    p.part     = reinterpret_cast<float *>(reinterpret_cast<char *>(p.counters) + counter_bytes(sms));
     const int     all = p.ratio * p.n_q, rows = all < KD_ROWS ? all : KD_ROWS;
     const int64_t units  = (int64_t) p.t.n_seq * p.c.n_head_kv * ((all + KD_ROWS - 1) / KD_ROWS);
     const int64_t blocks = units * (((int64_t) p.t.max_pages * p.c.P + KD_BLOCK - 1) / KD_BLOCK);  // at most

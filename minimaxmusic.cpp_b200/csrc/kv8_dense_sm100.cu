@@ -23,6 +23,10 @@
 //                 buffers j & 1, in the order QK(j+1), PV(j): the products of one tile beside the softmax of the next.
 //   warpgroup 2   softmax, one row per thread.   warpgroup 3   the same for tile 1 (TWO), or O's sums.
 //
+// Where the blocks of rows are fewer than half the SMs, each block's key tiles are cut into parts, one CTA each, all at
+// once; a part leaves O, m, l and R in the workspace, and the last to arrive joins them in their order.  256 tokens
+// over 8192 (one sequence, 32 heads on 8, D = 128, BF16): 65 us against 190 in one part each.
+//
 // Softmax.  s = S * (row factor * key scale of the column's page), in log2 units; weights 2^(s - m); the
 // value scale b = f 2^e of a page is multiplied into them, P = 2^(s - m) * 2^(m + e - R + KE_OFF) * f, so
 // that O is in units of 2^(R - KE_OFF).  m and R (the largest s + e of any page) are lazy: a tile's weights are
@@ -37,6 +41,8 @@
 #include "kv8.cuh"
 #include "tc_sm100.cuh"
 
+#include <algorithm>
+
 namespace mm3fa {
 
 constexpr int KE_THREADS = 512;
@@ -45,6 +51,9 @@ constexpr int KE_N       = 128;  // keys per tile
 constexpr int KE_TMEM    = 512;
 constexpr int KE_EMU     = 1;    // of every 8 pairs of weights, those by polynomial where P is rounded to F16 anyway
 constexpr int KE_OFF     = 8;    // P is held times 2^8 at the maxima: a tile's may be 2^7 above those taken before
+// Tiles of a part, at least: 1, 2, 4 take 25.2, 24.4, 28.4 us for 64 tokens over 1000 (BF16), 32.6, 28.3, 30.3 over 2000.
+constexpr int KE_PART  = 2;
+constexpr int KE_PARTS = 32;  // parts of a block of rows, at most: a joining thread holds a factor of each
 constexpr int KE_REGS_LAUNCH  = 128;  // 65536 / 512
 constexpr int KE_REGS_SOFTMAX = 192;  // 2 x 192 + 96 + 32 = 4 x 128
 constexpr int KE_REGS_CONVERT = 96;
@@ -165,16 +174,22 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
 
     // ---- the work item: row blocks last first, so that the longest causal ones start first
     const int hs = p.c.n_head_kv * p.t.n_seq, all_rows = p.ratio * p.n_q;
-    const int blk = (all_rows + KE_ROWS - 1) / KE_ROWS - 1 - (int) blockIdx.x / hs;
-    const int h = (int) blockIdx.x % hs % p.c.n_head_kv, s = (int) blockIdx.x % hs / p.c.n_head_kv;
+    const int items = (int) gridDim.x / p.parts, item = (int) blockIdx.x % items, part = (int) blockIdx.x / items;
+    const int blk = (all_rows + KE_ROWS - 1) / KE_ROWS - 1 - item / hs;
+    const int h = item % hs % p.c.n_head_kv, s = item % hs / p.c.n_head_kv;
     const int nq = p.q_len ? min(max(p.q_len[s], 0), p.n_q) : p.n_q;
     const int n  = min(max(p.kv_len[s], 0), p.t.max_pages * p.c.P);
-    const int row0 = blk * KE_ROWS, rows = min(nq * p.ratio - row0, KE_ROWS);  // rows of this block
-    const bool two = TWO && rows > KE_M;
+    const int row0 = blk * KE_ROWS, its_rows = min(nq * p.ratio - row0, KE_ROWS);  // rows of this block
     // keys that its last row sees
-    const int q_last = rows > 0 ? (row0 + rows - 1) / p.ratio : 0;
-    const int keys   = rows > 0 ? (p.causal ? max(n - (nq - 1 - q_last), 0) : n) : 0;
-    const int tiles  = (keys + KE_N - 1) / KE_N;
+    const int q_last    = its_rows > 0 ? (row0 + its_rows - 1) / p.ratio : 0;
+    const int its_keys  = its_rows > 0 ? (p.causal ? max(n - (nq - 1 - q_last), 0) : n) : 0;
+    const int its_tiles = (its_keys + KE_N - 1) / KE_N;
+    // this CTA's part of the tiles; a block with few of them has fewer parts
+    const int  parts = min(p.parts, max(1, (its_tiles + KE_PART - 1) / KE_PART));
+    const int  tile0 = (int) ((unsigned) its_tiles * (unsigned) min(part, parts) / (unsigned) parts);
+    const int  tiles = (int) ((unsigned) its_tiles * (unsigned) min(part + 1, parts) / (unsigned) parts) - tile0;
+    const int  rows  = part < parts ? its_rows : 0, before = tile0 * KE_N, keys = its_keys - before;
+    const bool two   = TWO && rows > KE_M;
 
     if (wg == 0) {
         // ======================================================= conversion
@@ -182,7 +197,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
         constexpr int LD = D / 16 * KE_N / 128;  // 16-code pieces per thread and tile
         // thread: rows 32 warp + 8 i + (lane & 7), pieces (lane >> 3) + 4 k: a warp reads whole 64-byte runs, and the
         // stores of eight lanes fall into eight rows, so into different banks
-        const int * row = p.t.pages + (int64_t) s * p.t.stride;
+        const int * row = p.t.pages + (int64_t) s * p.t.stride + (before >> p.c.log2p);
         int         pg0 = -1, pg1 = -1;
         auto        fetch = [&](int j) {  // table entries of the warp's 32 rows of tile j
             const int k0 = j * KE_N + 32 * warp, i = k0 >> p.c.log2p;
@@ -469,6 +484,103 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 }
             }
         };
+        // ---- parts of a block: each leaves its O, maxima and sums, row r of thread r, and the last to arrive joins them in
+        // their order
+        constexpr int SLOT = KE_M * (D + 4);  // floats: [D / 4][row] of four, then m, l and R of the rows
+        float *       slot = p.part + (int64_t) ((item * p.parts + part) * (TWO ? 2 : 1) + t) * SLOT;
+        const int     own  = quad * 32 + lane;
+        auto          give = [&](int c, const uint32_t (&o)[32]) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                reinterpret_cast<uint4 *>(slot)[(c * 8 + k) * KE_M + own] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            }
+        };
+        auto give_state = [&](float m, float l, float R) {
+            slot[D * KE_M + own] = m, slot[(D + 1) * KE_M + own] = l, slot[(D + 2) * KE_M + own] = R;
+        };
+        auto arrive = [&] {  // by the 128 threads of a Q tile; true for the last part
+            int * last = reinterpret_cast<int *>(smem + L::OFF_MISC + 8 + 4 * t);
+            __threadfence();
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+            if (own == 0) {
+                uint32_t * count = p.counters + item * 2 + t;
+                *last            = atomicAdd(count, 1u) == (uint32_t) (parts - 1);
+                if (*last) {
+                    *count = 0;
+                }
+                __threadfence();
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+            return *reinterpret_cast<volatile int *>(last) != 0;
+        };
+        auto join = [&] {  // the result's rows from the parts, into shared memory; every product is done
+            const float * first = p.part + (int64_t) (item * p.parts * (TWO ? 2 : 1) + t) * SLOT;
+            constexpr int STEP  = (TWO ? 2 : 1) * SLOT;
+            float         m = -INFINITY, R = -INFINITY, l = 0.0f, f[KE_PARTS];
+#pragma unroll 4
+            for (int k = 0; k < parts; k++) {
+                m = fmaxf(m, __ldcg(first + k * STEP + D * KE_M + own)), R = fmaxf(R, __ldcg(first + k * STEP + (D + 2) * KE_M + own));
+            }
+#pragma unroll 4
+            for (int k = 0; k < parts; k++) {  // (a sum of NaN passes through a factor of 0)
+                const float mk = __ldcg(first + k * STEP + D * KE_M + own), Rk = __ldcg(first + k * STEP + (D + 2) * KE_M + own);
+                l += __ldcg(first + k * STEP + (D + 1) * KE_M + own) * (mk == -INFINITY ? 0.0f : ex2(mk - m));
+                f[k] = Rk == -INFINITY ? 0.0f : ex2(Rk - R);
+            }
+            const float inv = l != 0.0f ? (1.0f / (1 << KE_OFF)) / l : 0.0f, up = R == -INFINITY ? 0.0f : ex2(R - m);
+            // 32 columns of a part at a time through this thread's own places in K's and V's shared memory
+            constexpr int  NS   = (TWO ? 2 : 4) * L::KT / (KE_M * 128);
+            const uint32_t ring = smem_addr(smem + L::OFF_K + t * 2 * L::KT) + (uint32_t) own * 16;
+            int            fc = 0, fk = 0, fs = 0, at = 0;
+            auto           fetch = [&] {
+                if (fc < D / 32) {
+                    const float * src = first + fk * STEP + (fc * 8 * KE_M + own) * 4;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (uint32_t) ((fs * 8 + e) * KE_M * 16)),
+                                     "l"(src + e * KE_M * 4)
+                                     : "memory");
+                    }
+                    fc = fk + 1 == parts ? fc + 1 : fc, fk = fk + 1 == parts ? 0 : fk + 1;
+                }
+                fs = fs + 1 == NS ? 0 : fs + 1;
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+#pragma unroll 1
+            for (int i = 0; i < NS - 1; i++) {
+                fetch();
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+                float a[32];
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    a[e] = 0.0f;
+                }
+#pragma unroll 1
+                for (int k = 0; k < parts; k++) {
+                    fetch();
+                    asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
+                    const float g = f[k];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        float4 x;
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                                     : "r"(ring + (uint32_t) ((at * 8 + e) * KE_M * 16)));
+                        a[4 * e] = fmaf(x.x, g, a[4 * e]), a[4 * e + 1] = fmaf(x.y, g, a[4 * e + 1]);
+                        a[4 * e + 2] = fmaf(x.z, g, a[4 * e + 2]), a[4 * e + 3] = fmaf(x.w, g, a[4 * e + 3]);
+                    }
+                    at = at + 1 == NS ? 0 : at + 1;
+                }
+                uint32_t o[32];
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    o[e] = __float_as_uint(a[e] * inv * up);
+                }
+                stage_cols(c, o);
+            }
+        };
         // ---- Q: rows [ra, ra + 16) of the tile by one warp, whole rows at a time, all loads in flight
         auto stage_q = [&](int ra) {
             constexpr int E = D / 32, B = 8;
@@ -615,7 +727,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 if (!ok) {
                     atomicExch(abort_f, 1);
                 }
-                const float inv = grows[4 * KE_M + r], up = grows[5 * KE_M + r];
+                const float inv = parts > 1 ? 1.0f : grows[4 * KE_M + r], up = parts > 1 ? 1.0f : grows[5 * KE_M + r];
 #pragma unroll
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t o[32];
@@ -623,9 +735,22 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                     for (int e = 0; e < 32; e++) {
                         o[e] = __float_as_uint(ok ? acc[c * 32 + e] * inv * up : 0.0f);
                     }
-                    stage_cols(c, o);
+                    if (parts > 1) {
+                        give(c, o);
+                    } else {
+                        stage_cols(c, o);
+                    }
                 }
-                store_rows();
+                bool mine_too = true;
+                if (parts > 1) {
+                    mine_too = arrive();
+                    if (mine_too) {
+                        join();
+                    }
+                }
+                if (mine_too) {
+                    store_rows();
+                }
             }
         } else if (tile_rows > 0) {
             if (!dn_wait_warp(&bar[KB_QREADY + t], 0, deadline)) {
@@ -635,7 +760,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
             const int  rw    = row0 + t * KE_M + r;
             const bool live  = r < tile_rows;
             const int  my_q  = (int) kv8_div((uint32_t) rw, p.ratio_inv);
-            const int  lim   = !live ? 0x7fffffff : p.causal ? n - (nq - 1 - my_q) : n;  // keys of this row
+            const int  lim   = !live ? 0x7fffffff : (p.causal ? n - (nq - 1 - my_q) : n) - before;  // keys of this row
             const int  warp_lim = (int) __reduce_min_sync(0xffffffffu, (unsigned) max(lim, 0));
             float      m = -INFINITY, l = 0.0f, R = -INFINITY;
             bool       ok = true;
@@ -812,6 +937,10 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                     atomicExch(abort_f, 1);
                 }
                 grows[4 * KE_M + r] = inv, grows[5 * KE_M + r] = up;
+                if (parts > 1) {
+                    give_state(m, l, R);
+                    __threadfence();  // the summing threads' arrival speaks for these too
+                }
                 dn_mbar_arrive(&bar[KB_LAST]);
             }
             if (TWO) {
@@ -839,11 +968,25 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
-                    o[e] = __float_as_uint(have ? __uint_as_float(o[e]) * inv * up : 0.0f);
+                    o[e] = __float_as_uint(have ? __uint_as_float(o[e]) * (parts > 1 ? 1.0f : inv) * (parts > 1 ? 1.0f : up) : 0.0f);
                 }
-                stage_cols(c, o);
+                if (parts > 1) {
+                    give(c, o);
+                } else {
+                    stage_cols(c, o);
+                }
             }
-            store_rows();
+            bool mine_too = true;
+            if (parts > 1) {
+                give_state(m, l, R);
+                mine_too = arrive();
+                if (mine_too) {
+                    join();
+                }
+            }
+            if (mine_too) {
+                store_rows();
+            }
             }
         }
     }
@@ -875,7 +1018,7 @@ cudaError_t launch_one(const Kv8AttnParams & p, cudaStream_t stream) {
         return cudaErrorInvalidConfiguration;
     }
     constexpr int   smem = KeSmem<D, QP, TWO>::TOTAL, step = TWO ? 256 : 128;
-    const int64_t   rows = (int64_t) p.ratio * p.n_q, ctas = (rows + step - 1) / step * p.c.n_head_kv * p.t.n_seq;
+    const int64_t   rows = (int64_t) p.ratio * p.n_q, ctas = (rows + step - 1) / step * p.c.n_head_kv * p.t.n_seq * p.parts;
     const cudaError_t e  = once.smem(kern, smem);
     return e != cudaSuccess ? e : kv8_launch(kern, dim3((unsigned) ctas), KE_THREADS, smem, stream, p);
 }
@@ -892,6 +1035,14 @@ cudaError_t launch_d(const Kv8AttnParams & p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int kv8_dense_parts(int64_t items, int64_t tokens, int sms) {
+    return (int) std::max<int64_t>(1, std::min<int64_t>({ sms / items, (tokens + KE_N * KE_PART - 1) / (KE_N * KE_PART), KE_PARTS }));
+}
+
+size_t kv8_dense_part_bytes(int D, int64_t items, int tile, int parts) {
+    return parts > 1 ? (size_t) (items * parts) * (size_t) tile * (size_t) (D + 4) * 4 : 0;
+}
 
 int kv8_dense_tile(const Kv8AttnParams & p) {
     return p.o.type == KV_BF16 && (int64_t) p.t.max_pages * p.c.P <= KE_LONG ? 2 * KE_M : KE_M;

@@ -223,7 +223,7 @@ class Kv8Cache:
             make = self._torch.empty if q_len is None else self._torch.zeros
             out = make((q.shape[0], q.shape[2], q.shape[1], q.shape[3]), dtype=q.dtype, device=q.device)
         if ws is None:
-            shape = (q.shape[2], q.shape[1], n)
+            shape = (q.shape[2], q.shape[1], n, table.shape[1])
             need = self._need.get(shape)
             if need is None:
                 need = self._need[shape] = self._call("attn_workspace", self._desc, qd, td)

@@ -24,11 +24,11 @@ def ints(*v, dev="cuda"):
 # ---------------------------------------------------------------- attention
 
 def repeats(st, rows):
-    """How often a batch is repeated so that the kernel for many rows takes its `rows` rows per kv head (0: never): two
-    units of 16 rows for each SM, and each wave of CTAs of 128 rows."""
+    """How often a batch is repeated so that the kernel for many rows takes its `rows` rows per kv head (0: never): five
+    units of 16 rows for every two SMs and each wave of CTAs of 128 rows."""
     sms = torch.cuda.get_device_properties(0).multi_processor_count
     heads, units, tiles = st.N * st.Hkv, -(-rows // 16), -(-rows // 128)
-    return next((r for r in range(1, 400) if r * heads * units >= 2 * sms * -(-r * heads * tiles // sms)), 0) if st.D <= 128 else 0
+    return next((r for r in range(1, 400) if 2 * r * heads * units >= 5 * sms * -(-r * heads * tiles // sms)), 0) if st.D <= 128 else 0
 
 
 def many(st, rows):
@@ -257,6 +257,26 @@ def test_attend_one_score_far_above_those_before(cuda_device, n_q, dtype):
             q[..., 0] = jump
             run_attend(st, 2, n_q, DTYPES[dtype], q=q.to(DTYPES[dtype]), scale=1.0, causal=False, what=f"{at} {jump}")
             st.k[..., 0] = 0
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_many_rows_over_long_caches(cuda_device, D, dtype):
+    """Some hundred rows over long caches, whose keys are split: sequences of many parts beside ones of one, of none, with
+    missing pages, rows that see nothing of the last parts, ragged rows."""
+    dt = DTYPES[dtype]
+    st = R.State([5000, 130, 0, 2600], 2, D, 64, seed=22, device=cuda_device)
+    run_attend(st, 8, 64, dt)
+    run_attend(st, 8, 64, dt, causal=False, softcap=3.0)
+    run_attend(st, 8, 90, dt, q_len=[90, 33, 5, 70])
+    st.table[0, 20:50] = -1
+    run_attend(st, 8, 64, dt)
+    st = R.State([5000], 1, D, 32, seed=23, device=cuda_device)
+    run_attend(st, 1, 1200, dt)
+    run_attend(st, 3, 1000, dt, q_len=[999])
+    st.vs[0, st.table[0, :120].long()] *= 1e-30  # the first parts' values are far below the last's
+    st.ks[0, st.table[0, 130:].long()] *= 20
+    run_attend(st, 3, 1000, dt, causal=False)
 
 
 @pytest.mark.parametrize("D", [64, 128])
