@@ -527,7 +527,7 @@ MM3FA_API size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_t
  *          as they were
  *   causal row i sees keys [0, kv_len - (q_len - 1 - i)); otherwise every row sees [0, kv_len)
  *   logit_softcap  0 disables; otherwise s <- softcap * tanh(s / softcap)
- *   workspace      zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this
+ *   workspace      its first 64 KiB zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this
  *                  function alone, of any shapes and caches that it is large enough for
  * A row that sees no key becomes zeros.
  */
@@ -536,7 +536,7 @@ MM3FA_API int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_ten
                              int causal, mm3fa_tensor * dst, void * workspace, size_t workspace_bytes, void * stream);
 
 /* Bytes of device workspace the page operations below need for n_seq sequences (0: a cache that they
- * would refuse).  Zero-fill it once; one per stream.  A table's n_seq * max_pages stays below 2^31. */
+ * would refuse).  Zero-fill its first 64 KiB once; one per stream.  A table's n_seq * max_pages stays below 2^31. */
 MM3FA_API size_t mm3fa_kv8_pages_workspace(const mm3fa_kv8 * cache, int n_seq);
 
 /*

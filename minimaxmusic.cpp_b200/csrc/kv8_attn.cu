@@ -933,6 +933,7 @@ cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStrea
 // CTAs that an SM holds at once: what KdSmem plans for
 constexpr int KD_CTAS_MOST = KdSmem<64, 1, true>::CTAS;
 
+// (with the status within the 64 KiB that a caller has zeroed)
 size_t counter_bytes(int sms) {
     return ((size_t) sms * KD_CTAS_MOST * 4 + 255) / 256 * 256;
 }

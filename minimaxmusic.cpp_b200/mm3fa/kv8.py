@@ -25,6 +25,8 @@ _CACHE = struct.Struct("@6i4P")                 # struct mm3fa_kv8
 _PACK_TABLE = struct.Struct("@Pq2i").pack       # struct mm3fa_kv8_table
 _PACK_TENSOR = struct.Struct("@2i4q4QP").pack   # struct mm3fa_tensor
 
+_ZEROED = 1 << 16  # bytes of a workspace that have to be zero before its first use
+
 _fns = None
 
 
@@ -169,13 +171,14 @@ class Kv8Cache:
             raise MM3FAError(st, "mm3fa_kv8_" + name)
 
     def _workspace(self, key, nbytes):
-        """(address, bytes) of the workspace of an operation on a stream, zero-filled when it is made."""
+        """(address, bytes) of the workspace of an operation on a stream, zero-filled as far as it has to be when it is made."""
         buf = self._ws.get(key)
         if buf is not None and buf[1] >= nbytes:
             return buf
         torch = self._torch
         if nbytes > 0:
-            made = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=self.device)
+            made = torch.empty(max(nbytes, _ZEROED), dtype=torch.uint8, device=self.device)
+            made[:_ZEROED].zero_()
             self._kept.append(made)
             at = made.data_ptr(), made.numel()
             # one made during a capture is zeroed by each replay of the graph: nothing else may use it
@@ -212,8 +215,8 @@ class Kv8Cache:
                stream=None):
         """softmax(scale * q k^T) v of the queries q (N, n_head, n_q, D) over the first kv_len[s] tokens of each
         sequence; causal: the rows are the last tokens.  out: (N, n_q, n_head, D), F32 or q's type; made in
-        q's type when not given, with zeros in the rows behind q_len.  ws: a zero-filled uint8 tensor
-        instead of the cache's own workspace of the stream, for graphs that may run at the same time."""
+        q's type when not given, with zeros in the rows behind q_len.  ws: a uint8 tensor, its
+        first 64 KiB zero, instead of the cache's own workspace of the stream, for graphs that may run at the same time."""
         if stream is not None:  # what is allocated here belongs to that stream too
             with self._on(stream):
                 return self.attend(layer, q, table, kv_len, scale, out, q_len, causal, logit_softcap, ws)
