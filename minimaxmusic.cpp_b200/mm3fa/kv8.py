@@ -179,11 +179,13 @@ class Kv8Cache:
         if nbytes > 0:
             made = torch.empty(max(nbytes, _ZEROED), dtype=torch.uint8, device=self.device)
             made[:_ZEROED].zero_()
-            self._kept.append(made)
             at = made.data_ptr(), made.numel()
-            # one made during a capture is zeroed by each replay of the graph: nothing else may use it
-            if self._dev < 0 or not torch.cuda.is_current_stream_capturing():
+            # one made during a capture is zeroed by each replay of the graph: nothing else may use it, or read it before
+            if self._dev >= 0 and torch.cuda.is_current_stream_capturing():
+                key = None
+            else:
                 self._ws[key] = at
+            self._kept.append((key, made))
             return at
         return None, 0
 
@@ -286,14 +288,15 @@ class Kv8Cache:
 
     def check(self, stream=None):
         """Synchronises the stream and raises MM3FAError where a page operation on it found too few free pages
-        (ERR_PAGES) or a bounded device wait of an attention expired (ERR_TIMEOUT)."""
+        (ERR_PAGES) or a bounded device wait of an attention expired (ERR_TIMEOUT).  Captured calls are among them where an
+        earlier call on the stream had made their workspace; otherwise the graph has one of its own, which is not read."""
         if stream is not None:
             with self._on(stream):
                 return self.check()
         st = self._stream()
         for op in ("pages", "attn"):
-            buf = self._ws.get((op, st))
-            if buf is not None:
-                status, _ = workspace_status(buf[0], st)
-                if status != OK:
-                    raise MM3FAError(status, "Kv8Cache")
+            for key, buf in self._kept:  # a call before the workspace grew may have left its status in an older one
+                if key == (op, st):
+                    status, _ = workspace_status(buf.data_ptr(), st)
+                    if status != OK:
+                        raise MM3FAError(status, "Kv8Cache")

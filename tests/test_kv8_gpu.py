@@ -598,6 +598,43 @@ def test_fork_without_enough_pages(cuda_device):
     assert check_fork(st, [0], [1])[4]  # the pages that dst gives up are not given out in the same call
 
 
+def test_status_left_in_an_outgrown_workspace(cuda_device):
+    """A call that found too few pages is reported though a larger one came between it and the check."""
+    c = mm3fa.Kv8Cache.allocate(1, 5300, 1, 16, 64, cuda_device)
+    refs = torch.ones(5300, dtype=I32, device=cuda_device)
+    for n in (2, 500):
+        table = torch.full((n, 1), -1, dtype=I32, device=cuda_device)
+        c.reserve(table, refs, torch.ones(n, dtype=I32, device=cuda_device))
+        refs.zero_()
+    with pytest.raises(mm3fa.MM3FAError) as e:
+        c.check()
+    assert e.value.status == mm3fa.ERR_PAGES
+    c.check()
+
+
+def test_status_of_captured_calls(cuda_device):
+    """check reports what a replayed call found where the stream had a workspace before the capture, and reads no
+    workspace that only a graph has written."""
+    c = mm3fa.Kv8Cache.allocate(1, 4, 1, 16, 64, cuda_device)
+    refs, table, one = torch.ones(4, dtype=I32, device=cuda_device), torch.full((1, 1), -1, dtype=I32, device=cuda_device), ints(1)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g in graphs:
+        with torch.cuda.graph(g, stream=side):
+            c.reserve(table, refs, one)
+        c.check(side)
+        with torch.cuda.stream(side):
+            g.replay()
+            if g is graphs[0]:
+                c.check()
+                c.reserve(table, torch.zeros_like(refs), ints(0))  # makes the stream's workspace
+            else:
+                with pytest.raises(mm3fa.MM3FAError):
+                    c.check()
+    assert int(table[0, 0]) == -1
+
+
 def test_fork_missing_pages_and_no_pairs(cuda_device):
     st = R.State([100, 50], 2, 64, 16, spare=9, seed=3, device=cuda_device)
     st.table[0, 2] = -1
