@@ -756,7 +756,9 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
             if (!dn_wait_warp(&bar[KB_QREADY + t], 0, deadline)) {
                 atomicExch(abort_f, 1);
             }
-            const float factor = factors[t * KE_M + r];
+            // a row of NaN (its Q is 0) is taken like the others, and made NaN at the end if it has seen a key
+            const float * its    = factors + t * KE_M + r;
+            const float   factor = *its != *its ? 1.0f : *its;
             const int  rw    = row0 + t * KE_M + r;
             const bool live  = r < tile_rows;
             const int  my_q  = (int) kv8_div((uint32_t) rw, p.ratio_inv);
@@ -796,7 +798,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
 #pragma unroll
                 for (int g = 0; g < 8; g++) {
                     whole &= sc[g].w != 0.0f;
-                    plain &= !(factor * sc[g].x <= 0.0f);  // NaN: a row of NaN, whose neighbours go on as without it
+                    plain &= !(factor * sc[g].x <= 0.0f);
                 }
                 plain = __all_sync(0xffffffffu, plain);
                 // The weights are taken with the maxima as they are (only a row's first tile has none), and the maxima found
@@ -930,6 +932,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 tc_fence_before();
                 dn_mbar_arrive(&bar[KB_PREADY + buf]);
             }
+            l = *its != *its && m != -INFINITY ? NAN : l;
             // O (units of 2^(R - KE_OFF)) over the sum (2^m); rows without keys, and without a value scale, are 0
             const float inv = l != 0.0f ? (1.0f / (1 << KE_OFF)) / l : 0.0f, up = R == -INFINITY ? 0.0f : ex2(R - m);
             if (!TWO) {
