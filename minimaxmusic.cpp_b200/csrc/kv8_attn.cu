@@ -52,6 +52,9 @@ constexpr int KD_PART    = 4;
 // for 16 of 4096 (32: parts).  Whole against flat: 26.6 against 33.2 us for 50 of 1000, 89.9 against 91.6 for 110 of 2000.
 constexpr int KD_CROSS   = 32;
 
+constexpr int KD_SM_BYTES  = 228 * 1024;  // shared memory of an SM
+constexpr int KD_CTA_BYTES = 1024;        // what each CTA on it takes beside its own
+
 template <int D, int NT, bool HP>
 struct KdSmem {
     // CTAs per SM and stages per warp: what shared memory and registers hold
@@ -62,11 +65,18 @@ struct KdSmem {
     static constexpr int HEAD  = 32;                   // scales and flags
     static constexpr int STAGE = 2 * TILE + HEAD;
     static constexpr int RING  = KD_WARPS * NS * STAGE;
-    static constexpr int Q     = ND * NT * 8 * D;      // [digit][row][dim], chunks swizzled like K's
-    static constexpr int OROW  = D + 4;                // floats per row of the merge buffer
     static constexpr int STATE = 2 * NT * 8 * 3 * 4;   // m, l, R
-    static constexpr int FIXED = RING + Q + STATE + NT * 8 * 4;
-    static size_t        bytes(int rows) { return FIXED + (size_t) 2 * rows * OROW * 4; }
+    static constexpr int FIXED = RING + STATE + NT * 8 * 4;
+    // a segment's digits of q, [digit][row][dim], chunks swizzled like K's; at its end the merge buffer in their place.
+    // (Beside them it left two CTAs an SM of three: F32, 48 sequences of up to 10240, D = 128, 8 rows a kv head 169 us
+    // against 127; D = 64, 16 rows, F16, of up to 8000 tokens 84 against 69)
+    static constexpr int Q     = ND * NT * 8 * D;
+    static constexpr int OROW  = D + 4;                // floats per row of the merge buffer
+    __host__ __device__ static constexpr int bytes(int rows) {
+        return FIXED + (Q > 2 * rows * OROW * 4 ? Q : 2 * rows * OROW * 4);
+    }
+    static_assert(CTAS * (bytes(NT * 8) + KD_CTA_BYTES) <= KD_SM_BYTES, "the CTAs that the cuts count on do not fit on an SM");
+    static_assert(FIXED % 16 == 0, "the digits are read by 16 bytes");
 };
 
 __device__ __forceinline__ uint32_t kd_prmt(uint32_t a, uint32_t b, uint32_t sel) {
@@ -196,10 +206,10 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
     __shared__ int sh_last[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     char *    ring   = smem + warp * NS * L::STAGE;
-    char *    qf     = smem + L::RING;
-    float *   state  = reinterpret_cast<float *>(qf + L::Q);          // [2][row][m, l, R]
+    float *   state  = reinterpret_cast<float *>(smem + L::RING);     // [2][row][m, l, R]
     float *   qscale = state + 2 * NT * 8 * 3;                        // [row]
-    float *   obuf   = reinterpret_cast<float *>(smem + L::FIXED);    // [2][row][OROW]
+    char *    qf     = smem + L::FIXED;
+    float *   obuf   = reinterpret_cast<float *>(smem + L::FIXED);    // [2][row][OROW], over the digits
     const int all_rows = p.ratio * p.n_q, groups = (all_rows + KD_ROWS - 1) / KD_ROWS;
     const int units = p.c.n_head_kv * groups;  // of a sequence
     kv8_dep_wait();
@@ -728,9 +738,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
         }
 #pragma unroll 1
         for (int round = 0; round < 2; round++) {
-            if (round == 1) {
-                __syncthreads();
-            }
+            __syncthreads();  // the digits are not read any more; then: the two states are there
             if ((warp < 2) == (round == 1)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
