@@ -519,9 +519,9 @@ MM3FA_API size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_t
  * dst = softmax(scale * q k^T [softcap]) v over each sequence's pages of one layer.
  *   q      F32, F16 or BF16 [D, n_q, n_head, n_seq], any strides along dims 1 to 3; query head h reads
  *          kv head h / (n_head / n_head_kv)
- *   dst    [D, n_head, n_q, n_seq], F32 or q's type and not in q's memory.  An F32 result is computed to
- *          F32's precision: q and the softmax weights keep 22 bits.  For a 16-bit one q keeps 11 bits or more
- *          and the weights 22 (F16) or 11 (BF16)
+ *   dst    [D, n_head, n_q, n_seq], F32 or q's type and not in q's memory.  In the products an element of q is off by
+ *          at most 2^-22 of itself or 2^-30 of the largest one of its row and head (from 2^-121 on); the softmax
+ *          weights keep 22 bits, for a BF16 result 11; sums are F32
  *   kv_len device int32 [n_seq]: tokens that the cache holds, the query rows' own among them
  *   q_len  device int32 [n_seq] or NULL: rows of sequence s (NULL: n_q); rows from q_len[s] on are left
  *          as they were

@@ -3,9 +3,12 @@
 //
 // Mathematics.  With codes c and page scales a (keys) and b (values), s_j = scale * a * (q . c_j) and
 //     o = sum_j 2^(s_j - m) b c_j / sum_j 2^(s_j - m)          (s in log2 units, m a running maximum).
-//   * q . c in integers: a row of q becomes fixed-point numbers of three 8-bit digits, the largest element
-//     127.5 * 2^16 (two digits and 2^8 for 16-bit results: half a step is 2^-16 of the row's largest element, below
-//     what the result keeps), and each digit's dot with the codes is exact on the 8-bit tensor cores.
+//   * q . c in integers: a row of q becomes fixed-point numbers of four 8-bit digits, the largest element in
+//     [2^29, 2^30), and each digit's dot with the codes is exact on the 8-bit tensor cores.  No element is off by more
+//     than 2^-30 of the row's largest; F32 ones down to 2^-6 of it, F16 ones to 2^-19 and BF16 ones to 2^-22 are exact.
+//     (With three digits for F32 and two for 16-bit results the small elements beside a large one decided wrongly: one of
+//     1000 among N(0, 1), with keys of 0 there, put F16 results 5 half steps off.  48 sequences of up to 10240 tokens
+//     took 105 us in BF16 so, 115 now; F32 118 and 119.)
 //   * P . c in F16, which holds the codes exactly.  The value scale of a page goes into the weights,
 //     P = 2^(s - m) * 2^(m + e - R) * f with b = f 2^e, f in [1, 2), and R the running maximum of (a tile's
 //     largest s) + e: O is held in units of 2^R, the sum in units of 2^m, so that pages with scales of
@@ -55,12 +58,12 @@ constexpr int KD_CROSS   = 32;
 constexpr int KD_SM_BYTES  = 228 * 1024;  // shared memory of an SM
 constexpr int KD_CTA_BYTES = 1024;        // what each CTA on it takes beside its own
 
-template <int D, int NT, bool HP>
+template <int D, int NT>
 struct KdSmem {
     // CTAs per SM and stages per warp: what shared memory and registers hold
     static constexpr int CTAS  = D == 64 ? (NT == 1 ? 4 : 3) : (D == 128 ? (NT == 1 ? 3 : 2) : 1);
     static constexpr int NS    = D == 64 ? (NT == 1 ? 3 : 4) : (D == 128 ? 2 : (NT == 1 ? 3 : 2));
-    static constexpr int ND    = HP ? 3 : 2;           // digits of q
+    static constexpr int ND    = 4;                    // digits of q
     static constexpr int TILE  = KD_BLOCK * D;         // bytes of K or V
     static constexpr int HEAD  = 32;                   // scales and flags
     static constexpr int STAGE = 2 * TILE + HEAD;
@@ -197,10 +200,10 @@ struct KdPart {
     int s, u, c0, n;
 };
 
-// HP: an F32 result; PL: the weights' remainders too
+// HP: an F32 result; PL: the remainders of the weights too
 template <int D, int NT, bool HP, bool PL, bool CAP>
-__global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decode_kernel(const Kv8AttnParams p) {
-    using L          = KdSmem<D, NT, HP>;
+__global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT>::CTAS) kv8_decode_kernel(const Kv8AttnParams p) {
+    using L          = KdSmem<D, NT>;
     constexpr int NS = L::NS, ND = L::ND, CH = D / 64, MT = D / 16, E = D / 32, QR = NT * 8 / KD_WARPS;
     extern __shared__ __align__(16) char smem[];
     __shared__ int sh_last[2];
@@ -466,14 +469,15 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             }
             odd = __any_sync(0xffffffffu, odd);
-            // digits 127, 127, 127 at the largest element (the lowest 63: room for the division's roundings).  A row
-            // far from 1 is brought near by an exact power of two; one with an infinity or NaN gives NaN
-            constexpr float TOP = HP ? 8355647.0f : 32639.0f;
-            const float     up  = amax > 0x1p100f ? 0x1p-80f : (amax < 0x1p-100f ? 0x1p80f : 1.0f);
-            const float     mul = odd || amax == 0.0f ? 0.0f : __fdividef(TOP, amax * up);
+            // a power of two brings the largest element to [2^29, 2^30): the products are exact, and the fourth digit, with
+            // what the others carry into it, stays below 128.  A row near the smallest numbers is brought up first, so that
+            // the power is a number; one with an infinity or NaN gives NaN
+            const float up  = amax < 0x1p-90f ? 0x1p64f : 1.0f;
+            const int   ex  = min(max((int) (__float_as_uint(amax * up) >> 23) - 127, -90), 127);
+            const float mul = __uint_as_float((uint32_t) (29 - ex + 127) << 23);
             if (lane == 0) {
-                const float back = odd ? NAN : (mul > 0.0f ? __fdividef(1.0f, mul) / up : 0.0f);
-                qscale[rr]       = back * (CAP ? p.scale / p.softcap : p.scale * LOG2E);
+                const float back = odd ? NAN : __uint_as_float((uint32_t) (ex - 29 + 127) << 23);
+                qscale[rr]       = back * (CAP ? p.scale / p.softcap : p.scale * LOG2E) * (up == 1.0f ? 1.0f : 0x1p-64f);
             }
             uint32_t dig[ND][(E + 3) / 4];
 #pragma unroll
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                 int v = odd ? 0 : __float2int_rn(xq[i][e] * up * mul);
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
-                    const int low8 = (int8_t) v;  // digits in [-128, 127], the last in [-127, 127]
+                    const int low8 = (int8_t) v;  // digits in [-128, 127]
                     dig[d][e >> 2] |= (uint32_t) (low8 & 255) << (8 * (e & 3));
                     v = (v - low8) >> 8;
                 }
@@ -578,7 +582,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT, HP>::CTAS) kv8_decod
                         for (int e = 0; e < 4; e++) {
                             // |digit dots| < 2^22 (D = 256): two of them fit an int
                             const float lo   = (float) (acc[a][nt][1][e] * 256 + acc[a][nt][0][e]);
-                            s[a0 + a][nt][e] = HP ? fmaf((float) acc[a][nt][ND - 1][e], 65536.0f, lo) : lo;
+                            s[a0 + a][nt][e] = fmaf((float) (acc[a][nt][3][e] * 256 + acc[a][nt][2][e]), 65536.0f, lo);
                         }
                     }
                 }
@@ -917,9 +921,9 @@ namespace {
 
 template <int D, int NT, bool HP, bool PL, bool CAP>
 cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
-    const size_t smem = KdSmem<D, NT, HP>::bytes(rows);
+    const size_t smem = KdSmem<D, NT>::bytes(rows);
     static Kv8Once once;
-    const cudaError_t e = once.smem(kv8_decode_kernel<D, NT, HP, PL, CAP>, KdSmem<D, NT, HP>::bytes(NT * 8));
+    const cudaError_t e = once.smem(kv8_decode_kernel<D, NT, HP, PL, CAP>, KdSmem<D, NT>::bytes(NT * 8));
     return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, HP, PL, CAP>, dim3(ctas), KD_THREADS, smem, stream, p);
 }
 
@@ -939,7 +943,7 @@ cudaError_t launch_d(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStrea
 }
 
 // CTAs that an SM holds at once: what KdSmem plans for
-constexpr int KD_CTAS_MOST = KdSmem<64, 1, true>::CTAS;
+constexpr int KD_CTAS_MOST = KdSmem<64, 1>::CTAS;
 
 // (with the status within the 64 KiB that a caller has zeroed)
 size_t counter_bytes(int sms) {
@@ -947,8 +951,8 @@ size_t counter_bytes(int sms) {
 }
 
 int ctas_per_sm(int D, int rows) {
-    return rows <= 8 ? (D == 64 ? KdSmem<64, 1, true>::CTAS : D == 128 ? KdSmem<128, 1, true>::CTAS : KdSmem<256, 1, true>::CTAS)
-                     : (D == 64 ? KdSmem<64, 2, true>::CTAS : D == 128 ? KdSmem<128, 2, true>::CTAS : KdSmem<256, 2, true>::CTAS);
+    return rows <= 8 ? (D == 64 ? KdSmem<64, 1>::CTAS : D == 128 ? KdSmem<128, 1>::CTAS : KdSmem<256, 1>::CTAS)
+                     : (D == 64 ? KdSmem<64, 2>::CTAS : D == 128 ? KdSmem<128, 2>::CTAS : KdSmem<256, 2>::CTAS);
 }
 
 // The kernel for many rows (D <= 128) takes a call that gives every SM of each wave of its CTAs five units of this

@@ -2,8 +2,8 @@
 // prompt) on the 5th-generation tensor cores (tcgen05 + TMEM), sm_100a.
 //
 // Rows of a unit (kv head, sequence) are (query, head of the group) pairs in that order, so that all query heads of
-// a kv head share each K/V tile.  Q is brought to [1, 2) at its row's largest element by a power of two and
-// rounded to F16; an F32 result takes its F16 remainder as a second operand (QP = 2), an F32 or F16 result that of
+// a kv head share each K/V tile.  Q is brought to [2^14, 2^15) at its row's largest element by a power of two and
+// rounded to F16 (what a 16-bit q has is kept, but for elements below 2^-28 of the largest); an F32 result takes its F16 remainder as a second operand (QP = 2), an F32 or F16 result that of
 // the weights P (PP = 2): the product then runs twice, the remainder first, where the accumulator is small.
 //
 // The tensor core truncates what it adds to an F32 accumulator: each of a tile's K = 16 steps loses up to 2^-23 of
@@ -652,9 +652,11 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
                 }
 #pragma unroll
                 for (int i = 0; i < B; i++) {
-                    // the exponent of the largest element; a row with an infinity or NaN gives NaN
+                    // the largest element goes to [2^14, 2^15), the upper end of F16's range: an element keeps F16's 11 bits
+                    // down to 2^-28 of it, and its remainder another 11 to 2^-17.  (Rows below 2^-112, where the power would not be
+                    // a number, stay that much lower.)  A row with an infinity or NaN gives NaN
                     const bool  odd = top[i] >= 0x7f800000u;
-                    const int   ex  = top[i] == 0 || odd ? 0 : min(max((int) (top[i] >> 23) - 127, -126), 126);
+                    const int   ex  = (top[i] == 0 || odd ? 0 : max((int) (top[i] >> 23) - 127, -112)) - 14;
                     const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23);
                     mine_f          = lane == i ? (odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23)) : mine_f;
                     uint32_t w[E / 2], v[E / 2];
