@@ -18,6 +18,29 @@ def attend(st, q, out_dtype=None, causal=True):
     return out
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n_q", [1, 4, 16, 70])
+def test_f32_results_keep_22_bits(cuda_device, n_q, D, dtype):
+    """F32 results of queries of each type, from 64 keys to thousands."""
+    st = R.State([64, 500, 3001], 2, D, 64, seed=25, device=cuda_device)
+    q = st.randn(3, 8, n_q, D).to(DTYPES[dtype])
+    copies = many(st, 4 * n_q).N // 3
+    got = attend(st, q.repeat(copies, 1, 1, 1), torch.float32)
+    st.table, st.len, st.N = st.table[:3], st.len[:3], 3
+    E.check(st, q, got[:3], f"D {D}, {n_q} rows")
+
+
+@pytest.mark.parametrize("n_q", [1, 70])
+def test_f32_results_over_long_caches(cuda_device, n_q):
+    """20001 keys, values of both signs and of one."""
+    st = R.State([20001, 700, 9999], 2, 128, 64, seed=15, device=cuda_device)
+    q = st.randn(3, 8, n_q, 128)
+    E.check(st, q, attend(st, q), "both signs")
+    st.v.abs_()
+    E.check(st, q, attend(st, q), "one sign")
+
+
 def one_large(st, n_q, x, dtype):
     """Queries with one element of +-x in a dimension where every key is 0, the others around 1."""
     q = st.randn(st.N, 8, n_q, st.D).to(dtype)
