@@ -511,7 +511,7 @@ MM3FA_API int mm3fa_kv8_append(const mm3fa_kv8 * cache, int layer, const mm3fa_t
 MM3FA_API int mm3fa_kv8_read(const mm3fa_kv8 * cache, int layer, const mm3fa_kv8_table * table, const int32_t * start,
                              const int32_t * n, mm3fa_tensor * k_out, mm3fa_tensor * v_out, void * stream);
 
-/* Bytes of device workspace mm3fa_kv8_attn needs (0: operands it would refuse). */
+/* Bytes of device workspace mm3fa_kv8_attn needs, 64 KiB at least (0: operands it would refuse). */
 MM3FA_API size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q,
                                           const mm3fa_kv8_table * table);
 
@@ -535,8 +535,8 @@ MM3FA_API int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_ten
                              const int32_t * kv_len, const int32_t * q_len, float scale, float logit_softcap,
                              int causal, mm3fa_tensor * dst, void * workspace, size_t workspace_bytes, void * stream);
 
-/* Bytes of device workspace the page operations below need for n_seq sequences (0: a cache that they
- * would refuse).  Zero-fill its first 64 KiB once; one per stream.  A table's n_seq * max_pages stays below 2^31. */
+/* Bytes of device workspace the page operations below need for n_seq sequences, 64 KiB at least (0: a cache
+ * that they would refuse).  Zero-fill its first 64 KiB once; one per stream.  A table's n_seq * max_pages stays below 2^31. */
 MM3FA_API size_t mm3fa_kv8_pages_workspace(const mm3fa_kv8 * cache, int n_seq);
 
 /*

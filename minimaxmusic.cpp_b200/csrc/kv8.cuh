@@ -77,6 +77,8 @@ struct Kv8PoolCopy {
     int64_t  page_bytes;  // of one layer's K or V, a multiple of 16
 };
 
+constexpr size_t KV8_WS_ZEROED = 1 << 16;  // bytes of a workspace that a caller zeroes: none is smaller
+
 // Workspace of the page operations (int32 words from its base; 64 words of status and counts first).
 constexpr int KV8_WS_COPIES = 32;  // page copies that the plan wants done
 constexpr int KV8_WS_FAILED = 33;  // nonzero: too few pages, nothing changes

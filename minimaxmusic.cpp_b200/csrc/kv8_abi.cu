@@ -169,7 +169,7 @@ Kv8StoreParams store_params(const mm3fa_kv8 * c, int layer, const mm3fa_tensor *
 }
 
 size_t pages_workspace(const mm3fa_kv8 * c, int64_t n_seq) {
-    return 4 * ((size_t) KV8_WS_HEAD + 3 * (size_t) c->n_pages + 2 * (size_t) n_seq);
+    return std::max(KV8_WS_ZEROED, 4 * ((size_t) KV8_WS_HEAD + 3 * (size_t) c->n_pages + 2 * (size_t) n_seq));
 }
 
 // The workspace's parts; MM3FA_ERR_WORKSPACE where it is missing, too small or not 4-byte aligned.
@@ -282,8 +282,9 @@ size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q,
         q->ne[2] / cache->n_head_kv * q->ne[1] > (1 << 24)) {
         return 0;
     }
-    return kv8_attn_workspace_bytes(cache->head_dim, q->ne[1] * (q->ne[2] / cache->n_head_kv), (int64_t) cache->n_head_kv * table->n_seq,
-                                    (int64_t) table->max_pages * cache->page_tokens, host_sm_count());
+    return std::max(KV8_WS_ZEROED, kv8_attn_workspace_bytes(cache->head_dim, q->ne[1] * (q->ne[2] / cache->n_head_kv),
+                                                            (int64_t) cache->n_head_kv * table->n_seq,
+                                                            (int64_t) table->max_pages * cache->page_tokens, host_sm_count()));
 }
 
 int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, const mm3fa_kv8_table * table,

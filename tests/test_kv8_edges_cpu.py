@@ -1,0 +1,27 @@
+"""What the header promises of the 8-bit paged cache's workspaces and sizes, on host tensors."""
+import pytest
+import torch
+
+import kv8_ref
+import mm3fa
+from mm3fa import kv8
+
+no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="host tensors are accepted up to the device check only")
+
+
+def make(**kw):
+    kw = {"lens": [70, 5], "Hkv": 2, "D": 64, "P": 32, "room": [80, 40], **kw}
+    return kv8_ref.State(**kw)
+
+
+@pytest.mark.parametrize("n_pages,n_seq", [(1, 1), (512, 2), (100000, 65535)])
+def test_a_workspace_holds_what_has_to_be_zeroed(n_pages, n_seq):
+    """The first 64 KiB of a workspace are to be zeroed: it has as many bytes."""
+    c = kv8._CACHE.pack(64, 32, 2, n_pages, 1, 0, *[1 << 20] * 4)
+    f = kv8._calls()
+    assert f["pages_workspace"](c, n_seq) >= 1 << 16
+    assert f["pages_workspace"](c, n_seq) >= 4 * (3 * n_pages + 2 * n_seq)
+    q = kv8._PACK_TENSOR(0, 0, 64, 1, 2, n_seq, 4, 256, 256, 512, 1 << 20)
+    assert f["attn_workspace"](c, q, kv8._PACK_TABLE(1 << 20, 3, 3, n_seq)) >= 1 << 16
+    bad = kv8._CACHE.pack(65, 32, 2, n_pages, 1, 0, *[1 << 20] * 4)
+    assert f["pages_workspace"](bad, n_seq) == 0 and f["attn_workspace"](bad, q, kv8._PACK_TABLE(1 << 20, 3, 3, n_seq)) == 0
