@@ -189,6 +189,14 @@ class Kv8Cache:
             return at
         return None, 0
 
+    def _given(self, ws):
+        """(address, bytes) of a caller's workspace."""
+        if ws.get_device() != self._dev:
+            raise self._elsewhere(ws)
+        if not ws.is_contiguous():
+            raise MM3FAError(ERR_STRIDE, "Kv8Cache: workspace")
+        return ws.data_ptr(), ws.numel() * ws.element_size()
+
     # ------------------------------------------------------------ operators
 
     def append(self, layer, k_new, v_new, table, start, n_new=None, stream=None):
@@ -234,7 +242,7 @@ class Kv8Cache:
                 need = self._need[shape] = self._call("attn_workspace", self._desc, qd, td)
             ptr, cap = self._workspace(("attn", st), need)
         else:
-            ptr, cap = ws.data_ptr(), ws.numel() * ws.element_size()
+            ptr, cap = self._given(ws)
         self._run("attn", self._desc, layer, qd, td, self._ints(kv_len, n, "kv_len"),
                    None if q_len is None else self._ints(q_len, n, "q_len"), scale, logit_softcap, 1 if causal else 0,
                    self._rows(out), ptr, cap, st)

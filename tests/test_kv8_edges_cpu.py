@@ -25,3 +25,29 @@ def test_a_workspace_holds_what_has_to_be_zeroed(n_pages, n_seq):
     assert f["attn_workspace"](c, q, kv8._PACK_TABLE(1 << 20, 3, 3, n_seq)) >= 1 << 16
     bad = kv8._CACHE.pack(65, 32, 2, n_pages, 1, 0, *[1 << 20] * 4)
     assert f["pages_workspace"](bad, n_seq) == 0 and f["attn_workspace"](bad, q, kv8._PACK_TABLE(1 << 20, 3, 3, n_seq)) == 0
+
+
+class Elsewhere:
+    """A workspace on a device that the cache is not on."""
+    device = "cuda:0"
+
+    def __init__(self):
+        self.t = torch.zeros(1 << 22, dtype=torch.uint8)
+
+    def get_device(self):
+        return 0
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+@no_gpu
+def test_a_given_workspace_is_checked():
+    """A workspace of another device, or one with gaps, is refused before its address goes anywhere."""
+    s = make()
+    c, q, out = s.cache(), torch.zeros(2, 4, 3, 64), torch.zeros(2, 3, 4, 64)
+    with pytest.raises(ValueError):
+        c.attend(0, q, s.table, s.len, 0.1, out, ws=Elsewhere())
+    with pytest.raises(mm3fa.MM3FAError) as e:
+        c.attend(0, q, s.table, s.len, 0.1, out, ws=torch.zeros(1 << 22, dtype=torch.uint8)[::2])
+    assert e.value.status == mm3fa.ERR_STRIDE
