@@ -529,7 +529,7 @@ MM3FA_API size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_t
  *   logit_softcap  0 disables; otherwise s <- softcap * tanh(s / softcap)
  *   workspace      its first 64 KiB zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this
  *                  function alone, of any shapes and caches that it is large enough for
- * A row that sees no key becomes zeros.
+ * A row that sees no key becomes zeros.  kv_len is clamped to the table's tokens, of which there are up to 2^31 - 8192.
  */
 MM3FA_API int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, const mm3fa_kv8_table * table,
                              const int32_t * kv_len, const int32_t * q_len, float scale, float logit_softcap,

@@ -57,6 +57,11 @@ int check_table(const mm3fa_kv8 * c, const mm3fa_kv8_table * t) {
     return aligned_to(t->pages, 4) ? MM3FA_OK : MM3FA_ERR_ALIGN;
 }
 
+// The attention rounds token counts up to its blocks and looks some ahead, in 32 bits.
+bool attn_tokens_fit(const mm3fa_kv8 * c, const mm3fa_kv8_table * t) {
+    return (int64_t) t->max_pages * c->page_tokens <= (int64_t) 1 + INT32_MAX - 8192;
+}
+
 // Rows [D, ne1, ne2, ne3] of a floating type; strides are any multiples of the element size.
 int check_rows(const mm3fa_tensor * t, int64_t D) {
     if (!t) {
@@ -277,7 +282,7 @@ int mm3fa_kv8_read(const mm3fa_kv8 * cache, int layer, const mm3fa_kv8_table * t
 }
 
 size_t mm3fa_kv8_attn_workspace(const mm3fa_kv8 * cache, const mm3fa_tensor * q, const mm3fa_kv8_table * table) {
-    if (!q || check_cache(cache) != MM3FA_OK || check_table(cache, table) != MM3FA_OK || q->ne[1] < 1 || q->ne[2] < 1 ||
+    if (!q || check_cache(cache) != MM3FA_OK || check_table(cache, table) != MM3FA_OK || !attn_tokens_fit(cache, table) || q->ne[1] < 1 || q->ne[2] < 1 ||
         q->ne[2] % cache->n_head_kv || q->ne[1] > (1 << 24) || q->ne[2] > (1 << 20) ||
         q->ne[2] / cache->n_head_kv * q->ne[1] > (1 << 24)) {
         return 0;
@@ -317,7 +322,7 @@ int mm3fa_kv8_attn(const mm3fa_kv8 * cache, int layer, const mm3fa_tensor * q, c
     }
     // rows of a kv head, and 32-key blocks of all rows at the table's full length, are counted in 32 bits
     const int64_t rows = H / cache->n_head_kv * q->ne[1];
-    if (q->ne[1] > (1 << 24) || H > (1 << 20) || rows > (1 << 24) || rows * (H / cache->n_head_kv) > INT32_MAX ||
+    if (!attn_tokens_fit(cache, table) || q->ne[1] > (1 << 24) || H > (1 << 20) || rows > (1 << 24) || rows * (H / cache->n_head_kv) > INT32_MAX ||
         ((rows + 15) / 16) * cache->n_head_kv * table->n_seq > (int64_t) INT32_MAX / (((int64_t) table->max_pages * cache->page_tokens + 31) / 32)) {
         return MM3FA_ERR_UNSUPPORTED;
     }

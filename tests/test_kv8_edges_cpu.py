@@ -51,3 +51,16 @@ def test_a_given_workspace_is_checked():
     with pytest.raises(mm3fa.MM3FAError) as e:
         c.attend(0, q, s.table, s.len, 0.1, out, ws=torch.zeros(1 << 22, dtype=torch.uint8)[::2])
     assert e.value.status == mm3fa.ERR_STRIDE
+
+
+@no_gpu
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+def test_a_table_whose_token_positions_leave_32_bits(P):
+    """The attention rounds token counts up to its tiles in 32 bits: tables that near to 2^31 tokens are refused."""
+    f, at = kv8._calls(), 1 << 20
+    c = kv8._CACHE.pack(64, P, 1, 9, 1, 0, at, at, at, at)
+    q = kv8._PACK_TENSOR(0, 0, 64, 1, 1, 1, 4, 256, 256, 256, at)
+    for tokens, want in ((2 ** 31 - 8192, mm3fa.ERR_DEVICE), (2 ** 31 - 8192 + P, mm3fa.ERR_UNSUPPORTED), (2 ** 31 - P, mm3fa.ERR_UNSUPPORTED)):
+        t = kv8._PACK_TABLE(at, tokens // P, tokens // P, 1)
+        assert f["attn"](c, 0, q, t, at, None, 1.0, 0.0, 1, q, at, 1 << 40, None) == want
+        assert (f["attn_workspace"](c, q, t) == 0) == (want == mm3fa.ERR_UNSUPPORTED)
