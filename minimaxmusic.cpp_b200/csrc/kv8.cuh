@@ -132,7 +132,8 @@ __device__ __forceinline__ int kv8_page(const Kv8Table & t, int n_pages, int s, 
 // ------------------------------------------------------------------ host helpers
 
 // Launches with programmatic stream serialisation (MM3FA_PDL=0 turns it off): the CTAs may start
-// once the previous kernel's have exited; every kernel here starts with griddepcontrol.wait.
+// once the previous kernel's have exited or have let their dependents go (the peer wait does so at its entry);
+// every kernel here waits with griddepcontrol.wait, for that kernel's end, before it reads anything or takes a time.
 template <typename... KArgs, typename... Args>
 cudaError_t kv8_launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
     static const bool pdl = [] {

@@ -168,9 +168,9 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem     = *tmem_slot;
-    const uint64_t deadline = global_timer_ns() + p.timeout_ns;
+    const uint32_t tmem = *tmem_slot;
     kv8_dep_wait();
+    const uint64_t deadline = global_timer_ns() + p.timeout_ns;  // the time of the kernel before is not this one's
 
     // ---- the work item: row blocks last first, so that the longest causal ones start first
     const int hs = p.c.n_head_kv * p.t.n_seq, all_rows = p.ratio * p.n_q;

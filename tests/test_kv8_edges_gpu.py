@@ -36,3 +36,44 @@ def test_attend_nan_in_a_row_that_sees_no_key(cuda_device, D, G, n_q, n0, dtype,
         assert got[0, hidden:, 1].isnan().all()
         got[0, hidden:, 1] = want[0, hidden:, 1]
         assert torch.equal(got, want)
+
+
+def test_wait_limit_starts_after_the_previous_kernel(cuda_device, tmp_path):
+    """The bounded waits of the many-row kernel count from its own start.  It is launched behind a peer wait, which lets its
+    successor launch at once and then runs to its own limit: that time is not the attention's.  In a process of its own,
+    with a limit of 1 ms."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = f"""
+import ctypes, sys
+sys.path[:0] = [{here!r}, {os.path.join(os.path.dirname(here), "minimaxmusic.cpp_b200")!r}]
+import torch
+import kv8_ref as R
+import mm3fa
+from mm3fa import ggml
+dev = torch.device("cuda", 0)
+st = R.State([4000] * 8, 4, 128, 64, seed=31, device=dev)
+c, q = st.cache(), st.randn(8, 8, 512, 128)
+want = c.attend(0, q, st.table, st.len, 0.1, logit_softcap=5.0).clone()
+c.check()
+recv, epochs, ws = (torch.zeros(n, dtype=torch.uint8, device=dev) for n in (1 << 20, 256, 1 << 16))
+res = torch.zeros(1, 1, 4, 128, device=dev)
+peers = mm3fa.Peers()
+peers.n_ranks, peers.rank, peers.recv_slot_bytes = 2, 0, 1 << 20
+peers.recv[0] = peers.recv[1] = recv.data_ptr()
+s = torch.cuda.current_stream().cuda_stream
+for _ in range(20):
+    out = torch.zeros_like(want)
+    mm3fa.peer_wait(peers, 0, epochs.data_ptr(), ggml.make(ggml.GGML_TYPE_F32, [128, 4, 1, 1], res.data_ptr()), ws.data_ptr(), s)
+    c.attend(0, q, st.table, st.len, 0.1, out=out, logit_softcap=5.0)
+    c.check()
+    assert torch.equal(out, want)
+    assert mm3fa.workspace_status(ws.data_ptr(), s)[0] == mm3fa.ERR_TIMEOUT  # the peer's words never come
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "MM3FA_WAIT_TIMEOUT_MS": "1"}, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stdout + r.stderr
