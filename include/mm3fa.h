@@ -193,6 +193,12 @@ MM3FA_API int mm3fa_supports(const mm3fa_tensor * q, const mm3fa_tensor * k, con
 MM3FA_API int mm3fa_workspace_status(void * workspace, void * stream, uint32_t * status_out);
 
 /*
+ * A number that differs from capture to capture while `stream` is being captured into a graph; 0 otherwise.
+ * (A workspace that a captured call zeroes belongs to that graph: no eager call and no other graph may share it.)
+ */
+MM3FA_API uint64_t mm3fa_capture_id(void * stream);
+
+/*
  * Diagnostics: launches one CTA that waits on an mbarrier nothing arrives on, bounded by
  * timeout_us, and records the expiry in the workspace status word exactly as the attention
  * kernels do.  Lets tests check the timeout path without faulting or hanging the GPU.
@@ -468,7 +474,10 @@ MM3FA_API int mm3fa_ipc_close(void * dev_ptr);
  * page that entry j of its table row names, the same page in every layer; an entry outside
  * [0, n_pages) names none: its keys are absent from the attention, its rows are neither stored nor
  * read.  refs[page] counts the table entries that name a page; 0 is a free page.
- * Table, lengths and counts are device memory, so that a step can be captured and replayed.
+ * Table, lengths and counts are device memory, so that a step can be captured and replayed.  A workspace that the
+ * graph itself zeroes would lose at each replay what the one before found: bytes 16 to 23 of an attention's or page
+ * operation's workspace may hold the device address of a second status word (two uint32, read and cleared by
+ * mm3fa_workspace_status), in which the same bits are set; 0: none.
  * No counterpart in the reference, whose cache is one F16 slab per set (src/qwen3-lm.h:215-267).
  * ------------------------------------------------------------------------------------------ */
 typedef struct mm3fa_kv8 {

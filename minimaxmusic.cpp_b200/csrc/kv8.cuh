@@ -79,6 +79,10 @@ struct Kv8PoolCopy {
 
 constexpr size_t KV8_WS_ZEROED = 1 << 16;  // bytes of a workspace that a caller zeroes: none is smaller
 
+// Words of a workspace that may hold the address of a second status word (0: none): a graph that zeroes its workspace at
+// every replay leaves there what its calls found.
+constexpr int KV8_WS_ALSO = 4;
+
 // Workspace of the page operations (int32 words from its base; 64 words of status and counts first).
 constexpr int KV8_WS_COPIES = 32;  // page copies that the plan wants done
 constexpr int KV8_WS_FAILED = 33;  // nonzero: too few pages, nothing changes
@@ -127,6 +131,15 @@ __device__ __forceinline__ int kv8_page(const Kv8Table & t, int n_pages, int s, 
     }
     const int p = t.pages[(int64_t) s * t.stride + j];
     return (unsigned) p < (unsigned) n_pages ? p : -1;
+}
+
+// Sets a bit of the workspace's status, and of the second status word where there is one.
+__device__ __forceinline__ void kv8_report(uint32_t * status, uint32_t bit) {
+    atomicOr(status, bit);
+    const uint64_t also = status[KV8_WS_ALSO] | (uint64_t) status[KV8_WS_ALSO + 1] << 32;  // (the workspace may be 4-byte aligned)
+    if (also) {
+        atomicOr(reinterpret_cast<uint32_t *>(also), bit);
+    }
 }
 
 // ------------------------------------------------------------------ host helpers

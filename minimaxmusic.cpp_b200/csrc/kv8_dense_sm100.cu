@@ -1003,7 +1003,7 @@ __global__ void __launch_bounds__(KE_THREADS, 1) kv8_dense_kernel(const Kv8AttnP
         tmem_dealloc(tmem, KE_TMEM);
     }
     if (tid == 0 && *abort_f) {
-        atomicOr(&p.status[0], ST_TIMEOUT);
+        kv8_report(p.status, ST_TIMEOUT);
         atomicExch(&p.status[1], blockIdx.x);
     }
 }

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_fork_plan_kernel(const Kv8Pl
         p.head[KV8_WS_COPIES] = failed ? 0 : total;
         p.head[KV8_WS_FAILED] = failed;
         if (failed) {
-            atomicOr(p.status, ST_PAGES);
+            kv8_report(p.status, ST_PAGES);
         }
     }
     if (failed) {
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv8_reserve_kernel(const Kv8Plan
     __syncthreads();
     if (found < total || over) {
         if (tid == 0) {
-            atomicOr(p.status, ST_PAGES);
+            kv8_report(p.status, ST_PAGES);
         }
         return;
     }

@@ -1125,6 +1125,16 @@ int mm3fa_workspace_status(void * workspace, void * stream, uint32_t * status_ou
     return MM3FA_OK;
 }
 
+uint64_t mm3fa_capture_id(void * stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long      id     = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? (uint64_t) id + 1 : 0;
+}
+
 int mm3fa_selftest_bounded_wait(void * workspace, uint32_t timeout_us, void * stream) {
     if (!workspace) {
         return MM3FA_ERR_NULL;

@@ -26,6 +26,7 @@ _PACK_TABLE = struct.Struct("@Pq2i").pack       # struct mm3fa_kv8_table
 _PACK_TENSOR = struct.Struct("@2i4q4QP").pack   # struct mm3fa_tensor
 
 _ZEROED = 1 << 16  # bytes of a workspace that have to be zero before its first use
+_ALSO = slice(16, 24)  # of a workspace: address of a second status word
 
 _fns = None
 
@@ -50,8 +51,26 @@ def _calls():
             fn = getattr(L, "mm3fa_kv8_" + name)
             fn.restype, fn.argtypes = res, args
             fns[name] = fn
+        fns["capture_id"] = fn = L.mm3fa_capture_id
+        fn.restype, fn.argtypes = ctypes.c_uint64, [vp]
         _fns = fns
     return _fns
+
+
+_STATUS_SLOTS = 1 << 16
+_status_words = {}  # device -> [int32 [_STATUS_SLOTS, 4], slots given out]
+
+
+def _status_memory(device):
+    """Status words for calls of graphs, of which a graph keeps the address: never freed, and none given out twice (but in
+    turn when all have been)."""
+    import torch
+
+    if device not in _status_words:
+        _status_words[device] = [torch.zeros(_STATUS_SLOTS, 4, dtype=torch.int32, device=device), 0]
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()  # zero for every stream
+    return _status_words[device]
 
 
 def _types():
@@ -85,8 +104,12 @@ class Kv8Cache:
         self._dev = k.get_device()  # -1: host tensors, on which the C ABI's checks run but no kernel does
         self._fns = None
         self._ws = {}    # (operation, stream) -> address and bytes of a zero-filled workspace
-        self._kept = []  # the workspaces, outgrown ones too: a captured graph may still use them
+        self._kept = []  # these, outgrown ones too: their status has not been read
         self._need = {}  # workspace bytes by shape
+        self._capture = None  # the last capture, and its workspaces by (operation, stream)
+        self._is_capturing, self._current_device = torch._C._cuda_isCurrentStreamCapturing, torch._C._cuda_getDevice
+        self._found = {}  # (operation, stream), or None: the status of calls of graphs
+        self._status = None if self._dev < 0 else _status_memory(self.device)
 
     @classmethod
     def allocate(cls, n_layers: int, n_pages: int, n_head_kv: int, page_tokens: int, head_dim: int, device="cuda"):
@@ -172,22 +195,50 @@ class Kv8Cache:
 
     def _workspace(self, key, nbytes):
         """(address, bytes) of the workspace of an operation on a stream, zero-filled as far as it has to be when it is made."""
+        # the current stream is key's where the current device is the cache's
+        if self._dev >= 0 and (self._is_capturing() or self._current_device() != self._dev):
+            capture = self._call("capture_id", key[1])
+            if capture:
+                return self._workspace_of_graph(capture, key, nbytes)
+        if self._capture:
+            self._capture = None
         buf = self._ws.get(key)
         if buf is not None and buf[1] >= nbytes:
             return buf
-        torch = self._torch
         if nbytes > 0:
-            made = torch.empty(max(nbytes, _ZEROED), dtype=torch.uint8, device=self.device)
-            made[:_ZEROED].zero_()
-            at = made.data_ptr(), made.numel()
-            # one made during a capture is zeroed by each replay of the graph: nothing else may use it, or read it before
-            if self._dev >= 0 and torch.cuda.is_current_stream_capturing():
-                key = None
-            else:
-                self._ws[key] = at
+            made = self._made(nbytes)
+            self._ws[key] = at = made.data_ptr(), made.numel()
             self._kept.append((key, made))
             return at
         return None, 0
+
+    def _made(self, nbytes):
+        made = self._torch.empty(max(nbytes, _ZEROED), dtype=self._torch.uint8, device=self.device)
+        made[:_ZEROED].zero_()
+        return made
+
+    def _workspace_of_graph(self, capture, key, nbytes):
+        """A workspace that a graph zeroes when it is replayed: one for all calls of an operation that a stream of the
+        capture makes, shared with nothing else.  It lives in the graph's memory, like all that is allocated in a
+        capture; this class lets it go at its next call elsewhere (one that the capture makes later is zeroed in turn).
+        What the calls find goes to a status word of the stream where it has a workspace, else to one of the cache."""
+        if self._capture is None or self._capture[0] != capture:
+            self._capture = capture, {}
+        made = self._capture[1].get(key)
+        if made is None or made.numel() < nbytes:
+            if nbytes <= 0:
+                return None, 0
+            made = self._capture[1][key] = self._made(nbytes)
+            made[_ALSO].view(self._torch.int64).fill_(self._status_word(key if key in self._ws else None).data_ptr())
+        return made.data_ptr(), made.numel()
+
+    def _status_word(self, key):
+        word = self._found.get(key)
+        if word is None:
+            words, n = self._status
+            self._status[1] = n + 1
+            word = self._found[key] = words[n % _STATUS_SLOTS]
+        return word
 
     def _given(self, ws):
         """(address, bytes) of a caller's workspace."""
@@ -226,7 +277,7 @@ class Kv8Cache:
         """softmax(scale * q k^T) v of the queries q (N, n_head, n_q, D) over the first kv_len[s] tokens of each
         sequence; causal: the rows are the last tokens.  out: (N, n_q, n_head, D), F32 or q's type; made in
         q's type when not given, with zeros in the rows behind q_len.  ws: a uint8 tensor, its
-        first 64 KiB zero, instead of the cache's own workspace of the stream, for graphs that may run at the same time."""
+        first 64 KiB zero, instead of the cache's own workspace of the stream; it serves one stream at a time."""
         if stream is not None:  # what is allocated here belongs to that stream too
             with self._on(stream):
                 return self.attend(layer, q, table, kv_len, scale, out, q_len, causal, logit_softcap, ws)
@@ -252,59 +303,67 @@ class Kv8Cache:
         """Bytes of the workspace that `attend` needs for these operands."""
         return self._call("attn_workspace", self._desc, self._rows(q), self._table(table))
 
-    def _pages_ws(self, n_seq, stream):
+    def _pages_ws(self, n_seq, stream, ws=None):
+        if ws is not None:
+            return self._given(ws)
         need = self._need.get(n_seq)
         if need is None:
             need = self._need[n_seq] = self._call("pages_workspace", self._desc, n_seq)
         return self._workspace(("pages", stream), need)
 
-    def reserve(self, table, refs, n_tok, stream=None):
-        """Gives each sequence's row of `table` the pages for n_tok[s] tokens (in place)."""
+    def pages_workspace(self, n_seq) -> int:
+        """Bytes of the workspace that `reserve`, `fork`, `free` and `compact` need for n_seq sequences."""
+        return self._call("pages_workspace", self._desc, n_seq)
+
+    def reserve(self, table, refs, n_tok, stream=None, ws=None):
+        """Gives each sequence's row of `table` the pages for n_tok[s] tokens (in place).  ws: as for `attend`."""
         if stream is not None:
             with self._on(stream):
-                return self.reserve(table, refs, n_tok)
+                return self.reserve(table, refs, n_tok, ws=ws)
         st, n = self._stream(), table.shape[0]
         self._run("reserve", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
-                   self._ints(n_tok, n, "n_tok"), *self._pages_ws(n, st), st)
+                   self._ints(n_tok, n, "n_tok"), *self._pages_ws(n, st, ws), st)
 
-    def fork(self, src, dst, table, kv_len, refs, table_out, kv_len_out, refs_out, deep=False, stream=None):
+    def fork(self, src, dst, table, kv_len, refs, table_out, kv_len_out, refs_out, deep=False, stream=None, ws=None):
         """Sequence dst[i] becomes a copy of sequence src[i] (-1, or src None: empty); full pages are shared unless
-        `deep`.  The results go to the *_out tensors, which may not overlap the others."""
+        `deep`.  The results go to the *_out tensors, which may not overlap the others.  ws: as for `attend`."""
         if stream is not None:
             with self._on(stream):
-                return self.fork(src, dst, table, kv_len, refs, table_out, kv_len_out, refs_out, deep)
+                return self.fork(src, dst, table, kv_len, refs, table_out, kv_len_out, refs_out, deep, ws=ws)
         st, n = self._stream(), table.shape[0]
         pairs = dst.shape[0]
         self._run("fork", self._desc, self._table(table), self._ints(kv_len, n, "kv_len"),
                    self._ints(refs, self.n_pages, "refs"), None if src is None else self._ints(src, pairs, "src"),
                    self._ints(dst, pairs, "dst"), pairs, FORK_DEEP if deep else 0, self._table(table_out),
                    self._ints(kv_len_out, n, "kv_len_out"), self._ints(refs_out, self.n_pages, "refs_out"),
-                   *self._pages_ws(n, st), st)
+                   *self._pages_ws(n, st, ws), st)
 
-    def free(self, seqs, table, kv_len, refs, table_out, kv_len_out, refs_out, stream=None):
+    def free(self, seqs, table, kv_len, refs, table_out, kv_len_out, refs_out, stream=None, ws=None):
         """Empties the sequences `seqs` (int32 [n]): `fork` from nothing."""
-        self.fork(None, seqs, table, kv_len, refs, table_out, kv_len_out, refs_out, stream=stream)
+        self.fork(None, seqs, table, kv_len, refs, table_out, kv_len_out, refs_out, stream=stream, ws=ws)
 
-    def compact(self, table, refs, table_out, refs_out, stream=None):
-        """Moves the live pages to the front of the pool; the results go to the *_out tensors."""
+    def compact(self, table, refs, table_out, refs_out, stream=None, ws=None):
+        """Moves the live pages to the front of the pool; the results go to the *_out tensors.  ws: as for `attend`."""
         if stream is not None:
             with self._on(stream):
-                return self.compact(table, refs, table_out, refs_out)
+                return self.compact(table, refs, table_out, refs_out, ws=ws)
         st, n = self._stream(), table.shape[0]
         self._run("compact", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
-                   self._table(table_out), self._ints(refs_out, self.n_pages, "refs_out"), *self._pages_ws(n, st), st)
+                   self._table(table_out), self._ints(refs_out, self.n_pages, "refs_out"), *self._pages_ws(n, st, ws), st)
 
-    def check(self, stream=None):
+    def check(self, stream=None, captured=False, ws=None):
         """Synchronises the stream and raises MM3FAError where a page operation on it found too few free pages
-        (ERR_PAGES) or a bounded device wait of an attention expired (ERR_TIMEOUT).  Captured calls are among them where an
-        earlier call on the stream had made their workspace; otherwise the graph has one of its own, which is not read."""
+        (ERR_PAGES) or a bounded device wait of an attention expired (ERR_TIMEOUT).  Calls that a graph replays are among
+        them where an earlier call on the stream of the capture had made its workspace; captured=True: those of all
+        graphs (wait for the streams that replay them first).  ws: a workspace that calls were given."""
         if stream is not None:
             with self._on(stream):
-                return self.check()
+                return self.check(captured=captured, ws=ws)
         st = self._stream()
-        for op in ("pages", "attn"):
-            for key, buf in self._kept:  # a call before the workspace grew may have left its status in an older one
-                if key == (op, st):
-                    status, _ = workspace_status(buf.data_ptr(), st)
-                    if status != OK:
-                        raise MM3FAError(status, "Kv8Cache")
+        bufs = [buf for key, buf in self._kept if key[1] == st]  # outgrown ones too
+        bufs += [word for key, word in self._found.items() if captured or (key and key[1] == st)]
+        bufs += [ws] if ws is not None else []
+        for buf in bufs:
+            status, _ = workspace_status(buf.data_ptr(), st)
+            if status != OK:
+                raise MM3FAError(status, "Kv8Cache")

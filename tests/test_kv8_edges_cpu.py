@@ -64,3 +64,29 @@ def test_a_table_whose_token_positions_leave_32_bits(P):
         t = kv8._PACK_TABLE(at, tokens // P, tokens // P, 1)
         assert f["attn"](c, 0, q, t, at, None, 1.0, 0.0, 1, q, at, 1 << 40, None) == want
         assert (f["attn_workspace"](c, q, t) == 0) == (want == mm3fa.ERR_UNSUPPORTED)
+
+
+@no_gpu
+def test_a_given_workspace_of_page_operations_is_checked():
+    s = make()
+    c = s.cache()
+    t2, l2, r2 = torch.empty_like(s.table), torch.empty_like(s.len), torch.empty_like(s.refs)
+    one = torch.tensor([0], dtype=torch.int32)
+    calls = (lambda ws: c.reserve(s.table, s.refs, s.len, ws=ws), lambda ws: c.compact(s.table, s.refs, t2, r2, ws=ws),
+             lambda ws: c.fork(one, one, s.table, s.len, s.refs, t2, l2, r2, ws=ws),
+             lambda ws: c.free(one, s.table, s.len, s.refs, t2, l2, r2, ws=ws))
+    need = c.pages_workspace(2)
+    for f in calls:
+        for ws, want in ((torch.zeros(need, dtype=torch.uint8), mm3fa.ERR_DEVICE), (torch.zeros(need - 1, dtype=torch.uint8), mm3fa.ERR_WORKSPACE),
+                         (torch.zeros(need + 8, dtype=torch.uint8)[2:], mm3fa.ERR_WORKSPACE),
+                         (torch.zeros(2 * need, dtype=torch.uint8)[::2], mm3fa.ERR_STRIDE)):
+            with pytest.raises(mm3fa.MM3FAError) as e:
+                f(ws)
+            assert e.value.status == want
+        with pytest.raises(ValueError):
+            f(Elsewhere())
+
+
+@no_gpu
+def test_no_capture_without_a_device():
+    assert kv8._calls()["capture_id"](None) == 0

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import kv8_ref as R
+import mm3fa
 from test_kv8_gpu import DTYPES, many
 
 pytestmark = pytest.mark.gpu
@@ -53,6 +54,7 @@ sys.path[:0] = [{here!r}, {os.path.join(os.path.dirname(here), "minimaxmusic.cpp
 import torch
 import kv8_ref as R
 import mm3fa
+import mm3fa
 from mm3fa import ggml
 dev = torch.device("cuda", 0)
 st = R.State([4000] * 8, 4, 128, 64, seed=31, device=dev)
@@ -77,3 +79,161 @@ print("done")
     r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "MM3FA_WAIT_TIMEOUT_MS": "1"}, capture_output=True,
                        text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stdout + r.stderr
+
+
+# ---------------------------------------------------------------- graphs
+
+def small_cache(dev, n_pages=6, n_free=0):
+    """A cache of n_pages pages of which n_free are free, and a table of one sequence without any."""
+    c = mm3fa.Kv8Cache.allocate(3, n_pages, 2, 16, 64, dev)
+    refs = torch.ones(n_pages, dtype=torch.int32, device=dev)
+    refs[:n_free] = 0
+    return c, refs, torch.full((1, 4), -1, dtype=torch.int32, device=dev)
+
+
+def captured(fn, stream=None):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        fn()
+    return g
+
+
+def test_captured_calls_share_a_workspace_that_goes_with_the_graph(cuda_device):
+    """36 attentions of one capture hold one workspace, and none when the graph is gone."""
+    st = R.State([500, 1200], 4, 128, 64, seed=32, device=cuda_device)
+    c, q = st.cache(), st.randn(2, 16, 1, 128)
+    outs = torch.zeros(36, 2, 1, 16, 128, device=cuda_device)
+    want = c.attend(0, q, st.table, st.len, 0.1).clone()
+    need = c.attend_workspace(q, st.table)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    g = captured(lambda: [c.attend(0, q, st.table, st.len, 0.1, out=o) for o in outs])
+    assert torch.cuda.memory_allocated() - before <= 2 * need
+    for _ in range(2):
+        outs.zero_()
+        g.replay()
+        assert all(torch.equal(o, want) for o in outs)
+    del g
+    c.attend(0, q, st.table, st.len, 0.1)  # lets go of the capture
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+
+
+def test_captured_calls_that_outgrow_their_workspace(cuda_device):
+    """Calls of growing and of alternating shapes in one capture, with other allocations between them."""
+    sts = [R.State([9000, 700], 8, D, 64, seed=D, device=cuda_device) for D in (64, 128)]
+    shapes = [(st, n_q) for n_q in (1, 40, 2) for st in sts]
+    qs = [st.randn(2, 16, n_q, st.D) for st, n_q in shapes]
+    caches = [st.cache() for st in sts]
+    want = [caches[i % 2].attend(0, q, st.table, st.len, 0.1).clone() for i, ((st, _), q) in enumerate(zip(shapes, qs))]
+    got = []
+
+    def calls():
+        for i, ((st, _), q) in enumerate(zip(shapes, qs)):
+            got.append(caches[i % 2].attend(0, q, st.table, st.len, 0.1))
+            got.append(torch.full((1 << 20,), 255, dtype=torch.uint8, device=cuda_device))
+
+    g = captured(calls)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got[::2], want))
+
+
+def test_a_replayed_call_without_pages_is_reported(cuda_device):
+    """check(captured=True) raises for it, though replays that found pages came after it, and only once; the default
+    reads what streams of the program's own have found."""
+    c, refs, table = small_cache(cuda_device)
+    n_tok = torch.ones(1, dtype=torch.int32, device=cuda_device)
+    g = captured(lambda: c.reserve(table, refs, n_tok))
+    c.check(captured=True)  # nothing has run
+    g.replay()
+    refs[3] = 0
+    g.replay()
+    assert int(table[0, 0]) == 3
+    torch.cuda.synchronize()
+    with pytest.raises(mm3fa.MM3FAError) as e:
+        c.check(captured=True)
+    assert e.value.status == mm3fa.ERR_PAGES
+    c.check(captured=True)
+    table.fill_(-1)
+    g.replay()  # no page again
+    torch.cuda.synchronize()
+    with pytest.raises(mm3fa.MM3FAError):
+        c.check(captured=True)
+    other, _, _ = small_cache(cuda_device)
+    g.replay()
+    torch.cuda.synchronize()
+    other.check(captured=True)  # another cache's status is its own
+
+
+def test_a_replayed_fork_without_pages_is_reported(cuda_device):
+    c, refs, table = small_cache(cuda_device)
+    table = torch.tensor([[0, -1], [-1, -1]], dtype=torch.int32, device=cuda_device)
+    n = torch.tensor([5, 0], dtype=torch.int32, device=cuda_device)
+    pair = [torch.tensor([i], dtype=torch.int32, device=cuda_device) for i in (0, 1)]
+    outs = [torch.empty_like(t) for t in (table, n, refs)]
+    g = captured(lambda: c.fork(*pair, table, n, refs, *outs))
+    g.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(mm3fa.MM3FAError) as e:
+        c.check(captured=True)
+    assert e.value.status == mm3fa.ERR_PAGES
+    assert torch.equal(outs[0], table)
+
+
+def test_graphs_of_one_stream_at_the_same_time(cuda_device):
+    """Two graphs captured on a stream that has a workspace, replayed on two streams while a third makes eager calls: none
+    shares a workspace with another."""
+    st = R.State([3000, 5000], 4, 128, 64, seed=33, device=cuda_device)
+    c = st.cache()
+    qs = [st.randn(2, 16, n_q, 128) for n_q in (1, 3, 2)]
+    side = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side[0]):
+        want = [c.attend(0, q, st.table, st.len, 0.1).clone() for q in qs]
+    torch.cuda.synchronize()
+    outs = [[torch.empty_like(w) for _ in range(8)] for w in want]
+    graphs = [captured(lambda: [c.attend(0, q, st.table, st.len, 0.1, out=o) for o in os], side[0]) for q, os in zip(qs, outs[:2])]
+    for _ in range(20):
+        for g, s in zip(graphs, side[1:]):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(side[0]):
+            for o in outs[2]:
+                c.attend(0, qs[2], st.table, st.len, 0.1, out=o)
+    torch.cuda.synchronize()
+    for w, os in zip(want, outs):
+        assert all(torch.equal(o, w) for o in os)
+
+
+def test_a_workspace_for_page_operations(cuda_device):
+    """reserve, fork, free and compact with a workspace of the caller's, eager and captured; check reads it."""
+    c, refs, table = small_cache(cuda_device, n_free=2)
+    ws = torch.zeros(c.pages_workspace(1), dtype=torch.uint8, device=cuda_device)
+    ws[1 << 16:] = 255
+    n_tok = torch.full((1,), 17, dtype=torch.int32, device=cuda_device)
+    c.reserve(table, refs, n_tok, ws=ws)
+    c.check(ws=ws)
+    assert table.tolist() == [[0, 1, -1, -1]]
+    outs = [torch.empty_like(t) for t in (table, n_tok, refs)]
+    zero = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    c.free(zero, table, n_tok, refs, *outs, ws=ws)
+    assert outs[0].tolist() == [[-1] * 4] and outs[2].tolist() == [0, 0, 1, 1, 1, 1]
+    t2, r2 = torch.empty_like(table), torch.empty_like(refs)
+    c.compact(outs[0], outs[2], t2, r2, ws=ws)
+    assert r2.tolist() == [1, 1, 1, 1, 0, 0]
+    refs.fill_(1)
+    table.fill_(-1)
+    torch.cuda.synchronize()
+    g = captured(lambda: c.reserve(table, refs, n_tok, ws=ws))
+    g.replay()
+    torch.cuda.synchronize()
+    c.check(captured=True)
+    with pytest.raises(mm3fa.MM3FAError) as e:
+        c.check(ws=ws)
+    assert e.value.status == mm3fa.ERR_PAGES
+    c.check(ws=ws)
+    for bad in (ws.cpu(), ):
+        with pytest.raises(ValueError):
+            c.reserve(table, refs, n_tok, ws=bad)
