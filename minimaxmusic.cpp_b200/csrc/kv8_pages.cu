@@ -9,7 +9,8 @@
 //
 // The plan is latency: one CTA, since every rank needs the counts before it (9 to 10 us with the copy, for 16
 // sequences of up to 700 tokens).  The copy is memory: deep copies of 3 of 8 sequences of 900 to 2500 tokens in 36 layers
-// (0.77 GB read and written) take 155 us, 76 % of the copy bandwidth of 6.54 TB/s; moving half of a pool of such 88, 79 %.
+// (0.77 GB read and written) take 155 us, 76 % of the copy bandwidth of 6.54 TB/s, in a graph over three caches in turn, and 124 to
+// 141 as calls on one; moving half of a pool of such 88, 79 %.
 //
 // A call that finds too few free pages changes nothing and leaves a bit in the workspace's status.
 #include "kv8.cuh"
