@@ -8,12 +8,15 @@
 //     than 2^-30 of the row's largest; F32 ones down to 2^-6 of it, F16 ones to 2^-19 and BF16 ones to 2^-22 are exact.
 //     (With three digits for F32 and two for 16-bit results the small elements beside a large one decided wrongly: one of
 //     1000 among N(0, 1), with keys of 0 there, put F16 results 5 half steps off.  48 sequences of up to 10240 tokens
-//     took 105 us in BF16 so, 115 now; F32 118 and 119.)
+//     took 105 us in BF16 so, 115 now; F32 118 and 120.)
 //   * P . c in F16, which holds the codes exactly.  The value scale of a page goes into the weights,
 //     P = 2^(s - m) * 2^(m + e - R) * f with b = f 2^e, f in [1, 2), and R the running maximum of (a tile's
 //     largest s) + e: O is held in units of 2^R, the sum in units of 2^m, so that pages with scales of
 //     any size stay in F16's range.  Weights are rounded to F16 (half a step: 2^-12), which
 //     is below what a BF16 result keeps; for F32 and F16 results their remainder is a second operand.  O, sums and maxima are F32.
+//     The tensor core truncates what it adds to an F32 accumulator, always towards zero: 4e-10 of the result a key (3.4e-6
+//     over 8000).  For an F32 result, and for 16-bit ones of tables over KD_LONG tokens, it sums the keys of a block from 0, and
+//     O takes the sums by additions that round (1e-7 over 8000; 48 sequences of up to 10240, F32: 123 us against 120).
 //
 // Work.  A unit is (sequence, kv head, 16 query rows): rows of all query heads of the group share the
 // cache's bytes.  A unit's keys come in blocks of 32.  Every CTA finds its work from the lengths on the
@@ -39,6 +42,7 @@
 // 57 us).  Two stages for three CTAs of an SM against three stages for two, D = 128, one row per head:
 // 116 us against 129 for the 48 sequences, 20.4 against 19.4 for the two.
 #include "kv8.cuh"
+#include "tc_sm100.cuh"
 
 #include <algorithm>
 
@@ -56,6 +60,10 @@ constexpr int KD_PART    = 4;
 // What a crossing costs, in blocks.  0, 8, 32: 24.8, 19.8, 20.4 us for 2 sequences of 8192 (0: flat), 40.1, 40.1, 39.0
 // for 16 of 4096 (32: parts).  Whole against flat: 29.5 against 35.8 us for 50 of 1000, 92.6 against 101.4 for 110 of 2000.
 constexpr int KD_CROSS   = 32;
+
+// Tokens up to which sums in the tensor core's truncating accumulators (4e-10 of the result a key) stay an eighth of F16's
+// half step.
+constexpr int KD_LONG    = 65536;
 
 constexpr int KD_SM_BYTES  = 228 * 1024;  // shared memory of an SM
 constexpr int KD_CTA_BYTES = 1024;        // what each CTA on it takes beside its own
@@ -202,8 +210,8 @@ struct KdPart {
     int s, u, c0, n;
 };
 
-// HP: an F32 result; PL: the remainders of the weights too
-template <int D, int NT, bool HP, bool PL, bool CAP>
+// FS: each block's products summed from 0 (with PL); PL: the remainders of the weights too
+template <int D, int NT, bool FS, bool PL, bool CAP>
 __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT>::CTAS) kv8_decode_kernel(const Kv8AttnParams p) {
     using L          = KdSmem<D, NT>;
     constexpr int NS = L::NS, ND = L::ND, CH = D / 64, MT = D / 16, E = D / 32, QR = NT * 8 / KD_WARPS;
@@ -414,7 +422,7 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT>::CTAS) kv8_decode_ke
         char * dst = p.o.data + (int64_t) hq * p.o.nb1 + (int64_t) qi * p.o.nb2 + (int64_t) s * p.o.nb3;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
-            if (HP) {
+            if (p.o.type == KV_F32) {
                 float * f = reinterpret_cast<float *>(dst) + lane * E + e;
                 if (p.o.vec) {
                     *reinterpret_cast<float2 *>(f) = make_float2(v[e], v[e + 1]);
@@ -691,37 +699,58 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT>::CTAS) kv8_decode_ke
                 }
             }
             // O^T += V^T P^T: dims of chunk g (two per row pair of an MMA), keys 2t, 2t + 1, 2t + 8, 2t + 9
+            // (FS: both halves of the keys side by side, where registers allow)
             const char * vt = st + L::TILE;
+            constexpr int WORDS = D == 64 ? 2 : 4, AV = FS && (D <= 128 || NT == 1) ? 2 : 1;
 #pragma unroll
-            for (int a = 0; a < 2; a++) {
+            for (int a0 = 0; a0 < 2; a0 += AV) {
 #pragma unroll
                 for (int j = 0; j < (D + 127) / 128; j++) {
-                    constexpr int WORDS = D == 64 ? 2 : 4;
-                    uint32_t      w[4][WORDS];
+                    uint32_t w[AV][4][WORDS];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = (16 * a + (i & 1) + 8 * (i >> 1)) * D;  // beyond row 2 t
-                        if (D == 64) {
-                            const uint2 u = *reinterpret_cast<const uint2 *>(vt + r + v_at);
-                            w[i][0] = u.x, w[i][1] = u.y;
-                        } else {
-                            const uint4 u = *reinterpret_cast<const uint4 *>(vt + r + (v_at ^ ((i & 1) << 4)) + 128 * j);
-                            w[i][0] = u.x, w[i][1] = u.y, w[i][WORDS - 2] = u.z, w[i][WORDS - 1] = u.w;
+                    for (int a = 0; a < AV; a++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r = (16 * (a0 + a) + (i & 1) + 8 * (i >> 1)) * D;  // beyond row 2 t
+                            if (D == 64) {
+                                const uint2 u = *reinterpret_cast<const uint2 *>(vt + r + v_at);
+                                w[a][i][0] = u.x, w[a][i][1] = u.y;
+                            } else {
+                                const uint4 u = *reinterpret_cast<const uint4 *>(vt + r + (v_at ^ ((i & 1) << 4)) + 128 * j);
+                                w[a][i][0] = u.x, w[a][i][1] = u.y, w[a][i][WORDS - 2] = u.z, w[a][i][WORDS - 1] = u.w;
+                            }
                         }
                     }
 #pragma unroll
                     for (int k = 0; k < WORDS; k++) {
-                        const uint32_t x0 = w[0][k] ^ 0x80808080u, x1 = w[1][k] ^ 0x80808080u;
-                        const uint32_t x2 = w[2][k] ^ 0x80808080u, x3 = w[3][k] ^ 0x80808080u;
 #pragma unroll
                         for (int q = 0; q < 2; q++) {
-                            const uint32_t y = kd_prmt(x0, x1, q ? 0x7362 : 0x5140), z = kd_prmt(x2, x3, q ? 0x7362 : 0x5140);
-                            const uint32_t f[4] = { kd_half2(y, 0x4140), kd_half2(y, 0x4342), kd_half2(z, 0x4140), kd_half2(z, 0x4342) };
+                            float x[NT][4];
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
-                                kd_mma(o[j * 8 + 2 * k + q][nt], f, ph[a][nt][0], ph[a][nt][1]);
-                                if (PL) {
-                                    kd_mma(o[j * 8 + 2 * k + q][nt], f, pl[a][nt][0], pl[a][nt][1]);
+                                x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.0f;
+                            }
+#pragma unroll
+                            for (int a = 0; a < AV; a++) {
+                                const uint32_t x0 = w[a][0][k] ^ 0x80808080u, x1 = w[a][1][k] ^ 0x80808080u;
+                                const uint32_t x2 = w[a][2][k] ^ 0x80808080u, x3 = w[a][3][k] ^ 0x80808080u;
+                                const uint32_t y = kd_prmt(x0, x1, q ? 0x7362 : 0x5140), z = kd_prmt(x2, x3, q ? 0x7362 : 0x5140);
+                                const uint32_t f[4] = { kd_half2(y, 0x4140), kd_half2(y, 0x4342), kd_half2(z, 0x4140), kd_half2(z, 0x4342) };
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) {
+                                    float(&to)[4] = FS ? x[nt] : o[j * 8 + 2 * k + q][nt];
+                                    if (PL) {
+                                        kd_mma(to, f, pl[a0 + a][nt][0], pl[a0 + a][nt][1]);
+                                    }
+                                    kd_mma(to, f, ph[a0 + a][nt][0], ph[a0 + a][nt][1]);
+                                }
+                            }
+                            if (FS) {
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) {
+                                    float(&to)[4] = o[j * 8 + 2 * k + q][nt];
+                                    f2unpack(fadd2(f2pack(to[0], to[1]), f2pack(x[nt][0], x[nt][1])), to[0], to[1]);
+                                    f2unpack(fadd2(f2pack(to[2], to[3]), f2pack(x[nt][2], x[nt][3])), to[2], to[3]);
                                 }
                             }
                         }
@@ -921,17 +950,18 @@ __global__ void __launch_bounds__(KD_THREADS, KdSmem<D, NT>::CTAS) kv8_decode_ke
 
 namespace {
 
-template <int D, int NT, bool HP, bool PL, bool CAP>
+template <int D, int NT, bool FS, bool PL, bool CAP>
 cudaError_t launch_one(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
     const size_t smem = KdSmem<D, NT>::bytes(rows);
     static Kv8Once once;
-    const cudaError_t e = once.smem(kv8_decode_kernel<D, NT, HP, PL, CAP>, KdSmem<D, NT>::bytes(NT * 8));
-    return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, HP, PL, CAP>, dim3(ctas), KD_THREADS, smem, stream, p);
+    const cudaError_t e = once.smem(kv8_decode_kernel<D, NT, FS, PL, CAP>, KdSmem<D, NT>::bytes(NT * 8));
+    return e != cudaSuccess ? e : kv8_launch(kv8_decode_kernel<D, NT, FS, PL, CAP>, dim3(ctas), KD_THREADS, smem, stream, p);
 }
 
 template <int D, int NT, bool CAP>
 cudaError_t launch_nt(const Kv8AttnParams & p, unsigned ctas, int rows, cudaStream_t stream) {
-    return p.o.type == KV_F32   ? launch_one<D, NT, true, true, CAP>(p, ctas, rows, stream)
+    const bool fresh = p.o.type == KV_F32 || (int64_t) p.t.max_pages * p.c.P > KD_LONG;
+    return fresh                ? launch_one<D, NT, true, true, CAP>(p, ctas, rows, stream)
            : p.o.type == KV_F16 ? launch_one<D, NT, false, true, CAP>(p, ctas, rows, stream)
                                 : launch_one<D, NT, false, false, CAP>(p, ctas, rows, stream);
 }

@@ -68,8 +68,6 @@ def _status_memory(device):
 
     if device not in _status_words:
         _status_words[device] = [torch.zeros(_STATUS_SLOTS, 4, dtype=torch.int32, device=device), 0]
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream(device).synchronize()  # zero for every stream
     return _status_words[device]
 
 
@@ -277,7 +275,8 @@ class Kv8Cache:
         """softmax(scale * q k^T) v of the queries q (N, n_head, n_q, D) over the first kv_len[s] tokens of each
         sequence; causal: the rows are the last tokens.  out: (N, n_q, n_head, D), F32 or q's type; made in
         q's type when not given, with zeros in the rows behind q_len.  ws: a uint8 tensor, its
-        first 64 KiB zero, instead of the cache's own workspace of the stream; it serves one stream at a time."""
+        first 64 KiB zero, instead of the cache's own workspace of the stream; it serves one stream at a time.  (Calls in a
+        capture that torch.cuda.graph has not begun need one: their graph has no memory of its own.)"""
         if stream is not None:  # what is allocated here belongs to that stream too
             with self._on(stream):
                 return self.attend(layer, q, table, kv_len, scale, out, q_len, causal, logit_softcap, ws)

@@ -72,3 +72,28 @@ def test_queries_near_the_smallest_and_largest_numbers(cuda_device, f, dtype, n_
     """Rows that a power of two alone cannot bring to their place, with a scale that brings the scores back."""
     st = R.State([300, 37], 2, 128, 64, seed=12, device=cuda_device)
     run_attend(st, 8, n_q, DTYPES[dtype], q=(st.randn(2, 8, n_q, 128) * f).to(DTYPES[dtype]), scale=0.1 / f)
+
+
+@pytest.mark.parametrize("N,n,H,D,n_q", [(64, 8000, 32, 128, 1), (64, 8000, 16, 64, 1), (20, 8000, 32, 128, 4), (32, 4000, 8, 256, 1),
+                                         (16, 4000, 8, 256, 12)])
+def test_f32_sums_over_many_long_sequences(cuda_device, N, n, H, D, n_q):
+    """So many units that each CTA walks thousands of keys of one, with values of one sign: nothing is lost on the way."""
+    st = R.State([n] * N, 8, D, 64, seed=34, device=cuda_device)
+    st.v.abs_()
+    q = st.randn(N, H, n_q, D)
+    got = attend(st, q)
+    st.table, st.len, st.N = st.table[:3], st.len[:3], 3
+    E.check(st, q[:3], got[:3], f"{N} of {n}")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n_q", [1, 4, 70])
+def test_tables_of_more_than_65536_tokens(cuda_device, n_q, D, dtype):
+    """The sums that long tables get, in 16-bit results too."""
+    st = R.State([300, 1000, 5], 2, D, 128, seed=35, device=cuda_device)
+    wide = torch.full((3, 600), -1, dtype=torch.int32, device=cuda_device)
+    wide[:, :st.table.shape[1]] = st.table
+    st.table = wide
+    run_attend(st, 8, n_q, DTYPES[dtype])
+    run_attend(st, 8, n_q, DTYPES[dtype], softcap=4.0)
