@@ -34,13 +34,13 @@
 //
 // Bound.  One token of 48 sequences of 1 to 10240 tokens (32 heads on 8, D = 128, BF16): 115 us in a graph, 67 % of the copy
 // bandwidth of 6.54 TB/s (125 us for a call by itself); issue slots are half busy and DRAM half, each of an SM's 12 warps
-// waiting for its own next block.  110 of 2000 each: 92 us and 75 %.  For two of 8192 (19.4 us, 33.6 MB, floor 5.1 us; 19.3
+// waiting for its own next block.  110 of 2000 each: 93 us and 75 %.  For two of 8192 (F32: 19.8 us, 33.6 MB, floor 5.1 us; 19.5
 // where 36 layers' caches are read in turn) the start - lengths, table, first pages, one after another - and the join of the
-// parts through global memory are most of the 9 us that a call over a hundred tokens takes, and the 9 blocks of a CTA, 2 or 3
+// parts through global memory are most of the 9.6 us that a call over a hundred tokens takes, and the 9 blocks of a CTA, 2 or 3
 // a warp, end before the rings reach their rate: the decode over an F16 slab, which joins in clusters, takes 14.4 there.  From
 // 9 rows on (NT = 2) it is issue: 0.9 us for a block of a CTA, two CTAs an SM (16 sequences of 1024, 64 rows per kv head:
-// 57 us).  Two stages for three CTAs of an SM against three stages for two, D = 128, one row per head:
-// 116 us against 129 for the 48 sequences, 20.4 against 19.4 for the two.
+// 58 us).  Two stages for three CTAs of an SM against three stages for two, D = 128, one row per head:
+// 115 us against 130 for the 48 sequences, 20.8 against 19.2 for the two.
 #include "kv8.cuh"
 #include "tc_sm100.cuh"
 
@@ -53,12 +53,12 @@ constexpr int KD_THREADS = 32 * KD_WARPS;
 constexpr int KD_BLOCK   = 32;     // keys per block
 constexpr int KD_ROWS    = 16;     // query rows per unit
 constexpr int KD_OFF     = 12;     // P is held times 2^12: F16 keeps 11 bits down to 2^-26 of the largest weight
-// 2 sequences of 300: 9.9 us whole, 9.6 in parts; 100 of 400: 29.4 whole, 35.9 flat.
+// 2 sequences of 300: 10.4 us whole, 9.6 in parts (F32; BF16 10.0 and 9.8); 100 of 400 (BF16): 29.3 whole, 35.9 flat.
 constexpr int KD_WHOLE   = 16;
-// Blocks of a part, at least: 4, 8, 16 take 11.2, 11.5, 14.2 us for one sequence of 2000.
+// Blocks of a part, at least: 4, 8, 16 take 11.8, 11.8, 14.8 us for one sequence of 2000.
 constexpr int KD_PART    = 4;
-// What a crossing costs, in blocks.  0, 8, 32: 24.8, 19.8, 20.4 us for 2 sequences of 8192 (0: flat), 40.1, 40.1, 39.0
-// for 16 of 4096 (32: parts).  Whole against flat: 29.5 against 35.8 us for 50 of 1000, 92.6 against 101.4 for 110 of 2000.
+// What a crossing costs, in blocks.  0, 8, 32: 25.5, 20.1, 20.7 us for 2 sequences of 8192 (0: flat), 40.2, 39.9, 39.1
+// for 16 of 4096 (32: parts).  Whole against flat: 29.5 against 35.7 us for 50 of 1000, 92.7 against 101.3 for 110 of 2000.
 constexpr int KD_CROSS   = 32;
 
 // Tokens up to which sums in the tensor core's truncating accumulators (4e-10 of the result a key) stay an eighth of F16's
@@ -989,10 +989,10 @@ int ctas_per_sm(int D, int rows) {
 
 // The kernel for many rows (D <= 128) takes a call that gives every SM of each wave of its CTAs five units of this
 // kernel for two, a part of a block's keys counted like the whole.  BF16, D = 128, this kernel against that at 1.7 such
-// units per SM (4 sequences of 4096, 32 rows per kv head): 38 us against 35; at 2.0 (one of 8192, 32 rows) 30 against 36; at
+// units per SM (4 sequences of 4096, 32 rows per kv head): 39 us against 35; at 2.0 (one of 8192, 32 rows) 30 against 36; at
 // 2.6 (16 of 1024, 48 rows) 52 against 31; at 3.5 (4 of 4096, 64 rows) 65 against 35; at 3.9 (one of 8192, 64 rows) 38
-// against 36, and of 256 rows 99 against 46.  F32: 53 against 36 at 2.6, 67 against 41 at 3.5, 39 against 38 at 3.9; F16 with
-// D = 64: 31 against 24 at 2.6.  The host knows the table's capacity, not the lengths: two sequences of 100 tokens in
+// against 36, and of 256 rows 99 against 46.  F32: 54 against 37 at 2.6, 69 against 41 at 3.5, 40 against 38 at 3.9; F16 with
+// D = 64: 31 against 25 at 2.6.  The host knows the table's capacity, not the lengths: two sequences of 100 tokens in
 // tables for 8192 (48 rows, F32) count 9 parts each and take 14 us here against 10.
 bool many_rows(Kv8AttnParams & p, int sms) {
     const int64_t heads = (int64_t) p.t.n_seq * p.c.n_head_kv, rows = (int64_t) p.ratio * p.n_q;

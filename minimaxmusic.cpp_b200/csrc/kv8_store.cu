@@ -12,7 +12,7 @@
 // A page's rows stay in registers between the maximum and the codes, so that they are read once, and the codes
 // take no division where a product is sure of them.  Appending 2 prompts of 4096 F32 rows (8 heads, D = 128) and reading
 // them back took 60 us with two readings of the rows and a remainder for every code, 53 without the second reading, 38
-// so: 24 for the append (84 MB, 53 % of the copy bandwidth of 6.54 TB/s) and 20 for the read (64 %) where each runs alone.
+// so: 20 for the append (84 MB, 63 % of the copy bandwidth of 6.54 TB/s) and 25 for the read (52 %) in graphs of their own.
 // The append is bound by issue (slots 68 % busy, DRAM 34 %, 44 % of the warps): the launch bound of 1024 threads holds every
 // page size to 64 registers a thread.  The read moves 4 codes a lane and load.  Rows of 16 bits take longer though they are
 // half the bytes: 33 us in F16, 36 in BF16.  One token is latency: 6 us for the two.
