@@ -5,7 +5,7 @@ import torch
 
 import kv8_ref as R
 import mm3fa
-from test_kv8_gpu import DTYPES, many
+from test_kv8_gpu import DTYPES, many, run_attend
 
 pytestmark = pytest.mark.gpu
 
@@ -237,3 +237,12 @@ def test_a_workspace_for_page_operations(cuda_device):
     for bad in (ws.cpu(), ):
         with pytest.raises(ValueError):
             c.reserve(table, refs, n_tok, ws=bad)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n_q", [1, 70])
+def test_attend_causal_length_beyond_the_table(cuda_device, n_q, dtype):
+    """A length beyond the table is the table's, for the causal rows too: the last row sees all of its tokens."""
+    st = R.State([128, 64, 10], 2, 64, 64, seed=36, device=cuda_device)
+    st.len = torch.tensor([2 ** 31 - 1, -5, 200], dtype=torch.int32, device=cuda_device)
+    run_attend(st, 4, n_q, DTYPES[dtype])
