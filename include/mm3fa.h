@@ -588,6 +588,81 @@ MM3FA_API int mm3fa_kv8_compact(const mm3fa_kv8 * cache, const mm3fa_kv8_table *
                                 mm3fa_kv8_table * table_out, int32_t * refs_out, void * workspace,
                                 size_t workspace_bytes, void * stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Decoding with a tree of drafted tokens over slab caches (the views of mm3fa_flash_attn_ext's k and v).  Per step:
+ * the nodes' K and V rows are stored behind the kv_len tokens of each sequence, node i's in row kv_len + i (by
+ * mm3fa_decode_prologue with one set per node and a cache view whose nb[3] is 0, say), mm3fa_tree_attn computes every
+ * layer's attention, mm3fa_tree_verify decides which nodes stay, and mm3fa_tree_commit moves their rows together.
+ * Node 0 is the root: the token that the step before gave.  A parent comes before its children; a parents[i] outside
+ * [0, i) is none (the node sees the cached tokens and itself, and no walk reaches it).  Up to 256 nodes.
+ * Sequence s goes by tree s % n_tree, so that the sets of a CFG batch can share trees.
+ * No counterpart in the reference, which decodes one token of each set per step (src/qwen3-lm.h:645-934).
+ * ------------------------------------------------------------------------------------------ */
+typedef struct mm3fa_tree {
+    const int32_t * parents;   /* device [n_tree][stride], of which [0, max_nodes) are used */
+    int64_t         stride;    /* entries; 0: all trees have these parents */
+    const int32_t * n_nodes;   /* device [n_tree]: nodes [0, n_nodes) count (clamped to [0, max_nodes]); NULL: max_nodes */
+    int32_t         max_nodes;
+    int32_t         n_tree;
+} mm3fa_tree;
+
+/* Bytes of device workspace mm3fa_tree_attn needs, 64 KiB at least (0: operands it would refuse). */
+MM3FA_API size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v,
+                                           const mm3fa_tree * tree);
+
+/*
+ * dst = softmax(scale * q k^T [softcap]) v, node i of sequence s seeing keys [0, kv_len[s]), and kv_len[s] + j for
+ * itself and its ancestors j.
+ *   q       F32, F16 or BF16 [D, max_nodes, n_head, n_seq], any strides along dims 1 to 3
+ *   k, v    F16, BF16, Q8_0 or F32 [D, n_kv, n_head_kv, n_seq], of one type, any strides along dims 1 to 3
+ *   dst     [D, n_head, max_nodes, n_seq], F32 or q's type, not in q's memory; rows of nodes that do not count are left as
+ *           they were
+ *   kv_len  device int32 [n_seq], clamped to [0, n_kv]; rows from n_kv on are absent
+ *   logit_softcap  0 disables; otherwise s <- softcap * tanh(s / softcap)
+ *   workspace      its first 64 KiB zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this
+ *                  function alone, of any shapes that it is large enough for
+ * D 64, 128 or 256; at most 64 query heads per kv head.  q is not rounded to the cache's type.  What a node does not see
+ * has no influence, not-a-number or infinite values included; a node that sees nothing gets zeros.
+ */
+MM3FA_API int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v,
+                              const mm3fa_tree * tree, const int32_t * kv_len, float scale, float logit_softcap,
+                              mm3fa_tensor * dst, void * workspace, size_t workspace_bytes, void * stream);
+
+/*
+ * Verifies drafted tokens.  From node 0, with p = softmax(logits of the current node / temperature), the children of the
+ * current node are tried in their order; with r = p and M = 1 at first, child i with token x is accepted, and becomes the
+ * current node, where accept[i] * q(x) * M < r(x); otherwise r <- max(r - M q, 0) and M <- sum of r.  q is the row of
+ * `draft` at the current node, the distribution that its children were drawn from; without `draft`, 1 at x and 0
+ * elsewhere.  The next token is the first at which the sum of r so far exceeds sample * sum of r (of p, where nothing is left
+ * of r): the tokens then follow the target's distribution whatever the draft's.
+ *   logits   F32, F16 or BF16 [V, max_nodes, n_tree]: row i is the target's behind node i; NaN counts as -inf
+ *   draft    F32, F16 or BF16 probabilities of the same sizes, or NULL; NaN and negative ones count as 0
+ *   tokens   device int32 [n_tree][max_nodes]: the nodes' tokens (node 0's is not used; one outside [0, V) is never accepted)
+ *   accept   device F32 [n_tree][max_nodes], sample device F32 [n_tree]: random numbers, uniform in [0, 1)
+ *   temperature  0: greedy, a child is accepted where its token is the lowest of those with the largest logit, which
+ *                is also the next token
+ *   path     device int32 [n_tree][max_nodes]: the accepted nodes in order, node 0 first, then -1
+ *   n_path   device int32 [n_tree]: how many (0 where a tree has no nodes)
+ *   token    device int32 [n_tree]: the next token (-1 where a tree has no nodes or no logit is above -inf)
+ * Decisions are taken from F32 logits in F64; V up to 2^22.  Only the rows of accepted nodes are read.
+ */
+MM3FA_API int mm3fa_tree_verify(const mm3fa_tensor * logits, const mm3fa_tensor * draft, const mm3fa_tree * tree,
+                                const int32_t * tokens, const float * accept, const float * sample, float temperature,
+                                int32_t * path, int32_t * n_path, int32_t * token, void * stream);
+
+/*
+ * Moves the accepted nodes' rows behind the cached tokens: in every layer, for K and V, row kv_len[s] + path[i] goes to
+ * row kv_len[s] + i, in place, and kv_len_out[s] = kv_len[s] + n_path.
+ *   k, v    n_layers tensors each, [D, rows, n_head_kv, n_seq] F32, F16, BF16 or Q8_0; all of one type and shape, those
+ *           of K with the same strides, and those of V
+ *   path, n_path   as mm3fa_tree_verify leaves them, [n_tree][max_nodes] and [n_tree]; a path ends at an entry that is not
+ *           above the one before it or names no row, and counts up to there
+ *   kv_len, kv_len_out  device int32 [n_seq], not in the same memory; a sequence of negative length keeps it
+ */
+MM3FA_API int mm3fa_tree_commit(const mm3fa_tensor * k, const mm3fa_tensor * v, int n_layers, const int32_t * path,
+                                const int32_t * n_path, int max_nodes, int n_tree, const int32_t * kv_len,
+                                int32_t * kv_len_out, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

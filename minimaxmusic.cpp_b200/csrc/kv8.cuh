@@ -144,15 +144,19 @@ __device__ __forceinline__ void kv8_report(uint32_t * status, uint32_t bit) {
 
 // ------------------------------------------------------------------ host helpers
 
+inline bool kv8_pdl() {
+    static const bool pdl = [] {
+        const char * e = std::getenv("MM3FA_PDL");
+        return !(e && std::atoi(e) == 0);
+    }();
+    return pdl;
+}
+
 // Launches with programmatic stream serialisation (MM3FA_PDL=0 turns it off): the CTAs may start
 // once the previous kernel's have exited or have let their dependents go (the peer wait does so at its entry);
 // every kernel here waits with griddepcontrol.wait, for that kernel's end, before it reads anything or takes a time.
 template <typename... KArgs, typename... Args>
 cudaError_t kv8_launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
-    static const bool pdl = [] {
-        const char * e = std::getenv("MM3FA_PDL");
-        return !(e && std::atoi(e) == 0);
-    }();
     cudaLaunchConfig_t  cfg{};
     cudaLaunchAttribute attr[1];
     cfg.gridDim          = grid;
@@ -161,7 +165,7 @@ cudaError_t kv8_launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t sm
     cfg.stream           = stream;
     cfg.attrs            = attr;
     cfg.numAttrs         = 0;
-    if (pdl) {
+    if (kv8_pdl()) {
         attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs                                       = 1;

@@ -385,3 +385,4 @@ def ipc_close(ptr: int) -> None:
 
 
 from .kv8 import Kv8Cache  # noqa: E402,F401  (uses the names above)
+from .tree import CacheLayers, DraftTree  # noqa: E402,F401

@@ -16,17 +16,13 @@ from __future__ import annotations
 import ctypes
 import struct
 
-from . import ERR_SHAPE, ERR_STRIDE, ERR_TYPE, OK, MM3FAError, lib, workspace_status
-from .ggml import GGML_TYPE_BF16, GGML_TYPE_F16, GGML_TYPE_F32
+from . import ERR_SHAPE, ERR_STRIDE, ERR_TYPE, MM3FAError, lib
+from .on_device import _PACK_TENSOR, OnDevice  # noqa: F401
 
 FORK_DEEP = 1  # MM3FA_KV8_FORK_DEEP
 
 _CACHE = struct.Struct("@6i4P")                 # struct mm3fa_kv8
 _PACK_TABLE = struct.Struct("@Pq2i").pack       # struct mm3fa_kv8_table
-_PACK_TENSOR = struct.Struct("@2i4q4QP").pack   # struct mm3fa_tensor
-
-_ZEROED = 1 << 16  # bytes of a workspace that have to be zero before its first use
-_ALSO = slice(16, 24)  # of a workspace: address of a second status word
 
 _fns = None
 
@@ -57,27 +53,7 @@ def _calls():
     return _fns
 
 
-_STATUS_SLOTS = 1 << 16
-_status_words = {}  # device -> [int32 [_STATUS_SLOTS, 4], slots given out]
-
-
-def _status_memory(device):
-    """Status words for calls of graphs, of which a graph keeps the address: never freed, and none given out twice (but in
-    turn when all have been)."""
-    import torch
-
-    if device not in _status_words:
-        _status_words[device] = [torch.zeros(_STATUS_SLOTS, 4, dtype=torch.int32, device=device), 0]
-    return _status_words[device]
-
-
-def _types():
-    import torch
-
-    return {torch.float32: (GGML_TYPE_F32, 4), torch.float16: (GGML_TYPE_F16, 2), torch.bfloat16: (GGML_TYPE_BF16, 2)}
-
-
-class Kv8Cache:
+class Kv8Cache(OnDevice):
     """int8 pages [n_layers, n_pages, n_head_kv, page_tokens, head_dim] of K and V and their F32 scales
     [n_layers, n_pages, n_head_kv]; the tensors stay the caller's."""
 
@@ -93,21 +69,10 @@ class Kv8Cache:
         if not all(t.device == k.device for t in (v, k_scale, v_scale)):
             raise ValueError("Kv8Cache: k, v and their scales have to be on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = k.device
         self.n_layers, self.n_pages, self.n_head_kv, self.page_tokens, self.head_dim = k.shape
         self._desc = _CACHE.pack(self.head_dim, self.page_tokens, self.n_head_kv, self.n_pages, self.n_layers, 0,
                                  k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
-        self._torch, self._int32 = torch, torch.int32
-        self._dt = _types()
-        self._dev = k.get_device()  # -1: host tensors, on which the C ABI's checks run but no kernel does
-        self._fns = None
-        self._ws = {}    # (operation, stream) -> address and bytes of a zero-filled workspace
-        self._kept = []  # these, outgrown ones too: their status has not been read
-        self._need = {}  # workspace bytes by shape
-        self._capture = None  # the last capture, and its workspaces by (operation, stream)
-        self._is_capturing, self._current_device = torch._C._cuda_isCurrentStreamCapturing, torch._C._cuda_getDevice
-        self._found = {}  # (operation, stream), or None: the status of calls of graphs
-        self._status = None if self._dev < 0 else _status_memory(self.device)
+        self._on_device_of(k)
 
     @classmethod
     def allocate(cls, n_layers: int, n_pages: int, n_head_kv: int, page_tokens: int, head_dim: int, device="cuda"):
@@ -119,26 +84,12 @@ class Kv8Cache:
         scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)]
         return cls(codes[0], codes[1], scales[0], scales[1])
 
+    _prefix = "mm3fa_kv8_"
+
+    def _calls(self):
+        return _calls()
+
     # ------------------------------------------------------------ descriptors
-
-    def _elsewhere(self, t):
-        return ValueError(f"Kv8Cache: a tensor on {t.device}, the cache is on {self.device}")
-
-    def _rows(self, t):
-        """mm3fa_tensor [D, rows, heads, seqs] of a torch tensor (seqs, heads, rows, D)."""
-        if t.dim() != 4:
-            raise MM3FAError(ERR_SHAPE, "Kv8Cache: rows of 4 dimensions are wanted")
-        ty = self._dt.get(t.dtype)
-        if ty is None:
-            raise MM3FAError(ERR_TYPE, "Kv8Cache")
-        if t.get_device() != self._dev:
-            raise self._elsewhere(t)
-        a, b, c, d = t.shape
-        sa, sb, sc, sd = t.stride()
-        if sd != 1 and d > 1:
-            raise MM3FAError(ERR_STRIDE, "Kv8Cache: the head dimension has to be contiguous")
-        ty, e = ty
-        return _PACK_TENSOR(ty, 0, d, c, b, a, e, sc * e, sb * e, sa * e, t.data_ptr())
 
     def _table(self, t):
         if t.dim() != 2:
@@ -152,99 +103,6 @@ class Kv8Cache:
         if one != 1 and pages > 1:
             raise MM3FAError(ERR_STRIDE, "Kv8Cache: table")
         return _PACK_TABLE(t.data_ptr(), stride if n > 1 else pages, pages, n)
-
-    def _ints(self, t, n, what):
-        """Address of an int32 tensor of n entries."""
-        if t.dtype is not self._int32:
-            raise MM3FAError(ERR_TYPE, "Kv8Cache: " + what)
-        if t.get_device() != self._dev:
-            raise self._elsewhere(t)
-        if t.dim() != 1 or t.shape[0] != n:
-            raise MM3FAError(ERR_SHAPE, "Kv8Cache: " + what)
-        if n > 1 and t.stride(0) != 1:
-            raise MM3FAError(ERR_STRIDE, "Kv8Cache: " + what)
-        return t.data_ptr()
-
-    def _stream(self):
-        return 0 if self._dev < 0 else self._torch._C._cuda_getCurrentRawStream(self._dev)
-
-    def _on(self, stream):
-        """A context in which `stream` is the current one."""
-        if stream.device_index != self._dev:
-            raise ValueError(f"Kv8Cache: a stream of device {stream.device_index}, the cache is on {self.device}")
-        return self._torch.cuda.stream(stream)
-
-    def _call(self, name, *args):
-        """A library call with the cache's device current; its result."""
-        fn = (self._fns or self._bind())[name]
-        if self._dev < 0 or self._torch._C._cuda_getDevice() == self._dev:
-            return fn(*args)
-        with self._torch.cuda.device(self.device):
-            return fn(*args)
-
-    def _bind(self):
-        self._fns = _calls()
-        return self._fns
-
-    def _run(self, name, *args):
-        st = self._call(name, *args)
-        if st:
-            raise MM3FAError(st, "mm3fa_kv8_" + name)
-
-    def _workspace(self, key, nbytes):
-        """(address, bytes) of the workspace of an operation on a stream, zero-filled as far as it has to be when it is made."""
-        # the current stream is key's where the current device is the cache's
-        if self._dev >= 0 and (self._is_capturing() or self._current_device() != self._dev):
-            capture = self._call("capture_id", key[1])
-            if capture:
-                return self._workspace_of_graph(capture, key, nbytes)
-        if self._capture:
-            self._capture = None
-        buf = self._ws.get(key)
-        if buf is not None and buf[1] >= nbytes:
-            return buf
-        if nbytes > 0:
-            made = self._made(nbytes)
-            self._ws[key] = at = made.data_ptr(), made.numel()
-            self._kept.append((key, made))
-            return at
-        return None, 0
-
-    def _made(self, nbytes):
-        made = self._torch.empty(max(nbytes, _ZEROED), dtype=self._torch.uint8, device=self.device)
-        made[:_ZEROED].zero_()
-        return made
-
-    def _workspace_of_graph(self, capture, key, nbytes):
-        """A workspace that a graph zeroes when it is replayed: one for all calls of an operation that a stream of the
-        capture makes, shared with nothing else.  It lives in the graph's memory, like all that is allocated in a
-        capture; this class lets it go at its next call elsewhere (one that the capture makes later is zeroed in turn).
-        What the calls find goes to a status word of the stream where it has a workspace, else to one of the cache."""
-        if self._capture is None or self._capture[0] != capture:
-            self._capture = capture, {}
-        made = self._capture[1].get(key)
-        if made is None or made.numel() < nbytes:
-            if nbytes <= 0:
-                return None, 0
-            made = self._capture[1][key] = self._made(nbytes)
-            made[_ALSO].view(self._torch.int64).fill_(self._status_word(key if key in self._ws else None).data_ptr())
-        return made.data_ptr(), made.numel()
-
-    def _status_word(self, key):
-        word = self._found.get(key)
-        if word is None:
-            words, n = self._status
-            self._status[1] = n + 1
-            word = self._found[key] = words[n % _STATUS_SLOTS]
-        return word
-
-    def _given(self, ws):
-        """(address, bytes) of a caller's workspace."""
-        if ws.get_device() != self._dev:
-            raise self._elsewhere(ws)
-        if not ws.is_contiguous():
-            raise MM3FAError(ERR_STRIDE, "Kv8Cache: workspace")
-        return ws.data_ptr(), ws.numel() * ws.element_size()
 
     # ------------------------------------------------------------ operators
 
@@ -349,20 +207,3 @@ class Kv8Cache:
         st, n = self._stream(), table.shape[0]
         self._run("compact", self._desc, self._table(table), self._ints(refs, self.n_pages, "refs"),
                    self._table(table_out), self._ints(refs_out, self.n_pages, "refs_out"), *self._pages_ws(n, st, ws), st)
-
-    def check(self, stream=None, captured=False, ws=None):
-        """Synchronises the stream and raises MM3FAError where a page operation on it found too few free pages
-        (ERR_PAGES) or a bounded device wait of an attention expired (ERR_TIMEOUT).  Calls that a graph replays are among
-        them where an earlier call on the stream of the capture had made its workspace; captured=True: those of all
-        graphs (wait for the streams that replay them first).  ws: a workspace that calls were given."""
-        if stream is not None:
-            with self._on(stream):
-                return self.check(captured=captured, ws=ws)
-        st = self._stream()
-        bufs = [buf for key, buf in self._kept if key[1] == st]  # outgrown ones too
-        bufs += [word for key, word in self._found.items() if captured or (key and key[1] == st)]
-        bufs += [ws] if ws is not None else []
-        for buf in bufs:
-            status, _ = workspace_status(buf.data_ptr(), st)
-            if status != OK:
-                raise MM3FAError(status, "Kv8Cache")
