@@ -135,7 +135,7 @@ extern "C" {
 
 size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v, const mm3fa_tree * tree) {
     TreeAttnParams p{};
-    return prepare_attn(q, k, v, tree, p) == MM3FA_OK ? KV8_WS_ZEROED : 0;
+    return prepare_attn(q, k, v, tree, p) != MM3FA_OK ? 0 : tree_attn_tc_takes(p) ? tree_attn_tc_workspace(p, host_sm_count()) : KV8_WS_ZEROED;
 }
 
 int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v, const mm3fa_tree * tree, const int32_t * kv_len,
@@ -176,7 +176,9 @@ int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_
     p.softcap    = logit_softcap;
     p.status     = static_cast<uint32_t *>(workspace);
     p.timeout_ns = host_wait_timeout_ns();
-    return host_record_cuda(launch_tree_attn(p, static_cast<cudaStream_t>(stream)));
+    // 16-bit slabs at D = 64 and 128 on the tensor cores; the others (F32, Q8_0, D = 256, unaligned rows) on CUDA cores
+    return host_record_cuda(tree_attn_tc_takes(p) ? launch_tree_attn_tc(p, host_sm_count(), static_cast<cudaStream_t>(stream)) :
+                                                    launch_tree_attn(p, static_cast<cudaStream_t>(stream)));
 }
 
 int mm3fa_tree_verify(const mm3fa_tensor * logits, const mm3fa_tensor * draft, const mm3fa_tree * tree, const int32_t * tokens,
