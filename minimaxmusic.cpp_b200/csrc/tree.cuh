@@ -27,7 +27,6 @@ struct TreeAttnParams {
     float       scale, softcap;
     // workspace
     uint32_t *  status;
-    uint32_t *  counters;
     float *     part;
     uint64_t    timeout_ns;
 };

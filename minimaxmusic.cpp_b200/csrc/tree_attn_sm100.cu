@@ -8,8 +8,13 @@
 //
 // Split.  The tiles of all units are one line, in the order of sequence and kv head, and each group takes an equal piece of
 // it, found on the device from the lengths: a long sequence is cut over many groups, short ones are several to a
-// group, and no group waits for another.  A piece that is not a whole unit leaves O, m and l in the workspace, and the
-// last group to arrive joins them in their order.
+// group, and no group waits for another.  (A group's piece may so have parts of two units, and whole ones between.)
+// A part of a unit leaves O, m and l in the workspace, and a second kernel joins the parts in their order: by the last
+// CTA to arrive, one SM of 148 would read all parts of a unit (25 us for 9 parts of 96 rows, at one SM's bandwidth).
+// That kernel is left out where the slab is too short for a part.
+//
+// Most of the code runs once in a CTA, and its first run costs what the instruction cache costs: what does not feed the
+// tensor core is in rolled loops or functions.
 //
 // 384 threads:
 //   warp 0       TMA: K and V tiles through one ring, in the order in which the products take them
@@ -39,11 +44,13 @@ constexpr int TS_M       = 128;  // rows of a block
 constexpr int TS_N       = 128;  // keys of a tile
 constexpr int TS_TMEM    = 512;  // columns: S of two tiles, P V of two tiles
 constexpr int TS_OFF     = 14;   // weights are held times 2^14: F16 keeps 11 bits of one down to 2^-28 of the largest
+constexpr int TJ_ROWS    = 8;    // rows of a joining CTA
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
 constexpr int TS_REGS_SOFTMAX = 208;  // 2 x 208 + 88 = 3 x 168
 constexpr int TS_REGS_ISSUE   = 88;
 static_assert(2 * TS_REGS_SOFTMAX + TS_REGS_ISSUE <= 3 * TS_REGS_LAUNCH, "more registers than the launch has");
-constexpr int TS_SPACE = 64;  // words of the workspace before the counters
+constexpr int TS_SPACE = 256;  // bytes of the workspace before the list of units in parts
+constexpr int TS_LEAST = 2;    // tiles of a part, at least: it costs about as much as a tile
 
 template <int D, int PARTS>
 struct TsSmem {
@@ -142,10 +149,60 @@ __device__ __forceinline__ float2 ts_unpack(uint32_t u) {
     return BF16 ? bf2_to_f2(u) : h2_to_f2(u);
 }
 
+// (functions of their own: see the instruction cache above)
+__device__ __noinline__ float ts_tanh(float x) {
+    return tanhf(x);
+}
+
+// elements [e0, e0 + E) of a row that is not aligned: F32, or 16-bit pairs
+template <int E>
+__device__ __noinline__ uint4 ts_load_elements(const char * row, bool f32, int e0) {
+    uint32_t x[4] = { 0, 0, 0, 0 };
+    if (f32) {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            x[e] = reinterpret_cast<const uint32_t *>(row)[e0 + e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            x[e / 2] = reinterpret_cast<const uint16_t *>(row)[e0 + e] | (uint32_t) reinterpret_cast<const uint16_t *>(row)[e0 + e + 1] << 16;
+        }
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
 // Floats of a part: O of its rows, then m and l of each; a multiple of 16 bytes.
 __host__ __device__ constexpr int ts_slot_floats(int rows, int D) {
     return (rows * (D + 2) + 3) / 4 * 4;
 }
+
+// 4 values to elements [e, e + 4) of a row
+__device__ __forceinline__ void ts_store4(char * row, int e, const float4 & f, int type, bool vec) {
+    if (type == KV_F32) {
+        float * o = reinterpret_cast<float *>(row) + e;
+        if (vec) {
+            *reinterpret_cast<float4 *>(o) = f;
+        } else {
+            o[0] = f.x, o[1] = f.y, o[2] = f.z, o[3] = f.w;
+        }
+        return;
+    }
+    const uint32_t a = type == KV_F16 ? ts_pack<false>(f.x, f.y) : ts_pack<true>(f.x, f.y);
+    const uint32_t b = type == KV_F16 ? ts_pack<false>(f.z, f.w) : ts_pack<true>(f.z, f.w);
+    uint16_t *     o = reinterpret_cast<uint16_t *>(row) + e;
+    if (vec) {
+        *reinterpret_cast<uint2 *>(o) = make_uint2(a, b);
+    } else {
+        o[0] = (uint16_t) a, o[1] = (uint16_t) (a >> 16), o[2] = (uint16_t) b, o[3] = (uint16_t) (b >> 16);
+    }
+}
+
+// What the group that has a unit's first part leaves for the joining kernel.
+struct TsJoin {
+    int     s, h, parts, rows;  // parts 0: the group has no such unit
+    int64_t part0, part1;       // where the first part and the second are, in floats; the others follow at even steps
+};
 
 // Key tiles of a sequence's units; 0 where none of its nodes counts.
 struct TsSeq {
@@ -161,39 +218,69 @@ __device__ __forceinline__ TsSeq ts_seq(const TreeAttnParams & p, int s) {
     return q;
 }
 
+// The line of W tiles in G even pieces, piece g from `at(g)` on.  A border closer than TS_LEAST tiles to a unit's start or end
+// goes there, so that no part of a unit has less.
+struct TsLine {
+    int W, G, each, more;  // `more` pieces have a tile more than `each`
+
+    __device__ __forceinline__ TsLine(int W_, int groups) : W(W_), G(max(1, min(groups, W_ / TS_LEAST))) {
+        each = W / G;
+        more = W - each * G;
+    }
+
+    __device__ __forceinline__ int at(int g) const {
+        return g * each + min(g, more);
+    }
+
+    // the last piece that starts at tile x or before
+    __device__ __forceinline__ int last(int x) const {
+        const int y = more * (each + 1);
+        return min(G - 1, x < y ? x / (each + 1) : each > 0 ? more + (x - y) / each : G - 1);
+    }
+
+    // border x, of a unit of n tiles that starts at `first` and holds x
+    static __device__ __forceinline__ int border(int x, int first, int n) {
+        return x - first < TS_LEAST ? first : first + n - x < TS_LEAST ? first + n : x;
+    }
+};
+
 // The pieces of a group: tiles [a, b) of unit (s, h), one after another.  Every role walks them by itself.
 struct TsPieces {
     const TreeAttnParams & p;
-    int                    s;
-    int64_t                first, x, end;  // first: of sequence s on the line of tiles
+    int                    s, first, x, end;  // first: of sequence s on the line of tiles; end: before its move to a border
     TsSeq                  q;
-    int                    h, a, b;
+    int                    h, a, b, unit;     // unit: where the unit starts
 
-    __device__ __forceinline__ TsPieces(const TreeAttnParams & p_, int s_, int64_t first_, int64_t x_, int64_t end_)
-        : p(p_), s(s_), first(first_), x(x_), end(end_), q{ 0, 0, 0, 0 }, h(0), a(0), b(0) {
+    __device__ __forceinline__ TsPieces(const TreeAttnParams & p_, int s_, int first_, int x_, int end_)
+        : p(p_), s(s_), first(first_), x(x_), end(end_), q{ 0, 0, 0, 0 }, h(0), a(0), b(0), unit(0) {
         if (x < end) {
             q = ts_seq(p, s);
+            const int u = first + (x - first) / q.tiles * q.tiles;
+            x           = TsLine::border(x, u, q.tiles);
         }
     }
 
     // the next piece that has rows in block rb
     __device__ __forceinline__ bool next(int rb) {
         while (x < end) {
-            const int64_t all = (int64_t) q.tiles * p.n_head_kv;
+            const int all = q.tiles * p.n_head_kv;
             if (x - first >= all) {
                 first += all;
                 q = ts_seq(p, ++s);
                 continue;
             }
-            const int at = (int) (x - first);
             if (q.nodes * p.ratio <= rb * TS_M) {  // (this block is empty: on to the next sequence)
                 x = first + all;
                 continue;
             }
-            h = at / q.tiles;
-            a = at - h * q.tiles;
-            b = (int) min((int64_t) q.tiles, a + (end - x));
-            x += b - a;
+            h    = (x - first) / q.tiles;
+            unit = first + h * q.tiles;
+            a    = x - unit;
+            b    = unit + q.tiles <= end ? q.tiles : TsLine::border(end, unit, q.tiles) - unit;
+            if (b <= a) {
+                return false;
+            }
+            x = unit + b;
             return true;
         }
         return false;
@@ -212,9 +299,8 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     uint32_t * misc      = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
     uint32_t * tmem_slot = misc;
     int *      abort_f   = reinterpret_cast<int *>(misc + 1);
-    int *      last_f    = reinterpret_cast<int *>(misc + 2);
     int *      start_s   = reinterpret_cast<int *>(misc + 3);
-    int64_t *  line      = reinterpret_cast<int64_t *>(misc + 4);   // the whole line's tiles, the first one of start_s
+    int *      line      = reinterpret_cast<int *>(misc + 4);       // the whole line's tiles, the first one of start_s
     int *      dirty     = reinterpret_cast<int *>(misc + 8);       // a V row of the piece's nodes held what is no number
     int *      sums      = reinterpret_cast<int *>(misc + 16);      // [12] warps' counts
     float *    factors   = reinterpret_cast<float *>(smem + L::OFF_F);
@@ -239,8 +325,12 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
 
     // ---- the group's piece of the line of tiles
     const int group = (int) blockIdx.x / blocks, rb = (int) blockIdx.x % blocks;
+    TsJoin *  join  = reinterpret_cast<TsJoin *>(reinterpret_cast<char *>(p.status) + TS_SPACE) + blockIdx.x;
+    if (tid == 0) {
+        join->parts = 0;
+    }
     {
-        // each thread sums some sequences' tiles of one kv head; all of them are below 2^30 (checked by the host)
+        // each thread sums some sequences' tiles of one kv head; all tiles are fewer than 2^30 (checked by the host)
         const int each = (p.n_seq + TS_THREADS - 1) / TS_THREADS, s0 = min(tid * each, p.n_seq), s1 = min(s0 + each, p.n_seq);
         int       mine = 0;
         for (int s = s0; s < s1; s++) {
@@ -264,13 +354,13 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             before += w < warp ? sums[w] : 0;
             all += sums[w];
         }
-        const int64_t W = (int64_t) all * p.n_head_kv, G = min((int64_t) groups, W);
-        int64_t       from = group < G ? W * group / G : W;
-        int64_t       at   = (int64_t) (before + upto - mine) * p.n_head_kv;
-        if (group < G && from >= at && from < at + (int64_t) mine * p.n_head_kv) {  // it starts among this thread's
+        const TsLine ln(all * p.n_head_kv, groups);
+        const int    from = ln.at(group);
+        int          at   = (before + upto - mine) * p.n_head_kv;
+        if (group < ln.G && from >= at && from < at + mine * p.n_head_kv) {  // it starts among this thread's
             int s = s0;
             for (;; s++) {
-                const int64_t n = (int64_t) ts_seq(p, s).tiles * p.n_head_kv;
+                const int n = ts_seq(p, s).tiles * p.n_head_kv;
                 if (from < at + n) {
                     break;
                 }
@@ -279,14 +369,13 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             *start_s = s, line[1] = at;
         }
         if (tid == 0) {
-            line[0] = W;
+            line[0] = ln.W;
         }
         __syncthreads();
     }
     const uint32_t tmem = *tmem_slot;
-    const int64_t  W = line[0], G = max((int64_t) 1, min((int64_t) groups, W));
-    const int64_t  from = group < G ? W * group / G : W, to = group < G ? W * (group + 1) / G : W;
-    TsPieces       it(p, *start_s, line[1], from, to);
+    const TsLine   ln(line[0], groups);
+    TsPieces       it(p, *start_s, line[1], group < ln.G ? ln.at(group) : ln.W, group < ln.G ? ln.at(group + 1) : ln.W);
 
     if (wg == 0) {
         regs_dec<TS_REGS_ISSUE>();
@@ -472,74 +561,77 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             const int  its_rows = min(it.q.nodes * p.ratio - rb * TS_M, TS_M);
             const bool live = r < its_rows, warp_live = quad * 32 < its_rows;
             const int  held = it.q.L, nodes = it.q.nodes;
-            // ---- Q: 16 rows by each warp, 4 at a time
+            // ---- Q: 16 rows by each warp, all loads in flight, 8 rows at a time
             {
-                constexpr int E = D / 32;
-                const int     ra = (w * 4 + quad) * 16, e0 = lane * E;
-                char *        to = qs + (e0 / 64) * (TS_M * 128) + (e0 % 8) * 2;
-                const float   sign = p.scale < 0.0f ? -1.0f : 1.0f;
-#pragma unroll 1
-                for (int i0 = 0; i0 < 16; i0 += 4) {
-                    float x[4][E];
+                constexpr int  E = D / 32, B = 8;
+                const int      ra = (w * 4 + quad) * 16, e0 = lane * E, in = its_rows - ra;
+                char *         to = qs + (e0 / 64) * (TS_M * 128) + ra * 128 + (e0 % 8) * 2;
+                const float    sign = p.scale < 0.0f ? -1.0f : 1.0f, by = fabsf(cap ? p.scale / p.softcap : p.scale * LOG2E);
+                // lane i: the address of row i
+                const int      rl = rb * TS_M + ra + (lane & 15), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
+                const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
+                uint32_t       u[2][B][E];  // F32 values, or 16-bit pairs in the first half
+                const bool     f32 = p.q.type == KV_F32, f16 = p.q.type == KV_F16;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int    rr = rb * TS_M + ra + i0 + i, nd = rr / p.ratio, hd = it.h * p.ratio + rr - nd * p.ratio;
-                        const char * src = p.q.data + (int64_t) nd * p.q.nb1 + (int64_t) hd * p.q.nb2 + (int64_t) it.s * p.q.nb3;
-                        const bool   in  = ra + i0 + i < its_rows;
+                for (int i = 0; i < 2 * B; i++) {
+                    const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i));
+                    uint32_t (&x)[E] = u[i / B][i % B];
 #pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            x[i][e] = 0.0f;
+                    for (int e = 0; e < E; e++) {
+                        x[e] = 0u;
+                    }
+                    if (i < in && p.q.vec) {
+                        if (E == 4 && f32) {
+                            const uint4 f = *reinterpret_cast<const uint4 *>(src + lane * 16);
+                            x[0] = f.x, x[1] = f.y, x[E - 2] = f.z, x[E - 1] = f.w;
+                        } else if (E == 4 || f32) {
+                            const uint2 f = *reinterpret_cast<const uint2 *>(src + lane * 8);
+                            x[0] = f.x, x[1] = f.y;
+                        } else {
+                            x[0] = *reinterpret_cast<const uint32_t *>(src + lane * 4);
                         }
-                        if (in && p.q.type == KV_F32) {
-                            if (p.q.vec && E == 4) {
-                                const float4 f = *reinterpret_cast<const float4 *>(src + lane * 16);
-                                x[i][0] = f.x, x[i][1] = f.y, x[i][E - 2] = f.z, x[i][E - 1] = f.w;
-                            } else {
+                    }
+                }
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+                    if (!p.q.vec) {  // by elements, a row after another
 #pragma unroll
-                                for (int e = 0; e < E; e++) {
-                                    x[i][e] = reinterpret_cast<const float *>(src)[e0 + e];
+                        for (int i = 0; i < B; i++) {
+                            const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, half * B + i));
+                            if (half * B + i < in) {
+                                const uint4 f = ts_load_elements<E>(src, f32, e0);
+                                u[0][i][0] = f.x, u[0][i][1] = f.y;
+                                if (E == 4) {
+                                    u[0][i][E - 2] = f.z, u[0][i][E - 1] = f.w;
                                 }
-                            }
-                        } else if (in) {
-                            uint32_t u[E / 2];
-                            if (p.q.vec && E == 4) {
-                                const uint2 f = *reinterpret_cast<const uint2 *>(src + lane * 8);
-                                u[0] = f.x, u[E / 2 - 1] = f.y;
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < E; e += 2) {
-                                    u[e / 2] = reinterpret_cast<const uint16_t *>(src)[e0 + e] | (uint32_t) reinterpret_cast<const uint16_t *>(src)[e0 + e + 1] << 16;
-                                }
-                            }
-#pragma unroll
-                            for (int e = 0; e < E; e += 2) {
-                                const float2 f = p.q.type == KV_F16 ? h2_to_f2(u[e / 2]) : bf2_to_f2(u[e / 2]);
-                                x[i][e] = f.x, x[i][e + 1] = f.y;
                             }
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < B; i++) {
+                        float    x[E];
                         uint32_t top = 0;
 #pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
+                        for (int e = 0; e < E; e += 2) {
+                            const float2 a = f16 ? h2_to_f2(u[0][i][e / 2]) : bf2_to_f2(u[0][i][e / 2]);
+                            x[e]     = f32 ? __uint_as_float(u[0][i][e]) : a.x;
+                            x[e + 1] = f32 ? __uint_as_float(u[0][i][e + 1]) : a.y;
+                            top      = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(x[e + 1]) & 0x7fffffffu));
                         }
                         top = __reduce_max_sync(0xffffffffu, top);
                         // a row with an infinity or NaN gives NaN.  F16: the largest element goes to [2^14, 2^15)
                         const bool  odd = top >= 0x7f800000u;
                         const int   ex  = BF16 ? 0 : (top == 0 || odd ? 0 : max((int) (top >> 23) - 127, -112)) - 14;
                         const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
-                        const int   rt  = ra + i0 + i;
                         uint32_t    hi[E / 2], lo[E / 2];
 #pragma unroll
                         for (int e = 0; e < E; e += 2) {
-                            const float a = odd ? 0.0f : x[i][e] * dn, b = odd ? 0.0f : x[i][e + 1] * dn;
+                            const float a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
                             hi[e / 2]      = ts_pack<BF16>(a, b);
                             const float2 f = ts_unpack<BF16>(hi[e / 2]);
                             lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
                         }
-                        char * at = to + rt * 128 + ((((e0 % 64) / 8) ^ (rt & 7)) << 4);
+                        char * at = to + (half * B + i) * 128 + ((((e0 % 64) / 8) ^ i) << 4);  // ra and B: multiples of 8
                         if (E == 4) {
                             *reinterpret_cast<uint2 *>(at) = make_uint2(hi[0], hi[E / 2 - 1]);
                             if (PARTS == 2) {
@@ -551,8 +643,12 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                                 *reinterpret_cast<uint32_t *>(at + L::QT) = lo[0];
                             }
                         }
-                        if (lane == 0) {
-                            factors[rt] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * fabsf(cap ? p.scale / p.softcap : p.scale * LOG2E);
+                        if (lane == i) {
+                            factors[ra + half * B + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
+                        }
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            u[0][i][e] = u[1][i][e];
                         }
                     }
                 }
@@ -616,7 +712,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             tmem_ld_wait_tie(v);
 #pragma unroll
                             for (int e = 0; e < 32; e++) {
-                                v[e] = __float_as_uint(p.softcap * LOG2E * tanhf(__uint_as_float(v[e]) * fcap));
+                                v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
                             }
                             tmem_st32(s_col + (uint32_t) (c * 32), v);
                         }
@@ -756,128 +852,52 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     }
                 }
             }
-            auto address = [&](int row_of_block) {
-                const int rr = rb * TS_M + row_of_block, nd = rr / p.ratio, hd = it.h * p.ratio + rr - nd * p.ratio;
-                return p.o.data + (int64_t) hd * p.o.nb1 + (int64_t) nd * p.o.nb2 + (int64_t) it.s * p.o.nb3;
-            };
-            if (it.a == 0 && it.b == it.q.tiles) {
-                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-                if (live) {
-                    char * out = address(r);
-                    if (p.o.type == KV_F32) {
-                        float * o = reinterpret_cast<float *>(out) + at;
-#pragma unroll
-                        for (int e = 0; e < D / 2; e += 4) {
-                            const float4 f = make_float4(res[e] * inv, res[e + 1] * inv, res[e + 2] * inv, res[e + 3] * inv);
-                            if (p.o.vec) {
-                                *reinterpret_cast<float4 *>(o + e) = f;
-                            } else {
-                                o[e] = f.x, o[e + 1] = f.y, o[e + 2] = f.z, o[e + 3] = f.w;
-                            }
-                        }
-                    } else {
-                        uint16_t * o = reinterpret_cast<uint16_t *>(out) + at;
-#pragma unroll
-                        for (int e = 0; e < D / 2; e += 8) {
-                            uint32_t u[4];
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const float a = res[e + 2 * k] * inv, b = res[e + 2 * k + 1] * inv;
-                                u[k] = p.o.type == KV_F16 ? ts_pack<false>(a, b) : ts_pack<true>(a, b);
-                            }
-                            if (p.o.vec) {
-                                *reinterpret_cast<uint4 *>(o + e) = make_uint4(u[0], u[1], u[2], u[3]);
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    o[e + 2 * k] = (uint16_t) u[k], o[e + 2 * k + 1] = (uint16_t) (u[k] >> 16);
-                                }
-                            }
-                        }
-                    }
-                }
-            } else {
-                // ---- a part of a unit: leave it, and join all of them if it is the last
-                const int     slot_floats = ts_slot_floats(slot_rows, D);
-                const int64_t unit = it.x - it.b;  // (where the unit starts on the line)
-                auto slot_of = [&](int64_t g, int64_t unit_at) {  // a group's first piece has its first slot, another one the second
-                    const int second = W * g / G < unit_at ? 1 : 0;
-                    return p.part + ((g * blocks + rb) * 2 + second) * (int64_t) slot_floats;
-                };
-                float * slot = slot_of(group, unit);
-                if (live) {
-#pragma unroll
-                    for (int e = 0; e < D / 2; e += 4) {
-                        *reinterpret_cast<float4 *>(slot + r * D + at + e) = make_float4(res[e], res[e + 1], res[e + 2], res[e + 3]);
-                    }
-                    if (w == 0) {
+            // ---- the result, or a part's sums into the workspace
+            {
+                const bool whole = it.a == 0 && it.b == it.q.tiles;
+                uint64_t   al;  // where this row goes
+                if (whole) {
+                    const int hd = it.h * p.ratio + row - my_node * p.ratio;
+                    al = reinterpret_cast<uint64_t>(p.o.data + (int64_t) hd * p.o.nb1 + (int64_t) my_node * p.o.nb2 + (int64_t) it.s * p.o.nb3);
+                } else {
+                    // the unit's parts: the first belongs to the piece before the first one that starts inside the unit, in its
+                    // second slot unless the unit is its first; the others are their pieces' first
+                    const int     pa = it.a == 0 ? group + 1 : ln.last(it.unit + TS_LEAST - 1) + 1, floats = ts_slot_floats(slot_rows, D);
+                    const int64_t step = (int64_t) blocks * 2 * floats, part1 = ((int64_t) pa * blocks + rb) * 2 * floats;
+                    const int64_t part0 = part1 - step + (ln.at(pa - 1) <= it.unit - TS_LEAST ? floats : 0);
+                    float *       slot  = p.part + (it.a == 0 ? part0 : part1 + (group - pa) * step);
+                    al = reinterpret_cast<uint64_t>(slot + r * D);
+                    if (live && w == 0) {
                         *reinterpret_cast<float2 *>(slot + slot_rows * D + 2 * r) = make_float2(M, l);
                     }
-                }
-                __threadfence();
-                softmax_barrier();
-                const int64_t g0 = ((unit + 1) * G - 1) / W, g1 = ((unit + it.q.tiles) * G - 1) / W;
-                if (own == 0) {
-                    uint32_t * count = p.counters + g0 * blocks + rb;
-                    *last_f          = atomicAdd(count, 1u) == (uint32_t) (g1 - g0);
-                    if (*last_f) {
-                        *count = 0;
+                    if (own == 0 && it.a == 0) {
+                        *join = { it.s, it.h, ln.last(it.unit + it.q.tiles - TS_LEAST) - pa + 2, its_rows, part0, part1 };
                     }
-                    __threadfence();
                 }
-                softmax_barrier();
-                if (*reinterpret_cast<volatile int *>(last_f)) {
-                    constexpr int E = D / 32;
-                    for (int rj = w * 4 + quad; rj < its_rows; rj += 8) {
-                        float Mj = -INFINITY, lj = 0.0f, o[E];
+                // by whole rows, 32 columns at a time through this warp's part of the exchange
+                const float inv   = whole ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+                float4 *    stage = xch + w * (TS_M * 8) + quad * 32 * 8;
+                const int   type = whole ? p.o.type : (int) KV_F32;
+                const bool  vec = !whole || p.o.vec;
+                if (warp_live) {
 #pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            o[e] = 0.0f;
-                        }
-                        for (int64_t g = g0 + lane; g <= g1; g += 32) {
-                            Mj = fmaxf(Mj, __ldcg(slot_of(g, unit) + slot_rows * D + 2 * rj));
-                        }
+                    for (int c = 0; c < D / 64; c++) {
 #pragma unroll
-                        for (int d = 16; d > 0; d >>= 1) {
-                            Mj = fmaxf(Mj, __shfl_xor_sync(0xffffffffu, Mj, d));
+                        for (int k = 0; k < 8; k++) {
+                            stage[lane * 8 + (k ^ (lane & 7))] = make_float4(res[c * 32 + k * 4] * inv, res[c * 32 + k * 4 + 1] * inv,
+                                                                             res[c * 32 + k * 4 + 2] * inv, res[c * 32 + k * 4 + 3] * inv);
                         }
-#pragma unroll 4
-                        for (int64_t g = g0; g <= g1; g++) {
-                            const float * sl = slot_of(g, unit);
-                            const float2  x  = __ldcg(reinterpret_cast<const float2 *>(sl + slot_rows * D + 2 * rj));
-                            const float   f  = x.x == Mj ? 1.0f : ex2(x.x - Mj);
-                            lj = fmaf(x.y, f, lj);
-                            if (E == 4) {
-                                const float4 v = __ldcg(reinterpret_cast<const float4 *>(sl + rj * D) + lane);
-                                o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]), o[E - 2] = fmaf(v.z, f, o[E - 2]), o[E - 1] = fmaf(v.w, f, o[E - 1]);
-                            } else {
-                                const float2 v = __ldcg(reinterpret_cast<const float2 *>(sl + rj * D) + lane);
-                                o[0] = fmaf(v.x, f, o[0]), o[1] = fmaf(v.y, f, o[1]);
+                        __syncwarp();
+#pragma unroll 1
+                        for (int i = lane >> 3; i < 32; i += 4) {
+                            const int    k = lane & 7;
+                            const float4 f = stage[i * 8 + (k ^ (i & 7))];
+                            char *       to = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, al, i));
+                            if (quad * 32 + i < its_rows) {
+                                ts_store4(to, at + c * 32 + k * 4, f, type, vec);
                             }
                         }
-                        const float inv = lj != 0.0f ? 1.0f / lj : 0.0f;
-                        char *      out = address(rj);
-#pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            o[e] *= inv;
-                        }
-                        if (p.o.type == KV_F32) {
-                            if (p.o.vec && E == 4) {
-                                reinterpret_cast<float4 *>(out)[lane] = make_float4(o[0], o[1], o[E - 2], o[E - 1]);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < E; e++) {
-                                    reinterpret_cast<float *>(out)[lane * E + e] = o[e];
-                                }
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < E; e += 2) {
-                                const uint32_t u = p.o.type == KV_F16 ? ts_pack<false>(o[e], o[e + 1]) : ts_pack<true>(o[e], o[e + 1]);
-                                reinterpret_cast<uint16_t *>(out)[lane * E + e]     = (uint16_t) u;
-                                reinterpret_cast<uint16_t *>(out)[lane * E + e + 1] = (uint16_t) (u >> 16);
-                            }
-                        }
+                        __syncwarp();
                     }
                 }
             }
@@ -903,6 +923,51 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     }
 }
 
+// Joins the parts of units: one row by D / 4 lanes, the parts in their order.
+template <int D>
+__global__ void __launch_bounds__(TJ_ROWS * D / 4) tree_attn_join_kernel(const TreeAttnParams p, int blocks, int slot_rows) {
+    kv8_dep_wait();
+    constexpr int PER = 8;  // parts loaded at a time
+    const TsJoin  t   = *(reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE) + blockIdx.x);
+    const int     rb = (int) blockIdx.x % blocks, lane = threadIdx.x % (D / 4), r = (int) blockIdx.y * TJ_ROWS + threadIdx.x / (D / 4);
+    if (t.parts == 0 || r >= t.rows) {
+        return;
+    }
+    const int64_t step = (int64_t) blocks * 2 * ts_slot_floats(slot_rows, D);
+    auto          part = [&](int k) { return p.part + (k == 0 ? t.part0 : t.part1 + (k - 1) * step); };
+    float         M = -INFINITY, l = 0.0f;
+    float4        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k0 = 0; k0 < t.parts; k0 += PER) {
+        float2 x[PER];
+        float4 v[PER];
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            const float * at = part(min(k0 + k, t.parts - 1));
+            x[k] = *reinterpret_cast<const float2 *>(at + slot_rows * D + 2 * r);
+            v[k] = *(reinterpret_cast<const float4 *>(at + r * D) + lane);
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            top = fmaxf(top, x[k].x);
+        }
+        const float g = M == top ? 1.0f : ex2(M - top);
+        l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            if (k0 + k < t.parts) {
+                const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
+                l = fmaf(x[k].y, f, l);
+                o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
+            }
+        }
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const int   row = rb * TS_M + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
+    ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * lane,
+              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
+}
+
 template <int D, bool BF16, int PARTS>
 cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
     auto             kern = tree_attn_tc_kernel<D, BF16, PARTS>;
@@ -926,8 +991,13 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
         return cudaErrorInvalidValue;
     }
     const int blocks = tree_attn_blocks(p), groups = tree_attn_groups(p, sms);
-    return kv8_launch(kern, dim3((unsigned) (groups * blocks)), TS_THREADS, smem, stream, tmk, tmv, p, blocks, groups,
-                      std::min(p.t.max_nodes * p.ratio, TS_M));
+    const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
+    e = kv8_launch(kern, dim3((unsigned) (groups * blocks)), TS_THREADS, smem, stream, tmk, tmv, p, blocks, groups, rows);
+    if (e != cudaSuccess || p.n_kv <= (2 * TS_LEAST - 1) * TS_N) {
+        return e;  // (no unit is in parts)
+    }
+    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) (groups * blocks), (unsigned) ((rows + TJ_ROWS - 1) / TJ_ROWS)), TJ_ROWS * D / 4, 0, stream, p,
+                      blocks, rows);
 }
 
 template <int D, bool BF16>
@@ -966,7 +1036,6 @@ size_t tree_attn_tc_workspace(const TreeAttnParams & p, int sms) {
 }
 
 cudaError_t launch_tree_attn_tc(TreeAttnParams p, int sms, cudaStream_t stream) {
-    p.counters = p.status + TS_SPACE;
     p.part     = reinterpret_cast<float *>(reinterpret_cast<char *>(p.status) + KV8_WS_ZEROED);
     if (p.D == 64) {
         return p.k.type == KV_BF16 ? launch_d<64, true>(p, sms, stream) : launch_d<64, false>(p, sms, stream);
