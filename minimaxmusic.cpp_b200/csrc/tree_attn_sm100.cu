@@ -6,29 +6,32 @@
 // unit beside one another: groups of RB CTAs, each with one block, walk the same keys at the same time, so a K/V
 // tile comes from HBM once.
 //
-// Split.  The tiles of all units are one line, in the order of sequence and kv head, and each group takes an equal piece of
-// it, found on the device from the lengths: a long sequence is cut over many groups, short ones are several to a
-// group, and no group waits for another.  (A group's piece may so have parts of two units, and whole ones between.)
+// Split, found on the device from the lengths, so that a captured call follows them:
+//   units up to groups   every unit in even parts of about the same size, one part a group (TsPlan)
+//   more units           the tiles of all units are one line, in the order of sequence and kv head, and each group takes an
+//                        equal piece of it: whole units, and a part of one at either end
 // A part of a unit leaves O, m and l in the workspace, and a second kernel joins the parts in their order: by the last
 // CTA to arrive, one SM of 148 would read all parts of a unit (25 us for 9 parts of 96 rows, at one SM's bandwidth).
 // That kernel is left out where the slab is too short for a part.
-//
-// Most of the code runs once in a CTA, and its first run costs what the instruction cache costs: what does not feed the
-// tensor core is in rolled loops or functions.
 //
 // 384 threads:
 //   warp 0       TMA: K and V tiles through one ring, in the order in which the products take them
 //   warp 1       TMEM allocation and every tcgen05.mma: QK(j + 1), then P V(j), P in TMEM over S
 //   warps 2, 3   the V rows of tiles that hold nodes: those behind the last node become zero, and so do elements that are
-//                no numbers (their weight may be 0; who sees such a node gets them added at the end)
-//   warpgroups 1, 2   softmax of the even and the odd tiles, one row per thread, and the sum of their P V in registers:
-//                two streams with maxima and sums of their own, joined at the piece's end
+//                no numbers (their weight may be 0; who sees such a node gets them added at the end); then the next
+//                piece's Q, beside the softmax of this one's last tiles
+//   warpgroups 1, 2   softmax of the even and the odd tiles, one row per thread: two streams with maxima, sums and O of their
+//                own, joined at the piece's end
 //
-// Numerics.  q is brought to [2^14, 2^15) at its row's largest element by a power of two where the cache is F16, and rounded
-// to the cache's type; where the result is F32, or q has another type than the cache, the remainder is a second operand, and
-// so is that of the weights (PARTS 2; the remainder's product runs first, where the accumulator is small).  The tensor core
-// truncates what it adds to an accumulator, up to 2^-23 of it in each step of 16 keys, always towards zero: every tile's
-// P V starts afresh and is added in registers, rounded to nearest.
+// Numerics.  Where q has the cache's type and the result no more bits (PARTS 1), O stays in TMEM and is multiplied there when
+// a row's maximum grows by more than 2^TS_GROW.  The tensor core truncates what it adds to an accumulator, up to 2^-23 of it in
+// each step of 16 keys, always towards zero (measured 7e-7 a tile of 128 keys): up to TS_LONG keys a stream's sum stays within
+// 1e-4, a fifth of F16's half step.  Else (PARTS 2) q is two parts of the cache's type (F16: brought to [2^14, 2^15) at its row's largest
+// element by a power of two), and so are the weights, the remainder's product first, where the accumulator is small;
+// every tile's P V starts afresh and is added in registers, rounded to nearest.
+//
+// Most of the code runs once in a CTA, and its first run costs what the instruction cache costs: what does not feed the
+// tensor core is in rolled loops or functions (a Q staging unrolled over all rows took 5 us, 3.5 as it is).
 #include "fa_decode.cuh"
 #include "tc_sm100.cuh"
 #include "tree.cuh"
@@ -43,14 +46,21 @@ constexpr int TS_THREADS = 384;
 constexpr int TS_M       = 128;  // rows of a block
 constexpr int TS_N       = 128;  // keys of a tile
 constexpr int TS_TMEM    = 512;  // columns: S of two tiles, P V of two tiles
-constexpr int TS_OFF     = 14;   // weights are held times 2^14: F16 keeps 11 bits of one down to 2^-28 of the largest
+constexpr int TS_GROW    = 7;    // (PARTS 1) log2 of what a weight may exceed the maximum of the tiles before by
+constexpr int TS_LONG    = 32768;
+constexpr int TS_SPACE   = 256;  // bytes of the workspace before the list of units in parts
+constexpr int TS_LEAST   = 4;    // tiles of a part, at least: a part costs as much as about two tiles, and the joining kernel
+constexpr int TS_PIECES  = 4;    // pieces that warp 0 may be ahead
+constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for
 constexpr int TJ_ROWS    = 8;    // rows of a joining CTA
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
 constexpr int TS_REGS_SOFTMAX = 208;  // 2 x 208 + 88 = 3 x 168
 constexpr int TS_REGS_ISSUE   = 88;
 static_assert(2 * TS_REGS_SOFTMAX + TS_REGS_ISSUE <= 3 * TS_REGS_LAUNCH, "more registers than the launch has");
-constexpr int TS_SPACE = 256;  // bytes of the workspace before the list of units in parts
-constexpr int TS_LEAST = 2;    // tiles of a part, at least: it costs about as much as a tile
+
+// log2 of what a weight at the maximum is held as: F16 keeps 11 bits of one down to 2^-(14 + offset) of it, and holds 2^15
+template <int PARTS>
+constexpr float TS_OFF = PARTS == 2 ? 14.0f : 15.0f - TS_GROW;
 
 template <int D, int PARTS>
 struct TsSmem {
@@ -58,17 +68,17 @@ struct TsSmem {
     static constexpr int QT     = HALVES * TS_M * 128;
     static constexpr int KT     = HALVES * TS_N * 128;
     static constexpr int NS     = D == 128 ? (PARTS == 2 ? 4 : 5) : 8;  // tiles in the ring
-    static constexpr int XCH    = 2 * TS_M * 32 * 4;                    // exchange of the two streams' sums, in Q's place
-    static constexpr int Q_ALL  = PARTS * QT > XCH ? PARTS * QT : XCH;
     static constexpr int OFF_Q    = 0;
-    static constexpr int OFF_RING = OFF_Q + Q_ALL;
-    static constexpr int OFF_ANC  = OFF_RING + NS * KT;           // [TREE_MAX][TREE_MAX / 32] bits
+    static constexpr int OFF_RING = OFF_Q + PARTS * QT;
+    static constexpr int OFF_XCH  = OFF_RING + NS * KT;           // [stream][row] 16 columns
+    static constexpr int OFF_ANC  = OFF_XCH + 2 * TS_M * 64;      // [TREE_MAX][TREE_MAX / 32] bits
     static constexpr int OFF_PAR  = OFF_ANC + TREE_MAX * (TREE_MAX / 32) * 4;
-    static constexpr int OFF_F    = OFF_PAR + TREE_MAX * 4;       // [row] factors
-    static constexpr int OFF_ML   = OFF_F + TS_M * 4;             // [stream][row] (m, l)
+    static constexpr int OFF_F    = OFF_PAR + TREE_MAX * 4;       // [2 pieces][row] factors
+    static constexpr int OFF_ML   = OFF_F + 2 * TS_M * 4;         // [stream][row] (m, l)
     static constexpr int OFF_BAR  = OFF_ML + 2 * TS_M * 8;
-    static constexpr int OFF_MISC = OFF_BAR + 48 * 8;
-    static constexpr int TOTAL    = OFF_MISC + 256 + 1024;        // + alignment
+    static constexpr int OFF_PIECE = OFF_BAR + 40 * 8;            // [TS_PIECES]
+    static constexpr int OFF_MISC  = OFF_PIECE + TS_PIECES * 48;
+    static constexpr int TOTAL     = OFF_MISC + 32 + 1024;        // + alignment
 };
 static_assert(TsSmem<128, 1>::TOTAL <= 232448 && TsSmem<128, 2>::TOTAL <= 232448 && TsSmem<64, 2>::TOTAL <= 232448, "shared memory");
 
@@ -77,17 +87,20 @@ enum : int {
     TB_EMPTY  = 8,   // [8] products
     TB_SFULL  = 16,  // [2]
     TB_PREADY = 18,  // [2] 128 softmax threads
-    TB_OFULL  = 20,  // [2]
+    TB_OFULL  = 20,  // [2] a tile's P V (PARTS 1: the last of a piece)
     TB_OFREE  = 22,  // [2] 128 softmax threads
-    TB_QREADY = 24,  // 256
-    TB_LOOK   = 25,  // warp 1: a V tile with nodes is there
-    TB_FIX    = 26,  // 64 threads of warps 2, 3: it can be taken
-    TB_DONE   = 27,
-    TB_COUNT  = 28,
+    TB_QREADY = 24,  // 64
+    TB_QFREE  = 25,  // the last QK of a piece
+    TB_LOOK   = 26,  // warp 1: a V tile with nodes is there
+    TB_FIX    = 27,  // 64 threads of warps 2, 3: it can be taken
+    TB_DONE   = 28,
+    TB_PIECE  = 29,  // [TS_PIECES] warp 0
+    TB_PFREE  = 33,  // [TS_PIECES] the 11 other warps
+    TB_COUNT  = 37,
 };
 
 __host__ __device__ constexpr uint32_t ts_arrivals(int b) {
-    return b == TB_QREADY ? 256u : b == TB_FIX ? 64u : ((b >= TB_PREADY && b < TB_OFULL) || (b >= TB_OFREE && b < TB_QREADY)) ? 128u : 1u;
+    return b >= TB_PFREE ? (uint32_t) (TS_THREADS / 32 - 1) : b == TB_QREADY || b == TB_FIX ? 64u : b == TB_PREADY || b == TB_PREADY + 1 || b == TB_OFREE || b == TB_OFREE + 1 ? 128u : 1u;
 }
 
 // kind::f16 instruction descriptor: F16 x F16 or BF16 x BF16 -> F32, M = 128
@@ -112,8 +125,36 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t * r) {
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t * r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16_wait(uint32_t * r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
 __device__ __forceinline__ void softmax_barrier() {  // the 256 threads of both streams
     asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
+__device__ __forceinline__ bool softmax_all(bool x) {  // the same, and whether x holds for all of them
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(x ? 1u : 0u)
+        : "memory");
+    return all != 0;
 }
 
 template <bool BF16>
@@ -149,9 +190,12 @@ __device__ __forceinline__ float2 ts_unpack(uint32_t u) {
     return BF16 ? bf2_to_f2(u) : h2_to_f2(u);
 }
 
-// (functions of their own: see the instruction cache above)
-__device__ __noinline__ float ts_tanh(float x) {
-    return tanhf(x);
+// tanh within 4e-7 of its value: (1 - e) / (1 + e) with e = exp(-2 |x|), below 1/4 its series (a call would not leave the
+// registers that the softmax has)
+__device__ __forceinline__ float ts_tanh(float x) {
+    const float a = fabsf(x), e = ex2(-2.0f * LOG2E * a), x2 = x * x;
+    const float t = __fdividef(1.0f - e, 1.0f + e), p = fmaf(fmaf(fmaf(-17.0f / 315.0f, x2, 2.0f / 15.0f), x2, -1.0f / 3.0f) * x2, a, a);
+    return copysignf(a < 0.25f ? p : t, x);
 }
 
 // elements [e0, e0 + E) of a row that is not aligned: F32, or 16-bit pairs
@@ -170,6 +214,12 @@ __device__ __noinline__ uint4 ts_load_elements(const char * row, bool f32, int e
         }
     }
     return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
+// eight 16-bit elements that are not aligned
+__device__ __forceinline__ uint4 ts_load8(const char * at) {
+    const uint16_t * h = reinterpret_cast<const uint16_t *>(at);
+    return make_uint4(h[0] | (uint32_t) h[1] << 16, h[2] | (uint32_t) h[3] << 16, h[4] | (uint32_t) h[5] << 16, h[6] | (uint32_t) h[7] << 16);
 }
 
 // Floats of a part: O of its rows, then m and l of each; a multiple of 16 bytes.
@@ -244,48 +294,285 @@ struct TsLine {
     }
 };
 
-// The pieces of a group: tiles [a, b) of unit (s, h), one after another.  Every role walks them by itself.
-struct TsPieces {
-    const TreeAttnParams & p;
-    int                    s, first, x, end;  // first: of sequence s on the line of tiles; end: before its move to a border
-    TsSeq                  q;
-    int                    h, a, b, unit;     // unit: where the unit starts
+// Tiles [a, b) of a unit, for one block of its rows, as warp 0 tells the others.
+struct __align__(16) TsPiece {
+    int     s, h, a, b;
+    int     rows;                   // rows of the block; 0: there is no further piece
+    int     L, nodes, keys, tiles;  // of the sequence
+    int     unit;                   // where the unit starts
+    int64_t slot;                   // floats, where it is a part
+};
 
-    __device__ __forceinline__ TsPieces(const TreeAttnParams & p_, int s_, int first_, int x_, int end_)
-        : p(p_), s(s_), first(first_), x(x_), end(end_), q{ 0, 0, 0, 0 }, h(0), a(0), b(0), unit(0) {
-        if (x < end) {
-            q = ts_seq(p, s);
-            const int u = first + (x - first) / q.tiles * q.tiles;
-            x           = TsLine::border(x, u, q.tiles);
+// A group's pieces, one after another.
+struct TsPlan {
+    const TreeAttnParams & p;
+    int                    group, rb, blocks, floats;  // floats of a part's slot; a group has two
+    int                    even;                       // 0, or the tiles of a part, at most
+    TsLine                 ln;
+    int                    s, first, x, end;  // first: of sequence s on the line (even: among the parts); end: before its move to a border
+    TsSeq                  q;
+
+    __device__ __forceinline__ TsPlan(const TreeAttnParams & p_, int group_, int groups, int rb_, int blocks_, int floats_)
+        : p(p_), group(group_), rb(rb_), blocks(blocks_), floats(floats_), even(0), ln(0, 1), s(0), first(0), x(0), end(0), q{ 0, 0, 0, 0 } {
+        // each lane sums some sequences; all tiles are fewer than 2^30 (checked by the host)
+        const int lane = threadIdx.x & 31, each = (p.n_seq + 31) / 32, s0 = min(lane * each, p.n_seq), s1 = min(s0 + each, p.n_seq);
+        int       mine = 0, units = 0, most = 0;
+#pragma unroll 1
+        for (int i = s0; i < s1; i++) {
+            const int n = ts_seq(p, i).tiles;
+            mine += n, units += n > 0, most = max(most, n);
+        }
+        const int W = __reduce_add_sync(0xffffffffu, mine) * p.n_head_kv, U = __reduce_add_sync(0xffffffffu, units) * p.n_head_kv;
+        most = __reduce_max_sync(0xffffffffu, most);
+        int from, to;
+        if (p.n_seq <= TS_EVEN && U <= groups) {
+            // the fewest tiles to a part that need no more than all groups: each lane tries one of 32 numbers between what
+            // even shares would be and what is enough
+            const int lo = max(TS_LEAST, (W + groups - 1) / groups);
+            const int hi = max(lo, U < groups ? min(most, (W + groups - U - 1) / (groups - U)) : most);
+            const int t  = lo + lane * ((hi - lo + 30) / 31);
+            int       parts = 0;
+#pragma unroll 1
+            for (int i = 0; i < p.n_seq; i++) {
+                parts += (ts_seq(p, i).tiles + t - 1) / t;
+            }
+            const unsigned fits = __ballot_sync(0xffffffffu, parts * p.n_head_kv <= groups);
+            even = __shfl_sync(0xffffffffu, t, __ffs(fits) - 1);  // (the last lane's fits)
+            mine = 0;
+#pragma unroll 1
+        for (int i = s0; i < s1; i++) {
+                mine += (ts_seq(p, i).tiles + even - 1) / even;
+            }
+            from = group, to = group + 1;
+        } else {
+            ln   = TsLine(W, groups);
+            from = group < ln.G ? ln.at(group) : W, to = group < ln.G ? ln.at(group + 1) : W;
+        }
+        mine *= p.n_head_kv;
+        int at = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, at, d);
+            at += lane >= d ? y : 0;
+        }
+        at -= mine;
+        const unsigned here = __ballot_sync(0xffffffffu, from < to && from >= at && from < at + mine);  // it starts among this lane's
+        if (here == 0) {
+            return;  // (nothing for this group)
+        }
+        int i = s0;
+        if (here >> lane & 1u) {
+#pragma unroll 1
+            for (;; i++) {
+                const int n = weight(ts_seq(p, i).tiles);
+                if (from < at + n) {
+                    break;
+                }
+                at += n;
+            }
+        }
+        const int src = __ffs(here) - 1;
+        s = __shfl_sync(0xffffffffu, i, src), first = __shfl_sync(0xffffffffu, at, src);
+        q = ts_seq(p, s);
+        x = from, end = to;
+        if (!even) {
+            x = TsLine::border(x, first + (x - first) / q.tiles * q.tiles, q.tiles);
         }
     }
 
-    // the next piece that has rows in block rb
-    __device__ __forceinline__ bool next(int rb) {
+    // a sequence's length on the line, or its parts
+    __device__ __forceinline__ int weight(int tiles) const {
+        return (even ? (tiles + even - 1) / even : tiles) * p.n_head_kv;
+    }
+
+    // the next piece that has rows in this block
+    __device__ __forceinline__ TsPiece next() {
+        TsPiece c = {};
+#pragma unroll 1
         while (x < end) {
-            const int all = q.tiles * p.n_head_kv;
+            const int all = weight(q.tiles);
             if (x - first >= all) {
                 first += all;
                 q = ts_seq(p, ++s);
                 continue;
             }
-            if (q.nodes * p.ratio <= rb * TS_M) {  // (this block is empty: on to the next sequence)
+            const int rows = q.nodes * p.ratio - rb * TS_M;
+            if (rows <= 0) {  // (the block is empty: on to the next sequence)
                 x = first + all;
                 continue;
             }
-            h    = (x - first) / q.tiles;
-            unit = first + h * q.tiles;
-            a    = x - unit;
-            b    = unit + q.tiles <= end ? q.tiles : TsLine::border(end, unit, q.tiles) - unit;
-            if (b <= a) {
-                return false;
+            c.s = s, c.L = q.L, c.nodes = q.nodes, c.keys = q.keys, c.tiles = q.tiles;
+            if (even) {
+                const int parts = (q.tiles + even - 1) / even, i = x - first;
+                c.h          = i / parts;
+                const int k  = i - c.h * parts;
+                c.unit = x - k, c.a = k * q.tiles / parts, c.b = (k + 1) * q.tiles / parts;
+                x++;
+            } else {
+                c.h    = (x - first) / q.tiles;
+                c.unit = first + c.h * q.tiles;
+                c.a    = x - c.unit;
+                c.b    = c.unit + q.tiles <= end ? q.tiles : TsLine::border(end, c.unit, q.tiles) - c.unit;
+                x      = c.b > c.a ? c.unit + c.b : end;
             }
-            x = unit + b;
-            return true;
+            c.rows = c.b > c.a ? min(rows, TS_M) : 0;
+            c.slot = part(c, second(c), group - second(c) + 1);
+            return c;
         }
-        return false;
+        return c;
+    }
+
+    // the group that has the second part of a piece's unit
+    __device__ __forceinline__ int second(const TsPiece & c) const {
+        return even ? c.unit + 1 : c.a == 0 ? group + 1 : ln.last(c.unit + TS_LEAST - 1) + 1;
+    }
+
+    // Where a unit's parts are: the first in a slot of the group before `g`, its second one unless the unit is the first that
+    // the group has; the others in the first slots of g and the groups behind it.
+    __device__ __forceinline__ int64_t part(const TsPiece & c, int g, int k) const {
+        const int64_t slots = ((int64_t) (g - 1 + k) * blocks + rb) * 2;
+        return (slots + (k == 0 && !even && ln.at(g - 1) <= c.unit - TS_LEAST ? 1 : 0)) * floats;
+    }
+
+    // what the joining kernel has to know of a unit, from its first part
+    __device__ __forceinline__ TsJoin join(const TsPiece & c) const {
+        const int g = second(c), parts = even ? (c.tiles + even - 1) / even : ln.last(c.unit + c.tiles - TS_LEAST) - g + 2;
+        return { c.s, c.h, parts, c.rows, part(c, g, 0), part(c, g, 1) };
     }
 };
+
+// Rows ra .. ra + 15 of a block's Q for the products, by a warp; rows that do not count are zeros.
+template <int D, bool BF16, int PARTS>
+__device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPiece & it, int rb, int ra, char * qs, float * factors, int lane) {
+    constexpr int E = D / 32, QT = TsSmem<D, PARTS>::QT;
+    const int     in = it.rows - ra;
+    // lane i, and 16 + i: the address of row i
+    const int      rl = rb * TS_M + ra + (lane & 15), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
+    const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
+    // (not 0, whose product with the -inf of a key that is not seen would be no number)
+    const float    by = fmaxf(fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E), 0x1p-126f);
+    if constexpr (PARTS == 1) {
+        // as it is, but for the sign of the scale: 16 bytes by each lane, all loads in flight
+        constexpr int  PER = D / 8, N = D / 16;  // lanes of a row, loads of a lane
+        const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+        const int      ck = lane % PER;
+        uint4          u[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int    rw  = i * (32 / PER) + lane / PER;
+            const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, rw));
+            u[i] = make_uint4(0, 0, 0, 0);
+            if (rw < in && p.q.vec) {
+                u[i] = *reinterpret_cast<const uint4 *>(src + ck * 16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int rw = i * (32 / PER) + lane / PER;
+            *reinterpret_cast<uint4 *>(qs + (ck / 8) * (TS_M * 128) + (ra + rw) * 128 + (((ck % 8) ^ (rw & 7)) << 4)) =
+                make_uint4(u[i].x ^ flip, u[i].y ^ flip, u[i].z ^ flip, u[i].w ^ flip);
+        }
+        if (!p.q.vec) {
+#pragma unroll 1
+            for (int rw = lane / PER; rw < 16; rw += 32 / PER) {
+                const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, rw));
+                if (rw < in) {
+                    const uint4 f = ts_load8(src + ck * 16);
+                    *reinterpret_cast<uint4 *>(qs + (ck / 8) * (TS_M * 128) + (ra + rw) * 128 + (((ck % 8) ^ (rw & 7)) << 4)) =
+                        make_uint4(f.x ^ flip, f.y ^ flip, f.z ^ flip, f.w ^ flip);
+                }
+            }
+        }
+        if (lane < 16) {
+            factors[ra + lane] = by;
+        }
+    } else {
+        // two parts of the cache's type.  A row with an infinity or NaN becomes zeros with a factor of NaN
+        const bool  f32 = p.q.type == KV_F32, f16 = p.q.type == KV_F16;
+        const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+        const int   e0 = lane * E;
+        if ((lane & 15) < in) {  // all rows are on their way while the first are worked on
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(al + (lane >> 4) * 128));
+            if (f32 && D == 128) {
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(al + 256 + (lane >> 4) * 128));
+            }
+        }
+        char * to = qs + ra * 128 + (e0 / 64) * (TS_M * 128) + (e0 % 8) * 2;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 16; i0 += 4) {
+            float x[4][E];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i0 + i));
+                uint4        u   = make_uint4(0, 0, 0, 0);  // F32 values, or 16-bit pairs
+                if (i0 + i < in) {
+                    if (!p.q.vec) {
+                        u = ts_load_elements<E>(src, f32, e0);
+                    } else if (E == 4 && f32) {
+                        u = *reinterpret_cast<const uint4 *>(src + lane * 16);
+                    } else if (E == 4 || f32) {
+                        const uint2 f = *reinterpret_cast<const uint2 *>(src + lane * 8);
+                        u.x = f.x, u.y = f.y;
+                    } else {
+                        u.x = *reinterpret_cast<const uint32_t *>(src + lane * 4);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const uint32_t pair = e ? u.y : u.x;
+                    const float2   a    = f16 ? h2_to_f2(pair) : bf2_to_f2(pair);
+                    x[i][e]     = f32 ? __uint_as_float((&u.x)[e]) : a.x;
+                    x[i][e + 1] = f32 ? __uint_as_float((&u.x)[e + 1]) : a.y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
+                }
+                top = __reduce_max_sync(0xffffffffu, top);
+                const bool  odd = top >= 0x7f800000u;
+                const int   ex  = BF16 ? 0 : (top == 0 || odd ? 0 : max((int) (top >> 23) - 127, -112)) - 14;
+                const float dn  = odd ? 0.0f : __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
+                uint32_t    hi[E / 2], lo[E / 2];
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float a = odd ? 0.0f : x[i][e] * dn, b = odd ? 0.0f : x[i][e + 1] * dn;
+                    hi[e / 2]      = ts_pack<BF16>(a, b);
+                    const float2 f = ts_unpack<BF16>(hi[e / 2]);
+                    lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
+                }
+                char * at = to + (i0 + i) * 128 + ((((e0 % 64) / 8) ^ ((i0 + i) & 7)) << 4);  // (ra: a multiple of 8)
+                if (E == 4) {
+                    *reinterpret_cast<uint2 *>(at)      = make_uint2(hi[0], hi[E / 2 - 1]);
+                    *reinterpret_cast<uint2 *>(at + QT) = make_uint2(lo[0], lo[E / 2 - 1]);
+                } else {
+                    *reinterpret_cast<uint32_t *>(at)      = hi[0];
+                    *reinterpret_cast<uint32_t *>(at + QT) = lo[0];
+                }
+                if (lane == i) {
+                    factors[ra + i0 + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
+                }
+            }
+        }
+    }
+}
+
+// The next piece that warp 0 tells of; false: there is none, or it did not come in time.  By whole warps.
+__device__ __forceinline__ bool ts_take(TsPiece & it, const TsPiece * told, uint64_t * bar, uint32_t pieces, int lane, uint64_t deadline) {
+    const uint32_t k = pieces % TS_PIECES;
+    if (!dn_wait_warp(&bar[TB_PIECE + k], (pieces / TS_PIECES) & 1, deadline)) {
+        return false;
+    }
+    it = told[k];
+    __syncwarp();
+    if (lane == 0) {
+        dn_mbar_arrive(&bar[TB_PFREE + k]);
+    }
+    return it.rows > 0;
+}
 
 template <int D, bool BF16, int PARTS>
 __global__ void __launch_bounds__(TS_THREADS, 1)
@@ -296,13 +583,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     extern __shared__ __align__(16) char smem_raw[];
     char *     smem      = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t * bar       = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
-    uint32_t * misc      = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
-    uint32_t * tmem_slot = misc;
-    int *      abort_f   = reinterpret_cast<int *>(misc + 1);
-    int *      start_s   = reinterpret_cast<int *>(misc + 3);
-    int *      line      = reinterpret_cast<int *>(misc + 4);       // the whole line's tiles, the first one of start_s
-    int *      dirty     = reinterpret_cast<int *>(misc + 8);       // a V row of the piece's nodes held what is no number
-    int *      sums      = reinterpret_cast<int *>(misc + 16);      // [12] warps' counts
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
+    int *      abort_f   = reinterpret_cast<int *>(smem + L::OFF_MISC + 4);
+    int *      dirty     = reinterpret_cast<int *>(smem + L::OFF_MISC + 8);  // [2 pieces] a V row of a node held what is no number
     float *    factors   = reinterpret_cast<float *>(smem + L::OFF_F);
     float2 *   ml        = reinterpret_cast<float2 *>(smem + L::OFF_ML);
     uint32_t * anc       = reinterpret_cast<uint32_t *>(smem + L::OFF_ANC);
@@ -313,7 +596,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         for (int i = 0; i < TB_COUNT; i++) {
             mbar_init(&bar[i], ts_arrivals(i));
         }
-        *abort_f = 0, *start_s = 0, line[1] = 0, *dirty = 0;
+        *abort_f = 0, dirty[0] = 0, dirty[1] = 0;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -322,68 +605,28 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     }
     kv8_dep_wait();
     const uint64_t deadline = global_timer_ns() + p.timeout_ns;
-
-    // ---- the group's piece of the line of tiles
-    const int group = (int) blockIdx.x / blocks, rb = (int) blockIdx.x % blocks;
-    TsJoin *  join  = reinterpret_cast<TsJoin *>(reinterpret_cast<char *>(p.status) + TS_SPACE) + blockIdx.x;
-    if (tid == 0) {
-        join->parts = 0;
-    }
-    {
-        // each thread sums some sequences' tiles of one kv head; all tiles are fewer than 2^30 (checked by the host)
-        const int each = (p.n_seq + TS_THREADS - 1) / TS_THREADS, s0 = min(tid * each, p.n_seq), s1 = min(s0 + each, p.n_seq);
-        int       mine = 0;
-        for (int s = s0; s < s1; s++) {
-            mine += ts_seq(p, s).tiles;
-        }
-        int upto = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, d);
-            upto += lane >= d ? y : 0;
-        }
-        if (lane == 31) {
-            sums[warp] = upto;
-        }
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        int before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < TS_THREADS / 32; w++) {
-            before += w < warp ? sums[w] : 0;
-            all += sums[w];
-        }
-        const TsLine ln(all * p.n_head_kv, groups);
-        const int    from = ln.at(group);
-        int          at   = (before + upto - mine) * p.n_head_kv;
-        if (group < ln.G && from >= at && from < at + mine * p.n_head_kv) {  // it starts among this thread's
-            int s = s0;
-            for (;; s++) {
-                const int n = ts_seq(p, s).tiles * p.n_head_kv;
-                if (from < at + n) {
-                    break;
-                }
-                at += n;
-            }
-            *start_s = s, line[1] = at;
-        }
-        if (tid == 0) {
-            line[0] = ln.W;
-        }
-        __syncthreads();
-    }
+    const int      rb = (int) blockIdx.x % blocks;
+    TsPiece *      told = reinterpret_cast<TsPiece *>(smem + L::OFF_PIECE);
+    TsPiece        it;
+    uint32_t       pieces = 0;  // that a warp has taken
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const TsLine   ln(line[0], groups);
-    TsPieces       it(p, *start_s, line[1], group < ln.G ? ln.at(group) : ln.W, group < ln.G ? ln.at(group + 1) : ln.W);
 
     if (wg == 0) {
         regs_dec<TS_REGS_ISSUE>();
         bool ok = true;
+        auto next = [&] {
+            return ok && ts_take(it, told, bar, pieces, lane, deadline);
+        };
         if (warp == 0) {
-            // =================================================== TMA
+            // =================================================== the pieces, TMA
+            TsPlan   plan(p, (int) blockIdx.x / blocks, groups, rb, blocks, ts_slot_floats(slot_rows, D));
+            TsJoin * join = reinterpret_cast<TsJoin *>(reinterpret_cast<char *>(p.status) + TS_SPACE) + blockIdx.x;
             if (lane == 0) {
                 uint32_t c = 0;
+                join->parts = 0;
                 auto     load = [&](const CUtensorMap * tm, int tile) {
                     const int slot = (int) (c % NS);
                     if (ok && c >= (uint32_t) NS && !mbar_wait_bounded(&bar[TB_EMPTY + slot], (c / NS - 1) & 1, deadline)) {
@@ -398,15 +641,30 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         c++;
                     }
                 };
-                while (ok && it.next(rb)) {
+                do {
+                    it = plan.next();
+                    if (pieces >= (uint32_t) TS_PIECES && !mbar_wait_bounded(&bar[TB_PFREE + pieces % TS_PIECES], (pieces / TS_PIECES - 1) & 1, deadline)) {
+                        ok = false;
+                        break;
+                    }
+                    told[pieces % TS_PIECES] = it;
+                    dn_mbar_arrive(&bar[TB_PIECE + pieces % TS_PIECES]);
+                    pieces++;
+                    if (it.rows == 0) {
+                        break;
+                    }
+                    if (it.a == 0 && it.b < it.tiles) {
+                        *join = plan.join(it);
+                    }
                     load(&tmk, it.a);
+#pragma unroll 1
                     for (int j = it.a; ok && j < it.b; j++) {
                         if (j + 1 < it.b) {
                             load(&tmk, j + 1);
                         }
                         load(&tmv, j);
                     }
-                }
+                } while (ok);
                 if (!ok) {  // copies that are under way have to land
                     const uint64_t limit = global_timer_ns() + p.timeout_ns;
                     for (uint32_t i = c > (uint32_t) NS ? c - NS : 0; i < c; i++) {
@@ -426,81 +684,108 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
                 tc_fence_after();
             };
-            uint32_t c = 0, tc = 0, fixes = 0, pieces = 0;
-            auto     qk = [&](uint32_t t) {
-                const int slot = (int) (c % NS), buf = (int) (t & 1);
-                wait(TB_FULL + slot, c / NS);
-#pragma unroll 1
-                for (int part = PARTS - 1; part >= 0; part--) {
-                    uint64_t qa = q_d + (uint64_t) ((part * L::QT) >> 4), kb = k_d + (uint64_t) ((slot * L::KT) >> 4);
-#pragma unroll
-                    for (int hf = 0; hf < L::HALVES; hf++) {
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            umma_f16(tmem + (uint32_t) (buf * TS_N), qa + (uint64_t) (2 * k), kb + (uint64_t) (2 * k), id_qk, PARTS - 1 - part + hf + k > 0 ? 1u : 0u);
-                        }
-                        qa += (TS_M * 128) >> 4, kb += (TS_N * 128) >> 4;
-                    }
-                }
-                umma_commit(&bar[TB_EMPTY + slot]);
-                umma_commit(&bar[TB_SFULL + buf]);
-                c++;
-            };
-            while (it.next(rb)) {
+            uint32_t c = 0, tc = 0, looks = 0, used0 = 0, used1 = 0;  // used: pieces in which a stream had tiles
+            while (next()) {
                 wait(TB_QREADY, pieces++);
-                qk(tc);
-                for (int j = it.a; j < it.b; j++, tc++) {
+#pragma unroll 1
+                for (int j = it.a - 1; j < it.b; j++) {  // QK(j + 1), then P V(j)
                     if (j + 1 < it.b) {
-                        qk(tc + 1);
+                        const int slot = (int) (c % NS), buf = (int) ((tc + (j >= it.a ? 1 : 0)) & 1);
+                        wait(TB_FULL + slot, c / NS);
+#pragma unroll 1
+                        for (int part = PARTS - 1; part >= 0; part--) {
+                            uint64_t qa = q_d + (uint64_t) ((part * L::QT) >> 4), kb = k_d + (uint64_t) ((slot * L::KT) >> 4);
+#pragma unroll
+                            for (int hf = 0; hf < L::HALVES; hf++) {
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    umma_f16(tmem + (uint32_t) (buf * TS_N), qa + (uint64_t) (2 * k), kb + (uint64_t) (2 * k), id_qk,
+                                             PARTS - 1 - part + hf + k > 0 ? 1u : 0u);
+                                }
+                                qa += (TS_M * 128) >> 4, kb += (TS_N * 128) >> 4;
+                            }
+                        }
+                        umma_commit(&bar[TB_EMPTY + slot]);
+                        umma_commit(&bar[TB_SFULL + buf]);
+                        c++;
+                        if (j + 2 == it.b) {
+                            umma_commit(&bar[TB_QFREE]);
+                        }
+                    }
+                    if (j < it.a) {
+                        continue;
                     }
                     const int slot = (int) (c % NS), buf = (int) (tc & 1);
                     wait(TB_FULL + slot, c / NS);
-                    const bool nodes = (j + 1) * TS_N > it.q.L;
+                    const bool nodes = (j + 1) * TS_N > it.L;
                     if (nodes && lane == 0) {
                         dn_mbar_arrive(&bar[TB_LOOK]);
                     }
                     wait(TB_PREADY + buf, tc >> 1);
-                    if (tc >= 2) {
+                    if (PARTS == 2 && tc >= 2) {
                         wait(TB_OFREE + buf, (tc >> 1) - 1);
                     }
+                    if (PARTS == 1 && j - it.a < 2) {  // the stream's first tile of the piece
+                        const uint32_t before = buf ? used1++ : used0++;
+                        if (before > 0) {
+                            wait(TB_OFREE + buf, before - 1);
+                        }
+                    }
                     if (nodes) {
-                        wait(TB_FIX, fixes++);
+                        wait(TB_FIX, looks++);
                     }
 #pragma unroll 1
                     for (int part = PARTS - 1; part >= 0; part--) {
-                        uint32_t a = tmem + (uint32_t) (buf * TS_N + part * 16);
-                        uint64_t b = v_d + (uint64_t) ((slot * L::KT) >> 4);
+                        uint32_t pa = tmem + (uint32_t) (buf * TS_N + part * 16);
+                        uint64_t vb = v_d + (uint64_t) ((slot * L::KT) >> 4);
+                        uint32_t add = PARTS == 2 ? (uint32_t) (PARTS - 1 - part) : j - it.a < 2 ? 0u : 1u;
 #pragma unroll
                         for (int k = 0; k < 8; k++) {  // P of 32 keys: 16 columns, then 16 of its remainder
-                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), a + (uint32_t) ((k >> 1) * 16 * PARTS + (k & 1) * 8), b + (uint64_t) ((k * 16 * 128) >> 4),
-                                        id_pv, PARTS - 1 - part + k > 0 ? 1u : 0u);
+                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), pa + (uint32_t) ((k >> 1) * 16 * PARTS + (k & 1) * 8), vb + (uint64_t) ((k * 16 * 128) >> 4),
+                                        id_pv, add);
+                            add = 1u;
                         }
                     }
                     umma_commit(&bar[TB_EMPTY + slot]);
-                    umma_commit(&bar[TB_OFULL + buf]);
-                    c++;
+                    if (PARTS == 2 || j + 2 >= it.b) {
+                        umma_commit(&bar[TB_OFULL + buf]);
+                    }
+                    c++, tc++;
                 }
             }
             // every product issued has to be complete before TMEM and shared memory are given up
             umma_commit(&bar[TB_DONE]);
             dn_wait_warp(&bar[TB_DONE], 0, global_timer_ns() + p.timeout_ns);
         } else {
-            // =================================================== V rows of tiles that hold nodes
+            // =================================================== V rows of tiles that hold nodes, and the next piece's Q
             const int t64 = tid - 64;
-            uint32_t  c = 0, fixes = 0;
-            while (it.next(rb)) {
+            uint32_t  c = 0, looks = 0;
+            while (next()) {
                 const int n = it.b - it.a;
-                for (int j = max(it.a, it.q.L / TS_N); j < it.b; j++) {
+                if (pieces > 0) {
+                    if (ok && !dn_wait_warp(&bar[TB_QFREE], (pieces - 1) & 1, deadline)) {
+                        ok = false;
+                    }
+#pragma unroll 1
+                    for (int ra = (warp & 1) * 16; ra < TS_M; ra += 32) {
+                        ts_stage16<D, BF16, PARTS>(p, it, rb, ra, smem + L::OFF_Q, factors + (pieces & 1) * TS_M, lane);
+                    }
+                    fence_proxy_async_smem();
+                    dn_mbar_arrive(&bar[TB_QREADY]);
+                }
+#pragma unroll 1
+                for (int j = max(it.a, it.L / TS_N); j < it.b; j++) {
                     const uint32_t i    = c + (uint32_t) (2 * (j - it.a) + (j + 1 < it.b ? 2 : 1));  // its place in the ring's order
                     const int      slot = (int) (i % NS);
                     // (warp 1 has seen the tile land and keeps its place until it is looked at, so that the second wait
                     // finds the phase it names)
-                    if (ok && (!dn_wait_warp(&bar[TB_LOOK], fixes & 1, deadline) || !dn_wait_warp(&bar[TB_FULL + slot], (i / NS) & 1, deadline))) {
+                    if (ok && (!dn_wait_warp(&bar[TB_LOOK], looks & 1, deadline) || !dn_wait_warp(&bar[TB_FULL + slot], (i / NS) & 1, deadline))) {
                         ok = false;
                     }
                     char *    tile = smem + L::OFF_RING + slot * L::KT;
-                    const int r0 = max(0, it.q.L - j * TS_N), end = it.q.keys - j * TS_N;
+                    const int r0 = max(0, it.L - j * TS_N), end = it.keys - j * TS_N;
                     bool      odd = false;
+#pragma unroll 1
                     for (int e = t64; e < (TS_N - r0) * 8 * L::HALVES; e += 64) {
                         const int r  = r0 + e / (8 * L::HALVES), ck = e % (8 * L::HALVES);
                         uint4 *   at = reinterpret_cast<uint4 *>(tile + (ck >> 3) * (TS_N * 128) + r * 128 + (ck & 7) * 16);
@@ -527,13 +812,14 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         }
                     }
                     if (odd) {
-                        atomicExch(dirty, 1);
+                        atomicExch(&dirty[pieces & 1], 1);
                     }
                     fence_proxy_async_smem();
                     dn_mbar_arrive(&bar[TB_FIX]);
-                    fixes++;
+                    looks++;
                 }
                 c += (uint32_t) (2 * n);
+                pieces++;
             }
         }
         if (!ok) {
@@ -547,9 +833,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         const uint32_t s_col = tmem + tl + (uint32_t) (w * TS_N), o_col = tmem + tl + 256u + (uint32_t) (w * D);
         const int      my_node = row / p.ratio;
         const bool     cap = p.softcap > 0.0f;
-        char *         qs  = smem + L::OFF_Q;
-        float4 *       xch = reinterpret_cast<float4 *>(smem + L::OFF_Q);
-        uint32_t       tc = 0;
+        float4 *       give = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + w * (TS_M * 4), *take = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + (w ^ 1) * (TS_M * 4);
+        const uint32_t * bits = anc + min(my_node, TREE_MAX - 1) * (TREE_MAX / 32);
+        uint32_t       tc = 0, used = 0;
         bool           ok = true;
         auto           wait = [&](int b, uint32_t i) {
             if (ok && !dn_wait_warp(&bar[b], i & 1, deadline)) {
@@ -557,103 +843,18 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             }
             tc_fence_after();
         };
-        while (it.next(rb)) {
-            const int  its_rows = min(it.q.nodes * p.ratio - rb * TS_M, TS_M);
+        // (all of them go on, or none: they meet at barriers)
+        while (softmax_all(ts_take(it, told, bar, pieces, lane, deadline))) {
+            const int  its_rows = it.rows;
             const bool live = r < its_rows, warp_live = quad * 32 < its_rows;
-            const int  held = it.q.L, nodes = it.q.nodes;
-            // ---- Q: 16 rows by each warp, all loads in flight, 8 rows at a time
-            {
-                constexpr int  E = D / 32, B = 8;
-                const int      ra = (w * 4 + quad) * 16, e0 = lane * E, in = its_rows - ra;
-                char *         to = qs + (e0 / 64) * (TS_M * 128) + ra * 128 + (e0 % 8) * 2;
-                const float    sign = p.scale < 0.0f ? -1.0f : 1.0f, by = fabsf(cap ? p.scale / p.softcap : p.scale * LOG2E);
-                // lane i: the address of row i
-                const int      rl = rb * TS_M + ra + (lane & 15), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
-                const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
-                uint32_t       u[2][B][E];  // F32 values, or 16-bit pairs in the first half
-                const bool     f32 = p.q.type == KV_F32, f16 = p.q.type == KV_F16;
-#pragma unroll
-                for (int i = 0; i < 2 * B; i++) {
-                    const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i));
-                    uint32_t (&x)[E] = u[i / B][i % B];
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        x[e] = 0u;
-                    }
-                    if (i < in && p.q.vec) {
-                        if (E == 4 && f32) {
-                            const uint4 f = *reinterpret_cast<const uint4 *>(src + lane * 16);
-                            x[0] = f.x, x[1] = f.y, x[E - 2] = f.z, x[E - 1] = f.w;
-                        } else if (E == 4 || f32) {
-                            const uint2 f = *reinterpret_cast<const uint2 *>(src + lane * 8);
-                            x[0] = f.x, x[1] = f.y;
-                        } else {
-                            x[0] = *reinterpret_cast<const uint32_t *>(src + lane * 4);
-                        }
-                    }
-                }
-#pragma unroll 1
-                for (int half = 0; half < 2; half++) {
-                    if (!p.q.vec) {  // by elements, a row after another
-#pragma unroll
-                        for (int i = 0; i < B; i++) {
-                            const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, half * B + i));
-                            if (half * B + i < in) {
-                                const uint4 f = ts_load_elements<E>(src, f32, e0);
-                                u[0][i][0] = f.x, u[0][i][1] = f.y;
-                                if (E == 4) {
-                                    u[0][i][E - 2] = f.z, u[0][i][E - 1] = f.w;
-                                }
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < B; i++) {
-                        float    x[E];
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const float2 a = f16 ? h2_to_f2(u[0][i][e / 2]) : bf2_to_f2(u[0][i][e / 2]);
-                            x[e]     = f32 ? __uint_as_float(u[0][i][e]) : a.x;
-                            x[e + 1] = f32 ? __uint_as_float(u[0][i][e + 1]) : a.y;
-                            top      = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(x[e + 1]) & 0x7fffffffu));
-                        }
-                        top = __reduce_max_sync(0xffffffffu, top);
-                        // a row with an infinity or NaN gives NaN.  F16: the largest element goes to [2^14, 2^15)
-                        const bool  odd = top >= 0x7f800000u;
-                        const int   ex  = BF16 ? 0 : (top == 0 || odd ? 0 : max((int) (top >> 23) - 127, -112)) - 14;
-                        const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
-                        uint32_t    hi[E / 2], lo[E / 2];
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const float a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
-                            hi[e / 2]      = ts_pack<BF16>(a, b);
-                            const float2 f = ts_unpack<BF16>(hi[e / 2]);
-                            lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
-                        }
-                        char * at = to + (half * B + i) * 128 + ((((e0 % 64) / 8) ^ i) << 4);  // ra and B: multiples of 8
-                        if (E == 4) {
-                            *reinterpret_cast<uint2 *>(at) = make_uint2(hi[0], hi[E / 2 - 1]);
-                            if (PARTS == 2) {
-                                *reinterpret_cast<uint2 *>(at + L::QT) = make_uint2(lo[0], lo[E / 2 - 1]);
-                            }
-                        } else {
-                            *reinterpret_cast<uint32_t *>(at) = hi[0];
-                            if (PARTS == 2) {
-                                *reinterpret_cast<uint32_t *>(at + L::QT) = lo[0];
-                            }
-                        }
-                        if (lane == i) {
-                            factors[ra + half * B + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
-                        }
-#pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            u[0][i][e] = u[1][i][e];
-                        }
-                    }
-                }
+            const int  held = it.L, nodes = it.nodes;
+            if (pieces == 0) {
+                ts_stage16<D, BF16, PARTS>(p, it, rb, (w * 4 + quad) * 16, smem + L::OFF_Q, factors, lane);
                 fence_proxy_async_smem();
-                dn_mbar_arrive(&bar[TB_QREADY]);
+                __syncwarp();
+                if (lane < 8) {
+                    dn_mbar_arrive(&bar[TB_QREADY]);
+                }
             }
             // ---- each node's ancestors, where the piece has tiles with nodes
             const bool tail = it.b * TS_N > held;
@@ -663,20 +864,30 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
                 softmax_barrier();
                 if (own < nodes) {
-                    uint32_t * bits = anc + own * (TREE_MAX / 32);
+                    uint32_t * to = anc + own * (TREE_MAX / 32);
 #pragma unroll
                     for (int k = 0; k < TREE_MAX / 32; k++) {
-                        bits[k] = 0;
+                        to[k] = 0;
                     }
                     for (int at = own; at >= 0; at = par[at]) {
-                        bits[at >> 5] |= held + at < p.n_kv ? 1u << (at & 31) : 0u;
+                        to[at >> 5] |= held + at < p.n_kv ? 1u << (at & 31) : 0u;
                     }
                 }
+                softmax_barrier();
             }
-            softmax_barrier();  // (and all of Q's factors are there)
-            const float    f0 = factors[r], factor = cap || f0 != f0 ? 1.0f : f0;
-            const float    fcap = f0 != f0 ? 1.0f : f0;
-            const uint32_t * bits = anc + min(my_node, TREE_MAX - 1) * (TREE_MAX / 32);
+            // ---- where this row goes: the result, or a part's slot
+            const bool whole = it.a == 0 && it.b == it.tiles;
+            const int  type = whole ? p.o.type : (int) KV_F32;
+            uint64_t   al;
+            if (whole) {
+                const int hd = it.h * p.ratio + row - my_node * p.ratio;
+                al = reinterpret_cast<uint64_t>(p.o.data + (int64_t) hd * p.o.nb1 + (int64_t) my_node * p.o.nb2 + (int64_t) it.s * p.o.nb3);
+            } else {
+                al = reinterpret_cast<uint64_t>(p.part + it.slot + r * D);
+            }
+            wait(TB_QREADY, pieces);
+            const float f0 = factors[(pieces & 1) * TS_M + r], factor = cap || f0 != f0 ? 1.0f : f0;
+            const float fcap = f0 != f0 ? 1.0f : f0;
             // which of the 32 keys from k0 on the row sees
             auto seen = [&](int k0) -> uint32_t {
                 const int o = k0 - held;  // in nodes
@@ -687,85 +898,158 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     return 0u;
                 }
                 if (o < 0) {
-                    return (1u << -o) - 1u | bits[0] << -o;
+                    return ((1u << -o) - 1u) | bits[0] << -o;
                 }
                 const uint32_t lo = bits[o >> 5], hi = o + 32 < TREE_MAX ? bits[(o >> 5) + 1] : 0u;
                 return __funnelshift_r(lo, hi, o & 31);
             };
-            float m = -INFINITY, l = 0.0f, acc[D];
+            float m = -INFINITY, l = 0.0f, acc[PARTS == 2 ? D : 1];
+            bool  any = false;  // the stream has a tile of the piece
+            if constexpr (PARTS == 2) {
 #pragma unroll
-            for (int e = 0; e < D; e++) {
-                acc[e] = 0.0f;
+                for (int e = 0; e < D; e++) {
+                    acc[e] = 0.0f;
+                }
             }
+#pragma unroll 1
             for (int j = it.a; j < it.b; j++, tc++) {
                 if ((int) (tc & 1) != w) {
                     continue;
                 }
+                const bool masked = (j + 1) * TS_N > held;
                 wait(TB_SFULL + w, tc >> 1);
-                float g = 1.0f;
-                if (warp_live) {
-                    if (cap) {
+                if (cap && warp_live) {  // s = cap * tanh(S * factor), in log2 units, over S
+#pragma unroll 1
+                    for (int c = 0; c < 8; c++) {
+                        uint32_t v[16];
+                        tmem_ld16(s_col + (uint32_t) (c * 16), v);
+                        tmem_ld16_wait(v);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
+                        }
+                        tmem_st16(s_col + (uint32_t) (c * 16), v);
+                    }
+                    tmem_st_wait();
+                }
+                if constexpr (PARTS == 1) {
+                    if (warp_live) {
+                        uint32_t v[TS_N];
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            tmem_ld32(s_col + (uint32_t) (c * 32), &v[c * 32]);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            tmem_ld_wait_tie(&v[c * 32]);
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                const uint32_t see = live ? seen(j * TS_N + c * 32) : 0u;
+#pragma unroll
+                                for (int e = 0; e < 32; e++) {
+                                    v[c * 32 + e] = see >> e & 1u ? v[c * 32 + e] : 0xff800000u;
+                                }
+                            }
+                        }
+                        float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
+#pragma unroll
+                        for (int e = 2; e < TS_N - 2; e += 4) {
+                            a = fmax3(a, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                            b = fmax3(b, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+                        }
+                        const float top = fmaxf(fmax3(a, __uint_as_float(v[TS_N - 2]), __uint_as_float(v[TS_N - 1])), b);
+                        const float mn   = fmaxf(m, top * factor);
+                        const bool  grew = mn > m + (float) TS_GROW;  // (at first too)
+                        if (any && __any_sync(0xffffffffu, grew)) {
+                            // P V(j - 2) is complete: QK(j) was issued after it
+                            const float g = grew ? ex2(m - mn) : 1.0f;
+                            l *= g;
+#pragma unroll 1
+                            for (int c = 0; c < D / 16; c++) {
+                                uint32_t o[16];
+                                tmem_ld16(o_col + (uint32_t) (c * 16), o);
+                                tmem_ld16_wait(o);
+#pragma unroll
+                                for (int e = 0; e < 16; e++) {
+                                    o[e] = __float_as_uint(__uint_as_float(o[e]) * g);
+                                }
+                                tmem_st16(o_col + (uint32_t) (c * 16), o);
+                            }
+                        }
+                        m = grew ? mn : m;
+                        const float    nm = (m == -INFINITY ? 0.0f : -m) + TS_OFF<PARTS>;
+                        const uint64_t nm2 = f2pack(nm, nm), fa2 = f2pack(factor, factor);
+                        uint64_t       sum2 = 0ull;
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            uint32_t hi[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                float x, y;
+                                f2unpack(ffma2(f2pack(__uint_as_float(v[c * 32 + 2 * i]), __uint_as_float(v[c * 32 + 2 * i + 1])), fa2, nm2), x, y);
+                                const uint64_t p2 = f2pack(ex2(x), ex2(y));
+                                sum2 = fadd2(sum2, p2);
+                                f2unpack(p2, x, y);
+                                hi[i] = ts_pack<BF16>(x, y);
+                            }
+                            tmem_st16(s_col + (uint32_t) (c * 16), hi);
+                        }
+                        float x, y;
+                        f2unpack(sum2, x, y);
+                        l += x + y;
+                        tmem_st_wait();
+                    }
+                    any = true;
+                    tc_fence_before();
+                    dn_mbar_arrive(&bar[TB_PREADY + w]);
+                } else {
+                    float g = 1.0f;
+                    if (warp_live) {
+                        float top = -INFINITY;
 #pragma unroll 1
                         for (int c = 0; c < 4; c++) {
                             uint32_t v[32];
                             tmem_ld32(s_col + (uint32_t) (c * 32), v);
                             tmem_ld_wait_tie(v);
-#pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
-                            }
-                            tmem_st32(s_col + (uint32_t) (c * 32), v);
-                        }
-                        tmem_st_wait();
-                    }
-                    const bool masked = (j + 1) * TS_N > held;
-                    float      top = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t v[32];
-                        tmem_ld32(s_col + (uint32_t) (c * 32), v);
-                        tmem_ld_wait_tie(v);
-                        if (masked) {
-                            const uint32_t see = live ? seen(j * TS_N + c * 32) : 0u;
-#pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                v[e] = see >> e & 1u ? v[e] : 0xff800000u;
-                            }
-                        }
-                        float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
-#pragma unroll
-                        for (int e = 2; e < 30; e += 4) {
-                            a = fmax3(a, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-                            b = fmax3(b, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-                        }
-                        top = fmax3(top, fmax3(a, __uint_as_float(v[30]), __uint_as_float(v[31])), b);
-                    }
-                    // (a factor of 0 makes a product with -inf no number)
-                    const float mn = fmaxf(m, top == -INFINITY ? top : top * factor);
-                    g = m == mn ? 1.0f : ex2(m - mn);
-                    m = mn;
-                    const float    nm = (m == -INFINITY ? 0.0f : -m) + (float) TS_OFF;
-                    const uint64_t nm2 = f2pack(nm, nm), fa2 = f2pack(factor, factor);
-                    uint64_t       sum2 = 0ull;
-#pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t v[32], hi[16], lo[PARTS == 2 ? 16 : 1];
-                        tmem_ld32(s_col + (uint32_t) (c * 32), v);
-                        tmem_ld_wait_tie(v);
-                        const uint32_t see = !masked ? 0xffffffffu : live ? seen(j * TS_N + c * 32) : 0u;
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            float          x, y;
-                            f2unpack(ffma2(f2pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), fa2, nm2), x, y);
                             if (masked) {
-                                x = see >> (2 * i) & 1u ? x : -INFINITY, y = see >> (2 * i + 1) & 1u ? y : -INFINITY;
+                                const uint32_t see = live ? seen(j * TS_N + c * 32) : 0u;
+#pragma unroll
+                                for (int e = 0; e < 32; e++) {
+                                    v[e] = see >> e & 1u ? v[e] : 0xff800000u;
+                                }
                             }
-                            const uint64_t p2 = f2pack(ex2(x), ex2(y));
-                            sum2 = fadd2(sum2, p2);
-                            f2unpack(p2, x, y);
-                            if (PARTS == 1) {
-                                hi[i] = ts_pack<BF16>(x, y);
-                            } else {
+                            float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
+#pragma unroll
+                            for (int e = 2; e < 30; e += 4) {
+                                a = fmax3(a, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                                b = fmax3(b, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+                            }
+                            top = fmax3(top, fmax3(a, __uint_as_float(v[30]), __uint_as_float(v[31])), b);
+                        }
+                        const float mn = fmaxf(m, top * factor);
+                        g = m == mn ? 1.0f : ex2(m - mn);
+                        m = mn;
+                        const float    nm = (m == -INFINITY ? 0.0f : -m) + TS_OFF<PARTS>;
+                        const uint64_t nm2 = f2pack(nm, nm), fa2 = f2pack(factor, factor);
+                        uint64_t       sum2 = 0ull;
+#pragma unroll 1
+                        for (int c = 0; c < 4; c++) {
+                            uint32_t v[32], hi[16], lo[16];
+                            tmem_ld32(s_col + (uint32_t) (c * 32), v);
+                            tmem_ld_wait_tie(v);
+                            const uint32_t see = !masked ? 0xffffffffu : live ? seen(j * TS_N + c * 32) : 0u;
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                float x, y;
+                                f2unpack(ffma2(f2pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), fa2, nm2), x, y);
+                                if (masked) {
+                                    x = see >> (2 * i) & 1u ? x : -INFINITY, y = see >> (2 * i + 1) & 1u ? y : -INFINITY;
+                                }
+                                const uint64_t p2 = f2pack(ex2(x), ex2(y));
+                                sum2 = fadd2(sum2, p2);
+                                f2unpack(p2, x, y);
                                 // the remainder is above 0, so that its product with an infinite value has the sign of
                                 // the other part's (2^-38 of the row's largest weight is far below F32's last bit)
                                 hi[i] = ts_pack_rz<BF16>(x, y);
@@ -773,138 +1057,136 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                                 f2unpack(ffma2(f2pack(f.x, f.y), f2pack(-1.0f, -1.0f), p2), x, y);
                                 lo[i] = masked ? ts_pack<BF16>(x, y) : ts_positive<BF16>(ts_pack<BF16>(x, y));
                             }
-                        }
-                        tmem_st16(s_col + (uint32_t) (c * 16 * PARTS), hi);
-                        if (PARTS == 2) {
+                            tmem_st16(s_col + (uint32_t) (c * 32), hi);
                             tmem_st16(s_col + (uint32_t) (c * 32 + 16), lo);
                         }
+                        float x, y;
+                        f2unpack(sum2, x, y);
+                        l = fmaf(l, g, x + y);
+                        tmem_st_wait();
                     }
-                    float x, y;
-                    f2unpack(sum2, x, y);
-                    l = fmaf(l, g, x + y);
-                    tmem_st_wait();
-                }
-                tc_fence_before();
-                dn_mbar_arrive(&bar[TB_PREADY + w]);
-                wait(TB_OFULL + w, tc >> 1);
-                if (warp_live) {
+                    tc_fence_before();
+                    dn_mbar_arrive(&bar[TB_PREADY + w]);
+                    wait(TB_OFULL + w, tc >> 1);
+                    if (warp_live) {
 #pragma unroll
-                    for (int c = 0; c < D / 32; c++) {
-                        uint32_t o[32];
-                        tmem_ld32(o_col + (uint32_t) (c * 32), o);
-                        tmem_ld_wait_tie(o);
+                        for (int c = 0; c < D / 32; c++) {
+                            uint32_t o[32];
+                            tmem_ld32(o_col + (uint32_t) (c * 32), o);
+                            tmem_ld_wait_tie(o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            acc[c * 32 + e] = fmaf(acc[c * 32 + e], g, __uint_as_float(o[e]));
+                            for (int e = 0; e < 32; e++) {
+                                acc[c * 32 + e] = fmaf(acc[c * 32 + e], g, __uint_as_float(o[e]));
+                            }
                         }
                     }
+                    tc_fence_before();
+                    dn_mbar_arrive(&bar[TB_OFREE + w]);
                 }
-                tc_fence_before();
-                dn_mbar_arrive(&bar[TB_OFREE + w]);
             }
-            // ---- the two streams' maxima and sums, then each takes half of the columns
+            // ---- the two streams' maxima and sums
             ml[w * TS_M + r] = make_float2(m, l);
+            if (PARTS == 1 && any) {
+                wait(TB_OFULL + w, used++);
+            }
             softmax_barrier();
             const float2 other = ml[(w ^ 1) * TS_M + r];
             const float  M = fmaxf(m, other.x), mine_f = m == M ? 1.0f : ex2(m - M), other_f = other.x == M ? 1.0f : ex2(other.x - M);
             l = w == 0 ? fmaf(l, mine_f, other.y * other_f) : fmaf(other.y, other_f, l * mine_f);
             l = f0 != f0 && M != -INFINITY ? NAN : l;
-            float res[D / 2];
+            const float inv = whole && l != 0.0f ? 1.0f / l : whole ? 0.0f : 1.0f;
+            if (!whole && live && w == 0) {  // behind the slot's rows
+                *(reinterpret_cast<float2 *>(al + (int64_t) (slot_rows - r) * D * 4) + r) = make_float2(M, l);
+            }
+            // ---- the sums: each stream takes half of the columns, 16 at a time, and stores them by whole rows
+            const bool odd = tail && dirty[pieces & 1] && live;
+            auto       columns = [&](int c, uint32_t (&o)[16]) {  // of this stream's sums, 16 from c on
+                if constexpr (PARTS == 1) {
+                    if (any) {
+                        tmem_ld16(o_col + (uint32_t) c, o);
+                        tmem_ld16_wait(o);
+                    } else {
 #pragma unroll
-            for (int c = 0; c < D / 64; c++) {
-                // to the other stream: columns 32 c .. of its half
-                float4 * give = xch + w * (TS_M * 8), *take = xch + (w ^ 1) * (TS_M * 8);
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    float4 f;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        (&f.x)[e] = w ? acc[c * 32 + k * 4 + e] : acc[D / 2 + c * 32 + k * 4 + e];
+                        for (int e = 0; e < 16; e++) {
+                            o[e] = 0u;
+                        }
                     }
-                    give[r * 8 + (k ^ (r & 7))] = f;
+                }
+            };
+            const int swz = (r >> 1) & 3;
+#pragma unroll PARTS == 2 ? D / 32 : 1
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t o[16];
+                const int theirs = (w ^ 1) * (D / 2) + c * 16, mine = w * (D / 2) + c * 16;
+                columns(theirs, o);
+                if constexpr (PARTS == 2) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        o[e] = __float_as_uint(w ? acc[c * 16 + e] : acc[D / 2 + c * 16 + e]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    give[r * 4 + (k ^ swz)] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
                 }
                 softmax_barrier();
+                columns(mine, o);
+                float x[16];
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float4 f = take[r * 8 + (k ^ (r & 7))];
+                for (int k = 0; k < 4; k++) {
+                    const float4 f = take[r * 4 + (k ^ swz)];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float a = w ? acc[D / 2 + c * 32 + k * 4 + e] : acc[c * 32 + k * 4 + e];
-                        // (the same operations in the same order whichever stream's it is)
-                        res[c * 32 + k * 4 + e] = a * mine_f + (&f.x)[e] * other_f;
+                        float a = __uint_as_float(o[4 * k + e]);
+                        if constexpr (PARTS == 2) {
+                            a = w ? acc[D / 2 + c * 16 + k * 4 + e] : acc[c * 16 + k * 4 + e];
+                        }
+                        x[4 * k + e] = a * mine_f + (&f.x)[e] * other_f;
                     }
                 }
-                softmax_barrier();
-            }
-            const int at = w * (D / 2);  // this thread's columns
-            if (tail && *dirty && live) {
-                // elements that are no numbers, of nodes that the row sees: they were left out of the products
-                for (int n = 0; n < nodes; n++) {
-                    const int key = held + n;
-                    if (key / TS_N < it.a || key / TS_N >= it.b || !(bits[n >> 5] >> (n & 31) & 1u)) {
-                        continue;
-                    }
-                    const uint16_t * v = reinterpret_cast<const uint16_t *>(p.v.data + (int64_t) key * p.v.nb1 + (int64_t) it.h * p.v.nb2 + (int64_t) it.s * p.v.nb3) + at;
+                if (odd) {
+                    // elements that are no numbers, of nodes that the row sees: they were left out of the products
+#pragma unroll 1
+                    for (int n = 0; n < nodes; n++) {
+                        const int key = held + n;
+                        if (key / TS_N < it.a || key / TS_N >= it.b || !(bits[n >> 5] >> (n & 31) & 1u)) {
+                            continue;
+                        }
+                        const uint16_t * v = reinterpret_cast<const uint16_t *>(p.v.data + (int64_t) key * p.v.nb1 + (int64_t) it.h * p.v.nb2 + (int64_t) it.s * p.v.nb3) + mine;
 #pragma unroll
-                    for (int e = 0; e < D / 2; e++) {
-                        const float x = ts_unpack<BF16>(v[e]).x;
-                        res[e] += fabsf(x) < INFINITY ? 0.0f : x;
+                        for (int e = 0; e < 16; e++) {
+                            const float y = ts_unpack<BF16>(v[e]).x;
+                            x[e] += fabsf(y) < INFINITY ? 0.0f : y;
+                        }
                     }
                 }
-            }
-            // ---- the result, or a part's sums into the workspace
-            {
-                const bool whole = it.a == 0 && it.b == it.q.tiles;
-                uint64_t   al;  // where this row goes
-                if (whole) {
-                    const int hd = it.h * p.ratio + row - my_node * p.ratio;
-                    al = reinterpret_cast<uint64_t>(p.o.data + (int64_t) hd * p.o.nb1 + (int64_t) my_node * p.o.nb2 + (int64_t) it.s * p.o.nb3);
-                } else {
-                    // the unit's parts: the first belongs to the piece before the first one that starts inside the unit, in its
-                    // second slot unless the unit is its first; the others are their pieces' first
-                    const int     pa = it.a == 0 ? group + 1 : ln.last(it.unit + TS_LEAST - 1) + 1, floats = ts_slot_floats(slot_rows, D);
-                    const int64_t step = (int64_t) blocks * 2 * floats, part1 = ((int64_t) pa * blocks + rb) * 2 * floats;
-                    const int64_t part0 = part1 - step + (ln.at(pa - 1) <= it.unit - TS_LEAST ? floats : 0);
-                    float *       slot  = p.part + (it.a == 0 ? part0 : part1 + (group - pa) * step);
-                    al = reinterpret_cast<uint64_t>(slot + r * D);
-                    if (live && w == 0) {
-                        *reinterpret_cast<float2 *>(slot + slot_rows * D + 2 * r) = make_float2(M, l);
-                    }
-                    if (own == 0 && it.a == 0) {
-                        *join = { it.s, it.h, ln.last(it.unit + it.q.tiles - TS_LEAST) - pa + 2, its_rows, part0, part1 };
-                    }
-                }
-                // by whole rows, 32 columns at a time through this warp's part of the exchange
-                const float inv   = whole ? (l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
-                float4 *    stage = xch + w * (TS_M * 8) + quad * 32 * 8;
-                const int   type = whole ? p.o.type : (int) KV_F32;
-                const bool  vec = !whole || p.o.vec;
+                softmax_barrier();  // (what this stream gave has been taken: its place holds the rows now)
                 if (warp_live) {
 #pragma unroll
-                    for (int c = 0; c < D / 64; c++) {
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            stage[lane * 8 + (k ^ (lane & 7))] = make_float4(res[c * 32 + k * 4] * inv, res[c * 32 + k * 4 + 1] * inv,
-                                                                             res[c * 32 + k * 4 + 2] * inv, res[c * 32 + k * 4 + 3] * inv);
-                        }
-                        __syncwarp();
-#pragma unroll 1
-                        for (int i = lane >> 3; i < 32; i += 4) {
-                            const int    k = lane & 7;
-                            const float4 f = stage[i * 8 + (k ^ (i & 7))];
-                            char *       to = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, al, i));
-                            if (quad * 32 + i < its_rows) {
-                                ts_store4(to, at + c * 32 + k * 4, f, type, vec);
-                            }
-                        }
-                        __syncwarp();
+                    for (int k = 0; k < 4; k++) {
+                        give[r * 4 + (k ^ swz)] = make_float4(x[4 * k] * inv, x[4 * k + 1] * inv, x[4 * k + 2] * inv, x[4 * k + 3] * inv);
                     }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = lane >> 2; i < 32; i += 8) {
+                        const int    k = lane & 3;
+                        const float4 f = give[(quad * 32 + i) * 4 + (k ^ ((i >> 1) & 3))];
+                        char *       to = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, al, i));
+                        if (quad * 32 + i < its_rows) {
+                            ts_store4(to, mine + k * 4, f, type, !whole || p.o.vec);
+                        }
+                    }
+                    __syncwarp();
                 }
             }
-            softmax_barrier();  // Q's memory and the ancestors are free
-            if (own == 0) {
-                *dirty = 0;  // (the next piece's tiles are looked at when all threads have staged its Q)
+            if (PARTS == 1 && any) {
+                tc_fence_before();
+                dn_mbar_arrive(&bar[TB_OFREE + w]);
             }
+            if (own == 0) {
+                dirty[pieces & 1] = 0;  // (set again two pieces on, when this thread has been through the next)
+            }
+            pieces++;
         }
         if (!ok) {
             atomicExch(abort_f, 1);
@@ -993,7 +1275,7 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
     const int blocks = tree_attn_blocks(p), groups = tree_attn_groups(p, sms);
     const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
     e = kv8_launch(kern, dim3((unsigned) (groups * blocks)), TS_THREADS, smem, stream, tmk, tmv, p, blocks, groups, rows);
-    if (e != cudaSuccess || p.n_kv <= (2 * TS_LEAST - 1) * TS_N) {
+    if (e != cudaSuccess || p.n_kv <= TS_LEAST * TS_N) {
         return e;  // (no unit is in parts)
     }
     return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) (groups * blocks), (unsigned) ((rows + TJ_ROWS - 1) / TJ_ROWS)), TJ_ROWS * D / 4, 0, stream, p,
@@ -1002,8 +1284,8 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
 
 template <int D, bool BF16>
 cudaError_t launch_d(const TreeAttnParams & p, int sms, cudaStream_t stream) {
-    // one part where q is the cache's type and the result has no more bits
-    return p.q.type == p.k.type && p.o.type == p.q.type ? launch_one<D, BF16, 1>(p, sms, stream) : launch_one<D, BF16, 2>(p, sms, stream);
+    // one part where q is the cache's type, the result has no more bits, and the truncated sums stay small
+    return p.q.type == p.k.type && p.o.type == p.q.type && p.n_kv <= TS_LONG ? launch_one<D, BF16, 1>(p, sms, stream) : launch_one<D, BF16, 2>(p, sms, stream);
 }
 
 }  // namespace
