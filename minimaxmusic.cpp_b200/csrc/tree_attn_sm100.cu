@@ -52,7 +52,7 @@ constexpr int TS_SPACE   = 256;  // bytes of the workspace before the list of un
 constexpr int TS_LEAST   = 4;    // tiles of a part, at least: a part costs as much as about two tiles, and the joining kernel
 constexpr int TS_PIECES  = 4;    // pieces that warp 0 may be ahead
 constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for
-constexpr int TJ_ROWS    = 8;    // rows of a joining CTA
+constexpr int TJ_UNITS   = 512;  // units in parts, at most one a CTA: there are no more CTAs than SMs or blocks of a unit
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
 constexpr int TS_REGS_SOFTMAX = 208;  // 2 x 208 + 88 = 3 x 168
 constexpr int TS_REGS_ISSUE   = 88;
@@ -88,19 +88,18 @@ enum : int {
     TB_SFULL  = 16,  // [2]
     TB_PREADY = 18,  // [2] 128 softmax threads
     TB_OFULL  = 20,  // [2] a tile's P V (PARTS 1: the last of a piece)
-    TB_OFREE  = 22,  // [2] 128 softmax threads
-    TB_QREADY = 24,  // 64
-    TB_QFREE  = 25,  // the last QK of a piece
-    TB_LOOK   = 26,  // warp 1: a V tile with nodes is there
-    TB_FIX    = 27,  // 64 threads of warps 2, 3: it can be taken
-    TB_DONE   = 28,
-    TB_PIECE  = 29,  // [TS_PIECES] warp 0
-    TB_PFREE  = 33,  // [TS_PIECES] the 11 other warps
-    TB_COUNT  = 37,
+    TB_QREADY = 22,  // 64
+    TB_QFREE  = 23,  // the last QK of a piece
+    TB_LOOK   = 24,  // warp 1: a V tile with nodes is there
+    TB_FIX    = 25,  // 64 threads of warps 2, 3: it can be taken
+    TB_DONE   = 26,
+    TB_PIECE  = 27,  // [TS_PIECES] warp 0
+    TB_PFREE  = 31,  // [TS_PIECES] the 11 other warps
+    TB_COUNT  = 35,
 };
 
 __host__ __device__ constexpr uint32_t ts_arrivals(int b) {
-    return b >= TB_PFREE ? (uint32_t) (TS_THREADS / 32 - 1) : b == TB_QREADY || b == TB_FIX ? 64u : b == TB_PREADY || b == TB_PREADY + 1 || b == TB_OFREE || b == TB_OFREE + 1 ? 128u : 1u;
+    return b >= TB_PFREE ? (uint32_t) (TS_THREADS / 32 - 1) : b == TB_QREADY || b == TB_FIX ? 64u : b == TB_PREADY || b == TB_PREADY + 1 ? 128u : 1u;
 }
 
 // kind::f16 instruction descriptor: F16 x F16 or BF16 x BF16 -> F32, M = 128
@@ -179,12 +178,6 @@ __device__ __forceinline__ uint32_t ts_pack_rz(float lo, float hi) {
     return u;
 }
 
-// each of two numbers that are not negative, or the smallest positive one
-template <bool BF16>
-__device__ __forceinline__ uint32_t ts_positive(uint32_t u) {
-    return __vmaxu2(u, BF16 ? 0x00800080u : 0x00010001u);
-}
-
 template <bool BF16>
 __device__ __forceinline__ float2 ts_unpack(uint32_t u) {
     return BF16 ? bf2_to_f2(u) : h2_to_f2(u);
@@ -198,31 +191,7 @@ __device__ __forceinline__ float ts_tanh(float x) {
     return copysignf(a < 0.25f ? p : t, x);
 }
 
-// elements [e0, e0 + E) of a row that is not aligned: F32, or 16-bit pairs
-template <int E>
-__device__ __noinline__ uint4 ts_load_elements(const char * row, bool f32, int e0) {
-    uint32_t x[4] = { 0, 0, 0, 0 };
-    if (f32) {
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            x[e] = reinterpret_cast<const uint32_t *>(row)[e0 + e];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            x[e / 2] = reinterpret_cast<const uint16_t *>(row)[e0 + e] | (uint32_t) reinterpret_cast<const uint16_t *>(row)[e0 + e + 1] << 16;
-        }
-    }
-    return make_uint4(x[0], x[1], x[2], x[3]);
-}
-
-// eight 16-bit elements that are not aligned
-__device__ __forceinline__ uint4 ts_load8(const char * at) {
-    const uint16_t * h = reinterpret_cast<const uint16_t *>(at);
-    return make_uint4(h[0] | (uint32_t) h[1] << 16, h[2] | (uint32_t) h[3] << 16, h[4] | (uint32_t) h[5] << 16, h[6] | (uint32_t) h[7] << 16);
-}
-
-// Floats of a part: O of its rows, then m and l of each; a multiple of 16 bytes.
+// Floats of a part: O as [D / 4][row] of four, then m and l of each row; a multiple of 16 bytes.
 __host__ __device__ constexpr int ts_slot_floats(int rows, int D) {
     return (rows * (D + 2) + 3) / 4 * 4;
 }
@@ -254,6 +223,15 @@ struct TsJoin {
     int64_t part0, part1;       // where the first part and the second are, in floats; the others follow at even steps
 };
 
+// (functions of their own, for the instruction cache's sake)
+__device__ __noinline__ int ts_div(int a, int b) {
+    return (int) ((unsigned) a / (unsigned) b);
+}
+
+__device__ __forceinline__ int ts_up(int a, int b) {
+    return ts_div(a + b - 1, b);
+}
+
 // Key tiles of a sequence's units; 0 where none of its nodes counts.
 struct TsSeq {
     int L, nodes, keys, tiles;
@@ -274,7 +252,7 @@ struct TsLine {
     int W, G, each, more;  // `more` pieces have a tile more than `each`
 
     __device__ __forceinline__ TsLine(int W_, int groups) : W(W_), G(max(1, min(groups, W_ / TS_LEAST))) {
-        each = W / G;
+        each = ts_div(W, G);
         more = W - each * G;
     }
 
@@ -285,7 +263,7 @@ struct TsLine {
     // the last piece that starts at tile x or before
     __device__ __forceinline__ int last(int x) const {
         const int y = more * (each + 1);
-        return min(G - 1, x < y ? x / (each + 1) : each > 0 ? more + (x - y) / each : G - 1);
+        return min(G - 1, x < y ? ts_div(x, each + 1) : each > 0 ? more + ts_div(x - y, each) : G - 1);
     }
 
     // border x, of a unit of n tiles that starts at `first` and holds x
@@ -328,20 +306,20 @@ struct TsPlan {
         if (p.n_seq <= TS_EVEN && U <= groups) {
             // the fewest tiles to a part that need no more than all groups: each lane tries one of 32 numbers between what
             // even shares would be and what is enough
-            const int lo = max(TS_LEAST, (W + groups - 1) / groups);
-            const int hi = max(lo, U < groups ? min(most, (W + groups - U - 1) / (groups - U)) : most);
+            const int lo = max(TS_LEAST, ts_up(W, groups));
+            const int hi = max(lo, U < groups ? min(most, ts_up(W, groups - U)) : most);
             const int t  = lo + lane * ((hi - lo + 30) / 31);
             int       parts = 0;
 #pragma unroll 1
             for (int i = 0; i < p.n_seq; i++) {
-                parts += (ts_seq(p, i).tiles + t - 1) / t;
+                parts += ts_up(ts_seq(p, i).tiles, t);
             }
             const unsigned fits = __ballot_sync(0xffffffffu, parts * p.n_head_kv <= groups);
             even = __shfl_sync(0xffffffffu, t, __ffs(fits) - 1);  // (the last lane's fits)
             mine = 0;
 #pragma unroll 1
-        for (int i = s0; i < s1; i++) {
-                mine += (ts_seq(p, i).tiles + even - 1) / even;
+            for (int i = s0; i < s1; i++) {
+                mine += ts_up(ts_seq(p, i).tiles, even);
             }
             from = group, to = group + 1;
         } else {
@@ -376,13 +354,13 @@ struct TsPlan {
         q = ts_seq(p, s);
         x = from, end = to;
         if (!even) {
-            x = TsLine::border(x, first + (x - first) / q.tiles * q.tiles, q.tiles);
+            x = TsLine::border(x, first + ts_div(x - first, q.tiles) * q.tiles, q.tiles);
         }
     }
 
     // a sequence's length on the line, or its parts
     __device__ __forceinline__ int weight(int tiles) const {
-        return (even ? (tiles + even - 1) / even : tiles) * p.n_head_kv;
+        return (even ? ts_up(tiles, even) : tiles) * p.n_head_kv;
     }
 
     // the next piece that has rows in this block
@@ -403,13 +381,13 @@ struct TsPlan {
             }
             c.s = s, c.L = q.L, c.nodes = q.nodes, c.keys = q.keys, c.tiles = q.tiles;
             if (even) {
-                const int parts = (q.tiles + even - 1) / even, i = x - first;
-                c.h          = i / parts;
+                const int parts = ts_up(q.tiles, even), i = x - first;
+                c.h          = ts_div(i, parts);
                 const int k  = i - c.h * parts;
-                c.unit = x - k, c.a = k * q.tiles / parts, c.b = (k + 1) * q.tiles / parts;
+                c.unit = x - k, c.a = ts_div(k * q.tiles, parts), c.b = ts_div((k + 1) * q.tiles, parts);
                 x++;
             } else {
-                c.h    = (x - first) / q.tiles;
+                c.h    = ts_div(x - first, q.tiles);
                 c.unit = first + c.h * q.tiles;
                 c.a    = x - c.unit;
                 c.b    = c.unit + q.tiles <= end ? q.tiles : TsLine::border(end, c.unit, q.tiles) - c.unit;
@@ -436,148 +414,129 @@ struct TsPlan {
 
     // what the joining kernel has to know of a unit, from its first part
     __device__ __forceinline__ TsJoin join(const TsPiece & c) const {
-        const int g = second(c), parts = even ? (c.tiles + even - 1) / even : ln.last(c.unit + c.tiles - TS_LEAST) - g + 2;
+        const int g = second(c), parts = even ? ts_up(c.tiles, even) : ln.last(c.unit + c.tiles - TS_LEAST) - g + 2;
         return { c.s, c.h, parts, c.rows, part(c, g, 0), part(c, g, 1) };
     }
 };
 
-// Rows ra .. ra + 15 of a block's Q for the products, by a warp; rows that do not count are zeros.
+// Rows ra .. ra + 15 of a block's Q for the products, by a warp; rows that do not count are zeros.  All copies are in
+// flight at once, and land where the row's products will read it: PARTS 1, as they are; PARTS 2, a row's bytes lie in
+// the places of its own two parts (F32: all of them), and the warp replaces one row after another.
 template <int D, bool BF16, int PARTS>
 __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPiece & it, int rb, int ra, char * qs, float * factors, int lane) {
-    constexpr int E = D / 32, QT = TsSmem<D, PARTS>::QT;
-    const int     in = it.rows - ra;
+    constexpr int E = D / 32, QT = TsSmem<D, PARTS>::QT, BLOCK = TS_M * 128;
+    const int     in = it.rows - ra, esz = p.q.type == KV_F32 ? 4 : 2;
     // lane i, and 16 + i: the address of row i
     const int      rl = rb * TS_M + ra + (lane & 15), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
     const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
     // (not 0, whose product with the -inf of a key that is not seen would be no number)
     const float    by = fmaxf(fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E), 0x1p-126f);
-    if constexpr (PARTS == 1) {
-        // as it is, but for the sign of the scale: 16 bytes by each lane, all loads in flight
-        constexpr int  PER = D / 8, N = D / 16;  // lanes of a row, loads of a lane
-        const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
-        const int      ck = lane % PER;
-        uint4          u[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int    rw  = i * (32 / PER) + lane / PER;
-            const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, rw));
-            u[i] = make_uint4(0, 0, 0, 0);
-            if (rw < in && p.q.vec) {
-                u[i] = *reinterpret_cast<const uint4 *>(src + ck * 16);
+    // chunk ck of 16 bytes of row i: block ck / 8 of 64 columns (F32: the two blocks of either part in turn)
+    auto place = [&](int i, int ck) {
+        const int blk = ck >> 3;
+        return qs + (blk % (D / 64)) * BLOCK + (blk / (D / 64)) * QT + (ra + i) * 128 + (((ck & 7) ^ (PARTS == 1 ? i & 7 : 0)) << 4);  // (ra: a multiple of 8)
+    };
+    const int chunks = D * esz / 16, per = 32 / chunks, ck = lane % chunks;
+#pragma unroll 1
+    for (int i = lane / chunks; i < 16; i += per) {
+        const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i)) + ck * 16;
+        char *       to  = place(i, ck);
+        if (p.q.vec || i >= in) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(i < in ? src : p.q.data), "r"(i < in && p.q.vec ? 16 : 0) : "memory");
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < 16; e += esz) {
+                if (esz == 4) {
+                    *reinterpret_cast<uint32_t *>(to + e) = *reinterpret_cast<const uint32_t *>(src + e);
+                } else {
+                    *reinterpret_cast<uint16_t *>(to + e) = *reinterpret_cast<const uint16_t *>(src + e);
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int rw = i * (32 / PER) + lane / PER;
-            *reinterpret_cast<uint4 *>(qs + (ck / 8) * (TS_M * 128) + (ra + rw) * 128 + (((ck % 8) ^ (rw & 7)) << 4)) =
-                make_uint4(u[i].x ^ flip, u[i].y ^ flip, u[i].z ^ flip, u[i].w ^ flip);
-        }
-        if (!p.q.vec) {
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    if constexpr (PARTS == 1) {
+        if (p.scale < 0.0f) {  // (the maximum of a row's scores is taken before they are multiplied)
 #pragma unroll 1
-            for (int rw = lane / PER; rw < 16; rw += 32 / PER) {
-                const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, rw));
-                if (rw < in) {
-                    const uint4 f = ts_load8(src + ck * 16);
-                    *reinterpret_cast<uint4 *>(qs + (ck / 8) * (TS_M * 128) + (ra + rw) * 128 + (((ck % 8) ^ (rw & 7)) << 4)) =
-                        make_uint4(f.x ^ flip, f.y ^ flip, f.z ^ flip, f.w ^ flip);
-                }
+            for (int i = lane / chunks; i < 16; i += per) {
+                uint4 * at = reinterpret_cast<uint4 *>(place(i, ck));
+                *at        = make_uint4(at->x ^ 0x80008000u, at->y ^ 0x80008000u, at->z ^ 0x80008000u, at->w ^ 0x80008000u);
             }
         }
         if (lane < 16) {
             factors[ra + lane] = by;
         }
     } else {
-        // two parts of the cache's type.  A row with an infinity or NaN becomes zeros with a factor of NaN
-        const bool  f32 = p.q.type == KV_F32, f16 = p.q.type == KV_F16;
+        // a row with an infinity or NaN becomes zeros with a factor of NaN
         const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
         const int   e0 = lane * E;
-        if ((lane & 15) < in) {  // all rows are on their way while the first are worked on
-            asm volatile("prefetch.global.L1 [%0];" ::"l"(al + (lane >> 4) * 128));
-            if (f32 && D == 128) {
-                asm volatile("prefetch.global.L1 [%0];" ::"l"(al + 256 + (lane >> 4) * 128));
-            }
-        }
-        char * to = qs + ra * 128 + (e0 / 64) * (TS_M * 128) + (e0 % 8) * 2;
-#pragma unroll 1
-        for (int i0 = 0; i0 < 16; i0 += 4) {
-            float x[4][E];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i0 + i));
-                uint4        u   = make_uint4(0, 0, 0, 0);  // F32 values, or 16-bit pairs
-                if (i0 + i < in) {
-                    if (!p.q.vec) {
-                        u = ts_load_elements<E>(src, f32, e0);
-                    } else if (E == 4 && f32) {
-                        u = *reinterpret_cast<const uint4 *>(src + lane * 16);
-                    } else if (E == 4 || f32) {
-                        const uint2 f = *reinterpret_cast<const uint2 *>(src + lane * 8);
-                        u.x = f.x, u.y = f.y;
-                    } else {
-                        u.x = *reinterpret_cast<const uint32_t *>(src + lane * 4);
-                    }
-                }
+#pragma unroll 4
+        for (int i = 0; i < 16; i++) {
+            const char * at = place(i, e0 * esz / 16) + e0 * esz % 16;
+            float        x[E];
+            if (esz == 4) {
 #pragma unroll
                 for (int e = 0; e < E; e += 2) {
-                    const uint32_t pair = e ? u.y : u.x;
-                    const float2   a    = f16 ? h2_to_f2(pair) : bf2_to_f2(pair);
-                    x[i][e]     = f32 ? __uint_as_float((&u.x)[e]) : a.x;
-                    x[i][e + 1] = f32 ? __uint_as_float((&u.x)[e + 1]) : a.y;
+                    const float2 f = reinterpret_cast<const float2 *>(at)[e / 2];
+                    x[e] = f.x, x[e + 1] = f.y;
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                const bool  odd = top >= 0x7f800000u;
-                const int   ex  = BF16 ? 0 : (top == 0 || odd ? 0 : max((int) (top >> 23) - 127, -112)) - 14;
-                const float dn  = odd ? 0.0f : __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
-                uint32_t    hi[E / 2], lo[E / 2];
+            } else {
 #pragma unroll
                 for (int e = 0; e < E; e += 2) {
-                    const float a = odd ? 0.0f : x[i][e] * dn, b = odd ? 0.0f : x[i][e + 1] * dn;
-                    hi[e / 2]      = ts_pack<BF16>(a, b);
-                    const float2 f = ts_unpack<BF16>(hi[e / 2]);
-                    lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
+                    const uint32_t u = reinterpret_cast<const uint32_t *>(at)[e / 2];
+                    const float2   f = p.q.type == KV_F16 ? h2_to_f2(u) : bf2_to_f2(u);
+                    x[e] = f.x, x[e + 1] = f.y;
                 }
-                char * at = to + (i0 + i) * 128 + ((((e0 % 64) / 8) ^ ((i0 + i) & 7)) << 4);  // (ra: a multiple of 8)
-                if (E == 4) {
-                    *reinterpret_cast<uint2 *>(at)      = make_uint2(hi[0], hi[E / 2 - 1]);
-                    *reinterpret_cast<uint2 *>(at + QT) = make_uint2(lo[0], lo[E / 2 - 1]);
-                } else {
-                    *reinterpret_cast<uint32_t *>(at)      = hi[0];
-                    *reinterpret_cast<uint32_t *>(at + QT) = lo[0];
-                }
-                if (lane == i) {
-                    factors[ra + i0 + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
-                }
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+            }
+            top = __reduce_max_sync(0xffffffffu, top);  // (and the row has been read)
+            const bool  odd = top >= 0x7f800000u;
+            const int   ex  = BF16 ? 0 : (top == 0 || odd ? 0 : max((int) (top >> 23) - 127, -112)) - 14;
+            const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
+            uint32_t    hi[E / 2], lo[E / 2];
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
+                hi[e / 2]      = ts_pack<BF16>(a, b);
+                const float2 f = ts_unpack<BF16>(hi[e / 2]);
+                lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
+            }
+            char * to = qs + (e0 / 64) * BLOCK + (ra + i) * 128 + ((((e0 % 64) / 8) ^ (i & 7)) << 4) + (e0 % 8) * 2;
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) {
+                reinterpret_cast<uint32_t *>(to)[e]      = hi[e];
+                reinterpret_cast<uint32_t *>(to + QT)[e] = lo[e];
+            }
+            if (lane == 0) {
+                factors[ra + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
             }
         }
     }
 }
 
-// The next piece that warp 0 tells of; false: there is none, or it did not come in time.  By whole warps.
-__device__ __forceinline__ bool ts_take(TsPiece & it, const TsPiece * told, uint64_t * bar, uint32_t pieces, int lane, uint64_t deadline) {
+// Waits for the next piece that warp 0 tells of; false: there is none, or it did not come in time.  By whole warps.
+__device__ __forceinline__ bool ts_take(const TsPiece * told, uint64_t * bar, uint32_t pieces, uint64_t deadline) {
     const uint32_t k = pieces % TS_PIECES;
-    if (!dn_wait_warp(&bar[TB_PIECE + k], (pieces / TS_PIECES) & 1, deadline)) {
-        return false;
-    }
-    it = told[k];
+    return dn_wait_warp(&bar[TB_PIECE + k], (pieces / TS_PIECES) & 1, deadline) && told[k].rows > 0;
+}
+
+// What warp 0 told is not needed any more.
+__device__ __forceinline__ void ts_drop(uint64_t * bar, uint32_t pieces, int lane) {
     __syncwarp();
     if (lane == 0) {
-        dn_mbar_arrive(&bar[TB_PFREE + k]);
+        dn_mbar_arrive(&bar[TB_PFREE + pieces % TS_PIECES]);
     }
-    return it.rows > 0;
 }
 
 template <int D, bool BF16, int PARTS>
 __global__ void __launch_bounds__(TS_THREADS, 1)
     tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TreeAttnParams p, int blocks,
-                        int groups, int slot_rows) {
+                        int groups, int slot_rows, int joined) {
     using L          = TsSmem<D, PARTS>;
     constexpr int NS = L::NS;
     extern __shared__ __align__(16) char smem_raw[];
@@ -604,6 +563,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         tmem_relinquish();
     }
     kv8_dep_wait();
+    if (joined) {  // the joining kernel may take its place; it waits for this one's end
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
     const uint64_t deadline = global_timer_ns() + p.timeout_ns;
     const int      rb = (int) blockIdx.x % blocks;
     TsPiece *      told = reinterpret_cast<TsPiece *>(smem + L::OFF_PIECE);
@@ -618,7 +580,12 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         regs_dec<TS_REGS_ISSUE>();
         bool ok = true;
         auto next = [&] {
-            return ok && ts_take(it, told, bar, pieces, lane, deadline);
+            if (!ok || !ts_take(told, bar, pieces, deadline)) {
+                return false;
+            }
+            it = told[pieces % TS_PIECES];
+            ts_drop(bar, pieces, lane);
+            return true;
         };
         if (warp == 0) {
             // =================================================== the pieces, TMA
@@ -627,20 +594,6 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             if (lane == 0) {
                 uint32_t c = 0;
                 join->parts = 0;
-                auto     load = [&](const CUtensorMap * tm, int tile) {
-                    const int slot = (int) (c % NS);
-                    if (ok && c >= (uint32_t) NS && !mbar_wait_bounded(&bar[TB_EMPTY + slot], (c / NS - 1) & 1, deadline)) {
-                        ok = false;
-                    }
-                    if (ok) {
-                        mbar_arrive_expect_tx(&bar[TB_FULL + slot], (uint32_t) L::KT);
-#pragma unroll
-                        for (int hf = 0; hf < L::HALVES; hf++) {
-                            ts_load(smem + L::OFF_RING + slot * L::KT + hf * (TS_N * 128), tm, hf * 64, tile * TS_N, it.h, it.s, &bar[TB_FULL + slot]);
-                        }
-                        c++;
-                    }
-                };
                 do {
                     it = plan.next();
                     if (pieces >= (uint32_t) TS_PIECES && !mbar_wait_bounded(&bar[TB_PFREE + pieces % TS_PIECES], (pieces / TS_PIECES - 1) & 1, deadline)) {
@@ -656,13 +609,23 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     if (it.a == 0 && it.b < it.tiles) {
                         *join = plan.join(it);
                     }
-                    load(&tmk, it.a);
+                    // K(a), K(a + 1), V(a), .., K(b - 1), V(b - 2), V(b - 1)
+                    const int n = it.b - it.a;
 #pragma unroll 1
-                    for (int j = it.a; ok && j < it.b; j++) {
-                        if (j + 1 < it.b) {
-                            load(&tmk, j + 1);
+                    for (int i = 0; i < 2 * n; i++) {
+                        const bool          isk  = i == 0 || ((i & 1) && (i + 1) / 2 < n);
+                        const int           tile = it.a + (isk ? (i + 1) / 2 : i == 2 * n - 1 ? n - 1 : i / 2 - 1), slot = (int) (c % NS);
+                        const CUtensorMap * tm   = isk ? &tmk : &tmv;
+                        if (c >= (uint32_t) NS && !mbar_wait_bounded(&bar[TB_EMPTY + slot], (c / NS - 1) & 1, deadline)) {
+                            ok = false;
+                            break;
                         }
-                        load(&tmv, j);
+                        mbar_arrive_expect_tx(&bar[TB_FULL + slot], (uint32_t) L::KT);
+#pragma unroll
+                        for (int hf = 0; hf < L::HALVES; hf++) {
+                            ts_load(smem + L::OFF_RING + slot * L::KT + hf * (TS_N * 128), tm, hf * 64, tile * TS_N, it.h, it.s, &bar[TB_FULL + slot]);
+                        }
+                        c++;
                     }
                 } while (ok);
                 if (!ok) {  // copies that are under way have to land
@@ -684,7 +647,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
                 tc_fence_after();
             };
-            uint32_t c = 0, tc = 0, looks = 0, used0 = 0, used1 = 0;  // used: pieces in which a stream had tiles
+            uint32_t c = 0, tc = 0, looks = 0;
             while (next()) {
                 wait(TB_QREADY, pieces++);
 #pragma unroll 1
@@ -721,27 +684,18 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     if (nodes && lane == 0) {
                         dn_mbar_arrive(&bar[TB_LOOK]);
                     }
-                    wait(TB_PREADY + buf, tc >> 1);
-                    if (PARTS == 2 && tc >= 2) {
-                        wait(TB_OFREE + buf, (tc >> 1) - 1);
-                    }
-                    if (PARTS == 1 && j - it.a < 2) {  // the stream's first tile of the piece
-                        const uint32_t before = buf ? used1++ : used0++;
-                        if (before > 0) {
-                            wait(TB_OFREE + buf, before - 1);
-                        }
-                    }
+                    wait(TB_PREADY + buf, tc >> 1);  // (the stream has read the P V of its tile before)
                     if (nodes) {
                         wait(TB_FIX, looks++);
                     }
 #pragma unroll 1
                     for (int part = PARTS - 1; part >= 0; part--) {
-                        uint32_t pa = tmem + (uint32_t) (buf * TS_N + part * 16);
+                        uint32_t pa = tmem + (uint32_t) (buf * TS_N + part * 8);
                         uint64_t vb = v_d + (uint64_t) ((slot * L::KT) >> 4);
                         uint32_t add = PARTS == 2 ? (uint32_t) (PARTS - 1 - part) : j - it.a < 2 ? 0u : 1u;
 #pragma unroll
-                        for (int k = 0; k < 8; k++) {  // P of 32 keys: 16 columns, then 16 of its remainder
-                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), pa + (uint32_t) ((k >> 1) * 16 * PARTS + (k & 1) * 8), vb + (uint64_t) ((k * 16 * 128) >> 4),
+                        for (int k = 0; k < 8; k++) {  // P of 16 keys: 8 columns, then 8 of its remainder
+                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), pa + (uint32_t) (k * 8 * PARTS), vb + (uint64_t) ((k * 16 * 128) >> 4),
                                         id_pv, add);
                             add = 1u;
                         }
@@ -844,50 +798,44 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             tc_fence_after();
         };
         // (all of them go on, or none: they meet at barriers)
-        while (softmax_all(ts_take(it, told, bar, pieces, lane, deadline))) {
-            const int  its_rows = it.rows;
-            const bool live = r < its_rows, warp_live = quad * 32 < its_rows;
-            const int  held = it.L, nodes = it.nodes;
-            if (pieces == 0) {
-                ts_stage16<D, BF16, PARTS>(p, it, rb, (w * 4 + quad) * 16, smem + L::OFF_Q, factors, lane);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane < 8) {
-                    dn_mbar_arrive(&bar[TB_QREADY]);
+        while (softmax_all(ts_take(told, bar, pieces, deadline))) {
+            // (read where it is needed: the sums leave few registers)
+            const TsPiece & it = told[pieces % TS_PIECES];
+            const int       tile0 = it.a, tile1 = it.b, held = it.L;
+            const bool      live = r < it.rows, warp_live = quad * 32 < it.rows;
+            // ---- Q of the first piece, and each node's ancestors, where the piece has tiles with nodes
+            const bool tail = tile1 * TS_N > held;
+            {
+                const int nodes = it.nodes, parent = tail && own < nodes ? tree_parent(p.t, it.s % p.t.n_tree, own) : -1;
+                if (pieces == 0) {
+                    ts_stage16<D, BF16, PARTS>(p, it, rb, (w * 4 + quad) * 16, smem + L::OFF_Q, factors, lane);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane < 8) {
+                        dn_mbar_arrive(&bar[TB_QREADY]);
+                    }
                 }
-            }
-            // ---- each node's ancestors, where the piece has tiles with nodes
-            const bool tail = it.b * TS_N > held;
-            if (tail) {
-                if (own < nodes) {
-                    par[own] = tree_parent(p.t, it.s % p.t.n_tree, own);
-                }
-                softmax_barrier();
-                if (own < nodes) {
-                    uint32_t * to = anc + own * (TREE_MAX / 32);
+                if (tail) {
+                    if (own < nodes) {
+                        par[own] = parent;
+                    }
+                    softmax_barrier();
+                    if (own < nodes) {
+                        uint32_t * to = anc + own * (TREE_MAX / 32);
 #pragma unroll
-                    for (int k = 0; k < TREE_MAX / 32; k++) {
-                        to[k] = 0;
+                        for (int k = 0; k < TREE_MAX / 32; k++) {
+                            to[k] = 0;
+                        }
+#pragma unroll 1
+                        for (int at = own; at >= 0; at = par[at]) {
+                            to[at >> 5] |= held + at < p.n_kv ? 1u << (at & 31) : 0u;
+                        }
                     }
-                    for (int at = own; at >= 0; at = par[at]) {
-                        to[at >> 5] |= held + at < p.n_kv ? 1u << (at & 31) : 0u;
-                    }
+                    softmax_barrier();
                 }
-                softmax_barrier();
-            }
-            // ---- where this row goes: the result, or a part's slot
-            const bool whole = it.a == 0 && it.b == it.tiles;
-            const int  type = whole ? p.o.type : (int) KV_F32;
-            uint64_t   al;
-            if (whole) {
-                const int hd = it.h * p.ratio + row - my_node * p.ratio;
-                al = reinterpret_cast<uint64_t>(p.o.data + (int64_t) hd * p.o.nb1 + (int64_t) my_node * p.o.nb2 + (int64_t) it.s * p.o.nb3);
-            } else {
-                al = reinterpret_cast<uint64_t>(p.part + it.slot + r * D);
             }
             wait(TB_QREADY, pieces);
             const float f0 = factors[(pieces & 1) * TS_M + r], factor = cap || f0 != f0 ? 1.0f : f0;
-            const float fcap = f0 != f0 ? 1.0f : f0;
             // which of the 32 keys from k0 on the row sees
             auto seen = [&](int k0) -> uint32_t {
                 const int o = k0 - held;  // in nodes
@@ -912,21 +860,26 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
             }
 #pragma unroll 1
-            for (int j = it.a; j < it.b; j++, tc++) {
+            for (int j = tile0; j < tile1; j++, tc++) {
                 if ((int) (tc & 1) != w) {
                     continue;
                 }
-                const bool masked = (j + 1) * TS_N > held;
                 wait(TB_SFULL + w, tc >> 1);
-                if (cap && warp_live) {  // s = cap * tanh(S * factor), in log2 units, over S
+                if (warp_live && (cap || (j + 1) * TS_N > held)) {
+                    // over S: with a softcap, s = cap * tanh(S * factor) in log2 units; -inf for a key that the row does not see
+                    const float fcap = f0 != f0 ? 1.0f : f0;
 #pragma unroll 1
                     for (int c = 0; c < 8; c++) {
                         uint32_t v[16];
                         tmem_ld16(s_col + (uint32_t) (c * 16), v);
                         tmem_ld16_wait(v);
+                        const uint32_t see = (live ? seen(j * TS_N + (c >> 1) * 32) : 0u) >> (16 * (c & 1));
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
+                            if (cap) {
+                                v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
+                            }
+                            v[e] = see >> e & 1u ? v[e] : 0xff800000u;
                         }
                         tmem_st16(s_col + (uint32_t) (c * 16), v);
                     }
@@ -942,16 +895,6 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
                             tmem_ld_wait_tie(&v[c * 32]);
-                        }
-                        if (masked) {
-#pragma unroll
-                            for (int c = 0; c < 4; c++) {
-                                const uint32_t see = live ? seen(j * TS_N + c * 32) : 0u;
-#pragma unroll
-                                for (int e = 0; e < 32; e++) {
-                                    v[c * 32 + e] = see >> e & 1u ? v[c * 32 + e] : 0xff800000u;
-                                }
-                            }
                         }
                         float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
 #pragma unroll
@@ -1013,13 +956,6 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             uint32_t v[32];
                             tmem_ld32(s_col + (uint32_t) (c * 32), v);
                             tmem_ld_wait_tie(v);
-                            if (masked) {
-                                const uint32_t see = live ? seen(j * TS_N + c * 32) : 0u;
-#pragma unroll
-                                for (int e = 0; e < 32; e++) {
-                                    v[e] = see >> e & 1u ? v[e] : 0xff800000u;
-                                }
-                            }
                             float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
 #pragma unroll
                             for (int e = 2; e < 30; e += 4) {
@@ -1034,31 +970,38 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         const float    nm = (m == -INFINITY ? 0.0f : -m) + TS_OFF<PARTS>;
                         const uint64_t nm2 = f2pack(nm, nm), fa2 = f2pack(factor, factor);
                         uint64_t       sum2 = 0ull;
-#pragma unroll 1
-                        for (int c = 0; c < 4; c++) {
-                            uint32_t v[32], hi[16], lo[16];
-                            tmem_ld32(s_col + (uint32_t) (c * 32), v);
-                            tmem_ld_wait_tie(v);
-                            const uint32_t see = !masked ? 0xffffffffu : live ? seen(j * TS_N + c * 32) : 0u;
+                        // 16 columns and the load of the next ones; over them 8 of the weights' first part and 8 of the second
+                        uint32_t v[2][16];
+                        auto     weights = [&](uint32_t (&s16)[16], int c) {
+                            uint32_t hi[16];
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
+                            for (int i = 0; i < 8; i++) {
                                 float x, y;
-                                f2unpack(ffma2(f2pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), fa2, nm2), x, y);
-                                if (masked) {
-                                    x = see >> (2 * i) & 1u ? x : -INFINITY, y = see >> (2 * i + 1) & 1u ? y : -INFINITY;
-                                }
+                                f2unpack(ffma2(f2pack(__uint_as_float(s16[2 * i]), __uint_as_float(s16[2 * i + 1])), fa2, nm2), x, y);
                                 const uint64_t p2 = f2pack(ex2(x), ex2(y));
                                 sum2 = fadd2(sum2, p2);
                                 f2unpack(p2, x, y);
-                                // the remainder is above 0, so that its product with an infinite value has the sign of
-                                // the other part's (2^-38 of the row's largest weight is far below F32's last bit)
+                                // the remainder of a weight above 0 is above 0, so that its product with an infinite value has
+                                // the sign of the other part's (2^-38 of the row's largest weight is far below F32's last bit)
                                 hi[i] = ts_pack_rz<BF16>(x, y);
                                 const float2 f = ts_unpack<BF16>(hi[i]);
                                 f2unpack(ffma2(f2pack(f.x, f.y), f2pack(-1.0f, -1.0f), p2), x, y);
-                                lo[i] = masked ? ts_pack<BF16>(x, y) : ts_positive<BF16>(ts_pack<BF16>(x, y));
+                                hi[8 + i] = __vmaxu2(ts_pack<BF16>(x, y), __vminu2(hi[i], BF16 ? 0x00800080u : 0x00010001u));
                             }
-                            tmem_st16(s_col + (uint32_t) (c * 32), hi);
-                            tmem_st16(s_col + (uint32_t) (c * 32 + 16), lo);
+                            tmem_st16(s_col + (uint32_t) (c * 16), hi);
+                        };
+                        tmem_ld16(s_col, v[0]);
+                        tmem_ld16_wait(v[0]);
+#pragma unroll 1
+                        for (int c = 0; c < 8; c += 2) {
+                            tmem_ld16(s_col + (uint32_t) (c * 16 + 16), v[1]);
+                            weights(v[0], c);
+                            tmem_ld16_wait(v[1]);
+                            if (c < 6) {
+                                tmem_ld16(s_col + (uint32_t) (c * 16 + 32), v[0]);
+                            }
+                            weights(v[1], c + 1);
+                            tmem_ld16_wait(v[0]);
                         }
                         float x, y;
                         f2unpack(sum2, x, y);
@@ -1080,11 +1023,21 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             }
                         }
                     }
-                    tc_fence_before();
-                    dn_mbar_arrive(&bar[TB_OFREE + w]);
                 }
             }
             // ---- the two streams' maxima and sums
+            if constexpr (PARTS == 2) {  // to where PARTS 1 has them
+#pragma unroll
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        o[e] = __float_as_uint(acc[c * 32 + e]);
+                    }
+                    tmem_st32(o_col + (uint32_t) (c * 32), o);
+                }
+                tmem_st_wait();
+            }
             ml[w * TS_M + r] = make_float2(m, l);
             if (PARTS == 1 && any) {
                 wait(TB_OFULL + w, used++);
@@ -1094,37 +1047,36 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             const float  M = fmaxf(m, other.x), mine_f = m == M ? 1.0f : ex2(m - M), other_f = other.x == M ? 1.0f : ex2(other.x - M);
             l = w == 0 ? fmaf(l, mine_f, other.y * other_f) : fmaf(other.y, other_f, l * mine_f);
             l = f0 != f0 && M != -INFINITY ? NAN : l;
-            const float inv = whole && l != 0.0f ? 1.0f / l : whole ? 0.0f : 1.0f;
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            const bool  whole = tile0 == 0 && tile1 == it.tiles;
+            uint64_t    al;  // where this row goes, or the part's slot
+            if (whole) {
+                const int hd = it.h * p.ratio + row - my_node * p.ratio;
+                al = reinterpret_cast<uint64_t>(p.o.data + (int64_t) hd * p.o.nb1 + (int64_t) my_node * p.o.nb2 + (int64_t) it.s * p.o.nb3);
+            } else {
+                al = reinterpret_cast<uint64_t>(p.part + it.slot);
+            }
             if (!whole && live && w == 0) {  // behind the slot's rows
-                *(reinterpret_cast<float2 *>(al + (int64_t) (slot_rows - r) * D * 4) + r) = make_float2(M, l);
+                reinterpret_cast<float2 *>(al + (int64_t) slot_rows * D * 4)[r] = make_float2(M, l);
             }
             // ---- the sums: each stream takes half of the columns, 16 at a time, and stores them by whole rows
             const bool odd = tail && dirty[pieces & 1] && live;
             auto       columns = [&](int c, uint32_t (&o)[16]) {  // of this stream's sums, 16 from c on
-                if constexpr (PARTS == 1) {
-                    if (any) {
-                        tmem_ld16(o_col + (uint32_t) c, o);
-                        tmem_ld16_wait(o);
-                    } else {
+                tmem_ld16(o_col + (uint32_t) c, o);
+                tmem_ld16_wait(o);
+                if (PARTS == 1 && !any) {  // (what is there is not the piece's)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            o[e] = 0u;
-                        }
+                    for (int e = 0; e < 16; e++) {
+                        o[e] = 0u;
                     }
                 }
             };
             const int swz = (r >> 1) & 3;
-#pragma unroll PARTS == 2 ? D / 32 : 1
+#pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
                 uint32_t o[16];
                 const int theirs = (w ^ 1) * (D / 2) + c * 16, mine = w * (D / 2) + c * 16;
                 columns(theirs, o);
-                if constexpr (PARTS == 2) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        o[e] = __float_as_uint(w ? acc[c * 16 + e] : acc[D / 2 + c * 16 + e]);
-                    }
-                }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     give[r * 4 + (k ^ swz)] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
@@ -1137,19 +1089,15 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     const float4 f = take[r * 4 + (k ^ swz)];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        float a = __uint_as_float(o[4 * k + e]);
-                        if constexpr (PARTS == 2) {
-                            a = w ? acc[D / 2 + c * 16 + k * 4 + e] : acc[c * 16 + k * 4 + e];
-                        }
-                        x[4 * k + e] = a * mine_f + (&f.x)[e] * other_f;
+                        x[4 * k + e] = __uint_as_float(o[4 * k + e]) * mine_f + (&f.x)[e] * other_f;
                     }
                 }
                 if (odd) {
                     // elements that are no numbers, of nodes that the row sees: they were left out of the products
 #pragma unroll 1
-                    for (int n = 0; n < nodes; n++) {
+                    for (int n = 0; n < it.nodes; n++) {
                         const int key = held + n;
-                        if (key / TS_N < it.a || key / TS_N >= it.b || !(bits[n >> 5] >> (n & 31) & 1u)) {
+                        if (key / TS_N < tile0 || key / TS_N >= tile1 || !(bits[n >> 5] >> (n & 31) & 1u)) {
                             continue;
                         }
                         const uint16_t * v = reinterpret_cast<const uint16_t *>(p.v.data + (int64_t) key * p.v.nb1 + (int64_t) it.h * p.v.nb2 + (int64_t) it.s * p.v.nb3) + mine;
@@ -1161,7 +1109,13 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     }
                 }
                 softmax_barrier();  // (what this stream gave has been taken: its place holds the rows now)
-                if (warp_live) {
+                if (!whole && live) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        reinterpret_cast<float4 *>(al)[(mine / 4 + k) * slot_rows + r] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+                    }
+                }
+                if (whole && warp_live) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         give[r * 4 + (k ^ swz)] = make_float4(x[4 * k] * inv, x[4 * k + 1] * inv, x[4 * k + 2] * inv, x[4 * k + 3] * inv);
@@ -1172,20 +1126,18 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         const int    k = lane & 3;
                         const float4 f = give[(quad * 32 + i) * 4 + (k ^ ((i >> 1) & 3))];
                         char *       to = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, al, i));
-                        if (quad * 32 + i < its_rows) {
-                            ts_store4(to, mine + k * 4, f, type, !whole || p.o.vec);
+                        if (quad * 32 + i < it.rows) {
+                            ts_store4(to, mine + k * 4, f, p.o.type, p.o.vec);
                         }
                     }
                     __syncwarp();
                 }
             }
-            if (PARTS == 1 && any) {
-                tc_fence_before();
-                dn_mbar_arrive(&bar[TB_OFREE + w]);
-            }
+            tc_fence_before();
             if (own == 0) {
                 dirty[pieces & 1] = 0;  // (set again two pieces on, when this thread has been through the next)
             }
+            ts_drop(bar, pieces, lane);
             pieces++;
         }
         if (!ok) {
@@ -1205,49 +1157,75 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     }
 }
 
-// Joins the parts of units: one row by D / 4 lanes, the parts in their order.
+// Joins the parts of units, in their order.  Items of 32 rows and 16 columns over all CTAs: a warp has four columns, a lane
+// a row, and every load of 8 parts in flight.
 template <int D>
-__global__ void __launch_bounds__(TJ_ROWS * D / 4) tree_attn_join_kernel(const TreeAttnParams p, int blocks, int slot_rows) {
+__global__ void __launch_bounds__(128) tree_attn_join_kernel(const TreeAttnParams p, int blocks, int groups, int slot_rows) {
+    constexpr int  PER = 8;  // parts loaded at a time
+    __shared__ int list[TJ_UNITS], counts[4];
+    const int      tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     kv8_dep_wait();
-    constexpr int PER = 8;  // parts loaded at a time
-    const TsJoin  t   = *(reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE) + blockIdx.x);
-    const int     rb = (int) blockIdx.x % blocks, lane = threadIdx.x % (D / 4), r = (int) blockIdx.y * TJ_ROWS + threadIdx.x / (D / 4);
-    if (t.parts == 0 || r >= t.rows) {
-        return;
+    const TsJoin * units = reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE);
+    int            n_units = 0;
+    for (int i0 = 0; i0 < groups * blocks; i0 += 128) {  // which groups have one, in their order
+        const bool     has = i0 + tid < groups * blocks && units[i0 + tid].parts > 0;
+        const unsigned all = __ballot_sync(0xffffffffu, has);
+        if (lane == 0) {
+            counts[warp] = __popc(all);
+        }
+        __syncthreads();
+        int at = n_units + __popc(all & ((1u << lane) - 1u));
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            at += w < warp ? counts[w] : 0;
+            n_units += counts[w];
+        }
+        if (has) {
+            list[at] = i0 + tid;
+        }
+        __syncthreads();
     }
     const int64_t step = (int64_t) blocks * 2 * ts_slot_floats(slot_rows, D);
-    auto          part = [&](int k) { return p.part + (k == 0 ? t.part0 : t.part1 + (k - 1) * step); };
-    float         M = -INFINITY, l = 0.0f;
-    float4        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k0 = 0; k0 < t.parts; k0 += PER) {
-        float2 x[PER];
-        float4 v[PER];
-#pragma unroll
-        for (int k = 0; k < PER; k++) {
-            const float * at = part(min(k0 + k, t.parts - 1));
-            x[k] = *reinterpret_cast<const float2 *>(at + slot_rows * D + 2 * r);
-            v[k] = *(reinterpret_cast<const float4 *>(at + r * D) + lane);
+    const int     quarters = (slot_rows + 31) / 32, per_unit = quarters * (D / 16);
+    for (int item = blockIdx.x; item < n_units * per_unit; item += (int) gridDim.x) {
+        const int    u = list[item / per_unit], rest = item % per_unit, r = rest % quarters * 32 + lane, k4 = rest / quarters * 4 + warp;
+        const TsJoin t = units[u];
+        if (r >= t.rows) {
+            continue;
         }
-        float top = M;
+        auto   part = [&](int k) { return p.part + (k == 0 ? t.part0 : t.part1 + (k - 1) * step); };
+        float  M = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k0 = 0; k0 < t.parts; k0 += PER) {
+            float2 x[PER];
+            float4 v[PER];
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            top = fmaxf(top, x[k].x);
-        }
-        const float g = M == top ? 1.0f : ex2(M - top);
-        l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
+            for (int k = 0; k < PER; k++) {
+                const float * at = part(min(k0 + k, t.parts - 1));
+                x[k] = reinterpret_cast<const float2 *>(at + slot_rows * D)[r];
+                v[k] = reinterpret_cast<const float4 *>(at)[k4 * slot_rows + r];
+            }
+            float top = M;
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            if (k0 + k < t.parts) {
-                const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
-                l = fmaf(x[k].y, f, l);
-                o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
+            for (int k = 0; k < PER; k++) {
+                top = fmaxf(top, x[k].x);
+            }
+            const float g = M == top ? 1.0f : ex2(M - top);
+            l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                if (k0 + k < t.parts) {
+                    const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
+                    l = fmaf(x[k].y, f, l);
+                    o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
+                }
             }
         }
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        const int   row = u % blocks * TS_M + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
+        ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * k4,
+                  make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
     }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    const int   row = rb * TS_M + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
-    ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * lane,
-              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
 }
 
 template <int D, bool BF16, int PARTS>
@@ -1274,12 +1252,12 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
     }
     const int blocks = tree_attn_blocks(p), groups = tree_attn_groups(p, sms);
     const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
-    e = kv8_launch(kern, dim3((unsigned) (groups * blocks)), TS_THREADS, smem, stream, tmk, tmv, p, blocks, groups, rows);
+    e = kv8_launch(kern, dim3((unsigned) (groups * blocks)), TS_THREADS, smem, stream, tmk, tmv, p, blocks, groups, rows, p.n_kv > TS_LEAST * TS_N ? 1 : 0);
     if (e != cudaSuccess || p.n_kv <= TS_LEAST * TS_N) {
         return e;  // (no unit is in parts)
     }
-    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) (groups * blocks), (unsigned) ((rows + TJ_ROWS - 1) / TJ_ROWS)), TJ_ROWS * D / 4, 0, stream, p,
-                      blocks, rows);
+    const int items = groups * blocks * ((rows + 31) / 32) * (D / 16);
+    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) std::min(items, 4 * sms)), 128, 0, stream, p, blocks, groups, rows);
 }
 
 template <int D, bool BF16>
