@@ -47,6 +47,7 @@ constexpr int TS_M       = 128;  // rows of a block
 constexpr int TS_N       = 128;  // keys of a tile
 constexpr int TS_TMEM    = 512;  // columns: S of two tiles, P V of two tiles
 constexpr int TS_GROW    = 7;    // (PARTS 1) log2 of what a weight may exceed the maximum of the tiles before by
+constexpr int TS_EMU     = 2;    // (PARTS 1) of every 8 pairs of weights, those by polynomial: the special-function unit is the bound
 constexpr int TS_LONG    = 32768;
 constexpr int TS_SPACE   = 256;  // bytes of the workspace before the list of units in parts
 constexpr int TS_LEAST   = 4;    // tiles of a part, at least: a part costs as much as about two tiles, and the joining kernel
@@ -251,7 +252,9 @@ __device__ __forceinline__ TsSeq ts_seq(const TreeAttnParams & p, int s) {
 struct TsLine {
     int W, G, each, more;  // `more` pieces have a tile more than `each`
 
-    __device__ __forceinline__ TsLine(int W_, int groups) : W(W_), G(max(1, min(groups, W_ / TS_LEAST))) {
+    __device__ __forceinline__ void cut(int W_, int groups) {
+        W    = W_;
+        G    = max(1, min(groups, W_ / TS_LEAST));
         each = ts_div(W, G);
         more = W - each * G;
     }
@@ -290,15 +293,18 @@ struct TsPlan {
     int                    s, first, x, end;  // first: of sequence s on the line (even: among the parts); end: before its move to a border
     TsSeq                  q;
 
-    __device__ __forceinline__ TsPlan(const TreeAttnParams & p_, int group_, int groups, int rb_, int blocks_, int floats_)
-        : p(p_), group(group_), rb(rb_), blocks(blocks_), floats(floats_), even(0), ln(0, 1), s(0), first(0), x(0), end(0), q{ 0, 0, 0, 0 } {
+    __device__ __forceinline__ TsPlan(const TreeAttnParams & p_, int group_, int rb_, int blocks_, int floats_)
+        : p(p_), group(group_), rb(rb_), blocks(blocks_), floats(floats_), even(0), s(0), first(0), x(0), end(0), q{ 0, 0, 0, 0 } {}
+
+    __device__ __forceinline__ void find(int groups) {  // by a whole warp
         // each lane sums some sequences; all tiles are fewer than 2^30 (checked by the host)
         const int lane = threadIdx.x & 31, each = (p.n_seq + 31) / 32, s0 = min(lane * each, p.n_seq), s1 = min(s0 + each, p.n_seq);
         int       mine = 0, units = 0, most = 0;
+        TsSeq     own = { 0, 0, 0, 0 };  // the lane's last sequence, its only one where there are up to 32
 #pragma unroll 1
         for (int i = s0; i < s1; i++) {
-            const int n = ts_seq(p, i).tiles;
-            mine += n, units += n > 0, most = max(most, n);
+            own = ts_seq(p, i);
+            mine += own.tiles, units += own.tiles > 0, most = max(most, own.tiles);
         }
         const int W = __reduce_add_sync(0xffffffffu, mine) * p.n_head_kv, U = __reduce_add_sync(0xffffffffu, units) * p.n_head_kv;
         most = __reduce_max_sync(0xffffffffu, most);
@@ -312,18 +318,19 @@ struct TsPlan {
             int       parts = 0;
 #pragma unroll 1
             for (int i = 0; i < p.n_seq; i++) {
-                parts += ts_up(ts_seq(p, i).tiles, t);
+                const int n = each == 1 ? __shfl_sync(0xffffffffu, own.tiles, i) : ts_seq(p, i).tiles;
+                parts += (n + t - 1) / t;
             }
             const unsigned fits = __ballot_sync(0xffffffffu, parts * p.n_head_kv <= groups);
             even = __shfl_sync(0xffffffffu, t, __ffs(fits) - 1);  // (the last lane's fits)
             mine = 0;
 #pragma unroll 1
             for (int i = s0; i < s1; i++) {
-                mine += ts_up(ts_seq(p, i).tiles, even);
+                mine += ts_up((each == 1 ? own : ts_seq(p, i)).tiles, even);
             }
             from = group, to = group + 1;
         } else {
-            ln   = TsLine(W, groups);
+            ln.cut(W, groups);
             from = group < ln.G ? ln.at(group) : W, to = group < ln.G ? ln.at(group + 1) : W;
         }
         mine *= p.n_head_kv;
@@ -339,7 +346,7 @@ struct TsPlan {
             return;  // (nothing for this group)
         }
         int i = s0;
-        if (here >> lane & 1u) {
+        if (each > 1 && (here >> lane & 1u)) {
 #pragma unroll 1
             for (;; i++) {
                 const int n = weight(ts_seq(p, i).tiles);
@@ -351,7 +358,9 @@ struct TsPlan {
         }
         const int src = __ffs(here) - 1;
         s = __shfl_sync(0xffffffffu, i, src), first = __shfl_sync(0xffffffffu, at, src);
-        q = ts_seq(p, s);
+        q = each == 1 ? TsSeq{ __shfl_sync(0xffffffffu, own.L, src), __shfl_sync(0xffffffffu, own.nodes, src), __shfl_sync(0xffffffffu, own.keys, src),
+                               __shfl_sync(0xffffffffu, own.tiles, src) } :
+                        ts_seq(p, s);
         x = from, end = to;
         if (!even) {
             x = TsLine::border(x, first + ts_div(x - first, q.tiles) * q.tiles, q.tiles);
@@ -471,58 +480,62 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
         // a row with an infinity or NaN becomes zeros with a factor of NaN
         const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
         const int   e0 = lane * E;
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) {
-            const char * at = place(i, e0 * esz / 16) + e0 * esz % 16;
-            float        x[E];
-            if (esz == 4) {
+#pragma unroll 1
+        for (int i0 = 0; i0 < 16; i0 += 4) {
+            float    x[4][E];
+            uint32_t top[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const char * at = place(i0 + i, e0 * esz / 16) + e0 * esz % 16;
+                top[i] = 0;
 #pragma unroll
                 for (int e = 0; e < E; e += 2) {
-                    const float2 f = reinterpret_cast<const float2 *>(at)[e / 2];
-                    x[e] = f.x, x[e + 1] = f.y;
+                    float2 f;
+                    if (esz == 4) {
+                        f = reinterpret_cast<const float2 *>(at)[e / 2];
+                    } else {
+                        const uint32_t u = reinterpret_cast<const uint32_t *>(at)[e / 2];
+                        f = p.q.type == KV_F16 ? h2_to_f2(u) : bf2_to_f2(u);
+                    }
+                    x[i][e] = f.x, x[i][e + 1] = f.y;
+                    top[i]  = max(top[i], max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
                 }
-            } else {
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                top[i] = __reduce_max_sync(0xffffffffu, top[i]);  // (and the rows have been read)
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool  odd = top[i] >= 0x7f800000u;
+                const int   ex  = BF16 ? 0 : (top[i] == 0 || odd ? 0 : max((int) (top[i] >> 23) - 127, -112)) - 14;
+                const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
+                uint32_t    hi[E / 2], lo[E / 2];
 #pragma unroll
                 for (int e = 0; e < E; e += 2) {
-                    const uint32_t u = reinterpret_cast<const uint32_t *>(at)[e / 2];
-                    const float2   f = p.q.type == KV_F16 ? h2_to_f2(u) : bf2_to_f2(u);
-                    x[e] = f.x, x[e + 1] = f.y;
+                    const float a = odd ? 0.0f : x[i][e] * dn, b = odd ? 0.0f : x[i][e + 1] * dn;
+                    hi[e / 2]      = ts_pack<BF16>(a, b);
+                    const float2 f = ts_unpack<BF16>(hi[e / 2]);
+                    lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
                 }
-            }
-            uint32_t top = 0;
+                char * to = qs + (e0 / 64) * BLOCK + (ra + i0 + i) * 128 + ((((e0 % 64) / 8) ^ ((i0 + i) & 7)) << 4) + (e0 % 8) * 2;
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-            }
-            top = __reduce_max_sync(0xffffffffu, top);  // (and the row has been read)
-            const bool  odd = top >= 0x7f800000u;
-            const int   ex  = BF16 ? 0 : (top == 0 || odd ? 0 : max((int) (top >> 23) - 127, -112)) - 14;
-            const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
-            uint32_t    hi[E / 2], lo[E / 2];
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float a = odd ? 0.0f : x[e] * dn, b = odd ? 0.0f : x[e + 1] * dn;
-                hi[e / 2]      = ts_pack<BF16>(a, b);
-                const float2 f = ts_unpack<BF16>(hi[e / 2]);
-                lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
-            }
-            char * to = qs + (e0 / 64) * BLOCK + (ra + i) * 128 + ((((e0 % 64) / 8) ^ (i & 7)) << 4) + (e0 % 8) * 2;
-#pragma unroll
-            for (int e = 0; e < E / 2; e++) {
-                reinterpret_cast<uint32_t *>(to)[e]      = hi[e];
-                reinterpret_cast<uint32_t *>(to + QT)[e] = lo[e];
-            }
-            if (lane == 0) {
-                factors[ra + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
+                for (int e = 0; e < E / 2; e++) {
+                    reinterpret_cast<uint32_t *>(to)[e]      = hi[e];
+                    reinterpret_cast<uint32_t *>(to + QT)[e] = lo[e];
+                }
+                if (lane == 0) {
+                    factors[ra + i0 + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
+                }
             }
         }
     }
 }
 
-// Waits for the next piece that warp 0 tells of; false: there is none, or it did not come in time.  By whole warps.
+// Waits for the next piece that warp 0 tells of (the first is there since the block's barrier); false: there is none, or it did not come in time.  By whole warps.
 __device__ __forceinline__ bool ts_take(const TsPiece * told, uint64_t * bar, uint32_t pieces, uint64_t deadline) {
     const uint32_t k = pieces % TS_PIECES;
-    return dn_wait_warp(&bar[TB_PIECE + k], (pieces / TS_PIECES) & 1, deadline) && told[k].rows > 0;
+    return (pieces == 0 || dn_wait_warp(&bar[TB_PIECE + k], (pieces / TS_PIECES) & 1, deadline)) && told[k].rows > 0;
 }
 
 // What warp 0 told is not needed any more.
@@ -571,6 +584,11 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     TsPiece *      told = reinterpret_cast<TsPiece *>(smem + L::OFF_PIECE);
     TsPiece        it;
     uint32_t       pieces = 0;  // that a warp has taken
+    TsPlan         plan(p, (int) blockIdx.x / blocks, rb, blocks, ts_slot_floats(slot_rows, D));
+    if (warp == 0) {
+        plan.find(groups);
+        told[0] = plan.next();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -589,18 +607,21 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         };
         if (warp == 0) {
             // =================================================== the pieces, TMA
-            TsPlan   plan(p, (int) blockIdx.x / blocks, groups, rb, blocks, ts_slot_floats(slot_rows, D));
             TsJoin * join = reinterpret_cast<TsJoin *>(reinterpret_cast<char *>(p.status) + TS_SPACE) + blockIdx.x;
             if (lane == 0) {
                 uint32_t c = 0;
                 join->parts = 0;
                 do {
-                    it = plan.next();
-                    if (pieces >= (uint32_t) TS_PIECES && !mbar_wait_bounded(&bar[TB_PFREE + pieces % TS_PIECES], (pieces / TS_PIECES - 1) & 1, deadline)) {
-                        ok = false;
-                        break;
+                    if (pieces == 0) {
+                        it = told[0];
+                    } else {
+                        it = plan.next();
+                        if (pieces >= (uint32_t) TS_PIECES && !mbar_wait_bounded(&bar[TB_PFREE + pieces % TS_PIECES], (pieces / TS_PIECES - 1) & 1, deadline)) {
+                            ok = false;
+                            break;
+                        }
+                        told[pieces % TS_PIECES] = it;
                     }
-                    told[pieces % TS_PIECES] = it;
                     dn_mbar_arrive(&bar[TB_PIECE + pieces % TS_PIECES]);
                     pieces++;
                     if (it.rows == 0) {
@@ -932,7 +953,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             for (int i = 0; i < 16; i++) {
                                 float x, y;
                                 f2unpack(ffma2(f2pack(__uint_as_float(v[c * 32 + 2 * i]), __uint_as_float(v[c * 32 + 2 * i + 1])), fa2, nm2), x, y);
-                                const uint64_t p2 = f2pack(ex2(x), ex2(y));
+                                const uint64_t p2 = (i & 7) < TS_EMU ? exp2_poly2(f2pack(x, y)) : f2pack(ex2(x), ex2(y));
                                 sum2 = fadd2(sum2, p2);
                                 f2unpack(p2, x, y);
                                 hi[i] = ts_pack<BF16>(x, y);
