@@ -2,9 +2,10 @@
 // (tcgen05 + TMEM), sm_100a.
 //
 // Rows of a unit (sequence, kv head) are (node, head of the group) pairs in that order; a block has 128 of them, so the
-// query heads of a kv head and the nodes share each K/V tile of 128 keys.  All CTAs (one per SM) are RB = blocks of a
-// unit beside one another: groups of RB CTAs, each with one block, walk the same keys at the same time, so a K/V
-// tile comes from HBM once.
+// query heads of a kv head and the nodes share each K/V tile of 128 keys.  One CTA per SM.  Where all trees have the same
+// nodes, the CTAs with a unit's blocks are a group, beside one another, that walks the same keys at the same time, so that
+// a K/V tile comes from HBM once; where each tree says how many it has, the blocks are units of their own, since a group's CTAs
+// would have nothing to do for the smaller trees (8 trees of up to 200 nodes: 128 us in groups of 7).
 //
 // Split, found on the device from the lengths, so that a captured call follows them:
 //   units up to groups   every unit in even parts of about the same size, one part a group (TsPlan)
@@ -52,6 +53,7 @@ constexpr int TS_LONG    = 32768;
 constexpr int TS_SPACE   = 256;  // bytes of the workspace before the list of units in parts
 constexpr int TS_LEAST   = 4;    // tiles of a part, at least: a part costs as much as about two tiles, and the joining kernel
 constexpr int TS_PIECES  = 4;    // pieces that warp 0 may be ahead
+constexpr int TS_COST    = 3;    // tiles' time that a unit takes beside them
 constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for
 constexpr int TJ_UNITS   = 512;  // units in parts, at most one a CTA: there are no more CTAs than SMs or blocks of a unit
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
@@ -78,7 +80,7 @@ struct TsSmem {
     static constexpr int OFF_ML   = OFF_F + 2 * TS_M * 4;         // [stream][row] (m, l)
     static constexpr int OFF_BAR  = OFF_ML + 2 * TS_M * 8;
     static constexpr int OFF_PIECE = OFF_BAR + 40 * 8;            // [TS_PIECES]
-    static constexpr int OFF_MISC  = OFF_PIECE + TS_PIECES * 48;
+    static constexpr int OFF_MISC  = OFF_PIECE + TS_PIECES * 64;
     static constexpr int TOTAL     = OFF_MISC + 32 + 1024;        // + alignment
 };
 static_assert(TsSmem<128, 1>::TOTAL <= 232448 && TsSmem<128, 2>::TOTAL <= 232448 && TsSmem<64, 2>::TOTAL <= 232448, "shared memory");
@@ -220,7 +222,8 @@ __device__ __forceinline__ void ts_store4(char * row, int e, const float4 & f, i
 
 // What the group that has a unit's first part leaves for the joining kernel.
 struct TsJoin {
-    int     s, h, parts, rows;  // parts 0: the group has no such unit
+    int     s, h, parts, rows;  // parts 0: the CTA has no such unit
+    int64_t row0;               // the block's first row
     int64_t part0, part1;       // where the first part and the second are, in floats; the others follow at even steps
 };
 
@@ -247,14 +250,14 @@ __device__ __forceinline__ TsSeq ts_seq(const TreeAttnParams & p, int s) {
     return q;
 }
 
-// The line of W tiles in G even pieces, piece g from `at(g)` on.  A border closer than TS_LEAST tiles to a unit's start or end
-// goes there, so that no part of a unit has less.
+// The line of all units' tiles, each unit with TS_COST more, in G even pieces, piece g from `at(g)` on.  A border closer than
+// TS_LEAST tiles to a unit's start or end goes there, so that no part of a unit has less.
 struct TsLine {
     int W, G, each, more;  // `more` pieces have a tile more than `each`
 
     __device__ __forceinline__ void cut(int W_, int groups) {
         W    = W_;
-        G    = max(1, min(groups, W_ / TS_LEAST));
+        G    = max(1, min(groups, W_ / (TS_COST + TS_LEAST)));
         each = ts_div(W, G);
         more = W - each * G;
     }
@@ -269,32 +272,35 @@ struct TsLine {
         return min(G - 1, x < y ? ts_div(x, each + 1) : each > 0 ? more + ts_div(x - y, each) : G - 1);
     }
 
-    // border x, of a unit of n tiles that starts at `first` and holds x
+    // border x, of a unit that starts at `first`, is n long and holds x
     static __device__ __forceinline__ int border(int x, int first, int n) {
-        return x - first < TS_LEAST ? first : first + n - x < TS_LEAST ? first + n : x;
+        return x - first < TS_COST + TS_LEAST ? first : first + n - x < TS_LEAST ? first + n : x;
     }
 };
 
 // Tiles [a, b) of a unit, for one block of its rows, as warp 0 tells the others.
 struct __align__(16) TsPiece {
     int     s, h, a, b;
-    int     rows;                   // rows of the block; 0: there is no further piece
+    int     rb, rows;               // the block of rows, how many it has; 0: there is no further piece
     int     L, nodes, keys, tiles;  // of the sequence
     int     unit;                   // where the unit starts
     int64_t slot;                   // floats, where it is a part
 };
 
+static_assert(sizeof(TsPiece) == 64, "shared memory");
+
 // A group's pieces, one after another.
 struct TsPlan {
     const TreeAttnParams & p;
-    int                    group, rb, blocks, floats;  // floats of a part's slot; a group has two
-    int                    even;                       // 0, or the tiles of a part, at most
+    int                    group, beside, wide, floats;  // floats of a part's slot; a CTA has two
+    int                    even;                         // 0, or the tiles of a part, at most
     TsLine                 ln;
     int                    s, first, x, end;  // first: of sequence s on the line (even: among the parts); end: before its move to a border
     TsSeq                  q;
 
-    __device__ __forceinline__ TsPlan(const TreeAttnParams & p_, int group_, int rb_, int blocks_, int floats_)
-        : p(p_), group(group_), rb(rb_), blocks(blocks_), floats(floats_), even(0), s(0), first(0), x(0), end(0), q{ 0, 0, 0, 0 } {}
+    // wide: the CTAs of a group, each with the block of its place (1: the blocks are units of their own)
+    __device__ __forceinline__ TsPlan(const TreeAttnParams & p_, int wide_, int floats_)
+        : p(p_), group((int) blockIdx.x / wide_), beside((int) blockIdx.x % wide_), wide(wide_), floats(floats_), even(0), s(0), first(0), x(0), end(0), q{ 0, 0, 0, 0 } {}
 
     __device__ __forceinline__ void find(int groups) {  // by a whole warp
         // each lane sums some sequences; all tiles are fewer than 2^30 (checked by the host)
@@ -304,9 +310,9 @@ struct TsPlan {
 #pragma unroll 1
         for (int i = s0; i < s1; i++) {
             own = ts_seq(p, i);
-            mine += own.tiles, units += own.tiles > 0, most = max(most, own.tiles);
+            mine += own.tiles * heads(own), units += own.tiles > 0 ? heads(own) : 0, most = max(most, own.tiles);
         }
-        const int W = __reduce_add_sync(0xffffffffu, mine) * p.n_head_kv, U = __reduce_add_sync(0xffffffffu, units) * p.n_head_kv;
+        const int W = __reduce_add_sync(0xffffffffu, mine), U = __reduce_add_sync(0xffffffffu, units);
         most = __reduce_max_sync(0xffffffffu, most);
         int from, to;
         if (p.n_seq <= TS_EVEN && U <= groups) {
@@ -318,22 +324,27 @@ struct TsPlan {
             int       parts = 0;
 #pragma unroll 1
             for (int i = 0; i < p.n_seq; i++) {
-                const int n = each == 1 ? __shfl_sync(0xffffffffu, own.tiles, i) : ts_seq(p, i).tiles;
-                parts += (n + t - 1) / t;
+                TsSeq c = own;
+                if (each == 1) {
+                    c.tiles = __shfl_sync(0xffffffffu, own.tiles, i), c.nodes = __shfl_sync(0xffffffffu, own.nodes, i);
+                } else {
+                    c = ts_seq(p, i);
+                }
+                parts += (c.tiles + t - 1) / t * heads(c);
             }
-            const unsigned fits = __ballot_sync(0xffffffffu, parts * p.n_head_kv <= groups);
+            const unsigned fits = __ballot_sync(0xffffffffu, parts <= groups);
             even = __shfl_sync(0xffffffffu, t, __ffs(fits) - 1);  // (the last lane's fits)
             mine = 0;
 #pragma unroll 1
             for (int i = s0; i < s1; i++) {
-                mine += ts_up((each == 1 ? own : ts_seq(p, i)).tiles, even);
+                mine += weight(each == 1 ? own : ts_seq(p, i));
             }
             from = group, to = group + 1;
         } else {
-            ln.cut(W, groups);
-            from = group < ln.G ? ln.at(group) : W, to = group < ln.G ? ln.at(group + 1) : W;
+            ln.cut(W + U * TS_COST, groups);
+            from = group < ln.G ? ln.at(group) : ln.W, to = group < ln.G ? ln.at(group + 1) : ln.W;
+            mine += units * TS_COST;
         }
-        mine *= p.n_head_kv;
         int at = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -349,7 +360,7 @@ struct TsPlan {
         if (each > 1 && (here >> lane & 1u)) {
 #pragma unroll 1
             for (;; i++) {
-                const int n = weight(ts_seq(p, i).tiles);
+                const int n = weight(ts_seq(p, i));
                 if (from < at + n) {
                     break;
                 }
@@ -363,68 +374,78 @@ struct TsPlan {
                         ts_seq(p, s);
         x = from, end = to;
         if (!even) {
-            x = TsLine::border(x, first + ts_div(x - first, q.tiles) * q.tiles, q.tiles);
+            x = TsLine::border(x, first + ts_div(x - first, q.tiles + TS_COST) * (q.tiles + TS_COST), q.tiles + TS_COST);
         }
     }
 
-    // a sequence's length on the line, or its parts
-    __device__ __forceinline__ int weight(int tiles) const {
-        return (even ? ts_up(tiles, even) : tiles) * p.n_head_kv;
+    // units of a sequence: its kv heads, by its blocks of rows where these are on their own
+    __device__ __forceinline__ int heads(const TsSeq & c) const {
+        return wide > 1 ? p.n_head_kv : p.n_head_kv * ((c.nodes * p.ratio + TS_M - 1) / TS_M);
     }
 
-    // the next piece that has rows in this block
+    // a sequence's length on the line, or its parts
+    __device__ __forceinline__ int weight(const TsSeq & c) const {
+        return c.tiles == 0 ? 0 : (even ? ts_up(c.tiles, even) : c.tiles + TS_COST) * heads(c);
+    }
+
+    // the next piece that has rows in this CTA's block
     __device__ __forceinline__ TsPiece next() {
         TsPiece c = {};
 #pragma unroll 1
         while (x < end) {
-            const int all = weight(q.tiles);
+            const int all = weight(q);
             if (x - first >= all) {
                 first += all;
                 q = ts_seq(p, ++s);
                 continue;
             }
-            const int rows = q.nodes * p.ratio - rb * TS_M;
-            if (rows <= 0) {  // (the block is empty: on to the next sequence)
-                x = first + all;
+            const int n = even ? ts_up(q.tiles, even) : q.tiles + TS_COST, i = ts_div(x - first, n);  // a unit's length, the unit
+            const int bl = wide > 1 ? 1 : (q.nodes * p.ratio + TS_M - 1) / TS_M;
+            c.h    = i / bl;
+            c.rb   = wide > 1 ? beside : i - c.h * bl;
+            c.rows = min(q.nodes * p.ratio - c.rb * TS_M, TS_M);
+            if (c.rows <= 0) {  // (the block is empty: on to the next sequence)
+                c.rows = 0;
+                x      = first + all;
                 continue;
             }
             c.s = s, c.L = q.L, c.nodes = q.nodes, c.keys = q.keys, c.tiles = q.tiles;
+            c.unit = first + i * n;
             if (even) {
-                const int parts = ts_up(q.tiles, even), i = x - first;
-                c.h          = ts_div(i, parts);
-                const int k  = i - c.h * parts;
-                c.unit = x - k, c.a = ts_div(k * q.tiles, parts), c.b = ts_div((k + 1) * q.tiles, parts);
+                const int k = x - c.unit;
+                c.a = ts_div(k * q.tiles, n), c.b = ts_div((k + 1) * q.tiles, n);
                 x++;
             } else {
-                c.h    = ts_div(x - first, q.tiles);
-                c.unit = first + c.h * q.tiles;
-                c.a    = x - c.unit;
-                c.b    = c.unit + q.tiles <= end ? q.tiles : TsLine::border(end, c.unit, q.tiles) - c.unit;
-                x      = c.b > c.a ? c.unit + c.b : end;
+                const int to = c.unit + n <= end ? c.unit + n : TsLine::border(end, c.unit, n);
+                c.a = max(x - c.unit - TS_COST, 0), c.b = to - c.unit - TS_COST;
+                if (to <= x) {
+                    c.rows = 0;
+                }
+                x = c.rows ? to : end;
             }
-            c.rows = c.b > c.a ? min(rows, TS_M) : 0;
             c.slot = part(c, second(c), group - second(c) + 1);
             return c;
         }
+        c.rows = 0;
         return c;
     }
 
     // the group that has the second part of a piece's unit
     __device__ __forceinline__ int second(const TsPiece & c) const {
-        return even ? c.unit + 1 : c.a == 0 ? group + 1 : ln.last(c.unit + TS_LEAST - 1) + 1;
+        return even ? c.unit + 1 : c.a == 0 ? group + 1 : ln.last(c.unit + TS_COST + TS_LEAST - 1) + 1;
     }
 
     // Where a unit's parts are: the first in a slot of the group before `g`, its second one unless the unit is the first that
     // the group has; the others in the first slots of g and the groups behind it.
     __device__ __forceinline__ int64_t part(const TsPiece & c, int g, int k) const {
-        const int64_t slots = ((int64_t) (g - 1 + k) * blocks + rb) * 2;
+        const int64_t slots = ((int64_t) (g - 1 + k) * wide + beside) * 2;
         return (slots + (k == 0 && !even && ln.at(g - 1) <= c.unit - TS_LEAST ? 1 : 0)) * floats;
     }
 
     // what the joining kernel has to know of a unit, from its first part
     __device__ __forceinline__ TsJoin join(const TsPiece & c) const {
-        const int g = second(c), parts = even ? ts_up(c.tiles, even) : ln.last(c.unit + c.tiles - TS_LEAST) - g + 2;
-        return { c.s, c.h, parts, c.rows, part(c, g, 0), part(c, g, 1) };
+        const int g = second(c), parts = even ? ts_up(c.tiles, even) : ln.last(c.unit + c.tiles + TS_COST - TS_LEAST) - g + 2;
+        return { c.s, c.h, parts, c.rows, c.rb * TS_M, part(c, g, 0), part(c, g, 1) };
     }
 };
 
@@ -432,11 +453,11 @@ struct TsPlan {
 // flight at once, and land where the row's products will read it: PARTS 1, as they are; PARTS 2, a row's bytes lie in
 // the places of its own two parts (F32: all of them), and the warp replaces one row after another.
 template <int D, bool BF16, int PARTS>
-__device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPiece & it, int rb, int ra, char * qs, float * factors, int lane) {
+__device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPiece & it, int ra, char * qs, float * factors, int lane) {
     constexpr int E = D / 32, QT = TsSmem<D, PARTS>::QT, BLOCK = TS_M * 128;
     const int     in = it.rows - ra, esz = p.q.type == KV_F32 ? 4 : 2;
     // lane i, and 16 + i: the address of row i
-    const int      rl = rb * TS_M + ra + (lane & 15), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
+    const int      rl = it.rb * TS_M + ra + (lane & 15), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
     const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
     // (not 0, whose product with the -inf of a key that is not seen would be no number)
     const float    by = fmaxf(fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E), 0x1p-126f);
@@ -548,7 +569,7 @@ __device__ __forceinline__ void ts_drop(uint64_t * bar, uint32_t pieces, int lan
 
 template <int D, bool BF16, int PARTS>
 __global__ void __launch_bounds__(TS_THREADS, 1)
-    tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TreeAttnParams p, int blocks,
+    tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TreeAttnParams p, int wide,
                         int groups, int slot_rows, int joined) {
     using L          = TsSmem<D, PARTS>;
     constexpr int NS = L::NS;
@@ -580,11 +601,10 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
     const uint64_t deadline = global_timer_ns() + p.timeout_ns;
-    const int      rb = (int) blockIdx.x % blocks;
     TsPiece *      told = reinterpret_cast<TsPiece *>(smem + L::OFF_PIECE);
     TsPiece        it;
     uint32_t       pieces = 0;  // that a warp has taken
-    TsPlan         plan(p, (int) blockIdx.x / blocks, rb, blocks, ts_slot_floats(slot_rows, D));
+    TsPlan         plan(p, wide, ts_slot_floats(slot_rows, D));
     if (warp == 0) {
         plan.find(groups);
         told[0] = plan.next();
@@ -743,7 +763,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     }
 #pragma unroll 1
                     for (int ra = (warp & 1) * 16; ra < TS_M; ra += 32) {
-                        ts_stage16<D, BF16, PARTS>(p, it, rb, ra, smem + L::OFF_Q, factors + (pieces & 1) * TS_M, lane);
+                        ts_stage16<D, BF16, PARTS>(p, it, ra, smem + L::OFF_Q, factors + (pieces & 1) * TS_M, lane);
                     }
                     fence_proxy_async_smem();
                     dn_mbar_arrive(&bar[TB_QREADY]);
@@ -803,13 +823,11 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     } else {
         // ======================================================= softmax and sums
         regs_inc<TS_REGS_SOFTMAX>();
-        const int      w = wg - 1, quad = warp & 3, r = quad * 32 + lane, row = rb * TS_M + r, own = tid - 128;
+        const int      w = wg - 1, quad = warp & 3, r = quad * 32 + lane, own = tid - 128;
         const uint32_t tl    = (uint32_t) (quad * 32) << 16;
         const uint32_t s_col = tmem + tl + (uint32_t) (w * TS_N), o_col = tmem + tl + 256u + (uint32_t) (w * D);
-        const int      my_node = row / p.ratio;
         const bool     cap = p.softcap > 0.0f;
         float4 *       give = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + w * (TS_M * 4), *take = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + (w ^ 1) * (TS_M * 4);
-        const uint32_t * bits = anc + min(my_node, TREE_MAX - 1) * (TREE_MAX / 32);
         uint32_t       tc = 0, used = 0;
         bool           ok = true;
         auto           wait = [&](int b, uint32_t i) {
@@ -823,13 +841,15 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             // (read where it is needed: the sums leave few registers)
             const TsPiece & it = told[pieces % TS_PIECES];
             const int       tile0 = it.a, tile1 = it.b, held = it.L;
+            const int       row = it.rb * TS_M + r, my_node = row / p.ratio;
+            const uint32_t * bits = anc + min(my_node, TREE_MAX - 1) * (TREE_MAX / 32);
             const bool      live = r < it.rows, warp_live = quad * 32 < it.rows;
             // ---- Q of the first piece, and each node's ancestors, where the piece has tiles with nodes
             const bool tail = tile1 * TS_N > held;
             {
                 const int nodes = it.nodes, parent = tail && own < nodes ? tree_parent(p.t, it.s % p.t.n_tree, own) : -1;
                 if (pieces == 0) {
-                    ts_stage16<D, BF16, PARTS>(p, it, rb, (w * 4 + quad) * 16, smem + L::OFF_Q, factors, lane);
+                    ts_stage16<D, BF16, PARTS>(p, it, (w * 4 + quad) * 16, smem + L::OFF_Q, factors, lane);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane < 8) {
@@ -1181,15 +1201,15 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
 // Joins the parts of units, in their order.  Items of 32 rows and 16 columns over all CTAs: a warp has four columns, a lane
 // a row, and every load of 8 parts in flight.
 template <int D>
-__global__ void __launch_bounds__(128) tree_attn_join_kernel(const TreeAttnParams p, int blocks, int groups, int slot_rows) {
+__global__ void __launch_bounds__(128) tree_attn_join_kernel(const TreeAttnParams p, int wide, int groups, int slot_rows) {
     constexpr int  PER = 8;  // parts loaded at a time
     __shared__ int list[TJ_UNITS], counts[4];
     const int      tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     kv8_dep_wait();
     const TsJoin * units = reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE);
     int            n_units = 0;
-    for (int i0 = 0; i0 < groups * blocks; i0 += 128) {  // which groups have one, in their order
-        const bool     has = i0 + tid < groups * blocks && units[i0 + tid].parts > 0;
+    for (int i0 = 0; i0 < groups * wide; i0 += 128) {  // which groups have one, in their order
+        const bool     has = i0 + tid < groups * wide && units[i0 + tid].parts > 0;
         const unsigned all = __ballot_sync(0xffffffffu, has);
         if (lane == 0) {
             counts[warp] = __popc(all);
@@ -1206,7 +1226,7 @@ __global__ void __launch_bounds__(128) tree_attn_join_kernel(const TreeAttnParam
         }
         __syncthreads();
     }
-    const int64_t step = (int64_t) blocks * 2 * ts_slot_floats(slot_rows, D);
+    const int64_t step = (int64_t) wide * 2 * ts_slot_floats(slot_rows, D);
     const int     quarters = (slot_rows + 31) / 32, per_unit = quarters * (D / 16);
     for (int item = blockIdx.x; item < n_units * per_unit; item += (int) gridDim.x) {
         const int    u = list[item / per_unit], rest = item % per_unit, r = rest % quarters * 32 + lane, k4 = rest / quarters * 4 + warp;
@@ -1243,7 +1263,7 @@ __global__ void __launch_bounds__(128) tree_attn_join_kernel(const TreeAttnParam
             }
         }
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        const int   row = u % blocks * TS_M + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
+        const int   row = (int) t.row0 + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
         ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * k4,
                   make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
     }
@@ -1271,14 +1291,14 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
         !encode_kv_tensor_map(&tmv, p.v.data, BF16, D, p.n_kv, p.n_head_kv, p.n_seq, p.v.nb1, p.v.nb2, p.v.nb3, TS_N)) {
         return cudaErrorInvalidValue;
     }
-    const int blocks = tree_attn_blocks(p), groups = tree_attn_groups(p, sms);
+    const int wide = tree_attn_wide(p), groups = tree_attn_groups(p, sms);
     const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
-    e = kv8_launch(kern, dim3((unsigned) (groups * blocks)), TS_THREADS, smem, stream, tmk, tmv, p, blocks, groups, rows, p.n_kv > TS_LEAST * TS_N ? 1 : 0);
+    e = kv8_launch(kern, dim3((unsigned) (groups * wide)), TS_THREADS, smem, stream, tmk, tmv, p, wide, groups, rows, p.n_kv > TS_LEAST * TS_N ? 1 : 0);
     if (e != cudaSuccess || p.n_kv <= TS_LEAST * TS_N) {
         return e;  // (no unit is in parts)
     }
-    const int items = groups * blocks * ((rows + 31) / 32) * (D / 16);
-    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) std::min(items, 4 * sms)), 128, 0, stream, p, blocks, groups, rows);
+    const int items = groups * wide * ((rows + 31) / 32) * (D / 16);
+    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) std::min(items, 4 * sms)), 128, 0, stream, p, wide, groups, rows);
 }
 
 template <int D, bool BF16>
@@ -1299,21 +1319,22 @@ bool tree_attn_tc_takes(const TreeAttnParams & p) {
         }
     }
     return (p.k.type == KV_F16 || p.k.type == KV_BF16) && (p.D == 64 || p.D == 128) && tensor_maps_available() &&
-           (int64_t) p.n_seq * p.n_head_kv * ((p.n_kv + TS_N - 1) / TS_N) < (1 << 30);
+           (int64_t) p.n_seq * p.n_head_kv * ((p.t.max_nodes * p.ratio + TS_M - 1) / TS_M) * ((p.n_kv + TS_N - 1) / TS_N + TS_COST) < (1 << 30);
 }
 
-int tree_attn_blocks(const TreeAttnParams & p) {
-    return (p.t.max_nodes * p.ratio + TS_M - 1) / TS_M;
+int tree_attn_wide(const TreeAttnParams & p) {
+    return p.t.n_nodes ? 1 : (p.t.max_nodes * p.ratio + TS_M - 1) / TS_M;
 }
 
 int tree_attn_groups(const TreeAttnParams & p, int sms) {
-    const int64_t tiles = (int64_t) p.n_seq * p.n_head_kv * ((p.n_kv + TS_N - 1) / TS_N);
-    return (int) std::max<int64_t>(1, std::min<int64_t>(sms / tree_attn_blocks(p), tiles));
+    const int64_t blocks = (p.t.max_nodes * p.ratio + TS_M - 1) / TS_M, wide = tree_attn_wide(p);
+    const int64_t tiles = (int64_t) p.n_seq * p.n_head_kv * ((p.n_kv + TS_N - 1) / TS_N) * (wide == 1 ? blocks : 1);
+    return (int) std::max<int64_t>(1, std::min<int64_t>(sms / wide, tiles));
 }
 
 size_t tree_attn_tc_workspace(const TreeAttnParams & p, int sms) {
-    const int blocks = tree_attn_blocks(p), rows = std::min(p.t.max_nodes * p.ratio, TS_M);
-    return KV8_WS_ZEROED + (size_t) tree_attn_groups(p, sms) * blocks * 2 * ts_slot_floats(rows, p.D) * 4;
+    const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
+    return KV8_WS_ZEROED + (size_t) tree_attn_groups(p, sms) * tree_attn_wide(p) * 2 * ts_slot_floats(rows, p.D) * 4;
 }
 
 cudaError_t launch_tree_attn_tc(TreeAttnParams p, int sms, cudaStream_t stream) {
