@@ -14,15 +14,20 @@
 // shared memory, in the order of the ranks, and every thread takes the same decisions from them.
 // The decisions come from F32 exponentials summed in F64; the last row's sums (and the M that lead to them) are taken in
 // F64 throughout, since the next token's place among 10^5 borders moves with the twelfth digit of a partial sum.
+//
+// Bound: HBM where there are many trees, else the passes of a walk, one after another (a row, and a rejection's sum): a slice
+// of up to 8 entries a thread is kept in registers between them.  F64 runs at half of F32's rate here, and exp2() is some
+// 40 instructions of it: with a table of 32 powers, one in each lane, and a polynomial it is 12.
 #include "tree.cuh"
 
 namespace mm3fa {
 
 namespace {
 
-constexpr int TV_THREADS = 1024;
+constexpr int TV_THREADS = 1024;  // of a CTA, at most
 constexpr int TV_WARPS   = TV_THREADS / 32;
-constexpr int TV_CHUNK   = 256;  // entries whose sum is kept: 8 for each lane of a warp
+constexpr int TV_RANKS   = 8;     // CTAs of a tree, at most
+constexpr int TV_CHUNK   = 256;   // entries whose sum is kept: 8 for each lane of a warp
 constexpr int TV_E       = TV_CHUNK / 32;
 
 struct TvShared {
@@ -90,6 +95,22 @@ __device__ __forceinline__ float clean_draft(float q) {
     return fmaxf(q, 0.0f);  // NaN: 0
 }
 
+// 2^y for -1000 < y <= 0, within 2e-16 + 1e-15: y = n + k / 32 + r with |r| <= 1/64, 2^(k / 32) from lane k (`power` of
+// each lane), 2^r by its series to the fifth power, n into the exponent.  By whole warps.
+__device__ __forceinline__ double exp2_near(double y, double power) {
+    const double magic = 0x1.8p+47;  // adding it rounds to a multiple of 1/32
+    const double t = y + magic, r = y - (t - magic);
+    const int    n = __double2loint(t);  // 32 n + k
+    const double pw = __shfl_sync(0xffffffffu, power, n & 31);
+    // ln(2)^i / i!
+    double s = fma(1.3333558146428443e-3, r, 9.618129107628477e-3);
+    s = fma(s, r, 5.550410866482158e-2);
+    s = fma(s, r, 2.4022650695910072e-1);
+    s = fma(s, r, 6.9314718055994531e-1);
+    s = fma(s, r, 1.0) * pw;
+    return __hiloint2double(__double2hiint(s) + ((n >> 5) << 20), __double2loint(s));
+}
+
 // LT, DT: types of logits and drafts (DT -1: fixed choices)
 template <int LT, int DT>
 struct Walk {
@@ -98,21 +119,33 @@ struct Walk {
     double *                 sums;  // of the CTA's chunks
     const char *             lrow;  // the current node's rows
     const char *             qrow;
-    int                      lo, hi, n_ranks;  // the CTA's slice
-    uint32_t                 rank;
-    int                      turn;
-    int                      tid, lane, warp;
+    int                      lo, hi, n_ranks, n_warps;  // the CTA's slice
+    int                      rank, turn, tid, lane, warp;
+    bool                     held;  // a chunk a warp at most: kept from pass to pass
+    double                   power;
+    float                    x[TV_E], q[DT >= 0 ? TV_E : 1];
 
-    __device__ __forceinline__ void sync() const {
-        if (n_ranks > 1) {
-            cluster_sync();
-        } else {
-            __syncthreads();
+    // the chunk from i0 on: its logits, and the drafts where they are asked for
+    __device__ __forceinline__ void load(int i0, bool drafts) {
+#pragma unroll
+        for (int e = 0; e < TV_E; e++) {
+            const int i = i0 + e * 32 + lane;
+            x[e]        = i < hi ? load1<LT>(lrow, i) : -INFINITY;
+            if (DT >= 0 && drafts) {
+                q[e] = i < hi ? load1<DT>(qrow, i) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < TV_E; e++) {
+            x[e] = clean_logit(x[e]);
+            if (DT >= 0 && drafts) {
+                q[e] = clean_draft(q[e]);
+            }
         }
     }
 
     // the sum of a value of every thread over the cluster, the same in every thread
-    __device__ double total(double a) {
+    __device__ __forceinline__ double total(double a) {
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) {
             a += __shfl_xor_sync(0xffffffffu, a, d);
@@ -122,38 +155,53 @@ struct Walk {
             sh.warp_a[warp] = a;
         }
         __syncthreads();
-        a = 0.0;
-#pragma unroll 8
-        for (int w = 0; w < TV_WARPS; w++) {
-            a += sh.warp_a[w];
+        a = lane < n_warps ? sh.warp_a[lane] : 0.0;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, d);
         }
         if (n_ranks > 1) {
             if (tid == 0) {
                 sh.rank_a[turn] = a;
             }
             cluster_sync();
-            a = 0.0;
-            for (int r = 0; r < n_ranks; r++) {
-                a += ld_rank_f64(&sh.rank_a[turn], r);
+            a = lane < n_ranks ? ld_rank_f64(&sh.rank_a[turn], lane) : 0.0;
+#pragma unroll
+            for (int d = TV_RANKS / 2; d > 0; d >>= 1) {
+                a += __shfl_xor_sync(0xffffffffu, a, d);
             }
+            a = __shfl_sync(0xffffffffu, a, 0);
             turn ^= 1;
         }
         return a;
     }
 
-    // (m, sum of 2^((x - m) / t)) over the row
-    __device__ void row_mass(float & m_out, double & z_out) {
+    // (m, sum of 2^((x - m) / t)) of each lane, joined over the warp
+    __device__ __forceinline__ void join(float & m, double & z) const {
         const float a = (float) p.inv_t;
-        float       m = -INFINITY, s = 0.0f;
-        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += TV_WARPS * TV_CHUNK) {
-            float x[TV_E], top = -INFINITY;
+        float       top = m;
 #pragma unroll
-            for (int e = 0; e < TV_E; e++) {
-                const int i = i0 + e * 32 + lane;
-                x[e]        = i < hi ? clean_logit(load1<LT>(lrow, i)) : -INFINITY;
-            }
+        for (int d = 16; d > 0; d >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        }
+        z = m > -INFINITY ? z * (double) exp2f((m - top) * a) : 0.0;
 #pragma unroll
-            for (int e = 0; e < TV_E; e++) {
+        for (int d = 16; d > 0; d >>= 1) {
+            z += __shfl_xor_sync(0xffffffffu, z, d);
+        }
+        m = top;
+    }
+
+    // (m, sum of 2^((x - m) / t)) over the row
+    __device__ __forceinline__ void row_mass(float & m, double & z) {
+        const float a = (float) p.inv_t;
+        float       s = 0.0f;
+        m = -INFINITY;
+        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
+            load(i0, held);
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < TV_E; e++) {
                 top = fmaxf(top, x[e]);
             }
             if (top > m) {
@@ -167,141 +215,127 @@ struct Walk {
                 }
             }
         }
-        float top = m;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        }
-        double z = m > -INFINITY ? (double) s * (double) exp2f((m - top) * a) : 0.0;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            z += __shfl_xor_sync(0xffffffffu, z, d);
-        }
+        z = (double) s;
+        join(m, z);
         __syncthreads();
         if (lane == 0) {
-            sh.warp_m[warp] = top, sh.warp_a[warp] = z;
+            sh.warp_m[warp] = m, sh.warp_a[warp] = z;
         }
         __syncthreads();
-        m = -INFINITY;
-#pragma unroll 8
-        for (int w = 0; w < TV_WARPS; w++) {
-            m = fmaxf(m, sh.warp_m[w]);
-        }
-        z = 0.0;
-#pragma unroll 8
-        for (int w = 0; w < TV_WARPS; w++) {
-            z += sh.warp_m[w] > -INFINITY ? sh.warp_a[w] * (double) exp2f((sh.warp_m[w] - m) * a) : 0.0;
-        }
+        m = lane < n_warps ? sh.warp_m[lane] : -INFINITY, z = lane < n_warps ? sh.warp_a[lane] : 0.0;
+        join(m, z);
         if (n_ranks > 1) {
             if (tid == 0) {
                 sh.rank_m[turn] = m, sh.rank_a[turn] = z;
             }
             cluster_sync();
-            m = -INFINITY;
-            for (int r = 0; r < n_ranks; r++) {
-                m = fmaxf(m, ld_rank_f32(&sh.rank_m[turn], r));
-            }
-            z = 0.0;
-            for (int r = 0; r < n_ranks; r++) {
-                const float mr = ld_rank_f32(&sh.rank_m[turn], r);
-                z += mr > -INFINITY ? ld_rank_f64(&sh.rank_a[turn], r) * (double) exp2f((mr - m) * a) : 0.0;
-            }
+            m = lane < n_ranks ? ld_rank_f32(&sh.rank_m[turn], lane) : -INFINITY, z = lane < n_ranks ? ld_rank_f64(&sh.rank_a[turn], lane) : 0.0;
+            join(m, z);
             turn ^= 1;
         }
-        m_out = m, z_out = z;
     }
 
     // the lowest index of the row's largest logit (-1: none is above -inf)
-    __device__ int row_argmax() {
+    __device__ __forceinline__ int row_argmax() {
         float m = -INFINITY;
         int   at = 0x7fffffff;
-        for (int i = lo + tid; i < hi; i += TV_THREADS) {
-            const float x = clean_logit(load1<LT>(lrow, i));
-            if (x > m) {
-                m = x, at = i;
+        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
+            load(i0, false);
+#pragma unroll
+            for (int e = 0; e < TV_E; e++) {
+                if (x[e] > m) {
+                    m = x[e], at = i0 + e * 32 + lane;
+                }
             }
         }
-        auto take = [&](float x, int i) {
-            if (x > m || (x == m && i < at)) {
-                m = x, at = i;
+        auto join = [&] {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) {
+                const float y = __shfl_xor_sync(0xffffffffu, m, d);
+                const int   i = __shfl_xor_sync(0xffffffffu, at, d);
+                if (y > m || (y == m && i < at)) {
+                    m = y, at = i;
+                }
             }
         };
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            const float x = __shfl_xor_sync(0xffffffffu, m, d);
-            take(x, __shfl_xor_sync(0xffffffffu, at, d));
-        }
+        join();
         __syncthreads();
         if (lane == 0) {
             sh.warp_m[warp] = m, sh.warp_i[warp] = at;
         }
         __syncthreads();
-        for (int w = 0; w < TV_WARPS; w++) {
-            take(sh.warp_m[w], sh.warp_i[w]);
-        }
+        m = lane < n_warps ? sh.warp_m[lane] : -INFINITY, at = lane < n_warps ? sh.warp_i[lane] : 0x7fffffff;
+        join();
         if (n_ranks > 1) {
             if (tid == 0) {
                 sh.rank_m[turn] = m, sh.rank_i[turn] = at;
             }
             cluster_sync();
-            for (int r = 0; r < n_ranks; r++) {
-                take(ld_rank_f32(&sh.rank_m[turn], r), ld_rank_i32(&sh.rank_i[turn], r));
-            }
+            m = lane < n_ranks ? ld_rank_f32(&sh.rank_m[turn], lane) : -INFINITY, at = lane < n_ranks ? ld_rank_i32(&sh.rank_i[turn], lane) : 0x7fffffff;
+            join();
             turn ^= 1;
         }
         return m > -INFINITY ? at : -1;
     }
 
     // sum of max(p - c q, 0), in F32 terms
-    __device__ double left_mass(float m, double z, double c) {
+    __device__ __forceinline__ double left_mass(float m, double z, double c) {
         const float a = (float) p.inv_t, iz = (float) (1.0 / z), cf = (float) c;
         double      sum = 0.0;
-        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += TV_WARPS * TV_CHUNK) {
-            float x[TV_E], q[TV_E], s = 0.0f;
-#pragma unroll
-            for (int e = 0; e < TV_E; e++) {
-                const int i = i0 + e * 32 + lane;
-                x[e]        = i < hi ? clean_logit(load1<LT>(lrow, i)) : -INFINITY;
-                q[e]        = i < hi ? clean_draft(load1<DT>(qrow, i)) : 0.0f;
+        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
+            if (!held) {
+                load(i0, true);
             }
+            float s = 0.0f;
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
-                s += fmaxf(exp2f((x[e] - m) * a) * iz - cf * q[e], 0.0f);
+                s += fmaxf(exp2f((x[e] - m) * a) * iz - cf * q[DT >= 0 ? e : 0], 0.0f);
             }
             sum += (double) s;
         }
         return total(sum);
     }
 
-    __device__ __forceinline__ double weight(float x, float m) const {
-        return exp2(((double) x - (double) m) * p.inv_t);
+    // 2^((v - m) / t); 0 where that is below 2^-1000.  By whole warps.
+    __device__ __forceinline__ double weight(float v, float m) const {
+        const bool   in = (v - m) * (float) p.inv_t > -1000.0f;
+        const double w  = exp2_near(((double) (in ? v : m) - (double) m) * p.inv_t, power);
+        return in ? w : 0.0;
     }
 
-    // what is left of entry i: max(p - c q, 0), or the weight of a token that was not rejected
-    __device__ __forceinline__ double left(int i, float m, double iz, double c, int n_gone) const {
-        double w = weight(clean_logit(load1<LT>(lrow, i)), m);
-        if constexpr (DT >= 0) {
-            return c > 0.0 ? fmax(w * iz - c * (double) clean_draft(load1<DT>(qrow, i)), 0.0) : w;
-        } else {
-            for (int k = 0; k < n_gone; k++) {
-                w = sh.gone[k] == i ? 0.0 : w;
+    // what is left of the chunk's entry e: max(p - c q, 0), or the weight of a token that was not rejected.  By whole warps.
+    __device__ __forceinline__ double left(int e, float m, double iz, double c) const {
+        const double w = weight(x[e], m);
+        return DT >= 0 && c > 0.0 ? fmax(w * iz - c * (double) q[DT >= 0 ? e : 0], 0.0) : w;
+    }
+
+    // the chunk from i0 on for `left`: the rejected tokens of fixed choices count as -inf
+    __device__ __forceinline__ void load_left(int i0, int n_gone) {
+        if (!held || DT < 0) {
+            load(i0, true);
+        }
+        for (int k = 0; DT < 0 && k < n_gone; k++) {
+            const int at = sh.gone[k] - i0;
+            if (at >= 0 && at < TV_CHUNK && (at & 31) == lane) {
+#pragma unroll
+                for (int e = 0; e < TV_E; e++) {
+                    x[e] = e == at >> 5 ? -INFINITY : x[e];
+                }
             }
-            return w;
         }
     }
 
     // sum of `left` over the row; the sums of the CTA's chunks are kept
-    __device__ double left_sums(float m, double iz, double c, int n_gone) {
+    __device__ __forceinline__ double left_sums(float m, double iz, double c, int n_gone) {
         double sum = 0.0;
         __syncthreads();
-        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += TV_WARPS * TV_CHUNK) {
+        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
+            load_left(i0, n_gone);
             double s = 0.0;
-#pragma unroll 4
+#pragma unroll
             for (int e = 0; e < TV_E; e++) {
-                const int i = i0 + e * 32 + lane;
-                s += i < hi ? left(i, m, iz, c, n_gone) : 0.0;
+                s += left(e, m, iz, c);
             }
-            sum += s;
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) {
                 s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -309,13 +343,23 @@ struct Walk {
             if (lane == 0) {
                 sums[(i0 - lo) / TV_CHUNK] = s;
             }
+            sum += lane == 0 ? s : 0.0;
         }
         return total(sum);
     }
 
+    __device__ __forceinline__ double prefix(double s) const {  // over the lanes up to this one
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, s, d);
+            s += lane >= d ? y : 0.0;
+        }
+        return s;
+    }
+
     // the first entry at which the sum of what is left exceeds u times all of it, by the CTA that holds it; the chunks'
     // sums of the last left_sums() are in place
-    __device__ void sample(float u, float m, double iz, double c, int n_gone, int * out) {
+    __device__ __forceinline__ void sample(float u, float m, double iz, double c, int n_gone, int * out) {
         const int n_chunks = hi > lo ? (hi - lo + TV_CHUNK - 1) / TV_CHUNK : 0;
         // this CTA's sum, and the ranks' before it, from the same numbers in the same order everywhere
         __syncthreads();
@@ -332,95 +376,69 @@ struct Walk {
         if (tid == 0) {
             sh.rank_a[turn] = mine;
         }
-        sync();
-        if (warp == 0) {
-            double all = 0.0, before = 0.0;
-            int    last = -1, owner = -1;
-            for (int r = 0; r < n_ranks; r++) {
-                all += ld_rank_f64(&sh.rank_a[turn], r);
-            }
-            const double target = (double) fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f) * all;
-            double       run = 0.0;
-            for (int r = 0; r < n_ranks; r++) {
-                const double x = ld_rank_f64(&sh.rank_a[turn], r);
-                if (x > 0.0) {
-                    last = r;
-                    if (owner < 0 && run + x > target) {
-                        owner = r, before = run;
-                    }
-                }
-                run += x;
-            }
-            if (owner < 0) {  // (cannot be: the sums of ranks end at `all`, which is above the target)
-                owner = last, before = -INFINITY;
-            }
-            if (owner == (int) rank) {
-                // the chunk, then the entry: a warp's prefix sums over the rest that is in the way
-                int    chunk = -1;
-                double start = before;
-                for (int k0 = 0; k0 < n_chunks && chunk < 0; k0 += 32) {
-                    const double x = k0 + lane < n_chunks ? sums[k0 + lane] : 0.0;
-                    double       s = x;
-#pragma unroll
-                    for (int d = 1; d < 32; d <<= 1) {
-                        const double y = __shfl_up_sync(0xffffffffu, s, d);
-                        s += lane >= d ? y : 0.0;
-                    }
-                    const unsigned over = __ballot_sync(0xffffffffu, x > 0.0 && start + s > target);
-                    if (over) {
-                        const int k = __ffs(over) - 1;
-                        chunk       = k0 + k;
-                        start += __shfl_sync(0xffffffffu, s - x, k);
-                    } else {
-                        start += __shfl_sync(0xffffffffu, s, 31);
-                    }
-                }
-                if (chunk < 0) {  // roundings between two orders of summing: the last entry that holds anything
-                    for (int k = 0; k < n_chunks; k++) {
-                        chunk = sums[k] > 0.0 ? k : chunk;
-                    }
-                    start = -INFINITY;
-                }
-                int token = -1, backup = -1;
-                for (int e = 0; e < TV_E && token < 0; e++) {
-                    const int    i = lo + chunk * TV_CHUNK + e * 32 + lane;
-                    const double x = i < hi ? left(i, m, iz, c, n_gone) : 0.0;
-                    double       s = x;
-#pragma unroll
-                    for (int d = 1; d < 32; d <<= 1) {
-                        const double y = __shfl_up_sync(0xffffffffu, s, d);
-                        s += lane >= d ? y : 0.0;
-                    }
-                    const unsigned over = __ballot_sync(0xffffffffu, x > 0.0 && start + s > target);
-                    const unsigned some = __ballot_sync(0xffffffffu, x > 0.0);
-                    if (over) {
-                        token = lo + chunk * TV_CHUNK + e * 32 + __ffs(over) - 1;
-                    }
-                    backup = some ? lo + chunk * TV_CHUNK + e * 32 + 31 - __clz(some) : backup;
-                    start += __shfl_sync(0xffffffffu, s, 31);
-                }
-                if (lane == 0) {
-                    *out = token >= 0 ? token : backup;
-                }
+        if (n_ranks > 1) {
+            cluster_sync();
+        } else {
+            __syncthreads();
+        }
+        if (warp != 0) {
+            return;
+        }
+        const double r = lane < n_ranks ? ld_rank_f64(&sh.rank_a[turn], lane) : 0.0, upto = prefix(r), all = __shfl_sync(0xffffffffu, upto, 31);
+        const double target = (double) fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f) * all;
+        const unsigned has = __ballot_sync(0xffffffffu, r > 0.0), past = __ballot_sync(0xffffffffu, r > 0.0 && upto > target);
+        // (a rounding could leave the target at the very end: the last that holds anything)
+        const int owner = past ? __ffs(past) - 1 : 31 - __clz(has);
+        if (has == 0 || owner != rank) {
+            return;
+        }
+        double start = past ? __shfl_sync(0xffffffffu, upto - r, owner) : -INFINITY;
+        int    chunk = -1, last = 0;
+        for (int k0 = 0; k0 < n_chunks && chunk < 0; k0 += 32) {
+            const double   v = k0 + lane < n_chunks ? sums[k0 + lane] : 0.0, s = prefix(v);
+            const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && start + s > target), some = __ballot_sync(0xffffffffu, v > 0.0);
+            last = some ? k0 + 31 - __clz(some) : last;
+            if (over) {
+                chunk = k0 + __ffs(over) - 1;
+                start += __shfl_sync(0xffffffffu, s - v, __ffs(over) - 1);
+            } else {
+                start += __shfl_sync(0xffffffffu, s, 31);
             }
         }
-        turn ^= 1;
+        if (chunk < 0) {
+            chunk = last, start = -INFINITY;
+        }
+        const int i0 = lo + chunk * TV_CHUNK;
+        held         = false;  // (the chunk need not be this warp's)
+        load_left(i0, n_gone);
+        int token = -1, backup = 0;
+#pragma unroll
+        for (int e = 0; e < TV_E; e++) {
+            const double   v = left(e, m, iz, c), s = prefix(v);
+            const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && start + s > target), some = __ballot_sync(0xffffffffu, v > 0.0);
+            token  = token < 0 && over ? i0 + e * 32 + __ffs(over) - 1 : token;
+            backup = some ? i0 + e * 32 + 31 - __clz(some) : backup;
+            start += __shfl_sync(0xffffffffu, s, 31);
+        }
+        if (lane == 0) {
+            *out = token >= 0 ? token : backup;
+        }
     }
 };
 
 template <int LT, int DT>
-__global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVerifyParams p, int n_ranks) {
+__global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVerifyParams p, int n_ranks, int ahead) {
     kv8_dep_wait();
     extern __shared__ double tv_sums[];
     __shared__ TvShared      sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, T = p.t.max_nodes;
     const int tree = (int) blockIdx.x / n_ranks;
-    const uint32_t rank = n_ranks > 1 ? cluster_rank() : 0;
+    const int rank = n_ranks > 1 ? (int) cluster_rank() : 0;
     const int n    = tree_nodes(p.t, tree);
     int * path     = p.path + (int64_t) tree * T;
     if (n == 0) {
         if (rank == 0) {
-            for (int i = tid; i < T; i += TV_THREADS) {
+            for (int i = tid; i < T; i += (int) blockDim.x) {
                 path[i] = -1;
             }
             if (tid == 0) {
@@ -430,7 +448,7 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
         return;
     }
     const char * lbase = p.logits.data + (int64_t) tree * p.logits.nb2, *qbase = DT >= 0 ? p.draft.data + (int64_t) tree * p.draft.nb2 : nullptr;
-    for (int i = tid; i < n; i += TV_THREADS) {
+    for (int i = tid; i < n; i += (int) blockDim.x) {
         const int pr = tree_parent(p.t, tree, i), x = p.tokens[(int64_t) tree * T + i];
         const bool ok = i > 0 && pr >= 0 && x >= 0 && x < p.V;  // a token outside the vocabulary is never accepted
         sh.par[i] = ok ? pr : -1, sh.tok[i] = x, sh.u[i] = p.accept[(int64_t) tree * T + i];
@@ -440,22 +458,21 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
             sh.qx[i] = ok ? clean_draft(load1<DT>(qbase + (int64_t) pr * p.draft.nb1, x)) : 0.0f;
         }
     }
+    if (tid == 0) {
+        sh.path[0] = 0;
+    }  // (a row's pass has barriers before any of these are read)
     // slices of whole chunks
-    const int chunks = (p.V + TV_CHUNK - 1) / TV_CHUNK, each = (chunks + n_ranks - 1) / n_ranks;
-    Walk<LT, DT> w{ p, sh, tv_sums, lbase, qbase, 0, 0, n_ranks, rank, 0, tid, lane, warp };
-    w.lo = min((int) rank * each * TV_CHUNK, p.V), w.hi = min(((int) rank + 1) * each * TV_CHUNK, p.V);
-    __syncthreads();
+    const int chunks = (p.V + TV_CHUNK - 1) / TV_CHUNK, each = (chunks + n_ranks - 1) / n_ranks, n_warps = (int) blockDim.x / 32;
+    Walk<LT, DT> w{ p, sh, tv_sums, lbase, qbase, min(rank * each * TV_CHUNK, p.V), min((rank + 1) * each * TV_CHUNK, p.V), n_ranks, n_warps, rank, 0, tid, lane, warp,
+                    each <= n_warps, exp2((double) lane / 32.0) };
     int    cur = 0, n_path = 1, n_gone, n_no, best = -1;
     float  m = 0.0f;
     double z = 0.0;
-    if (tid == 0) {
-        sh.path[0] = 0;
-    }
+    const bool greedy = p.inv_t == 0.0;
     for (;;) {
         w.lrow = lbase + (int64_t) cur * p.logits.nb1;
         w.qrow = DT >= 0 ? qbase + (int64_t) cur * p.draft.nb1 : nullptr;
         n_gone = n_no = 0;
-        const bool greedy = p.inv_t == 0.0;
         if (greedy) {
             best = w.row_argmax();
         } else {
@@ -464,6 +481,7 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
         }
         int    next = -1;
         double c = 0.0, M = 1.0;
+        bool   first = true;
         for (int k0 = cur / 32 * 32; best >= 0 && next < 0 && k0 < n; k0 += 32) {
             unsigned kids = __ballot_sync(0xffffffffu, k0 + lane < n && k0 + lane > cur && sh.par[min(k0 + lane, TREE_MAX - 1)] == cur);
             while (kids && next < 0) {
@@ -472,6 +490,15 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
                 if (greedy) {
                     next = sh.tok[i] == best ? i : -1;
                     continue;
+                }
+                if (ahead && first) {
+                    // (few trees: the likeliest next row comes nearer while this one is decided on)
+                    const char * row = lbase + (int64_t) i * p.logits.nb1;
+                    constexpr int esz = LT == KV_F32 ? 4 : 2;
+                    for (int64_t b = (int64_t) w.lo * esz + tid * 128; b < (int64_t) w.hi * esz; b += (int64_t) blockDim.x * 128) {
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(row + b));
+                    }
+                    first = false;
                 }
                 const double px = w.weight(sh.lx[i], m) / z, q = (double) sh.qx[i];
                 double       r  = fmax(px - c * q, 0.0);
@@ -507,18 +534,20 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
         }
         n_path++;
     }
-    if (p.inv_t != 0.0 && best >= 0) {
-        double iz = 1.0, c = 0.0;
-        if (DT >= 0 && n_no > 0) {
-            iz = 1.0 / w.left_sums(m, 1.0, 0.0, 0);
-            c  = 1.0;
-            for (int k = 1; k < n_no; k++) {
-                c += w.left_sums(m, iz, c, 0);
+    if (!greedy && best >= 0) {
+        // the F64 sums: with drafts Z and the M again, then what is left; the target's own distribution, where nothing is
+        const int last = DT >= 0 ? n_no : 0;
+        double    iz = 1.0, c = 0.0;
+        for (int k = 0;; k++) {
+            const double sum = w.left_sums(m, iz, c, n_gone);
+            if (k < last) {
+                iz = k == 0 ? 1.0 / sum : iz;
+                c += k == 0 ? 1.0 : sum;
+            } else if (sum > 0.0 || (c == 0.0 && n_gone == 0)) {
+                break;
+            } else {
+                c = 0.0, n_gone = 0;
             }
-        }
-        if (!(w.left_sums(m, iz, c, n_gone) > 0.0)) {  // nothing is left: the target's own distribution
-            c = 0.0, n_gone = 0;
-            w.left_sums(m, iz, c, n_gone);
         }
         w.sample(p.sample[tree], m, iz, c, n_gone, p.token + tree);
     } else if (rank == 0 && tid == 0) {
@@ -526,7 +555,7 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
     }
     __syncthreads();
     if (rank == 0) {
-        for (int i = tid; i < T; i += TV_THREADS) {
+        for (int i = tid; i < T; i += (int) blockDim.x) {
             path[i] = i < n_path ? sh.path[i] : -1;
         }
         if (tid == 0) {
@@ -539,19 +568,31 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
 }
 
 template <int LT, int DT>
-cudaError_t launch_one(const TreeVerifyParams & p, int n_ranks, cudaStream_t stream) {
+cudaError_t launch_one(const TreeVerifyParams & p, int sms, cudaStream_t stream) {
     static Kv8Once once;
-    const int      chunks = (p.V + TV_CHUNK - 1) / TV_CHUNK;
-    const size_t   smem   = (size_t) ((chunks + n_ranks - 1) / n_ranks) * sizeof(double);
-    cudaError_t    e      = once.smem(tree_verify_kernel<LT, DT>, 160 << 10);
+    cudaError_t    e = once.smem(tree_verify_kernel<LT, DT>, 160 << 10);
     if (e != cudaSuccess) {
         return e;
     }
+    // CTAs of a tree: up to 8 (the portable size), 8 chunks each or more.  Their threads: a warp for each chunk, up to what
+    // lets all trees run at once at 1024 threads an SM (64 registers each), but 8 warps at least
+    const int chunks  = (p.V + TV_CHUNK - 1) / TV_CHUNK;
+    int       n_ranks = 1;
+    while (n_ranks < TV_RANKS && chunks >= 16 * n_ranks) {
+        n_ranks *= 2;
+    }
+    const int     each = (chunks + n_ranks - 1) / n_ranks;
+    const int64_t room = (int64_t) TV_WARPS * sms / ((int64_t) p.t.n_tree * n_ranks);
+    int           n_warps = 8;
+    while (n_warps < TV_WARPS && n_warps < each && 2 * n_warps <= room) {
+        n_warps *= 2;
+    }
+    const bool          ahead = (int64_t) p.t.n_tree * n_ranks <= sms;
     cudaLaunchConfig_t  cfg{};
     cudaLaunchAttribute attr[2];
     cfg.gridDim          = dim3((unsigned) (p.t.n_tree * n_ranks));
-    cfg.blockDim         = dim3(TV_THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim         = dim3((unsigned) (32 * n_warps));
+    cfg.dynamicSmemBytes = (size_t) each * sizeof(double);
     cfg.stream           = stream;
     cfg.attrs            = attr;
     cfg.numAttrs         = 0;
@@ -567,39 +608,34 @@ cudaError_t launch_one(const TreeVerifyParams & p, int n_ranks, cudaStream_t str
         attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs++;
     }
-    return cudaLaunchKernelEx(&cfg, tree_verify_kernel<LT, DT>, p, n_ranks);
+    return cudaLaunchKernelEx(&cfg, tree_verify_kernel<LT, DT>, p, n_ranks, ahead ? 1 : 0);
 }
 
 template <int LT>
-cudaError_t launch_l(const TreeVerifyParams & p, int n_ranks, cudaStream_t stream) {
+cudaError_t launch_l(const TreeVerifyParams & p, int sms, cudaStream_t stream) {
     if (!p.draft.data) {
-        return launch_one<LT, -1>(p, n_ranks, stream);
+        return launch_one<LT, -1>(p, sms, stream);
     }
     switch (p.draft.type) {
         case KV_F32:
-            return launch_one<LT, KV_F32>(p, n_ranks, stream);
+            return launch_one<LT, KV_F32>(p, sms, stream);
         case KV_F16:
-            return launch_one<LT, KV_F16>(p, n_ranks, stream);
+            return launch_one<LT, KV_F16>(p, sms, stream);
         default:
-            return launch_one<LT, KV_BF16>(p, n_ranks, stream);
+            return launch_one<LT, KV_BF16>(p, sms, stream);
     }
 }
 
 }  // namespace
 
 cudaError_t launch_tree_verify(const TreeVerifyParams & p, int sms, cudaStream_t stream) {
-    // CTAs of a tree: as many as the SMs give each tree, up to 8 (the portable size), with two chunks a warp or more
-    int n_ranks = 1;
-    while (n_ranks < 8 && 2 * n_ranks * p.t.n_tree <= sms && p.V >= 2 * n_ranks * TV_WARPS * TV_CHUNK / 4) {
-        n_ranks *= 2;
-    }
     switch (p.logits.type) {
         case KV_F32:
-            return launch_l<KV_F32>(p, n_ranks, stream);
+            return launch_l<KV_F32>(p, sms, stream);
         case KV_F16:
-            return launch_l<KV_F16>(p, n_ranks, stream);
+            return launch_l<KV_F16>(p, sms, stream);
         default:
-            return launch_l<KV_BF16>(p, n_ranks, stream);
+            return launch_l<KV_BF16>(p, sms, stream);
     }
 }
 
