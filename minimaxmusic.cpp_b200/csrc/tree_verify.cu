@@ -86,30 +86,40 @@ __device__ __forceinline__ float load1(const char * row, int64_t i) {
     return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(row)[i]);
 }
 
+// 2^y on the special-function unit, 0 below 2^-126
+__device__ __forceinline__ float power2(float y) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+    return r;
+}
+
 // A logit as the sums take it: NaN counts as -inf, +inf as the largest number.
 __device__ __forceinline__ float clean_logit(float x) {
-    return x != x ? -INFINITY : fminf(x, 3.402823466e38f);
+    return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);  // (the maximum of NaN and a number is the number)
 }
 
 __device__ __forceinline__ float clean_draft(float q) {
     return fmaxf(q, 0.0f);  // NaN: 0
 }
 
-// 2^y for -1000 < y <= 0, within 2e-16 + 1e-15: y = n + k / 32 + r with |r| <= 1/64, 2^(k / 32) from lane k (`power` of
-// each lane), 2^r by its series to the fifth power, n into the exponent.  By whole warps.
-__device__ __forceinline__ double exp2_near(double y, double power) {
-    const double magic = 0x1.8p+47;  // adding it rounds to a multiple of 1/32
-    const double t = y + magic, r = y - (t - magic);
-    const int    n = __double2loint(t);  // 32 n + k
+// sum + 2^(x t + c) for exponents from -1000 to 0, to 12 digits: the exponent is n + k / 32 + r with |r| <= 1/64; 2^(k / 32)
+// comes from lane k (`power` of each lane), n goes into its exponent, and 2^r is its series to the fourth power.  By whole
+// warps; 9 instructions of F64.
+__device__ __forceinline__ double add_power(double x, double t, double c, double power, double sum) {
+    const double magic = 0x1.8p+47;  // a number this large is a multiple of 1/32
+    const double y = fma(x, t, c) + magic, r = fma(x, t, c - (y - magic));
+    const int    n = __double2loint(y);  // 32 n + k
     const double pw = __shfl_sync(0xffffffffu, power, n & 31);
     // ln(2)^i / i!
-    double s = fma(1.3333558146428443e-3, r, 9.618129107628477e-3);
-    s = fma(s, r, 5.550410866482158e-2);
+    double s = fma(9.618129107628477e-3, r, 5.550410866482158e-2);
     s = fma(s, r, 2.4022650695910072e-1);
     s = fma(s, r, 6.9314718055994531e-1);
-    s = fma(s, r, 1.0) * pw;
-    return __hiloint2double(__double2hiint(s) + ((n >> 5) << 20), __double2loint(s));
+    s = fma(s, r, 1.0);
+    return fma(s, __hiloint2double(__double2hiint(pw) + ((n >> 5) << 20), __double2loint(pw)), sum);
 }
+
+// Sums of weights below this are none: an entry of -inf counts as 2^-800 of the largest.
+constexpr double TV_NONE = 0x1p-600;
 
 // LT, DT: types of logits and drafts (DT -1: fixed choices)
 template <int LT, int DT>
@@ -123,24 +133,49 @@ struct Walk {
     int                      rank, turn, tid, lane, warp;
     bool                     held;  // a chunk a warp at most: kept from pass to pass
     double                   power;
+    bool                     coarse;  // logits so large that only the largest has a weight: that of `only`, taken as 0
+    float                    only;
     float                    x[TV_E], q[DT >= 0 ? TV_E : 1];
 
     // the chunk from i0 on: its logits, and the drafts where they are asked for
     __device__ __forceinline__ void load(int i0, bool drafts) {
+        if (i0 + TV_CHUNK <= hi) {
+            const char * at = lrow + (int64_t) (i0 + lane) * (LT == KV_F32 ? 4 : 2);
 #pragma unroll
-        for (int e = 0; e < TV_E; e++) {
-            const int i = i0 + e * 32 + lane;
-            x[e]        = i < hi ? load1<LT>(lrow, i) : -INFINITY;
+            for (int e = 0; e < TV_E; e++) {
+                x[e] = load1<LT>(at, e * 32);
+            }
             if (DT >= 0 && drafts) {
-                q[e] = i < hi ? load1<DT>(qrow, i) : 0.0f;
+                const char * qt = qrow + (int64_t) (i0 + lane) * (DT == KV_F32 ? 4 : 2);
+#pragma unroll
+                for (int e = 0; e < TV_E; e++) {
+                    q[DT >= 0 ? e : 0] = load1<DT>(qt, e * 32);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < TV_E; e++) {
+                const int i = i0 + e * 32 + lane;
+                x[e]        = i < hi ? load1<LT>(lrow, i) : -INFINITY;
+                if (DT >= 0 && drafts) {
+                    q[DT >= 0 ? e : 0] = i < hi ? load1<DT>(qrow, i) : 0.0f;
+                }
             }
         }
 #pragma unroll
         for (int e = 0; e < TV_E; e++) {
             x[e] = clean_logit(x[e]);
             if (DT >= 0 && drafts) {
-                q[e] = clean_draft(q[e]);
+                q[DT >= 0 ? e : 0] = clean_draft(q[DT >= 0 ? e : 0]);
             }
+        }
+    }
+
+    // brings the slice's part of a row to L2: the passes then wait for L2 only, a few thousand bytes at a time
+    __device__ __forceinline__ void fetch(const char * row, int esz) const {
+        const uint64_t from = (reinterpret_cast<uint64_t>(row) + (uint64_t) lo * esz + 15) & ~15ull, to = (reinterpret_cast<uint64_t>(row) + (uint64_t) hi * esz) & ~15ull;
+        if (tid == 0 && from < to) {
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"((uint32_t) (to - from)) : "memory");
         }
     }
 
@@ -184,7 +219,7 @@ struct Walk {
         for (int d = 16; d > 0; d >>= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         }
-        z = m > -INFINITY ? z * (double) exp2f((m - top) * a) : 0.0;
+        z = m > -INFINITY ? z * (double) power2((m - top) * a) : 0.0;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) {
             z += __shfl_xor_sync(0xffffffffu, z, d);
@@ -205,13 +240,13 @@ struct Walk {
                 top = fmaxf(top, x[e]);
             }
             if (top > m) {
-                s *= exp2f((m - top) * a);
+                s *= power2((m - top) * a);
                 m = top;
             }
             if (m > -INFINITY) {
 #pragma unroll
                 for (int e = 0; e < TV_E; e++) {
-                    s += exp2f((x[e] - m) * a);
+                    s += power2((x[e] - m) * a);
                 }
             }
         }
@@ -289,17 +324,17 @@ struct Walk {
             float s = 0.0f;
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
-                s += fmaxf(exp2f((x[e] - m) * a) * iz - cf * q[DT >= 0 ? e : 0], 0.0f);
+                s += fmaxf(power2((x[e] - m) * a) * iz - cf * q[DT >= 0 ? e : 0], 0.0f);
             }
             sum += (double) s;
         }
         return total(sum);
     }
 
-    // 2^((v - m) / t); 0 where that is below 2^-1000.  By whole warps.
+    // 2^((v - m) / t), 0 where that is below 2^-800.  By whole warps.
     __device__ __forceinline__ double weight(float v, float m) const {
-        const bool   in = (v - m) * (float) p.inv_t > -1000.0f;
-        const double w  = exp2_near(((double) (in ? v : m) - (double) m) * p.inv_t, power);
+        const bool in = (v - m) * (float) p.inv_t > -800.0f;
+        const double w  = add_power((double) (in ? v : m) - (double) m, p.inv_t, 0.0, power, 0.0);
         return in ? w : 0.0;
     }
 
@@ -311,8 +346,14 @@ struct Walk {
 
     // the chunk from i0 on for `left`: the rejected tokens of fixed choices count as -inf
     __device__ __forceinline__ void load_left(int i0, int n_gone) {
-        if (!held || DT < 0) {
+        if (!held || DT < 0 || coarse) {
             load(i0, true);
+        }
+        if (coarse) {
+#pragma unroll
+            for (int e = 0; e < TV_E; e++) {
+                x[e] = x[e] == only ? 0.0f : -INFINITY;
+            }
         }
         for (int k = 0; DT < 0 && k < n_gone; k++) {
             const int at = sh.gone[k] - i0;
@@ -327,14 +368,22 @@ struct Walk {
 
     // sum of `left` over the row; the sums of the CTA's chunks are kept
     __device__ __forceinline__ double left_sums(float m, double iz, double c, int n_gone) {
-        double sum = 0.0;
+        const double shift = -(double) m * p.inv_t;
+        const float  floor = m - 800.0f / (float) p.inv_t;  // (F32 is 128 / t coarse there at most)
+        double       sum   = 0.0;
         __syncthreads();
         for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
             load_left(i0, n_gone);
             double s = 0.0;
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
-                s += left(e, m, iz, c);
+                const double v = (double) fmaxf(x[e], floor);
+                if (DT < 0) {
+                    s = add_power(v, p.inv_t, shift, power, s);
+                } else {
+                    const double w = add_power(v, p.inv_t, shift, power, 0.0);
+                    s += c > 0.0 ? fmax(w * iz - c * (double) q[DT >= 0 ? e : 0], 0.0) : w;
+                }
             }
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) {
@@ -386,7 +435,7 @@ struct Walk {
         }
         const double r = lane < n_ranks ? ld_rank_f64(&sh.rank_a[turn], lane) : 0.0, upto = prefix(r), all = __shfl_sync(0xffffffffu, upto, 31);
         const double target = (double) fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f) * all;
-        const unsigned has = __ballot_sync(0xffffffffu, r > 0.0), past = __ballot_sync(0xffffffffu, r > 0.0 && upto > target);
+        const unsigned has = __ballot_sync(0xffffffffu, r > TV_NONE), past = __ballot_sync(0xffffffffu, r > TV_NONE && upto > target);
         // (a rounding could leave the target at the very end: the last that holds anything)
         const int owner = past ? __ffs(past) - 1 : 31 - __clz(has);
         if (has == 0 || owner != rank) {
@@ -396,7 +445,7 @@ struct Walk {
         int    chunk = -1, last = 0;
         for (int k0 = 0; k0 < n_chunks && chunk < 0; k0 += 32) {
             const double   v = k0 + lane < n_chunks ? sums[k0 + lane] : 0.0, s = prefix(v);
-            const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && start + s > target), some = __ballot_sync(0xffffffffu, v > 0.0);
+            const unsigned over = __ballot_sync(0xffffffffu, v > TV_NONE && start + s > target), some = __ballot_sync(0xffffffffu, v > TV_NONE);
             last = some ? k0 + 31 - __clz(some) : last;
             if (over) {
                 chunk = k0 + __ffs(over) - 1;
@@ -415,7 +464,7 @@ struct Walk {
 #pragma unroll
         for (int e = 0; e < TV_E; e++) {
             const double   v = left(e, m, iz, c), s = prefix(v);
-            const unsigned over = __ballot_sync(0xffffffffu, v > 0.0 && start + s > target), some = __ballot_sync(0xffffffffu, v > 0.0);
+            const unsigned over = __ballot_sync(0xffffffffu, v > TV_NONE && start + s > target), some = __ballot_sync(0xffffffffu, v > TV_NONE);
             token  = token < 0 && over ? i0 + e * 32 + __ffs(over) - 1 : token;
             backup = some ? i0 + e * 32 + 31 - __clz(some) : backup;
             start += __shfl_sync(0xffffffffu, s, 31);
@@ -464,15 +513,19 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
     // slices of whole chunks
     const int chunks = (p.V + TV_CHUNK - 1) / TV_CHUNK, each = (chunks + n_ranks - 1) / n_ranks, n_warps = (int) blockDim.x / 32;
     Walk<LT, DT> w{ p, sh, tv_sums, lbase, qbase, min(rank * each * TV_CHUNK, p.V), min((rank + 1) * each * TV_CHUNK, p.V), n_ranks, n_warps, rank, 0, tid, lane, warp,
-                    each <= n_warps, exp2((double) lane / 32.0) };
+                    each <= n_warps, exp2((double) lane / 32.0), false, 0.0f };
     int    cur = 0, n_path = 1, n_gone, n_no, best = -1;
     float  m = 0.0f;
     double z = 0.0;
     const bool greedy = p.inv_t == 0.0;
+    constexpr int ESZ = LT == KV_F32 ? 4 : 2;
     for (;;) {
         w.lrow = lbase + (int64_t) cur * p.logits.nb1;
         w.qrow = DT >= 0 ? qbase + (int64_t) cur * p.draft.nb1 : nullptr;
         n_gone = n_no = 0;
+        if (!w.held) {
+            w.fetch(w.lrow, ESZ);
+        }
         if (greedy) {
             best = w.row_argmax();
         } else {
@@ -493,11 +546,7 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
                 }
                 if (ahead && first) {
                     // (few trees: the likeliest next row comes nearer while this one is decided on)
-                    const char * row = lbase + (int64_t) i * p.logits.nb1;
-                    constexpr int esz = LT == KV_F32 ? 4 : 2;
-                    for (int64_t b = (int64_t) w.lo * esz + tid * 128; b < (int64_t) w.hi * esz; b += (int64_t) blockDim.x * 128) {
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(row + b));
-                    }
+                    w.fetch(lbase + (int64_t) i * p.logits.nb1, ESZ);
                     first = false;
                 }
                 const double px = w.weight(sh.lx[i], m) / z, q = (double) sh.qx[i];
@@ -537,13 +586,16 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
     if (!greedy && best >= 0) {
         // the F64 sums: with drafts Z and the M again, then what is left; the target's own distribution, where nothing is
         const int last = DT >= 0 ? n_no : 0;
+        if (fabsf(m) * (float) p.inv_t > 0x1p30f) {
+            w.coarse = true, w.only = m, m = 0.0f;
+        }
         double    iz = 1.0, c = 0.0;
         for (int k = 0;; k++) {
             const double sum = w.left_sums(m, iz, c, n_gone);
             if (k < last) {
                 iz = k == 0 ? 1.0 / sum : iz;
                 c += k == 0 ? 1.0 : sum;
-            } else if (sum > 0.0 || (c == 0.0 && n_gone == 0)) {
+            } else if (sum > TV_NONE || (c == 0.0 && n_gone == 0)) {
                 break;
             } else {
                 c = 0.0, n_gone = 0;
@@ -582,7 +634,7 @@ cudaError_t launch_one(const TreeVerifyParams & p, int sms, cudaStream_t stream)
         n_ranks *= 2;
     }
     const int     each = (chunks + n_ranks - 1) / n_ranks;
-    const int64_t room = (int64_t) TV_WARPS * sms / ((int64_t) p.t.n_tree * n_ranks);
+    const int64_t room = (int64_t) TV_WARPS * (sms * 7 / 8) / ((int64_t) p.t.n_tree * n_ranks);  // (clusters do not fill the last SMs of a GPC)
     int           n_warps = 8;
     while (n_warps < TV_WARPS && n_warps < each && 2 * n_warps <= room) {
         n_warps *= 2;
