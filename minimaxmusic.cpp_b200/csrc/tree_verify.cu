@@ -137,38 +137,48 @@ struct Walk {
     float                    only;
     float                    x[TV_E], q[DT >= 0 ? TV_E : 1];
 
-    // the chunk from i0 on: its logits, and the drafts where they are asked for
-    __device__ __forceinline__ void load(int i0, bool drafts) {
+    // the chunk from i0 on
+    __device__ __forceinline__ void load(float (&v)[TV_E], int i0) const {
         if (i0 + TV_CHUNK <= hi) {
             const char * at = lrow + (int64_t) (i0 + lane) * (LT == KV_F32 ? 4 : 2);
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
-                x[e] = load1<LT>(at, e * 32);
-            }
-            if (DT >= 0 && drafts) {
-                const char * qt = qrow + (int64_t) (i0 + lane) * (DT == KV_F32 ? 4 : 2);
-#pragma unroll
-                for (int e = 0; e < TV_E; e++) {
-                    q[DT >= 0 ? e : 0] = load1<DT>(qt, e * 32);
-                }
+                v[e] = load1<LT>(at, e * 32);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
                 const int i = i0 + e * 32 + lane;
-                x[e]        = i < hi ? load1<LT>(lrow, i) : -INFINITY;
-                if (DT >= 0 && drafts) {
-                    q[DT >= 0 ? e : 0] = i < hi ? load1<DT>(qrow, i) : 0.0f;
-                }
+                v[e]        = i < hi ? load1<LT>(lrow, i) : -INFINITY;
             }
         }
+    }
+
+    static __device__ __forceinline__ void clean(float (&v)[TV_E]) {
 #pragma unroll
         for (int e = 0; e < TV_E; e++) {
-            x[e] = clean_logit(x[e]);
-            if (DT >= 0 && drafts) {
-                q[DT >= 0 ? e : 0] = clean_draft(q[DT >= 0 ? e : 0]);
+            v[e] = clean_logit(v[e]);
+        }
+    }
+
+    __device__ __forceinline__ void load_drafts(int i0) {
+        if constexpr (DT >= 0) {
+#pragma unroll
+            for (int e = 0; e < TV_E; e++) {
+                const int i = i0 + e * 32 + lane;
+                q[e]        = i < hi ? load1<DT>(qrow, i) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < TV_E; e++) {
+                q[e] = clean_draft(q[e]);
             }
         }
+    }
+
+    __device__ __forceinline__ void load_both(int i0) {
+        load(x, i0);
+        load_drafts(i0);
+        clean(x);
     }
 
     // brings the slice's part of a row to L2: the passes then wait for L2 only, a few thousand bytes at a time
@@ -232,12 +242,11 @@ struct Walk {
         const float a = (float) p.inv_t;
         float       s = 0.0f;
         m = -INFINITY;
-        for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
-            load(i0, held);
-            float top = x[0];
+        auto add = [&](const float (&v)[TV_E]) {
+            float top = v[0];
 #pragma unroll
             for (int e = 1; e < TV_E; e++) {
-                top = fmaxf(top, x[e]);
+                top = fmaxf(top, v[e]);
             }
             if (top > m) {
                 s *= power2((m - top) * a);
@@ -246,7 +255,32 @@ struct Walk {
             if (m > -INFINITY) {
 #pragma unroll
                 for (int e = 0; e < TV_E; e++) {
-                    s += power2((x[e] - m) * a);
+                    s += power2((v[e] - m) * a);
+                }
+            }
+        };
+        const int step = n_warps * TV_CHUNK;
+        if constexpr (DT >= 0) {
+            for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += step) {
+                load(x, i0);
+                if (held) {
+                    load_drafts(i0);
+                }
+                clean(x);
+                add(x);
+            }
+        } else {
+            for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += 2 * step) {  // two chunks' loads in flight: 52 us against 56
+                float y[TV_E];
+                load(x, i0);
+                if (i0 + step < hi) {
+                    load(y, i0 + step);
+                }
+                clean(x);
+                add(x);
+                if (i0 + step < hi) {
+                    clean(y);
+                    add(y);
                 }
             }
         }
@@ -275,7 +309,8 @@ struct Walk {
         float m = -INFINITY;
         int   at = 0x7fffffff;
         for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
-            load(i0, false);
+            load(x, i0);
+            clean(x);
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
                 if (x[e] > m) {
@@ -319,7 +354,7 @@ struct Walk {
         double      sum = 0.0;
         for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
             if (!held) {
-                load(i0, true);
+                load_both(i0);
             }
             float s = 0.0f;
 #pragma unroll
@@ -347,7 +382,7 @@ struct Walk {
     // the chunk from i0 on for `left`: the rejected tokens of fixed choices count as -inf
     __device__ __forceinline__ void load_left(int i0, int n_gone) {
         if (!held || DT < 0 || coarse) {
-            load(i0, true);
+            load_both(i0);
         }
         if (coarse) {
 #pragma unroll

@@ -81,7 +81,7 @@ class CacheLayers:
         self.k, self.v = list(k), list(v)
         if not self.k or len(self.k) != len(self.v):
             raise MM3FAError(ERR_SHAPE, "CacheLayers")
-        self.n_layers, self.device, self.n_seq = len(self.k), self.k[0].device, self.k[0].shape[0]
+        self.n_layers, self.device, self._sets = len(self.k), self.k[0].device, self.k[0].shape[:1]
         types, dev = _types(), self.k[0].get_device()
         self._desc = [b"".join(_slab(t, types, dev, "CacheLayers") for t in x) for x in (self.k, self.v)]
 
@@ -101,6 +101,11 @@ class DraftTree(OnDevice):
             raise MM3FAError(ERR_STRIDE, "DraftTree: parents")
         self.parents, self.n_nodes = parents, n_nodes
         self.n_tree, self.max_nodes = parents.shape
+        self._each, self._per_node = self._torch.Size((self.n_tree,)), parents.shape
+        self._f32 = self._torch.float32
+        # results of `verify` are made like these
+        self._nodes_like = parents if parents.is_contiguous() else self._torch.empty_like(parents, memory_format=self._torch.contiguous_format)
+        self._trees_like = self._torch.empty(self.n_tree, dtype=self._int32, device=self.device)
         counts = 0 if n_nodes is None else self._ints(n_nodes, self.n_tree, "n_nodes")
         self._desc = _PACK_TREE(parents.data_ptr(), parents.stride(0) if self.n_tree > 1 else self.max_nodes, counts,
                                 self.max_nodes, self.n_tree)
@@ -108,23 +113,31 @@ class DraftTree(OnDevice):
     def _calls(self):
         return _calls()
 
-    def _each_node(self, t, dtype, what):
-        """Address of a contiguous tensor [n_tree, T]."""
+    def _flat(self, t, dtype, shape, what):
+        """Address of a contiguous tensor of a type and shape."""
+        if t.dtype is dtype and t.shape == shape and t.get_device() == self._dev and t.is_contiguous():
+            return t.data_ptr()
         if t.dtype is not dtype:
             raise MM3FAError(ERR_TYPE, "DraftTree: " + what)
         if t.get_device() != self._dev:
             raise self._elsewhere(t)
-        if t.dim() != 2 or t.shape[0] != self.n_tree or t.shape[1] != self.max_nodes:
-            raise MM3FAError(ERR_SHAPE, "DraftTree: " + what)
-        if not t.is_contiguous():
-            raise MM3FAError(ERR_STRIDE, "DraftTree: " + what)
-        return t.data_ptr()
+        raise MM3FAError(ERR_SHAPE if t.shape != shape else ERR_STRIDE, "DraftTree: " + what)
 
     def _rows_of_nodes(self, t, what):
         """mm3fa_tensor [V, T, n_tree, 1] of a tensor (n_tree, T, V)."""
         if t.dim() != 3:
             raise MM3FAError(ERR_SHAPE, "DraftTree: " + what)
-        return self._rows(t[None])
+        ty = self._dt.get(t.dtype)
+        if ty is None:
+            raise MM3FAError(ERR_TYPE, "DraftTree: " + what)
+        if t.get_device() != self._dev:
+            raise self._elsewhere(t)
+        n, T, V = t.shape
+        sn, st, sv = t.stride()
+        if sv != 1 and V > 1:
+            raise MM3FAError(ERR_STRIDE, "DraftTree: " + what)
+        ty, e = ty
+        return _PACK_TENSOR(ty, 0, V, T, n, 1, e, st * e, sn * e, n * sn * e, t.data_ptr())
 
     def attend(self, q, k, v, kv_len, scale, out=None, logit_softcap=0.0, ws=None, stream=None):
         """softmax(scale * q k^T) v of the queries q (N, n_head, T, D), where node i of a sequence sees the first kv_len[s]
@@ -137,18 +150,19 @@ class DraftTree(OnDevice):
                 return self.attend(q, k, v, kv_len, scale, out, logit_softcap, ws)
         qd, st = self._rows(q), self._stream()
         kd, vd = _slab(k, self._dt, self._dev, "DraftTree"), _slab(v, self._dt, self._dev, "DraftTree")
+        shape = q.shape
         if out is None:
             make = self._torch.empty if self.n_nodes is None else self._torch.zeros
-            out = make((q.shape[0], q.shape[2], q.shape[1], q.shape[3]), dtype=q.dtype, device=q.device)
+            out = make((shape[0], shape[2], shape[1], shape[3]), dtype=q.dtype, device=q.device)
         if ws is None:
-            shape = (q.shape, k.shape, q.dtype, k.dtype)
-            need = self._need.get(shape)
+            key = shape, k.shape, k.dtype
+            need = self._need.get(key)
             if need is None:
-                need = self._need[shape] = self._call("attn_workspace", qd, kd, vd, self._desc)
+                need = self._need[key] = self._call("attn_workspace", qd, kd, vd, self._desc)
             ptr, cap = self._workspace(("attn", st), need)
         else:
             ptr, cap = self._given(ws)
-        self._run("attn", qd, kd, vd, self._desc, self._ints(kv_len, q.shape[0], "kv_len"), scale, logit_softcap, self._rows(out),
+        self._run("attn", qd, kd, vd, self._desc, self._flat(kv_len, self._int32, shape[:1], "kv_len"), scale, logit_softcap, self._rows(out),
                   ptr, cap, st)
         return out
 
@@ -165,19 +179,15 @@ class DraftTree(OnDevice):
         if stream is not None:
             with self._on(stream):
                 return self.verify(logits, tokens, accept, sample, draft, temperature, out)
-        f32 = self._torch.float32
-        if sample.dtype is not f32:
-            raise MM3FAError(ERR_TYPE, "DraftTree: sample")
+        i32, f32, each, per_node, flat = self._int32, self._f32, self._each, self._per_node, self._flat
         if out is None:
-            n, T = self.n_tree, self.max_nodes
-            made = self._torch.empty(n * (T + 2), dtype=self._int32, device=self.device)
-            out = made[:n * T].view(n, T), made[n * T:n * T + n], made[n * T + n:]
+            like = self._torch.empty_like  # (a third of what empty() takes)
+            out = like(self._nodes_like), like(self._trees_like), like(self._trees_like)
         path, n_path, token = out
         self._run("verify", self._rows_of_nodes(logits, "logits"), None if draft is None else self._rows_of_nodes(draft, "draft"),
-                  self._desc, self._each_node(tokens, self._int32, "tokens"), self._each_node(accept, f32, "accept"),
-                  self._ints(sample.view(self._int32), self.n_tree, "sample"), temperature,
-                  self._each_node(path, self._int32, "path"), self._ints(n_path, self.n_tree, "n_path"),
-                  self._ints(token, self.n_tree, "token"), self._stream())
+                  self._desc, flat(tokens, i32, per_node, "tokens"), flat(accept, f32, per_node, "accept"),
+                  flat(sample, f32, each, "sample"), temperature, flat(path, i32, per_node, "path"),
+                  flat(n_path, i32, each, "n_path"), flat(token, i32, each, "token"), self._stream())
         return out
 
     def commit(self, layers, path, n_path, kv_len, kv_len_out=None, stream=None):
@@ -190,8 +200,8 @@ class DraftTree(OnDevice):
             raise self._elsewhere(layers)
         if kv_len_out is None:
             kv_len_out = self._torch.empty_like(kv_len)
-        n = layers.n_seq
-        self._run("commit", *layers._desc, layers.n_layers, self._each_node(path, self._int32, "path"),
-                  self._ints(n_path, self.n_tree, "n_path"), self.max_nodes, self.n_tree, self._ints(kv_len, n, "kv_len"),
-                  self._ints(kv_len_out, n, "kv_len_out"), self._stream())
+        i32, flat, sets = self._int32, self._flat, layers._sets
+        self._run("commit", *layers._desc, layers.n_layers, flat(path, i32, self._per_node, "path"),
+                  flat(n_path, i32, self._each, "n_path"), self.max_nodes, self.n_tree, flat(kv_len, i32, sets, "kv_len"),
+                  flat(kv_len_out, i32, sets, "kv_len_out"), self._stream())
         return kv_len_out
