@@ -55,7 +55,7 @@ constexpr int TS_LEAST   = 4;    // tiles of a part, at least: a part costs as m
 constexpr int TS_PIECES  = 4;    // pieces that warp 0 may be ahead
 constexpr int TS_COST    = 3;    // tiles' time that a unit takes beside them
 constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for
-constexpr int TJ_UNITS   = 512;  // units in parts, at most one a CTA: there are no more CTAs than SMs or blocks of a unit
+constexpr int TJ_WARPS   = 8;    // of a joining CTA
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
 constexpr int TS_REGS_SOFTMAX = 208;  // 2 x 208 + 88 = 3 x 168
 constexpr int TS_REGS_ISSUE   = 88;
@@ -91,18 +91,18 @@ enum : int {
     TB_SFULL  = 16,  // [2]
     TB_PREADY = 18,  // [2] 128 softmax threads
     TB_OFULL  = 20,  // [2] a tile's P V (PARTS 1: the last of a piece)
-    TB_QREADY = 22,  // 64
-    TB_QFREE  = 23,  // the last QK of a piece
-    TB_LOOK   = 24,  // warp 1: a V tile with nodes is there
-    TB_FIX    = 25,  // 64 threads of warps 2, 3: it can be taken
-    TB_DONE   = 26,
-    TB_PIECE  = 27,  // [TS_PIECES] warp 0
-    TB_PFREE  = 31,  // [TS_PIECES] the 11 other warps
-    TB_COUNT  = 35,
+    TB_QREADY = 22,  // [2 pieces] 64.  (Two: a piece's may follow the one before while the softmax has not waited for that yet)
+    TB_QFREE  = 24,  // the last QK of a piece
+    TB_LOOK   = 25,  // warp 1: a V tile with nodes is there
+    TB_FIX    = 26,  // 64 threads of warps 2, 3: it can be taken
+    TB_DONE   = 27,
+    TB_PIECE  = 28,  // [TS_PIECES] warp 0
+    TB_PFREE  = 32,  // [TS_PIECES] the 11 other warps
+    TB_COUNT  = 36,
 };
 
 __host__ __device__ constexpr uint32_t ts_arrivals(int b) {
-    return b >= TB_PFREE ? (uint32_t) (TS_THREADS / 32 - 1) : b == TB_QREADY || b == TB_FIX ? 64u : b == TB_PREADY || b == TB_PREADY + 1 ? 128u : 1u;
+    return b >= TB_PFREE ? (uint32_t) (TS_THREADS / 32 - 1) : b == TB_QREADY || b == TB_QREADY + 1 || b == TB_FIX ? 64u : b == TB_PREADY || b == TB_PREADY + 1 ? 128u : 1u;
 }
 
 // kind::f16 instruction descriptor: F16 x F16 or BF16 x BF16 -> F32, M = 128
@@ -227,9 +227,13 @@ struct TsJoin {
     int64_t part0, part1;       // where the first part and the second are, in floats; the others follow at even steps
 };
 
-// (functions of their own, for the instruction cache's sake)
-__device__ __noinline__ int ts_div(int a, int b) {
+// a / b for 0 <= a and 0 < b.  Below 2^20 in F32: (a + 1/2) / b is at least 1 / 2b from a whole number, and off by less.
+__device__ __noinline__ int ts_div_large(int a, int b) {
     return (int) ((unsigned) a / (unsigned) b);
+}
+
+__device__ __forceinline__ int ts_div(int a, int b) {
+    return a < (1 << 20) ? (int) __fdividef((float) a + 0.5f, (float) b) : ts_div_large(a, b);
 }
 
 __device__ __forceinline__ int ts_up(int a, int b) {
@@ -318,8 +322,8 @@ struct TsPlan {
         if (p.n_seq <= TS_EVEN && U <= groups) {
             // the fewest tiles to a part that need no more than all groups: each lane tries one of 32 numbers between what
             // even shares would be and what is enough
-            const int lo = max(TS_LEAST, ts_up(W, groups));
-            const int hi = max(lo, U < groups ? min(most, ts_up(W, groups - U)) : most);
+            const int lo = max(TS_LEAST + 1, ts_up(W + U, groups));
+            const int hi = max(lo, U < groups ? min(most + 1, ts_up(W + U, groups - U)) : most + 1);
             const int t  = lo + lane * ((hi - lo + 30) / 31);
             int       parts = 0;
 #pragma unroll 1
@@ -330,7 +334,7 @@ struct TsPlan {
                 } else {
                     c = ts_seq(p, i);
                 }
-                parts += (c.tiles + t - 1) / t * heads(c);
+                parts += c.tiles > 0 ? ts_up(c.tiles + 1, t) * heads(c) : 0;
             }
             const unsigned fits = __ballot_sync(0xffffffffu, parts <= groups);
             even = __shfl_sync(0xffffffffu, t, __ffs(fits) - 1);  // (the last lane's fits)
@@ -383,9 +387,14 @@ struct TsPlan {
         return wide > 1 ? p.n_head_kv : p.n_head_kv * ((c.nodes * p.ratio + TS_M - 1) / TS_M);
     }
 
-    // a sequence's length on the line, or its parts
+    // a unit's length on the line, or its parts: these share its tiles and one more, for what the nodes' masks take
+    __device__ __forceinline__ int length(const TsSeq & c) const {
+        return even ? ts_up(c.tiles + 1, even) : c.tiles + TS_COST;
+    }
+
+    // a sequence's
     __device__ __forceinline__ int weight(const TsSeq & c) const {
-        return c.tiles == 0 ? 0 : (even ? ts_up(c.tiles, even) : c.tiles + TS_COST) * heads(c);
+        return c.tiles == 0 ? 0 : length(c) * heads(c);
     }
 
     // the next piece that has rows in this CTA's block
@@ -393,15 +402,15 @@ struct TsPlan {
         TsPiece c = {};
 #pragma unroll 1
         while (x < end) {
-            const int all = weight(q);
+            const int n = q.tiles > 0 ? length(q) : 0, all = n * heads(q);
             if (x - first >= all) {
                 first += all;
                 q = ts_seq(p, ++s);
                 continue;
             }
-            const int n = even ? ts_up(q.tiles, even) : q.tiles + TS_COST, i = ts_div(x - first, n);  // a unit's length, the unit
+            const int i = ts_div(x - first, n);  // the unit
             const int bl = wide > 1 ? 1 : (q.nodes * p.ratio + TS_M - 1) / TS_M;
-            c.h    = i / bl;
+            c.h    = bl == 1 ? i : ts_div(i, bl);
             c.rb   = wide > 1 ? beside : i - c.h * bl;
             c.rows = min(q.nodes * p.ratio - c.rb * TS_M, TS_M);
             if (c.rows <= 0) {  // (the block is empty: on to the next sequence)
@@ -413,7 +422,7 @@ struct TsPlan {
             c.unit = first + i * n;
             if (even) {
                 const int k = x - c.unit;
-                c.a = ts_div(k * q.tiles, n), c.b = ts_div((k + 1) * q.tiles, n);
+                c.a = ts_div(k * (q.tiles + 1), n), c.b = min(ts_div((k + 1) * (q.tiles + 1), n), q.tiles);
                 x++;
             } else {
                 const int to = c.unit + n <= end ? c.unit + n : TsLine::border(end, c.unit, n);
@@ -444,7 +453,7 @@ struct TsPlan {
 
     // what the joining kernel has to know of a unit, from its first part
     __device__ __forceinline__ TsJoin join(const TsPiece & c) const {
-        const int g = second(c), parts = even ? ts_up(c.tiles, even) : ln.last(c.unit + c.tiles + TS_COST - TS_LEAST) - g + 2;
+        const int g = second(c), parts = even ? ts_up(c.tiles + 1, even) : ln.last(c.unit + c.tiles + TS_COST - TS_LEAST) - g + 2;
         return { c.s, c.h, parts, c.rows, c.rb * TS_M, part(c, g, 0), part(c, g, 1) };
     }
 };
@@ -452,12 +461,12 @@ struct TsPlan {
 // Rows ra .. ra + 15 of a block's Q for the products, by a warp; rows that do not count are zeros.  All copies are in
 // flight at once, and land where the row's products will read it: PARTS 1, as they are; PARTS 2, a row's bytes lie in
 // the places of its own two parts (F32: all of them), and the warp replaces one row after another.
-template <int D, bool BF16, int PARTS>
+template <int D, bool BF16, int PARTS, int UNROLL>
 __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPiece & it, int ra, char * qs, float * factors, int lane) {
     constexpr int E = D / 32, QT = TsSmem<D, PARTS>::QT, BLOCK = TS_M * 128;
     const int     in = it.rows - ra, esz = p.q.type == KV_F32 ? 4 : 2;
-    // lane i, and 16 + i: the address of row i
-    const int      rl = it.rb * TS_M + ra + (lane & 15), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
+    // lane i, and 16 + i: the address of row i (of the last one, behind it)
+    const int      rl = it.rb * TS_M + max(min(ra + (lane & 15), it.rows - 1), 0), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
     const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
     // (not 0, whose product with the -inf of a key that is not seen would be no number)
     const float    by = fmaxf(fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E), 0x1p-126f);
@@ -466,20 +475,24 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
         const int blk = ck >> 3;
         return qs + (blk % (D / 64)) * BLOCK + (blk / (D / 64)) * QT + (ra + i) * 128 + (((ck & 7) ^ (PARTS == 1 ? i & 7 : 0)) << 4);  // (ra: a multiple of 8)
     };
-    const int chunks = D * esz / 16, per = 32 / chunks, ck = lane % chunks;
+    const int chunks = D * esz / 16, per = 32 / chunks, ck = lane % chunks, i1 = lane / chunks;
+    if (p.q.vec) {
+#pragma unroll UNROLL
+        for (int i = i1; i < 16; i += per) {
+            const uint64_t src = __shfl_sync(0xffffffffu, al, i) + ck * 16;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(place(i, ck))), "l"(src), "r"(i < in ? 16 : 0) : "memory");
+        }
+    } else {
 #pragma unroll 1
-    for (int i = lane / chunks; i < 16; i += per) {
-        const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i)) + ck * 16;
-        char *       to  = place(i, ck);
-        if (p.q.vec || i >= in) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(i < in ? src : p.q.data), "r"(i < in && p.q.vec ? 16 : 0) : "memory");
-        } else {
+        for (int i = i1; i < 16; i += per) {
+            const char * src = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, al, i)) + ck * 16;
+            char *       to  = place(i, ck);
 #pragma unroll 1
             for (int e = 0; e < 16; e += esz) {
                 if (esz == 4) {
-                    *reinterpret_cast<uint32_t *>(to + e) = *reinterpret_cast<const uint32_t *>(src + e);
+                    *reinterpret_cast<uint32_t *>(to + e) = i < in ? *reinterpret_cast<const uint32_t *>(src + e) : 0u;
                 } else {
-                    *reinterpret_cast<uint16_t *>(to + e) = *reinterpret_cast<const uint16_t *>(src + e);
+                    *reinterpret_cast<uint16_t *>(to + e) = i < in ? *reinterpret_cast<const uint16_t *>(src + e) : (uint16_t) 0;
                 }
             }
         }
@@ -690,7 +703,8 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             };
             uint32_t c = 0, tc = 0, looks = 0;
             while (next()) {
-                wait(TB_QREADY, pieces++);
+                wait(TB_QREADY + (int) (pieces & 1), pieces >> 1);
+                pieces++;
 #pragma unroll 1
                 for (int j = it.a - 1; j < it.b; j++) {  // QK(j + 1), then P V(j)
                     if (j + 1 < it.b) {
@@ -763,10 +777,10 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     }
 #pragma unroll 1
                     for (int ra = (warp & 1) * 16; ra < TS_M; ra += 32) {
-                        ts_stage16<D, BF16, PARTS>(p, it, ra, smem + L::OFF_Q, factors + (pieces & 1) * TS_M, lane);
+                        ts_stage16<D, BF16, PARTS, 1>(p, it, ra, smem + L::OFF_Q, factors + (pieces & 1) * TS_M, lane);
                     }
                     fence_proxy_async_smem();
-                    dn_mbar_arrive(&bar[TB_QREADY]);
+                    dn_mbar_arrive(&bar[TB_QREADY + (pieces & 1)]);
                 }
 #pragma unroll 1
                 for (int j = max(it.a, it.L / TS_N); j < it.b; j++) {
@@ -849,7 +863,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             {
                 const int nodes = it.nodes, parent = tail && own < nodes ? tree_parent(p.t, it.s % p.t.n_tree, own) : -1;
                 if (pieces == 0) {
-                    ts_stage16<D, BF16, PARTS>(p, it, (w * 4 + quad) * 16, smem + L::OFF_Q, factors, lane);
+                    ts_stage16<D, BF16, PARTS, 4>(p, it, (w * 4 + quad) * 16, smem + L::OFF_Q, factors, lane);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane < 8) {
@@ -875,7 +889,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     softmax_barrier();
                 }
             }
-            wait(TB_QREADY, pieces);
+            wait(TB_QREADY + (int) (pieces & 1), pieces >> 1);
             const float f0 = factors[(pieces & 1) * TS_M + r], factor = cap || f0 != f0 ? 1.0f : f0;
             // which of the 32 keys from k0 on the row sees
             auto seen = [&](int k0) -> uint32_t {
@@ -906,23 +920,33 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     continue;
                 }
                 wait(TB_SFULL + w, tc >> 1);
-                if (warp_live && (cap || (j + 1) * TS_N > held)) {
-                    // over S: with a softcap, s = cap * tanh(S * factor) in log2 units; -inf for a key that the row does not see
+                if (warp_live && cap) {  // over S: s = cap * tanh(S * factor), in log2 units
                     const float fcap = f0 != f0 ? 1.0f : f0;
 #pragma unroll 1
                     for (int c = 0; c < 8; c++) {
                         uint32_t v[16];
                         tmem_ld16(s_col + (uint32_t) (c * 16), v);
                         tmem_ld16_wait(v);
-                        const uint32_t see = (live ? seen(j * TS_N + (c >> 1) * 32) : 0u) >> (16 * (c & 1));
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            if (cap) {
-                                v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
-                            }
-                            v[e] = see >> e & 1u ? v[e] : 0xff800000u;
+                            v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
                         }
                         tmem_st16(s_col + (uint32_t) (c * 16), v);
+                    }
+                    tmem_st_wait();
+                }
+                if (warp_live && (j + 1) * TS_N > held) {  // over S: -inf for a key that the row does not see
+#pragma unroll 1
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t v[32];
+                        tmem_ld32(s_col + (uint32_t) (c * 32), v);
+                        const uint32_t see = live ? seen(j * TS_N + c * 32) : 0u;
+                        tmem_ld_wait_tie(v);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            v[e] = see >> e & 1u ? v[e] : 0xff800000u;
+                        }
+                        tmem_st32(s_col + (uint32_t) (c * 32), v);
                     }
                     tmem_st_wait();
                 }
@@ -1059,8 +1083,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             tmem_ld32(o_col + (uint32_t) (c * 32), o);
                             tmem_ld_wait_tie(o);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                acc[c * 32 + e] = fmaf(acc[c * 32 + e], g, __uint_as_float(o[e]));
+                            for (int e = 0; e < 32; e += 2) {
+                                f2unpack(ffma2(f2pack(acc[c * 32 + e], acc[c * 32 + e + 1]), f2pack(g, g), f2pack(__uint_as_float(o[e]), __uint_as_float(o[e + 1]))),
+                                         acc[c * 32 + e], acc[c * 32 + e + 1]);
                             }
                         }
                     }
@@ -1198,75 +1223,53 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     }
 }
 
-// Joins the parts of units, in their order.  Items of 32 rows and 16 columns over all CTAs: a warp has four columns, a lane
-// a row, and every load of 8 parts in flight.
+// Joins the parts of units, in their order: the units of the first kernel's CTA blockIdx.x, 32 rows and four columns by each
+// warp, a row by each lane, the loads of 16 parts in flight.
 template <int D>
-__global__ void __launch_bounds__(128) tree_attn_join_kernel(const TreeAttnParams p, int wide, int groups, int slot_rows) {
-    constexpr int  PER = 8;  // parts loaded at a time
-    __shared__ int list[TJ_UNITS], counts[4];
-    const int      tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__global__ void __launch_bounds__(32 * TJ_WARPS) tree_attn_join_kernel(const TreeAttnParams p, int wide, int slot_rows) {
     kv8_dep_wait();
-    const TsJoin * units = reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE);
-    int            n_units = 0;
-    for (int i0 = 0; i0 < groups * wide; i0 += 128) {  // which groups have one, in their order
-        const bool     has = i0 + tid < groups * wide && units[i0 + tid].parts > 0;
-        const unsigned all = __ballot_sync(0xffffffffu, has);
-        if (lane == 0) {
-            counts[warp] = __popc(all);
-        }
-        __syncthreads();
-        int at = n_units + __popc(all & ((1u << lane) - 1u));
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            at += w < warp ? counts[w] : 0;
-            n_units += counts[w];
-        }
-        if (has) {
-            list[at] = i0 + tid;
-        }
-        __syncthreads();
+    constexpr int PER = 16;  // parts loaded at a time
+    const TsJoin  t = reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE)[blockIdx.x];
+    const int     item = (int) blockIdx.y * TJ_WARPS + (int) threadIdx.x / 32, k4 = item % (D / 4), r = item / (D / 4) * 32 + (int) threadIdx.x % 32;
+    if (t.parts == 0 || r >= t.rows) {
+        return;
     }
     const int64_t step = (int64_t) wide * 2 * ts_slot_floats(slot_rows, D);
-    const int     quarters = (slot_rows + 31) / 32, per_unit = quarters * (D / 16);
-    for (int item = blockIdx.x; item < n_units * per_unit; item += (int) gridDim.x) {
-        const int    u = list[item / per_unit], rest = item % per_unit, r = rest % quarters * 32 + lane, k4 = rest / quarters * 4 + warp;
-        const TsJoin t = units[u];
-        if (r >= t.rows) {
-            continue;
-        }
-        auto   part = [&](int k) { return p.part + (k == 0 ? t.part0 : t.part1 + (k - 1) * step); };
-        float  M = -INFINITY, l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k0 = 0; k0 < t.parts; k0 += PER) {
-            float2 x[PER];
-            float4 v[PER];
+    float         M = -INFINITY, l = 0.0f;
+    float4        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int k0 = 0; k0 < t.parts; k0 += PER) {
+        float2 x[PER];
+        float4 v[PER];
 #pragma unroll
-            for (int k = 0; k < PER; k++) {
-                const float * at = part(min(k0 + k, t.parts - 1));
+        for (int k = 0; k < PER; k++) {
+            x[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (k0 + k < t.parts) {
+                const float * at = p.part + (k0 + k == 0 ? t.part0 : t.part1 + (k0 + k - 1) * step);
                 x[k] = reinterpret_cast<const float2 *>(at + slot_rows * D)[r];
                 v[k] = reinterpret_cast<const float4 *>(at)[k4 * slot_rows + r];
             }
-            float top = M;
+        }
+        float top = M;
 #pragma unroll
-            for (int k = 0; k < PER; k++) {
-                top = fmaxf(top, x[k].x);
-            }
-            const float g = M == top ? 1.0f : ex2(M - top);
-            l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
+        for (int k = 0; k < PER; k++) {
+            top = fmaxf(top, x[k].x);
+        }
+        const float g = M == top ? 1.0f : ex2(M - top);
+        l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
 #pragma unroll
-            for (int k = 0; k < PER; k++) {
-                if (k0 + k < t.parts) {
-                    const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
-                    l = fmaf(x[k].y, f, l);
-                    o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
-                }
+        for (int k = 0; k < PER; k++) {
+            if (k0 + k < t.parts) {
+                const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
+                l = fmaf(x[k].y, f, l);
+                o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
             }
         }
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        const int   row = (int) t.row0 + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
-        ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * k4,
-                  make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
     }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const int   row = (int) t.row0 + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
+    ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * k4,
+              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
 }
 
 template <int D, bool BF16, int PARTS>
@@ -1293,12 +1296,13 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
     }
     const int wide = tree_attn_wide(p), groups = tree_attn_groups(p, sms);
     const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
-    e = kv8_launch(kern, dim3((unsigned) (groups * wide)), TS_THREADS, smem, stream, tmk, tmv, p, wide, groups, rows, p.n_kv > TS_LEAST * TS_N ? 1 : 0);
+    e = kv8_launch(kern, dim3((unsigned) (groups * wide)), TS_THREADS, smem, stream, tmk, tmv, p, wide, groups, rows, p.n_kv <= TS_LEAST * TS_N ? 0 : 1);
     if (e != cudaSuccess || p.n_kv <= TS_LEAST * TS_N) {
         return e;  // (no unit is in parts)
     }
-    const int items = groups * wide * ((rows + 31) / 32) * (D / 16);
-    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) std::min(items, 4 * sms)), 128, 0, stream, p, wide, groups, rows);
+    const int items = (rows + 31) / 32 * (D / 4);
+    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) (groups * wide), (unsigned) ((items + TJ_WARPS - 1) / TJ_WARPS)), 32 * TJ_WARPS, 0, stream, p,
+                      wide, rows);
 }
 
 template <int D, bool BF16>

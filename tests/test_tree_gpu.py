@@ -243,6 +243,30 @@ def test_attend_is_the_same_every_time(cuda_device):
             assert torch.equal(c.run(), want)
 
 
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("lens", [[(i * 37) % 100 for i in range(64)], [(i * 211) % 1500 for i in range(48)]])
+def test_attend_many_short_pieces(cuda_device, lens, dtype, cache):
+    """More units than SMs, of a tile or a few: every CTA goes from unit to unit, its warps at different places.  Back to
+    back and in a graph, no wait runs out and every result is the same."""
+    c = Case(cuda_device, lens, len(lens), 32, 8, 128, 13, dtype, cache, seed=16, n_nodes=[1 + i % 13 for i in range(len(lens))])
+    tree = c.tree()
+    want = c.check().clone()
+    outs = [c.run(tree=tree) for _ in range(30)]
+    tree.check()
+    assert all(torch.equal(o, want) for o in outs)
+    out = c.out()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for _ in range(20):
+            c.run(tree=tree, out=out)
+    for _ in range(10):
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        tree.check(captured=True)
+        assert torch.equal(out, want)
+
+
 def test_attend_on_streams_and_in_graphs(cuda_device):
     """Two streams at once, a given stream, and two graphs replayed side by side with other lengths and trees."""
     c = Case(cuda_device, [3000, 1200], 1, 16, 4, 128, 20, "f32", "f16", seed=14)
