@@ -56,6 +56,7 @@ constexpr int TS_PIECES  = 4;    // pieces that warp 0 may be ahead
 constexpr int TS_COST    = 3;    // tiles' time that a unit takes beside them
 constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for
 constexpr int TJ_WARPS   = 8;    // of a joining CTA
+constexpr int TJ_UNITS   = 512;  // units in parts, at most one a CTA: there are no more CTAs than SMs or blocks of a unit
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
 constexpr int TS_REGS_SOFTMAX = 208;  // 2 x 208 + 88 = 3 x 168
 constexpr int TS_REGS_ISSUE   = 88;
@@ -1223,53 +1224,79 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     }
 }
 
-// Joins the parts of units, in their order: the units of the first kernel's CTA blockIdx.x, 32 rows and four columns by each
-// warp, a row by each lane, the loads of 16 parts in flight.
+// Joins the parts of units, in their order: 32 rows and four columns by each warp, a row by each lane, the loads of 16 parts
+// in flight.  Every CTA finds the units in parts from what the first kernel's CTAs have left, and takes its share of all
+// (a CTA for each of those CTAs and each share of a unit: 2368 of them take longer to come and go than to work).
 template <int D>
-__global__ void __launch_bounds__(32 * TJ_WARPS) tree_attn_join_kernel(const TreeAttnParams p, int wide, int slot_rows) {
+__global__ void __launch_bounds__(32 * TJ_WARPS) tree_attn_join_kernel(const TreeAttnParams p, int ctas, int wide, int slot_rows) {
+    constexpr int  PER = 16;  // parts loaded at a time
+    __shared__ int list[TJ_UNITS], counts[TJ_WARPS];
+    const int      tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     kv8_dep_wait();
-    constexpr int PER = 16;  // parts loaded at a time
-    const TsJoin  t = reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE)[blockIdx.x];
-    const int     item = (int) blockIdx.y * TJ_WARPS + (int) threadIdx.x / 32, k4 = item % (D / 4), r = item / (D / 4) * 32 + (int) threadIdx.x % 32;
-    if (t.parts == 0 || r >= t.rows) {
-        return;
+    const TsJoin * units   = reinterpret_cast<const TsJoin *>(reinterpret_cast<const char *>(p.status) + TS_SPACE);
+    int            n_units = 0;
+    for (int i0 = 0; i0 < ctas; i0 += 32 * TJ_WARPS) {
+        const bool     has = i0 + tid < ctas && units[i0 + tid].parts > 0;
+        const unsigned all = __ballot_sync(0xffffffffu, has);
+        if (lane == 0) {
+            counts[warp] = __popc(all);
+        }
+        __syncthreads();
+        int at = n_units + __popc(all & ((1u << lane) - 1u));
+#pragma unroll
+        for (int w = 0; w < TJ_WARPS; w++) {
+            at += w < warp ? counts[w] : 0;
+            n_units += counts[w];
+        }
+        if (has) {
+            list[at] = i0 + tid;
+        }
+        __syncthreads();
     }
-    const int64_t step = (int64_t) wide * 2 * ts_slot_floats(slot_rows, D);
-    float         M = -INFINITY, l = 0.0f;
-    float4        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int quarters = (slot_rows + 31) / 32, per_unit = quarters * (D / 4);
+    for (int item = (int) blockIdx.x * TJ_WARPS + warp; item < n_units * per_unit; item += (int) gridDim.x * TJ_WARPS) {
+        const TsJoin t = units[list[item / per_unit]];
+        const int    k4 = item % per_unit / quarters, r = item % quarters * 32 + lane;
+        if (r >= t.rows) {
+            continue;
+        }
+        const int64_t step = (int64_t) wide * 2 * ts_slot_floats(slot_rows, D);
+        float         M = -INFINITY, l = 0.0f;
+        float4        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-    for (int k0 = 0; k0 < t.parts; k0 += PER) {
-        float2 x[PER];
-        float4 v[PER];
+        for (int k0 = 0; k0 < t.parts; k0 += PER) {
+            float2 x[PER];
+            float4 v[PER];
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            x[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (k0 + k < t.parts) {
-                const float * at = p.part + (k0 + k == 0 ? t.part0 : t.part1 + (k0 + k - 1) * step);
-                x[k] = reinterpret_cast<const float2 *>(at + slot_rows * D)[r];
-                v[k] = reinterpret_cast<const float4 *>(at)[k4 * slot_rows + r];
+            for (int k = 0; k < PER; k++) {
+                x[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (k0 + k < t.parts) {
+                    const float * at = p.part + (k0 + k == 0 ? t.part0 : t.part1 + (k0 + k - 1) * step);
+                    x[k] = reinterpret_cast<const float2 *>(at + slot_rows * D)[r];
+                    v[k] = reinterpret_cast<const float4 *>(at)[k4 * slot_rows + r];
+                }
+            }
+            float top = M;
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                top = fmaxf(top, x[k].x);
+            }
+            const float g = M == top ? 1.0f : ex2(M - top);
+            l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
+#pragma unroll
+            for (int k = 0; k < PER; k++) {
+                if (k0 + k < t.parts) {
+                    const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
+                    l = fmaf(x[k].y, f, l);
+                    o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
+                }
             }
         }
-        float top = M;
-#pragma unroll
-        for (int k = 0; k < PER; k++) {
-            top = fmaxf(top, x[k].x);
-        }
-        const float g = M == top ? 1.0f : ex2(M - top);
-        l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
-#pragma unroll
-        for (int k = 0; k < PER; k++) {
-            if (k0 + k < t.parts) {
-                const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
-                l = fmaf(x[k].y, f, l);
-                o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
-            }
-        }
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        const int   row = (int) t.row0 + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
+        ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * k4,
+                  make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
     }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    const int   row = (int) t.row0 + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
-    ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * k4,
-              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
 }
 
 template <int D, bool BF16, int PARTS>
@@ -1300,9 +1327,8 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
     if (e != cudaSuccess || p.n_kv <= TS_LEAST * TS_N) {
         return e;  // (no unit is in parts)
     }
-    const int items = (rows + 31) / 32 * (D / 4);
-    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) (groups * wide), (unsigned) ((items + TJ_WARPS - 1) / TJ_WARPS)), 32 * TJ_WARPS, 0, stream, p,
-                      wide, rows);
+    const int items = groups * wide * ((rows + 31) / 32) * (D / 4);
+    return kv8_launch(tree_attn_join_kernel<D>, dim3((unsigned) std::min((items + TJ_WARPS - 1) / TJ_WARPS, 2 * sms)), 32 * TJ_WARPS, 0, stream, p, groups * wide, wide, rows);
 }
 
 template <int D, bool BF16>
