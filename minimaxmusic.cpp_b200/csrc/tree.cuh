@@ -75,6 +75,6 @@ int         tree_attn_groups(const TreeAttnParams & p, int sms);
 size_t      tree_attn_tc_workspace(const TreeAttnParams & p, int sms);
 cudaError_t launch_tree_attn_tc(TreeAttnParams p, int sms, cudaStream_t stream);
 cudaError_t launch_tree_verify(const TreeVerifyParams & p, int sms, cudaStream_t stream);
-cudaError_t launch_tree_commit(const TreeCommitParams & p, int unit, cudaStream_t stream);
+cudaError_t launch_tree_commit(const TreeCommitParams & p, int unit, int sms, cudaStream_t stream);
 
 }  // namespace mm3fa

@@ -276,7 +276,7 @@ int mm3fa_tree_commit(const mm3fa_tensor * k, const mm3fa_tensor * v, int n_laye
     if (S % n_tree) {
         return MM3FA_ERR_SHAPE;
     }
-    // (a launch's units, one for each layer, K or V, set and head, are a grid of 32 bits)
+    // (sets and heads are counted in 32 bits)
     if (row > (1 << 20) || k->ne[2] > (1 << 20) || S > 65535 || 2 * (int64_t) TREE_LAYERS * S * k->ne[2] > INT32_MAX) {
         return MM3FA_ERR_UNSUPPORTED;
     }
@@ -313,7 +313,7 @@ int mm3fa_tree_commit(const mm3fa_tensor * k, const mm3fa_tensor * v, int n_laye
             p.k[i] = static_cast<char *>(k[l + i].data);
             p.v[i] = static_cast<char *>(v[l + i].data);
         }
-        const int st = host_record_cuda(launch_tree_commit(p, unit, static_cast<cudaStream_t>(stream)));
+        const int st = host_record_cuda(launch_tree_commit(p, unit, host_sm_count(), static_cast<cudaStream_t>(stream)));
         if (st != MM3FA_OK) {
             return st;
         }
