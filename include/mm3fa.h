@@ -606,7 +606,8 @@ typedef struct mm3fa_tree {
     int32_t         n_tree;
 } mm3fa_tree;
 
-/* Bytes of device workspace mm3fa_tree_attn needs, 64 KiB at least (0: operands it would refuse). */
+/* Bytes of device workspace mm3fa_tree_attn needs, 64 KiB at least (0: operands it would refuse); by types and sizes, whatever
+ * the addresses and strides. */
 MM3FA_API size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v,
                                            const mm3fa_tree * tree);
 

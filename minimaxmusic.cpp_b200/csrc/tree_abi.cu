@@ -135,7 +135,8 @@ extern "C" {
 
 size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v, const mm3fa_tree * tree) {
     TreeAttnParams p{};
-    return prepare_attn(q, k, v, tree, p) != MM3FA_OK ? 0 : tree_attn_tc_takes(p) ? tree_attn_tc_workspace(p, host_sm_count()) : KV8_WS_ZEROED;
+    // (the same for rows of every alignment and stride)
+    return prepare_attn(q, k, v, tree, p) != MM3FA_OK ? 0 : tree_attn_tc_sizes(p) ? tree_attn_tc_workspace(p, host_sm_count()) : KV8_WS_ZEROED;
 }
 
 int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v, const mm3fa_tree * tree, const int32_t * kv_len,

@@ -1339,7 +1339,13 @@ cudaError_t launch_d(const TreeAttnParams & p, int sms, cudaStream_t stream) {
 
 }  // namespace
 
-// 16-bit slabs whose strides a tensor map takes, at D = 64 and 128
+// 16-bit slabs at D = 64 and 128
+bool tree_attn_tc_sizes(const TreeAttnParams & p) {
+    return (p.k.type == KV_F16 || p.k.type == KV_BF16) && (p.D == 64 || p.D == 128) && tensor_maps_available() &&
+           (int64_t) p.n_seq * p.n_head_kv * ((p.t.max_nodes * p.ratio + TS_M - 1) / TS_M) * ((p.n_kv + TS_N - 1) / TS_N + TS_COST) < (1 << 30);
+}
+
+// of these, slabs whose strides a tensor map takes
 bool tree_attn_tc_takes(const TreeAttnParams & p) {
     for (const Kv8Rows * x : { &p.k, &p.v }) {
         const int64_t most = (int64_t) 1 << 40;
@@ -1348,8 +1354,7 @@ bool tree_attn_tc_takes(const TreeAttnParams & p) {
             return false;
         }
     }
-    return (p.k.type == KV_F16 || p.k.type == KV_BF16) && (p.D == 64 || p.D == 128) && tensor_maps_available() &&
-           (int64_t) p.n_seq * p.n_head_kv * ((p.t.max_nodes * p.ratio + TS_M - 1) / TS_M) * ((p.n_kv + TS_N - 1) / TS_N + TS_COST) < (1 << 30);
+    return tree_attn_tc_sizes(p);
 }
 
 int tree_attn_wide(const TreeAttnParams & p) {

@@ -143,6 +143,20 @@ def test_attend_strides(cuda_device):
         assert (ob[:, 0] == 7).all() and (ob[:, :, 8] == 7).all() and (ob[..., :off] == 7).all() and (ob[..., off + D:] == 7).all()
 
 
+def test_attend_strides_in_turn(cuda_device):
+    """One tree with slabs of the same shape, first with rows that are not 16-byte aligned, then with aligned ones."""
+    c = Case(cuda_device, [4000, 3000], 1, 8, 2, 128, 12, "f32", "f16", seed=8)
+    tree, big = c.tree(), torch.zeros(2, 2, c.rows, 131, dtype=torch.float16, device=cuda_device)
+    aligned, c.k = c.k, big[..., 1:129]
+    c.k.copy_(aligned)
+    need = tree.attend_workspace(c.q, c.k, c.v)
+    c.check(c.run(tree=tree))
+    c.k = aligned
+    assert tree.attend_workspace(c.q, c.k, c.v) == need
+    c.check(c.run(tree=tree))
+    tree.check()
+
+
 @pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("bf16", "bf16"), ("f32", "q8_0")])
 def test_attend_scales_and_softcap(cuda_device, dtype, cache):
     c = Case(cuda_device, [300, 5], 1, 8, 2, 128, 10, dtype, cache, seed=8)
