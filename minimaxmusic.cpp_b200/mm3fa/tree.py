@@ -158,7 +158,9 @@ class DraftTree(OnDevice):
             key = shape, k.shape, k.dtype
             need = self._need.get(key)
             if need is None:
-                need = self._need[key] = self._call("attn_workspace", qd, kd, vd, self._desc)
+                need = self._call("attn_workspace", qd, kd, vd, self._desc)
+                if need:  # (0: the call is refused, and others of that shape may not be)
+                    self._need[key] = need
             ptr, cap = self._workspace(("attn", st), need)
         else:
             ptr, cap = self._given(ws)

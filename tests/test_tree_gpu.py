@@ -143,6 +143,19 @@ def test_attend_strides(cuda_device):
         assert (ob[:, 0] == 7).all() and (ob[:, :, 8] == 7).all() and (ob[..., :off] == 7).all() and (ob[..., off + D:] == 7).all()
 
 
+def test_attend_after_a_refusal(cuda_device):
+    """A refused call leaves nothing behind that a later one of the same shapes meets."""
+    c = Case(cuda_device, [300, 150], 1, 8, 2, 64, 6, "f16", "f16", seed=9)
+    tree, v = c.tree(), c.v
+    for bad in (v.float(), v[:, :, :-1], v[:, :1]):
+        c.v = bad
+        with pytest.raises(mm3fa.MM3FAError):
+            c.run(tree=tree)
+    c.v = v
+    c.check(c.run(tree=tree))
+    tree.check()
+
+
 def test_attend_strides_in_turn(cuda_device):
     """One tree with slabs of the same shape, first with rows that are not 16-byte aligned, then with aligned ones."""
     c = Case(cuda_device, [4000, 3000], 1, 8, 2, 128, 12, "f32", "f16", seed=8)
