@@ -53,7 +53,7 @@ constexpr int TS_LONG    = 32768;
 constexpr int TS_SPACE   = 256;  // bytes of the workspace before the list of units in parts
 constexpr int TS_LEAST   = 4;    // tiles of a part, at least: a part costs as much as about two tiles, and the joining kernel
 constexpr int TS_PIECES  = 4;    // pieces that warp 0 may be ahead
-constexpr int TS_COST    = 3;    // tiles' time that a unit takes beside them
+constexpr int TS_COST    = 5;    // tiles' time that a unit takes beside them
 constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for
 constexpr int TJ_WARPS   = 8;    // of a joining CTA
 constexpr int TJ_UNITS   = 512;  // units in parts, at most one a CTA: there are no more CTAs than SMs or blocks of a unit
@@ -1224,12 +1224,71 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     }
 }
 
-// Joins the parts of units, in their order: 32 rows and four columns by each warp, a row by each lane, the loads of 16 parts
-// in flight.  Every CTA finds the units in parts from what the first kernel's CTAs have left, and takes its share of all
-// (a CTA for each of those CTAs and each share of a unit: 2368 of them take longer to come and go than to work).
+// Joins the parts of a unit, in their order, for 32 rows, a row by each lane, and 4 * COLS columns from c4 on: the loads of
+// PER parts in flight.
+template <int COLS, int PER>
+__device__ __forceinline__ void ts_join(const TreeAttnParams & p, const TsJoin & t, int64_t step, int slot_rows, int D, int r, int c4) {
+    float  M = -INFINITY, l = 0.0f;
+    float4 o[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; c++) {
+        o[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+#pragma unroll 1
+    for (int k0 = 0; k0 < t.parts; k0 += PER) {
+        float2 x[PER];
+        float4 v[PER][COLS];
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            x[k] = make_float2(-INFINITY, 0.0f);
+            if (k0 + k < t.parts) {
+                const float * at = p.part + (k0 + k == 0 ? t.part0 : t.part1 + (k0 + k - 1) * step);
+                x[k] = reinterpret_cast<const float2 *>(at + slot_rows * D)[r];
+#pragma unroll
+                for (int c = 0; c < COLS; c++) {
+                    v[k][c] = reinterpret_cast<const float4 *>(at)[(c4 + c) * slot_rows + r];
+                }
+            }
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            top = fmaxf(top, x[k].x);
+        }
+        const float g = M == top ? 1.0f : ex2(M - top);
+        l *= g, M = top;
+#pragma unroll
+        for (int c = 0; c < COLS; c++) {
+            o[c].x *= g, o[c].y *= g, o[c].z *= g, o[c].w *= g;
+        }
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            if (k0 + k < t.parts) {
+                const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
+                l = fmaf(x[k].y, f, l);
+#pragma unroll
+                for (int c = 0; c < COLS; c++) {
+                    o[c].x = fmaf(v[k][c].x, f, o[c].x), o[c].y = fmaf(v[k][c].y, f, o[c].y);
+                    o[c].z = fmaf(v[k][c].z, f, o[c].z), o[c].w = fmaf(v[k][c].w, f, o[c].w);
+                }
+            }
+        }
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const int   row = (int) t.row0 + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
+    char *      to  = p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3;
+#pragma unroll
+    for (int c = 0; c < COLS; c++) {
+        ts_store4(to, 4 * (c4 + c), make_float4(o[c].x * inv, o[c].y * inv, o[c].z * inv, o[c].w * inv), p.o.type, p.o.vec);
+    }
+}
+
+// The joining kernel.  Every CTA finds the units in parts from what the first kernel's CTAs have left, and takes its share of
+// all (a CTA for each of those CTAs and each share of a unit: 2368 of them take longer to come and go than to work).  A warp
+// takes 32 rows and four columns of a unit where that gives each warp one turn: few units, of many parts.  Otherwise 16
+// columns at a time: the units on a line have two or three parts, and a turn is the wait for its loads.
 template <int D>
-__global__ void __launch_bounds__(32 * TJ_WARPS) tree_attn_join_kernel(const TreeAttnParams p, int ctas, int wide, int slot_rows) {
-    constexpr int  PER = 16;  // parts loaded at a time
+__global__ void __launch_bounds__(32 * TJ_WARPS, 2) tree_attn_join_kernel(const TreeAttnParams p, int ctas, int wide, int slot_rows) {
     __shared__ int list[TJ_UNITS], counts[TJ_WARPS];
     const int      tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     kv8_dep_wait();
@@ -1253,49 +1312,21 @@ __global__ void __launch_bounds__(32 * TJ_WARPS) tree_attn_join_kernel(const Tre
         }
         __syncthreads();
     }
-    const int quarters = (slot_rows + 31) / 32, per_unit = quarters * (D / 4);
-    for (int item = (int) blockIdx.x * TJ_WARPS + warp; item < n_units * per_unit; item += (int) gridDim.x * TJ_WARPS) {
+    const int     warps = (int) gridDim.x * TJ_WARPS, quarters = (slot_rows + 31) / 32;
+    const bool    few   = n_units * quarters * (D / 4) <= warps;
+    const int     per_unit = quarters * (few ? D / 4 : D / 16);
+    const int64_t step     = (int64_t) wide * 2 * ts_slot_floats(slot_rows, D);
+    for (int item = (int) blockIdx.x * TJ_WARPS + warp; item < n_units * per_unit; item += warps) {
         const TsJoin t = units[list[item / per_unit]];
-        const int    k4 = item % per_unit / quarters, r = item % quarters * 32 + lane;
+        const int    c = item % per_unit / quarters, r = item % quarters * 32 + lane;
         if (r >= t.rows) {
             continue;
         }
-        const int64_t step = (int64_t) wide * 2 * ts_slot_floats(slot_rows, D);
-        float         M = -INFINITY, l = 0.0f;
-        float4        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 1
-        for (int k0 = 0; k0 < t.parts; k0 += PER) {
-            float2 x[PER];
-            float4 v[PER];
-#pragma unroll
-            for (int k = 0; k < PER; k++) {
-                x[k] = make_float2(-INFINITY, 0.0f), v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (k0 + k < t.parts) {
-                    const float * at = p.part + (k0 + k == 0 ? t.part0 : t.part1 + (k0 + k - 1) * step);
-                    x[k] = reinterpret_cast<const float2 *>(at + slot_rows * D)[r];
-                    v[k] = reinterpret_cast<const float4 *>(at)[k4 * slot_rows + r];
-                }
-            }
-            float top = M;
-#pragma unroll
-            for (int k = 0; k < PER; k++) {
-                top = fmaxf(top, x[k].x);
-            }
-            const float g = M == top ? 1.0f : ex2(M - top);
-            l *= g, o.x *= g, o.y *= g, o.z *= g, o.w *= g, M = top;
-#pragma unroll
-            for (int k = 0; k < PER; k++) {
-                if (k0 + k < t.parts) {
-                    const float f = x[k].x == M ? 1.0f : ex2(x[k].x - M);
-                    l = fmaf(x[k].y, f, l);
-                    o.x = fmaf(v[k].x, f, o.x), o.y = fmaf(v[k].y, f, o.y), o.z = fmaf(v[k].z, f, o.z), o.w = fmaf(v[k].w, f, o.w);
-                }
-            }
+        if (few) {
+            ts_join<1, 10>(p, t, step, slot_rows, D, r, c);
+        } else {
+            ts_join<4, 2>(p, t, step, slot_rows, D, r, 4 * c);
         }
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        const int   row = (int) t.row0 + r, node = row / p.ratio, head = t.h * p.ratio + row - node * p.ratio;
-        ts_store4(p.o.data + (int64_t) head * p.o.nb1 + (int64_t) node * p.o.nb2 + (int64_t) t.s * p.o.nb3, 4 * k4,
-                  make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), p.o.type, p.o.vec);
     }
 }
 
