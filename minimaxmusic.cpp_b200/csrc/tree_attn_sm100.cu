@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     uint64_t * bar       = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
     int *      abort_f   = reinterpret_cast<int *>(smem + L::OFF_MISC + 4);
-    int *      dirty     = reinterpret_cast<int *>(smem + L::OFF_MISC + 8);  // [2 pieces] a V row of a node held what is no number
+    int *      dirty     = reinterpret_cast<int *>(smem + L::OFF_MISC + 8);  // [4 pieces] a V row of a node held what is no number
     float *    factors   = reinterpret_cast<float *>(smem + L::OFF_F);
     float2 *   ml        = reinterpret_cast<float2 *>(smem + L::OFF_ML);
     uint32_t * anc       = reinterpret_cast<uint32_t *>(smem + L::OFF_ANC);
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         for (int i = 0; i < TB_COUNT; i++) {
             mbar_init(&bar[i], ts_arrivals(i));
         }
-        *abort_f = 0, dirty[0] = 0, dirty[1] = 0;
+        *abort_f = 0, dirty[0] = 0, dirty[1] = 0, dirty[2] = 0, dirty[3] = 0;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         }
                     }
                     if (odd) {
-                        atomicExch(&dirty[pieces & 1], 1);
+                        atomicExch(&dirty[pieces & 3], 1);
                     }
                     fence_proxy_async_smem();
                     dn_mbar_arrive(&bar[TB_FIX]);
@@ -842,7 +842,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         const uint32_t tl    = (uint32_t) (quad * 32) << 16;
         const uint32_t s_col = tmem + tl + (uint32_t) (w * TS_N), o_col = tmem + tl + 256u + (uint32_t) (w * D);
         const bool     cap = p.softcap > 0.0f;
-        float4 *       give = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + w * (TS_M * 4), *take = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + (w ^ 1) * (TS_M * 4);
+        float4 *       turn = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + w * (TS_M * 4);  // 16 columns of a warp's rows, on their way out
         uint32_t       tc = 0, used = 0;
         bool           ok = true;
         auto           wait = [&](int b, uint32_t i) {
@@ -855,6 +855,11 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         while (softmax_all(ts_take(told, bar, pieces, deadline))) {
             // (read where it is needed: the sums leave few registers)
             const TsPiece & it = told[pieces % TS_PIECES];
+            if (own == 0) {
+                // of the piece before, which all have left: that place's next piece, the third from here, cannot have been looked
+                // at before all came through the loop's head again
+                dirty[(pieces + 3) & 3] = 0;
+            }
             const int       tile0 = it.a, tile1 = it.b, held = it.L;
             const int       row = it.rb * TS_M + r, my_node = row / p.ratio;
             const uint32_t * bits = anc + min(my_node, TREE_MAX - 1) * (TREE_MAX / 32);
@@ -1109,7 +1114,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             if (PARTS == 1 && any) {
                 wait(TB_OFULL + w, used++);
             }
+            tc_fence_before();
             softmax_barrier();
+            tc_fence_after();
             const float2 other = ml[(w ^ 1) * TS_M + r];
             const float  M = fmaxf(m, other.x), mine_f = m == M ? 1.0f : ex2(m - M), other_f = other.x == M ? 1.0f : ex2(other.x - M);
             l = w == 0 ? fmaf(l, mine_f, other.y * other_f) : fmaf(other.y, other_f, l * mine_f);
@@ -1126,38 +1133,24 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             if (!whole && live && w == 0) {  // behind the slot's rows
                 reinterpret_cast<float2 *>(al + (int64_t) slot_rows * D * 4)[r] = make_float2(M, l);
             }
-            // ---- the sums: each stream takes half of the columns, 16 at a time, and stores them by whole rows
-            const bool odd = tail && dirty[pieces & 1] && live;
-            auto       columns = [&](int c, uint32_t (&o)[16]) {  // of this stream's sums, 16 from c on
-                tmem_ld16(o_col + (uint32_t) c, o);
-                tmem_ld16_wait(o);
-                if (PARTS == 1 && !any) {  // (what is there is not the piece's)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        o[e] = 0u;
-                    }
-                }
-            };
-            const int swz = (r >> 1) & 3;
+            // ---- the sums: each stream takes half of the columns of both, 16 at a time, and stores them by whole rows (a
+            // warpgroup's warps reach the lanes of the other's; the loop's head holds the next piece's products back)
+            const bool odd = tail && dirty[pieces & 3] && live;
+            // (PARTS 1: what is there is the piece's where the stream had a tile of it)
+            const bool mine_is = PARTS == 2 || any, theirs_is = PARTS == 2 || !any || tile1 - tile0 > 1;
+            const int  swz = (r >> 1) & 3;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
-                uint32_t o[16];
-                const int theirs = (w ^ 1) * (D / 2) + c * 16, mine = w * (D / 2) + c * 16;
-                columns(theirs, o);
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    give[r * 4 + (k ^ swz)] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
-                }
-                softmax_barrier();
-                columns(mine, o);
+                const int mine = w * (D / 2) + c * 16;
+                uint32_t  o[16], q[16];
+                tmem_ld16(tmem + tl + 256u + (uint32_t) (w * D + mine), o);
+                tmem_ld16(tmem + tl + 256u + (uint32_t) ((w ^ 1) * D + mine), q);
+                tmem_ld16_wait(o);
+                tmem_ld16_wait(q);
                 float x[16];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float4 f = take[r * 4 + (k ^ swz)];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[4 * k + e] = __uint_as_float(o[4 * k + e]) * mine_f + (&f.x)[e] * other_f;
-                    }
+                for (int e = 0; e < 16; e++) {
+                    x[e] = (mine_is ? __uint_as_float(o[e]) * mine_f : 0.0f) + (theirs_is ? __uint_as_float(q[e]) * other_f : 0.0f);
                 }
                 if (odd) {
                     // elements that are no numbers, of nodes that the row sees: they were left out of the products
@@ -1175,7 +1168,6 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         }
                     }
                 }
-                softmax_barrier();  // (what this stream gave has been taken: its place holds the rows now)
                 if (!whole && live) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
@@ -1185,13 +1177,13 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 if (whole && warp_live) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        give[r * 4 + (k ^ swz)] = make_float4(x[4 * k] * inv, x[4 * k + 1] * inv, x[4 * k + 2] * inv, x[4 * k + 3] * inv);
+                        turn[r * 4 + (k ^ swz)] = make_float4(x[4 * k] * inv, x[4 * k + 1] * inv, x[4 * k + 2] * inv, x[4 * k + 3] * inv);
                     }
                     __syncwarp();
 #pragma unroll 1
                     for (int i = lane >> 2; i < 32; i += 8) {
                         const int    k = lane & 3;
-                        const float4 f = give[(quad * 32 + i) * 4 + (k ^ ((i >> 1) & 3))];
+                        const float4 f = turn[(quad * 32 + i) * 4 + (k ^ ((i >> 1) & 3))];
                         char *       to = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, al, i));
                         if (quad * 32 + i < it.rows) {
                             ts_store4(to, mine + k * 4, f, p.o.type, p.o.vec);
@@ -1201,9 +1193,6 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
             }
             tc_fence_before();
-            if (own == 0) {
-                dirty[pieces & 1] = 0;  // (set again two pieces on, when this thread has been through the next)
-            }
             ts_drop(bar, pieces, lane);
             pieces++;
         }
