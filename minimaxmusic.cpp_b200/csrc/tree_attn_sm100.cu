@@ -793,33 +793,35 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         ok = false;
                     }
                     char *    tile = smem + L::OFF_RING + slot * L::KT;
-                    const int r0 = max(0, it.L - j * TS_N), end = it.keys - j * TS_N;
-                    bool      odd = false;
+                    // A thread has the same 16 bytes of every STEP-th row.  One more in an exponent of ones alone sets the
+                    // bit above it, which is how a word's halves are told from numbers (compared one by one: 2 us a tile, and
+                    // the product and the next piece's Q wait for this).
+                    constexpr int      PER_ROW = 8 * L::HALVES, STEP = 64 / PER_ROW;
+                    constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = BF16 ? 0x00800080u : 0x04000400u;
+                    const int          ck = t64 % PER_ROW, end = min(it.keys - j * TS_N, TS_N);
+                    char *             col = tile + (ck >> 3) * (TS_N * 128) + (ck & 7) * 16;
+                    const int          first = max(0, it.L - j * TS_N) + t64 / PER_ROW;
+                    bool               odd = false;
 #pragma unroll 1
-                    for (int e = t64; e < (TS_N - r0) * 8 * L::HALVES; e += 64) {
-                        const int r  = r0 + e / (8 * L::HALVES), ck = e % (8 * L::HALVES);
-                        uint4 *   at = reinterpret_cast<uint4 *>(tile + (ck >> 3) * (TS_N * 128) + r * 128 + (ck & 7) * 16);
-                        if (r >= end) {
-                            *at = make_uint4(0, 0, 0, 0);
-                            continue;
-                        }
-                        uint4              w    = *at;
-                        constexpr uint32_t EXP  = BF16 ? 0x7f80u : 0x7c00u;
-                        bool               here = false;
+                    for (int row = first; row < end; row += 4 * STEP) {
+                        uint32_t no = 0;
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            uint32_t & u = (&w.x)[k];
-                            if ((u & EXP) == EXP) {
-                                u &= 0xffff0000u, here = true;
-                            }
-                            if ((u >> 16 & EXP) == EXP) {
-                                u &= 0xffffu, here = true;
-                            }
+                        for (int k = 0; k < 4; k++) {  // (past the end: the row is looked at once more)
+                            const uint4 u = *reinterpret_cast<const uint4 *>(col + (row + k * STEP < end ? row + k * STEP : row) * 128);
+                            no |= ((u.x & EXP) + ONE) | ((u.y & EXP) + ONE) | ((u.z & EXP) + ONE) | ((u.w & EXP) + ONE);
                         }
-                        if (here) {
-                            *at = w;
+                        if (no & 0x80008000u) {
                             odd = true;
+#pragma unroll 1
+                            for (int k = 0; k < 16 && row + (k >> 2) * STEP < end; k++) {
+                                uint32_t * at = reinterpret_cast<uint32_t *>(col + (row + (k >> 2) * STEP) * 128) + (k & 3);
+                                *at &= ~__vcmpeq2(*at & EXP, EXP);
+                            }
                         }
+                    }
+#pragma unroll 1
+                    for (int row = first + max(0, (end - first + STEP - 1) / STEP) * STEP; row < TS_N; row += STEP) {
+                        *reinterpret_cast<uint4 *>(col + row * 128) = make_uint4(0, 0, 0, 0);
                     }
                     if (odd) {
                         atomicExch(&dirty[pieces & 3], 1);
