@@ -5,10 +5,12 @@
 // query heads of a kv head and the nodes share each K/V tile of 128 keys.  One CTA per SM.  Where all trees have the same
 // nodes, the CTAs with a unit's blocks are a group, beside one another, that walks the same keys at the same time, so that
 // a K/V tile comes from HBM once; where each tree says how many it has, the blocks are units of their own, since a group's CTAs
-// would have nothing to do for the smaller trees (8 trees of up to 200 nodes: 128 us in groups of 7).
+// would have nothing to do for the smaller trees (8 trees of up to 200 nodes, before later steps: 128 us in groups of 7, 99 as
+// units).
 //
 // Split, found on the device from the lengths, so that a captured call follows them:
-//   units up to groups   every unit in even parts of about the same size, one part a group (TsPlan)
+//   units up to groups   every unit in even parts of about the same size, one part a group (TsPlan; 2 sequences of 8192: 30 us,
+//                        37 on a line; of 97 and 311: 17 and 32)
 //   more units           the tiles of all units are one line, in the order of sequence and kv head, and each group takes an
 //                        equal piece of it: whole units, and a part of one at either end
 // A part of a unit leaves O, m and l in the workspace, and a second kernel joins the parts in their order: by the last
@@ -29,7 +31,13 @@
 // each step of 16 keys, always towards zero (measured 7e-7 a tile of 128 keys): up to TS_LONG keys a stream's sum stays within
 // 1e-4, a fifth of F16's half step.  Else (PARTS 2) q is two parts of the cache's type (F16: brought to [2^14, 2^15) at its row's largest
 // element by a power of two), and so are the weights, the remainder's product first, where the accumulator is small;
-// every tile's P V starts afresh and is added in registers, rounded to nearest.
+// every tile's P V starts afresh and is added in registers, rounded to nearest: 22 bits of q and weights in F16, 16 in BF16 (an
+// F32 result is off by 5e-7 and 3.5e-6 of its norm; a third part would not fit in TMEM beside S and O of two tiles).  PARTS 1
+// takes 22 us at 2 x 8192 and 24 nodes (BF16) where PARTS 2 takes 31, and 32 at 64 nodes where that takes 49.
+//
+// Bound: HBM for batches (48 sequences of 1 to 10240, BF16: 165 us, 1013 MB at 6.1 TB/s); few sequences the start (plan 2.7 us, Q
+// 6, first S 7.6) and the joining (7); many nodes each stream's chain of S, weights, P V (2 us a tile, the tensor pipe 38%
+// active), and the ends of pieces (8 trees of up to 200 nodes over 1900-4100 tokens: 80 us for 45.6 GFLOP).
 //
 // Most of the code runs once in a CTA, and its first run costs what the instruction cache costs: what does not feed the
 // tensor core is in rolled loops or functions (a Q staging unrolled over all rows took 5 us, 3.5 as it is).
@@ -48,13 +56,12 @@ constexpr int TS_M       = 128;  // rows of a block
 constexpr int TS_N       = 128;  // keys of a tile
 constexpr int TS_TMEM    = 512;  // columns: S of two tiles, P V of two tiles
 constexpr int TS_GROW    = 7;    // (PARTS 1) log2 of what a weight may exceed the maximum of the tiles before by
-constexpr int TS_EMU     = 2;    // (PARTS 1) of every 8 pairs of weights, those by polynomial: the special-function unit is the bound
 constexpr int TS_LONG    = 32768;
 constexpr int TS_SPACE   = 256;  // bytes of the workspace before the list of units in parts
-constexpr int TS_LEAST   = 4;    // tiles of a part, at least: a part costs as much as about two tiles, and the joining kernel
+constexpr int TS_LEAST   = 3;    // tiles of a part, at least (8 trees of up to 200 nodes: 79 us, 82 with 4, 85 with 8)
 constexpr int TS_PIECES  = 4;    // pieces that warp 0 may be ahead
 constexpr int TS_COST    = 5;    // tiles' time that a unit takes beside them
-constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for
+constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for: five for each lane
 constexpr int TJ_WARPS   = 8;    // of a joining CTA
 constexpr int TJ_UNITS   = 512;  // units in parts, at most one a CTA: there are no more CTAs than SMs or blocks of a unit
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
@@ -1005,7 +1012,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             for (int i = 0; i < 16; i++) {
                                 float x, y;
                                 f2unpack(ffma2(f2pack(__uint_as_float(v[c * 32 + 2 * i]), __uint_as_float(v[c * 32 + 2 * i + 1])), fa2, nm2), x, y);
-                                const uint64_t p2 = (i & 7) < TS_EMU ? exp2_poly2(f2pack(x, y)) : f2pack(ex2(x), ex2(y));
+                                const uint64_t p2 = f2pack(ex2(x), ex2(y));
                                 sum2 = fadd2(sum2, p2);
                                 f2unpack(p2, x, y);
                                 hi[i] = ts_pack<BF16>(x, y);
