@@ -294,6 +294,26 @@ def test_attend_many_short_pieces(cuda_device, lens, dtype, cache):
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f32", "f16")])
+def test_attend_infinite_values_in_some_of_many(cuda_device, dtype, cache):
+    """Many units for every CTA, some with an infinite V element in a node's row: the units before and after them, of the same
+    CTA, are as without it."""
+    N, T = 120, 5
+    c = Case(cuda_device, [(i * 29) % 90 for i in range(N)], 1, 8, 8, 64, T, dtype, cache, seed=18, parents=[[-1, 0, 0, 1, 1]])
+    want = c.check().clone()
+    v = c.v.clone()
+    some = [i for i in range(N) if i % 5 in (1, 2)]
+    for i in some:
+        v[i, :, int(c.len[i]) + 1, 7] = float("inf")  # seen by nodes 1, 3 and 4
+    tree = c.tree()
+    for _ in range(5):
+        got = tree.attend(c.q, c.k, v, c.len, c.scale, out=c.out())
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[torch.tensor(some)[:, None], torch.tensor([1, 3, 4]), :, 7] = True
+        assert (got[hit] == float("inf")).all() and torch.equal(got[~hit], want[~hit])
+    tree.check()
+
+
 def test_attend_on_streams_and_in_graphs(cuda_device):
     """Two streams at once, a given stream, and two graphs replayed side by side with other lengths and trees."""
     c = Case(cuda_device, [3000, 1200], 1, 16, 4, 128, 20, "f32", "f16", seed=14)
@@ -521,6 +541,15 @@ def test_commit(cuda_device, L, N, n_tree, Hkv, D, T, cache):
     counts = [max(1, T - 3 * t) if t % 2 else max(1, T // 3) for t in range(n_tree)]
     k, v = (slabs(cuda_device, L, N, Hkv, T + 60, D, cache, seed) for seed in (1, 2))
     check_commit(cuda_device, k, v, [rising(rng, T, n) for n in counts], counts, [rng.randint(0, 60) for _ in range(N)])
+
+
+@pytest.mark.parametrize("L,N,Hkv", [(37, 64, 8), (97, 65, 5), (13, 1200, 8)])
+def test_commit_many_sets_and_layers(cuda_device, L, N, Hkv):
+    """More sets, heads and layers than there are warps: some take one layer more than others."""
+    rng = random.Random(L)
+    counts = [1 + i % 5 for i in range(N)]
+    k, v = (slabs(cuda_device, L, N, Hkv, 20, 64, "f16", seed) for seed in (5, 6))
+    check_commit(cuda_device, k, v, [rising(rng, 9, n) for n in counts], counts, [rng.randint(0, 12) for _ in range(N)])
 
 
 def test_commit_paths_that_end_early(cuda_device):
