@@ -35,9 +35,9 @@
 // F32 result is off by 5e-7 and 3.5e-6 of its norm; a third part would not fit in TMEM beside S and O of two tiles).  PARTS 1
 // takes 22 us at 2 x 8192 and 24 nodes (BF16) where PARTS 2 takes 31, and 32 at 64 nodes where that takes 49.
 //
-// Bound: HBM for batches (48 sequences of 1 to 10240, BF16: 165-187 us by where
-// the slabs lie, 1013 MB at 5.4-6.1 TB/s); few sequences the start (plan 2.7 us, Q
-// 6, first S 7.6) and the joining (7); many nodes each stream's chain of S, weights, P V (2 us a tile, the tensor pipe 38%
+// Bound: HBM for batches at full clock (48 sequences of 1 to 10240, 13 nodes, BF16, 1013 MB: 166 us, 6.1 TB/s, at 1965 MHz; under a
+// lasting load the power cap takes the clock to 1430-1550 MHz, and the tiles' own work counts too: 177-188); few sequences
+// the start (plan 2.7 us, Q 6, first S 7.6) and the joining (7); many nodes each stream's chain of S, weights, P V (2 us a tile, the tensor pipe 38%
 // active), and the ends of pieces (8 trees of up to 200 nodes over 1900-4100 tokens: 80 us for 45.6 GFLOP).
 //
 // Most of the code runs once in a CTA, and its first run costs what the instruction cache costs: what does not feed the
