@@ -65,6 +65,7 @@ constexpr int TS_COST    = 5;    // tiles' time that a unit takes beside them
 constexpr int TS_EVEN    = 160;  // sequences for which even parts are looked for: five for each lane
 constexpr int TJ_WARPS   = 8;    // of a joining CTA
 constexpr int TJ_UNITS   = 512;  // units in parts, at most one a CTA: there are no more CTAs than SMs or blocks of a unit
+constexpr float TS_MOST       = 3.402823466e38f;  // F32's largest number
 constexpr int TS_REGS_LAUNCH  = 168;  // 65536 / 384, a multiple of 8
 constexpr int TS_REGS_SOFTMAX = 208;  // 2 x 208 + 88 = 3 x 168
 constexpr int TS_REGS_ISSUE   = 88;
@@ -477,8 +478,9 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
     // lane i, and 16 + i: the address of row i (of the last one, behind it)
     const int      rl = it.rb * TS_M + max(min(ra + (lane & 15), it.rows - 1), 0), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
     const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
-    // (not 0, whose product with the -inf of a key that is not seen would be no number)
-    const float    by = fmaxf(fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E), 0x1p-126f);
+    // what a score is multiplied by is above 0 and finite: 0 by the -inf of a key that is not seen, and an infinity by a score of
+    // 0, would be no number
+    const float    by = fminf(fmaxf(fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E), 0x1p-126f), TS_MOST);
     // chunk ck of 16 bytes of row i: block ck / 8 of 64 columns (F32: the two blocks of either part in turn)
     auto place = [&](int i, int ck) {
         const int blk = ck >> 3;
@@ -568,7 +570,8 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
                     reinterpret_cast<uint32_t *>(to + QT)[e] = lo[e];
                 }
                 if (lane == 0) {
-                    factors[ra + i0 + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
+                    // (2^-149 for a product below F32's smallest number: the scores are 0 in effect)
+                    factors[ra + i0 + i] = odd ? NAN : fminf(fmaxf(__uint_as_float((uint32_t) (127 + ex) << 23) * by, 0x1p-149f), TS_MOST);
                 }
             }
         }
