@@ -1350,9 +1350,12 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
         return e;
     }
     alignas(64) CUtensorMap tmk, tmv;
-    if (!encode_kv_tensor_map(&tmk, p.k.data, BF16, D, p.n_kv, p.n_head_kv, p.n_seq, p.k.nb1, p.k.nb2, p.k.nb3, TS_N) ||
-        !encode_kv_tensor_map(&tmv, p.v.data, BF16, D, p.n_kv, p.n_head_kv, p.n_seq, p.v.nb1, p.v.nb2, p.v.nb3, TS_N)) {
-        return cudaErrorInvalidValue;
+    for (CUtensorMap * tm : { &tmk, &tmv }) {
+        const Kv8Rows & x = tm == &tmk ? p.k : p.v;
+        // (the stride of a slab's only row is never stepped, and may be one that a map does not take)
+        if (!encode_kv_tensor_map(tm, x.data, BF16, D, p.n_kv, p.n_head_kv, p.n_seq, p.n_kv > 1 ? x.nb1 : 2 * D, x.nb2, x.nb3, TS_N)) {
+            return cudaErrorInvalidValue;
+        }
     }
     const int wide = tree_attn_wide(p), groups = tree_attn_groups(p, sms);
     const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);

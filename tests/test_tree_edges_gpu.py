@@ -25,3 +25,19 @@ def test_attend_scales_whose_products_leave_f32(cuda_device, D, dtype, cache):
     c.q = torch.zeros_like(q)
     for kw in ({"scale": 3e38}, {"scale": -3e38}, {"scale": 1e30, "logit_softcap": 1e-20}):
         c.check(**kw)
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+def test_attend_slabs_of_one_row(cuda_device, which, dtype, cache):
+    """n_kv = 1: the row stride is never used, whatever it is (262 bytes are not a multiple of 16, 0 is below a row)."""
+    for N, Hkv in ((2, 2), (1, 1), (3, 1), (1, 2)):
+        for row in (131, 0):
+            c = Case(cuda_device, [i % 2 for i in range(N)], 1, 2 * Hkv, Hkv, 128, 3, dtype, cache, seed=N, rows=1)
+            for name in which:
+                x = getattr(c, name)
+                big = torch.full((N, Hkv, 8, 131), float("nan"), dtype=x.dtype, device=cuda_device)
+                view = big.as_strided((N, Hkv, 1, 128), (Hkv * 8 * 131, 8 * 131, row, 1))
+                view.copy_(x)
+                setattr(c, name, view)
+            c.check()
