@@ -661,7 +661,8 @@ MM3FA_API int mm3fa_tree_verify(const mm3fa_tensor * logits, const mm3fa_tensor 
  *           of K with the same strides, and those of V
  *   path, n_path   as mm3fa_tree_verify leaves them, [n_tree][max_nodes] and [n_tree]; a path ends at an entry that is not
  *           above the one before it or names no row, and counts up to there
- *   kv_len, kv_len_out  device int32 [n_seq], not in the same memory; a sequence of negative length keeps it
+ *   kv_len, kv_len_out  device int32 [n_seq], kv_len_out in none of the memory of kv_len, path and n_path; a sequence of
+ *           negative length keeps it
  */
 MM3FA_API int mm3fa_tree_commit(const mm3fa_tensor * k, const mm3fa_tensor * v, int n_layers, const int32_t * path,
                                 const int32_t * n_path, int max_nodes, int n_tree, const int32_t * kv_len,

@@ -286,8 +286,10 @@ int mm3fa_tree_commit(const mm3fa_tensor * k, const mm3fa_tensor * v, int n_laye
             return MM3FA_ERR_ALIGN;
         }
     }
-    // every unit reads the lengths that one of them replaces
-    if (overlap(kv_len, 4 * (size_t) S, kv_len_out, 4 * (size_t) S)) {
+    // every unit, and every launch of more than TREE_LAYERS layers, reads what one of them would replace
+    const size_t out_bytes = 4 * (size_t) S, trees = (size_t) n_tree;
+    if (overlap(kv_len, out_bytes, kv_len_out, out_bytes) || overlap(n_path, 4 * trees, kv_len_out, out_bytes) ||
+        overlap(path, 4 * trees * (size_t) max_nodes, kv_len_out, out_bytes)) {
         return MM3FA_ERR_UNSUPPORTED;
     }
     if (host_device_major() != 10) {

@@ -194,7 +194,7 @@ class DraftTree(OnDevice):
 
     def commit(self, layers, path, n_path, kv_len, kv_len_out=None, stream=None):
         """Moves the rows of the nodes on each path behind the cached tokens, in all of `layers` (CacheLayers), and returns
-        the new lengths (in kv_len_out where it is given; it may not be kv_len)."""
+        the new lengths (in kv_len_out where it is given; it may not be in the memory of kv_len, path or n_path)."""
         if stream is not None:
             with self._on(stream):
                 return self.commit(layers, path, n_path, kv_len, kv_len_out)
