@@ -616,8 +616,8 @@ MM3FA_API size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_t
  * itself and its ancestors j.
  *   q       F32, F16 or BF16 [D, max_nodes, n_head, n_seq], any strides along dims 1 to 3
  *   k, v    F16, BF16, Q8_0 or F32 [D, n_kv, n_head_kv, n_seq], of one type, any strides along dims 1 to 3
- *   dst     [D, n_head, max_nodes, n_seq], F32 or q's type, not in q's memory; rows of nodes that do not count are left as
- *           they were
+ *   dst     [D, n_head, max_nodes, n_seq], F32 or q's type, not in q's memory, which is refused (rows of both in turn in one
+ *           buffer are told apart where they have the same strides); rows of nodes that do not count are left as they were
  *   kv_len  device int32 [n_seq], clamped to [0, n_kv]; rows from n_kv on are absent
  *   logit_softcap  0 disables; otherwise s <- softcap * tanh(s / softcap)
  *   workspace      its first 64 KiB zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this

@@ -91,6 +91,53 @@ bool overlap(const void * a, size_t a_bytes, const void * b, size_t b_bytes) {
     return x < y + b_bytes && y < x + a_bytes;
 }
 
+// Whether a row of `a` and one of `b` share bytes, told from their extents, and, where these cross, for tensors whose strides
+// are the same along each dimension (`of_b`: b's dimension of a's) and those above another's extent: rows in turn in one buffer.
+// Others are taken to share some.
+bool rows_share(const mm3fa_tensor * a, const mm3fa_tensor * b, const int (&of_b)[4]) {
+    const int64_t wa = row_bytes(a->type, a->ne[0]), wb = row_bytes(b->type, b->ne[0]);
+    int64_t       from_a = 0, end_a = wa, from_b = 0, end_b = wb;  // from the first row (strides may lead down)
+    int           dims[3], n = 0;
+    bool          alike = true;
+    for (int i = 1; i < 4; i++) {
+        const int     j = of_b[i];
+        const int64_t ea = (a->ne[i] - 1) * (int64_t) a->nb[i], eb = (b->ne[j] - 1) * (int64_t) b->nb[j];
+        (ea < 0 ? from_a : end_a) += ea, (eb < 0 ? from_b : end_b) += eb;
+        if (a->ne[i] > 1) {
+            alike     = alike && a->nb[i] == b->nb[j];
+            dims[n++] = i;
+        }
+    }
+    // a's first row from b's
+    const int64_t d = (int64_t) (reinterpret_cast<uintptr_t>(a->data) - reinterpret_cast<uintptr_t>(b->data));
+    if (d + from_a >= end_b || d + end_a <= from_b) {
+        return false;
+    }
+    std::sort(dims, dims + n, [&](int x, int y) { return (int64_t) a->nb[x] > (int64_t) a->nb[y]; });
+    int64_t below = std::max(wa, wb);  // of a row, or of the dimensions of smaller strides
+    for (int k = n - 1; k >= 0; k--) {
+        alike = alike && (int64_t) a->nb[dims[k]] >= below;
+        below = (a->ne[dims[k]] - 1) * (int64_t) a->nb[dims[k]] + below;
+    }
+    if (!alike) {
+        return true;
+    }
+    // Differences of two rows' places: d + sum of t_i nb_i, |t_i| < ne_i.  What the smaller strides add is less than a stride, so
+    // that of each t_i two values can bring it near 0
+    for (int pick = 0; pick < 1 << n; pick++) {
+        int64_t x = d;
+        for (int k = 0; k < n; k++) {
+            const int64_t nb = (int64_t) a->nb[dims[k]], most = a->ne[dims[k]] - 1;
+            const int64_t t  = -(x >= 0 ? x / nb : -((-x + nb - 1) / nb)) - (pick >> k & 1);
+            x += std::min(std::max(t, -most), most) * nb;
+        }
+        if (x < wb && -x < wa) {
+            return true;
+        }
+    }
+    return false;
+}
+
 // The attention's operands; fills its parameters but for the workspace.
 int prepare_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v, const mm3fa_tree * tree, TreeAttnParams & p) {
     int st = check_tree(tree);
@@ -164,6 +211,9 @@ int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_
     }
     if (!aligned_to(kv_len, 4)) {
         return MM3FA_ERR_ALIGN;
+    }
+    if (rows_share(q, dst, { 0, 2, 1, 3 })) {  // a CTA may still have to read what another writes
+        return MM3FA_ERR_UNSUPPORTED;
     }
     if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < mm3fa_tree_attn_workspace(q, k, v, tree)) {
         return MM3FA_ERR_WORKSPACE;

@@ -142,8 +142,8 @@ class DraftTree(OnDevice):
     def attend(self, q, k, v, kv_len, scale, out=None, logit_softcap=0.0, ws=None, stream=None):
         """softmax(scale * q k^T) v of the queries q (N, n_head, T, D), where node i of a sequence sees the first kv_len[s]
         rows of its slabs k, v (N, n_head_kv, rows, D), and row kv_len[s] + j for itself and its ancestors j.
-        out: (N, T, n_head, D), F32 or q's type; made in q's type when not given, with zeros in the rows of nodes that do
-        not count.  ws: a uint8 tensor, its first 64 KiB zero, instead of this object's own workspace of the stream; it serves
+        out: (N, T, n_head, D), F32 or q's type, not in q's memory; made in q's type when not given, with zeros in the rows of
+        nodes that do not count.  ws: a uint8 tensor, its first 64 KiB zero, instead of this object's own workspace of the stream; it serves
         one stream at a time.  (Calls in a capture that torch.cuda.graph has not begun need one.)"""
         if stream is not None:  # what is allocated here belongs to that stream too
             with self._on(stream):

@@ -23,3 +23,36 @@ def test_commit_refuses_lengths_in_memory_that_it_reads():
         for start, want in ((at - N, mm3fa.ERR_DEVICE), (at - 1, mm3fa.ERR_UNSUPPORTED), (at + size - 1, mm3fa.ERR_UNSUPPORTED), (at + size, mm3fa.ERR_DEVICE)):
             if start >= 0:
                 assert a(mem[start:start + N]) == want, (at, start)
+
+
+@no_gpu
+def test_attend_refuses_results_in_the_queries_memory():
+    """A result's row in memory of a query's, which another CTA may still have to read; rows between one another's are fine."""
+    N, H, T, D = 2, 4, 5, 64
+    t, k, n, ws = mm3fa.DraftTree(ints(1, T)), torch.zeros(N, 2, 30, D), ints(N), torch.zeros(1 << 24, dtype=torch.uint8)
+    a = lambda q, out: status(t.attend, q, k, k, n, 0.1, out=out, ws=ws)
+    mem = torch.zeros(8 * N * T * H * D)
+    rows = lambda at, sn, st, sh: mem.as_strided((N, T, H, D), (sn, st, sh, 1), at)
+    whole = (T * H * D, H * D, D)
+    size = N * T * H * D
+    q = rows(size, *whole).transpose(1, 2)
+    for at, want in ((0, mm3fa.ERR_DEVICE), (2 * size, mm3fa.ERR_DEVICE), (size, mm3fa.ERR_UNSUPPORTED), (1, mm3fa.ERR_UNSUPPORTED),
+                     (2 * size - 1, mm3fa.ERR_UNSUPPORTED), (size + D, mm3fa.ERR_UNSUPPORTED)):
+        assert a(q, rows(at, *whole)) == want, at
+    # queries and results in turn in one buffer: by rows, by nodes, by sequences
+    for strides, offs in (((2 * T * H * D, 2 * H * D, 2 * D), D), ((2 * T * H * D, 2 * H * D, D), H * D), ((2 * T * H * D, H * D, D), T * H * D)):
+        q = rows(0, *strides).transpose(1, 2)
+        assert a(q, rows(offs, *strides)) == mm3fa.ERR_DEVICE
+        for off in (0, offs - 1, offs + 1):
+            assert a(q, rows(off, *strides)) == mm3fa.ERR_UNSUPPORTED, (strides, off)
+    # a 16-bit query's F32 result is twice as wide
+    half = mem.half()
+    q = half.as_strided((N, T, H, D), (4 * T * H * D, 4 * H * D, 4 * D, 1)).transpose(1, 2)
+    f32 = lambda at: half.view(torch.float32).as_strided((N, T, H, D), (2 * T * H * D, 2 * H * D, 2 * D, 1), at)
+    assert a(q, f32(D // 2)) == mm3fa.ERR_DEVICE and a(q, f32(D)) == mm3fa.ERR_DEVICE
+    assert a(q, f32(0)) == mm3fa.ERR_UNSUPPORTED and a(q, f32(D // 2 - 1)) == mm3fa.ERR_UNSUPPORTED and a(q, f32(D + 1)) == mm3fa.ERR_UNSUPPORTED
+    # one query for all heads or nodes
+    q = mem[:D].expand(N, H, T, D)
+    assert a(q, rows(D, *whole)) == mm3fa.ERR_DEVICE and a(q, rows(D - 1, *whole)) == mm3fa.ERR_UNSUPPORTED
+    q = rows(3 * D, 0, 0, 0).transpose(1, 2)
+    assert a(q, rows(0, *whole)) == mm3fa.ERR_UNSUPPORTED
