@@ -658,7 +658,7 @@ MM3FA_API int mm3fa_tree_verify(const mm3fa_tensor * logits, const mm3fa_tensor 
  * Moves the accepted nodes' rows behind the cached tokens: in every layer, for K and V, row kv_len[s] + path[i] goes to
  * row kv_len[s] + i, in place, and kv_len_out[s] = kv_len[s] + n_path.
  *   k, v    n_layers tensors each, [D, rows, n_head_kv, n_seq] F32, F16, BF16 or Q8_0; all of one type and shape, those
- *           of K with the same strides, and those of V
+ *           of K with the same strides, and those of V; a slab named more than once (layers that share one) is moved once
  *   path, n_path   as mm3fa_tree_verify leaves them, [n_tree][max_nodes] and [n_tree]; a path ends at an entry that is not
  *           above the one before it or names no row, and counts up to there
  *   kv_len, kv_len_out  device int32 [n_seq], kv_len_out in none of the memory of kv_len, path and n_path; a sequence of

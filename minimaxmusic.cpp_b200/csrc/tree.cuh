@@ -45,7 +45,7 @@ struct TreeVerifyParams {
 };
 
 struct TreeCommitParams {
-    char *      k[TREE_LAYERS];
+    char *      k[TREE_LAYERS];  // null: a slab that was named before, which is moved once
     char *      v[TREE_LAYERS];
     int64_t     k_nb1, k_nb2, k_nb3, v_nb1, v_nb2, v_nb3;
     int         row_bytes;

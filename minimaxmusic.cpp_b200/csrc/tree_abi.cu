@@ -91,6 +91,31 @@ bool overlap(const void * a, size_t a_bytes, const void * b, size_t b_bytes) {
     return x < y + b_bytes && y < x + a_bytes;
 }
 
+// Whether the K slab (V slab) of layer l is one that the list names before: layers that share their cache.  `apart`: none is.
+bool named_before(const mm3fa_tensor * k, const mm3fa_tensor * v, int l, bool of_v, bool apart) {
+    if (apart) {
+        return false;
+    }
+    const void * x = of_v ? v[l].data : k[l].data;
+    const bool   alike = k->nb[1] == v->nb[1] && k->nb[2] == v->nb[2] && k->nb[3] == v->nb[3];
+    for (int i = 0; i < l; i++) {
+        if ((of_v ? v : k)[i].data == x || (alike && (of_v ? k : v)[i].data == x)) {
+            return true;
+        }
+    }
+    return of_v && alike && k[l].data == x;
+}
+
+// Whether all slabs are surely different ones: their addresses rise, K's apart from V's.
+bool slabs_apart(const mm3fa_tensor * k, const mm3fa_tensor * v, int n) {
+    for (int i = 1; i < n; i++) {
+        if (k[i].data <= k[i - 1].data || v[i].data <= v[i - 1].data) {
+            return false;
+        }
+    }
+    return k[n - 1].data < v[0].data || v[n - 1].data < k[0].data;
+}
+
 // Whether a row of `a` and one of `b` share bytes, told from their extents, and, where these cross, for tensors whose strides
 // are the same along each dimension (`of_b`: b's dimension of a's) and those above another's extent: rows in turn in one buffer.
 // Others are taken to share some.
@@ -359,12 +384,13 @@ int mm3fa_tree_commit(const mm3fa_tensor * k, const mm3fa_tensor * v, int n_laye
     p.kv_len    = kv_len;
     p.T         = max_nodes;
     p.n_tree    = n_tree;
+    const bool apart = slabs_apart(k, v, n_layers);
     for (int l = 0; l < n_layers; l += TREE_LAYERS) {
         p.n_layers = std::min(TREE_LAYERS, n_layers - l);
         p.len_out  = l == 0 ? kv_len_out : nullptr;
         for (int i = 0; i < p.n_layers; i++) {
-            p.k[i] = static_cast<char *>(k[l + i].data);
-            p.v[i] = static_cast<char *>(v[l + i].data);
+            p.k[i] = named_before(k, v, l + i, false, apart) ? nullptr : static_cast<char *>(k[l + i].data);
+            p.v[i] = named_before(k, v, l + i, true, apart) ? nullptr : static_cast<char *>(v[l + i].data);
         }
         const int st = host_record_cuda(launch_tree_commit(p, unit, host_sm_count(), static_cast<cudaStream_t>(stream)));
         if (st != MM3FA_OK) {

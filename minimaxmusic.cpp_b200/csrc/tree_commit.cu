@@ -44,6 +44,7 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_commit_kernel(const __grid
         const int      skip = stay == 0xffffffffu ? 32 : __ffs(~stay) - 1, items = rows * pieces;
         constexpr int  B    = 4;
         for (int layer = blockIdx.y; layer < p.n_layers; layer += (int) gridDim.y) {
+            const bool has_k = p.k[layer] != nullptr, has_v = p.v[layer] != nullptr;
             char * k = p.k[layer] + k0, *v = p.v[layer] + v0;
             for (int e0 = min(skip, rows) * pieces; e0 < items; e0 += 32 * B) {
                 // (batches may end inside a row: a later batch's sources lie at or behind its own destinations, which lie
@@ -54,8 +55,12 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_commit_kernel(const __grid
                     const int e = e0 + b * 32 + lane, r = min(e / pieces, 31), src = __shfl_sync(0xffffffffu, at, r);
                     if (e < items) {
                         const int64_t off = (int64_t) (e - r * pieces) * (int) sizeof(U);
-                        x[b] = *reinterpret_cast<const U *>(k + src * p.k_nb1 + off);
-                        y[b] = *reinterpret_cast<const U *>(v + src * p.v_nb1 + off);
+                        if (has_k) {
+                            x[b] = *reinterpret_cast<const U *>(k + src * p.k_nb1 + off);
+                        }
+                        if (has_v) {
+                            y[b] = *reinterpret_cast<const U *>(v + src * p.v_nb1 + off);
+                        }
                     }
                 }
                 __syncwarp();
@@ -64,8 +69,12 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_commit_kernel(const __grid
                     const int e = e0 + b * 32 + lane, r = e / pieces;
                     if (e < items) {
                         const int64_t off = (int64_t) (e - r * pieces) * (int) sizeof(U);
-                        *reinterpret_cast<U *>(k + (i0 + r) * p.k_nb1 + off) = x[b];
-                        *reinterpret_cast<U *>(v + (i0 + r) * p.v_nb1 + off) = y[b];
+                        if (has_k) {
+                            *reinterpret_cast<U *>(k + (i0 + r) * p.k_nb1 + off) = x[b];
+                        }
+                        if (has_v) {
+                            *reinterpret_cast<U *>(v + (i0 + r) * p.v_nb1 + off) = y[b];
+                        }
                     }
                 }
                 __syncwarp();

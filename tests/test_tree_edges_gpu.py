@@ -1,10 +1,12 @@
 """Tree decoding on the GPU where its ranges end, against the 64-bit references of tests/tree_ref.py."""
+import random
+
 import pytest
 import torch
 
 import mm3fa
 import tree_ref as R
-from test_tree_gpu import Case
+from test_tree_gpu import Case, rising, slabs
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +43,24 @@ def test_attend_slabs_of_one_row(cuda_device, which, dtype, cache):
                 view.copy_(x)
                 setattr(c, name, view)
             c.check()
+
+
+@pytest.mark.parametrize("L", [3, 100])
+def test_commit_slabs_that_layers_share(cuda_device, L):
+    """Layers that read one another's slabs name them again: each is moved once, whichever layers and whichever of K and V name it."""
+    rng = random.Random(L)
+    T, N, Hkv = 24, 3, 2
+    some = slabs(cuda_device, 5, N, Hkv, T + 40, 64, "f16", 7)
+    before = [x.clone() for x in some]
+    k = [some[(0, 0, 1, 2)[i % 4]] for i in range(L)]
+    v = [some[(3, 3, 4, 2)[i % 4]] for i in range(L)]
+    if L == 3:
+        k[2], v[2] = some[4], some[0]
+    used = {x.data_ptr() for x in k + v}
+    path = torch.tensor([rising(rng, T, 11)] * N, dtype=torch.int32, device=cuda_device)
+    n_path, lens = (torch.tensor(x, dtype=torch.int32, device=cuda_device) for x in ([11] * N, [0, 7, 33]))
+    want, want_len = R.commit(before, path, n_path, lens)
+    got = mm3fa.DraftTree(torch.full((N, T), -1, dtype=torch.int32, device=cuda_device)).commit(mm3fa.CacheLayers(k, v), path, n_path, lens)
+    assert torch.equal(got, want_len)
+    for x, old, w in zip(some, before, want):
+        assert torch.equal(x, w if x.data_ptr() in used else old)
