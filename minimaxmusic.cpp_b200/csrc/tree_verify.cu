@@ -102,12 +102,12 @@ __device__ __forceinline__ float clean_draft(float q) {
     return fmaxf(q, 0.0f);  // NaN: 0
 }
 
-// sum + 2^(x t + c) for exponents from -1000 to 0, to 12 digits: the exponent is n + k / 32 + r with |r| <= 1/64; 2^(k / 32)
-// comes from lane k (`power` of each lane), n goes into its exponent, and 2^r is its series to the fourth power.  By whole
-// warps; 9 instructions of F64.
-__device__ __forceinline__ double add_power(double x, double t, double c, double power, double sum) {
+// sum + 2^(d t) for exponents from -1000 to 0, to 12 digits: the exponent is n + k / 32 + r with |r| <= 1/64; 2^(k / 32) comes
+// from lane k (`power` of each lane), n goes into its exponent, and 2^r is its series to the fourth power.  `none`: sum, and
+// less than 2^-1000.  By whole warps; 8 instructions of F64.
+__device__ __forceinline__ double add_power(double d, double t, double power, bool none, double sum) {
     const double magic = 0x1.8p+47;  // a number this large is a multiple of 1/32
-    const double y = fma(x, t, c) + magic, r = fma(x, t, c - (y - magic));
+    const double y = fma(d, t, magic), r = fma(d, t, magic - y);
     const int    n = __double2loint(y);  // 32 n + k
     const double pw = __shfl_sync(0xffffffffu, power, n & 31);
     // ln(2)^i / i!
@@ -115,10 +115,10 @@ __device__ __forceinline__ double add_power(double x, double t, double c, double
     s = fma(s, r, 2.4022650695910072e-1);
     s = fma(s, r, 6.9314718055994531e-1);
     s = fma(s, r, 1.0);
-    return fma(s, __hiloint2double(__double2hiint(pw) + ((n >> 5) << 20), __double2loint(pw)), sum);
+    return fma(s, __hiloint2double(none ? 0 : __double2hiint(pw) + ((n >> 5) << 20), __double2loint(pw)), sum);
 }
 
-// Sums of weights below this are none: an entry of -inf counts as 2^-800 of the largest.
+// Sums of weights below this are none.
 constexpr double TV_NONE = 0x1p-600;
 
 // LT, DT: types of logits and drafts (DT -1: fixed choices)
@@ -133,8 +133,6 @@ struct Walk {
     int                      rank, turn, tid, lane, warp;
     bool                     held;  // a chunk a warp at most: kept from pass to pass
     double                   power;
-    bool                     coarse;  // logits so large that only the largest has a weight: that of `only`, taken as 0
-    float                    only;
     float                    x[TV_E], q[DT >= 0 ? TV_E : 1];
 
     // the chunk from i0 on
@@ -366,29 +364,27 @@ struct Walk {
         return total(sum);
     }
 
-    // 2^((v - m) / t), 0 where that is below 2^-800.  By whole warps.
-    __device__ __forceinline__ double weight(float v, float m) const {
+    // sum + 2^((v - m) / t), sum where that is below 2^-800 (or so near 0 that no sum changes by it).  By whole warps.
+    __device__ __forceinline__ double add_weight(float v, float m, double sum) const {
         const bool in = (v - m) * (float) p.inv_t > -800.0f;
-        const double w  = add_power((double) (in ? v : m) - (double) m, p.inv_t, 0.0, power, 0.0);
-        return in ? w : 0.0;
+        return add_power((double) (in ? v : m) - (double) m, p.inv_t, power, !in, sum);
+    }
+
+    // 2^((v - m) / t), 0 where that is below 2^-800 (a token of -inf is never accepted, with a number of 0 either).  By whole warps.
+    __device__ __forceinline__ double weight(float v, float m) const {
+        return (v - m) * (float) p.inv_t > -800.0f ? add_weight(v, m, 0.0) : 0.0;
     }
 
     // what is left of the chunk's entry e: max(p - c q, 0), or the weight of a token that was not rejected.  By whole warps.
     __device__ __forceinline__ double left(int e, float m, double iz, double c) const {
-        const double w = weight(x[e], m);
+        const double w = add_weight(x[e], m, 0.0);
         return DT >= 0 && c > 0.0 ? fmax(w * iz - c * (double) q[DT >= 0 ? e : 0], 0.0) : w;
     }
 
     // the chunk from i0 on for `left`: the rejected tokens of fixed choices count as -inf
     __device__ __forceinline__ void load_left(int i0, int n_gone) {
-        if (!held || DT < 0 || coarse) {
+        if (!held || DT < 0) {
             load_both(i0);
-        }
-        if (coarse) {
-#pragma unroll
-            for (int e = 0; e < TV_E; e++) {
-                x[e] = x[e] == only ? 0.0f : -INFINITY;
-            }
         }
         for (int k = 0; DT < 0 && k < n_gone; k++) {
             const int at = sh.gone[k] - i0;
@@ -403,22 +399,14 @@ struct Walk {
 
     // sum of `left` over the row; the sums of the CTA's chunks are kept
     __device__ __forceinline__ double left_sums(float m, double iz, double c, int n_gone) {
-        const double shift = -(double) m * p.inv_t;
-        const float  floor = m - 800.0f / (float) p.inv_t;  // (F32 is 128 / t coarse there at most)
-        double       sum   = 0.0;
+        double sum = 0.0;
         __syncthreads();
         for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
             load_left(i0, n_gone);
             double s = 0.0;
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
-                const double v = (double) fmaxf(x[e], floor);
-                if (DT < 0) {
-                    s = add_power(v, p.inv_t, shift, power, s);
-                } else {
-                    const double w = add_power(v, p.inv_t, shift, power, 0.0);
-                    s += c > 0.0 ? fmax(w * iz - c * (double) q[DT >= 0 ? e : 0], 0.0) : w;
-                }
+                s = DT < 0 ? add_weight(x[e], m, s) : s + left(e, m, iz, c);
             }
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) {
@@ -548,7 +536,7 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
     // slices of whole chunks
     const int chunks = (p.V + TV_CHUNK - 1) / TV_CHUNK, each = (chunks + n_ranks - 1) / n_ranks, n_warps = (int) blockDim.x / 32;
     Walk<LT, DT> w{ p, sh, tv_sums, lbase, qbase, min(rank * each * TV_CHUNK, p.V), min((rank + 1) * each * TV_CHUNK, p.V), n_ranks, n_warps, rank, 0, tid, lane, warp,
-                    each <= n_warps, exp2((double) lane / 32.0), false, 0.0f };
+                    each <= n_warps, exp2((double) lane / 32.0) };
     int    cur = 0, n_path = 1, n_gone, n_no, best = -1;
     float  m = 0.0f;
     double z = 0.0;
@@ -621,9 +609,6 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
     if (!greedy && best >= 0) {
         // the F64 sums: with drafts Z and the M again, then what is left; the target's own distribution, where nothing is
         const int last = DT >= 0 ? n_no : 0;
-        if (fabsf(m) * (float) p.inv_t > 0x1p30f) {
-            w.coarse = true, w.only = m, m = 0.0f;
-        }
         double    iz = 1.0, c = 0.0;
         for (int k = 0;; k++) {
             const double sum = w.left_sums(m, iz, c, n_gone);

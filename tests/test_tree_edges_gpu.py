@@ -6,7 +6,7 @@ import torch
 
 import mm3fa
 import tree_ref as R
-from test_tree_gpu import Case, rising, slabs
+from test_tree_gpu import Case, check_verify, rising, slabs
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,18 @@ def test_commit_slabs_that_layers_share(cuda_device, L):
     assert torch.equal(got, want_len)
     for x, old, w in zip(some, before, want):
         assert torch.equal(x, w if x.data_ptr() in used else old)
+
+
+@pytest.mark.parametrize("draft", [None, "f32"])
+@pytest.mark.parametrize("V", [300, 5003, 40000])
+@pytest.mark.parametrize("temperature", [2e-5, 1e-7, 1e6, 1e36, 3e38])
+def test_verify_temperatures(cuda_device, temperature, V, draft):
+    """From ones at which all but the largest logits vanish to ones at which every logit above -inf weighs the same."""
+    def edit(s, par):
+        x = s["logits"]
+        x[:, :, ::7] = float("-inf")
+        x[1] *= 1e4
+        x[2] -= 1e4
+        s["tokens"][3:, 1:] = x[3:, 0].argmax(-1)[:, None].to(torch.int32)
+        s["tokens"][5, 1:], s["accept"][5] = 14, 0.0  # a token of no probability, whatever the number
+    check_verify(cuda_device, 9, 12, V, "f32", draft, temperature, seed=V, edit=edit)
