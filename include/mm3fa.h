@@ -648,7 +648,9 @@ MM3FA_API int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, co
  *   path     device int32 [n_tree][max_nodes]: the accepted nodes in order, node 0 first, then -1
  *   n_path   device int32 [n_tree]: how many (0 where a tree has no nodes)
  *   token    device int32 [n_tree]: the next token (-1 where a tree has no nodes or no logit is above -inf)
- * Decisions are taken from F32 logits in F64; V up to 2^22.  Only the rows of accepted nodes are read.
+ * Decisions, and the next token, are the ones that F64 sums of the logits' exponentials give, to 12 digits; probabilities below
+ * 2^-800 of a row's largest count as 0.  V up to 2^22.  Of the rows of nodes that are not accepted, only the entries at their
+ * children's tokens are read.
  */
 MM3FA_API int mm3fa_tree_verify(const mm3fa_tensor * logits, const mm3fa_tensor * draft, const mm3fa_tree * tree,
                                 const int32_t * tokens, const float * accept, const float * sample, float temperature,

@@ -12,13 +12,17 @@
 // One cluster of CTAs per tree, each with a slice of the vocabulary.  Only the rows of nodes on the path are read, one
 // after another: T rows would be several times the bytes.  The sums over a row go from CTA to CTA through distributed
 // shared memory, in the order of the ranks, and every thread takes the same decisions from them.
-// The decisions come from F32 exponentials summed in F64; the last row's sums (and the M that lead to them) are taken in
-// F64 throughout, since the next token's place among 10^5 borders moves with the twelfth digit of a partial sum.
+// A decision is what F64 sums say, to 12 digits.  A row's first sum, and the M of drafts, are of F32 exponentials and off by
+// TV_CLOSE at most; where a decision is nearer to its border than that, and for the next token, whose place among 10^5 borders
+// moves with the twelfth digit of a partial sum, the row is summed again in F64 (and what the fixed choices that were turned
+// down leave is summed without them, so that a child with nearly all of the probability leaves all its digits to the rest).
 //
 // Bound: HBM where there are many trees, else the passes of a walk, one after another (a row, and a rejection's sum): a slice
 // of up to 8 entries a thread is kept in registers between them.  F64 runs at half of F32's rate here, and exp2() is some
-// 40 instructions of it: with a table of 32 powers, one in each lane, and a polynomial it is 12.
+// 40 instructions of it: with a table of 32 powers, one in each lane, and a polynomial it is 8.
 #include "tree.cuh"
+
+#include <type_traits>
 
 namespace mm3fa {
 
@@ -120,6 +124,11 @@ __device__ __forceinline__ double add_power(double d, double t, double power, bo
 
 // Sums of weights below this are none.
 constexpr double TV_NONE = 0x1p-600;
+
+// How far row_mass() is off, of its value, and left_mass(), of 1, at most.  With y the exponent of an entry: three F32 roundings
+// of y, on average over the entries by weight below log2(V) = 22 (their entropy), 22 * 3 * 2^-24 * ln 2; 2^-22 of ex2, and of each
+// of some 7 steps to a larger maximum; 16 F32 additions: less than 2^-17.  left_mass() has the row's sum in it, and its own exponentials.
+constexpr float TV_CLOSE = 0x1p-16f;
 
 // LT, DT: types of logits and drafts (DT -1: fixed choices)
 template <int LT, int DT>
@@ -238,23 +247,27 @@ struct Walk {
     // (m, sum of 2^((x - m) / t)) over the row
     __device__ __forceinline__ void row_mass(float & m, double & z) {
         const float a = (float) p.inv_t;
-        float       s = 0.0f;
+        float       from = -INFINITY;  // what the sum is relative to: near the maximum so far, so that it seldom moves
+        double      s = 0.0;
         m = -INFINITY;
-        auto add = [&](const float (&v)[TV_E]) {
-            float top = v[0];
+        auto add = [&](const auto &... v) {  // a chunk, or two
+            float top = -INFINITY;
 #pragma unroll
-            for (int e = 1; e < TV_E; e++) {
-                top = fmaxf(top, v[e]);
+            for (int e = 0; e < TV_E; e++) {
+                ((top = fmaxf(top, v[e])), ...);
             }
-            if (top > m) {
-                s *= power2((m - top) * a);
-                m = top;
+            if ((top - from) * a > 8.0f) {  // (at first too)
+                s *= (double) power2((from - top) * a);
+                from = top;
             }
-            if (m > -INFINITY) {
+            m = fmaxf(m, top);
+            if (from > -INFINITY) {
+                float part = 0.0f;
 #pragma unroll
                 for (int e = 0; e < TV_E; e++) {
-                    s += power2((v[e] - m) * a);
+                    ((part += power2((v[e] - from) * a)), ...);
                 }
+                s += (double) part;
             }
         };
         const int step = n_warps * TV_CHUNK;
@@ -271,18 +284,13 @@ struct Walk {
             for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += 2 * step) {  // two chunks' loads in flight: 52 us against 56
                 float y[TV_E];
                 load(x, i0);
-                if (i0 + step < hi) {
-                    load(y, i0 + step);
-                }
+                load(y, i0 + step);  // (-inf behind the slice)
                 clean(x);
-                add(x);
-                if (i0 + step < hi) {
-                    clean(y);
-                    add(y);
-                }
+                clean(y);
+                add(x, y);
             }
         }
-        z = (double) s;
+        z = m > from ? s * (double) power2((from - m) * a) : s;
         join(m, z);
         __syncthreads();
         if (lane == 0) {
@@ -347,8 +355,8 @@ struct Walk {
     }
 
     // sum of max(p - c q, 0), in F32 terms
-    __device__ __forceinline__ double left_mass(float m, double z, double c) {
-        const float a = (float) p.inv_t, iz = (float) (1.0 / z), cf = (float) c;
+    __device__ __forceinline__ double left_mass(float m, float iz, float c) {
+        const float a = (float) p.inv_t;
         double      sum = 0.0;
         for (int i0 = lo + warp * TV_CHUNK; i0 < hi; i0 += n_warps * TV_CHUNK) {
             if (!held) {
@@ -357,7 +365,7 @@ struct Walk {
             float s = 0.0f;
 #pragma unroll
             for (int e = 0; e < TV_E; e++) {
-                s += fmaxf(power2((x[e] - m) * a) * iz - cf * q[DT >= 0 ? e : 0], 0.0f);
+                s += fmaxf(power2((x[e] - m) * a) * iz - c * q[DT >= 0 ? e : 0], 0.0f);
             }
             sum += (double) s;
         }
@@ -542,72 +550,108 @@ __global__ void __launch_bounds__(TV_THREADS, 1) tree_verify_kernel(const TreeVe
     double z = 0.0;
     const bool greedy = p.inv_t == 0.0;
     constexpr int ESZ = LT == KV_F32 ? 4 : 2;
-    for (;;) {
-        w.lrow = lbase + (int64_t) cur * p.logits.nb1;
-        w.qrow = DT >= 0 ? qbase + (int64_t) cur * p.draft.nb1 : nullptr;
-        n_gone = n_no = 0;
-        if (!w.held) {
-            w.fetch(w.lrow, ESZ);
-        }
-        if (greedy) {
-            best = w.row_argmax();
-        } else {
-            w.row_mass(m, z);
-            best = m > -INFINITY ? 0 : -1;
-        }
-        int    next = -1;
-        double c = 0.0, M = 1.0;
-        bool   first = true;
-        for (int k0 = cur / 32 * 32; best >= 0 && next < 0 && k0 < n; k0 += 32) {
-            unsigned kids = __ballot_sync(0xffffffffu, k0 + lane < n && k0 + lane > cur && sh.par[min(k0 + lane, TREE_MAX - 1)] == cur);
-            while (kids && next < 0) {
-                const int i = k0 + __ffs(kids) - 1;
-                kids &= kids - 1;
-                if (greedy) {
-                    next = sh.tok[i] == best ? i : -1;
-                    continue;
-                }
-                if (ahead && first) {
-                    // (few trees: the likeliest next row comes nearer while this one is decided on)
-                    w.fetch(lbase + (int64_t) i * p.logits.nb1, ESZ);
-                    first = false;
-                }
-                const double px = w.weight(sh.lx[i], m) / z, q = (double) sh.qx[i];
-                double       r  = fmax(px - c * q, 0.0);
-                if (DT < 0) {
-                    r = px;
-                    for (int k = 0; k < n_gone; k++) {
-                        r = sh.gone[k] == sh.tok[i] ? 0.0 : r;
+    // The walk from node `cur` on, by F32 exponentials; false: it has come to a decision that is too near to its border for them.
+    // `exact`: by F64 ones.  (One after the other, and not the second's passes within the first, for the registers of its loop over
+    // a row: 64 trees of 150001 tokens took 60 us that way, and 68 with the passes in a function, for 55.)
+    auto walk = [&](auto exact) {
+        constexpr bool EXACT = decltype(exact)::value;
+        for (;;) {
+            w.lrow = lbase + (int64_t) cur * p.logits.nb1;
+            w.qrow = DT >= 0 ? qbase + (int64_t) cur * p.draft.nb1 : nullptr;
+            n_gone = n_no = 0;
+            if (!w.held) {
+                w.fetch(w.lrow, ESZ);
+            }
+            if (greedy) {
+                best = w.row_argmax();
+            } else {
+                w.row_mass(m, z);
+                best = m > -INFINITY ? 0 : -1;
+            }
+            int         next = -1;
+            float       c = 0.0f, M = 1.0f, c_off = 0.0f, M_off = 0.0f;  // and how far these may be off
+            const float izf = (float) (1.0 / z);
+            double      iz = 1.0, cx = 0.0, Mx = 1.0;  // EXACT: 1 / the row's sum, c, M (fixed choices: what is left of the row's sum)
+            if (EXACT && best >= 0) {
+                const double sum = w.left_sums(m, 1.0, 0.0, 0);
+                iz = 1.0 / sum, Mx = DT >= 0 ? 1.0 : sum;
+            }
+            bool first = true;
+            for (int k0 = cur / 32 * 32; best >= 0 && next < 0 && k0 < n; k0 += 32) {
+                unsigned kids = __ballot_sync(0xffffffffu, k0 + lane < n && k0 + lane > cur && sh.par[min(k0 + lane, TREE_MAX - 1)] == cur);
+                while (kids && next < 0) {
+                    const int i = k0 + __ffs(kids) - 1;
+                    kids &= kids - 1;
+                    if (greedy) {
+                        next = sh.tok[i] == best ? i : -1;
+                        continue;
                     }
-                }
-                if ((double) sh.u[i] * q * M < r) {
-                    next = i;
-                } else if (DT >= 0) {
-                    c += M;
+                    if (ahead && first) {
+                        // (few trees: the likeliest next row comes nearer while this one is decided on)
+                        w.fetch(lbase + (int64_t) i * p.logits.nb1, ESZ);
+                        first = false;
+                    }
+                    bool gone = false;
+                    for (int k = 0; DT < 0 && k < n_gone; k++) {
+                        gone = gone || sh.gone[k] == sh.tok[i];
+                    }
+                    const float q = sh.qx[i], u = sh.u[i];
+                    float       px = 0.0f;
+                    bool        taken;
+                    if constexpr (EXACT) {
+                        const double wx = gone ? 0.0 : w.weight(sh.lx[i], m), uq = (double) u * (double) q;
+                        taken = uq * Mx < (DT >= 0 ? fmax(wx * iz - cx * (double) q, 0.0) : wx);
+                    } else {
+                        px = gone ? 0.0f : power2((sh.lx[i] - m) * (float) p.inv_t) * izf;
+                        const float d = fmaxf(px - c * q, 0.0f) - u * q * M;
+                        // (px: 2^-17 of the row's sum, 126 * 3 * 2^-24 * ln 2 of its exponent, 2^-22 of ex2, and all of it below
+                        // 2^-126; 2^-22: the roundings of d)
+                        if (!gone && !(fabsf(d) > 0x1p-15f * px + c_off * q + M_off * fabsf(u * q) + 0x1p-22f * (c * q + fabsf(u * q) * M) + 0x1p-125f)) {
+                            return false;
+                        }
+                        taken = d > 0.0f;
+                    }
+                    if (taken) {
+                        next = i;
+                        continue;
+                    }
                     n_no++;
-                    M = w.left_mass(m, z, c);
-                } else if (r > 0.0) {
-                    M = fmax(M - r, 0.0);
-                    __syncthreads();
-                    if (tid == 0) {
-                        sh.gone[n_gone] = sh.tok[i];
+                    if (DT < 0 && !gone) {
+                        __syncthreads();
+                        if (tid == 0) {
+                            sh.gone[n_gone] = sh.tok[i];
+                        }
+                        __syncthreads();
+                        n_gone++;
                     }
-                    __syncthreads();
-                    n_gone++;
+                    if constexpr (EXACT) {
+                        if (DT >= 0 || !gone) {
+                            cx += DT >= 0 ? Mx : 0.0;
+                            Mx = w.left_sums(m, iz, cx, n_gone);
+                        }
+                    } else if constexpr (DT >= 0) {
+                        c += M, c_off += M_off + 0x1p-23f * c;
+                        M = (float) w.left_mass(m, izf, c), M_off = TV_CLOSE + c_off;  // (sum of q where p > c q: 1 / c at most, and c is 1 at least)
+                    } else {
+                        M = fmaxf(M - px, 0.0f), M_off += TV_CLOSE * px + 0x1p-23f;
+                    }
                 }
             }
+            if (next < 0) {
+                return true;
+            }
+            cur = next;
+            if (tid == 0) {
+                sh.path[n_path] = cur;
+            }
+            n_path++;
         }
-        if (next < 0) {
-            break;
-        }
-        cur = next;
-        if (tid == 0) {
-            sh.path[n_path] = cur;
-        }
-        n_path++;
+    };
+    if (!walk(std::false_type())) {
+        walk(std::true_type());
     }
     if (!greedy && best >= 0) {
-        // the F64 sums: with drafts Z and the M again, then what is left; the target's own distribution, where nothing is
+        // in F64, with drafts, the row's sum and the M again, then what is left; the target's own distribution, where nothing is
         const int last = DT >= 0 ? n_no : 0;
         double    iz = 1.0, c = 0.0;
         for (int k = 0;; k++) {

@@ -79,3 +79,64 @@ def test_verify_temperatures(cuda_device, temperature, V, draft):
         s["tokens"][3:, 1:] = x[3:, 0].argmax(-1)[:, None].to(torch.int32)
         s["tokens"][5, 1:], s["accept"][5] = 14, 0.0  # a token of no probability, whatever the number
     check_verify(cuda_device, 9, 12, V, "f32", draft, temperature, seed=V, edit=edit)
+
+
+def star_decisions(x, tokens, draft, temperature, turned_down):
+    """F64 [n] each, for the child of the root behind `turned_down` ones that were turned down: its number u is accepted where
+    u q M < r; and the sum c of the M before."""
+    n = x.shape[0]
+    each = torch.arange(n, device=x.device)
+    r, mass = torch.softmax(x.double() / temperature, -1), torch.ones(n, dtype=torch.float64, device=x.device)
+    c = torch.zeros_like(mass)
+    for i in range(1, turned_down + 2):
+        tok = tokens[:, i].long()
+        q = torch.zeros_like(r).scatter_(1, tok[:, None], 1.0) if draft is None else draft.double()
+        if i <= turned_down:
+            r, c = (r - mass[:, None] * q).clamp(min=0), c + mass
+            mass = r.sum(-1)
+    return q[each, tok], mass, r[each, tok], c
+
+
+@pytest.mark.parametrize("kind", ["likely", "dominant", "dominant twice", "rising", "drafts 0", "drafts 1", "drafts 3"])
+@pytest.mark.parametrize("V", [300, 5003, 150001, (1 << 22) - 5])
+def test_verify_decisions_next_to_their_border(cuda_device, V, kind):
+    """Numbers two F32 steps below a decision's border accept, and two above it do not: a step is 2^-24 to 2^-23 of the number,
+    F32 sums of the exponentials are off by more.  Children that had nearly all of the probability are turned down before."""
+    n, temperature = 2 if V > 1 << 20 else 24, torch.tensor(0.7).item()  # as the call takes it, an F32 number: 0.7 itself moves p by 10^-7
+    g = torch.Generator(device=cuda_device).manual_seed(V)
+    x = torch.randn(n, V, generator=g, device=cuda_device) * 1.5
+    if kind == "rising":
+        x = x.sort(-1).values
+    draft, down = None, {"likely": 1, "dominant": 1, "dominant twice": 2, "rising": 0}.get(kind, int(kind[-1]) if kind[-1].isdigit() else 0)
+    tokens = torch.stack([torch.arange(n, device=cuda_device) * 7 % 50 + 51 * i for i in range(5)], 1).to(torch.int32)
+    most = torch.logsumexp(x.double() / temperature, -1).float() * temperature
+    if kind.startswith("dominant"):  # all but 2e-6 of the probability, and all but 5e-5 of the rest
+        for i, more in ((1, 23.0 if down == 2 else 13.0), (2, 10.0))[:down]:
+            x.scatter_(1, tokens[:, i:i + 1].long(), (most + more * temperature)[:, None])
+    if kind == "likely":
+        x.scatter_(1, tokens[:, 1:2].long(), most[:, None])
+    if kind.startswith("drafts"):
+        draft = torch.softmax(x / temperature + 0.3 * torch.randn(n, V, generator=g, device=cuda_device), -1)
+        for i in range(1, down + 1):  # the draft thinks more of them than the target
+            draft.scatter_(1, tokens[:, i:i + 1].long(), 1.5 * torch.softmax(x / temperature, -1).gather(1, tokens[:, i:i + 1].long()))
+        _, mass, _, c = star_decisions(x, tokens, draft, temperature, down)
+        p = torch.softmax(x / temperature, -1).gather(1, tokens[:, down + 1:down + 2].long())
+        draft.scatter_(1, tokens[:, down + 1:down + 2].long(), p / (c + 0.5 * mass)[:, None].float())  # a border near 1/2
+    q, mass, r, _ = star_decisions(x, tokens, draft, temperature, down)
+    factor = q * mass
+    border = (r / factor).float()
+    assert ((border > 0) & (border < 0.999)).all()
+    accept = torch.full((n, 5), 1.0 - 2.0 ** -24, device=cuda_device)
+    T = down + 2
+    logits = x[:, None].expand(n, T, V).contiguous()
+    drafts = None if draft is None else draft[:, None].expand(n, T, V).contiguous()
+    tree = mm3fa.DraftTree(torch.tensor([[-1] + [0] * (T - 1)], dtype=torch.int32, device=cuda_device).expand(n, T).contiguous())
+    for way, taken in ((float("-inf"), True), (float("inf"), False)):
+        u = border
+        for _ in range(2):
+            u = torch.nextafter(u, torch.full_like(u, way))
+        accept[:, T - 1] = u
+        assert ((u.double() * factor < r) == taken).all()
+        path, n_path, token = tree.verify(logits, tokens[:, :T].contiguous(), accept[:, :T].contiguous(), torch.full((n,), 0.3, device=cuda_device),
+                                          draft=drafts, temperature=temperature)
+        assert ((n_path == 2) == taken).all() and (path[:, 1] == (T - 1 if taken else -1)).all(), (kind, taken)
