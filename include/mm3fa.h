@@ -622,10 +622,10 @@ MM3FA_API size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_t
  *   logit_softcap  0 disables; otherwise s <- softcap * tanh(s / softcap)
  *   workspace      its first 64 KiB zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this
  *                  function alone, of any shapes that it is large enough for
- * D 64, 128 or 256; at most 64 query heads per kv head.  q and the weights are not rounded to the cache's type: F16 slabs at
- * D 64 and 128 keep 22 bits of them (an F32 result is off by about 5e-7 of its norm), BF16 slabs 16 (3.5e-6), F32 and Q8_0
- * slabs and D 256 all 24.  Where q, slabs and dst have one 16-bit type, and the slabs up to 32768 rows, weights are rounded
- * to that type.  What a node does not see has no influence, not-a-number or infinite values included; a node that sees
+ * D 64, 128 or 256; at most 64 query heads per kv head.  q and the weights are not rounded to the cache's type: at D 64 and 128,
+ * F16 slabs keep 22 bits of them (an F32 result is off by about 5e-7 of its norm), BF16 slabs all 24 for an F32 result (4e-7) and
+ * 16 for others; F32 and Q8_0 slabs and D 256 all 24.  Where q, slabs and dst have one 16-bit type, and the slabs up to 32768
+ * rows, weights are rounded to that type.  What a node does not see has no influence, not-a-number or infinite values included; a node that sees
  * nothing gets zeros.
  */
 MM3FA_API int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v,

@@ -72,7 +72,7 @@ cudaError_t launch_tree_attn(const TreeAttnParams & p, cudaStream_t stream);
 bool        tree_attn_tc_takes(const TreeAttnParams & p);
 bool        tree_attn_tc_sizes(const TreeAttnParams & p);  // the same, but for the alignment and strides of rows
 int         tree_attn_wide(const TreeAttnParams & p);  // CTAs of a group
-int         tree_attn_groups(const TreeAttnParams & p, int sms);
+int         tree_attn_groups(const TreeAttnParams & p, int keys, int sms);
 size_t      tree_attn_tc_workspace(const TreeAttnParams & p, int sms);
 cudaError_t launch_tree_attn_tc(TreeAttnParams p, int sms, cudaStream_t stream);
 cudaError_t launch_tree_verify(const TreeVerifyParams & p, int sms, cudaStream_t stream);

@@ -19,7 +19,7 @@
 //
 // 384 threads:
 //   warp 0       TMA: K and V tiles through one ring, in the order in which the products take them
-//   warp 1       TMEM allocation and every tcgen05.mma: QK(j + 1), then P V(j), P in TMEM over S
+//   warp 1       TMEM allocation and every tcgen05.mma: QK(j + 1), then P V(j), P in TMEM over S (a third part behind it)
 //   warps 2, 3   the V rows of tiles that hold nodes: those behind the last node become zero, and so do elements that are
 //                no numbers (their weight may be 0; who sees such a node gets them added at the end); then the next
 //                piece's Q, beside the softmax of this one's last tiles
@@ -31,9 +31,11 @@
 // each step of 16 keys, always towards zero (measured 7e-7 a tile of 128 keys): up to TS_LONG keys a stream's sum stays within
 // 1e-4, a fifth of F16's half step.  Else (PARTS 2) q is two parts of the cache's type (F16: brought to [2^14, 2^15) at its row's largest
 // element by a power of two), and so are the weights, the remainder's product first, where the accumulator is small;
-// every tile's P V starts afresh and is added in registers, rounded to nearest: 22 bits of q and weights in F16, 16 in BF16 (an
-// F32 result is off by 5e-7 and 3.5e-6 of its norm; a third part would not fit in TMEM beside S and O of two tiles).  PARTS 1
-// takes 22 us at 2 x 8192 and 24 nodes (BF16) where PARTS 2 takes 31, and 32 at 64 nodes where that takes 49.
+// every tile's P V starts afresh and is added in registers, rounded to nearest: 22 bits of q and weights in F16 (an F32 result
+// is off by 5e-7 of its norm), 16 in BF16, which F32 results over BF16 slabs take three parts for (PARTS 3: 24 bits; 4e-7 of the
+// norm, 3.5e-6 with two), in tiles of 64 keys, as TMEM has no place for three parts of 128.  2 x 8192, 24 nodes: PARTS 1 22 us
+// (BF16), 2 31, 3 38; 64 nodes: 32, 49, 67; 48 sequences of up to 10240, 13 nodes: 166, 249, 381 (tiles of 80 keys, the most that
+// TMEM takes: 39, 70 and 375).
 //
 // Bound: HBM for batches at full clock (48 sequences of 1 to 10240, 13 nodes, BF16, 1013 MB: 166 us, 6.1 TB/s, at 1965 MHz; under a
 // lasting load the power cap takes the clock to 1430-1550 MHz, and the tiles' own work counts too: 177-188); few sequences
@@ -54,7 +56,7 @@ namespace {
 
 constexpr int TS_THREADS = 384;
 constexpr int TS_M       = 128;  // rows of a block
-constexpr int TS_N       = 128;  // keys of a tile
+constexpr int TS_S       = 128;  // columns of a tile's S, with the weights over it
 constexpr int TS_TMEM    = 512;  // columns: S of two tiles, P V of two tiles
 constexpr int TS_GROW    = 7;    // (PARTS 1) log2 of what a weight may exceed the maximum of the tiles before by
 constexpr int TS_LONG    = 32768;
@@ -73,14 +75,20 @@ static_assert(2 * TS_REGS_SOFTMAX + TS_REGS_ISSUE <= 3 * TS_REGS_LAUNCH, "more r
 
 // log2 of what a weight at the maximum is held as: F16 keeps 11 bits of one down to 2^-(14 + offset) of it, and holds 2^15
 template <int PARTS>
-constexpr float TS_OFF = PARTS == 2 ? 14.0f : 15.0f - TS_GROW;
+constexpr float TS_OFF = PARTS >= 2 ? 14.0f : 15.0f - TS_GROW;
+
+// keys of a tile: three parts of the weights of 128 keys would have no place in TMEM
+__host__ __device__ constexpr int ts_keys(int parts) {
+    return parts == 3 ? 64 : 128;
+}
 
 template <int D, int PARTS>
 struct TsSmem {
+    static constexpr int N      = ts_keys(PARTS);
     static constexpr int HALVES = D / 64;  // 128-byte column blocks
     static constexpr int QT     = HALVES * TS_M * 128;
-    static constexpr int KT     = HALVES * TS_N * 128;
-    static constexpr int NS     = D == 128 ? (PARTS == 2 ? 4 : 5) : 8;  // tiles in the ring
+    static constexpr int KT     = HALVES * N * 128;
+    static constexpr int NS     = D == 128 ? (PARTS == 3 ? 6 : PARTS == 2 ? 4 : 5) : 8;  // tiles in the ring
     static constexpr int OFF_Q    = 0;
     static constexpr int OFF_RING = OFF_Q + PARTS * QT;
     static constexpr int OFF_XCH  = OFF_RING + NS * KT;           // [stream][row] 16 columns
@@ -93,7 +101,7 @@ struct TsSmem {
     static constexpr int OFF_MISC  = OFF_PIECE + TS_PIECES * 64;
     static constexpr int TOTAL     = OFF_MISC + 32 + 1024;        // + alignment
 };
-static_assert(TsSmem<128, 1>::TOTAL <= 232448 && TsSmem<128, 2>::TOTAL <= 232448 && TsSmem<64, 2>::TOTAL <= 232448, "shared memory");
+static_assert(TsSmem<128, 1>::TOTAL <= 232448 && TsSmem<128, 2>::TOTAL <= 232448 && TsSmem<128, 3>::TOTAL <= 232448 && TsSmem<64, 2>::TOTAL <= 232448, "shared memory");
 
 enum : int {
     TB_FULL   = 0,   // [8] TMA
@@ -135,6 +143,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t * r) {
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t * r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t * r) {
@@ -255,12 +269,13 @@ struct TsSeq {
     int L, nodes, keys, tiles;
 };
 
+template <int N>
 __device__ __forceinline__ TsSeq ts_seq(const TreeAttnParams & p, int s) {
     TsSeq q;
     q.nodes = tree_nodes(p.t, s % p.t.n_tree);
     q.L     = min(max(p.kv_len[s], 0), p.n_kv);
     q.keys  = q.nodes > 0 ? min(q.L + q.nodes, p.n_kv) : 0;
-    q.tiles = (q.keys + TS_N - 1) / TS_N;
+    q.tiles = (q.keys + N - 1) / N;
     return q;
 }
 
@@ -304,6 +319,7 @@ struct __align__(16) TsPiece {
 static_assert(sizeof(TsPiece) == 64, "shared memory");
 
 // A group's pieces, one after another.
+template <int N>
 struct TsPlan {
     const TreeAttnParams & p;
     int                    group, beside, wide, floats;  // floats of a part's slot; a CTA has two
@@ -323,7 +339,7 @@ struct TsPlan {
         TsSeq     own = { 0, 0, 0, 0 };  // the lane's last sequence, its only one where there are up to 32
 #pragma unroll 1
         for (int i = s0; i < s1; i++) {
-            own = ts_seq(p, i);
+            own = ts_seq<N>(p, i);
             mine += own.tiles * heads(own), units += own.tiles > 0 ? heads(own) : 0, most = max(most, own.tiles);
         }
         const int W = __reduce_add_sync(0xffffffffu, mine), U = __reduce_add_sync(0xffffffffu, units);
@@ -342,7 +358,7 @@ struct TsPlan {
                 if (each == 1) {
                     c.tiles = __shfl_sync(0xffffffffu, own.tiles, i), c.nodes = __shfl_sync(0xffffffffu, own.nodes, i);
                 } else {
-                    c = ts_seq(p, i);
+                    c = ts_seq<N>(p, i);
                 }
                 parts += c.tiles > 0 ? ts_up(c.tiles + 1, t) * heads(c) : 0;
             }
@@ -351,7 +367,7 @@ struct TsPlan {
             mine = 0;
 #pragma unroll 1
             for (int i = s0; i < s1; i++) {
-                mine += weight(each == 1 ? own : ts_seq(p, i));
+                mine += weight(each == 1 ? own : ts_seq<N>(p, i));
             }
             from = group, to = group + 1;
         } else {
@@ -374,7 +390,7 @@ struct TsPlan {
         if (each > 1 && (here >> lane & 1u)) {
 #pragma unroll 1
             for (;; i++) {
-                const int n = weight(ts_seq(p, i));
+                const int n = weight(ts_seq<N>(p, i));
                 if (from < at + n) {
                     break;
                 }
@@ -385,7 +401,7 @@ struct TsPlan {
         s = __shfl_sync(0xffffffffu, i, src), first = __shfl_sync(0xffffffffu, at, src);
         q = each == 1 ? TsSeq{ __shfl_sync(0xffffffffu, own.L, src), __shfl_sync(0xffffffffu, own.nodes, src), __shfl_sync(0xffffffffu, own.keys, src),
                                __shfl_sync(0xffffffffu, own.tiles, src) } :
-                        ts_seq(p, s);
+                        ts_seq<N>(p, s);
         x = from, end = to;
         if (!even) {
             x = TsLine::border(x, first + ts_div(x - first, q.tiles + TS_COST) * (q.tiles + TS_COST), q.tiles + TS_COST);
@@ -415,7 +431,7 @@ struct TsPlan {
             const int n = q.tiles > 0 ? length(q) : 0, all = n * heads(q);
             if (x - first >= all) {
                 first += all;
-                q = ts_seq(p, ++s);
+                q = ts_seq<N>(p, ++s);
                 continue;
             }
             const int i = ts_div(x - first, n);  // the unit
@@ -469,8 +485,8 @@ struct TsPlan {
 };
 
 // Rows ra .. ra + 15 of a block's Q for the products, by a warp; rows that do not count are zeros.  All copies are in
-// flight at once, and land where the row's products will read it: PARTS 1, as they are; PARTS 2, a row's bytes lie in
-// the places of its own two parts (F32: all of them), and the warp replaces one row after another.
+// flight at once, and land where the row's products will read it: PARTS 1, as they are; else a row's bytes lie in the
+// places of its own first two parts (F32: all of them), and the warp replaces one row after another.
 template <int D, bool BF16, int PARTS, int UNROLL>
 __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPiece & it, int ra, char * qs, float * factors, int lane) {
     constexpr int E = D / 32, QT = TsSmem<D, PARTS>::QT, BLOCK = TS_M * 128;
@@ -555,19 +571,26 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
                 const bool  odd = top[i] >= 0x7f800000u;
                 const int   ex  = BF16 ? 0 : (top[i] == 0 || odd ? 0 : max((int) (top[i] >> 23) - 127, -112)) - 14;
                 const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
-                uint32_t    hi[E / 2], lo[E / 2];
+                uint32_t    hi[E / 2], lo[E / 2], third[E / 2];
 #pragma unroll
                 for (int e = 0; e < E; e += 2) {
                     const float a = odd ? 0.0f : x[i][e] * dn, b = odd ? 0.0f : x[i][e + 1] * dn;
                     hi[e / 2]      = ts_pack<BF16>(a, b);
                     const float2 f = ts_unpack<BF16>(hi[e / 2]);
                     lo[e / 2]      = ts_pack<BF16>(a - f.x, b - f.y);
+                    if (PARTS == 3) {
+                        const float2 g = ts_unpack<BF16>(lo[e / 2]);
+                        third[e / 2]   = ts_pack<BF16>(a - f.x - g.x, b - f.y - g.y);
+                    }
                 }
                 char * to = qs + (e0 / 64) * BLOCK + (ra + i0 + i) * 128 + ((((e0 % 64) / 8) ^ ((i0 + i) & 7)) << 4) + (e0 % 8) * 2;
 #pragma unroll
                 for (int e = 0; e < E / 2; e++) {
                     reinterpret_cast<uint32_t *>(to)[e]      = hi[e];
                     reinterpret_cast<uint32_t *>(to + QT)[e] = lo[e];
+                    if (PARTS == 3) {
+                        reinterpret_cast<uint32_t *>(to + 2 * QT)[e] = third[e];
+                    }
                 }
                 if (lane == 0) {
                     // (2^-149 for a product below F32's smallest number: the scores are 0 in effect)
@@ -597,7 +620,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TreeAttnParams p, int wide,
                         int groups, int slot_rows, int joined) {
     using L          = TsSmem<D, PARTS>;
-    constexpr int NS = L::NS;
+    constexpr int NS = L::NS, N = L::N;
     extern __shared__ __align__(16) char smem_raw[];
     char *     smem      = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     uint64_t * bar       = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR);
@@ -629,7 +652,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
     TsPiece *      told = reinterpret_cast<TsPiece *>(smem + L::OFF_PIECE);
     TsPiece        it;
     uint32_t       pieces = 0;  // that a warp has taken
-    TsPlan         plan(p, wide, ts_slot_floats(slot_rows, D));
+    TsPlan<N>      plan(p, wide, ts_slot_floats(slot_rows, D));
     if (warp == 0) {
         plan.find(groups);
         told[0] = plan.next();
@@ -689,7 +712,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         mbar_arrive_expect_tx(&bar[TB_FULL + slot], (uint32_t) L::KT);
 #pragma unroll
                         for (int hf = 0; hf < L::HALVES; hf++) {
-                            ts_load(smem + L::OFF_RING + slot * L::KT + hf * (TS_N * 128), tm, hf * 64, tile * TS_N, it.h, it.s, &bar[TB_FULL + slot]);
+                            ts_load(smem + L::OFF_RING + slot * L::KT + hf * (N * 128), tm, hf * 64, tile * N, it.h, it.s, &bar[TB_FULL + slot]);
                         }
                         c++;
                     }
@@ -704,9 +727,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             __syncwarp();
         } else if (warp == 1) {
             // =================================================== products
-            const uint32_t id_qk = ts_idesc(BF16, TS_N, false), id_pv = ts_idesc(BF16, D, true);
+            const uint32_t id_qk = ts_idesc(BF16, N, false), id_pv = ts_idesc(BF16, D, true);
             const uint64_t q_d = sw128_desc(smem_addr(smem + L::OFF_Q), 16, 1024), k_d = sw128_desc(smem_addr(smem + L::OFF_RING), 16, 1024);
-            const uint64_t v_d = sw128_desc(smem_addr(smem + L::OFF_RING), (uint32_t) (TS_N * 128), 1024);
+            const uint64_t v_d = sw128_desc(smem_addr(smem + L::OFF_RING), (uint32_t) (N * 128), 1024);
             auto wait = [&](int b, uint32_t i) {
                 if (ok && !dn_wait_warp(&bar[b], i & 1, deadline)) {
                     ok = false;
@@ -729,10 +752,10 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             for (int hf = 0; hf < L::HALVES; hf++) {
 #pragma unroll
                                 for (int k = 0; k < 4; k++) {
-                                    umma_f16(tmem + (uint32_t) (buf * TS_N), qa + (uint64_t) (2 * k), kb + (uint64_t) (2 * k), id_qk,
+                                    umma_f16(tmem + (uint32_t) (buf * TS_S), qa + (uint64_t) (2 * k), kb + (uint64_t) (2 * k), id_qk,
                                              PARTS - 1 - part + hf + k > 0 ? 1u : 0u);
                                 }
-                                qa += (TS_M * 128) >> 4, kb += (TS_N * 128) >> 4;
+                                qa += (TS_M * 128) >> 4, kb += (N * 128) >> 4;
                             }
                         }
                         umma_commit(&bar[TB_EMPTY + slot]);
@@ -747,7 +770,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     }
                     const int slot = (int) (c % NS), buf = (int) (tc & 1);
                     wait(TB_FULL + slot, c / NS);
-                    const bool nodes = (j + 1) * TS_N > it.L;
+                    const bool nodes = (j + 1) * N > it.L;
                     if (nodes && lane == 0) {
                         dn_mbar_arrive(&bar[TB_LOOK]);
                     }
@@ -757,18 +780,19 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     }
 #pragma unroll 1
                     for (int part = PARTS - 1; part >= 0; part--) {
-                        uint32_t pa = tmem + (uint32_t) (buf * TS_N + part * 8);
+                        // P of 16 keys: 8 columns, then 8 of its remainder; a second remainder behind them all
+                        const uint32_t pa = tmem + (uint32_t) (buf * TS_S + (part == 2 ? N : part * 8)), keys16 = PARTS == 1 || part == 2 ? 8u : 16u;
                         uint64_t vb = v_d + (uint64_t) ((slot * L::KT) >> 4);
-                        uint32_t add = PARTS == 2 ? (uint32_t) (PARTS - 1 - part) : j - it.a < 2 ? 0u : 1u;
+                        uint32_t add = PARTS >= 2 ? (uint32_t) (PARTS - 1 - part) : j - it.a < 2 ? 0u : 1u;
 #pragma unroll
-                        for (int k = 0; k < 8; k++) {  // P of 16 keys: 8 columns, then 8 of its remainder
-                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), pa + (uint32_t) (k * 8 * PARTS), vb + (uint64_t) ((k * 16 * 128) >> 4),
+                        for (int k = 0; k < N / 16; k++) {
+                            umma_f16_ts(tmem + 256u + (uint32_t) (buf * D), pa + (uint32_t) k * keys16, vb + (uint64_t) ((k * 16 * 128) >> 4),
                                         id_pv, add);
                             add = 1u;
                         }
                     }
                     umma_commit(&bar[TB_EMPTY + slot]);
-                    if (PARTS == 2 || j + 2 >= it.b) {
+                    if (PARTS >= 2 || j + 2 >= it.b) {
                         umma_commit(&bar[TB_OFULL + buf]);
                     }
                     c++, tc++;
@@ -795,7 +819,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     dn_mbar_arrive(&bar[TB_QREADY + (pieces & 1)]);
                 }
 #pragma unroll 1
-                for (int j = max(it.a, it.L / TS_N); j < it.b; j++) {
+                for (int j = max(it.a, it.L / N); j < it.b; j++) {
                     const uint32_t i    = c + (uint32_t) (2 * (j - it.a) + (j + 1 < it.b ? 2 : 1));  // its place in the ring's order
                     const int      slot = (int) (i % NS);
                     // (warp 1 has seen the tile land and keeps its place until it is looked at, so that the second wait
@@ -809,9 +833,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     // the product and the next piece's Q wait for this).
                     constexpr int      PER_ROW = 8 * L::HALVES, STEP = 64 / PER_ROW;
                     constexpr uint32_t EXP = BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = BF16 ? 0x00800080u : 0x04000400u;
-                    const int          ck = t64 % PER_ROW, end = min(it.keys - j * TS_N, TS_N);
-                    char *             col = tile + (ck >> 3) * (TS_N * 128) + (ck & 7) * 16;
-                    const int          first = max(0, it.L - j * TS_N) + t64 / PER_ROW;
+                    const int          ck = t64 % PER_ROW, end = min(it.keys - j * N, N);
+                    char *             col = tile + (ck >> 3) * (N * 128) + (ck & 7) * 16;
+                    const int          first = max(0, it.L - j * N) + t64 / PER_ROW;
                     bool               odd = false;
 #pragma unroll 1
                     for (int row = first; row < end; row += 4 * STEP) {
@@ -831,7 +855,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         }
                     }
 #pragma unroll 1
-                    for (int row = first + max(0, (end - first + STEP - 1) / STEP) * STEP; row < TS_N; row += STEP) {
+                    for (int row = first + max(0, (end - first + STEP - 1) / STEP) * STEP; row < N; row += STEP) {
                         *reinterpret_cast<uint4 *>(col + row * 128) = make_uint4(0, 0, 0, 0);
                     }
                     if (odd) {
@@ -853,7 +877,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
         regs_inc<TS_REGS_SOFTMAX>();
         const int      w = wg - 1, quad = warp & 3, r = quad * 32 + lane, own = tid - 128;
         const uint32_t tl    = (uint32_t) (quad * 32) << 16;
-        const uint32_t s_col = tmem + tl + (uint32_t) (w * TS_N), o_col = tmem + tl + 256u + (uint32_t) (w * D);
+        const uint32_t s_col = tmem + tl + (uint32_t) (w * TS_S), o_col = tmem + tl + 256u + (uint32_t) (w * D);
         const bool     cap = p.softcap > 0.0f;
         float4 *       turn = reinterpret_cast<float4 *>(smem + L::OFF_XCH) + w * (TS_M * 4);  // 16 columns of a warp's rows, on their way out
         uint32_t       tc = 0, used = 0;
@@ -878,7 +902,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             const uint32_t * bits = anc + min(my_node, TREE_MAX - 1) * (TREE_MAX / 32);
             const bool      live = r < it.rows, warp_live = quad * 32 < it.rows;
             // ---- Q of the first piece, and each node's ancestors, where the piece has tiles with nodes
-            const bool tail = tile1 * TS_N > held;
+            const bool tail = tile1 * N > held;
             {
                 const int nodes = it.nodes, parent = tail && own < nodes ? tree_parent(p.t, it.s % p.t.n_tree, own) : -1;
                 if (pieces == 0) {
@@ -925,9 +949,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 const uint32_t lo = bits[o >> 5], hi = o + 32 < TREE_MAX ? bits[(o >> 5) + 1] : 0u;
                 return __funnelshift_r(lo, hi, o & 31);
             };
-            float m = -INFINITY, l = 0.0f, acc[PARTS == 2 ? D : 1];
+            float m = -INFINITY, l = 0.0f, acc[PARTS >= 2 ? D : 1];
             bool  any = false;  // the stream has a tile of the piece
-            if constexpr (PARTS == 2) {
+            if constexpr (PARTS >= 2) {
 #pragma unroll
                 for (int e = 0; e < D; e++) {
                     acc[e] = 0.0f;
@@ -942,7 +966,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 if (warp_live && cap) {  // over S: s = cap * tanh(S * factor), in log2 units
                     const float fcap = f0 != f0 ? 1.0f : f0;
 #pragma unroll 1
-                    for (int c = 0; c < 8; c++) {
+                    for (int c = 0; c < N / 16; c++) {
                         uint32_t v[16];
                         tmem_ld16(s_col + (uint32_t) (c * 16), v);
                         tmem_ld16_wait(v);
@@ -954,12 +978,12 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     }
                     tmem_st_wait();
                 }
-                if (warp_live && (j + 1) * TS_N > held) {  // over S: -inf for a key that the row does not see
+                if (warp_live && (j + 1) * N > held) {  // over S: -inf for a key that the row does not see
 #pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
+                    for (int c = 0; c < N / 32; c++) {
                         uint32_t v[32];
                         tmem_ld32(s_col + (uint32_t) (c * 32), v);
-                        const uint32_t see = live ? seen(j * TS_N + c * 32) : 0u;
+                        const uint32_t see = live ? seen(j * N + c * 32) : 0u;
                         tmem_ld_wait_tie(v);
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
@@ -971,7 +995,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
                 if constexpr (PARTS == 1) {
                     if (warp_live) {
-                        uint32_t v[TS_N];
+                        uint32_t v[N];
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
                             tmem_ld32(s_col + (uint32_t) (c * 32), &v[c * 32]);
@@ -982,11 +1006,11 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         }
                         float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
 #pragma unroll
-                        for (int e = 2; e < TS_N - 2; e += 4) {
+                        for (int e = 2; e < N - 2; e += 4) {
                             a = fmax3(a, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
                             b = fmax3(b, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
                         }
-                        const float top = fmaxf(fmax3(a, __uint_as_float(v[TS_N - 2]), __uint_as_float(v[TS_N - 1])), b);
+                        const float top = fmaxf(fmax3(a, __uint_as_float(v[N - 2]), __uint_as_float(v[N - 1])), b);
                         const float mn   = fmaxf(m, top * factor);
                         const bool  grew = mn > m + (float) TS_GROW;  // (at first too)
                         if (any && __any_sync(0xffffffffu, grew)) {
@@ -1036,7 +1060,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     if (warp_live) {
                         float top = -INFINITY;
 #pragma unroll 1
-                        for (int c = 0; c < 4; c++) {
+                        for (int c = 0; c < N / 32; c++) {
                             uint32_t v[32];
                             tmem_ld32(s_col + (uint32_t) (c * 32), v);
                             tmem_ld_wait_tie(v);
@@ -1057,7 +1081,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         // 16 columns and the load of the next ones; over them 8 of the weights' first part and 8 of the second
                         uint32_t v[2][16];
                         auto     weights = [&](uint32_t (&s16)[16], int c) {
-                            uint32_t hi[16];
+                            uint32_t hi[16], third[8];
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
                                 float x, y;
@@ -1069,19 +1093,30 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                                 // the sign of the other part's (2^-38 of the row's largest weight is far below F32's last bit)
                                 hi[i] = ts_pack_rz<BF16>(x, y);
                                 const float2 f = ts_unpack<BF16>(hi[i]);
+                                const uint32_t least = __vminu2(hi[i], BF16 ? 0x00800080u : 0x00010001u);
                                 f2unpack(ffma2(f2pack(f.x, f.y), f2pack(-1.0f, -1.0f), p2), x, y);
-                                hi[8 + i] = __vmaxu2(ts_pack<BF16>(x, y), __vminu2(hi[i], BF16 ? 0x00800080u : 0x00010001u));
+                                if constexpr (PARTS == 3) {
+                                    const uint32_t mid = ts_pack_rz<BF16>(x, y);
+                                    const float2   g   = ts_unpack<BF16>(mid);
+                                    hi[8 + i] = __vmaxu2(mid, least);
+                                    third[i]  = __vmaxu2(ts_pack<BF16>(x - g.x, y - g.y), least);
+                                } else {
+                                    hi[8 + i] = __vmaxu2(ts_pack<BF16>(x, y), least);
+                                }
                             }
                             tmem_st16(s_col + (uint32_t) (c * 16), hi);
+                            if constexpr (PARTS == 3) {
+                                tmem_st8(s_col + (uint32_t) (N + c * 8), third);
+                            }
                         };
                         tmem_ld16(s_col, v[0]);
                         tmem_ld16_wait(v[0]);
 #pragma unroll 1
-                        for (int c = 0; c < 8; c += 2) {
+                        for (int c = 0; c < N / 16; c += 2) {
                             tmem_ld16(s_col + (uint32_t) (c * 16 + 16), v[1]);
                             weights(v[0], c);
                             tmem_ld16_wait(v[1]);
-                            if (c < 6) {
+                            if (c + 2 < N / 16) {
                                 tmem_ld16(s_col + (uint32_t) (c * 16 + 32), v[0]);
                             }
                             weights(v[1], c + 1);
@@ -1111,7 +1146,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
             }
             // ---- the two streams' maxima and sums
-            if constexpr (PARTS == 2) {  // to where PARTS 1 has them
+            if constexpr (PARTS >= 2) {  // to where PARTS 1 has them
 #pragma unroll
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t o[32];
@@ -1150,7 +1185,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
             // warpgroup's warps reach the lanes of the other's; the loop's head holds the next piece's products back)
             const bool odd = tail && dirty[pieces & 3] && live;
             // (PARTS 1: what is there is the piece's where the stream had a tile of it)
-            const bool mine_is = PARTS == 2 || any, theirs_is = PARTS == 2 || !any || tile1 - tile0 > 1;
+            const bool mine_is = PARTS >= 2 || any, theirs_is = PARTS >= 2 || !any || tile1 - tile0 > 1;
             const int  swz = (r >> 1) & 3;
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
@@ -1170,7 +1205,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
 #pragma unroll 1
                     for (int n = 0; n < it.nodes; n++) {
                         const int key = held + n;
-                        if (key / TS_N < tile0 || key / TS_N >= tile1 || !(bits[n >> 5] >> (n & 31) & 1u)) {
+                        if (key / N < tile0 || key / N >= tile1 || !(bits[n >> 5] >> (n & 31) & 1u)) {
                             continue;
                         }
                         const uint16_t * v = reinterpret_cast<const uint16_t *>(p.v.data + (int64_t) key * p.v.nb1 + (int64_t) it.h * p.v.nb2 + (int64_t) it.s * p.v.nb3) + mine;
@@ -1344,7 +1379,7 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
     if (regs != TS_REGS_LAUNCH) {
         return cudaErrorInvalidConfiguration;
     }
-    constexpr int smem = TsSmem<D, PARTS>::TOTAL;
+    constexpr int smem = TsSmem<D, PARTS>::TOTAL, N = TsSmem<D, PARTS>::N;
     cudaError_t   e    = once.smem(kern, smem);
     if (e != cudaSuccess) {
         return e;
@@ -1353,14 +1388,14 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
     for (CUtensorMap * tm : { &tmk, &tmv }) {
         const Kv8Rows & x = tm == &tmk ? p.k : p.v;
         // (the stride of a slab's only row is never stepped, and may be one that a map does not take)
-        if (!encode_kv_tensor_map(tm, x.data, BF16, D, p.n_kv, p.n_head_kv, p.n_seq, p.n_kv > 1 ? x.nb1 : 2 * D, x.nb2, x.nb3, TS_N)) {
+        if (!encode_kv_tensor_map(tm, x.data, BF16, D, p.n_kv, p.n_head_kv, p.n_seq, p.n_kv > 1 ? x.nb1 : 2 * D, x.nb2, x.nb3, N)) {
             return cudaErrorInvalidValue;
         }
     }
-    const int wide = tree_attn_wide(p), groups = tree_attn_groups(p, sms);
+    const int wide = tree_attn_wide(p), groups = tree_attn_groups(p, N, sms);
     const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
-    e = kv8_launch(kern, dim3((unsigned) (groups * wide)), TS_THREADS, smem, stream, tmk, tmv, p, wide, groups, rows, p.n_kv <= TS_LEAST * TS_N ? 0 : 1);
-    if (e != cudaSuccess || p.n_kv <= TS_LEAST * TS_N) {
+    e = kv8_launch(kern, dim3((unsigned) (groups * wide)), TS_THREADS, smem, stream, tmk, tmv, p, wide, groups, rows, p.n_kv <= TS_LEAST * N ? 0 : 1);
+    if (e != cudaSuccess || p.n_kv <= TS_LEAST * N) {
         return e;  // (no unit is in parts)
     }
     const int items = groups * wide * ((rows + 31) / 32) * (D / 4);
@@ -1369,16 +1404,30 @@ cudaError_t launch_one(const TreeAttnParams & p, int sms, cudaStream_t stream) {
 
 template <int D, bool BF16>
 cudaError_t launch_d(const TreeAttnParams & p, int sms, cudaStream_t stream) {
-    // one part where q is the cache's type, the result has no more bits, and the truncated sums stay small
-    return p.q.type == p.k.type && p.o.type == p.q.type && p.n_kv <= TS_LONG ? launch_one<D, BF16, 1>(p, sms, stream) : launch_one<D, BF16, 2>(p, sms, stream);
+    // one part where q is the cache's type, the result has no more bits, and the truncated sums stay small; three where two
+    // would not give what an F32 result holds
+    if (p.q.type == p.k.type && p.o.type == p.q.type && p.n_kv <= TS_LONG) {
+        return launch_one<D, BF16, 1>(p, sms, stream);
+    }
+    if constexpr (BF16) {
+        if (p.o.type == KV_F32) {
+            return launch_one<D, BF16, 3>(p, sms, stream);
+        }
+    }
+    return launch_one<D, BF16, 2>(p, sms, stream);
 }
 
 }  // namespace
 
+// keys of a tile, at least: the result's type decides, which neither the choice of kernel nor the workspace's size goes by
+static int least_keys(const TreeAttnParams & p) {
+    return ts_keys(p.k.type == KV_BF16 ? 3 : 2);
+}
+
 // 16-bit slabs at D = 64 and 128
 bool tree_attn_tc_sizes(const TreeAttnParams & p) {
     return (p.k.type == KV_F16 || p.k.type == KV_BF16) && (p.D == 64 || p.D == 128) && tensor_maps_available() &&
-           (int64_t) p.n_seq * p.n_head_kv * ((p.t.max_nodes * p.ratio + TS_M - 1) / TS_M) * ((p.n_kv + TS_N - 1) / TS_N + TS_COST) < (1 << 30);
+           (int64_t) p.n_seq * p.n_head_kv * ((p.t.max_nodes * p.ratio + TS_M - 1) / TS_M) * ((p.n_kv + least_keys(p) - 1) / least_keys(p) + TS_COST) < (1 << 30);
 }
 
 // of these, slabs whose strides a tensor map takes
@@ -1397,15 +1446,15 @@ int tree_attn_wide(const TreeAttnParams & p) {
     return p.t.n_nodes ? 1 : (p.t.max_nodes * p.ratio + TS_M - 1) / TS_M;
 }
 
-int tree_attn_groups(const TreeAttnParams & p, int sms) {
+int tree_attn_groups(const TreeAttnParams & p, int keys, int sms) {
     const int64_t blocks = (p.t.max_nodes * p.ratio + TS_M - 1) / TS_M, wide = tree_attn_wide(p);
-    const int64_t tiles = (int64_t) p.n_seq * p.n_head_kv * ((p.n_kv + TS_N - 1) / TS_N) * (wide == 1 ? blocks : 1);
+    const int64_t tiles = (int64_t) p.n_seq * p.n_head_kv * ((p.n_kv + keys - 1) / keys) * (wide == 1 ? blocks : 1);
     return (int) std::max<int64_t>(1, std::min<int64_t>(sms / wide, tiles));
 }
 
 size_t tree_attn_tc_workspace(const TreeAttnParams & p, int sms) {
     const int rows = std::min(p.t.max_nodes * p.ratio, TS_M);
-    return KV8_WS_ZEROED + (size_t) tree_attn_groups(p, sms) * tree_attn_wide(p) * 2 * ts_slot_floats(rows, p.D) * 4;
+    return KV8_WS_ZEROED + (size_t) tree_attn_groups(p, least_keys(p), sms) * tree_attn_wide(p) * 2 * ts_slot_floats(rows, p.D) * 4;
 }
 
 cudaError_t launch_tree_attn_tc(TreeAttnParams p, int sms, cudaStream_t stream) {

@@ -140,3 +140,19 @@ def test_verify_decisions_next_to_their_border(cuda_device, V, kind):
         path, n_path, token = tree.verify(logits, tokens[:, :T].contiguous(), accept[:, :T].contiguous(), torch.full((n,), 0.3, device=cuda_device),
                                           draft=drafts, temperature=temperature)
         assert ((n_path == 2) == taken).all() and (path[:, 1] == (T - 1 if taken else -1)).all(), (kind, taken)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D,H,Hkv,T,lens", [(128, 8, 2, 5, [3, 250]), (64, 8, 2, 24, [1000, 63, 64, 65, 2500]), (128, 32, 8, 24, [4000, 3000]),
+                                            (128, 16, 2, 70, [190, 191, 192, 193, 1200]), (64, 4, 4, 1, [0, 1, 127, 128])])
+@pytest.mark.parametrize("cache", ["bf16", "f16"])
+def test_attend_f32_results_keep_f32s_precision(cuda_device, D, H, Hkv, T, lens, dtype, cache):
+    """The error of all rows together, as random as the inputs: of a weight, by the roundings of its exponent (four, of numbers
+    around 7: 3.3e-7 by root mean square), 2^x (1.4e-7) and what the tensor core's sums of a score, whose last 8 additions are of
+    its size, lose towards zero (3e-7); of a result, by those of its own (8 a tile: 4e-7).  Together 7e-7; 2^-19 allows for some
+    2.5 times that.  (q and weights of 16 bits are off by 3.5e-6.)"""
+    c = Case(cuda_device, lens, 1, H, Hkv, D, T, dtype, cache, seed=T + D)
+    got = c.check(out=c.out(torch.float32))
+    want, _ = R.attend(c.q, c.k, c.v, c.parents, None, c.len, c.scale, c.out(torch.float32))
+    off = ((got.double() - want).norm() / want.norm()).item()
+    assert off <= 2.0 ** -19, off
