@@ -494,9 +494,7 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
     // lane i, and 16 + i: the address of row i (of the last one, behind it)
     const int      rl = it.rb * TS_M + max(min(ra + (lane & 15), it.rows - 1), 0), nl = rl / p.ratio, hl = it.h * p.ratio + rl - nl * p.ratio;
     const uint64_t al = reinterpret_cast<uint64_t>(p.q.data + (int64_t) nl * p.q.nb1 + (int64_t) hl * p.q.nb2 + (int64_t) it.s * p.q.nb3);
-    // what a score is multiplied by is above 0 and finite: 0 by the -inf of a key that is not seen, and an infinity by a score of
-    // 0, would be no number
-    const float    by = fminf(fmaxf(fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E), 0x1p-126f), TS_MOST);
+    const float    by = fabsf(p.softcap > 0.0f ? p.scale / p.softcap : p.scale * LOG2E);
     // chunk ck of 16 bytes of row i: block ck / 8 of 64 columns (F32: the two blocks of either part in turn)
     auto place = [&](int i, int ck) {
         const int blk = ck >> 3;
@@ -593,8 +591,7 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
                     }
                 }
                 if (lane == 0) {
-                    // (2^-149 for a product below F32's smallest number: the scores are 0 in effect)
-                    factors[ra + i0 + i] = odd ? NAN : fminf(fmaxf(__uint_as_float((uint32_t) (127 + ex) << 23) * by, 0x1p-149f), TS_MOST);
+                    factors[ra + i0 + i] = odd ? NAN : __uint_as_float((uint32_t) (127 + ex) << 23) * by;
                 }
             }
         }
@@ -933,7 +930,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
             }
             wait(TB_QREADY + (int) (pieces & 1), pieces >> 1);
-            const float f0 = factors[(pieces & 1) * TS_M + r], factor = cap || f0 != f0 ? 1.0f : f0;
+            // What a score is multiplied by is above 0 and finite: 0 by the -inf of a key that is not seen, and an infinity by a
+            // score of 0, would be no number.  (Where scale and q's powers of two give a product below 2^-149, the scores are 0 in effect)
+            const float f0 = factors[(pieces & 1) * TS_M + r], fx = f0 != f0 ? 1.0f : fminf(fmaxf(f0, 0x1p-149f), TS_MOST), factor = cap ? 1.0f : fx;
             // which of the 32 keys from k0 on the row sees
             auto seen = [&](int k0) -> uint32_t {
                 const int o = k0 - held;  // in nodes
@@ -964,7 +963,6 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                 }
                 wait(TB_SFULL + w, tc >> 1);
                 if (warp_live && cap) {  // over S: s = cap * tanh(S * factor), in log2 units
-                    const float fcap = f0 != f0 ? 1.0f : f0;
 #pragma unroll 1
                     for (int c = 0; c < N / 16; c++) {
                         uint32_t v[16];
@@ -972,7 +970,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         tmem_ld16_wait(v);
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fcap) * (p.softcap * LOG2E));
+                            v[e] = __float_as_uint(ts_tanh(__uint_as_float(v[e]) * fx) * (p.softcap * LOG2E));
                         }
                         tmem_st16(s_col + (uint32_t) (c * 16), v);
                     }
