@@ -29,13 +29,13 @@
 // Numerics.  Where q has the cache's type and the result no more bits (PARTS 1), O stays in TMEM and is multiplied there when
 // a row's maximum grows by more than 2^TS_GROW.  The tensor core truncates what it adds to an accumulator, up to 2^-23 of it in
 // each step of 16 keys, always towards zero (measured 7e-7 a tile of 128 keys): up to TS_LONG keys a stream's sum stays within
-// 1e-4, a fifth of F16's half step.  Else (PARTS 2) q is two parts of the cache's type (F16: brought to [2^14, 2^15) at its row's largest
-// element by a power of two), and so are the weights, the remainder's product first, where the accumulator is small;
+// 1e-4, a fifth of F16's half step.  Else (PARTS 2) q is two parts of the cache's type (brought to [2^14, 2^15), BF16 to [1, 2), at
+// its row's largest element by a power of two), and so are the weights, the remainder's product first, where the accumulator is small;
 // every tile's P V starts afresh and is added in registers, rounded to nearest: 22 bits of q and weights in F16 (an F32 result
 // is off by 5e-7 of its norm), 16 in BF16, which F32 results over BF16 slabs take three parts for (PARTS 3: 24 bits; 4e-7 of the
 // norm, 3.5e-6 with two), in tiles of 64 keys, as TMEM has no place for three parts of 128.  2 x 8192, 24 nodes: PARTS 1 22 us
-// (BF16), 2 31, 3 38; 64 nodes: 32, 49, 67; 48 sequences of up to 10240, 13 nodes: 166, 249, 381 (tiles of 80 keys, the most that
-// TMEM takes: 39, 70 and 375).
+// (BF16), 2 31, 3 39; 64 nodes: 32, 49, 68; 48 sequences of up to 10240, 13 nodes: 166, 249, 355 (tiles of 80 keys, the most that
+// TMEM takes, were no faster).
 //
 // Bound: HBM for batches at full clock (48 sequences of 1 to 10240, 13 nodes, BF16, 1013 MB: 166 us, 6.1 TB/s, at 1965 MHz; under a
 // lasting load the power cap takes the clock to 1430-1550 MHz, and the tiles' own work counts too: 177-188); few sequences
@@ -73,9 +73,10 @@ constexpr int TS_REGS_SOFTMAX = 208;  // 2 x 208 + 88 = 3 x 168
 constexpr int TS_REGS_ISSUE   = 88;
 static_assert(2 * TS_REGS_SOFTMAX + TS_REGS_ISSUE <= 3 * TS_REGS_LAUNCH, "more registers than the launch has");
 
-// log2 of what a weight at the maximum is held as: F16 keeps 11 bits of one down to 2^-(14 + offset) of it, and holds 2^15
-template <int PARTS>
-constexpr float TS_OFF = PARTS >= 2 ? 14.0f : 15.0f - TS_GROW;
+// log2 of what a weight at the maximum is held as: F16 keeps 11 bits of one down to 2^-(14 + offset) of it, and holds 2^15;
+// BF16, whose small numbers go as far as F32's, holds none above 1, so that sums of large values stay in F32
+template <bool BF16, int PARTS>
+constexpr float TS_OFF = BF16 ? (PARTS >= 2 ? 0.0f : -(float) TS_GROW) : PARTS >= 2 ? 14.0f : 15.0f - TS_GROW;
 
 // keys of a tile: three parts of the weights of 128 keys would have no place in TMEM
 __host__ __device__ constexpr int ts_keys(int parts) {
@@ -567,7 +568,9 @@ __device__ __forceinline__ void ts_stage16(const TreeAttnParams & p, const TsPie
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const bool  odd = top[i] >= 0x7f800000u;
-                const int   ex  = BF16 ? 0 : (top[i] == 0 || odd ? 0 : max((int) (top[i] >> 23) - 127, -112)) - 14;
+                // the row's largest element: F16 to [2^14, 2^15), where its remainders are no small numbers, BF16 to [1, 2) (4)
+                const int   ex  = BF16 ? (top[i] == 0 || odd ? 0 : min(max((int) (top[i] >> 23) - 127, -126), 126)) :
+                                         (top[i] == 0 || odd ? 0 : max((int) (top[i] >> 23) - 127, -112)) - 14;
                 const float dn  = __uint_as_float((uint32_t) (127 - ex) << 23) * sign;
                 uint32_t    hi[E / 2], lo[E / 2], third[E / 2];
 #pragma unroll
@@ -808,8 +811,9 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                     if (ok && !dn_wait_warp(&bar[TB_QFREE], (pieces - 1) & 1, deadline)) {
                         ok = false;
                     }
+                    // (what lies in rows behind the piece's stays: nothing of theirs is kept.  48 sequences of 52 rows: 355 us, 418)
 #pragma unroll 1
-                    for (int ra = (warp & 1) * 16; ra < TS_M; ra += 32) {
+                    for (int ra = (warp & 1) * 16; ra < it.rows; ra += 32) {
                         ts_stage16<D, BF16, PARTS, 1>(p, it, ra, smem + L::OFF_Q, factors + (pieces & 1) * TS_M, lane);
                     }
                     fence_proxy_async_smem();
@@ -1028,7 +1032,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                             }
                         }
                         m = grew ? mn : m;
-                        const float    nm = (m == -INFINITY ? 0.0f : -m) + TS_OFF<PARTS>;
+                        const float    nm = (m == -INFINITY ? 0.0f : -m) + TS_OFF<BF16, PARTS>;
                         const uint64_t nm2 = f2pack(nm, nm), fa2 = f2pack(factor, factor);
                         uint64_t       sum2 = 0ull;
 #pragma unroll
@@ -1073,7 +1077,7 @@ __global__ void __launch_bounds__(TS_THREADS, 1)
                         const float mn = fmaxf(m, top * factor);
                         g = m == mn ? 1.0f : ex2(m - mn);
                         m = mn;
-                        const float    nm = (m == -INFINITY ? 0.0f : -m) + TS_OFF<PARTS>;
+                        const float    nm = (m == -INFINITY ? 0.0f : -m) + TS_OFF<BF16, PARTS>;
                         const uint64_t nm2 = f2pack(nm, nm), fa2 = f2pack(factor, factor);
                         uint64_t       sum2 = 0ull;
                         // 16 columns and the load of the next ones; over them 8 of the weights' first part and 8 of the second

@@ -156,3 +156,28 @@ def test_attend_f32_results_keep_f32s_precision(cuda_device, D, H, Hkv, T, lens,
     want, _ = R.attend(c.q, c.k, c.v, c.parents, None, c.len, c.scale, c.out(torch.float32))
     off = ((got.double() - want).norm() / want.norm()).item()
     assert off <= 2.0 ** -19, off
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "bf16"), ("bf16", "bf16"), ("f16", "bf16"), ("f32", "f16"), ("bf16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_numbers_near_the_ends_of_f32(cuda_device, D, dtype, cache):
+    """Queries, keys and values far from 1, with a scale that brings the scores back: the results are the same but for a power of two."""
+    c = Case(cuda_device, [300, 5, 127], 1, 8, 2, D, 10, dtype, cache, seed=D + 1)
+    out = c.out(torch.float32)
+    q, k, v, scale = c.q, c.k, c.v, c.scale
+    for up in (120, 90, -90, -118):
+        if dtype != "f16":
+            c.q = (q.float() * 2.0 ** up).to(q.dtype)
+            c.check(out=out.clone(), scale=scale * 2.0 ** -up)
+        c.q = q
+        if cache != "f16":
+            c.k = (k.float() * 2.0 ** up).to(k.dtype)
+            c.check(out=out.clone(), scale=scale * 2.0 ** -up)
+            c.k = k
+            if up < 0:  # (rows far below the smallest numbers that results have are not asked for)
+                continue
+            c.v = (v.float() * 2.0 ** (up - 5)).to(v.dtype)
+            c.check(out=out.clone())
+            if dtype == cache:
+                c.check(out=c.out())
+            c.v = v
