@@ -181,3 +181,55 @@ def test_attend_numbers_near_the_ends_of_f32(cuda_device, D, dtype, cache):
             if dtype == cache:
                 c.check(out=c.out())
             c.v = v
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+@pytest.mark.parametrize("N,H,Hkv,T,most", [(20, 32, 8, 40, 3000), (7, 48, 8, 100, 700), (90, 16, 2, 33, 400)])
+def test_attend_groups_of_ctas_on_the_line(cuda_device, N, H, Hkv, T, most, dtype, cache):
+    """More units than groups, of several CTAs each: every tree has all its nodes and more than 128 rows a kv head."""
+    lens = [(i * 1237) % most for i in range(N)]
+    Case(cuda_device, lens, 1, H, Hkv, 128, T, dtype, cache, seed=N).check()
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "f16"), ("bf16", "bf16"), ("f32", "bf16")])
+@pytest.mark.parametrize("N,ratio,most,nodes", [(40, 4, 3000, None), (97, 8, 900, True), (140, 1, 2000, None), (33, 40, 1500, None)])
+def test_attend_even_parts_of_many_sequences(cuda_device, N, ratio, most, nodes, dtype, cache):
+    """Fewer units than CTAs, and more than 32 sequences: each lane of a planning warp has several."""
+    T = 3
+    lens = [(i * 1237) % most for i in range(N)]
+    Case(cuda_device, lens, N if nodes else 1, ratio, 1, 128, T, dtype, cache, seed=N, n_nodes=[i % (T + 1) for i in range(N)] if nodes else None).check()
+
+
+def far_apart(x, sets_apart):
+    """x (2, Hkv, rows, ...) copied to memory whose second set begins more than 2^32 bytes behind the first."""
+    big = torch.empty(sets_apart + x[0].numel(), dtype=x.dtype, device=x.device)
+    view = big.as_strided(x.shape, (sets_apart, *x[0].contiguous().stride()))
+    view.copy_(x)
+    return view
+
+
+@pytest.mark.parametrize("dtype,cache,odd", [("f32", "f32", 0), ("f32", "f16", 0), ("f32", "f16", 1), ("bf16", "bf16", 0)])
+def test_attend_sets_more_than_4_gib_apart(cuda_device, dtype, cache, odd):
+    """K and V of the second set behind 2^32 bytes, for the tensor-core kernel and the others (rows that are not aligned)."""
+    c = Case(cuda_device, [300, 77], 1, 8, 2, 128, 6, dtype, cache, seed=20)
+    apart = ((1 << 32) + (1 << 20)) // c.k.element_size() + odd
+    c.k, c.v = far_apart(c.k, apart), far_apart(c.v, apart)
+    assert c.k.stride(0) * c.k.element_size() > 1 << 32
+    c.check()
+
+
+def test_commit_and_verify_more_than_4_gib_apart(cuda_device):
+    rng = random.Random(4)
+    T, n = 20, 9
+    k, v = (slabs(cuda_device, 2, 2, 2, 60, 64, "f16", seed) for seed in (1, 2))
+    apart = ((1 << 32) + (1 << 20)) // 2
+    far = [[far_apart(x, apart) for x in xs] for xs in (k, v)]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)
+    path, lens = ints([rising(rng, T, n)]), ints([13, 38])
+    want = [R.commit(xs, path, ints([n]), lens)[0] for xs in (k, v)]
+    mm3fa.DraftTree(ints([[-1] * T])).commit(mm3fa.CacheLayers(*far), path, ints([n]), lens)
+    assert all(torch.equal(a, b) for xs, ws in zip(far, want) for a, b in zip(xs, ws))
+
+    def edit(s, par):
+        s["logits"] = far_apart(s["logits"], ((1 << 32) + (1 << 20)) // 4)
+    check_verify(cuda_device, 2, 12, 1025, "f32", None, 0.9, seed=3, edit=edit)
