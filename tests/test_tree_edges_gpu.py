@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import mm3fa
+import test_tree_gpu as base
 import tree_ref as R
 from test_tree_gpu import Case, check_verify, rising, slabs
 
@@ -233,3 +234,52 @@ def test_commit_and_verify_more_than_4_gib_apart(cuda_device):
     def edit(s, par):
         s["logits"] = far_apart(s["logits"], ((1 << 32) + (1 << 20)) // 4)
     check_verify(cuda_device, 2, 12, 1025, "f32", None, 0.9, seed=3, edit=edit)
+
+
+THREE = ("f32", "bf16")  # F32 results over BF16 slabs: three parts of q and weights, tiles of 64 keys
+
+
+@pytest.mark.parametrize("T,H,Hkv,lens", [(40, 8, 2, [500, 0, 77, 260]), (128, 4, 1, [200, 31, 1, 129]), (256, 5, 1, [300, 2, 3, 4]), (67, 3, 3, [10, 400, 5, 6])])
+def test_attend_large_trees_in_three_parts(cuda_device, T, H, Hkv, lens):
+    base.test_attend_large_trees(cuda_device, T, H, Hkv, lens, *THREE)
+
+
+def test_attend_what_is_seen_in_three_parts(cuda_device):
+    """What is not seen, infinite values that are, in one of a CTA's units and between others, slabs' ends."""
+    base.test_attend_what_is_not_seen_has_no_influence(cuda_device, *THREE)
+    base.test_attend_infinite_values_that_are_seen(cuda_device, *THREE)
+    base.test_attend_infinite_values_in_some_of_many(cuda_device, *THREE)
+    c = Case(cuda_device, [128, 133, 140, 139], 1, 4, 2, 128, 9, *THREE, rows=140)
+    c.len += torch.tensor([0, 0, 50, 0], dtype=torch.int32, device=cuda_device)
+    c.check()
+    for par in ([i - 1 for i in range(70)], [-1] + [0] * 69, [-1] * 70):
+        Case(cuda_device, [90, 128], 1, 4, 2, 64, 70, *THREE, seed=3, parents=[par]).check()
+
+
+@pytest.mark.parametrize("lens", [[(i * 37) % 100 for i in range(64)], [(i * 211) % 1500 for i in range(48)]])
+def test_attend_many_pieces_in_three_parts(cuda_device, lens):
+    """Units of one tile of 64 keys up to many, back to back and in a graph: no wait runs out, every result is the same."""
+    base.test_attend_many_short_pieces(cuda_device, lens, *THREE)
+
+
+@pytest.mark.parametrize("dtype,cache", [("f16", "bf16"), ("bf16", "f16")])
+def test_attend_of_other_types_than_the_slabs(cuda_device, dtype, cache):
+    base.test_attend_infinite_values_that_are_seen(cuda_device, dtype, cache)
+    base.test_attend_what_is_not_seen_has_no_influence(cuda_device, dtype, cache)
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("up", [10, 17, 24])
+def test_attend_small_elements_of_q_beside_a_large_one(cuda_device, up, cache):
+    """One element of 2^up in each row of q, where the keys are 0.  Over F16 slabs the others are off by 2^-22 of themselves or
+    2^-39 of the large one: a score by 2^(up - 39) |k| scale = 2^(up - 39) by root mean square, and the weights by as much;
+    four times that on top of the bound for scores around 1."""
+    c = Case(cuda_device, [300, 65], 1, 8, 2, 128, 10, "f32", cache, seed=up)
+    c.k[..., 5] = 0
+    c.q = c.q.clone()
+    c.q[..., 5] = 2.0 ** up
+    got = c.run()
+    want, spread = R.attend(c.q, c.k, c.v, c.parents, None, c.len, c.scale, c.out())
+    more = 4 * 2.0 ** (up - 39) if cache == "f16" else 0.0
+    off = (got.double() - want).norm(dim=-1)
+    assert (off <= (2.0 ** -17 + more) * spread + 2.0 ** -18 * want.norm(dim=-1)).all(), (off / want.norm(dim=-1)).max().item()
