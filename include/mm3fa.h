@@ -623,9 +623,13 @@ MM3FA_API size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_t
  *   workspace      its first 64 KiB zero-filled once after allocation, 16-byte aligned; one per stream, for calls of this
  *                  function alone, of any shapes that it is large enough for
  * D 64, 128 or 256; at most 64 query heads per kv head.  q and the weights are not rounded to the cache's type: at D 64 and 128,
- * F16 slabs keep 22 bits of them (an F32 result is off by about 5e-7 of its norm), BF16 slabs all 24 for an F32 result (4e-7) and
- * 16 for others; F32 and Q8_0 slabs and D 256 all 24.  Where q, slabs and dst have one 16-bit type, and the slabs up to 32768
- * rows, weights are rounded to that type.  What a node does not see has no influence, not-a-number or infinite values included; a node that sees
+ * F16 slabs keep 22 bits of them (an element of q is off by at most 2^-22 of itself or 2^-39 of the largest of its row and head),
+ * BF16 slabs all 24 for an F32 result and 16 for others; F32 and Q8_0 slabs and D 256 all 24.  An F32 result over 4000 tokens is
+ * off by 3e-7 to 5e-7 of its norm where scores are around 1, 5e-7 to 7e-7 where they are around 4, and 8e-7 to 1.1e-6 there with a
+ * softcap of 30 or 50 (a score is off by some 2^-22 of itself, and by 4e-7 of the softcap).  Where q, slabs and dst have one 16-bit
+ * type, and the slabs up to 32768 rows, weights are rounded to that type.
+ * F16 and BF16 slabs at D 64 and 128 with rows whose address and strides are multiples of 16 bytes go to the tensor cores.  Others
+ * take each node's keys one after another: over long slabs mm3fa_flash_attn_ext with the tree as a mask is several times faster.  What a node does not see has no influence, not-a-number or infinite values included; a node that sees
  * nothing gets zeros.
  */
 MM3FA_API int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v,
@@ -638,7 +642,8 @@ MM3FA_API int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, co
  * current node, where accept[i] * q(x) * M < r(x); otherwise r <- max(r - M q, 0) and M <- sum of r.  q is the row of
  * `draft` at the current node, the distribution that its children were drawn from; without `draft`, 1 at x and 0
  * elsewhere.  The next token is the first at which the sum of r so far exceeds sample * sum of r (of p, where nothing is left
- * of r): the tokens then follow the target's distribution whatever the draft's.
+ * of r): the tokens then follow the target's distribution whatever the draft's, where a node's children were each drawn from its
+ * row by themselves, with replacement (fixed choices: chosen without regard to the random numbers).
  *   logits   F32, F16 or BF16 [V, max_nodes, n_tree]: row i is the target's behind node i; NaN counts as -inf
  *   draft    F32, F16 or BF16 probabilities of the same sizes, or NULL; NaN and negative ones count as 0
  *   tokens   device int32 [n_tree][max_nodes]: the nodes' tokens (node 0's is not used; one outside [0, V) is never accepted)

@@ -8,8 +8,9 @@
 // node does not see are not read.  Every type is widened to F32 exactly, all arithmetic is F32.
 //
 // Bound: issue and the latency of its loads, a node's keys one after another: two sequences of 8192, 24 nodes, 32 heads on 8,
-// D = 128, F32 slabs take 2419 us, 300 tokens and 5 nodes 40.  For slabs and head sizes that the tensor cores do not take
-// (there 30 us at 8192 from F16, 17 at 300).
+// D = 128, F32 slabs take 2438 us, 300 tokens and 5 nodes 39.  For slabs and head sizes that the tensor cores do not take
+// (there 32 us at 8192 from F16, 17 at 300).  Its work is not split over a unit's keys, so that one node takes 1548 us at 8192, where
+// the decode kernels, with the tree as a mask, take 57; Q8_0 832 and 74, 4 nodes 841 and 32.
 #include "tree.cuh"
 
 namespace mm3fa {
