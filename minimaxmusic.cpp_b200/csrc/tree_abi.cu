@@ -249,7 +249,8 @@ int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_
     p.o          = rows_of(dst);
     p.kv_len     = kv_len;
     p.scale      = scale;
-    p.softcap    = logit_softcap;
+    // (from 1e30 on a cap changes no score of up to 1e26 in F32, and the quotients by it would leave F32's range)
+    p.softcap    = logit_softcap < 1e30f ? logit_softcap : 0.0f;
     p.status     = static_cast<uint32_t *>(workspace);
     p.timeout_ns = host_wait_timeout_ns();
     // 16-bit slabs at D = 64 and 128 on the tensor cores; the others (F32, Q8_0, D = 256, unaligned rows) on CUDA cores

@@ -283,3 +283,11 @@ def test_attend_small_elements_of_q_beside_a_large_one(cuda_device, up, cache):
     more = 4 * 2.0 ** (up - 39) if cache == "f16" else 0.0
     off = (got.double() - want).norm(dim=-1)
     assert (off <= (2.0 ** -17 + more) * spread + 2.0 ** -18 * want.norm(dim=-1)).all(), (off / want.norm(dim=-1)).max().item()
+
+
+@pytest.mark.parametrize("dtype,cache", SIXTEEN + [("f32", "f32"), ("f32", "q8_0")])
+@pytest.mark.parametrize("cap", [1e-38, 1e20, 1e31, 1e36, 3e38])
+def test_attend_softcaps_from_the_smallest_to_the_largest(cuda_device, cap, dtype, cache):
+    c = Case(cuda_device, [300, 5], 1, 8, 2, 128, 10, dtype, cache, seed=31)
+    for scale in (c.scale, -c.scale, 1e-3 * c.scale):
+        c.check(scale=scale, logit_softcap=torch.tensor(cap).item())
