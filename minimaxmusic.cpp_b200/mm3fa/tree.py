@@ -87,7 +87,9 @@ class CacheLayers:
 
 
 class DraftTree(OnDevice):
-    """Trees of up to 256 drafted tokens: parents int32 [n_tree, T], n_nodes int32 [n_tree] or None (T)."""
+    """Trees of up to 256 drafted tokens: parents int32 [n_tree, T], n_nodes int32 [n_tree] or None (T).  Both are read by every
+    call, so that one object serves a program's steps with new trees written over the last ones; it keeps the attention's
+    workspace of each stream (up to some 20 MB), which another object would make anew."""
 
     _prefix = "mm3fa_tree_"
 
