@@ -97,7 +97,10 @@ bool named_before(const mm3fa_tensor * k, const mm3fa_tensor * v, int l, bool of
         return false;
     }
     const void * x = of_v ? v[l].data : k[l].data;
-    const bool   alike = k->nb[1] == v->nb[1] && k->nb[2] == v->nb[2] && k->nb[3] == v->nb[3];
+    bool         alike = true;
+    for (int i = 1; i < 4; i++) {
+        alike = alike && (k->ne[i] == 1 || k->nb[i] == v->nb[i]);
+    }
     for (int i = 0; i < l; i++) {
         if ((of_v ? v : k)[i].data == x || (alike && (of_v ? k : v)[i].data == x)) {
             return true;

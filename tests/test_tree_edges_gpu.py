@@ -291,3 +291,17 @@ def test_attend_softcaps_from_the_smallest_to_the_largest(cuda_device, cap, dtyp
     c = Case(cuda_device, [300, 5], 1, 8, 2, 128, 10, dtype, cache, seed=31)
     for scale in (c.scale, -c.scale, 1e-3 * c.scale):
         c.check(scale=scale, logit_softcap=torch.tensor(cap).item())
+
+
+def test_commit_a_slab_of_one_head_as_k_and_v(cuda_device):
+    """K of one layer is V of the next, under strides that differ along a dimension of one entry alone."""
+    rng = random.Random(9)
+    T, N = 24, 3
+    some = slabs(cuda_device, 3, N, 1, T + 40, 64, "f16", 8)
+    before = [x.clone() for x in some]
+    other = lambda x: x.as_strided(x.shape, (x.stride(0), 8, x.stride(2), 1))
+    path, n_path, lens = (torch.tensor(x, dtype=torch.int32, device=cuda_device) for x in ([rising(rng, T, 11)] * N, [11] * N, [0, 7, 33]))
+    want, _ = R.commit(before, path, n_path, lens)
+    layers = mm3fa.CacheLayers([some[0], some[1]], [other(some[2]), other(some[0])])
+    mm3fa.DraftTree(torch.full((N, T), -1, dtype=torch.int32, device=cuda_device)).commit(layers, path, n_path, lens)
+    assert all(torch.equal(x, w) for x, w in zip(some, want))
