@@ -629,8 +629,9 @@ MM3FA_API size_t mm3fa_tree_attn_workspace(const mm3fa_tensor * q, const mm3fa_t
  * softcap of 30 or 50 (a score is off by some 2^-22 of itself, and by 4e-7 of the softcap).  Where q, slabs and dst have one 16-bit
  * type, and the slabs up to 32768 rows, weights are rounded to that type.
  * F16 and BF16 slabs at D 64 and 128 with rows whose address and strides are multiples of 16 bytes go to the tensor cores.  Others
- * take each node's keys one after another: over long slabs mm3fa_flash_attn_ext with the tree as a mask is several times faster.  What a node does not see has no influence, not-a-number or infinite values included; a node that sees
- * nothing gets zeros.
+ * take each node's keys one after another: over long slabs mm3fa_flash_attn_ext with the tree as a mask is many times faster.
+ * What a node does not see has no influence, not-a-number or infinite values included (an infinite element of a key that it sees
+ * may make its row no number, whatever the sign); a node that sees nothing gets zeros.
  */
 MM3FA_API int mm3fa_tree_attn(const mm3fa_tensor * q, const mm3fa_tensor * k, const mm3fa_tensor * v,
                               const mm3fa_tree * tree, const int32_t * kv_len, float scale, float logit_softcap,
